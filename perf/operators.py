@@ -225,7 +225,7 @@ def _own(s):
     M = 2 * c["F"]
     if c["kind"] == "gated":
         return fp6.gated_forward_native(E, Mb, s["x"], w, sc, M, c["act"], group_exps=ge, bias=s["bias"])
-    preact = torch.empty(c["N"], M, dtype=torch.float16, device=DEVICE)
+    preact = torch.empty(c["N"], M, device=DEVICE)
     h = fp6.gated_forward_native(E, Mb, s["x"], w, sc, M, c["act"], preact=preact, group_exps=ge, bias=s["bias"])
     dx, dp = fp6.gated_backward_native(E, Mb, s["dh"], preact, w, sc, c["K"], c["act"], group_exps=ge)
     return {"out": h, "grad_in": dx, "grad_preact": dp}
