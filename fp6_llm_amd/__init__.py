@@ -47,6 +47,7 @@ __all__ = [
     "Num_Wave", "HeuristicFuntion_SplitK",
     "weight_prepacking_native_cpu", "to_native", "linear_forward_native", "native_bytes",
     "weight_dequant_native_cuda", "weight_quantize_native_cuda", "heuristic_splitk_mi355x", "clear_caches",
+    "gated_forward_native", "gated_backward_native", "gate_up_pairs", "linear_input_grad_native", "adapter_forward_native",
 ]
 
 MI355X_CUS = 256
@@ -447,3 +448,6 @@ def linear_forward_eXmY_cuda(EXPONENT, MANTISSA, in_feats, weights, scales, spli
 
 def linear_forward_cuda(in_feats, weights, scales, splitK=1):
     return linear_forward_eXmY_cuda(3, 2, in_feats, weights, scales, splitK)
+
+
+from .ops import adapter_forward_native, gate_up_pairs, gated_backward_native, gated_forward_native, linear_input_grad_native  # noqa: E402,F401

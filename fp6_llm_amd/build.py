@@ -6,10 +6,10 @@ import sys
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
-# (source, object name, extra flags): the kernel file is compiled once per weight format (tag = 10*E + M), the objects in parallel
+# (source, object name, extra flags): the kernel files are compiled once per weight format (tag = 10*E + M), the objects in parallel
 FORMAT_TAGS = (32, 22, 23, 21)
-UNITS = [("fp6mi_host.cpp", "fp6mi_host.o", []), ("fp6mi_api.hip", "fp6mi_api.o", [])] + \
-        [("fp6mi_gemm.hip", "fp6mi_gemm_%d.o" % t, ["-DFP6MI_FORMAT=%d" % t]) for t in FORMAT_TAGS]
+UNITS = [("fp6mi_%s.hip" % f, "fp6mi_%s_%d.o" % (f, t), ["-DFP6MI_FORMAT=%d" % t]) for f in ("gemm", "block") for t in FORMAT_TAGS] + \
+        [("fp6mi_host.cpp", "fp6mi_host.o", []), ("fp6mi_api.hip", "fp6mi_api.o", []), ("fp6mi_ops.hip", "fp6mi_ops.o", [])]
 OBJ_DIR = os.path.join(HERE, "csrc", "obj")
 OUTPUT = os.path.join(HERE, "libfp6mi.so")
 # measurement aid for the benchmark (a read-only streaming kernel); not linked into the engine

@@ -570,13 +570,13 @@ inline LaunchCfg final_cfg(int xbits, size_t M, size_t N, size_t K, int splitK, 
 }
 
 int linear_native(const fp6mi::FormatOps &ops, hipStream_t st, const void *W, const void *sc, const void *gexp, const void *bias, const void *B, void *C, size_t M, size_t N, size_t K, float *ws,
-                  int splitK, const LaunchCfg *forced)
+                  int splitK, const LaunchCfg *forced, bool partial_only = false)
 {
     LaunchCfg c = forced ? *forced : final_cfg(ops.bits, M, N, K, splitK, gexp != nullptr, current_device_cus());
     if (c.kind == 0 && !(c.rt & (c.rt - 1)) && (M / 16) % c.rt) return FP6MI_ERR_SHAPE; // (3, 5, 6, 7 tiles per workgroup end in a workgroup with fewer)
     int rc = ops.gemm(c, st, W, sc, gexp, B, C, splitK > 1 ? ws : static_cast<float *>(const_cast<void *>(bias)), M, N, K, splitK); // (a workspace given without a split is no bias)
     if (rc != 0) return rc;
-    if (splitK > 1) {
+    if (splitK > 1 && !partial_only) {
         size_t MN = M * N; // M % 256 == 0, so MN % 4 == 0
         const size_t tile_rows = (size_t)c.wr * c.rt * 16, nblocks = (N + (size_t)c.nt * 16 - 1) / ((size_t)c.nt * 16);
         const size_t grid = c.kind >= 1 && M % tile_rows == 0 ? M / tile_rows * nblocks * splitK : 0; // gemm_tile and gemm_ws share the tile order
@@ -602,6 +602,26 @@ int linear_native(const fp6mi::FormatOps &ops, hipStream_t st, const void *W, co
 
 } // namespace
 
+namespace fp6mi {
+
+int current_cus() { return current_device_cus(); }
+
+int run_linear(int E, int Mb, void *stream, const void *W, const void *sc, const void *gexp, const void *bias, const void *B, void *C, size_t M, size_t N, size_t K, float *ws, int splitK,
+               bool partial_only)
+{
+    return linear_native(*ops_for(E, Mb), static_cast<hipStream_t>(stream), W, sc, gexp, bias, B, C, M, N, K, ws, splitK, nullptr, partial_only);
+}
+
+int reduce_partials(void *stream, void *C, const float *ws, size_t M, size_t N, int splits)
+{
+    const size_t MN = M * N;
+    hipLaunchKernelGGL(splitk_reduce<false>, dim3((uint32_t)((MN / 4 + 255) / 256)), dim3(256), 0, static_cast<hipStream_t>(stream), static_cast<half_t *>(C), ws, MN, splits,
+                       static_cast<const half_t *>(nullptr), (uint32_t)M);
+    return (int)hipGetLastError();
+}
+
+} // namespace fp6mi
+
 // ------------------------------------------------------------------------------------------------ C ABI
 
 extern "C" {
@@ -618,6 +638,7 @@ const char *fp6mi_error_string(int code)
     case FP6MI_ERR_ALIGN: return "weights, activations, output and workspace must be 16-byte aligned (scales, group exponents, bias: 2-byte)";
     case FP6MI_ERR_TOO_LARGE: return "splitK*M*N floats exceed the library's static workspace (fp6mi_static_workspace_bytes)";
     case FP6MI_ERR_CAPTURE: return "the stream is being captured and this call would have to allocate: convert the weights first (fp6mi_relayout_ref_to_native_gpu) or make the first call outside the capture";
+    case FP6MI_ERR_ACTIVATION: return "activation must be one of FP6MI_ACT_*";
     default: return code > 0 ? hipGetErrorString((hipError_t)code) : "unknown fp6mi error";
     }
 }
@@ -739,6 +760,14 @@ static int check_gemm_args(int E, int Mb, const void *W, const void *sc, const v
     if (reinterpret_cast<uintptr_t>(sc) & 1u) return FP6MI_ERR_ALIGN; // halfs; the tile kernel uses 8-byte loads where the pointer allows them
     return FP6MI_OK;
 }
+
+} // extern "C"
+int fp6mi::check_linear(int E, int Mb, const void *W, const void *sc, const void *gexp, const void *bias, const void *B, const void *C, size_t M, size_t N, size_t K, const float *ws, int splitK)
+{
+    if ((reinterpret_cast<uintptr_t>(gexp) & 1u) || (reinterpret_cast<uintptr_t>(bias) & 1u)) return FP6MI_ERR_ALIGN;
+    return check_gemm_args(E, Mb, W, sc, B, C, M, N, K, ws, splitK);
+}
+extern "C" {
 
 int fp6mi_linear_native(int E, int Mb, void *stream, const void *W, const void *sc, const void *B, void *C, size_t M, size_t N, size_t K,
                         float *ws, int splitK)

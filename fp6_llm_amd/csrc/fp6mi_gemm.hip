@@ -29,144 +29,7 @@ namespace {
 
 using fp6mi::LaunchCfg;
 
-typedef _Float16 half_t;
-typedef _Float16 v8h __attribute__((ext_vector_type(8)));
-typedef _Float16 v32h __attribute__((ext_vector_type(32)));
-typedef float    v4f __attribute__((ext_vector_type(4)));
-typedef uint32_t v2u __attribute__((ext_vector_type(2)));
-typedef uint32_t v4u __attribute__((ext_vector_type(4)));
-typedef uint32_t v6u __attribute__((ext_vector_type(6)));
-
-constexpr int kWave = 64;
-
-// Formats are named by the tag FM = 10*E + M.  `hw_e3m2` says which conversion instruction reads the 6-bit fields that the
-// native layout holds (BF6 = e3m2 or FP6 = e2m3); post_scale is the factor the epilogue owes the sums.
-template <int FM> struct Fmt;
-template <> struct Fmt<32> { static constexpr int bits = 6, man = 2, bias = 3, block_bytes = 3072; static constexpr bool hw_e3m2 = true;
-                             static constexpr float post_scale = 1.0f; static constexpr double max_value = 28.0; };
-template <> struct Fmt<22> { static constexpr int bits = 5, man = 2, bias = 1, block_bytes = 2560; static constexpr bool hw_e3m2 = true;
-                             static constexpr float post_scale = 4.0f; static constexpr double max_value = 7.0; };
-template <> struct Fmt<23> { static constexpr int bits = 6, man = 3, bias = 1, block_bytes = 3072; static constexpr bool hw_e3m2 = false;
-                             static constexpr float post_scale = 1.0f; static constexpr double max_value = 7.5; };
-template <> struct Fmt<21> { static constexpr int bits = 4, man = 1, bias = 1, block_bytes = 2048; static constexpr bool hw_e3m2 = false;
-                             static constexpr float post_scale = 1.0f; static constexpr double max_value = 6.0; };
-
-// The weights of one lane for one 16x256 block, as loaded from memory.
-template <int FM> struct WFrag;
-template <> struct WFrag<32> { v4u a, b, c; };
-template <> struct WFrag<23> { v4u a, b, c; };
-template <> struct WFrag<22> { v4u a, b; v2u s; };
-template <> struct WFrag<21> { v4u a, b; };
-
-template <int FM> __device__ __forceinline__ WFrag<FM> load_wfrag(const uint8_t *block, int lane)
-{
-    const v4u *p = reinterpret_cast<const v4u *>(block) + lane;
-    WFrag<FM>  f;
-    f.a = __builtin_nontemporal_load(p);
-    f.b = __builtin_nontemporal_load(p + 64);
-    if constexpr (Fmt<FM>::bits == 6) f.c = __builtin_nontemporal_load(p + 128);
-    if constexpr (Fmt<FM>::bits == 5) f.s = __builtin_nontemporal_load(reinterpret_cast<const v2u *>(block + 2048) + lane);
-    return f;
-}
-
-// One of the two or three loads of load_wfrag, for a kernel that spreads them over its compute.
-template <int FM> __device__ __forceinline__ void load_wfrag_part(WFrag<FM> &f, const uint8_t *block, int lane, int part)
-{
-    const v4u *p = reinterpret_cast<const v4u *>(block) + lane;
-    if (part == 0) f.a = __builtin_nontemporal_load(p);
-    if (part == 1) f.b = __builtin_nontemporal_load(p + 64);
-    if constexpr (Fmt<FM>::bits == 6) { if (part == 2) f.c = __builtin_nontemporal_load(p + 128); }
-    if constexpr (Fmt<FM>::bits == 5) { if (part == 2) f.s = __builtin_nontemporal_load(reinterpret_cast<const v2u *>(block + 2048) + lane); }
-}
-
-// A operands (8 halfs = k 8q..8q+7 of this lane's row) of the eight MFMA steps of a block.
-// FP5: a quarter of the values (exact; the epilogue multiplies the sums by 4).  The other formats: exact values.
-template <int FM> struct AOps { v8h s[8]; };
-
-__device__ __forceinline__ v8h slice8(const v32h &v, int i)
-{
-    switch (i) {
-    case 0: return __builtin_shufflevector(v, v, 0, 1, 2, 3, 4, 5, 6, 7);
-    case 1: return __builtin_shufflevector(v, v, 8, 9, 10, 11, 12, 13, 14, 15);
-    case 2: return __builtin_shufflevector(v, v, 16, 17, 18, 19, 20, 21, 22, 23);
-    default: return __builtin_shufflevector(v, v, 24, 25, 26, 27, 28, 29, 30, 31);
-    }
-}
-
-// FP5: 32 codes are stored in five dwords; the sixth dword of the 6-bit string the conversion instruction reads is parked
-// in the fixed-zero bits ("holes", bit 4 of every 6-bit field) of the other five and is put back here (layout: fp6mi_host.cpp).
-__device__ __forceinline__ v6u fp5_expand(uint32_t s0, uint32_t s1, uint32_t s2, uint32_t s3, uint32_t s4)
-{
-    constexpr uint32_t A = 0x10410410u, B = 0x04104104u, C = 0x41041041u;
-    uint32_t lo = (s0 & A) | (s1 & B), hi = (s2 & C) | (s3 & A) | (s4 & B);
-    return (v6u){ s0 & ~A, s1 & ~B, s2 & ~C, s3 & ~A, s4 & ~B, (hi << 1) | lo };
-}
-
-// FP4: 32 codes are stored in four dwords; the fifth and sixth dword of the 6-bit string sit in the fixed-zero bit pairs (the
-// two bits appended below every mantissa) of the other four, at their own bit positions (layout: fp6mi_host.cpp).
-__device__ __forceinline__ v6u fp4_expand(v4u s)
-{
-    constexpr uint32_t P = 0xC30C30C3u, Q = 0x30C30C30u, R = 0x0C30C30Cu;
-    return (v6u){ s[0] & ~P, s[1] & ~Q, s[2] & ~R, s[3] & ~P, (s[0] & P) | (s[2] & R), (s[1] & Q) | (s[3] & P) };
-}
-
-// The 192-bit string of 6-bit fields of MFMA steps 4h..4h+3 (half of a K block) of one lane, and its conversion.
-template <int FM> __device__ __forceinline__ v6u field_string(const WFrag<FM> &f, int h)
-{
-    if constexpr (Fmt<FM>::bits == 6)
-        return h == 0 ? (v6u){ f.a[0], f.a[1], f.a[2], f.a[3], f.b[0], f.b[1] } : (v6u){ f.b[2], f.b[3], f.c[0], f.c[1], f.c[2], f.c[3] };
-    else if constexpr (Fmt<FM>::bits == 5)
-        return h == 0 ? fp5_expand(f.a[0], f.a[1], f.a[2], f.a[3], f.s[0]) : fp5_expand(f.b[0], f.b[1], f.b[2], f.b[3], f.s[1]);
-    else
-        return fp4_expand(h == 0 ? f.a : f.b);
-}
-
-// The conversion instruction multiplies its 32 values by the power of two in the exponent field of `scale` at no cost.
-template <int FM> __device__ __forceinline__ v32h fields_to_halfs(v6u src, float scale)
-{
-    if constexpr (Fmt<FM>::hw_e3m2)
-        return __builtin_amdgcn_cvt_scalef32_pk32_f16_bf6(src, scale);
-    else
-        return __builtin_amdgcn_cvt_scalef32_pk32_f16_fp6(src, scale);
-}
-
-// Group exponents: one byte b per (row, 128 columns), meaning the factor 2^(b-127) on those weights (the E8M0 scale type of
-// the OCP MX formats).  A lane's 32-code string is exactly its row's share of one 128-column group, so the factor rides on
-// the conversion instruction.  Native layout of the bytes: [row tile][K block][row in tile][half of the block], 32 bytes per
-// block; `g` below is the lane's pair of bytes (half 0 in the low byte).  GS = false: no group exponents, factor 1.
-template <bool GS> __device__ __forceinline__ float group_factor(uint32_t g, int h)
-{
-    if constexpr (GS)
-        return __builtin_bit_cast(float, (h == 0 ? (g & 0xffu) : (g >> 8)) << 23);
-    else
-        return 1.0f;
-}
-// block = index of the 16x256 block counted from `gexp` (32 bytes each); nothing is computed or read without group exponents
-template <bool GS> __device__ __forceinline__ uint32_t load_group_exps(const uint8_t *gexp, size_t block, int lane)
-{
-    if constexpr (GS)
-        return *reinterpret_cast<const uint16_t *>(gexp + block * 32 + 2 * (lane & 15));
-    else
-        return 0;
-}
-
-template <int FM, bool GS> __device__ __forceinline__ void convert(const WFrag<FM> &f, AOps<FM> &o, uint32_t g)
-{
-    v32h h0 = fields_to_halfs<FM>(field_string<FM>(f, 0), group_factor<GS>(g, 0));
-    v32h h1 = fields_to_halfs<FM>(field_string<FM>(f, 1), group_factor<GS>(g, 1));
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        o.s[i]     = slice8(h0, i);
-        o.s[4 + i] = slice8(h1, i);
-    }
-}
-
-// `ws` of the GEMM kernels: the partial sums where K is split (splitk_reduce adds a bias then), else an fp16 bias [M] on any 2-byte boundary or null, which
-// the epilogue adds to the float32 sums.  gemm_stream and gemm_tile have instances of their own for it: a branch in the epilogue that no launch took cost the one 0.04-0.1 us (1 % of
-// 4096x4096 N 8), the other a register or two, in some instances spilled, and 0.2-0.5 % of calls of 5 us.  The kernels of larger tiles branch (gemm_ws +0.0-0.6 % on calls of
-// 9-20 us, as much as two builds of the same instructions differ by).  Instead of an addition behind the GEMM, us, e3m2, replayed: 4096x4096 N 1 6.1 -> 4.4, N 8 7.6 -> 5.0; 8192x8192 N 16 15.7 -> 12.9,
-// N 72 25.9 -> 22.1; 28672x8192 N 2048 680 -> 657.
-template <typename P> __device__ __forceinline__ const half_t *bias_of(P ws) { return reinterpret_cast<const half_t *>(ws); }
+#include "fp6mi_device.inc"
 
 // ---------------------------------------------------------------------------------------------------------------
 // gemm_stream: weight-bandwidth-bound GEMM for small batches.
@@ -186,233 +49,13 @@ template <typename P> __device__ __forceinline__ const half_t *bias_of(P ws) { r
 // Batches up to 4 keep operand-order loads: a quarter-wavefront then touches at most 4 lines, and the trip through LDS
 // would only add latency (measured: 1-4 % slower there).
 // ---------------------------------------------------------------------------------------------------------------
-constexpr int kXsRowBytes = 544;
-
-template <int FM, int RT> struct StageW {
-    WFrag<FM> w[RT];
-    uint32_t  g[RT]; // group exponents of the block (unused without them)
-};
-
-// LDS bytes per wavefront: the activation rows of one K block, or the RT*NT partial tiles of the epilogue (they share it)
-__host__ __device__ constexpr uint32_t stream_wave_bytes(int rows, int RT, int NT)
-{
-    return (uint32_t)(rows * kXsRowBytes > RT * NT * 1024 ? rows * kXsRowBytes : RT * NT * 1024);
-}
-
 template <int FM, bool GS, int NT, int RT, int WAVES, bool SPLIT, bool BIAS>
 __global__ __launch_bounds__(WAVES *kWave) void gemm_stream(const uint8_t *__restrict__ W, const half_t *__restrict__ scales,
                                                             const uint8_t *__restrict__ gexp, const half_t *__restrict__ X, half_t *__restrict__ C,
                                                             float *__restrict__ ws, uint32_t M, uint32_t N, uint32_t K,
                                                             uint32_t units, uint32_t splitK)
 {
-    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-
-    // every kernel argument is fetched by one batch of scalar loads at the top (left alone, the compiler fetches them in
-    // three batches, each a round trip to memory, as the code reaches their first use)
-    asm volatile("" ::"s"(W), "s"(scales), "s"(gexp), "s"(X), "s"(C), "s"(ws), "s"(M), "s"(N), "s"(K), "s"(units), "s"(splitK));
-    // the wavefront's index as a scalar: the K-block loop, its bounds and its branches then run on the scalar unit
-    const int      lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int      col = lane & 15, q = lane >> 4;
-    const uint32_t R0 = blockIdx.x * RT, split = blockIdx.y, nbase = blockIdx.z * (16 * NT);
-
-    // SPLIT = false is the launch with splitK == 1: its range is the whole of K and its epilogue writes fp16
-    uint32_t u0 = 0, u1 = units;
-    if constexpr (SPLIT) {
-        const uint32_t avg = units / splitK, extra = units % splitK;
-        u0 = split * avg + (split < extra ? split : extra);
-        u1 = u0 + avg + (split < extra ? 1u : 0u);
-    }
-
-    const size_t   tile_stride = (size_t)units * Fmt<FM>::block_bytes;
-    const uint8_t *wgroup = W + (size_t)R0 * tile_stride;
-    const uint8_t *ggroup = GS ? gexp + (size_t)R0 * units * 32 : nullptr;
-    // M is a multiple of 256, so 1, 2, 4 and 8 row tiles per workgroup divide its M/16 row tiles; 3, 5, 6 and 7 need not, and
-    // the last workgroup then holds fewer.  Its missing tiles stand in as copies of its last real one (same loads, same arithmetic,
-    // nothing stored): rlast is the largest r that names a real tile.
-    constexpr bool kRagged = (RT & (RT - 1)) != 0;
-    const uint32_t rlast = kRagged && R0 + RT > (M >> 4) ? (M >> 4) - 1 - R0 : RT - 1;
-    auto           real = [&](int r) -> uint32_t { return kRagged && (uint32_t)r > rlast ? rlast : (uint32_t)r; };
-
-    v4f acc[RT][NT];
-#pragma unroll
-    for (int r = 0; r < RT; r++)
-#pragma unroll
-        for (int t = 0; t < NT; t++) acc[r][t] = (v4f){ 0.f, 0.f, 0.f, 0.f };
-
-    // The epilogue gives thread e the output (row tile e/(256*NT), column tile, batch column, row e%16); its row scale is
-    // fetched now so that no global load sits on the tail of the kernel.
-    constexpr int kOutPerThread = (RT * NT * 256 + WAVES * kWave - 1) / (WAVES * kWave);
-    half_t        my_scale[kOutPerThread]; // kept as loaded: converting here would wait for the load before the weight loads issue
-#pragma unroll
-    for (int j = 0; j < kOutPerThread; j++) {
-        int e = threadIdx.x + j * WAVES * kWave;
-        my_scale[j] = scales[(R0 + real(e < RT * NT * 256 ? (e >> 8) / NT : 0)) * 16 + (e & 15)];
-    }
-
-    const uint32_t ncols = N - nbase;              // batch columns of this column block that exist (the launcher made sure of >= 1)
-    const bool     small = NT == 1 && ncols <= 8;  // 8 rows are staged instead of 16
-    const uint32_t wave_bytes = small ? stream_wave_bytes(8, RT, NT) : stream_wave_bytes(16 * NT, RT, NT);
-    uint8_t       *mine = lds + wave * wave_bytes;  // this wavefront's LDS area
-
-    // One K block at a time and no register double-buffering: the other wavefronts of the workgroup keep the memory system
-    // busy while this one converts, and a second stage in registers measured slower at every size.
-    // workgroups that share an L2 (ids congruent mod 8) start on different K blocks, so that the chip does not ask
-    // the same activation lines of the same L2 channel at the same moment
-    const uint32_t ufull = K / 256 < u1 ? K / 256 : u1; // the blocks before this one lie wholly inside K
-    uint32_t       u = u0 + ((wave + (blockIdx.x >> 3)) % WAVES);
-    // MODE 0: batches up to 4 load in operand order (a quarter-wavefront then touches at most 4 lines, and the detour through
-    // LDS would only add latency); MODE 1: 8 rows through LDS; MODE 2: 16*NT rows through LDS.  TAIL: the block is cut by K
-    // (only the last block of a K that is no multiple of 256).  The kernel chooses outside its K loop: a choice made per
-    // block inside the loop cost 0.2 us of a 4.9 us launch.
-    auto run = [&](auto mode_c, auto tail_c, uint32_t end) {
-        constexpr int  MODE = decltype(mode_c)::value, ROWS = MODE == 2 ? 16 * NT : 8, LOADS = MODE == 0 ? 4 : ROWS / 2;
-        constexpr bool TAIL = decltype(tail_c)::value;
-        static_assert(!(MODE == 0 && (TAIL || NT != 1)), "operand-order loads serve whole blocks of one column tile");
-        // MODE 0: lane (col, q) reads batch row col % 8 at MFMA step offset col / 8
-        const uint32_t prow = (uint32_t)(col & 7) < ncols ? col & 7 : ncols - 1;
-        const half_t  *xpaired = X + (size_t)(nbase + prow) * K + 8 * q + 32 * (col >> 3);
-        // MODE 1, 2: load i of a block brings rows 2i and 2i+1, lane l takes bytes 16*(l%32).. of row 2i + l/32: a scalar base per
-        // load plus one per-lane offset for the whole kernel.  Rows beyond the batch repeat its last row (an MFMA output column
-        // depends only on its own B column, and those columns are never stored).
-        const uint8_t *xbase = reinterpret_cast<const uint8_t *>(X + (size_t)nbase * K);
-        const uint32_t off_one = (lane & 31) * 16, off_pair = (lane >> 5) * (K * 2) + off_one; // K < 2^31
-        uint8_t       *xw = mine + (lane >> 5) * kXsRowBytes + (lane & 31) * 16;
-        const uint8_t *xr = mine + (ROWS == 8 ? col & 7 : col) * kXsRowBytes + q * 16;
-        constexpr int  kWParts = Fmt<FM>::bits == 4 ? 2 : 3;
-        // Through LDS, the activation loads are issued BEFORE the weight loads: the memory pipeline returns loads in order, so
-        // activations asked for first are back (from L2) long before the weights (from HBM), and their trip through LDS
-        // is over when the weights arrive.  Issued after the weights they cost 5-10 % at batch 16.  In operand order they go
-        // between the second and the third weight load of the first row tile.
-        constexpr int kWBeforeX = MODE == 0 ? 2 : 0;
-        for (; u < end; u += WAVES) {
-            StageW<FM, RT> cur;
-            v4u            xv[LOADS];
-            auto           wpart = [&](int i) {
-                const int r = i / kWParts, part = i % kWParts;
-                load_wfrag_part<FM>(cur.w[r], wgroup + real(r) * tile_stride + (size_t)u * Fmt<FM>::block_bytes, lane, part);
-            };
-#pragma unroll
-            for (int i = 0; i < kWBeforeX; i++) wpart(i);
-            // K positions beyond K count as zero activations against the zero weights the native layout holds there (0 x 0,
-            // whatever the row holds elsewhere: an infinite activation must not meet a padding weight): such a piece is read
-            // at the row's start (a valid address) and replaced by zeros
-            const bool beyond = TAIL && u * 256 + 8 * (lane & 31) >= K;
-#pragma unroll
-            for (int i = 0; i < LOADS; i++) {
-                if constexpr (MODE == 0) {
-                    xv[i] = *reinterpret_cast<const v4u *>(xpaired + (size_t)u * 256 + 64 * i);
-                } else {
-                    const uint32_t r0 = (uint32_t)(2 * i) < ncols ? 2 * i : ncols - 1;
-                    const uint8_t *sb = xbase + ((size_t)r0 * K + (size_t)u * 256) * 2;
-                    uint32_t       vo = (uint32_t)(2 * i + 1) < ncols ? off_pair : off_one;
-                    if (beyond) vo -= off_one;
-                    const v4u v = *reinterpret_cast<const v4u *>(sb + vo);
-                    xv[i] = beyond ? (v4u){ 0u, 0u, 0u, 0u } : v;
-                }
-            }
-#pragma unroll
-            for (int i = kWBeforeX; i < RT * kWParts; i++) wpart(i);
-#pragma unroll
-            for (int r = 0; r < RT; r++) cur.g[r] = load_group_exps<GS>(ggroup, (size_t)real(r) * units + u, lane);
-            __builtin_amdgcn_sched_barrier(0); // keep every load of the block issued before anything waits
-            v8h x[8][NT];
-            if constexpr (MODE == 0) {
-                // one load brought two MFMA steps: a DPP rotation of each 16-lane row by 8 moves the second step's data down to
-                // columns 0..7 (columns 8..15 then hold the other step's real, finite data and feed outputs never stored)
-#pragma unroll
-                for (int sl = 0; sl < 4; sl++) {
-                    v4u w;
-#pragma unroll
-                    for (int i = 0; i < 4; i++) w[i] = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)xv[sl][i], 0x128, 0xf, 0xf, false); // row_ror:8
-                    x[2 * sl][0]     = __builtin_bit_cast(v8h, xv[sl]);
-                    x[2 * sl + 1][0] = __builtin_bit_cast(v8h, w);
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < LOADS; i++) *reinterpret_cast<v4u *>(xw + 2 * i * kXsRowBytes) = xv[i];
-#pragma unroll
-                for (int s = 0; s < 8; s++)
-#pragma unroll
-                    for (int t = 0; t < NT; t++) x[s][t] = *reinterpret_cast<const v8h *>(xr + t * 16 * kXsRowBytes + 64 * s);
-                // the trip through LDS is issued before anything that waits for weights (left alone, the compiler moves register
-                // copies that feed the conversion above the LDS writes, and with them the wait for the weight loads)
-                __builtin_amdgcn_sched_barrier(0);
-            }
-#pragma unroll
-            for (int r = 0; r < RT; r++) {
-                AOps<FM> a;
-                convert<FM, GS>(cur.w[r], a, cur.g[r]);
-#pragma unroll
-                for (int s = 0; s < 8; s++)
-#pragma unroll
-                    for (int t = 0; t < NT; t++) acc[r][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a.s[s], x[s][t], acc[r][t], 0, 0, 0);
-            }
-        }
-    };
-    typedef std::integral_constant<int, 0> Direct;
-    typedef std::integral_constant<int, 1> Staged8;
-    typedef std::integral_constant<int, 2> StagedAll;
-    auto staged = [&](auto mode_c, bool whole_blocks) {
-        if (whole_blocks) run(mode_c, std::false_type{}, ufull);
-        run(mode_c, std::true_type{}, u1); // at most one block, and only when K is not a multiple of 256
-    };
-    if (small) {
-        if constexpr (NT == 1) {
-            if (ncols <= 4) {
-                run(Direct{}, std::false_type{}, ufull);
-                staged(Staged8{}, false);
-            } else {
-                staged(Staged8{}, true);
-            }
-        }
-    } else {
-        staged(StagedAll{}, true);
-    }
-
-    // acc[r][t][i] = sum for output row 16r + 4q+i, batch column 16t+col.  Each wavefront parks its tiles in its own LDS
-    // area (its activation rows are dead by now; nobody else ever touched them), then the workgroup sums them.
-#pragma unroll
-    for (int r = 0; r < RT; r++)
-#pragma unroll
-        for (int t = 0; t < NT; t++) *reinterpret_cast<v4f *>(mine + (r * NT + t) * 1024 + lane * 16) = acc[r][t];
-    half_t my_bias[BIAS ? kOutPerThread : 1];
-    if constexpr (BIAS) { // (under the wait for the other wavefronts)
-#pragma unroll
-        for (int j = 0; j < kOutPerThread; j++) {
-            const int e = threadIdx.x + j * WAVES * kWave;
-            my_bias[j] = bias_of(ws)[(R0 + real(e < RT * NT * 256 ? (e >> 8) / NT : 0)) * 16 + (e & 15)];
-        }
-    }
-    __syncthreads();
-
-#pragma unroll
-    for (int j = 0; j < kOutPerThread; j++) {
-        const int e = threadIdx.x + j * WAVES * kWave;
-        if (e >= RT * NT * 256) break;
-        int   rt = e >> 8, i8 = e & 255, n = i8 >> 4, mm = i8 & 15;
-        int   r = rt / NT, t = rt % NT;
-        int   idx = (((mm >> 2) * 16 + n) << 2) | (mm & 3);
-        float sum = 0.f;
-#pragma unroll
-        for (int w = 0; w < WAVES; w++) sum += *reinterpret_cast<const float *>(lds + w * wave_bytes + rt * 1024 + idx * 4);
-        uint32_t ng = nbase + 16 * t + n, mg = (R0 + r) * 16 + mm;
-        if (ng < N && (!kRagged || (uint32_t)r <= rlast)) {
-            float v = sum * ((float)my_scale[j] * Fmt<FM>::post_scale);
-            if constexpr (BIAS) v += (float)my_bias[j];
-            if constexpr (!SPLIT)
-                C[(size_t)ng * M + mg] = (half_t)v;
-            else
-                ws[((size_t)split * N + ng) * M + mg] = v;
-        }
-    }
-}
-
-// A operands of MFMA steps 4h..4h+3 (half of a K block) of one lane.
-template <int FM, bool GS> __device__ __forceinline__ void convert_half(const WFrag<FM> &f, int h, v8h (&o)[4], uint32_t g)
-{
-    v32h v = fields_to_halfs<FM>(field_string<FM>(f, h), group_factor<GS>(g, h));
-#pragma unroll
-    for (int i = 0; i < 4; i++) o[i] = slice8(v, i);
+#include "fp6mi_stream_tile.inc"
 }
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -431,296 +74,6 @@ template <int FM, bool GS> __device__ __forceinline__ void convert_half(const WF
 // Tiles of 48, 80 and 96 columns exist for the batches that the powers of two miss (FP6 e3m2, us, the best of 32, 64 and 128 columns -> 256 x 80 and
 // 256 x 96 here): 28672x8192 N 72 67.3 -> 48.0, N 160 117 -> 81; 8192x28672 N 72 69 -> 49, N 96 68.9 -> 57.9.
 // ---------------------------------------------------------------------------------------------------------------
-
-// One segment of a tile's K range: K blocks [u0, u1) of row block `mb` against the batch columns from `nbase`, accumulated
-// into acc.  On return the wavefronts with wk == 0 hold the sums of all WK K-wavefronts; the LDS buffers are free again
-// once every wavefront of the workgroup has passed a barrier.
-template <int FM, bool GS, int NT, int RT, int WR, int WK>
-__device__ __forceinline__ void tile_segment(v4f (&acc)[RT][NT], const uint8_t *__restrict__ W, const uint8_t *__restrict__ gexp,
-                                             const half_t *__restrict__ X, uint32_t N, uint32_t K, uint32_t units, uint32_t mb, uint32_t nbase,
-                                             uint32_t u0, uint32_t u1, uint8_t *lds, int tid, int lane, int wr, int wk, int col, int q)
-{
-    constexpr int  TN = NT * 16, NTHREADS = WR * WK * kWave;
-    constexpr int  kBufBytes = WK * TN * kXsRowBytes;
-    constexpr int  kPieces = WK * TN * 32, kPerThread = (kPieces + NTHREADS - 1) / NTHREADS;
-    const uint32_t R0 = (mb * WR + wr) * RT; // first row tile of this wavefront
-    const size_t   tile_stride = (size_t)units * Fmt<FM>::block_bytes;
-    const uint8_t *wgroup = W + (size_t)R0 * tile_stride;
-    const uint8_t *ggroup = GS ? gexp + (size_t)R0 * units * 32 : nullptr;
-
-#pragma unroll
-    for (int r = 0; r < RT; r++)
-#pragma unroll
-        for (int t = 0; t < NT; t++) acc[r][t] = (v4f){ 0.f, 0.f, 0.f, 0.f };
-
-    WFrag<FM> wcur[RT], wnxt[RT];
-    uint32_t  gcur[RT], gnxt[RT]; // group exponents travel with the weights (unused without them)
-    v4u       xr[kPerThread];
-
-    auto load_w = [&](WFrag<FM>(&dst)[RT], uint32_t(&gdst)[RT], uint32_t c0) {
-        const uint32_t u = c0 + wk;
-        if (u < u1) {
-#pragma unroll
-            for (int r = 0; r < RT; r++) {
-                dst[r]  = load_wfrag<FM>(wgroup + r * tile_stride + (size_t)u * Fmt<FM>::block_bytes, lane);
-                gdst[r] = load_group_exps<GS>(ggroup, (size_t)r * units + u, lane);
-            }
-        }
-    };
-    // Per-thread pieces of the activation chunk: piece p = tid + NTHREADS*j is 16 bytes, (K block p / (TN*32) of the chunk,
-    // batch column (p/32) % TN, halfs 8*(p%32)..+7).  Row pointers and LDS offsets are fixed for the whole kernel.
-    // Columns beyond N read the last real row (their outputs are never stored); positions beyond K or beyond the split are
-    // read at position 0 of the row (a valid address) and staged as zeros (zero weights meet them, or no wavefront does).
-    const half_t *xrow[kPerThread];
-    uint32_t      xlds[kPerThread];
-#pragma unroll
-    for (int j = 0; j < kPerThread; j++) {
-        const uint32_t p = tid + NTHREADS * j, n = nbase + (p >> 5) % TN;
-        xrow[j] = X + (size_t)(n < N ? n : N - 1) * K + (p & 31) * 8 + (size_t)(p / (TN * 32)) * 256;
-        xlds[j] = (p >> 5) * kXsRowBytes + (p & 31) * 16;
-    }
-    // `full` (a compile-time flag): the whole chunk lies inside K and inside the segment, so every piece is a plain load.  The
-    // K loop below is written out per case: one choice per chunk inside the loop costs a wait for the activation loads before
-    // the weight loads can be issued.
-    auto load_x = [&](auto full, uint32_t c0) {
-        if constexpr (decltype(full)::value) {
-#pragma unroll
-            for (int j = 0; j < kPerThread; j++)
-                if (kPieces % NTHREADS == 0 || tid + NTHREADS * j < kPieces) xr[j] = *reinterpret_cast<const v4u *>(xrow[j] + (size_t)c0 * 256);
-        } else {
-#pragma unroll
-            for (int j = 0; j < kPerThread; j++) {
-                const uint32_t p = tid + NTHREADS * j;
-                if (kPieces % NTHREADS == 0 || p < (uint32_t)kPieces) {
-                    const uint32_t u = c0 + p / (TN * 32), k = u * 256 + (p & 31) * 8;
-                    const bool     ok = k < K && u < u1;
-                    const v4u      v = *reinterpret_cast<const v4u *>(ok ? xrow[j] + (size_t)c0 * 256 : xrow[j] - ((p & 31) * 8 + (size_t)(p / (TN * 32)) * 256));
-                    xr[j] = ok ? v : (v4u){ 0u, 0u, 0u, 0u };
-                }
-            }
-        }
-    };
-    // The same loads one at a time (i = 0 .. kLoads-1: weights first, then activation pieces).  The 256 x 128 tile spreads them
-    // over its MFMA steps instead of issuing them in one burst: measured 10-12 % faster for batches from 1024 up (the burst keeps
-    // a wavefront, which issues in order, from starting its MFMAs until the CU has accepted its last load); for the smaller
-    // tiles, with fewer MFMAs between two loads, spreading measured 0-8 % slower and they keep the burst.
-    constexpr bool kSpreadLoads = NT >= 8 && WR * WK >= 8;
-    constexpr int  kWParts = Fmt<FM>::bits == 4 ? 2 : 3, kWLoads = RT * kWParts, kLoads = kWLoads + kPerThread, kPerStep = (kLoads + 7) / 8;
-    auto load_one = [&](auto full, int i, uint32_t c0) {
-        if (i < kWLoads) {
-            const int      r = i / kWParts, part = i % kWParts;
-            const uint32_t u = c0 + wk;
-            if (u < u1) {
-                load_wfrag_part<FM>(wnxt[r], wgroup + r * tile_stride + (size_t)u * Fmt<FM>::block_bytes, lane, part);
-                if (part == 0) gnxt[r] = load_group_exps<GS>(ggroup, (size_t)r * units + u, lane);
-            }
-        } else if (i < kLoads) {
-            const int      j = i - kWLoads;
-            const uint32_t p = tid + NTHREADS * j;
-            if (kPieces % NTHREADS == 0 || p < (uint32_t)kPieces) {
-                if constexpr (decltype(full)::value) {
-                    xr[j] = *reinterpret_cast<const v4u *>(xrow[j] + (size_t)c0 * 256);
-                } else {
-                    const uint32_t u = c0 + p / (TN * 32), k = u * 256 + (p & 31) * 8;
-                    const bool     ok = k < K && u < u1;
-                    const v4u      v = *reinterpret_cast<const v4u *>(ok ? xrow[j] + (size_t)c0 * 256 : xrow[j] - ((p & 31) * 8 + (size_t)(p / (TN * 32)) * 256));
-                    xr[j] = ok ? v : (v4u){ 0u, 0u, 0u, 0u };
-                }
-            }
-        }
-    };
-    auto store_x = [&](int buf) {
-#pragma unroll
-        for (int j = 0; j < kPerThread; j++)
-            if (kPieces % NTHREADS == 0 || tid + NTHREADS * j < kPieces) *reinterpret_cast<v4u *>(lds + buf * kBufBytes + xlds[j]) = xr[j];
-    };
-    typedef std::integral_constant<int, 0> NoNext;       // the last chunk: nothing to fetch
-    typedef std::integral_constant<int, 1> FullNext;     // the next chunk is a full one
-    typedef std::integral_constant<int, 2> PartialNext;  // the next chunk is cut by K or by the end of the segment
-    typedef std::integral_constant<bool, true> Full;
-    typedef std::integral_constant<bool, false> Partial;
-
-    if (u0 < u1) {
-        const uint32_t ufull = K / 256 < u1 ? K / 256 : u1; // chunks that end at or before this block are full
-        if (u0 + WK <= ufull)
-            load_x(Full{}, u0);
-        else
-            load_x(Partial{}, u0);
-        load_w(wcur, gcur, u0);
-        store_x(0);
-        __syncthreads();
-        int      buf = 0;
-        uint32_t c0 = u0;
-        // one chunk: fetch the next one (if any), compute this one, stage the next one's activations, barrier
-        auto chunk = [&](auto next) {
-            constexpr int  kNext = decltype(next)::value;
-            constexpr bool more = kNext != 0;
-            typedef std::integral_constant<bool, kNext == 1> NextIsFull;
-            if (more && (!kSpreadLoads || c0 + wk >= u1)) { // (a wavefront without a K block in this chunk has no MFMAs to spread over)
-                load_x(NextIsFull{}, c0 + WK);
-                load_w(wnxt, gnxt, c0 + WK);
-            }
-            if (c0 + wk < u1) {
-                const uint8_t *xs = lds + buf * kBufBytes + (wk * TN + col) * kXsRowBytes + q * 16;
-                v8h            a0[RT][4], a1[RT][4];
-#pragma unroll
-                for (int r = 0; r < RT; r++) convert_half<FM, GS>(wcur[r], 0, a0[r], gcur[r]);
-                // second half converted ahead of the first half's MFMAs: the VALU work then runs under the matrix pipe
-#pragma unroll
-                for (int r = 0; r < RT; r++) convert_half<FM, GS>(wcur[r], 1, a1[r], gcur[r]);
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-#pragma unroll
-                    for (int s = 0; s < 4; s++) {
-                        v8h b[NT];
-#pragma unroll
-                        for (int t = 0; t < NT; t++) b[t] = *reinterpret_cast<const v8h *>(xs + t * 16 * kXsRowBytes + (4 * h + s) * 64);
-#pragma unroll
-                        for (int r = 0; r < RT; r++)
-#pragma unroll
-                            for (int t = 0; t < NT; t++)
-                                acc[r][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(h == 0 ? a0[r][s] : a1[r][s], b[t], acc[r][t], 0, 0, 0);
-                        if constexpr (kSpreadLoads && more) {
-#pragma unroll
-                            for (int i = (4 * h + s) * kPerStep; i < (4 * h + s + 1) * kPerStep; i++) load_one(NextIsFull{}, i, c0 + WK);
-                        }
-                    }
-                }
-            }
-            if (more) {
-                store_x(buf ^ 1); // that buffer was last read before the barrier that ended the previous iteration
-#pragma unroll
-                for (int r = 0; r < RT; r++) wcur[r] = wnxt[r], gcur[r] = gnxt[r];
-            }
-            __syncthreads();
-            c0 += WK, buf ^= 1;
-        };
-        while (c0 + 2 * WK <= ufull) chunk(FullNext{});
-        while (c0 + WK < u1) chunk(PartialNext{});
-        chunk(NoNext{});
-    }
-
-    // acc[r][t][i]: output row (R0+r)*16 + 4q+i, batch column nbase + 16t + col
-    if (WK > 1) {
-        float *red = reinterpret_cast<float *>(lds); // [WK][WR][RT*NT][256]; the last barrier above freed the buffers
-#pragma unroll
-        for (int r = 0; r < RT; r++)
-#pragma unroll
-            for (int t = 0; t < NT; t++) *reinterpret_cast<v4f *>(&red[(((wk * WR + wr) * RT + r) * NT + t) * 256 + lane * 4]) = acc[r][t];
-        __syncthreads();
-        if (wk == 0) {
-#pragma unroll
-            for (int r = 0; r < RT; r++)
-#pragma unroll
-                for (int t = 0; t < NT; t++)
-#pragma unroll
-                    for (int k2 = 1; k2 < WK; k2++)
-                        acc[r][t] += *reinterpret_cast<const v4f *>(&red[(((k2 * WR + wr) * RT + r) * NT + t) * 256 + lane * 4]);
-        }
-    }
-}
-
-// The tile kernel's output goes through LDS.  An MFMA accumulator holds four consecutive rows of ONE batch column per lane, so
-// a store straight from the accumulators makes the 16 lanes of a quarter-wavefront write 8 or 16 bytes into each of 16
-// different lines (C and the partial sums are [N][M], rows contiguous); the memory pipeline takes a line at a time, and with
-// every workgroup finishing at the same moment nothing hides it: measured, those stores were 10-16 % of the GEMMs that split K
-// at batches 32-128 and 4-5 % at batch 512.  So the wavefronts that hold results scale them and park them in LDS as a
-// [column][row] tile (fp16 for the final output, fp32 for partial sums), and after a barrier every thread of the workgroup
-// stores 16 consecutive bytes of one column: a wavefront writes whole lines.
-//   stage: TN columns of TM rows, column stride TM * (2 or 4) + 16 bytes
-typedef _Float16 v4h __attribute__((ext_vector_type(4)));
-template <int NT, int RT, int WR> constexpr size_t tile_stage_bytes(bool partial) { return (size_t)NT * 16 * (WR * RT * 16 * (partial ? 4 : 2) + 16); }
-
-// first half: a wavefront that holds results scales them and parks them in the stage
-// (column tiles T0 .. T1-1 of it).  bias: of the tile's first row, or null; added before the one rounding to fp16
-template <int FM, int NT, int RT, int WR, typename OutT, int T0 = 0, int T1 = NT>
-__device__ __forceinline__ void tile_park(const v4f (&acc)[RT][NT], const v4h (&sc4)[RT], uint8_t *stage, int wr, int col, int q, const half_t *bias = nullptr)
-{
-    constexpr int TM = WR * RT * 16, kStride = TM * (int)sizeof(OutT) + 16;
-    v4h           b4[RT] = {};
-    if (sizeof(OutT) == 2 && bias) {
-#pragma unroll
-        for (int r = 0; r < RT; r++) {
-            const half_t *p = bias + (wr * RT + r) * 16 + 4 * q;
-            b4[r] = (v4h){ p[0], p[1], p[2], p[3] };
-        }
-    }
-#pragma unroll
-    for (int r = 0; r < RT; r++)
-#pragma unroll
-        for (int t = T0; t < T1; t++) {
-            v4f v;
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                v[i] = acc[r][t][i] * ((float)sc4[r][i] * Fmt<FM>::post_scale);
-                if constexpr (sizeof(OutT) == 2) v[i] += (float)b4[r][i]; // (one instruction with the scaling)
-            }
-            uint8_t *dst = stage + (16 * (t - T0) + col) * kStride + ((wr * RT + r) * 16 + 4 * q) * (int)sizeof(OutT);
-            if constexpr (sizeof(OutT) == 2)
-                *reinterpret_cast<v4h *>(dst) = (v4h){ (half_t)v[0], (half_t)v[1], (half_t)v[2], (half_t)v[3] };
-            else
-                *reinterpret_cast<v4f *>(dst) = v;
-        }
-}
-// second half, after a barrier: every thread of the workgroup stores 16-byte pieces of the stage's columns
-template <int NT, int RT, int WR, int NTHREADS, typename OutT>
-__device__ __forceinline__ void tile_flush(OutT *__restrict__ out, const uint8_t *stage, uint32_t M, uint32_t N, uint32_t mb, uint32_t nbase, int tid)
-{
-    constexpr int TM = WR * RT * 16, TN = NT * 16, kStride = TM * (int)sizeof(OutT) + 16, kPer16 = 16 / (int)sizeof(OutT); // outputs per 16 bytes
-    constexpr int kPiecesPerCol = TM / kPer16, kPieces = TN * kPiecesPerCol;
-#pragma unroll
-    for (int p = tid; p < kPieces; p += NTHREADS) {
-        const int      c = p / kPiecesPerCol, piece = p % kPiecesPerCol;
-        const uint32_t ng = nbase + c;
-        if (ng < N) {
-            const v4u d = *reinterpret_cast<const v4u *>(stage + c * kStride + piece * 16);
-            *reinterpret_cast<v4u *>(out + (size_t)ng * M + (size_t)mb * TM + piece * kPer16) = d;
-        }
-    }
-}
-
-template <int FM, int NT, int RT, int WR, int NTHREADS, typename OutT>
-__device__ __forceinline__ void tile_store(const v4f (&acc)[RT][NT], const v4h (&sc4)[RT], OutT *__restrict__ out, uint8_t *stage, bool holds_results,
-                                           uint32_t M, uint32_t N, uint32_t mb, uint32_t nbase, int tid, int wr, int col, int q, const half_t *bias)
-{
-    if (holds_results) tile_park<FM, NT, RT, WR, OutT>(acc, sc4, stage, wr, col, q, bias);
-    __syncthreads();
-    tile_flush<NT, RT, WR, NTHREADS, OutT>(out, stage, M, N, mb, nbase, tid);
-}
-
-// Workgroup id -> (row block, split, column block).  Ids that are congruent mod 8 run on one XCD and share its L2, so XCD x is given a
-// run of consecutive triples (the column blocks of a row block read the same weights, its splits write partial sums that one
-// reduction workgroup reads): the first (grid mod 8) XCDs take one triple more than the others.
-// Without a split the triples of the large tiles are counted in panels of 1024 rows, down the rows of a panel before the next column block:
-// the 32 or 64 workgroups that an XCD holds then cover about 1024 rows x 512-1024 columns, and what its L2 fetches for them is about
-// as small as it gets (with all the column blocks of one row block first, a long prompt's activations pass by once for every 256 or 512 rows).
-// Measured at FP6 e3m2, us, rows first -> panels: gemm_prefill 8192x8192 N 4096 582 -> 444, 14336x4096 N 3000 334 -> 306, 28672x8192 N 2048 832 -> 787;
-// gemm_ws 28672x8192 N 2048 914 -> 831, 8192x8192 N 4096 503 -> 472; gemm_tile 256 x 128 8192x8192 N 4096 488 -> 460
-// (forced: the dispatch gives some of these another shape).  What is fetched falls from 2267 to 784 MB (gemm_tile) and 4101 to 1629 (gemm_prefill 28672x8192).  Panels of 512, 2048 and 4096
-// rows: within 2 %, and up to 6 % behind.  128 x 32 tiles lose by 6 % and keep the rows.
-// In panels every XCD reads all the weights of a panel, by rows few XCDs read the same ones: activations that stay in an L2 of 4 MB anyway are no
-// reason for it (single rounds of 256-row tiles, K up to 1536: 0.8 us longer in panels with weights that come from memory, though less is fetched, 10.3 MB against
-// 14.6 at 1280x768 N 1658; level with weights that the caches hold).  Tiles of 256 rows are counted in panels where the activations take more than 2 MB, in a single round of the 256 CUs more than 4 MB and
-// with 128 workgroups at least (a few leave the order no part).  Time in panels / by rows on 440 problems (K 256 to 28288; activations kept and changed from
-// launch to launch), always -> by this rule: gemm_tile 256 x 64 1.02 (0.90-1.19) -> 0.99 (0.90-1.05), 256 x 128 0.99 (0.84-1.10) -> 0.98 (0.84-1.01),
-// gemm_ws 256 x 64 1.00 (0.87-1.11) -> 0.99 (0.87-1.04).  What it leaves to the rows was at most 4 % faster in panels, 1024x256 N 2537 1.18.  gemm_prefill
-// 0.98 (0.64-1.03) always.
-struct TileId { uint32_t mb, split, nb; };
-template <int TM, int TN> __device__ __forceinline__ TileId tile_of(uint32_t splitK, uint32_t nblocks, uint32_t N, uint32_t K)
-{
-    constexpr uint32_t kPanel = TM * TN >= 128 * 128 ? 1024 / TM : 1; // row blocks per panel
-    const uint32_t     q = gridDim.x >> 3, r = gridDim.x & 7u, x = blockIdx.x & 7u, id = x * q + (x < r ? x : r) + (blockIdx.x >> 3);
-    const uint64_t     X = (uint64_t)N * K * 2; // bytes of the activations
-    const bool         panels = kPanel > 1 && splitK == 1 && (TM < 256 || (gridDim.x > 256 ? X > 2u << 20 : gridDim.x >= 128 && X > 4u << 20));
-    if (panels) {
-        const uint32_t mblocks = gridDim.x / nblocks, first = id / (kPanel * nblocks) * kPanel, in = id - first * nblocks;
-        const uint32_t high = mblocks - first < kPanel ? mblocks - first : kPanel; // the last panel may be lower
-        return TileId{ first + in % high, 0, in / high };
-    }
-    const uint32_t rest = id / nblocks;
-    return TileId{ rest / splitK, rest % splitK, id % nblocks };
-}
-
 template <int FM, bool GS, int NT, int RT, int WR, int WK, bool BIAS>
 __global__ __launch_bounds__(WR *WK *kWave) void gemm_tile(const uint8_t *__restrict__ W, const half_t *__restrict__ scales,
                                                            const uint8_t *__restrict__ gexp, const half_t *__restrict__ X, half_t *__restrict__ C,
@@ -800,12 +153,6 @@ template <int FM, int NT, int RT, int WR, int SW, int SX> constexpr size_t ws_ri
 // problems of N 33 to 946 LDS / registers 0.89 (0.70-1.00).  With 256 rows LDS is full and SW is 2, one block ahead as in registers.
 template <bool GS, int WR> constexpr bool ws_exps_in_lds() { return GS && WR == 4; }
 template <bool GS, int RT, int WR, int SW> constexpr size_t ws_exps_ring_bytes() { return ws_exps_in_lds<GS, WR>() ? (size_t)SW * WR * RT * 64 : 0; }
-
-template <int N> __device__ __forceinline__ void wait_transfers_and_barrier()
-{
-    static_assert(N >= 0 && N <= 63, "s_waitcnt vmcnt holds six bits");
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
-}
 
 template <int FM, bool GS, int NT, int RT, int WR, int PW, int SW, int SX>
 __global__ __launch_bounds__((WR + PW) * kWave) void gemm_ws(const uint8_t *__restrict__ W, const half_t *__restrict__ scales,
@@ -1024,36 +371,6 @@ __global__ __launch_bounds__((WR + PW) * kWave) void gemm_ws(const uint8_t *__re
 // (FP5 with group exponents 4608x4544 N 777: 39.5 against 42.8).  Tiles of 256 x 128 (RT 8, 400+ registers, one wavefront per SIMD: 3-15 % slower than
 // gemm_tile's) and 256 x 256 (RT = NT = 8: spills) were left out.
 // ---------------------------------------------------------------------------------------------------------------
-// f(0), ..., f(RT - 1) with the index as a compile-time constant (a body this long is past what `#pragma unroll` takes)
-template <int RT, int R = 0, typename F> __device__ __forceinline__ void sections(const F &f)
-{
-    f(std::integral_constant<int, R>{});
-    if constexpr (R + 1 < RT) sections<RT, R + 1>(f);
-}
-
-struct RawHalf { v4u p; v2u s; uint32_t g; }; // one lane's codes of half a block of one row tile, as loaded (s, g: where the format has them)
-
-// raw codes of half H of a native block (and its group exponent): what field_string(., H) needs
-template <int FM, bool GS, int H> __device__ __forceinline__ void load_raw_half(RawHalf &f, const uint8_t *block, const uint8_t *gexp32, int lane)
-{
-    constexpr int kPiece = Fmt<FM>::bits == 6 ? 2048 : 1024; // the second half's 16-byte piece (6 bits: pieces a | b | c, b shared)
-    f.p = *reinterpret_cast<const v4u *>(block + H * kPiece + lane * 16);
-    if constexpr (Fmt<FM>::bits == 6) f.s = *reinterpret_cast<const v2u *>(block + 1024 + lane * 16 + 8 * H);
-    if constexpr (Fmt<FM>::bits == 5) f.s[0] = *reinterpret_cast<const uint32_t *>(block + 2048 + lane * 8 + 4 * H);
-    if constexpr (GS) f.g = gexp32[2 * (lane & 15) + H];
-}
-template <int FM, bool GS, int H> __device__ __forceinline__ v32h convert_raw_half(const RawHalf &f)
-{
-    v6u src;
-    if constexpr (Fmt<FM>::bits == 6)
-        src = H == 0 ? (v6u){ f.p[0], f.p[1], f.p[2], f.p[3], f.s[0], f.s[1] } : (v6u){ f.s[0], f.s[1], f.p[0], f.p[1], f.p[2], f.p[3] };
-    else if constexpr (Fmt<FM>::bits == 5)
-        src = fp5_expand(f.p[0], f.p[1], f.p[2], f.p[3], f.s[0]);
-    else
-        src = fp4_expand(f.p);
-    return fields_to_halfs<FM>(src, GS ? __builtin_bit_cast(float, f.g << 23) : 1.0f);
-}
-
 // (no __restrict__ on what the K loop reads: its loads must stay where the waits count them, on their side of the barriers)
 template <int FM, bool GS, int NT, int RT>
 __global__ __launch_bounds__(4 * kWave, 2) void gemm_prefill(const uint8_t *W, const half_t *__restrict__ scales, const uint8_t *gexp, const half_t *X,
@@ -1825,21 +1142,6 @@ __global__ __launch_bounds__(256) void quant_blocks(uint8_t *__restrict__ native
         quantize_block<FM, T, GROUPS, false>(x, sc, native, gexp, blk, K, U, lane);
 }
 // ------------------------------------------------------------------------------------------------ launch helpers
-
-// Lets `Kernel` use up to `bytes` of dynamic LDS.  The attribute belongs to the device's copy of the kernel: set once per device.
-template <auto Kernel> int allow_dynamic_lds(size_t bytes)
-{
-    static std::atomic<uint64_t> attr_set{ 0 }; // bit d: done on device d; setting it twice is harmless, so no lock
-    int                          dev = 0;
-    if (hipError_t e = hipGetDevice(&dev); e != hipSuccess) return (int)e;
-    const uint64_t bit = dev >= 0 && dev < 64 ? 1ull << dev : 0;
-    if (!(attr_set.load(std::memory_order_relaxed) & bit)) {
-        hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(Kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-        if (e != hipSuccess) return (int)e;
-        attr_set.fetch_or(bit, std::memory_order_relaxed);
-    }
-    return 0;
-}
 
 template <int FM, bool GS, int NT, int RT, int WAVES>
 int launch_stream(hipStream_t st, const void *W, const void *sc, const void *gexp, const void *B, void *C, float *ws, size_t M, size_t N, size_t K,

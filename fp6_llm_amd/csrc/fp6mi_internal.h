@@ -31,6 +31,27 @@ inline const FormatOps *ops_for(int E, int Mbits)
     return E == 3 ? &format_ops_32() : Mbits == 2 ? &format_ops_22() : Mbits == 3 ? &format_ops_23() : &format_ops_21();
 }
 
+// fp6mi_block.hip, compiled once per format: the kernels that read the same weights for another product
+struct BlockOps {
+    // dX[N,K] = dY[N,M] . dequant(W); gexp as above; premultiplied: dY holds its products with the mantissas of the row scales (fp6mi_scale.inc); ws: splits * N * K partial sums with
+    // splits > 1, which the caller reduces
+    int (*grad)(void *stream, const void *W, const void *sc, const void *gexp, const void *dY, bool premultiplied, void *dX, float *ws, size_t M, size_t N, size_t K, int splits);
+};
+const BlockOps &block_ops_32(), &block_ops_22(), &block_ops_23(), &block_ops_21();
+inline const BlockOps *block_ops_for(int E, int Mbits)
+{
+    return E == 3 ? &block_ops_32() : Mbits == 2 ? &block_ops_22() : Mbits == 3 ? &block_ops_23() : &block_ops_21();
+}
+
+// fp6mi_api.hip: parts of fp6mi_linear_native for the operators around it (fp6mi_ops.hip)
+int  check_linear(int E, int Mbits, const void *W, const void *sc, const void *gexp, const void *bias, const void *B, const void *C, size_t M, size_t N, size_t K, const float *ws, int splitK);
+int  current_cus();
+// the GEMM by the shape that fp6mi_linear_native takes; partial_only: with a split, the partial sums alone, [splitK][N][M] floats in ws (C is not touched)
+int  run_linear(int E, int Mbits, void *stream, const void *W, const void *sc, const void *gexp, const void *bias, const void *B, void *C, size_t M, size_t N, size_t K, float *ws, int splitK,
+                bool partial_only);
+// C[N,M] = fp16_rn(sum over splits of ws[s])
+int  reduce_partials(void *stream, void *C, const float *ws, size_t M, size_t N, int splits);
+
 // fp6mi_host.cpp
 int    prepack_ref(int E, int Mb, void *packed, const void *raw, size_t M, size_t K);
 int    unpack_ref(int E, int Mb, void *raw, const void *packed, size_t M, size_t K);

@@ -39,6 +39,7 @@ extern "C" {
 #define FP6MI_ERR_SPLITK (-5)    /* splitK < 1                              */
 #define FP6MI_ERR_ALIGN (-6)     /* a device pointer is not 16-byte aligned (scales, group exponents: 2-byte) */
 #define FP6MI_ERR_TOO_LARGE (-7) /* the problem exceeds the static workspace of fp6mi_linear_native_static */
+#define FP6MI_ERR_ACTIVATION (-9) /* not one of FP6MI_ACT_*                  */
 #define FP6MI_ERR_CAPTURE (-8)   /* the call would have to allocate while its stream is being captured */
 
 const char *fp6mi_error_string(int code);
@@ -219,6 +220,41 @@ int fp6mi_dequant_native_grouped_gpu(int E, int Mbits, void *stream, void *out_f
  * fp6mi_group_exps_bytes(M, K) bytes in native order. */
 int fp6mi_quantize_native_grouped_gpu(int E, int Mbits, void *stream, void *native_dev, void *scales_f16_dev,
                                       void *group_exps_native_dev, const void *weights_dev, int dtype, size_t M, size_t K);
+
+/* ---------------------------------------------------------------------------------- operators around the linear layer (beyond the reference)
+ * All of them take native-layout weights of M rows and K columns with row scales and, where group_exps_native is not NULL, group exponents; bias may be NULL. */
+
+/* Input gradient of the linear layer: dX[N,K] = dY[N,M] . (scale * 2^(b-127) * value)[M,K].  dY times the mantissa of its row's scale is rounded to fp16, the products are summed in
+ * FP32; a weight keeps its value but where value * 2^(b-127) times the power of two of its scale leaves fp16.  M up to 2^20.  splits > 1 cuts the sum over M into that many parts, whose partial sums take fp6mi_grad_workspace_bytes bytes. */
+int    fp6mi_linear_grad_native(int E, int Mbits, void *stream, const void *W_native, const void *scales_f16, const void *group_exps_native, const void *dY_f16,
+                                void *dX_f16, size_t M, size_t N, size_t K, float *workspace, int splits);
+int    fp6mi_heuristic_grad_splits(int E, int Mbits, size_t M, size_t N, size_t K, int num_cus);
+size_t fp6mi_grad_workspace_bytes(size_t N, size_t K, int splits);
+
+/* Gated feed-forward block: H[N,M/2] = act(B . Wg^T + bg) * (B . Wu^T + bu).  The two matrices are one of M rows in PAIR ORDER: 16 rows of Wg, the same 16 of Wu,
+ * and so on (scales, group exponents and bias likewise; in the native layout that is whole row tiles in turn).  preact, unless NULL, receives the
+ * pre-activations [N,M] in pair order, the FP32 sums as they are, for the backward pass.  workspace: fp6mi_gated_workspace_bytes bytes. */
+#define FP6MI_ACT_SILU 0
+#define FP6MI_ACT_GELU 1      /* g * P(g), P the normal distribution */
+#define FP6MI_ACT_GELU_TANH 2 /* its approximation by a hyperbolic tangent */
+int    fp6mi_gated_native(int E, int Mbits, void *stream, const void *W_native, const void *scales_f16, const void *group_exps_native, const void *bias_f16,
+                          const void *B_f16, void *H_f16, float *preact, size_t M, size_t N, size_t K, int activation, float *workspace, int splitK);
+size_t fp6mi_gated_workspace_bytes(size_t M, size_t N, int splitK);
+/* Its backward pass from the gradient of H: grad_preact[N,M] in pair order (the gradient that a bias sums over N, or an adapter beside the block takes; not written where it
+ * is NULL) and grad_in[N,K] = grad_preact . dequant(W).  The weights have no gradient.  workspace: fp6mi_gated_backward_workspace_bytes bytes, always; splits as in
+ * fp6mi_linear_grad_native. */
+int    fp6mi_gated_backward_native(int E, int Mbits, void *stream, const void *W_native, const void *scales_f16, const void *group_exps_native, const void *grad_out_f16,
+                                   const float *preact, void *grad_preact_f16, void *grad_in_f16, size_t M, size_t N, size_t K, int activation, float *workspace, int splits);
+size_t fp6mi_gated_backward_workspace_bytes(size_t M, size_t N, size_t K, int splits);
+
+/* The linear layer with a low-rank adapter for every batch row: C[n] = B[n] . W^T + bias + scaling[a] * (B[n] . A[a]^T) . Bm[a]^T with a = index[n]; a row whose index is
+ * no slot's number (-1, say) has none.  lora_a: fp16 [slots][R][K], lora_b: fp16 [slots][M][R], scaling: fp32 [slots], index: int32 [N], all on the device.  R is a multiple of 8 up
+ * to 256 (smaller ranks are padded with zeros).  The layer's output is rounded to fp16 before the adapter's part is added to it.  workspace: fp6mi_adapter_workspace_bytes
+ * bytes, always. */
+int    fp6mi_adapter_native(int E, int Mbits, void *stream, const void *W_native, const void *scales_f16, const void *group_exps_native, const void *bias_f16, const void *B_f16,
+                            void *C_f16, const void *lora_a_f16, const void *lora_b_f16, const float *scaling, const int *index, size_t M, size_t N, size_t K, size_t R, size_t slots,
+                            float *workspace, int splitK);
+size_t fp6mi_adapter_workspace_bytes(size_t M, size_t N, size_t K, size_t R, int splitK);
 
 #ifdef __cplusplus
 }
