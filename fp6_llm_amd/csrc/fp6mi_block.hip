@@ -1,6 +1,6 @@
 // gfx950 kernels around the FPx linear layer that read the native weight layout in another way than its GEMM, for ONE weight format per translation unit
 // (compiled like fp6mi_gemm.hip, with -DFP6MI_FORMAT=<10*E+M>).  No counterpart in the reference, whose only operator is the forward product.
-//   grad_tile   dX[N,K] = dY[N,M] . dequant(W)[M,K]: the input gradient of the linear layer
+//   grad_tile, grad_stream   dX[N,K] = dY[N,M] . dequant(W)[M,K]: the input gradient of the linear layer
 #include <hip/hip_runtime.h>
 
 #include <atomic>
@@ -28,15 +28,21 @@ namespace {
 // converted once per workgroup, written to LDS as rows, and read back by the transposing read (ds_read_b64_tr_b16: of a 4 x 16 piece, lane l of
 // sixteen gets column l).  Rows lie in LDS in the order in which those reads take them: row 8q + 4h + j of 32 is the (4q + j)-th of half h, 544 bytes apart, the
 // halves 16 bytes more, which leaves both the writes (eight rows, 16 bytes each) and the reads (eight rows, 32 bytes each) free of bank conflicts.
-// dY passes memory -> LDS without registers: piece p (16 bytes) of batch row n lies at slot p ^ swizzle(n) of its row.
-// Two stages, one barrier a chunk; weights are asked for two chunks ahead.
+// Piece p (16 bytes) of batch row n of dY lies at slot p ^ swizzle(n) of its row.  It passes through registers, where the mantissas are multiplied in.  (Behind a transfer straight to LDS
+// the compiler holds the next transposing read back until the transfer is there.)
+// What bounds it: with 128 x 128 outputs a wavefront (256 x 256 a workgroup, one wavefront to a SIMD) the MFMAs, of which 64 take an operand read of 24 KB; the LDS unit is busy for a third
+// of the time, bank conflicts are none.  What was gained on the way, 8192x8192 N 4096, us: 256 x 128 tiles, operands read as they are multiplied 1414; read a step ahead 498;
+// 256 x 256 466; other instructions spread between the MFMAs 448 (1.23 PFLOP/s; the fp16 library product of the card reaches 1.41).  22016x4096 N 4096 598, N 512 105 (8 splits),
+// 4608x4544 N 333 33 (4 splits).  Left out: 256 x 128 with two workgroups of four wavefronts to a CU (515) and chunks of 32 rows.
+// Two stages, one barrier a chunk.
 // ---------------------------------------------------------------------------------------------------------------
 typedef short v4s __attribute__((ext_vector_type(4)));
 typedef _Float16 v4hh __attribute__((ext_vector_type(4)));
 
 constexpr int kGradRow = 544, kGradHalf = 16 * kGradRow + 16, kGrad32 = 2 * kGradHalf; // bytes of a row, of 16 rows, of 32
-template <int NT, int WN, int OCC> struct GradTile {
-    static constexpr int TN = NT * WN * 16, kWStage = OCC / 32 * kGrad32, kXStage = TN * OCC * 2, kMant = kWStage + kXStage, kStage = kMant + OCC * 2;
+constexpr int kGradRows = 64; // weight rows of a chunk
+template <int NT, int WN> struct GradTile {
+    static constexpr int TN = NT * WN * 16, kWStage = kGradRows / 32 * kGrad32, kXStage = TN * kGradRows * 2, kStage = kWStage + kXStage;
     static constexpr int kOutFull = TN * (512 + 16), kOutPart = NT * 16 * (1024 + 16);
     static constexpr int kLds = 2 * kStage > kOutFull ? (2 * kStage > kOutPart ? 2 * kStage : kOutPart) : (kOutFull > kOutPart ? kOutFull : kOutPart);
 };
@@ -52,18 +58,17 @@ template <int FM, int H> __device__ __forceinline__ v6u raw_half_fields(const Ra
         return fp4_expand(f.p);
 }
 
-// What the conversion of a row's codes applies, 2^(e + b - 127) (and the factor that the format's fields owe), and the rest of its scale.  A scale that is zero, infinite or no number is
-// all mantissa.  (Powers of two beyond what the instruction takes have long left fp16.)
-template <int FM, bool GS> __device__ __forceinline__ float grad_factor(half_t scale, uint32_t g, half_t &mantissa)
+// One lane's 32 weights of a row (fields: their codes; g: the exponent byte of their group) as they are multiplied: value * 2^(b-127) * 2^e, e the exponent of the row's scale, which
+// the conversion instruction applies.  (Powers of two beyond what it takes have long left fp16.)
+template <int FM, bool GS> __device__ __forceinline__ v32h grad_weights(v6u fields, half_t scale, uint32_t g)
 {
-    int e = 0;
-    mantissa = split_scale(scale, e);
-    if constexpr (Fmt<FM>::post_scale == 4.0f) e += 2;
     static_assert(Fmt<FM>::post_scale == 1.0f || Fmt<FM>::post_scale == 4.0f, "a power of two");
-    int field = e + (GS ? (int)g : 127);
-    field = field < 0 ? 0 : field > 254 ? 254 : field;
-    return __builtin_bit_cast(float, (uint32_t)field << 23);
+    int field = scale_exponent(scale) + (Fmt<FM>::post_scale == 4.0f ? 2 : 0) + (GS ? (int)g : 127);
+    if constexpr (GS) field = field < 0 ? 0 : field > 254 ? 254 : field;
+    return fields_to_halfs<FM>(fields, __builtin_bit_cast(float, (uint32_t)field << 23));
 }
+
+__device__ __forceinline__ void wait_lds_and_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 // one lane's 4 x 16-bit share of a transposing read
 __device__ __forceinline__ v4hh read_transposed(const uint8_t *p)
@@ -72,18 +77,17 @@ __device__ __forceinline__ v4hh read_transposed(const uint8_t *p)
     return __builtin_bit_cast(v4hh, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s *)(p)));
 }
 
-template <int FM, bool GS, bool PRE, int NT, int WN, int OCC>
-__global__ __launch_bounds__(2 * WN *kWave) void grad_tile(const uint8_t *W, const half_t *scales, const uint8_t *gexp, const half_t *dY, half_t *__restrict__ dX,
+template <int FM, bool GS, bool PRE, int NT, int WN>
+__global__ __launch_bounds__(2 * WN *kWave, NT >= 6 ? 1 : 2) void grad_tile(const uint8_t *W, const half_t *scales, const uint8_t *gexp, const half_t *dY, half_t *__restrict__ dX,
                                                            float *__restrict__ ws, uint32_t M, uint32_t N, uint32_t K, uint32_t units, uint32_t splits,
                                                            uint32_t nblocks)
 {
-    typedef GradTile<NT, WN, OCC> T;
+    typedef GradTile<NT, WN> T;
     constexpr int TN = T::TN, RT = 8, WAVES = 2 * WN, NTHREADS = WAVES * kWave;
-    constexpr int kPieces = OCC / 8;                    // 16-byte pieces of a batch row of a stage
-    constexpr int kRowsPer = 64 / kPieces;              // batch rows of one transfer
-    constexpr int kDma = TN / kRowsPer / WAVES, kUnits = OCC / 16 * 2 / WAVES; // transfers, and half blocks to convert, of a wavefront
-    static_assert(kDma * WAVES * kRowsPer == TN && kUnits * WAVES == OCC / 8, "every wavefront does the same share");
-    constexpr int kLoads = kUnits * ((Fmt<FM>::bits == 4 ? 1 : 2) + (GS ? 1 : 0) + 1); // (codes, group exponent, row scale)
+    constexpr int OCC = kGradRows, kPieces = OCC / 8;                    // 16-byte pieces of a batch row of a stage
+    constexpr int kRowsPer = 64 / kPieces;              // batch rows of one load
+    constexpr int kX = TN / kRowsPer / WAVES, kUnits = OCC / 16 * 2 / WAVES; // loads of dY, and half blocks to convert, of a wavefront
+    static_assert(kX * WAVES * kRowsPer == TN && kUnits * WAVES == OCC / 8, "every wavefront does the same share");
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -104,104 +108,167 @@ __global__ __launch_bounds__(2 * WN *kWave) void grad_tile(const uint8_t *W, con
 #pragma unroll
         for (int t = 0; t < NT; t++) acc[r][t] = (v4f){ 0.f, 0.f, 0.f, 0.f };
 
-    // half blocks of this wavefront: number u = wave + WAVES * i of a chunk is half u & 1 of row tile u >> 1
-    struct Raw { RawHalf h; half_t sc; };
-    auto load_raw = [&](Raw &f, int i, uint32_t c) __attribute__((always_inline)) {
-        const uint32_t R = c * (OCC / 16) + ((wave + WAVES * i) >> 1);
-        const size_t   blk = (size_t)R * units + kb;
-        if (wi == 0)
-            load_raw_half<FM, GS, 0>(f.h, W + blk * Fmt<FM>::block_bytes, GS ? gexp + blk * 32 : nullptr, lane);
-        else
-            load_raw_half<FM, GS, 1>(f.h, W + blk * Fmt<FM>::block_bytes, GS ? gexp + blk * 32 : nullptr, lane);
-        f.sc = scales[R * 16 + col];
+    // What is fetched for a chunk, from pointers that go from chunk to chunk and stay at the last one: past the end it is fetched, converted and stored once more, and not used.
+    // Half blocks: number u = wave + WAVES * i of a chunk is half wi = u & 1 of row tile u >> 1.
+    const uint32_t wstep = units * Fmt<FM>::block_bytes, lane16 = lane * 16, lane8 = lane * 8, col2 = col * 2;
+    const uint8_t *wp = W + (size_t)(c0 * (OCC / 16) + (wave >> 1)) * wstep + (size_t)kb * Fmt<FM>::block_bytes;
+    const uint8_t *gp = GS ? gexp + ((size_t)(c0 * (OCC / 16) + (wave >> 1)) * units + kb) * 32 : nullptr;
+    const uint8_t *sp = reinterpret_cast<const uint8_t *>(scales) + ((size_t)c0 * OCC + (wave >> 1) * 16) * 2;
+    uint32_t       wleft = c1 - c0;
+    auto           load_codes = [&](auto half_c, RawHalf &f, half_t &sc, int i) __attribute__((always_inline)) {
+        constexpr int  H = decltype(half_c)::value, kPiece = Fmt<FM>::bits == 6 ? 2048 : 1024; // pieces as in load_raw_half
+        const uint8_t *block = wp + (size_t)(WAVES / 2 * i) * wstep;
+        f.p = *reinterpret_cast<const v4u *>(block + H * kPiece + lane16);
+        if constexpr (Fmt<FM>::bits == 6) f.s = *reinterpret_cast<const v2u *>(block + 1024 + 8 * H + lane16);
+        if constexpr (Fmt<FM>::bits == 5) f.s[0] = *reinterpret_cast<const uint32_t *>(block + 2048 + 4 * H + lane8);
+        if constexpr (GS) f.g = gp[(size_t)(WAVES / 2 * i) * units * 32 + H + col2];
+        sc = *reinterpret_cast<const half_t *>(sp + WAVES / 2 * i * 32 + col2);
     };
-    auto store_w = [&](const Raw &f, int i, uint32_t stage) __attribute__((always_inline)) {
-        const int rt = (wave + WAVES * i) >> 1, o = 16 * (rt & 1) + col; // row within 32
-        uint8_t  *dst = lds + stage * T::kStage + (rt >> 1) * kGrad32 + ((o >> 2) & 1) * kGradHalf + (4 * (o >> 3) + (o & 3)) * kGradRow + wi * 256 + q * 16;
-        half_t       mantissa;
-        const float  factor = grad_factor<FM, GS>(f.sc, f.h.g, mantissa);
-        const v32h   v = fields_to_halfs<FM>(wi == 0 ? raw_half_fields<FM, 0>(f.h) : raw_half_fields<FM, 1>(f.h), factor);
-#pragma unroll
-        for (int s = 0; s < 4; s++) *reinterpret_cast<v8h *>(dst + 64 * s) = slice8(v, s);
-        if (!PRE && wi == 0 && q == 0) *reinterpret_cast<half_t *>(lds + stage * T::kStage + T::kMant + (rt * 16 + col) * 2) = mantissa;
+    auto next_codes = [&]() __attribute__((always_inline)) {
+        const bool more = --wleft > 0 && wleft < 0x80000000u;
+        wp += more ? (size_t)(OCC / 16) * wstep : 0;
+        if constexpr (GS) gp += more ? (size_t)(OCC / 16) * units * 32 : 0;
+        sp += more ? OCC * 2 : 0;
     };
-
-    // transfer j of this wavefront fills batch rows kRowsPer * (wave + WAVES * j) .. of a stage; rows beyond N repeat the last one (never stored)
-    typedef __attribute__((address_space(3))) void lvoid;
-    auto swizzle = [](uint32_t n) { return kPieces == 8 ? n & 7 : (n >> 1) & 3; };
-    const uint32_t xrow = lane / kPieces, xlast = N - nbase < (uint32_t)TN ? N - 1 - nbase : TN - 1;
-    const auto     xbuf = __builtin_amdgcn_make_buffer_rsrc(const_cast<half_t *>(dY + (size_t)nbase * M), 0, (int)((xlast + 1) * M * 2), 0x00027000); // (the launcher bounds M)
-    auto           transfer = [&](int j, uint32_t c, uint32_t stage) __attribute__((always_inline)) {
-        uint32_t       n = kRowsPer * (wave + WAVES * j) + xrow;
-        const uint32_t piece = (lane % kPieces) ^ swizzle(n);
-        n = n < xlast ? n : xlast;
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(xbuf, (lvoid *)(lds + stage * T::kStage + T::kWStage + (wave + WAVES * j) * 1024), 16,
-                                                 n * M * 2 + c * (OCC * 2) + piece * 16, 0, 0, 0);
+    v32h           converted;
+    uint8_t *const wdst = lds + ((col >> 2) & 1) * kGradHalf + (4 * (col >> 3) + (col & 3)) * kGradRow + wi * 256 + q * 16; // row o = 16 * (rt & 1) + col of 32 is the (4 (o / 8) + o % 4)-th of its half
+    auto           write_w = [&](int i, int s, int stage) __attribute__((always_inline)) {
+        const int rt = (wave + WAVES * i) >> 1;
+        *reinterpret_cast<v8h *>(wdst + stage * T::kStage + (rt >> 1) * kGrad32 + (rt & 1) * 8 * kGradRow + 64 * s) = slice8(converted, s);
     };
 
-    const uint8_t *wread = lds + (4 * q + (col >> 2)) * kGradRow + (col & 3) * 8 + wi * 256;
-    auto           compute = [&](uint32_t stage) __attribute__((always_inline)) {
+    // batch rows: load j of this wavefront is of rows kRowsPer * (wave + WAVES * j) ..; rows beyond N repeat the last one (never stored)
+    auto           swizzle = [](uint32_t n) { return n & 7; };
+    const uint32_t xrow = lane / kPieces, xpiece = ((lane % kPieces) ^ swizzle(xrow)) * 16, nlast = N - nbase < (uint32_t)TN ? N - 1 - nbase : TN - 1;
+    uint32_t       xoff[kX]; // 32 bits: the launcher bounds M
 #pragma unroll
-        for (int kk = 0; kk < OCC / 32; kk++) {
-            v8h a[RT], b[NT];
-#pragma unroll
-            for (int t = 0; t < NT; t++) {
-                const int n = (wn * NT + t) * 16 + col;
-                b[t] = *reinterpret_cast<const v8h *>(lds + stage * T::kStage + T::kWStage + n * (OCC * 2) + (((4 * kk + q) ^ swizzle(n)) * 16));
-            }
-            if constexpr (!PRE) {
-                const v8h mant = *reinterpret_cast<const v8h *>(lds + stage * T::kStage + T::kMant + (32 * kk + 8 * q) * 2);
-#pragma unroll
-                for (int t = 0; t < NT; t++) b[t] = b[t] * mant;
-            }
-#pragma unroll
-            for (int r = 0; r < RT; r++) {
-                const uint8_t *p = wread + stage * T::kStage + kk * kGrad32 + r * 32;
-                const v4hh     lo = read_transposed(p), hi = read_transposed(p + kGradHalf);
-                a[r] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-            }
-#pragma unroll
-            for (int r = 0; r < RT; r++)
-#pragma unroll
-                for (int t = 0; t < NT; t++) acc[r][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[r], b[t], acc[r][t], 0, 0, 0);
-        }
-    };
-
-    if (c0 < c1) { // (more splits than chunks leave some empty: their partial sums are zeros)
-        Raw even[kUnits], odd[kUnits];
-#pragma unroll
-        for (int i = 0; i < kUnits; i++) load_raw(even[i], i, c0);
-#pragma unroll
-        for (int j = 0; j < kDma; j++) transfer(j, c0, 0);
-#pragma unroll
-        for (int i = 0; i < kUnits; i++) load_raw(odd[i], i, c0 + 1 < c1 ? c0 + 1 : c0);
-#pragma unroll
-        for (int i = 0; i < kUnits; i++) store_w(even[i], i, 0);
-        wait_transfers_and_barrier<0>();
-        // chunk c from stage `st`; `cur` holds the codes of the next one.  (After the last chunk one is fetched and converted once more, and not used: every chunk
-        // has the same waits.  Two copies of the code, so that codes on their way are never moved between registers.)
-        auto chunk = [&](auto st_c, uint32_t c, Raw(&cur)[kUnits], Raw(&after)[kUnits]) __attribute__((always_inline)) {
-            constexpr int  st = decltype(st_c)::value;
-            const uint32_t ct = c + 1 < c1 ? c + 1 : c, cr = c + 2 < c1 ? c + 2 : c1 - 1;
-#pragma unroll
-            for (int j = 0; j < kDma; j++) transfer(j, ct, st ^ 1);
-            __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int i = 0; i < kUnits; i++) load_raw(after[i], i, cr);
-            __builtin_amdgcn_sched_barrier(0);
-            compute(st);
-#pragma unroll
-            for (int i = 0; i < kUnits; i++) store_w(cur[i], i, st ^ 1);
-            wait_transfers_and_barrier<kLoads>();
-        };
-        typedef std::integral_constant<int, 0> Stage0;
-        typedef std::integral_constant<int, 1> Stage1;
-        for (uint32_t c = c0; c < c1; c += 2) {
-            chunk(Stage0{}, c, odd, even);
-            if (c + 1 < c1) chunk(Stage1{}, c + 1, even, odd);
-        }
+    for (int j = 0; j < kX; j++) {
+        const uint32_t n = kRowsPer * (wave + WAVES * j) + xrow;
+        xoff[j] = (n < nlast ? n : nlast) * M * 2 + xpiece;
     }
-    wait_transfers_and_barrier<0>(); // nothing is on its way to LDS any more, and nobody reads operands
+    const uint8_t *xp = reinterpret_cast<const uint8_t *>(dY + (size_t)nbase * M + (size_t)c0 * OCC), *ep = reinterpret_cast<const uint8_t *>(scales + (size_t)c0 * OCC);
+    uint32_t       xleft = c1 - c0;
+    v4u            xr[kX], xs; // xs: the scales of this lane's eight rows of a chunk
+    const bool     scales_aligned = (reinterpret_cast<uintptr_t>(scales) & 15u) == 0;
+    auto           load_x = [&]() __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < kX; j++) xr[j] = *reinterpret_cast<const v4u *>(xp + xoff[j]);
+        if constexpr (!PRE) {
+            if (scales_aligned) {
+                xs = *reinterpret_cast<const v4u *>(ep + xpiece);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; i++) xs[i] = *reinterpret_cast<const uint16_t *>(ep + xpiece + 4 * i) | (uint32_t)*reinterpret_cast<const uint16_t *>(ep + xpiece + 4 * i + 2) << 16;
+            }
+        }
+        const bool more = --xleft > 0 && xleft < 0x80000000u;
+        xp += more ? OCC * 2 : 0, ep += more ? OCC * 2 : 0;
+    };
+    auto store_x = [&](int stage) __attribute__((always_inline)) {
+        if constexpr (!PRE)
+            scale_mantissas(xs);
+#pragma unroll
+        for (int j = 0; j < kX; j++) {
+            if constexpr (!PRE) xr[j] = __builtin_bit_cast(v4u, __builtin_bit_cast(v8h, xr[j]) * __builtin_bit_cast(v8h, xs));
+            *reinterpret_cast<v4u *>(lds + stage * T::kStage + T::kWStage + (wave + WAVES * j) * 1024 + lane16) = xr[j];
+        }
+    };
+
+    // Operands of one MFMA step (32 rows).  A step is RT groups of NT MFMAs; behind a group's MFMAs its weights are replaced by the next step's, and the first half of the groups read
+    // the next step's batch rows into the other set.
+    v8h            a[RT], b[2][NT];
+    const uint8_t *wread = lds + (4 * q + (col >> 2)) * kGradRow + (col & 3) * 8 + wi * 256;
+    auto           read_a = [&](int r, int stage, int kk) __attribute__((always_inline)) {
+        const uint8_t *p = wread + stage * T::kStage + kk * kGrad32 + r * 32;
+        a[r] = __builtin_shufflevector(read_transposed(p), read_transposed(p + kGradHalf), 0, 1, 2, 3, 4, 5, 6, 7);
+    };
+    auto read_b = [&](auto set_c, int t, int stage, int kk) __attribute__((always_inline)) {
+        const int n = (wn * NT + t) * 16 + col;
+        b[decltype(set_c)::value][t] = *reinterpret_cast<const v8h *>(lds + stage * T::kStage + T::kWStage + n * (OCC * 2) + (((4 * kk + q) ^ swizzle(col)) * 16));
+    };
+    auto run = [&](auto half_c) __attribute__((always_inline)) {
+        typedef std::integral_constant<int, 0> Zero;
+        typedef std::integral_constant<int, 1> One;
+        constexpr int H = decltype(half_c)::value;
+        // a chunk is converted and stored in its predecessor's first step; the next one's batch rows and codes are asked for right behind
+        RawHalf raw[kUnits];
+        half_t  rsc[kUnits];
+#pragma unroll
+        for (int i = 0; i < kUnits; i++) load_codes(half_c, raw[i], rsc[i], i);
+        next_codes();
+        load_x();
+#pragma unroll
+        for (int i = 0; i < kUnits; i++) {
+            converted = grad_weights<FM, GS>(raw_half_fields<FM, H>(raw[i]), rsc[i], raw[i].g);
+#pragma unroll
+            for (int j = 0; j < 4; j++) write_w(i, j, 0);
+        }
+        store_x(0);
+#pragma unroll
+        for (int i = 0; i < kUnits; i++) load_codes(half_c, raw[i], rsc[i], i);
+        next_codes();
+        load_x();
+        wait_lds_and_barrier();
+#pragma unroll
+        for (int t = 0; t < NT; t++) read_b(Zero{}, t, 0, 0);
+#pragma unroll
+        for (int r = 0; r < RT; r++) read_a(r, 0, 0);
+        // A chunk, two steps, lies in stage `st`.  Its second step begins with the chunk's barrier: what it multiplies is in registers by then, so stage `st` is free for the next chunk but
+        // one, and the next chunk is there, whose first step is read now.
+        auto chunk = [&](auto st_c) __attribute__((always_inline)) {
+            constexpr int st = decltype(st_c)::value;
+            sections<2>([&](auto kk_c) __attribute__((always_inline)) {
+                constexpr int  kk = decltype(kk_c)::value;
+                constexpr bool last = kk == 1;
+                typedef std::integral_constant<int, kk ^ 1> Next;
+                if constexpr (last) wait_lds_and_barrier();
+                __builtin_amdgcn_sched_barrier(0);
+                sections<RT>([&](auto r_c) __attribute__((always_inline)) {
+                    constexpr int r = decltype(r_c)::value, rs = last ? st ^ 1 : st, rk = last ? 0 : kk + 1, kHalfRT = RT / 2;
+                    if constexpr (r < kHalfRT) {
+#pragma unroll
+                        for (int t = r * NT / kHalfRT; t < (r + 1) * NT / kHalfRT; t++) read_b(Next{}, t, rs, rk);
+                    }
+                    if constexpr (kk == 0) { // half blocks to convert: each takes RT / kUnits groups, one for the conversion and two for its writes
+                        constexpr int per = RT / kUnits, i = r / per, g = r % per, dst = st ^ 1;
+                        static_assert(per >= 4, "a conversion, its writes and the next loads need four groups");
+                        if constexpr (g == 0) converted = grad_weights<FM, GS>(raw_half_fields<FM, H>(raw[i]), rsc[i], raw[i].g);
+                        if constexpr (g == 1) {
+#pragma unroll
+                            for (int s = 0; s < 2; s++) write_w(i, s, dst);
+                        }
+                        if constexpr (g == 2) {
+#pragma unroll
+                            for (int s = 2; s < 4; s++) write_w(i, s, dst);
+                        }
+                        if constexpr (g == 3) load_codes(half_c, raw[i], rsc[i], i);
+                        if constexpr (r == RT - 2) store_x(dst);
+                        if constexpr (r == RT - 1) next_codes(), load_x();
+                    }
+#pragma unroll
+                    for (int t = 0; t < NT; t++) acc[r][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[r], b[kk][t], acc[r][t], 0, 0, 0);
+                    read_a(r, rs, rk);
+#pragma unroll
+                    for (int t = 0; t < NT; t++) { // one other instruction behind every MFMA, as far as they go (8192x8192 N 4096 in 256 x 256 tiles: 466 -> 448 us)
+                        __builtin_amdgcn_sched_group_barrier(0x08, 1, 0);
+                        __builtin_amdgcn_sched_group_barrier(0xA6, 1, 0);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                });
+            });
+        };
+        for (uint32_t c = c0; c < c1; c += 2) {
+            chunk(Zero{});
+            if (c + 1 < c1) chunk(One{});
+        }
+    };
+    if (c0 < c1) { // (more splits than chunks leave some empty: their partial sums are zeros)
+        if (wi == 0)
+            run(std::integral_constant<int, 0>{});
+        else
+            run(std::integral_constant<int, 1>{});
+    }
+    __syncthreads(); // nobody reads operands any more
 
     // acc[r][t][i]: input feature 256 kb + 128 wi + 16 r + 4 q + i of batch row nbase + 16 (wn NT + t) + col.  Out through LDS as in the other tile kernels.
     const uint32_t k0 = kb * 256;
@@ -236,37 +303,174 @@ __global__ __launch_bounds__(2 * WN *kWave) void grad_tile(const uint8_t *W, con
     }
 }
 
-template <int FM, bool GS, bool PRE, int NT, int WN, int OCC>
+// ---------------------------------------------------------------------------------------------------------------
+// grad_stream: the same product for up to 32 batch rows, where the weights' way from memory is the bound.
+//   grid = (blocks of 256 input features, splits)   block = WO wavefronts, which share the weight rows of a split among them, 32 rows (two native blocks) at a time in turn
+// Every wavefront is by itself until the end: it converts two native blocks, half of their columns after the other, into an LDS area of its own (rows 288 bytes apart, in grad_tile's
+// order; no barrier, the LDS unit serves a wavefront in order), reads them back transposed, and takes its batch rows from memory in operand order.  The codes of the next
+// 32 rows are asked for before this one's are converted.  Sums meet in LDS.  us, with the reduction of the splits, e3m2: 4096x4096 N 8 11.1 (16 splits), 8192x8192 N 1 15.7 (8), 22016x4096
+// N 8 21.7 (16, 3.1 TB/s).  Half blocks a wavefront, with more of them: 13.3, 35.6 and 47.0 (the codes that the halves share were fetched by two XCDs).
+// ---------------------------------------------------------------------------------------------------------------
+constexpr int kStreamRow = 288, kStreamHalf = 16 * kStreamRow + 16, kStreamMant = 2 * kStreamHalf, kStreamWave = kStreamMant + 64;
+template <int NT, int WO> constexpr int grad_stream_lds() { return WO * (NT * 8192 > kStreamWave ? NT * 8192 : kStreamWave); }
+
+template <int FM, bool GS, bool PRE, int NT, int WO>
+__global__ __launch_bounds__(WO *kWave) void grad_stream(const uint8_t *__restrict__ W, const half_t *__restrict__ scales, const uint8_t *__restrict__ gexp, const half_t *__restrict__ dY,
+                                                         half_t *__restrict__ dX, float *__restrict__ ws, uint32_t M, uint32_t N, uint32_t K, uint32_t units, uint32_t splits)
+{
+    constexpr int RT = 8, kWaveLds = grad_stream_lds<NT, WO>() / WO;
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    const int      tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 15, q = lane >> 4;
+    const uint32_t kb = blockIdx.x, split = blockIdx.y, chunks = M / 32;
+    const uint32_t avg = chunks / splits, extra = chunks % splits, c0 = split * avg + (split < extra ? split : extra), c1 = c0 + avg + (split < extra ? 1u : 0u);
+    uint8_t       *mine = lds + wave * kWaveLds;
+
+    v4f acc[2][RT][NT];
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+#pragma unroll
+        for (int r = 0; r < RT; r++)
+#pragma unroll
+            for (int t = 0; t < NT; t++) acc[h][r][t] = (v4f){ 0.f, 0.f, 0.f, 0.f };
+
+    struct Raw { WFrag<FM> w[2]; uint32_t g[2]; half_t sc[2]; v8h b[NT]; };
+    auto load = [&](Raw &f, uint32_t c) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const size_t blk = (size_t)(2 * c + i) * units + kb;
+            f.w[i] = load_wfrag<FM>(W + blk * Fmt<FM>::block_bytes, lane);
+            f.g[i] = load_group_exps<GS>(gexp, blk, lane);
+            f.sc[i] = scales[c * 32 + 16 * i + col];
+        }
+#pragma unroll
+        for (int t = 0; t < NT; t++) { // (rows beyond N repeat the last one and are not stored)
+            const uint32_t n = 16 * t + col < N ? 16 * t + col : N - 1;
+            f.b[t] = *reinterpret_cast<const v8h *>(dY + (size_t)n * M + c * 32 + 8 * q);
+        }
+    };
+    // (reads of other lanes' writes: the LDS unit serves a wavefront in order, the compiler has to leave them in this one)
+    auto in_order = [] {
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    };
+    uint8_t *const       wdst = mine + (col >> 2 & 1) * kStreamHalf + (4 * (col >> 3) + (col & 3)) * kStreamRow + q * 16;
+    const uint8_t *const wread = mine + (4 * q + (col >> 2)) * kStreamRow + (col & 3) * 8;
+    auto                 multiply = [&](Raw &f) __attribute__((always_inline)) {
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+#pragma unroll
+            for (int i = 0; i < 2; i++) { // row 16 i + col of 32: the (4 (2 i + col / 8) + col % 4)-th of its half
+                const v32h v = grad_weights<FM, GS>(field_string<FM>(f.w[i], h), f.sc[i], h == 0 ? f.g[i] & 0xffu : f.g[i] >> 8);
+#pragma unroll
+                for (int s = 0; s < 4; s++) *reinterpret_cast<v8h *>(wdst + i * 8 * kStreamRow + 64 * s) = slice8(v, s);
+                if (!PRE && h == 0 && q == 0) *reinterpret_cast<half_t *>(mine + kStreamMant + (16 * i + col) * 2) = scale_mantissa(f.sc[i]);
+            }
+            in_order();
+            if constexpr (!PRE) {
+                if (h == 0) {
+                    const v8h mant = *reinterpret_cast<const v8h *>(mine + kStreamMant + 16 * q);
+#pragma unroll
+                    for (int t = 0; t < NT; t++) f.b[t] = f.b[t] * mant;
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < RT; r++) {
+                const v8h a = __builtin_shufflevector(read_transposed(wread + r * 32), read_transposed(wread + kStreamHalf + r * 32), 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+                for (int t = 0; t < NT; t++) acc[h][r][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, f.b[t], acc[h][r][t], 0, 0, 0);
+            }
+            in_order();
+        }
+    };
+    Raw      even, odd;
+    uint32_t c = c0 + wave;
+    if (c < c1) load(even, c);
+    while (c < c1) {
+        if (c + WO < c1) load(odd, c + WO);
+        multiply(even);
+        c += WO;
+        if (c >= c1) break;
+        if (c + WO < c1) load(even, c + WO);
+        multiply(odd);
+        c += WO;
+    }
+
+    // 128 input features at a time, every wavefront parks its sums in its own area: [r][t][lane] of four input features
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        if (h == 1) __syncthreads();
+#pragma unroll
+        for (int r = 0; r < RT; r++)
+#pragma unroll
+            for (int t = 0; t < NT; t++) *reinterpret_cast<v4f *>(mine + (r * NT + t) * 1024 + lane * 16) = acc[h][r][t];
+        __syncthreads();
+        for (int p = tid; p < NT * 512; p += WO * kWave) { // input features 4 f .. of the 128, batch row n
+            const uint32_t f = p & 31, n = p >> 5, k = kb * 256 + h * 128 + 4 * f;
+            const uint8_t *src = lds + ((f >> 2) * NT + (n >> 4)) * 1024 + ((f & 3) * 16 + (n & 15)) * 16;
+            v4f            sum = *reinterpret_cast<const v4f *>(src);
+#pragma unroll
+            for (int w = 1; w < WO; w++) sum += *reinterpret_cast<const v4f *>(src + w * kWaveLds);
+            if (n < N && k < K) {
+                if (splits == 1)
+                    *reinterpret_cast<v4hh *>(dX + (size_t)n * K + k) = (v4hh){ (half_t)sum[0], (half_t)sum[1], (half_t)sum[2], (half_t)sum[3] };
+                else
+                    *reinterpret_cast<v4f *>(ws + ((size_t)split * N + n) * K + k) = sum;
+            }
+        }
+    }
+}
+
+template <int FM, bool GS, bool PRE, int NT, int WO>
+int launch_grad_stream(hipStream_t st, const void *W, const void *sc, const void *gexp, const void *dY, void *dX, float *ws, size_t M, size_t N, size_t K, int splits)
+{
+    constexpr int kLds = grad_stream_lds<NT, WO>();
+    static_assert(kLds <= 160 * 1024, "the wavefronts' areas do not fit in LDS");
+    const uint32_t units = (uint32_t)((K + 255) / 256);
+    if (kLds > 48 * 1024)
+        if (int rc = allow_dynamic_lds<&grad_stream<FM, GS, PRE, NT, WO>>(kLds)) return rc;
+    hipLaunchKernelGGL((grad_stream<FM, GS, PRE, NT, WO>), dim3(units, (uint32_t)splits), dim3(WO * kWave), kLds, st, static_cast<const uint8_t *>(W), static_cast<const half_t *>(sc),
+                       static_cast<const uint8_t *>(gexp), static_cast<const half_t *>(dY), static_cast<half_t *>(dX), ws, (uint32_t)M, (uint32_t)N, (uint32_t)K, units, (uint32_t)splits);
+    return (int)hipGetLastError();
+}
+
+template <int FM, bool GS, bool PRE, int NT, int WN>
 int launch_grad(hipStream_t st, const void *W, const void *sc, const void *gexp, const void *dY, void *dX, float *ws, size_t M, size_t N, size_t K, int splits)
 {
-    typedef GradTile<NT, WN, OCC> T;
+    typedef GradTile<NT, WN> T;
     static_assert(T::kLds <= 160 * 1024, "tile does not fit in LDS");
     const uint32_t units = (uint32_t)((K + 255) / 256), nblocks = (uint32_t)((N + T::TN - 1) / T::TN);
     const size_t   wgs = (size_t)units * (size_t)splits * nblocks;
     if (wgs > 0x7fffffffu || M > (size_t)1 << 20) return FP6MI_ERR_SHAPE; // (M: 32-bit offsets over TN batch rows)
     if (T::kLds > 48 * 1024)
-        if (int rc = allow_dynamic_lds<&grad_tile<FM, GS, PRE, NT, WN, OCC>>(T::kLds)) return rc;
-    hipLaunchKernelGGL((grad_tile<FM, GS, PRE, NT, WN, OCC>), dim3((uint32_t)wgs), dim3(2 * WN * kWave), T::kLds, st, static_cast<const uint8_t *>(W),
+        if (int rc = allow_dynamic_lds<&grad_tile<FM, GS, PRE, NT, WN>>(T::kLds)) return rc;
+    hipLaunchKernelGGL((grad_tile<FM, GS, PRE, NT, WN>), dim3((uint32_t)wgs), dim3(2 * WN * kWave), T::kLds, st, static_cast<const uint8_t *>(W),
                        static_cast<const half_t *>(sc), static_cast<const uint8_t *>(gexp), static_cast<const half_t *>(dY), static_cast<half_t *>(dX), ws,
                        (uint32_t)M, (uint32_t)N, (uint32_t)K, units, (uint32_t)splits, nblocks);
     return (int)hipGetLastError();
 }
 
+// rows: the batch rows of a workgroup, which say which kernel (fp6mi::grad_rows)
 template <int FM, bool GS, bool PRE>
-int grad_cfg(hipStream_t st, const void *W, const void *sc, const void *gexp, const void *dY, void *dX, float *ws, size_t M, size_t N, size_t K, int splits)
+int grad_cfg(int rows, hipStream_t st, const void *W, const void *sc, const void *gexp, const void *dY, void *dX, float *ws, size_t M, size_t N, size_t K, int splits)
 {
-    if (N <= 32) return launch_grad<FM, GS, PRE, 1, 2, 64>(st, W, sc, gexp, dY, dX, ws, M, N, K, splits);
-    if (N <= 64) return launch_grad<FM, GS, PRE, 2, 2, 64>(st, W, sc, gexp, dY, dX, ws, M, N, K, splits);
-    return launch_grad<FM, GS, PRE, 4, 2, 32>(st, W, sc, gexp, dY, dX, ws, M, N, K, splits);
+    switch (rows) {
+    case 16: return launch_grad_stream<FM, GS, PRE, 1, 8>(st, W, sc, gexp, dY, dX, ws, M, N, K, splits);
+    case 32: return launch_grad_stream<FM, GS, PRE, 2, 4>(st, W, sc, gexp, dY, dX, ws, M, N, K, splits);
+    case 128: return launch_grad<FM, GS, PRE, 2, 4>(st, W, sc, gexp, dY, dX, ws, M, N, K, splits);
+    case 192: return launch_grad<FM, GS, PRE, 6, 2>(st, W, sc, gexp, dY, dX, ws, M, N, K, splits);
+    case 256: return launch_grad<FM, GS, PRE, 8, 2>(st, W, sc, gexp, dY, dX, ws, M, N, K, splits);
+    default: return FP6MI_ERR_SHAPE;
+    }
 }
 
 template <int FM>
-int op_grad(void *stream, const void *W, const void *sc, const void *gexp, const void *dY, bool premultiplied, void *dX, float *ws, size_t M, size_t N, size_t K, int splits)
+int op_grad(int rows, void *stream, const void *W, const void *sc, const void *gexp, const void *dY, bool premultiplied, void *dX, float *ws, size_t M, size_t N, size_t K, int splits)
 {
     hipStream_t st = static_cast<hipStream_t>(stream);
     if (premultiplied)
-        return gexp ? grad_cfg<FM, true, true>(st, W, sc, gexp, dY, dX, ws, M, N, K, splits) : grad_cfg<FM, false, true>(st, W, sc, nullptr, dY, dX, ws, M, N, K, splits);
-    return gexp ? grad_cfg<FM, true, false>(st, W, sc, gexp, dY, dX, ws, M, N, K, splits) : grad_cfg<FM, false, false>(st, W, sc, nullptr, dY, dX, ws, M, N, K, splits);
+        return gexp ? grad_cfg<FM, true, true>(rows, st, W, sc, gexp, dY, dX, ws, M, N, K, splits) : grad_cfg<FM, false, true>(rows, st, W, sc, nullptr, dY, dX, ws, M, N, K, splits);
+    return gexp ? grad_cfg<FM, true, false>(rows, st, W, sc, gexp, dY, dX, ws, M, N, K, splits) : grad_cfg<FM, false, false>(rows, st, W, sc, nullptr, dY, dX, ws, M, N, K, splits);
 }
 
 } // namespace

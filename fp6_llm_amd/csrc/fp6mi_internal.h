@@ -33,9 +33,9 @@ inline const FormatOps *ops_for(int E, int Mbits)
 
 // fp6mi_block.hip, compiled once per format: the kernels that read the same weights for another product
 struct BlockOps {
-    // dX[N,K] = dY[N,M] . dequant(W); gexp as above; premultiplied: dY holds its products with the mantissas of the row scales (fp6mi_scale.inc); ws: splits * N * K partial sums with
+    // dX[N,K] = dY[N,M] . dequant(W); rows: batch rows of a workgroup, from grad_rows; gexp as above; premultiplied: dY holds its products with the mantissas of the row scales (fp6mi_scale.inc); ws: splits * N * K partial sums with
     // splits > 1, which the caller reduces
-    int (*grad)(void *stream, const void *W, const void *sc, const void *gexp, const void *dY, bool premultiplied, void *dX, float *ws, size_t M, size_t N, size_t K, int splits);
+    int (*grad)(int rows, void *stream, const void *W, const void *sc, const void *gexp, const void *dY, bool premultiplied, void *dX, float *ws, size_t M, size_t N, size_t K, int splits);
 };
 const BlockOps &block_ops_32(), &block_ops_22(), &block_ops_23(), &block_ops_21();
 inline const BlockOps *block_ops_for(int E, int Mbits)

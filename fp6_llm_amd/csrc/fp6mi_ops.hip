@@ -71,10 +71,9 @@ __global__ __launch_bounds__(256) void gated_grad(half_t *__restrict__ dpre, hal
 #pragma unroll
     for (int j = 0; j < 4; j++) {
         float       slope;
-        int         e;
         const float a = activation_slope<ACT>(g[j], slope), vg = (float)d[j] * u[j] * slope, vu = (float)d[j] * a;
         dg[j] = (half_t)vg, du[j] = (half_t)vu;
-        sg[j] = (half_t)(vg * (float)split_scale(scales[m + j], e)), su[j] = (half_t)(vu * (float)split_scale(scales[m + 16 + j], e));
+        sg[j] = (half_t)(vg * (float)scale_mantissa(scales[m + j])), su[j] = (half_t)(vu * (float)scale_mantissa(scales[m + 16 + j]));
     }
     if (dpre) {
         *reinterpret_cast<v4h *>(dpre + p) = dg;
@@ -268,6 +267,35 @@ int shrink(hipStream_t st, float *part, const void *x, const void *A, const int 
     return go(std::integral_constant<int, 16>{});
 }
 
+// ---------------------------------------------------------------------------------------------------------------
+// Which kernel takes an input gradient, named by the batch rows of its workgroup: grad_stream (16, 32) up to 32 rows, else the tile of grad_tile (128, 192, 256) that is the
+// fastest by this model of its time, us: rounds of one workgroup to a CU, each of which takes so long for 32 weight rows, and with a split the partial sums' way to memory and back.
+// Fitted to 7 matrices (1024x8192 to 28672x8192) x N 48 to 4096 x splits 1 to 32, off by 9 % rms; its choice of tile and split takes 1.01 times the fastest measured (at worst 1.14).
+// ---------------------------------------------------------------------------------------------------------------
+constexpr size_t kGradWorkspace = (size_t)256 << 20; // what a split of the heuristic's may take
+
+double grad_time(size_t M, size_t N, size_t K, int splits, int cus, int *rows)
+{
+    static const struct { int rows; double per32; } tiles[] = { { 128, 0.503 }, { 192, 0.690 }, { 256, 0.906 } };
+    double best = 0;
+    for (const auto &t : tiles) {
+        const size_t wgs = (K + 255) / 256 * ((N + t.rows - 1) / t.rows) * (size_t)splits, rounds = (wgs + cus - 1) / cus, steps = (M / 32 + splits - 1) / splits;
+        const double us = 6.1 + t.per32 * (double)rounds * (double)steps + (splits > 1 ? 2.75 + (double)splits * N * K * 8 / 6.08e6 : 0.0);
+        if (best == 0 || us < best) {
+            best = us;
+            if (rows) *rows = t.rows;
+        }
+    }
+    return best;
+}
+int grad_rows(size_t M, size_t N, size_t K, int splits)
+{
+    if (N <= 32) return N <= 16 ? 16 : 32;
+    int rows = 128;
+    grad_time(M, N, K, splits, 256, &rows);
+    return rows;
+}
+
 } // namespace
 
 // ------------------------------------------------------------------------------------------------ C ABI
@@ -279,11 +307,22 @@ int fp6mi_heuristic_grad_splits(int E, int Mb, size_t M, size_t N, size_t K, int
 {
     (void)E, (void)Mb;
     if (M == 0 || N == 0 || K == 0 || num_cus <= 0) return 1;
-    const size_t tiles = (K + 255) / 256 * ((N + (N <= 32 ? 31 : N <= 64 ? 63 : 127)) / (N <= 32 ? 32 : N <= 64 ? 64 : 128));
-    size_t       s = ((size_t)num_cus * 2 + tiles - 1) / tiles;
-    const size_t most = M / 256 > 0 ? M / 256 : 1;
-    if (tiles >= (size_t)num_cus) s = 1;
-    return (int)(s < most ? s : most);
+    if (N <= 32) { // a workgroup to a CU, of which every wavefront has 32 rows at least
+        const size_t units = (K + 255) / 256, s = ((size_t)num_cus + units / 2) / units, most = M / 256;
+        return (int)(s < 1 ? 1 : s < most ? s : most > 0 ? most : 1);
+    }
+    int    best = 1;
+    double t = grad_time(M, N, K, 1, num_cus, nullptr);
+    for (int s = 2; s <= 32 && (size_t)s * 128 <= M && fp6mi_grad_workspace_bytes(N, K, s) <= kGradWorkspace; s++)
+        if (const double ts = grad_time(M, N, K, s, num_cus, nullptr); ts < t) best = s, t = ts;
+    return best;
+}
+
+int fp6mi_query_grad_launch(int E, int Mb, size_t M, size_t N, size_t K, int splits)
+{
+    if (!fp6mi::supported(E, Mb)) return FP6MI_ERR_FORMAT;
+    if (M == 0 || M % 256 || M > (size_t)1 << 20 || K == 0 || K % 64 || N == 0) return FP6MI_ERR_SHAPE;
+    return splits < 1 ? FP6MI_ERR_SPLITK : grad_rows(M, N, K, splits);
 }
 
 static int check_grad(int E, int Mb, const void *W, const void *sc, const void *gexp, const void *dY, const void *dX, size_t M, size_t N, size_t K, const float *ws, int splits)
@@ -295,7 +334,7 @@ static int check_grad(int E, int Mb, const void *W, const void *sc, const void *
 
 static int run_grad(int E, int Mb, void *stream, const void *W, const void *sc, const void *gexp, const void *dY, bool premultiplied, void *dX, size_t M, size_t N, size_t K, float *ws, int splits)
 {
-    const int rc = fp6mi::block_ops_for(E, Mb)->grad(stream, W, sc, gexp, dY, premultiplied, dX, ws, M, N, K, splits);
+    const int rc = fp6mi::block_ops_for(E, Mb)->grad(grad_rows(M, N, K, splits), stream, W, sc, gexp, dY, premultiplied, dX, ws, M, N, K, splits);
     return rc != 0 || splits == 1 ? rc : fp6mi::reduce_partials(stream, dX, ws, K, N, splits);
 }
 

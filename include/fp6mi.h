@@ -228,6 +228,7 @@ int fp6mi_quantize_native_grouped_gpu(int E, int Mbits, void *stream, void *nati
  * FP32; a weight keeps its value but where value * 2^(b-127) times the power of two of its scale leaves fp16.  M up to 2^20.  splits > 1 cuts the sum over M into that many parts, whose partial sums take fp6mi_grad_workspace_bytes bytes. */
 int    fp6mi_linear_grad_native(int E, int Mbits, void *stream, const void *W_native, const void *scales_f16, const void *group_exps_native, const void *dY_f16,
                                 void *dX_f16, size_t M, size_t N, size_t K, float *workspace, int splits);
+int    fp6mi_query_grad_launch(int E, int Mbits, size_t M, size_t N, size_t K, int splits); /* batch rows of a workgroup of the kernel that takes it, or FP6MI_ERR_* */
 int    fp6mi_heuristic_grad_splits(int E, int Mbits, size_t M, size_t N, size_t K, int num_cus);
 size_t fp6mi_grad_workspace_bytes(size_t N, size_t K, int splits);
 
