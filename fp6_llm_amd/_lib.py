@@ -67,6 +67,7 @@ def lib():
         "fp6mi_grad_workspace_bytes": (sz, [sz, sz, ci]),
         "fp6mi_gated_native": (ci, [ci, ci, vp, vp, vp, vp, vp, vp, vp, vp, sz, sz, sz, ci, vp, ci]),
         "fp6mi_gated_workspace_bytes": (sz, [sz, sz, ci]),
+        "fp6mi_query_gated_launch": (ci, [ci, ci, sz, sz, sz, ci, ctypes.POINTER(ci)]),
         "fp6mi_gated_backward_workspace_bytes": (sz, [sz, sz, sz, ci]),
         "fp6mi_gated_backward_native": (ci, [ci, ci, vp, vp, vp, vp, vp, vp, vp, vp, sz, sz, sz, ci, vp, ci]),
         "fp6mi_adapter_native": (ci, [ci, ci, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, sz, sz, sz, sz, sz, vp, ci]),
@@ -88,7 +89,7 @@ EXPORTED = ["fp6mi_error_string", "fp6mi_version", "fp6mi_tuning_info", "fp6mi_p
             "fp6mi_relayout_ref_to_native_gpu", "fp6mi_dequant_native_gpu", "fp6mi_quantize_native_gpu", "fp6mi_query_launch", "fp6mi_launch_source", "fp6mi_query_kernel", "fp6mi_query_table",
             "fp6mi_group_exps_bytes", "fp6mi_pack_group_exps", "fp6mi_dequant_grouped", "fp6mi_linear_native_grouped", "fp6mi_linear_native_grouped_cfg", "fp6mi_linear_native_bias",
             "fp6mi_dequant_native_grouped_gpu", "fp6mi_quantize_native_grouped_gpu",
-            "fp6mi_linear_grad_native", "fp6mi_query_grad_launch", "fp6mi_heuristic_grad_splits", "fp6mi_grad_workspace_bytes", "fp6mi_gated_native", "fp6mi_gated_workspace_bytes",
+            "fp6mi_linear_grad_native", "fp6mi_query_grad_launch", "fp6mi_heuristic_grad_splits", "fp6mi_grad_workspace_bytes", "fp6mi_gated_native", "fp6mi_gated_workspace_bytes", "fp6mi_query_gated_launch",
             "fp6mi_gated_backward_native", "fp6mi_gated_backward_workspace_bytes", "fp6mi_adapter_native", "fp6mi_adapter_workspace_bytes"]
 
 

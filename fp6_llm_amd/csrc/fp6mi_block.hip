@@ -1,5 +1,6 @@
 // gfx950 kernels around the FPx linear layer that read the native weight layout in another way than its GEMM, for ONE weight format per translation unit
 // (compiled like fp6mi_gemm.hip, with -DFP6MI_FORMAT=<10*E+M>).  No counterpart in the reference, whose only operator is the forward product.
+//   gated_stream, gated_tile, gated_ws, gated_wide   H = act(X . Wg^T + bg) * (X . Wu^T + bu): the gated feed-forward block, on weights in pair order
 //   grad_tile, grad_stream   dX[N,K] = dY[N,M] . dequant(W)[M,K]: the input gradient of the linear layer
 #include <hip/hip_runtime.h>
 
@@ -14,8 +15,11 @@
 
 namespace {
 
+using fp6mi::LaunchCfg;
+
 #include "fp6mi_device.inc"
 #include "fp6mi_scale.inc"
+#include "fp6mi_activation.inc"
 
 // ---------------------------------------------------------------------------------------------------------------
 // grad_tile: the product that contracts over the weights' rows.
@@ -464,6 +468,191 @@ int grad_cfg(int rows, hipStream_t st, const void *W, const void *sc, const void
     }
 }
 
+// ---------------------------------------------------------------------------------------------------------------
+// The gated feed-forward block: the GEMM's kernels (fp6mi_gemm.hip: gemm_stream, gemm_tile, gemm_ws, gemm_wide and gemm_span) with another epilogue.
+// The weights are one matrix of M rows in pair order: a 16-row tile of the gate projection, the same tile of the up projection, and so on.  An even number of row tiles to a
+// wavefront (or, in gemm_stream, a workgroup) then holds both pre-activations of every output, and no launch, no trip through memory follows: 2 * N * M bytes written and read less.
+// The float32 sums are scaled and parked in LDS as the partial sums of a split are; on the way out a thread takes four rows of gate and the same four of up, adds the biases and
+// writes act(g) * u, and the pre-activations themselves where a backward pass will want them.
+// Parameters as in the GEMM's kernels; preact and bias may be null.
+// ---------------------------------------------------------------------------------------------------------------
+template <int NT, int RT, int WR, int NTHREADS>
+__device__ __forceinline__ void gated_flush(half_t *__restrict__ out, float *__restrict__ preact, const half_t *__restrict__ bias, uint32_t activation_code, const uint8_t *stage, uint32_t M,
+                                            uint32_t N, uint32_t mb, uint32_t nbase, int tid)
+{
+    constexpr int TM = WR * RT * 16, TN = NT * 16, kStride = TM * 4 + 16, kPerCol = TM / 8, kPieces = TN * kPerCol; // a piece: four outputs
+    for (int p = tid; p < kPieces; p += NTHREADS) {
+        const int      c = p / kPerCol, i = p % kPerCol;
+        const uint32_t ng = nbase + c, m = mb * TM + (i >> 2) * 32 + (i & 3) * 4;
+        if (ng < N) {
+            const uint8_t *src = stage + c * kStride + ((i >> 2) * 32 + (i & 3) * 4) * 4;
+            v4f            g = *reinterpret_cast<const v4f *>(src), u = *reinterpret_cast<const v4f *>(src + 64);
+            v4h            h;
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                if (bias) g[k] += (float)bias[m + k], u[k] += (float)bias[m + 16 + k];
+                h[k] = (half_t)(activated(activation_code, g[k]) * u[k]);
+            }
+            *reinterpret_cast<v4h *>(out + (size_t)ng * (M / 2) + (size_t)mb * (TM / 2) + i * 4) = h;
+            if (preact) {
+                *reinterpret_cast<v4f *>(preact + (size_t)ng * M + m) = g;
+                *reinterpret_cast<v4f *>(preact + (size_t)ng * M + m + 16) = u;
+            }
+        }
+    }
+}
+
+#define FP6MI_GATED 1
+template <int FM, bool GS, int NT, int RT, int WAVES>
+__global__ __launch_bounds__(WAVES *kWave) void gated_stream(const uint8_t *__restrict__ W, const half_t *__restrict__ scales, const uint8_t *__restrict__ gexp, const half_t *__restrict__ X,
+                                                             half_t *__restrict__ C, float *__restrict__ preact, const half_t *__restrict__ bias, uint32_t M, uint32_t N, uint32_t K,
+                                                             uint32_t units, uint32_t activation_code)
+{
+    static_assert(RT % 2 == 0, "pairs of row tiles");
+    constexpr bool     SPLIT = false;
+    constexpr uint32_t splitK = 1;
+    float *const       ws = preact;
+#include "fp6mi_stream_tile.inc"
+}
+
+template <int FM, bool GS, int NT, int RT, int WR, int WK>
+__global__ __launch_bounds__(WR *WK *kWave) void gated_tile(const uint8_t *__restrict__ W, const half_t *__restrict__ scales, const uint8_t *__restrict__ gexp, const half_t *__restrict__ X,
+                                                            half_t *__restrict__ C, float *__restrict__ preact, const half_t *__restrict__ bias, uint32_t M, uint32_t N, uint32_t K,
+                                                            uint32_t units, uint32_t activation_code, uint32_t nblocks)
+{
+    static_assert(RT % 2 == 0, "pairs of row tiles");
+    constexpr int NTHREADS = WR * WK * kWave;
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    const int      tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wr = wave % WR, wk = wave / WR, col = lane & 15, q = lane >> 4;
+    const TileId   id = tile_of<WR * RT * 16, NT * 16>(1, nblocks, N, K);
+    const uint32_t nbase = id.nb * NT * 16, R0 = (id.mb * WR + wr) * RT;
+    v4f            acc[RT][NT];
+    v4h            sc4[RT]; // fetched ahead of the K loop, as in gemm_tile
+#pragma unroll
+    for (int r = 0; r < RT; r++) {
+        const half_t *p = scales + (R0 + r) * 16 + 4 * q;
+        sc4[r] = (v4h){ p[0], p[1], p[2], p[3] };
+    }
+    tile_segment<FM, GS, NT, RT, WR, WK>(acc, W, gexp, X, N, K, units, id.mb, nbase, 0, units, lds, tid, lane, wr, wk, col, q);
+    if (WK > 1) __syncthreads(); // (the sums are parked where the partial sums of the K wavefronts met)
+    if (wk == 0) tile_park<FM, NT, RT, WR, float>(acc, sc4, lds, wr, col, q);
+    __syncthreads();
+    gated_flush<NT, RT, WR, NTHREADS>(C, preact, bias, activation_code, lds, M, N, id.mb, nbase, tid);
+}
+
+template <int FM, bool GS, int NT, int RT, int WR, int PW, int SW, int SX>
+__global__ __launch_bounds__((WR + PW) * kWave) void gated_ws(const uint8_t *__restrict__ W, const half_t *__restrict__ scales, const uint8_t *__restrict__ gexp, const half_t *__restrict__ X,
+                                                              half_t *__restrict__ C, float *__restrict__ preact, const half_t *__restrict__ bias, uint32_t M, uint32_t N, uint32_t K,
+                                                              uint32_t units, uint32_t activation_code, uint32_t nblocks)
+{
+    static_assert(RT % 2 == 0, "pairs of row tiles");
+    constexpr uint32_t splitK = 1;
+    float *const       ws = preact;
+#include "fp6mi_ws_tile.inc"
+}
+
+template <int FM, bool GS, int NT, int RT, int WK>
+__global__ __launch_bounds__(4 * WK *kWave, RT *NT <= 8 ? 4 : 2) void gated_wide(const uint8_t *W, const half_t *__restrict__ scales, const uint8_t *gexp, const half_t *X,
+                                                                                 half_t *__restrict__ C, float *__restrict__ preact, const half_t *__restrict__ bias, uint32_t M, uint32_t N,
+                                                                                 uint32_t K, uint32_t units, uint32_t activation_code, uint32_t nblocks)
+{
+    static_assert(RT % 2 == 0, "pairs of row tiles");
+    constexpr uint32_t splitK = 1;
+#include "fp6mi_wide_tile.inc"
+}
+#undef FP6MI_GATED
+
+struct GatedArgs {
+    hipStream_t st;
+    const void *W, *sc, *gexp, *B;
+    void       *C;
+    float      *preact;
+    const void *bias;
+    size_t      M, N, K;
+    int         activation;
+};
+
+template <int FM, bool GS, int NT, int RT, int WAVES> int launch_gated_stream(const GatedArgs &a)
+{
+    constexpr size_t kMaxLds = (size_t)WAVES * stream_wave_bytes(16 * NT, RT, NT);
+    static_assert(kMaxLds <= 160 * 1024, "the wavefronts' activation rows do not fit in LDS");
+    const uint32_t units = (uint32_t)((a.K + 255) / 256);
+    const dim3     grid((uint32_t)((a.M / 16 + RT - 1) / RT), 1, (uint32_t)((a.N + 16 * NT - 1) / (16 * NT)));
+    const size_t   lds_bytes = NT == 1 && a.N <= 8 ? (size_t)WAVES * stream_wave_bytes(8, RT, NT) : kMaxLds;
+    if (kMaxLds > 48 * 1024)
+        if (int rc = allow_dynamic_lds<&gated_stream<FM, GS, NT, RT, WAVES>>(kMaxLds)) return rc;
+    hipLaunchKernelGGL((gated_stream<FM, GS, NT, RT, WAVES>), grid, dim3(WAVES * kWave), lds_bytes, a.st, static_cast<const uint8_t *>(a.W), static_cast<const half_t *>(a.sc),
+                       static_cast<const uint8_t *>(a.gexp), static_cast<const half_t *>(a.B), static_cast<half_t *>(a.C), a.preact, static_cast<const half_t *>(a.bias), (uint32_t)a.M,
+                       (uint32_t)a.N, (uint32_t)a.K, units, (uint32_t)a.activation);
+    return (int)hipGetLastError();
+}
+// the kernels of tiles: TM x TN outputs of the GEMM a workgroup of THREADS
+template <auto Kernel, int TM, int TN, int THREADS> int launch_gated_tiles(const GatedArgs &a, size_t lds_bytes)
+{
+    if (a.M % TM) return FP6MI_ERR_SHAPE;
+    if (lds_bytes > 48 * 1024)
+        if (int rc = allow_dynamic_lds<Kernel>(lds_bytes)) return rc;
+    const uint32_t units = (uint32_t)((a.K + 255) / 256), nblocks = (uint32_t)((a.N + TN - 1) / TN);
+    const size_t   wgs = a.M / TM * nblocks;
+    if (wgs > 0x7fffffffu) return FP6MI_ERR_SHAPE;
+    hipLaunchKernelGGL(Kernel, dim3((uint32_t)wgs), dim3(THREADS), lds_bytes, a.st, static_cast<const uint8_t *>(a.W), static_cast<const half_t *>(a.sc), static_cast<const uint8_t *>(a.gexp),
+                       static_cast<const half_t *>(a.B), static_cast<half_t *>(a.C), a.preact, static_cast<const half_t *>(a.bias), (uint32_t)a.M, (uint32_t)a.N, (uint32_t)a.K, units,
+                       (uint32_t)a.activation, nblocks);
+    return (int)hipGetLastError();
+}
+constexpr size_t most_of(size_t a, size_t b) { return a > b ? a : b; }
+template <int FM, bool GS, int NT, int RT, int WR, int WK> int launch_gated_tile(const GatedArgs &a)
+{
+    constexpr size_t kLoop = most_of(2 * (size_t)WK * NT * 16 * kXsRowBytes, WK > 1 ? (size_t)WK * WR * RT * NT * 1024 : 0), kLds = most_of(kLoop, tile_stage_bytes<NT, RT, WR>(true));
+    static_assert(kLds <= 160 * 1024, "tile does not fit in LDS");
+    return launch_gated_tiles<&gated_tile<FM, GS, NT, RT, WR, WK>, WR * RT * 16, NT * 16, WR * WK * kWave>(a, kLds);
+}
+template <int FM, bool GS, int NT, int RT, int WR, int PW, int SW, int SX> int launch_gated_ws(const GatedArgs &a)
+{
+    constexpr size_t kLds = most_of(ws_ring_bytes<FM, NT, RT, WR, SW, SX>() + ws_exps_ring_bytes<GS, RT, WR, SW>(), tile_stage_bytes<NT, RT, WR>(true));
+    static_assert(kLds <= 160 * 1024, "the rings do not fit in LDS");
+    return launch_gated_tiles<&gated_ws<FM, GS, NT, RT, WR, PW, SW, SX>, WR * RT * 16, NT * 16, (WR + PW) * kWave>(a, kLds);
+}
+template <int FM, bool GS, int NT, int RT, int WK> int launch_gated_wide(const GatedArgs &a)
+{
+    constexpr size_t kSums = WK == 2 ? (size_t)4 * RT * 16 * ((NT + 1) / 2) * 128 : 0, kLds = most_of(most_of(WK * 2 * (size_t)NT * 16 * 256, tile_stage_bytes<(NT + 1) / 2, RT, 4>(true)), kSums);
+    static_assert(kLds <= 160 * 1024 / (3 - WK), "two workgroups of four wavefronts or one of eight do not fit in LDS");
+    if (a.K > (size_t)1 << 20) return FP6MI_ERR_SHAPE; // (32-bit offsets over TN rows)
+    return launch_gated_tiles<&gated_wide<FM, GS, NT, RT, WK>, 4 * RT * 16, NT * 16, 4 * WK * kWave>(a, kLds);
+}
+
+template <int FM, bool GS> int gated_cfg(const LaunchCfg &c, const GatedArgs &a)
+{
+#define FP6MI_CASE(NT, RT, WV) \
+    if (c.kind == 0 && c.nt == NT && c.rt == RT && c.wk == WV) return launch_gated_stream<FM, GS, NT, RT, WV>(a);
+    FP6MI_CASE(1, 2, 4) FP6MI_CASE(1, 2, 8) FP6MI_CASE(1, 2, 16) FP6MI_CASE(1, 4, 4) FP6MI_CASE(1, 4, 8) FP6MI_CASE(1, 6, 4) FP6MI_CASE(1, 6, 8) FP6MI_CASE(1, 8, 4)
+    FP6MI_CASE(2, 2, 4) FP6MI_CASE(2, 2, 8) FP6MI_CASE(2, 4, 4) FP6MI_CASE(2, 4, 8) FP6MI_CASE(2, 6, 4) FP6MI_CASE(2, 8, 4)
+#undef FP6MI_CASE
+#define FP6MI_CASE(NT, WR, WK) \
+    if (c.kind == 1 && c.nt == NT && c.wr == WR && c.wk == WK) return launch_gated_tile<FM, GS, NT, 2, WR, WK>(a);
+    FP6MI_CASE(2, 4, 1) FP6MI_CASE(2, 4, 2) FP6MI_CASE(2, 4, 4) FP6MI_CASE(3, 8, 1) FP6MI_CASE(4, 4, 2) FP6MI_CASE(4, 8, 1) FP6MI_CASE(5, 8, 1) FP6MI_CASE(6, 8, 1)
+#undef FP6MI_CASE
+    if (c.kind == 2 && c.wk == 4) { // (ring depths as in gemm_ws)
+#define FP6MI_CASE(NT, WR) \
+    if (c.nt == NT && c.wr == WR) return launch_gated_ws<FM, GS, NT, 2, WR, 4, WR == 4 && NT < 6 ? 3 : 2, WR == 4 && NT == 3 ? 3 : 2>(a);
+        FP6MI_CASE(4, 8) FP6MI_CASE(3, 4) FP6MI_CASE(4, 4) FP6MI_CASE(5, 4) FP6MI_CASE(6, 4)
+#undef FP6MI_CASE
+    }
+#define FP6MI_CASE(NT, RT, WK) \
+    if (c.kind == 2 && c.wr == 4 && c.nt == NT && c.rt == RT && c.wk == WK) return launch_gated_wide<FM, GS, NT, RT, WK>(a);
+    FP6MI_CASE(8, 4, 1) FP6MI_CASE(8, 4, 2) FP6MI_CASE(6, 4, 1) FP6MI_CASE(8, 2, 2) FP6MI_CASE(3, 2, 2) FP6MI_CASE(5, 2, 2) FP6MI_CASE(7, 2, 2) FP6MI_CASE(5, 4, 2) FP6MI_CASE(6, 4, 2)
+    FP6MI_CASE(7, 4, 2) FP6MI_CASE(4, 2, 2) FP6MI_CASE(6, 2, 2)
+#undef FP6MI_CASE
+    return FP6MI_ERR_SHAPE;
+}
+
+template <int FM>
+int op_gated(const LaunchCfg &c, void *stream, const void *W, const void *sc, const void *gexp, const void *bias, const void *B, void *C, float *preact, size_t M, size_t N, size_t K, int activation)
+{
+    const GatedArgs a = { static_cast<hipStream_t>(stream), W, sc, gexp, B, C, preact, bias, M, N, K, activation };
+    return gexp ? gated_cfg<FM, true>(c, a) : gated_cfg<FM, false>(c, a);
+}
+
 template <int FM>
 int op_grad(int rows, void *stream, const void *W, const void *sc, const void *gexp, const void *dY, bool premultiplied, void *dX, float *ws, size_t M, size_t N, size_t K, int splits)
 {
@@ -480,7 +669,7 @@ namespace fp6mi {
 #define FP6MI_OPS_NAME(f) FP6MI_OPS_NAME_(f)
 const BlockOps &FP6MI_OPS_NAME(FP6MI_FORMAT)()
 {
-    static const BlockOps ops = { &op_grad<FP6MI_FORMAT> };
+    static const BlockOps ops = { &op_gated<FP6MI_FORMAT>, &op_grad<FP6MI_FORMAT> };
     return ops;
 }
 } // namespace fp6mi

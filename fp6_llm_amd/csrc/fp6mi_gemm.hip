@@ -142,17 +142,6 @@ __global__ __launch_bounds__(WR *WK *kWave) void gemm_tile(const uint8_t *__rest
 // position touch eight different slots.  One barrier per K block: before it the loading wavefronts wait until the NEXT
 // block has landed (s_waitcnt with the number of transfers issued after it: they complete in order).
 // ---------------------------------------------------------------------------------------------------------------
-template <int FM, int NT, int RT, int WR, int SW, int SX> constexpr size_t ws_ring_bytes()
-{
-    return (size_t)SW * WR * RT * Fmt<FM>::block_bytes + (size_t)SX * NT * 16 * 512;
-}
-// Group exponents of 128 rows travel with the weights, in a ring of SW stages behind the activations', 4 bytes a row.  Loaded by the arithmetic
-// wavefronts, one block ahead, they were waited for at the barrier of every block, and the blocks that a ring of three has under way did not help: the
-// shapes that had won without exponents lost up to 28 % with them to those they had replaced.  us, shape before the ring of three / loads in registers /
-// through LDS: e2m1 8704x16192 N 53 29.5 / 38.1 / 29.1; e2m2 5632x10432 N 236 48.7 / 61.8 / 44.6; e2m1 1792x25984 N 672 133.8 / 144.7 / 101.0; over 167
-// problems of N 33 to 946 LDS / registers 0.89 (0.70-1.00).  With 256 rows LDS is full and SW is 2, one block ahead as in registers.
-template <bool GS, int WR> constexpr bool ws_exps_in_lds() { return GS && WR == 4; }
-template <bool GS, int RT, int WR, int SW> constexpr size_t ws_exps_ring_bytes() { return ws_exps_in_lds<GS, WR>() ? (size_t)SW * WR * RT * 64 : 0; }
 
 template <int FM, bool GS, int NT, int RT, int WR, int PW, int SW, int SX>
 __global__ __launch_bounds__((WR + PW) * kWave) void gemm_ws(const uint8_t *__restrict__ W, const half_t *__restrict__ scales,
@@ -160,193 +149,7 @@ __global__ __launch_bounds__((WR + PW) * kWave) void gemm_ws(const uint8_t *__re
                                                              float *__restrict__ ws, uint32_t M, uint32_t N, uint32_t K,
                                                              uint32_t units, uint32_t splitK, uint32_t nblocks)
 {
-    static_assert(SW >= SX && SX >= 2, "weights run at least as far ahead as activations; a stage is filled while another is read");
-    constexpr int TN = NT * 16, TILES = WR * RT, NTHREADS = (WR + PW) * kWave;
-    constexpr int kBlock = Fmt<FM>::block_bytes, kWStage = TILES * kBlock, kXStage = TN * 512, kXRing = SW * kWStage; // the activation ring follows the weight ring
-    constexpr bool kGLds = ws_exps_in_lds<GS, WR>();
-    constexpr int  kGStage = TILES * 64, kGRing = kXRing + SX * kXStage;
-    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-
-    asm volatile("" ::"s"(W), "s"(scales), "s"(gexp), "s"(X), "s"(C), "s"(ws), "s"(M), "s"(N), "s"(K), "s"(units), "s"(splitK), "s"(nblocks)); // one batch of argument loads
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int col = lane & 15, q = lane >> 4;
-
-    const TileId   id = tile_of<WR * RT * 16, NT * 16>(splitK, nblocks, N, K);
-    const uint32_t mb = id.mb, split = id.split, nb = id.nb;
-    const uint32_t nbase = nb * TN;
-    uint32_t       u0 = 0, u1 = units;
-    if (splitK > 1) {
-        const uint32_t avg = units / splitK, extra = units % splitK;
-        u0 = split * avg + (split < extra ? split : extra);
-        u1 = u0 + avg + (split < extra ? 1u : 0u);
-    }
-    const int nk = (int)(u1 - u0); // K blocks of this workgroup, numbered 0 .. nk-1 below
-
-    v4f acc[RT][NT];
-    v4h sc4[RT];
-#pragma unroll
-    for (int r = 0; r < RT; r++)
-#pragma unroll
-        for (int t = 0; t < NT; t++) acc[r][t] = (v4f){ 0.f, 0.f, 0.f, 0.f };
-
-    if (wave >= WR) {
-        // ---------------------------------------------------------------- loading wavefronts
-        // One instruction moves 64 x 16 bytes from memory straight into 1 KB of LDS, lane l to byte 16*l of the destination;
-        // each lane chooses its source address.  Instruction i of a weight (activation) stage fills its pieces 64*i .. 64*i+63;
-        // this wavefront issues the instructions pw, pw + PW, ...
-        typedef __attribute__((address_space(1))) void gvoid;
-        typedef __attribute__((address_space(3))) void lvoid;
-        const int     pw = wave - WR;
-        constexpr int PB = kBlock / 16, kWPieces = TILES * PB, kXPieces = TN * 32;
-        static_assert(kWPieces % 64 == 0 && kXPieces % 64 == 0, "a stage is a whole number of 1 KB instructions");
-        constexpr int kWInst = kWPieces / 64, kXInst = kXPieces / 64;
-        static_assert(kWInst % PW == 0 && kXInst % PW == 0, "every loading wavefront issues the same number of transfers (the waits count them)");
-        static_assert(!kGLds || TILES * 16 % PW == 0 && TILES * 16 / PW <= 64, "a stage of exponents is one transfer of every loading wavefront");
-        constexpr int kWPer = kWInst / PW, kXPer = kXInst / PW, kGRows = TILES * 16 / PW, kWSteps = kWPer + (kGLds ? 1 : 0);
-        // transfers issued after those of block j+1 when step j ends: the later of its two transfers is the activation one, issued
-        // SX-2 steps ago and followed there by that step's weight transfers when the weight ring is the deeper one
-        constexpr int kAhead = (SW > SX ? kWSteps : 0) + (SX - 2) * (kWSteps + kXPer);
-        // weight piece P (16 bytes) of a stage = piece P % PB of the block of tile P / PB: a straight copy
-        const uint8_t *wsrc[kWPer];
-#pragma unroll
-        for (int j = 0; j < kWPer; j++) {
-            const uint32_t P = (pw + PW * j) * 64 + lane, tile = P / PB, within = P % PB;
-            wsrc[j] = W + ((size_t)(mb * TILES + tile) * units + u0) * kBlock + within * 16;
-        }
-        const uint32_t grow = pw * kGRows + (kGLds ? lane % kGRows : 0);
-        const uint8_t *gsrc = kGLds ? gexp + ((size_t)(mb * TILES + grow / 16) * units + u0) * 32 + grow % 16 * 2 : nullptr;
-        // activation piece P of a stage = slot P % 32 of row P / 32, which holds piece slot ^ (row & 15) of that batch column's
-        // 256 halfs (columns beyond N repeat the last real one: their outputs are never stored)
-        const uint8_t *xsrc[kXPer];
-        uint32_t       xpiece[kXPer];
-#pragma unroll
-        for (int j = 0; j < kXPer; j++) {
-            const uint32_t P = (pw + PW * j) * 64 + lane, n = P >> 5, piece = (P & 31) ^ (n & 15);
-            const uint32_t row = nbase + n < N ? nbase + n : N - 1;
-            xsrc[j] = reinterpret_cast<const uint8_t *>(X + (size_t)row * K + (size_t)u0 * 256) + piece * 16;
-            xpiece[j] = piece;
-        }
-        auto fetch_w = [&](int k, int slot) { // weights of block k -> stage `slot` of the weight ring
-            uint8_t *st = lds + slot * kWStage;
-#pragma unroll
-            for (int j = 0; j < kWPer; j++)
-                __builtin_amdgcn_global_load_lds((gvoid *)(wsrc[j] + (size_t)k * kBlock), (lvoid *)(st + (pw + PW * j) * 1024), 16, 0, 0);
-            if constexpr (kGLds) // and their exponents: lane l takes the two of row pw * kGRows + l, which LDS receives as 32 bits
-                if (lane < kGRows)
-                    __builtin_amdgcn_global_load_lds((gvoid *)(gsrc + (size_t)k * 32), (lvoid *)(lds + kGRing + slot * kGStage + pw * kGRows * 4), 2, 0, 0);
-        };
-        auto fetch_x = [&](int k, int slot) { // activations of block k -> stage `slot` of the activation ring
-            uint8_t *st = lds + kXRing + slot * kXStage;
-            if ((u0 + k + 1) * 256 <= K) {
-#pragma unroll
-                for (int j = 0; j < kXPer; j++)
-                    __builtin_amdgcn_global_load_lds((gvoid *)(xsrc[j] + (size_t)k * 512), (lvoid *)(st + (pw + PW * j) * 1024), 16, 0, 0);
-            } else { // the block that K cuts goes through registers: positions beyond K are read at the block's start (a valid address) and stored as zeros
-#pragma unroll
-                for (int j = 0; j < kXPer; j++) {
-                    const bool ok = (u0 + k) * 256 + xpiece[j] * 8 < K;
-                    const v4u  v = *reinterpret_cast<const v4u *>(xsrc[j] + (size_t)k * 512 - (ok ? 0u : xpiece[j] * 16));
-                    *reinterpret_cast<v4u *>(st + (pw + PW * j) * 1024 + lane * 16) = ok ? v : (v4u){ 0u, 0u, 0u, 0u };
-                }
-            }
-        };
-        if (nk > 0) {
-            // step j (j = -(SW-1) .. nk-1; the negative ones fill the rings) issues the activations of block j+SX-1 and then the
-            // weights of block j+SW-1; it ends with a barrier before which block j+1 must have landed
-            int wslot = 0, xslot = 0; // ring positions the next transfers go to
-            for (int j = 1 - SW; j < nk; j++) {
-                const int kx = j + SX - 1, kw = j + SW - 1;
-                if (kx >= 0 && kx < nk) {
-                    fetch_x(kx, xslot);
-                    xslot = xslot + 1 == SX ? 0 : xslot + 1;
-                }
-                if (kw < nk) {
-                    fetch_w(kw, wslot);
-                    wslot = wslot + 1 == SW ? 0 : wslot + 1;
-                }
-                if (j >= -1) {
-                    // the count is exact only while every transfer it assumes was issued; at the end of K wait for everything
-                    // (block j+1's last transfer is followed by exactly kAhead others as long as this step still had weights to fetch)
-                    if (kw < nk)
-                        wait_transfers_and_barrier<kAhead>();
-                    else
-                        wait_transfers_and_barrier<0>();
-                }
-            }
-        }
-    } else {
-        // ---------------------------------------------------------------- arithmetic wavefronts
-        const int      wr = wave;
-        const uint32_t R0 = (mb * WR + wr) * RT; // first row tile of this wavefront
-#pragma unroll
-        for (int r = 0; r < RT; r++) {
-            const half_t *p = scales + (R0 + r) * 16 + 4 * q;
-            if ((reinterpret_cast<uintptr_t>(scales) & 7u) == 0)
-                sc4[r] = *reinterpret_cast<const v4h *>(p);
-            else
-                sc4[r] = (v4h){ p[0], p[1], p[2], p[3] };
-        }
-        const uint8_t *ggroup = GS ? gexp + ((size_t)R0 * units + u0) * 32 : nullptr;
-        uint32_t       xoff[8]; // B operand of MFMA step s: row col, piece 4s+q, at its swizzled slot
-#pragma unroll
-        for (int s8 = 0; s8 < 8; s8++) xoff[s8] = kXRing + col * 512 + 16 * ((4 * s8 + q) ^ col);
-        const uint32_t woff = wr * RT * kBlock + lane * 16;
-        if (nk > 0) {
-            uint32_t gnext[RT];
-#pragma unroll
-            for (int r = 0; r < RT; r++) gnext[r] = load_group_exps<GS && !kGLds>(ggroup, (size_t)r * units, lane);
-            __syncthreads(); // block 0 has landed
-            int wslot = 0, xslot = 0;
-            for (int k = 0; k < nk; k++) {
-                const uint8_t *wst = lds + wslot * kWStage, *xst = lds + xslot * kXStage, *gst = lds + kGRing + wslot * kGStage;
-                wslot = wslot + 1 == SW ? 0 : wslot + 1;
-                xslot = xslot + 1 == SX ? 0 : xslot + 1;
-                WFrag<FM> wf[RT];
-                uint32_t  g[RT];
-#pragma unroll
-                for (int r = 0; r < RT; r++) {
-                    const uint8_t *b = wst + woff + r * kBlock;
-                    wf[r].a = *reinterpret_cast<const v4u *>(b);
-                    wf[r].b = *reinterpret_cast<const v4u *>(b + 1024);
-                    if constexpr (Fmt<FM>::bits == 6) wf[r].c = *reinterpret_cast<const v4u *>(b + 2048);
-                    if constexpr (Fmt<FM>::bits == 5) wf[r].s = *reinterpret_cast<const v2u *>(wst + (wr * RT + r) * kBlock + 2048 + lane * 8);
-                    g[r] = kGLds ? *reinterpret_cast<const uint32_t *>(gst + (wr * RT + r) * 64 + col * 4) : gnext[r];
-                    if (GS && !kGLds && k + 1 < nk) gnext[r] = load_group_exps<GS>(ggroup, (size_t)r * units + k + 1, lane);
-                }
-                v8h a0[RT][4], a1[RT][4];
-#pragma unroll
-                for (int r = 0; r < RT; r++) convert_half<FM, GS>(wf[r], 0, a0[r], g[r]);
-#pragma unroll
-                for (int r = 0; r < RT; r++) convert_half<FM, GS>(wf[r], 1, a1[r], g[r]);
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-#pragma unroll
-                    for (int s = 0; s < 4; s++) {
-                        v8h b[NT];
-#pragma unroll
-                        for (int t = 0; t < NT; t++) b[t] = *reinterpret_cast<const v8h *>(xst + xoff[4 * h + s] + t * 16 * 512);
-#pragma unroll
-                        for (int r = 0; r < RT; r++)
-#pragma unroll
-                            for (int t = 0; t < NT; t++)
-                                acc[r][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(h == 0 ? a0[r][s] : a1[r][s], b[t], acc[r][t], 0, 0, 0);
-                    }
-                }
-                __syncthreads();
-            }
-        }
-    }
-    // every wavefront has passed the last barrier of the K loop: the rings are free, the output tile is parked there
-    uint8_t *stage = lds;
-    if (splitK == 1) {
-        if (wave < WR) tile_park<FM, NT, RT, WR, half_t>(acc, sc4, stage, wave, col, q, ws ? bias_of(ws) + mb * (WR * RT * 16) : nullptr);
-        __syncthreads();
-        tile_flush<NT, RT, WR, NTHREADS, half_t>(C, stage, M, N, mb, nbase, tid);
-    } else {
-        if (wave < WR) tile_park<FM, NT, RT, WR, float>(acc, sc4, stage, wave, col, q);
-        __syncthreads();
-        tile_flush<NT, RT, WR, NTHREADS, float>(ws + (size_t)split * N * M, stage, M, N, mb, nbase, tid);
-    }
+#include "fp6mi_ws_tile.inc"
 }
 
 // ---------------------------------------------------------------------------------------------------------------

@@ -33,6 +33,9 @@ inline const FormatOps *ops_for(int E, int Mbits)
 
 // fp6mi_block.hip, compiled once per format: the kernels that read the same weights for another product
 struct BlockOps {
+    // H[N,M/2] of the gated block on weights in pair order by launch shape c (FP6MI_ERR_SHAPE where its kernels lack it); gexp, bias and preact may be null
+    int (*gated)(const LaunchCfg &c, void *stream, const void *W, const void *sc, const void *gexp, const void *bias, const void *B, void *C, float *preact, size_t M, size_t N, size_t K,
+                 int activation);
     // dX[N,K] = dY[N,M] . dequant(W); rows: batch rows of a workgroup, from grad_rows; gexp as above; premultiplied: dY holds its products with the mantissas of the row scales (fp6mi_scale.inc); ws: splits * N * K partial sums with
     // splits > 1, which the caller reduces
     int (*grad)(int rows, void *stream, const void *W, const void *sc, const void *gexp, const void *dY, bool premultiplied, void *dX, float *ws, size_t M, size_t N, size_t K, int splits);
@@ -46,6 +49,8 @@ inline const BlockOps *block_ops_for(int E, int Mbits)
 // fp6mi_api.hip: parts of fp6mi_linear_native for the operators around it (fp6mi_ops.hip)
 int  check_linear(int E, int Mbits, const void *W, const void *sc, const void *gexp, const void *bias, const void *B, const void *C, size_t M, size_t N, size_t K, const float *ws, int splitK);
 int  current_cus();
+// the launch shape of fp6mi_linear_native
+LaunchCfg linear_shape(int E, int Mbits, size_t M, size_t N, size_t K, int splitK, bool grouped);
 // the GEMM by the shape that fp6mi_linear_native takes; partial_only: with a split, the partial sums alone, [splitK][N][M] floats in ws (C is not touched)
 int  run_linear(int E, int Mbits, void *stream, const void *W, const void *sc, const void *gexp, const void *bias, const void *B, void *C, size_t M, size_t N, size_t K, float *ws, int splitK,
                 bool partial_only);

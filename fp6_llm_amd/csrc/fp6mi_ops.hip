@@ -27,7 +27,7 @@ __device__ __forceinline__ size_t pair_index(size_t i, uint32_t F) // of output 
     return n * 2 * F + (f >> 4) * 32 + (f & 15);
 }
 
-// The outputs from the partial sums of a split product, which it adds up in split order, with the bias and, where they are wanted, the pre-activations.
+// What the kernels of fp6mi_block.hip do on their way out, for a split product: the outputs from its partial sums, which it adds up in split order, with the bias and, where they are wanted, the pre-activations.
 template <int ACT>
 __global__ __launch_bounds__(256) void gated_reduce(half_t *__restrict__ out, float *__restrict__ preact, const float *__restrict__ ws, const half_t *__restrict__ bias, size_t count,
                                                     uint32_t F, int splits)
@@ -92,6 +92,25 @@ template <typename F> int by_activation(int activation, const F &f)
     return f(std::integral_constant<int, FP6MI_ACT_GELU_TANH>{});
 }
 inline bool known_activation(int a) { return a == FP6MI_ACT_SILU || a == FP6MI_ACT_GELU || a == FP6MI_ACT_GELU_TANH; }
+
+// The launch shape of the gated block: the GEMM's, or the nearest that holds its row tiles in pairs (gemm_stream's odd numbers of them, gemm_tile's single ones) or that its kernels have.
+fp6mi::LaunchCfg gated_shape(int E, int Mb, size_t M, size_t N, size_t K, bool grouped)
+{
+    fp6mi::LaunchCfg c = fp6mi::linear_shape(E, Mb, M, N, K, 1, grouped);
+    if (c.kind == 0) {
+        c.rt += c.rt & 1;
+        if (c.rt == 8 || (c.rt == 6 && c.nt == 2)) c.wk = 4;
+        if (c.rt >= 4 && c.wk == 16) c.wk = 8;
+        return c;
+    }
+    if (c.kind == 2 && c.wk == 4 && c.nt == 2) return { 1, 2, 2, 4, 2 };                           // gemm_ws 256 x 32
+    if (c.kind == 2 && c.wr == 2) return { 2, 8, 4, 4, 1 };                                          // gemm_prefill
+    if (c.kind == 2) return c;
+    if (c.nt == 8) return K <= (size_t)1 << 20 ? fp6mi::LaunchCfg{ 2, 8, 4, 4, 1 } : fp6mi::LaunchCfg{ 1, 4, 2, 8, 1 };
+    if (c.nt == 2) return { 1, 2, 2, 4, c.wk >= 4 ? 4 : c.wk };
+    if (c.nt == 4 && c.wk == 2) return { 1, 4, 2, 4, 2 };
+    return { 1, c.nt, 2, 8, 1 };
+}
 
 // ---------------------------------------------------------------------------------------------------------------
 // Low-rank adapters of many requests: y[n] += s[a] * (x[n] . A[a]^T) . B[a]^T, a = index[n] (none where it is no slot's number).
@@ -344,7 +363,17 @@ int fp6mi_linear_grad_native(int E, int Mb, void *stream, const void *W, const v
     return rc != FP6MI_OK ? rc : run_grad(E, Mb, stream, W, sc, group_exps, dY, false, dX, M, N, K, ws, splits);
 }
 
-size_t fp6mi_gated_workspace_bytes(size_t M, size_t N, int splitK) { return fp6mi_workspace_bytes(M, N, splitK > 1 ? splitK : 2); }
+size_t fp6mi_gated_workspace_bytes(size_t M, size_t N, int splitK) { return fp6mi_workspace_bytes(M, N, splitK); }
+
+int fp6mi_query_gated_launch(int E, int Mb, size_t M, size_t N, size_t K, int grouped, int *shape)
+{
+    if (!fp6mi::supported(E, Mb)) return FP6MI_ERR_FORMAT;
+    if (M == 0 || M % 256 || K == 0 || K % 64 || N == 0) return FP6MI_ERR_SHAPE;
+    if (!shape) return FP6MI_ERR_NULL;
+    const fp6mi::LaunchCfg c = gated_shape(E, Mb, M, N, K, grouped != 0);
+    shape[0] = c.kind, shape[1] = c.nt, shape[2] = c.rt, shape[3] = c.wr, shape[4] = c.wk;
+    return FP6MI_OK;
+}
 
 int fp6mi_gated_native(int E, int Mb, void *stream, const void *W, const void *sc, const void *group_exps, const void *bias, const void *B, void *C, float *preact, size_t M, size_t N, size_t K,
                        int activation, float *ws, int splitK)
@@ -353,14 +382,13 @@ int fp6mi_gated_native(int E, int Mb, void *stream, const void *W, const void *s
     if (rc != FP6MI_OK) return rc;
     if (!known_activation(activation)) return FP6MI_ERR_ACTIVATION;
     if (preact && !aligned16(preact)) return FP6MI_ERR_ALIGN;
-    if (!ws) return FP6MI_ERR_WORKSPACE;
     if (N * (M / 2) > kMostOutputs) return FP6MI_ERR_SHAPE;
-    const int    splits = splitK > 1 ? splitK : 2;
+    if (splitK == 1) return fp6mi::block_ops_for(E, Mb)->gated(gated_shape(E, Mb, M, N, K, group_exps != nullptr), stream, W, sc, group_exps, bias, B, C, preact, M, N, K, activation);
     const size_t count = N * (M / 2);
-    if (const int e = fp6mi::run_linear(E, Mb, stream, W, sc, group_exps, nullptr, B, C, M, N, K, ws, splits, true)) return e;
+    if (const int e = fp6mi::run_linear(E, Mb, stream, W, sc, group_exps, nullptr, B, C, M, N, K, ws, splitK, true)) return e;
     return by_activation(activation, [&](auto act) {
-        hipLaunchKernelGGL(gated_reduce<decltype(act)::value>, dim3((uint32_t)((count / 4 + 255) / 256)), dim3(256), 0, static_cast<hipStream_t>(stream), static_cast<half_t *>(C),
-                           preact, ws, static_cast<const half_t *>(bias), count, (uint32_t)(M / 2), splits);
+        hipLaunchKernelGGL(gated_reduce<decltype(act)::value>, dim3((uint32_t)((count / 4 + 255) / 256)), dim3(256), 0, static_cast<hipStream_t>(stream), static_cast<half_t *>(C), preact, ws,
+                           static_cast<const half_t *>(bias), count, (uint32_t)(M / 2), splitK);
         return (int)hipGetLastError();
     });
 }

@@ -234,13 +234,15 @@ size_t fp6mi_grad_workspace_bytes(size_t N, size_t K, int splits);
 
 /* Gated feed-forward block: H[N,M/2] = act(B . Wg^T + bg) * (B . Wu^T + bu).  The two matrices are one of M rows in PAIR ORDER: 16 rows of Wg, the same 16 of Wu,
  * and so on (scales, group exponents and bias likewise; in the native layout that is whole row tiles in turn).  preact, unless NULL, receives the
- * pre-activations [N,M] in pair order, the FP32 sums as they are, for the backward pass.  workspace: fp6mi_gated_workspace_bytes bytes. */
+ * pre-activations [N,M] in pair order, the FP32 sums as they are, for the backward pass.  workspace: fp6mi_gated_workspace_bytes bytes, none without a split. */
 #define FP6MI_ACT_SILU 0
 #define FP6MI_ACT_GELU 1      /* g * P(g), P the normal distribution */
 #define FP6MI_ACT_GELU_TANH 2 /* its approximation by a hyperbolic tangent */
 int    fp6mi_gated_native(int E, int Mbits, void *stream, const void *W_native, const void *scales_f16, const void *group_exps_native, const void *bias_f16,
                           const void *B_f16, void *H_f16, float *preact, size_t M, size_t N, size_t K, int activation, float *workspace, int splitK);
 size_t fp6mi_gated_workspace_bytes(size_t M, size_t N, int splitK);
+/* Its launch shape without a split, in the terms of fp6mi_query_launch. */
+int fp6mi_query_gated_launch(int E, int Mbits, size_t M, size_t N, size_t K, int grouped, int *shape);
 /* Its backward pass from the gradient of H: grad_preact[N,M] in pair order (the gradient that a bias sums over N, or an adapter beside the block takes; not written where it
  * is NULL) and grad_in[N,K] = grad_preact . dequant(W).  The weights have no gradient.  workspace: fp6mi_gated_backward_workspace_bytes bytes, always; splits as in
  * fp6mi_linear_grad_native. */

@@ -423,7 +423,7 @@ def test_refusals_of_the_c_abi():
     assert grad(s=2) == -4 and grad(s=0) == -5 and grad(dy=p + 8) == -6 and grad(ge=p + 1) == -6 and grad(OC=(1 << 20) + 256) == -2
     gated = lambda act=0, x=p, h=p, pre=None, ws=p, s=1, OC=256, bias=None: L.fp6mi_gated_native(3, 2, None, p, p, None, bias, x, h, pre, OC, 4, 64, act, ws, s)   # noqa: E731
     assert gated(act=3) == -9 and gated(act=-1) == -9 and gated(OC=0) == -2 and gated(x=None) == -3 and gated(h=None) == -3 and gated(pre=p + 2) == -6 and gated(bias=p + 1) == -6
-    assert gated(s=2, ws=None) == -4 and gated(s=0) == -5
+    assert gated(s=2, ws=None) == -4 and gated(s=0) == -5 and L.fp6mi_query_gated_launch(3, 2, 256, 4, 64, 0, None) == -3
     back = lambda act=0, dh=p, pre=p, dp=p, dx=p, ws=p, s=1: L.fp6mi_gated_backward_native(3, 2, None, p, p, None, dh, pre, dp, dx, 256, 4, 64, act, ws, s)   # noqa: E731
     assert back(act=9) == -9 and back(dh=None) == -3 and back(pre=None) == -3 and back(ws=None) == -4 and back(dx=None) == -3 and back(dh=p + 4) == -6 and back(dp=p + 4) == -6 and back(s=0) == -5
     lora = lambda a=p, b=p, sc=p, ix=p, R=16, slots=2, ws=p, s=1: L.fp6mi_adapter_native(3, 2, None, p, p, None, None, p, p, a, b, sc, ix, 256, 4, 64, R, slots, ws, s)   # noqa: E731
