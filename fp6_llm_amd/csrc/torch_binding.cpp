@@ -10,6 +10,7 @@
 #include <c10/hip/HIPStream.h>
 #include <hip/hip_runtime_api.h>
 
+#include <climits>
 #include <map>
 #include <mutex>
 #include <string>
@@ -412,6 +413,156 @@ pybind11::object weight_quantize_native(int64_t E, int64_t Mb, pybind11::handle 
     raise_status(fp6mi_quantize_native_gpu((int)E, (int)Mb, stream, native.data_ptr(), scales.data_ptr(), w.data_ptr(), dtype, (size_t)OC, (size_t)IC), "fp6mi_quantize_native_gpu");
     return pybind11::make_tuple(native, scales);
 }
+
+// ---- the operators around the linear layer (fp6_llm_amd/ops.py): their checks in their order, and one call each.  A launch's own host time counts for them as for the linear layer:
+// with 1024 x 1024 weights at batch 1 a call of the gated block takes 5.3 us here and 14.0 through ctypes, of the input gradient 7.8 and 16.9, with adapters 11.0 and 22.1. ----
+typedef c10::optional<at::Tensor> OptTensor;
+
+struct WeightArgs { const void *w, *sc, *gexp; at::Tensor keep; }; // keep: scales that had to be made contiguous
+
+WeightArgs check_weights(int64_t E, int64_t Mb, const at::Tensor &native, const at::Tensor &scales, int64_t OC, int64_t IC, const OptTensor &gexp, const at::Device &dev)
+{
+    check_format(E, Mb);
+    if (OC < 256 || OC % 256 || IC < 64 || IC % 64) bad("need OC % 256 == 0 and IC % 64 == 0 (got OC=" + std::to_string(OC) + " IC=" + std::to_string(IC) + ")");
+    if (native.device() != dev || scales.device() != dev) bad("activations, weights and scales must be on the same GPU");
+    if (!native.is_contiguous() || (int64_t)native.numel() * (int64_t)native.element_size() != (int64_t)fp6mi_native_bytes((int)E, (int)Mb, (size_t)OC, (size_t)IC))
+        bad("native_weight must be contiguous and of the size for OC=" + std::to_string(OC) + " IC=" + std::to_string(IC));
+    if (scales.scalar_type() != at::kHalf || scales.numel() != OC) bad("scales must be float16 [OC]");
+    if (gexp.has_value() && (gexp->scalar_type() != at::kByte || gexp->device() != dev || !gexp->is_contiguous() || gexp->numel() != (int64_t)fp6mi_group_exps_bytes((size_t)OC, (size_t)IC)))
+        bad("group_exps must be the contiguous uint8 tensor of pack_group_exps(exps, OC, IC) on the weights' GPU");
+    WeightArgs a = { native.data_ptr(), nullptr, gexp.has_value() ? gexp->data_ptr() : nullptr, scales.is_contiguous() ? scales : scales.contiguous() };
+    a.sc = a.keep.data_ptr();
+    return a;
+}
+at::Tensor activations(const at::Tensor &t, const char *name, int64_t cols = -1)
+{
+    if (t.scalar_type() != at::kHalf || t.dim() != 2 || !t.is_cuda()) bad(std::string(name) + " must be a 2-D float16 tensor on the GPU");
+    if (t.size(0) < 1 || (cols >= 0 && t.size(1) != cols))
+        bad(std::string(name) + " must be [B >= 1, " + (cols < 0 ? "*" : std::to_string(cols)) + "], got [" + std::to_string(t.size(0)) + ", " + std::to_string(t.size(1)) + "]");
+    return t.is_contiguous() ? t : t.contiguous();
+}
+void check_tensor(const at::Tensor &t, at::IntArrayRef shape, at::ScalarType type, const at::Device &dev, const char *name)
+{
+    if (t.sizes() == shape && t.scalar_type() == type && t.is_contiguous() && t.device() == dev) return;
+    std::string s;
+    for (int64_t n : shape) s += (s.empty() ? "[" : ", ") + std::to_string(n);
+    bad(std::string(name) + " must be a contiguous " + (type == at::kHalf ? "float16 " : type == at::kFloat ? "float32 " : "int32 ") + s + "] tensor on the same GPU");
+}
+at::Tensor result(const OptTensor &out, at::IntArrayRef shape, const at::Device &dev, const char *name)
+{
+    if (!out.has_value()) return at::empty(shape, at::TensorOptions().dtype(at::kHalf).device(dev));
+    check_tensor(*out, shape, at::kHalf, dev, name);
+    return *out;
+}
+int64_t split_of(int64_t splitK, int (*heuristic)(int, int, size_t, size_t, size_t, int), int64_t E, int64_t Mb, int64_t OC, int64_t B, int64_t IC)
+{
+    if (splitK == INT64_MIN) return heuristic((int)E, (int)Mb, (size_t)OC, (size_t)B, (size_t)IC, 256); // (None: MI355X_CUS compute units)
+    if (splitK < 1 || splitK > INT_MAX) bad("splitK must be >= 1");
+    return splitK;
+}
+int linear_split(int E, int Mb, size_t OC, size_t B, size_t IC, int cus) { return fp6mi_heuristic_splitk_within(E, Mb, OC, B, IC, cus, (size_t)96 << 20); } // SPLIT_WORKSPACE_BYTES
+float *scratch(const OptTensor &given, const at::Device &dev, void *stream, size_t bytes, at::Tensor &keep)
+{
+    if (bytes == 0) return nullptr;
+    if (given.has_value()) {
+        if (given->scalar_type() != at::kFloat || (size_t)given->numel() * 4 < bytes || given->device() != dev || !given->is_contiguous())
+            bad("workspace must be a contiguous float32 tensor of at least " + std::to_string(bytes) + " bytes on the same GPU");
+        keep = *given;
+    } else {
+        keep = workspace_for(dev, stream, (int64_t)((bytes + 3) / 4));
+    }
+    return keep.data_ptr<float>();
+}
+const void *pointer(const OptTensor &t) { return t.has_value() ? t->data_ptr() : nullptr; }
+
+at::Tensor gated_forward(int64_t E, int64_t Mb, const at::Tensor &in_feats, const at::Tensor &native, const at::Tensor &scales, int64_t OC, int64_t activation, int64_t splitK,
+                         const OptTensor &out_opt, const OptTensor &preact, const OptTensor &ws_opt, const OptTensor &gexp, const OptTensor &bias)
+{
+    const at::Tensor   x = activations(in_feats, "in_feats");
+    const int64_t      B = x.size(0), IC = x.size(1);
+    const at::Device   dev = x.device();
+    const WeightArgs   w = check_weights(E, Mb, native, scales, OC, IC, gexp, dev);
+    const int64_t      s = split_of(splitK, &linear_split, E, Mb, OC, B, IC);
+    c10::hip::HIPGuard guard(dev.index());
+    const at::Tensor   out = result(out_opt, { B, OC / 2 }, dev, "out");
+    if (preact.has_value()) check_tensor(*preact, { B, OC }, at::kFloat, dev, "preact");
+    if (bias.has_value()) check_tensor(*bias, { OC }, at::kHalf, dev, "bias");
+    void      *stream = c10::hip::getCurrentHIPStream(dev.index()).stream();
+    at::Tensor keep;
+    float     *ws = scratch(ws_opt, dev, stream, fp6mi_gated_workspace_bytes((size_t)OC, (size_t)B, (int)s), keep);
+    raise_status(fp6mi_gated_native((int)E, (int)Mb, stream, w.w, w.sc, w.gexp, pointer(bias), x.data_ptr(), out.data_ptr(), preact.has_value() ? preact->data_ptr<float>() : nullptr,
+                                    (size_t)OC, (size_t)B, (size_t)IC, (int)activation, ws, (int)s),
+                 "fp6mi_gated_native");
+    return out;
+}
+
+pybind11::object gated_backward(int64_t E, int64_t Mb, const at::Tensor &grad_out, const at::Tensor &preact, const at::Tensor &native, const at::Tensor &scales, int64_t IC, int64_t activation,
+                                int64_t splitK, const OptTensor &grad_in_opt, const OptTensor &grad_preact_opt, bool want_preact, const OptTensor &ws_opt, const OptTensor &gexp)
+{
+    if (preact.scalar_type() != at::kFloat || preact.dim() != 2 || !preact.is_cuda() || !preact.is_contiguous())
+        bad("preact must be the contiguous float32 [B, OC] tensor that gated_forward_native filled");
+    const int64_t    B = preact.size(0), OC = preact.size(1);
+    const at::Device dev = preact.device();
+    const at::Tensor d = activations(grad_out, "grad_out", OC / 2);
+    if (d.size(0) != B || d.device() != dev) bad("grad_out and preact must have the same rows, on the same GPU");
+    const WeightArgs   w = check_weights(E, Mb, native, scales, OC, IC, gexp, dev);
+    const int64_t      s = split_of(splitK, &fp6mi_heuristic_grad_splits, E, Mb, OC, B, IC);
+    c10::hip::HIPGuard guard(dev.index());
+    const at::Tensor   grad_in = result(grad_in_opt, { B, IC }, dev, "grad_in");
+    OptTensor          grad_preact;
+    if (want_preact) grad_preact = result(grad_preact_opt, { B, OC }, dev, "grad_preact");
+    void      *stream = c10::hip::getCurrentHIPStream(dev.index()).stream();
+    at::Tensor keep;
+    float     *ws = scratch(ws_opt, dev, stream, fp6mi_gated_backward_workspace_bytes((size_t)OC, (size_t)B, (size_t)IC, (int)s), keep);
+    raise_status(fp6mi_gated_backward_native((int)E, (int)Mb, stream, w.w, w.sc, w.gexp, d.data_ptr(), preact.data_ptr<float>(), const_cast<void *>(pointer(grad_preact)), grad_in.data_ptr(),
+                                             (size_t)OC, (size_t)B, (size_t)IC, (int)activation, ws, (int)s),
+                 "fp6mi_gated_backward_native");
+    return pybind11::make_tuple(grad_in, grad_preact);
+}
+
+at::Tensor linear_input_grad(int64_t E, int64_t Mb, const at::Tensor &grad_out, const at::Tensor &native, const at::Tensor &scales, int64_t IC, int64_t splitK, const OptTensor &out_opt,
+                             const OptTensor &ws_opt, const OptTensor &gexp)
+{
+    const at::Tensor   d = activations(grad_out, "grad_out");
+    const int64_t      B = d.size(0), OC = d.size(1);
+    const at::Device   dev = d.device();
+    const WeightArgs   w = check_weights(E, Mb, native, scales, OC, IC, gexp, dev);
+    const int64_t      s = split_of(splitK, &fp6mi_heuristic_grad_splits, E, Mb, OC, B, IC);
+    c10::hip::HIPGuard guard(dev.index());
+    const at::Tensor   out = result(out_opt, { B, IC }, dev, "out");
+    void              *stream = c10::hip::getCurrentHIPStream(dev.index()).stream();
+    at::Tensor         keep;
+    float             *ws = scratch(ws_opt, dev, stream, fp6mi_grad_workspace_bytes((size_t)B, (size_t)IC, (int)s), keep);
+    raise_status(fp6mi_linear_grad_native((int)E, (int)Mb, stream, w.w, w.sc, w.gexp, d.data_ptr(), out.data_ptr(), (size_t)OC, (size_t)B, (size_t)IC, ws, (int)s), "fp6mi_linear_grad_native");
+    return out;
+}
+
+at::Tensor adapter_forward(int64_t E, int64_t Mb, const at::Tensor &in_feats, const at::Tensor &native, const at::Tensor &scales, int64_t OC, const at::Tensor &lora_a, const at::Tensor &lora_b,
+                           const at::Tensor &scaling, const at::Tensor &index, int64_t splitK, const OptTensor &out_opt, const OptTensor &ws_opt, const OptTensor &gexp, const OptTensor &bias)
+{
+    const at::Tensor x = activations(in_feats, "in_feats");
+    const int64_t    B = x.size(0), IC = x.size(1);
+    const at::Device dev = x.device();
+    const WeightArgs w = check_weights(E, Mb, native, scales, OC, IC, gexp, dev);
+    if (lora_a.dim() != 3 || lora_a.size(2) != IC || lora_a.size(0) < 1) bad("lora_a must be [slots, R, IC=" + std::to_string(IC) + "]");
+    const int64_t slots = lora_a.size(0), R = lora_a.size(1);
+    if (R < 8 || R % 8 || R > 256) bad("the rank must be a multiple of 8 up to 256, got " + std::to_string(R));
+    check_tensor(lora_a, { slots, R, IC }, at::kHalf, dev, "lora_a");
+    check_tensor(lora_b, { slots, OC, R }, at::kHalf, dev, "lora_b");
+    check_tensor(scaling, { slots }, at::kFloat, dev, "scaling");
+    check_tensor(index, { B }, at::kInt, dev, "index");
+    if (bias.has_value()) check_tensor(*bias, { OC }, at::kHalf, dev, "bias");
+    const int64_t      s = split_of(splitK, &linear_split, E, Mb, OC, B, IC);
+    c10::hip::HIPGuard guard(dev.index());
+    const at::Tensor   out = result(out_opt, { B, OC }, dev, "out");
+    void              *stream = c10::hip::getCurrentHIPStream(dev.index()).stream();
+    at::Tensor         keep;
+    float             *ws = scratch(ws_opt, dev, stream, fp6mi_adapter_workspace_bytes((size_t)OC, (size_t)B, (size_t)IC, (size_t)R, (int)s), keep);
+    raise_status(fp6mi_adapter_native((int)E, (int)Mb, stream, w.w, w.sc, w.gexp, pointer(bias), x.data_ptr(), out.data_ptr(), lora_a.data_ptr(), lora_b.data_ptr(), scaling.data_ptr<float>(),
+                                      index.data_ptr<int>(), (size_t)OC, (size_t)B, (size_t)IC, (size_t)R, (size_t)slots, ws, (int)s),
+                 "fp6mi_adapter_native");
+    return out;
+}
 } // namespace
 
 PYBIND11_MODULE(_fp6mi_torch, m)
@@ -429,6 +580,10 @@ PYBIND11_MODULE(_fp6mi_torch, m)
     m.def("weight_dequant_native", &weight_dequant_native, pybind11::arg("E").noconvert(), pybind11::arg("M").noconvert(), pybind11::arg("native"), pybind11::arg("scales"),
           pybind11::arg("OC").noconvert(), pybind11::arg("IC").noconvert(), pybind11::arg("group_exps"));
     m.def("weight_quantize_native", &weight_quantize_native, pybind11::arg("E").noconvert(), pybind11::arg("M").noconvert(), pybind11::arg("weight"), pybind11::arg("group_scales"));
+    m.def("gated_forward", &gated_forward);
+    m.def("gated_backward", &gated_backward);
+    m.def("linear_input_grad", &linear_input_grad);
+    m.def("adapter_forward", &adapter_forward);
     // the reference's bindings, name for name (fp6_llm/csrc/pybind.cpp:8-15)
     m.def("linear_forward_cuda", &fp6_linear_forward_cuda, "Computes FP6-FP16 GEMM.", pybind11::arg("in_feats"), pybind11::arg("weights"),
           pybind11::arg("scales"), pybind11::arg("splitK") = 1);

@@ -1,13 +1,15 @@
 """Operators around the FPx linear layer, on the same native-layout weights: the gated feed-forward block with its backward pass, the input gradient of a
 layer, and low-rank adapters of many requests beside a shared projection.  (The reference has the forward product alone.)
 
-The functions enqueue on the current stream and check shapes, types and devices on the host, like linear_forward_native; what they compute is in include/fp6mi.h."""
+The functions enqueue on the current stream and check shapes, types and devices on the host, like linear_forward_native; what they compute is in include/fp6mi.h.  They go through
+the torch extension where it is built (csrc/torch_binding.cpp makes the same checks), else through ctypes."""
 import threading
 
 import torch
 
 from . import _lib
 
+_HEURISTIC = -2 ** 63   # the extension's splitK for None
 ACTIVATIONS = {"silu": 0, "gelu": 1, "gelu_tanh": 2}
 MAX_RANK = 256
 _launch_lock = threading.Lock()   # the kernels of one call share a workspace: two threads on one stream must not interleave theirs (ctypes lets go of the interpreter's lock)
@@ -98,11 +100,13 @@ def gated_forward_native(EXPONENT, MANTISSA, in_feats, native_weight, scales, OC
     """out[B, OC/2] = act(in_feats @ gate^T + bias_g) * (in_feats @ up^T + bias_u): both projections of a gated feed-forward block, the activation ("silu", "gelu",
     "gelu_tanh") and the product.  native_weight, scales, group_exps and bias are those of one matrix of OC = 2F rows in pair order (gate_up_pairs).
     preact: contiguous float32 [B, OC] that receives the pre-activations in pair order, for gated_backward_native.  splitK: None for the heuristic's."""
-    from . import heuristic_splitk_mi355x
+    from . import _ext, heuristic_splitk_mi355x
+    act = _activation_code(activation)
+    if _ext is not None:
+        return _ext.gated_forward(EXPONENT, MANTISSA, in_feats, native_weight, scales, OC, act, _HEURISTIC if splitK is None else int(splitK), out, preact, workspace, group_exps, bias)
     x = _activations(in_feats, "in_feats")
     (B, IC), dev = x.shape, x.device
     _check_weights(EXPONENT, MANTISSA, native_weight, scales, OC, IC, group_exps, dev)
-    act = _activation_code(activation)
     s = _split(splitK, lambda: heuristic_splitk_mi355x(OC, B, IC, EXPONENT=EXPONENT, MANTISSA=MANTISSA))
     out = _result(out, (B, OC // 2), dev)
     if preact is not None:
@@ -124,6 +128,11 @@ def gated_backward_native(EXPONENT, MANTISSA, grad_out, preact, native_weight, s
                           group_exps=None):
     """The backward pass of gated_forward_native from grad_out [B, OC/2] and the preact [B, OC] it filled: (grad_in [B, IC], grad_preact [B, OC] in pair order).
     grad_preact is what a bias sums over the batch, or an adapter beside the block takes; False leaves it out (and None comes back).  The weights have no gradient."""
+    from . import _ext
+    act = _activation_code(activation)
+    if _ext is not None:
+        return _ext.gated_backward(EXPONENT, MANTISSA, grad_out, preact, native_weight, scales, IC, act, _HEURISTIC if splitK is None else int(splitK), grad_in,
+                                   None if grad_preact is False else grad_preact, grad_preact is not False, workspace, group_exps)
     if preact.dtype != torch.float32 or preact.dim() != 2 or preact.device.type != "cuda" or not preact.is_contiguous():
         raise ValueError("preact must be the contiguous float32 [B, OC] tensor that gated_forward_native filled")
     (B, OC), dev = preact.shape, preact.device
@@ -131,7 +140,6 @@ def gated_backward_native(EXPONENT, MANTISSA, grad_out, preact, native_weight, s
     if d.shape[0] != B or d.device != dev:
         raise ValueError("grad_out and preact must have the same rows, on the same GPU")
     _check_weights(EXPONENT, MANTISSA, native_weight, scales, OC, IC, group_exps, dev)
-    act = _activation_code(activation)
     s = _split(splitK, lambda: _grad_splits(EXPONENT, MANTISSA, OC, B, IC))
     grad_in = _result(grad_in, (B, IC), dev, "grad_in")
     grad_preact = None if grad_preact is False else _result(grad_preact, (B, OC), dev, "grad_preact")
@@ -145,6 +153,9 @@ def gated_backward_native(EXPONENT, MANTISSA, grad_out, preact, native_weight, s
 def linear_input_grad_native(EXPONENT, MANTISSA, grad_out, native_weight, scales, IC, splitK=None, out=None, workspace=None, group_exps=None):
     """out[B, IC] = grad_out[B, OC] @ dequant(W): the gradient of linear_forward_native with respect to in_feats, from the same native-layout weights.
     (grad_out times the mantissa of a row's scale is rounded to float16 once, the products are summed in float32.)  splitK: parts of the sum over OC, None for the heuristic's."""
+    from . import _ext
+    if _ext is not None:
+        return _ext.linear_input_grad(EXPONENT, MANTISSA, grad_out, native_weight, scales, IC, _HEURISTIC if splitK is None else int(splitK), out, workspace, group_exps)
     d = _activations(grad_out, "grad_out")
     (B, OC), dev = d.shape, d.device
     _check_weights(EXPONENT, MANTISSA, native_weight, scales, OC, IC, group_exps, dev)
@@ -162,7 +173,10 @@ def adapter_forward_native(EXPONENT, MANTISSA, in_feats, native_weight, scales, 
     out[n] = in_feats[n] @ dequant(W)^T + bias + scaling[a] * (in_feats[n] @ lora_a[a]^T) @ lora_b[a]^T,  a = index[n].
     lora_a: float16 [slots, R, IC], lora_b: float16 [slots, OC, R], scaling: float32 [slots], index: int32 [B], all on the GPU; a row whose index is no slot's number (-1,
     say) has no adapter.  R is a multiple of 8 up to 256: pad smaller ranks with zeros."""
-    from . import heuristic_splitk_mi355x
+    from . import _ext, heuristic_splitk_mi355x
+    if _ext is not None:
+        return _ext.adapter_forward(EXPONENT, MANTISSA, in_feats, native_weight, scales, OC, lora_a, lora_b, scaling, index, _HEURISTIC if splitK is None else int(splitK), out,
+                                    workspace, group_exps, bias)
     x = _activations(in_feats, "in_feats")
     (B, IC), dev = x.shape, x.device
     _check_weights(EXPONENT, MANTISSA, native_weight, scales, OC, IC, group_exps, dev)
