@@ -114,176 +114,433 @@ fp6mi::LaunchCfg gated_shape(int E, int Mb, size_t M, size_t N, size_t K, bool g
 
 // ---------------------------------------------------------------------------------------------------------------
 // Low-rank adapters of many requests: y[n] += s[a] * (x[n] . A[a]^T) . B[a]^T, a = index[n] (none where it is no slot's number).
-// Batch rows are taken sixteen at a time, in their order; the distinct adapters among the sixteen are found by comparing their numbers, and each gets its own pass
-// with the MFMA's other fifteen columns along for the ride.  So no sorting and no lists are needed, an adapter's matrices are read once for each sixteen rows that hold it,
-// and sixteen rows of one request take one pass.
+// Batch rows are taken 16 or 64 at a time, in their order, a lane holding the adapter of a row.  The lowest row that is left names the adapter of the next pass, a comparison of all
+// lanes the rows that share it, and the MFMA's other columns go along for the ride.  So no sorting and no lists are needed, an adapter's matrices are read once for
+// every tile that holds it, and a tile of one request takes one pass.  Passes of a tile are shared out over the grid's third dimension: they write different rows.
 // ---------------------------------------------------------------------------------------------------------------
 
-// The distinct adapters of batch rows 16 * tile ..: `mine` is the adapter of row (lane & 15) or -1, and the result has bit i set where row i is the first with its adapter.
-__device__ __forceinline__ uint32_t distinct_adapters(const int *__restrict__ index, uint32_t tile, uint32_t N, uint32_t slots, int &mine)
+// the adapter of row (lane) of a tile of ROWS rows, or -1
+template <int ROWS> __device__ __forceinline__ int adapter_of(const int *__restrict__ index, uint32_t tile, uint32_t N, uint32_t slots)
 {
-    const int      i = threadIdx.x & 15;
-    const uint32_t n = tile * 16 + i;
-    const int      v = n < N ? index[n] : -1;
-    mine = (uint32_t)v < slots ? v : -1;
-    bool first = mine >= 0;
-#pragma unroll
-    for (int j = 0; j < 15; j++) {
-        const int other = __shfl(mine, j, 16); // (every lane takes part)
-        first = first & !((j < i) & (other == mine));
+    const uint32_t lane = threadIdx.x & 63, n = tile * ROWS + lane;
+    const int      v = lane < ROWS && n < N ? index[n] : -1;
+    return (uint32_t)v < slots ? v : -1;
+}
+// The passes of this workgroup, numbered from the tile's first: blockIdx.z-th share of gridDim.z, of TOGETHER at least.  A workgroup without any ends before it has asked for anything but
+// the index.  (A further pass of a workgroup waits for the adapter's matrix alone, a further workgroup for everything: with tiles of 64 rows and 11 requests of random lengths
+// in 2048 rows, 10240 x 8192 at rank 64, one pass a workgroup made the call 366 us where this makes it 343.)
+struct Passes { uint32_t first, end; };
+template <uint32_t TOGETHER> __device__ __forceinline__ Passes passes_of(int mine)
+{
+    uint32_t count = 0;
+    for (uint64_t todo = __ballot(mine >= 0); todo; count++) todo &= ~__ballot(mine == __builtin_amdgcn_readlane(mine, __builtin_ctzll(todo)));
+    const uint32_t share = (count + gridDim.z - 1) / gridDim.z, per = share > TOGETHER ? share : TOGETHER, first = blockIdx.z * per;
+    return { first < count ? first : count, first + per < count ? first + per : count };
+}
+// f(adapter, rows that have it) for each of them.  The same in all wavefronts of a workgroup.
+template <typename F> __device__ __forceinline__ void each_adapter(int mine, Passes p, const F &f)
+{
+    uint32_t z = 0;
+    for (uint64_t todo = __ballot(mine >= 0); z < p.end; z++) {
+        const int      a = __builtin_amdgcn_readlane(mine, __builtin_ctzll(todo));
+        const uint64_t same = __ballot(mine == a);
+        todo &= ~same;
+        if (z >= p.first) f(a, same);
     }
-    return (uint32_t)__ballot(first) & 0xffffu;
 }
 
-// shrink: part[s][n][r] = sum over K range s of x[n, k] * A[a, r, k], fp32.  grid = (row tiles, K ranges, passes side by side); the four wavefronts of a workgroup take every fourth
-// 64 columns of its range and add up through LDS.
+// shrink: part[range][n][r] = sum over a range of K of x[n, k] * A[a, r, k], fp32.  grid = (tiles, K ranges, passes side by side).  Ranks are taken RT * 16 at a time.
+//
+// adapter_shrink, for few rows: tiles of sixteen, operands straight from memory, the four wavefronts of a workgroup taking every fourth 64 columns of its range and meeting in LDS.
+// Bound by latency: three round trips, to the index, to the operands and to the output (4096 columns, 32 rows of 32 requests, rank 16: 4.4 us).
 template <int RT>
 __global__ __launch_bounds__(256) void adapter_shrink(float *__restrict__ part, const half_t *__restrict__ x, const half_t *__restrict__ A, const int *__restrict__ index, uint32_t N,
                                                       uint32_t K, uint32_t R, uint32_t slots)
 {
     __shared__ __attribute__((aligned(16))) float sums[3][RT][256];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, q = lane >> 4;
-    int       mine;
-    uint32_t  firsts = distinct_adapters(index, blockIdx.x, N, slots, mine);
-    for (uint32_t z = blockIdx.z; z > 0 && firsts; z--) firsts &= firsts - 1;
+    const int mine = adapter_of<16>(index, blockIdx.x, N, slots), here = __shfl(mine, col);
+    const Passes mypasses = passes_of<1>(mine);
+    if (mypasses.first == mypasses.end) return;
 
     const uint32_t pieces = K / 64, avg = pieces / gridDim.y, extra = pieces % gridDim.y;
     const uint32_t p0 = blockIdx.y * avg + (blockIdx.y < extra ? blockIdx.y : extra), p1 = p0 + avg + (blockIdx.y < extra ? 1u : 0u);
     const uint32_t n = blockIdx.x * 16 + col;
     const half_t  *xrow = x + (size_t)(n < N ? n : N - 1) * K + 8 * q;
-    while (firsts) {
-        const int     a = __builtin_amdgcn_readlane(mine, __builtin_ctz(firsts));
-        const half_t *rows = A + (size_t)a * R * K + 8 * q;
-        v4f           acc[RT];
+    each_adapter(mine, mypasses, [&](int a, uint64_t) {
+        for (uint32_t r0 = 0; r0 < R; r0 += RT * 16) {
+            const half_t *rows[RT];
+            v4f           acc[RT];
 #pragma unroll
-        for (int r = 0; r < RT; r++) acc[r] = (v4f){ 0.f, 0.f, 0.f, 0.f };
-        for (uint32_t p = p0 + wave; p < p1; p += 4) {
+            for (int r = 0; r < RT; r++) {
+                const uint32_t row = r0 + r * 16 + col < R ? r0 + r * 16 + col : R - 1; // (rows beyond the rank are not stored)
+                rows[r] = A + ((size_t)a * R + row) * K + 8 * q;
+                acc[r] = (v4f){ 0.f, 0.f, 0.f, 0.f };
+            }
+            for (uint32_t p = p0 + wave; p < p1; p += 4) {
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-                const v8h b = *reinterpret_cast<const v8h *>(xrow + p * 64 + 32 * h);
+                for (int h = 0; h < 2; h++) {
+                    const v8h b = *reinterpret_cast<const v8h *>(xrow + (size_t)p * 64 + 32 * h);
+#pragma unroll
+                    for (int r = 0; r < RT; r++)
+                        acc[r] = __builtin_amdgcn_mfma_f32_16x16x32_f16(*reinterpret_cast<const v8h *>(rows[r] + (size_t)p * 64 + 32 * h), b, acc[r], 0, 0, 0);
+                }
+            }
+            if (wave > 0)
+#pragma unroll
+                for (int r = 0; r < RT; r++) *reinterpret_cast<v4f *>(&sums[wave - 1][r][lane * 4]) = acc[r];
+            __syncthreads();
+            if (wave == 0 && here == a) { // acc[r][i]: rank r0 + 16 r + 4 q + i of batch row n
 #pragma unroll
                 for (int r = 0; r < RT; r++) {
-                    const uint32_t row = r * 16 + col < R ? r * 16 + col : R - 1; // (rows beyond the rank are not stored)
-                    const v8h      w = *reinterpret_cast<const v8h *>(rows + (size_t)row * K + p * 64 + 32 * h);
-                    acc[r] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w, b, acc[r], 0, 0, 0);
+#pragma unroll
+                    for (int w = 0; w < 3; w++) acc[r] += *reinterpret_cast<const v4f *>(&sums[w][r][lane * 4]);
+                    const uint32_t rank = r0 + r * 16 + 4 * q;
+                    if (rank < R) *reinterpret_cast<v4f *>(part + ((size_t)blockIdx.y * N + n) * R + rank) = acc[r];
+                }
+            }
+            __syncthreads();
+        }
+    });
+}
+
+// adapter_shrink_tile, for many: tiles of 64 rows, sixteen a wavefront.  Rows and adapter pass through LDS in chunks of 128 columns, loaded as whole rows of 256 bytes a chunk ahead: in
+// operand order sixteen lanes ask for sixteen rows, whose addresses share an L2 channel where K is a power of two (8192 columns, N 2048, rank 64: 41 us, this 22 to 30).  LDS rows
+// are 272 bytes apart, the stride at which the operand reads are free of bank conflicts.
+template <int RT>
+__global__ __launch_bounds__(256) void adapter_shrink_tile(float *__restrict__ part, const half_t *__restrict__ x, const half_t *__restrict__ A, const int *__restrict__ index, uint32_t N,
+                                                           uint32_t K, uint32_t R, uint32_t slots)
+{
+    constexpr int kRow = 272, kX = 4, kA = RT; // bytes of an LDS row; loads of a thread
+    __shared__ __attribute__((aligned(16))) uint8_t lds[2][(64 + RT * 16) * kRow];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 15, q = lane >> 4;
+    const int mine = adapter_of<64>(index, blockIdx.x, N, slots), here = __shfl(mine, wave * 16 + col);
+    const Passes mypasses = passes_of<4>(mine);
+    if (mypasses.first == mypasses.end) return;
+
+    const uint32_t pieces = (K + 127) / 128, avg = pieces / gridDim.y, extra = pieces % gridDim.y;
+    const uint32_t p0 = blockIdx.y * avg + (blockIdx.y < extra ? blockIdx.y : extra), p1 = p0 + avg + (blockIdx.y < extra ? 1u : 0u);
+    const uint32_t at = (tid & 15) * 8; // this thread's columns of a chunk, of rows tid / 16, tid / 16 + 16, ...
+    const half_t  *xrow[kX];
+#pragma unroll
+    for (int j = 0; j < kX; j++) {
+        const uint32_t n = blockIdx.x * 64 + (tid >> 4) + 16 * j;
+        xrow[j] = x + (size_t)(n < N ? n : N - 1) * K;
+    }
+    each_adapter(mine, mypasses, [&](int a, uint64_t) {
+        for (uint32_t r0 = 0; r0 < R; r0 += RT * 16) {
+            const half_t *arow[kA];
+            v4f           acc[RT];
+            v8h           xr[kX], ar[kA];
+#pragma unroll
+            for (int j = 0; j < RT; j++) {
+                const uint32_t row = r0 + (tid >> 4) + 16 * j;
+                arow[j] = A + ((size_t)a * R + (row < R ? row : R - 1)) * K; // (rows beyond the rank are not stored)
+                acc[j] = (v4f){ 0.f, 0.f, 0.f, 0.f };
+            }
+            auto load = [&](uint32_t p) { // (columns beyond K, the second half of a last chunk, are read at the row's start and count as zeros in both)
+                const uint32_t k = p * 128 + at, kk = k < K ? k : 0;
+#pragma unroll
+                for (int j = 0; j < kX; j++) xr[j] = *reinterpret_cast<const v8h *>(xrow[j] + kk);
+#pragma unroll
+                for (int j = 0; j < kA; j++) ar[j] = *reinterpret_cast<const v8h *>(arow[j] + kk);
+                if (k >= K) {
+#pragma unroll
+                    for (int j = 0; j < kX; j++) xr[j] = (v8h)(half_t)0.f;
+#pragma unroll
+                    for (int j = 0; j < kA; j++) ar[j] = (v8h)(half_t)0.f;
+                }
+            };
+            auto store = [&](int buf) {
+#pragma unroll
+                for (int j = 0; j < kX; j++) *reinterpret_cast<v8h *>(lds[buf] + ((tid >> 4) + 16 * j) * kRow + (tid & 15) * 16) = xr[j];
+#pragma unroll
+                for (int j = 0; j < kA; j++) *reinterpret_cast<v8h *>(lds[buf] + (64 + (tid >> 4) + 16 * j) * kRow + (tid & 15) * 16) = ar[j];
+            };
+            if (p0 < p1) load(p0), store(0);
+            __syncthreads();
+            int buf = 0;
+            for (uint32_t p = p0; p < p1; p++, buf ^= 1) {
+                if (p + 1 < p1) load(p + 1);
+#pragma unroll
+                for (int s = 0; s < 4; s++) {
+                    const v8h b = *reinterpret_cast<const v8h *>(lds[buf] + (wave * 16 + col) * kRow + s * 64 + q * 16);
+#pragma unroll
+                    for (int r = 0; r < RT; r++)
+                        acc[r] = __builtin_amdgcn_mfma_f32_16x16x32_f16(*reinterpret_cast<const v8h *>(lds[buf] + (64 + r * 16 + col) * kRow + s * 64 + q * 16), b, acc[r], 0, 0, 0);
+                }
+                if (p + 1 < p1) store(buf ^ 1);
+                __syncthreads();
+            }
+            if (here == a) {
+#pragma unroll
+                for (int r = 0; r < RT; r++) {
+                    const uint32_t rank = r0 + r * 16 + 4 * q;
+                    if (rank < R) *reinterpret_cast<v4f *>(part + ((size_t)blockIdx.y * N + blockIdx.x * 64 + wave * 16 + col) * R + rank) = acc[r];
                 }
             }
         }
-        if (wave > 0)
-#pragma unroll
-            for (int r = 0; r < RT; r++) *reinterpret_cast<v4f *>(&sums[wave - 1][r][lane * 4]) = acc[r];
-        __syncthreads();
-        if (wave == 0) { // acc[r][i]: rank 16 r + 4 q + i of batch row n
-#pragma unroll
-            for (int r = 0; r < RT; r++) {
-#pragma unroll
-                for (int w = 0; w < 3; w++) acc[r] += *reinterpret_cast<const v4f *>(&sums[w][r][lane * 4]);
-                if (mine == a && r * 16 + 4 * q < R) *reinterpret_cast<v4f *>(part + ((size_t)blockIdx.y * N + n) * R + r * 16 + 4 * q) = acc[r];
-            }
-        }
-        __syncthreads();
-        for (uint32_t z = gridDim.z; z > 0 && firsts; z--) firsts &= firsts - 1;
-    }
+    });
 }
 
-// expand: y[n, m] += s[a] * sum over r of t[n, r] * B[a, m, r], t = the sum of part over the K ranges.  grid = (row tiles, blocks of 256 outputs).
-// t is held in fp16 for the MFMA, each row scaled by a power of two that puts its largest magnitude below 2^15: nothing overflows, what is rounded away is 2^-11 of a value at
-// most (2^-39 of the row's largest one for the smallest), and the factor is taken off the fp32 sums.
+// The sums over the K ranges of a row's ranks as the MFMA takes them: fp16, scaled by a power of two that puts the row's largest magnitude below 2^15.  Nothing overflows, what is
+// rounded away is 2^-11 of a value at most (2^-39 of the row's largest one for the smallest), and the factor is taken off the fp32 sums.
+// v: the ranks that this lane of GROUP holds of the row
+template <int GROUP, int COUNT> __device__ __forceinline__ int common_exponent(const float (&v)[COUNT])
+{
+    float top = 0.f;
+#pragma unroll
+    for (int j = 0; j < COUNT; j++) top = fmaxf(top, fabsf(v[j]));
+#pragma unroll
+    for (int d = 1; d < GROUP; d *= 2) top = fmaxf(top, __shfl_xor(top, d, GROUP));
+    const int e = top > 0.f && top < __builtin_inff() ? __builtin_amdgcn_frexp_expf(top) - 15 : 0; // top < 2^(e + 15)
+    return e < -120 ? -120 : e;
+}
+
+// For many rows that is a kernel of its own, a wavefront a row: ranks[n][R rounded up to 32], factor[n] = the power of two times the adapter's scaling
+__global__ __launch_bounds__(256) void adapter_ranks(half_t *__restrict__ ranks, float *__restrict__ factor, const float *__restrict__ part, const float *__restrict__ scaling,
+                                                     const int *__restrict__ index, uint32_t N, uint32_t R, uint32_t slots, uint32_t ranges)
+{
+    const uint32_t lane = threadIdx.x & 63, n = blockIdx.x * 4 + (threadIdx.x >> 6), Rp = (R + 31) & ~31u;
+    if (n >= N) return;
+    const int a = index[n];
+    if ((uint32_t)a >= slots) return;
+    float v[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        v[j] = 0.f;
+        if (lane + 64 * j < R) {
+            const float *at = part + (size_t)n * R + lane + 64 * j;
+            for (uint32_t s0 = 0; s0 < ranges; s0 += 8) { // eight ranges' sums on their way at once
+                float t[8];
+#pragma unroll
+                for (int u = 0; u < 8; u++) t[u] = at[(size_t)(s0 + u < ranges ? s0 + u : 0) * N * R];
+#pragma unroll
+                for (int u = 0; u < 8; u++) v[j] += s0 + u < ranges ? t[u] : 0.f;
+            }
+        }
+    }
+    const int e = common_exponent<64>(v);
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+        if (lane + 64 * j < Rp) ranks[(size_t)n * Rp + lane + 64 * j] = (half_t)ldexpf(v[j], -e);
+    if (lane == 0) factor[n] = ldexpf(1.f, e) * scaling[a];
+}
+
+// expand: y[n, m] += factor[n] * sum over r of t[n, r] * B[a, m, r].  grid = (tiles, blocks of 256 outputs, passes side by side); 64 outputs a wavefront.
+//
+// adapter_expand, for few rows: tiles of sixteen; forms t in LDS from the ranges' sums, which saves a launch and is bound by the latency of it (4096 outputs, 32 rows of 32 requests,
+// rank 16: 7.5 us).
 __global__ __launch_bounds__(256) void adapter_expand(half_t *__restrict__ y, const float *__restrict__ part, const half_t *__restrict__ B, const float *__restrict__ scaling,
                                                       const int *__restrict__ index, uint32_t M, uint32_t N, uint32_t R, uint32_t slots, uint32_t ranges)
 {
     constexpr int kRow = 256 + 8; // halfs
     __shared__ __attribute__((aligned(16))) half_t t16[16 * kRow];
-    __shared__ float                               factor[16];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, q = lane >> 4;
-    int       mine;
-    uint32_t  firsts = distinct_adapters(index, blockIdx.x, N, slots, mine);
-    if (!firsts) return;
-    // thread (row i = tid / 16, piece c = tid % 16) sums ranks c, c + 16, ...
-    {
-        const int      i = threadIdx.x >> 4, c = threadIdx.x & 15;
-        const uint32_t n = blockIdx.x * 16 + i;
-        const bool     has = __shfl(mine, i & 15, 16) >= 0; // (lane i of any sixteen holds row i's)
-        const uint32_t Rp = (R + 31) & ~31u;
-        float          v[16], top = 0.f;
+    __shared__ float                               row_factor[16];
+    const int      lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, q = lane >> 4;
+    const int      mine = adapter_of<16>(index, blockIdx.x, N, slots), here = __shfl(mine, col);
+    const uint32_t m0 = blockIdx.y * 256 + wave * 64, Rp = (R + 31) & ~31u, n = blockIdx.x * 16 + col;
+    const Passes mypasses = passes_of<1>(mine);
+    if (mypasses.first == mypasses.end) return;
+    half_t *const  yrow = y + (size_t)(n < N ? n : N - 1) * M + m0 + 4 * q;
+    v4h            yv[4];
 #pragma unroll
-        for (int j = 0; j < 16; j++) {
-            v[j] = 0.f;
-            const uint32_t r = c + 16 * j;
-            if (has && r < R)
-                for (uint32_t s = 0; s < ranges; s++) v[j] += part[((size_t)s * N + n) * R + r];
-            top = fmaxf(top, fabsf(v[j]));
-        }
-#pragma unroll
-        for (int d = 1; d < 16; d *= 2) top = fmaxf(top, __shfl_xor(top, d, 16));
-        int e = top > 0.f && top < __builtin_inff() ? __builtin_amdgcn_frexp_expf(top) - 15 : 0; // top < 2^(e + 15)
-        e = e < -120 ? -120 : e;
-#pragma unroll
-        for (int j = 0; j < 16; j++)
-            if (c + 16 * j < (int)Rp) t16[i * kRow + c + 16 * j] = (half_t)ldexpf(v[j], -e);
-        if (c == 0) factor[i] = ldexpf(1.f, e);
-    }
-    __syncthreads();
-    const uint32_t n = blockIdx.x * 16 + col;
-    const float    f = mine >= 0 ? factor[col] * scaling[mine] : 0.f;
-    const uint32_t m0 = blockIdx.y * 256 + wave * 64;
-    v4f            out[4];
-#pragma unroll
-    for (int o = 0; o < 4; o++) out[o] = (v4f){ 0.f, 0.f, 0.f, 0.f };
-    while (firsts) {
-        const int     a = __builtin_amdgcn_readlane(mine, __builtin_ctz(firsts));
+    for (int o = 0; o < 4; o++) yv[o] = *reinterpret_cast<const v4h *>(yrow + o * 16);
+    each_adapter(mine, mypasses, [&](int a, uint64_t same) {
         const half_t *rows = B + ((size_t)a * M + m0 + col) * R;
-        v4f           acc[4];
-#pragma unroll
-        for (int o = 0; o < 4; o++) acc[o] = (v4f){ 0.f, 0.f, 0.f, 0.f };
-        for (uint32_t r = 8 * q; r < R + 8 * q; r += 32) { // (the same number of steps in every lane; beyond the rank zeros meet zeros)
-            const v8h t = *reinterpret_cast<const v8h *>(t16 + col * kRow + r);
+        v8h           w[4]; // of the next step; beyond the rank the row's start, and zeros
+        auto          load_w = [&](uint32_t r) {
 #pragma unroll
             for (int o = 0; o < 4; o++) {
-                const v8h w = r < R ? *reinterpret_cast<const v8h *>(rows + (size_t)o * 16 * R + r) : (v8h)(half_t)0.f;
-                acc[o] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w, t, acc[o], 0, 0, 0);
+                w[o] = *reinterpret_cast<const v8h *>(rows + (size_t)o * 16 * R + (r < R ? r : 0));
+                if (r >= R) w[o] = (v8h)(half_t)0.f;
+            }
+        };
+        load_w(8 * q);
+        { // thread (row i = tid / 16, piece c = tid % 16) sums ranks c, c + 16, ...
+            const int      i = threadIdx.x >> 4, c = threadIdx.x & 15;
+            const bool     has = same >> i & 1;
+            const float   *src = part + (size_t)(has ? blockIdx.x * 16 + i : 0) * R; // (row 0 is there to be read)
+            float          v[16];
+            __syncthreads(); // (the pass before has read its ranks)
+#pragma unroll
+            for (int j = 0; j < 16; j++) v[j] = 0.f;
+#pragma unroll
+            for (int j = 0; j < 16; j++)
+                if (16 * j < (int)R) {
+                    const float *at = src + (c + 16 * j < (int)R ? c + 16 * j : 0);
+                    for (uint32_t s0 = 0; s0 < ranges; s0 += 8) { // eight ranges' sums on their way at once
+                        float t[8];
+#pragma unroll
+                        for (int u = 0; u < 8; u++) t[u] = at[(size_t)(s0 + u < ranges ? s0 + u : 0) * N * R];
+#pragma unroll
+                        for (int u = 0; u < 8; u++) v[j] += s0 + u < ranges ? t[u] : 0.f;
+                    }
+                }
+#pragma unroll
+            for (int j = 0; j < 16; j++) v[j] = has && c + 16 * j < (int)R ? v[j] : 0.f;
+            const int e = common_exponent<16>(v);
+#pragma unroll
+            for (int j = 0; j < 16; j++)
+                if (c + 16 * j < (int)Rp) t16[i * kRow + c + 16 * j] = (half_t)ldexpf(v[j], -e);
+            if (c == 0) row_factor[i] = ldexpf(1.f, e) * scaling[a];
+            __syncthreads();
+        }
+        v4f acc[4];
+#pragma unroll
+        for (int o = 0; o < 4; o++) acc[o] = (v4f){ 0.f, 0.f, 0.f, 0.f };
+        for (uint32_t r = 8 * q; r < R + 8 * q; r += 32) { // (the same number of steps in every lane)
+            const v8h t = *reinterpret_cast<const v8h *>(t16 + col * kRow + r);
+#pragma unroll
+            for (int o = 0; o < 4; o++) acc[o] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[o], t, acc[o], 0, 0, 0);
+            load_w(r + 32);
+        }
+        if (here == a) {
+            const float f = row_factor[col];
+#pragma unroll
+            for (int o = 0; o < 4; o++) {
+                v4h h;
+#pragma unroll
+                for (int i = 0; i < 4; i++) h[i] = (half_t)((float)yv[o][i] + f * acc[o][i]);
+                *reinterpret_cast<v4h *>(yrow + o * 16) = h;
+            }
+        }
+    });
+}
+
+// adapter_expand_tile, for many: tiles of 64 rows; t lies in memory (adapter_ranks).  An operand of B feeds four MFMAs.  y is read and written as whole row pieces of 512 bytes, the
+// products reaching them through LDS (sixteen rows a wavefront at once, 32 bytes each, where the row length is a multiple of 4 KB all of one L2 channel: 62 us for 10240 outputs
+// at N 2048, rank 64, eleven requests; this takes 49 to 64, and 26 where one request has all rows).  y is asked for when the products are ready: held from the start it costs 32
+// registers, and a workgroup of every three on a CU.
+constexpr int kExpandRow = 256 * 4 + 16;
+// STEPS: of 32 ranks, asked for at once
+template <int STEPS>
+__global__ __launch_bounds__(256, 2) void adapter_expand_tile(half_t *__restrict__ y, const half_t *__restrict__ ranks, const float *__restrict__ factors, const half_t *__restrict__ B,
+                                                              const int *__restrict__ index, uint32_t M, uint32_t N, uint32_t R, uint32_t slots)
+{
+    __shared__ __attribute__((aligned(16))) uint8_t lds[32 * kExpandRow]; // 32 of the rows at a time
+    const int      tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 15, q = lane >> 4;
+    const int      mine = adapter_of<64>(index, blockIdx.x, N, slots);
+    const uint32_t m0 = blockIdx.y * 256, Rp = (R + 31) & ~31u;
+    const Passes   mypasses = passes_of<4>(mine);
+    if (mypasses.first == mypasses.end) return;
+    // this thread's pieces of y: eight outputs each of rows tid / 32, tid / 32 + 8, ...
+    half_t *const  ybase = y + (size_t)blockIdx.x * 64 * M + m0 + (tid & 31) * 8;
+    const uint32_t nlast = N - blockIdx.x * 64 < 64 ? N - 1 - blockIdx.x * 64 : 63;
+    auto           yp = [&](int j) { const uint32_t n = (tid >> 5) + 8 * j; return ybase + (size_t)(n < nlast ? n : nlast) * M; };
+    const half_t *trow[4];
+    float         f[4];
+#pragma unroll
+    for (int s = 0; s < 4; s++) { // (rows without an adapter hold anything, and are not stored)
+        const uint32_t n = blockIdx.x * 64 + (16 * s + col < (int)nlast ? 16 * s + col : nlast);
+        trow[s] = ranks + (size_t)n * Rp;
+        f[s] = factors[n];
+    }
+    each_adapter(mine, mypasses, [&](int a, uint64_t same) {
+        const half_t *rows = B + ((size_t)a * M + m0 + wave * 64 + col) * R;
+        v4f           acc[4][4];
+#pragma unroll
+        for (int s = 0; s < 4; s++)
+#pragma unroll
+            for (int o = 0; o < 4; o++) acc[s][o] = (v4f){ 0.f, 0.f, 0.f, 0.f };
+        for (uint32_t r0 = 0; r0 < R; r0 += 32 * STEPS) { // (the same number of steps in every lane; beyond the rank zeros count)
+            v8h w[STEPS][4], t[STEPS][4];
+#pragma unroll
+            for (int i = 0; i < STEPS; i++) {
+                const uint32_t r = r0 + 32 * i + 8 * q;
+#pragma unroll
+                for (int o = 0; o < 4; o++) w[i][o] = *reinterpret_cast<const v8h *>(rows + (size_t)o * 16 * R + (r < R ? r : 0));
+#pragma unroll
+                for (int s = 0; s < 4; s++) t[i][s] = *reinterpret_cast<const v8h *>(trow[s] + (r < Rp ? r : 0));
+            }
+#pragma unroll
+            for (int i = 0; i < STEPS; i++) {
+                if (r0 + 32 * i + 8 * q >= R)
+#pragma unroll
+                    for (int o = 0; o < 4; o++) w[i][o] = t[i][o] = (v8h)(half_t)0.f;
+#pragma unroll
+                for (int s = 0; s < 4; s++)
+#pragma unroll
+                    for (int o = 0; o < 4; o++) acc[s][o] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[i][o], t[i][s], acc[s][o], 0, 0, 0);
             }
         }
 #pragma unroll
-        for (int o = 0; o < 4; o++) out[o] = mine == a ? acc[o] : out[o]; // (not a sum: another adapter's infinities stay out)
-        firsts &= firsts - 1;
-    }
-    if (mine >= 0) {
+        for (int h = 0; h < 2; h++) {
+            v8h yv[4];
 #pragma unroll
-        for (int o = 0; o < 4; o++) {
-            half_t   *p = y + (size_t)n * M + m0 + o * 16 + 4 * q;
-            const v4h v = *reinterpret_cast<const v4h *>(p);
-            v4h       w;
+            for (int j = 0; j < 4; j++) yv[j] = *reinterpret_cast<const v8h *>(yp(4 * h + j));
 #pragma unroll
-            for (int i = 0; i < 4; i++) w[i] = (half_t)((float)v[i] + f * out[o][i]);
-            *reinterpret_cast<v4h *>(p) = w;
+            for (int s = 0; s < 2; s++)
+#pragma unroll
+                for (int o = 0; o < 4; o++) *reinterpret_cast<v4f *>(lds + (16 * s + col) * kExpandRow + (wave * 64 + o * 16 + 4 * q) * 4) = acc[2 * h + s][o] * f[2 * h + s];
+            __syncthreads();
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const int row = (tid >> 5) + 8 * j;
+                if (same >> (32 * h + row) & 1) {
+                    const v4f lo = *reinterpret_cast<const v4f *>(lds + row * kExpandRow + (tid & 31) * 32), hi = *reinterpret_cast<const v4f *>(lds + row * kExpandRow + (tid & 31) * 32 + 16);
+                    v8h       out;
+#pragma unroll
+                    for (int i = 0; i < 8; i++) out[i] = (half_t)((float)yv[j][i] + (i < 4 ? lo[i & 3] : hi[i & 3]));
+                    *reinterpret_cast<v8h *>(yp(4 * h + j)) = out;
+                }
+            }
+            __syncthreads();
         }
-    }
+    });
 }
 
-// K ranges of the shrink: as many workgroups as fill the chip twice, each with 256 columns at least
-inline uint32_t shrink_ranges(size_t N, size_t K)
+// How an adapter call is cut: tiles of 64 rows where there are many, K ranges of 256 columns at least that fill the chip, and passes of a tile side by side as far as that leaves
+// no crowd of workgroups that find nothing to do (a round of them takes 2 us).
+struct AdapterPlan { uint32_t rows, tiles, ranges, shrink_side, expand_side; };
+inline AdapterPlan adapter_plan(size_t M, size_t N, size_t K, size_t slots)
 {
-    const size_t tiles = (N + 15) / 16, most = K / 256 > 0 ? K / 256 : 1;
-    const size_t want = tiles >= 512 ? 1 : (512 + tiles - 1) / tiles;
-    return (uint32_t)(want < most ? want : most);
+    AdapterPlan p;
+    p.rows = N > 256 ? 64 : 16;
+    p.tiles = (uint32_t)((N + p.rows - 1) / p.rows);
+    const size_t fill = 512, most = K / 256 > 0 ? K / 256 : 1, want = (fill + p.tiles - 1) / p.tiles;
+    p.ranges = (uint32_t)(want < most ? want : most);
+    const size_t rows = N < p.rows ? N : p.rows, passes = rows < slots ? rows : slots;
+    auto         side = [&](size_t workgroups, size_t room) { return (uint32_t)(workgroups * passes <= room ? passes : workgroups < room ? room / workgroups : 1); };
+    p.shrink_side = side((size_t)p.tiles * p.ranges, 2048);
+    p.expand_side = side(p.tiles * (M / 256), 4096);
+    return p;
 }
 inline size_t round16(size_t bytes) { return (bytes + 15) & ~(size_t)15; }
-
-int shrink(hipStream_t st, float *part, const void *x, const void *A, const int *index, size_t N, size_t K, size_t R, size_t slots, uint32_t ranges)
+// workspace, the same for any number of slots: the ranges' sums, then (tiles of 64 rows) the ranks in fp16 and the rows' factors, then the layer's own
+struct AdapterSpace { size_t part, ranks, factors, total; };
+inline AdapterSpace adapter_space(const AdapterPlan &p, size_t N, size_t R)
 {
-    const uint32_t tiles = (uint32_t)((N + 15) / 16), side = tiles >= 64 ? 1 : (uint32_t)(N < 16 ? N : 16);
-    const dim3     grid(tiles, ranges, side < slots ? side : (uint32_t)slots);
-    auto           go = [&](auto rt_c) {
-        hipLaunchKernelGGL((adapter_shrink<decltype(rt_c)::value>), grid, dim3(256), 0, st, part, static_cast<const half_t *>(x), static_cast<const half_t *>(A), index, (uint32_t)N, (uint32_t)K,
-                           (uint32_t)R, (uint32_t)slots);
+    AdapterSpace s;
+    s.part = 0;
+    s.ranks = round16((size_t)p.ranges * N * R * sizeof(float));
+    s.factors = s.ranks + (p.rows == 64 ? round16(N * ((R + 31) / 32 * 32) * 2) : 0);
+    s.total = s.factors + (p.rows == 64 ? round16(N * sizeof(float)) : 0);
+    return s;
+}
+
+int adapter_ranks_of(hipStream_t st, const AdapterPlan &p, float *part, const void *x, const void *A, const int *index, size_t N, size_t K, size_t R, size_t slots)
+{
+    auto go = [&](auto rt_c) {
+        constexpr int RT = decltype(rt_c)::value;
+        hipLaunchKernelGGL(p.rows == 64 ? adapter_shrink_tile<RT> : adapter_shrink<RT>, dim3(p.tiles, p.ranges, p.shrink_side), dim3(256), 0, st, part, static_cast<const half_t *>(x),
+                           static_cast<const half_t *>(A), index, (uint32_t)N, (uint32_t)K, (uint32_t)R, (uint32_t)slots);
         return (int)hipGetLastError();
     };
-    if (R <= 16) return go(std::integral_constant<int, 1>{});
-    if (R <= 32) return go(std::integral_constant<int, 2>{});
-    if (R <= 64) return go(std::integral_constant<int, 4>{});
-    if (R <= 128) return go(std::integral_constant<int, 8>{});
-    return go(std::integral_constant<int, 16>{});
+    return R <= 16 ? go(std::integral_constant<int, 1>{}) : R <= 32 ? go(std::integral_constant<int, 2>{}) : go(std::integral_constant<int, 4>{});
+}
+int adapter_expand_of(hipStream_t st, const AdapterPlan &p, void *y, const float *part, const half_t *ranks, const float *factors, const void *B, const float *scaling, const int *index, size_t M,
+                      size_t N, size_t R, size_t slots)
+{
+    const dim3 grid(p.tiles, (uint32_t)(M / 256), p.expand_side);
+    if (p.rows == 64) {
+        hipLaunchKernelGGL(R <= 32 ? adapter_expand_tile<1> : adapter_expand_tile<2>, grid, dim3(256), 0, st, static_cast<half_t *>(y), ranks, factors, static_cast<const half_t *>(B), index, (uint32_t)M, (uint32_t)N,
+                           (uint32_t)R, (uint32_t)slots);
+    } else {
+        hipLaunchKernelGGL(adapter_expand, grid, dim3(256), 0, st, static_cast<half_t *>(y), part, static_cast<const half_t *>(B), scaling, index, (uint32_t)M, (uint32_t)N, (uint32_t)R,
+                           (uint32_t)slots, p.ranges);
+    }
+    return (int)hipGetLastError();
 }
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -417,7 +674,7 @@ int fp6mi_gated_backward_native(int E, int Mb, void *stream, const void *W, cons
 
 size_t fp6mi_adapter_workspace_bytes(size_t M, size_t N, size_t K, size_t R, int splitK)
 {
-    return round16(shrink_ranges(N, K) * N * R * sizeof(float)) + fp6mi_workspace_bytes(M, N, splitK);
+    return N == 0 ? 0 : adapter_space(adapter_plan(M, N, K, 1), N, R).total + fp6mi_workspace_bytes(M, N, splitK);
 }
 
 int fp6mi_adapter_native(int E, int Mb, void *stream, const void *W, const void *sc, const void *group_exps, const void *bias, const void *B, void *C, const void *lora_a, const void *lora_b,
@@ -428,15 +685,21 @@ int fp6mi_adapter_native(int E, int Mb, void *stream, const void *W, const void 
     if (!lora_a || !lora_b || !scaling || !index) return FP6MI_ERR_NULL;
     if (!ws) return FP6MI_ERR_WORKSPACE;
     if (R == 0 || R % 8 || R > 256 || slots == 0 || slots > 0x7fffffffu) return FP6MI_ERR_SHAPE;
+    if (M / 256 > 65535) return FP6MI_ERR_SHAPE; // (a grid dimension)
     if (!aligned16(lora_a) || !aligned16(lora_b) || (reinterpret_cast<uintptr_t>(scaling) & 3u) || (reinterpret_cast<uintptr_t>(index) & 3u)) return FP6MI_ERR_ALIGN;
-    hipStream_t    st = static_cast<hipStream_t>(stream);
-    const uint32_t ranges = shrink_ranges(N, K);
-    float         *base_ws = ws + round16(ranges * N * R * sizeof(float)) / sizeof(float);
-    if (const int e = shrink(st, ws, B, lora_a, index, N, K, R, slots, ranges)) return e;
-    if (const int e = fp6mi::run_linear(E, Mb, stream, W, sc, group_exps, bias, B, C, M, N, K, splitK > 1 ? base_ws : nullptr, splitK, false)) return e;
-    hipLaunchKernelGGL(adapter_expand, dim3((uint32_t)((N + 15) / 16), (uint32_t)(M / 256)), dim3(256), 0, st, static_cast<half_t *>(C), ws, static_cast<const half_t *>(lora_b), scaling, index,
-                       (uint32_t)M, (uint32_t)N, (uint32_t)R, (uint32_t)slots, ranges);
-    return (int)hipGetLastError();
+    hipStream_t        st = static_cast<hipStream_t>(stream);
+    const AdapterPlan  p = adapter_plan(M, N, K, slots);
+    const AdapterSpace s = adapter_space(p, N, R);
+    uint8_t           *base = reinterpret_cast<uint8_t *>(ws);
+    half_t            *ranks = reinterpret_cast<half_t *>(base + s.ranks);
+    float             *factors = reinterpret_cast<float *>(base + s.factors);
+    if (const int e = adapter_ranks_of(st, p, ws, B, lora_a, index, N, K, R, slots)) return e;
+    if (p.rows == 64) {
+        hipLaunchKernelGGL(adapter_ranks, dim3((uint32_t)((N + 3) / 4)), dim3(256), 0, st, ranks, factors, ws, scaling, index, (uint32_t)N, (uint32_t)R, (uint32_t)slots, p.ranges);
+        if (const hipError_t e = hipGetLastError()) return (int)e;
+    }
+    if (const int e = fp6mi::run_linear(E, Mb, stream, W, sc, group_exps, bias, B, C, M, N, K, splitK > 1 ? reinterpret_cast<float *>(base + s.total) : nullptr, splitK, false)) return e;
+    return adapter_expand_of(st, p, C, ws, ranks, factors, lora_b, scaling, index, M, N, R, slots);
 }
 
 } // extern "C"

@@ -261,7 +261,8 @@ def adapters64(w, x, bias, a, b, s, index):
 
 
 ADAPTERS = [(3, 2, 256, 64, 1, 8, 1, False), (2, 2, 512, 320, 2, 16, 3, True), (2, 1, 256, 1024, 9, 24, 5, False), (2, 3, 768, 576, 16, 64, 40, True), (3, 2, 512, 512, 17, 40, 3, False),
-            (3, 2, 1024, 256, 50, 128, 4, True), (2, 2, 512, 832, 130, 256, 2, False), (2, 1, 768, 448, 300, 32, 7, True), (2, 3, 256, 1344, 1200, 72, 3, False)]
+            (3, 2, 1024, 256, 50, 128, 4, True), (2, 2, 512, 832, 130, 256, 2, False), (2, 1, 768, 448, 300, 32, 7, True), (2, 3, 256, 1344, 1200, 72, 3, False), (3, 2, 512, 256, 257, 8, 300, False),
+            (2, 2, 256, 576, 700, 200, 90, True)]
 
 
 @gpu
