@@ -36,7 +36,7 @@ if os.path.exists(_lib.LIB_PATH) and not os.environ.get("FP6MI_NO_TORCH_EXT"):
     try:
         _lib.lib()
         from . import _fp6mi_torch as _ext
-        if "bias" not in (_ext.linear_forward_native.__doc__ or "") or not hasattr(_ext, "adapter_forward"):   # the newest of the names and arguments used below
+        if "bias" not in (_ext.linear_forward_native.__doc__ or "") or not hasattr(_ext, "gradient_goes_elsewhere"):   # the newest of the names and arguments used below
             raise ImportError("the extension was built from an older tree")
     except (ImportError, OSError, AttributeError):   # extension not built or stale, or a stale library: the ctypes path reports what is wrong
         _ext = None

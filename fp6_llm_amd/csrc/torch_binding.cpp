@@ -14,7 +14,9 @@
 #include <map>
 #include <mutex>
 #include <string>
+#include <unordered_set>
 #include <utility>
+#include <vector>
 
 #include "fp6mi.h"
 #include "fp6_linear_torch.h"
@@ -563,6 +565,27 @@ at::Tensor adapter_forward(int64_t E, int64_t Mb, const at::Tensor &in_feats, co
                  "fp6mi_adapter_native");
     return out;
 }
+
+// Whether a backward pass from t would reach a node that runs on another stream of t's device than the current one: one that an eager graph made, a leaf's own (of an eager graph that
+// still lives) among them.
+bool gradient_goes_elsewhere(const at::Tensor &t)
+{
+    const c10::Stream                            here = c10::hip::getCurrentHIPStream(t.device().index()).unwrap();
+    std::vector<torch::autograd::Node *>         todo;
+    std::unordered_set<torch::autograd::Node *>  seen;
+    std::shared_ptr<torch::autograd::Node>       first = t.grad_fn();
+    if (!first) first = torch::autograd::impl::try_get_grad_accumulator(t);
+    if (first) todo.push_back(first.get());
+    while (!todo.empty()) {
+        torch::autograd::Node *node = todo.back();
+        todo.pop_back();
+        if (!node || !seen.insert(node).second) continue;
+        const auto stream = node->stream();
+        if (stream.has_value() && stream->device_index() == here.device_index() && stream->id() != here.id()) return true;
+        for (const auto &edge : node->next_edges()) todo.push_back(edge.function.get());
+    }
+    return false;
+}
 } // namespace
 
 PYBIND11_MODULE(_fp6mi_torch, m)
@@ -584,6 +607,7 @@ PYBIND11_MODULE(_fp6mi_torch, m)
     m.def("gated_backward", &gated_backward);
     m.def("linear_input_grad", &linear_input_grad);
     m.def("adapter_forward", &adapter_forward);
+    m.def("gradient_goes_elsewhere", &gradient_goes_elsewhere);
     // the reference's bindings, name for name (fp6_llm/csrc/pybind.cpp:8-15)
     m.def("linear_forward_cuda", &fp6_linear_forward_cuda, "Computes FP6-FP16 GEMM.", pybind11::arg("in_feats"), pybind11::arg("weights"),
           pybind11::arg("scales"), pybind11::arg("splitK") = 1);

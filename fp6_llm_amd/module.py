@@ -9,6 +9,7 @@ import torch
 from . import quant
 from . import (MI355X_CUS, group_exps_bytes, heuristic_splitk_mi355x, linear_forward_native, native_bytes, pack_group_exps, to_native,
                weight_dequant_native_cuda, weight_prepacking_native_cpu, weight_quantize_native_cuda)
+from . import ops
 
 _MAGIC = b"FP6MI\x00\x01\x00"   # name, NUL, layout version 1, reserved
 
@@ -30,12 +31,66 @@ class _AutoRows(int):
     pickled whole hold one.)"""
 
 
+def _differentiates(x):
+    """Whether a gradient is to reach x.  A backward pass that is captured must stay on its stream: where x, or a leaf that it was computed from, is also part of an eager graph that
+    still lives, its gradient is added up on that graph's stream, and a capture that goes there ends the process.  A call that would begin one is refused."""
+    if not (x.requires_grad and torch.is_grad_enabled()):
+        return False
+    if x.device.type == "cuda" and torch.cuda.is_current_stream_capturing() and ops.gradient_goes_elsewhere(x):
+        raise RuntimeError("the gradient of this input would leave the stream that is being captured: drop what an eager graph holds of it, or capture a detached copy that requires it")
+    return True
+
+
+def _rows_of(x, features):
+    """x[..., features] as float16 rows."""
+    if x.dim() < 1 or x.shape[-1] != features:
+        raise ValueError("need an input of %d features, got %s" % (features, list(x.shape)))
+    x2 = x.reshape(-1, features)
+    return x2 if x2.dtype == torch.float16 else x2.half()
+
+
+class _InputGradient(torch.autograd.Function):
+    """FPxLinear.forward, and the product with the weights the other way round.  What a backward pass needs is the weights alone."""
+
+    @staticmethod
+    def forward(ctx, x, layer):
+        ctx.save_for_backward(layer.weight_native, layer.scales, layer.group_exps)
+        ctx.format, ctx.in_features = (layer.exponent, layer.mantissa), layer.in_features
+        return FPxLinear.forward(layer, x)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        weight, scales, exps = ctx.saved_tensors
+        return ops.linear_input_grad_native(*ctx.format, grad.half(), weight, scales, ctx.in_features, group_exps=exps), None
+
+
+class _GatedBlock(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, block):
+        preact = torch.empty(x.shape[0], 2 * block.out_features, dtype=torch.float32, device=x.device)
+        y = block._values(x, preact)
+        ctx.save_for_backward(preact, block.weight_native, block.scales, block.group_exps)
+        ctx.format, ctx.in_features, ctx.activation = (block.exponent, block.mantissa), block.in_features, block.activation
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        preact, weight, scales, exps = ctx.saved_tensors
+        return ops.gated_backward_native(*ctx.format, grad, preact, weight, scales, ctx.in_features, ctx.activation, grad_preact=False, group_exps=exps)[0], None
+
+
 _CROSSOVER, _CROSSOVER_LIBRARY = 32768, 3072   # FPxLinear.PREFILL_CROSSOVER as it is shipped, and the one without the wide tiles
 
 
 class FPxLinear(torch.nn.Module):
     """y = x @ dequant(W)^T (+ bias) with W held in the native gfx950 layout.  Weights are buffers, not parameters:
-    the layer is inference-only, like the kernels."""
+    the layer is inference-only, like the kernels, but for input_gradient."""
+
+    # True: an input that requires a gradient gets one, through the quantized weights (a frozen layer under trained adapters, prompts or layers below it).  Weights and bias have
+    # none.  False, as it has always been: the kernels are no part of an autograd graph.
+    input_gradient = False
 
     # Batch size from which dequantize + FP16 library GEMM is no slower than the mixed-input kernels, measured through this module at 4096^2, 8192^2, 28672x8192,
     # 8192x28672, 11008x4096, 1024x8192, 1024^2, 4608x4544 and 2560x18944, FP6 with row scales and FP5 with group exponents.  Kernel time / time of dequantization +
@@ -184,13 +239,35 @@ class FPxLinear(torch.nn.Module):
         return (self._wide_tiles(x2.device) and _values_only(x2) and (not torch.is_autocast_enabled(kind) or torch.get_autocast_dtype(kind) == torch.float16)
                 and (not x2.is_contiguous() or x2.data_ptr() % 16 == 0))
 
-    def forward(self, x):
+    def _with_adapters(self, x, adapters, index):
+        if not isinstance(adapters, LowRankAdapters) or index is None:
+            raise ValueError("adapters must be a LowRankAdapters, with an index for every row")
+        if (adapters.in_features, adapters.out_features) != (self.in_features, self.out_features):
+            raise ValueError("the adapters are for %d -> %d features, the layer has %d -> %d" % (adapters.in_features, adapters.out_features, self.in_features, self.out_features))
+        if torch.is_grad_enabled() and (x.requires_grad or (self.bias is not None and self.bias.requires_grad)):
+            raise ValueError("a product with adapters has no gradient: call it under torch.no_grad()")
+        x2 = _rows_of(x, self.in_features)
+        if index.numel() != x2.shape[0] or (index.dim() != 1 and index.shape != x.shape[:-1]):
+            raise ValueError("index must name an adapter for each of the %d rows, got %s" % (x2.shape[0], list(index.shape)))
+        y = ops.adapter_forward_native(self.exponent, self.mantissa, x2, self.weight_native, self.scales, self.out_features, adapters.lora_a, adapters.lora_b, adapters.scaling,
+                                       index.reshape(-1), None, group_exps=self.group_exps, bias=self.bias)
+        return y.reshape(*x.shape[:-1], self.out_features)
+
+    def forward(self, x, adapters=None, index=None):
+        """adapters: a LowRankAdapters of this layer's shape, with index, int32, the slot of every row of x (-1: none)."""
+        if adapters is not None or index is not None:
+            return self._with_adapters(x, adapters, index)
         # (two reshapes to the shapes at hand take 0.7 us each; a trace, whose sizes are no plain numbers, keeps them)
         shape = x.shape
         plain = type(x) is torch.Tensor and len(shape) == 2 and type(shape[1]) is int and shape[1] == self.in_features
         x2 = x if plain else x.reshape(-1, self.in_features)
         if x2.dtype != torch.float16:
             x2 = x2.half()
+        if self.input_gradient and _differentiates(x):
+            if self.bias is not None and self.bias.requires_grad:
+                raise ValueError("input_gradient is for a layer whose bias requires no gradient")
+            y = _InputGradient.apply(x2, self)
+            return y if plain else y.reshape(*shape[:-1], self.out_features)
         rows, n = self._rows, x2.shape[0]
         if rows is not None and (n >= rows or (self._auto and n >= _CROSSOVER_LIBRARY and not self._kernels_take(x2))):
             w16 = weight_dequant_native_cuda(self.exponent, self.mantissa, self.weight_native, self.scales, self.out_features, self.in_features,
@@ -215,6 +292,108 @@ class FPxLinear(torch.nn.Module):
 
     def extra_repr(self):
         return "in_features=%d, out_features=%d, format=e%dm%d" % (self.in_features, self.out_features, self.exponent, self.mantissa)
+
+
+class FPxGatedLinear(torch.nn.Module):
+    """y = act(x @ gate^T + bias_g) * (x @ up^T + bias_u): the first half of a gated feed-forward block in one launch, on native-layout weights that hold both matrices in pair order
+    (ops.gate_up_pairs).  Differentiable in x; the weights are buffers and have no gradient."""
+
+    def __init__(self, in_features, out_features, exponent=3, mantissa=2, activation="silu", bias=None, split_k=None, group_scales=False):
+        """out_features: columns of y, the rows of gate and of up.  activation: "silu", "gelu" or "gelu_tanh".  bias: float16 [2 * out_features] in pair order."""
+        super().__init__()
+        if out_features < 128 or out_features % 128 or in_features < 64 or in_features % 64:
+            raise ValueError("FPxGatedLinear needs out_features %% 128 == 0 and in_features %% 64 == 0")
+        ops._activation_code(activation)
+        self.in_features, self.out_features, self.exponent, self.mantissa = in_features, out_features, exponent, mantissa
+        self.activation, self.split_k = activation, split_k
+        self.register_buffer("weight_native", torch.zeros(native_bytes(exponent, mantissa, 2 * out_features, in_features) // 4, dtype=torch.int32))
+        self.register_buffer("scales", torch.ones(2 * out_features, dtype=torch.float16))
+        self.register_buffer("bias", bias)
+        self.register_buffer("group_exps", torch.full((group_exps_bytes(2 * out_features, in_features),), 127, dtype=torch.uint8) if group_scales else None)
+
+    @classmethod
+    def from_layers(cls, gate, up, activation="silu", split_k=None):
+        """From two FPxLinear of one shape and format: their bytes, in pair order."""
+        for name in ("in_features", "out_features", "exponent", "mantissa"):
+            if getattr(gate, name) != getattr(up, name):
+                raise ValueError("gate and up must have the same %s" % name)
+        for name in ("bias", "group_exps"):
+            if (getattr(gate, name) is None) != (getattr(up, name) is None):
+                raise ValueError("gate and up must both have %s or both have none" % name)
+        F = gate.out_features
+        m = cls(gate.in_features, F, gate.exponent, gate.mantissa, activation, None if gate.bias is None else ops.gate_up_pairs(gate.bias, up.bias), split_k)
+        m = m.to(gate.weight_native.device)
+        m.weight_native = ops.gate_up_pairs(gate.weight_native, up.weight_native, rows=F)
+        m.scales = ops.gate_up_pairs(gate.scales, up.scales)
+        if gate.group_exps is not None:
+            m.group_exps = ops.gate_up_pairs(gate.group_exps, up.group_exps, rows=F)
+        return m
+
+    @classmethod
+    def from_float(cls, gate, up, exponent=3, mantissa=2, activation="silu", bias=None, split_k=None, group_scales=False):
+        """From two float [out_features, in_features] weights, quantized as FPxLinear.from_float does.  bias: (of gate, of up), float16."""
+        both = FPxLinear.from_float(ops.gate_up_pairs(gate.detach(), up.detach()), exponent, mantissa, group_scales=group_scales)
+        m = cls(gate.shape[1], gate.shape[0], exponent, mantissa, activation, None if bias is None else ops.gate_up_pairs(*bias), split_k).to(gate.device)
+        m.weight_native, m.scales, m.group_exps = both.weight_native, both.scales, both.group_exps
+        return m
+
+    def _values(self, x2, preact=None):
+        return ops.gated_forward_native(self.exponent, self.mantissa, x2, self.weight_native, self.scales, 2 * self.out_features, self.activation, self.split_k, preact=preact,
+                                        group_exps=self.group_exps, bias=self.bias)
+
+    def forward(self, x):
+        x2 = _rows_of(x, self.in_features)
+        if self.bias is not None and self.bias.requires_grad and torch.is_grad_enabled():
+            raise ValueError("the bias of FPxGatedLinear has no gradient")
+        y = _GatedBlock.apply(x2, self) if _differentiates(x) else self._values(x2)
+        return y if x.dim() == 2 else y.reshape(*x.shape[:-1], self.out_features)
+
+    def extra_repr(self):
+        return "in_features=%d, out_features=%d, format=e%dm%d, activation=%s" % (self.in_features, self.out_features, self.exponent, self.mantissa, self.activation)
+
+
+class LowRankAdapters(torch.nn.Module):
+    """Slots for the low-rank adapters of many requests to one FPxLinear: layer(x, adapters, index) adds scaling * (x @ a^T) @ b^T to every row, with the a, b and scaling of the slot
+    that the row's index names.  Buffers of fixed size, so a captured graph sees what set() and clear() write between its replays."""
+
+    def __init__(self, in_features, out_features, slots, rank):
+        """rank: the largest of any slot, up to 256; smaller ones are held with rows of zeros."""
+        super().__init__()
+        if out_features % 256 or in_features % 64:
+            raise ValueError("LowRankAdapters needs out_features %% 256 == 0 and in_features %% 64 == 0")
+        if slots < 1 or not 1 <= rank <= ops.MAX_RANK:
+            raise ValueError("LowRankAdapters needs a slot at least, and a rank from 1 to %d" % ops.MAX_RANK)
+        self.in_features, self.out_features, self.slots, self.rank = in_features, out_features, slots, (rank + 7) // 8 * 8
+        self.register_buffer("lora_a", torch.zeros(slots, self.rank, in_features, dtype=torch.float16))
+        self.register_buffer("lora_b", torch.zeros(slots, out_features, self.rank, dtype=torch.float16))
+        self.register_buffer("scaling", torch.zeros(slots, dtype=torch.float32))
+
+    @torch.no_grad()
+    def set(self, slot, a, b, scaling=1.0):
+        """a: [r, in_features], b: [out_features, r], r up to the rank.  For a fused layer lists of them, a pair for each part: their ranks add up, and a part's a reaches only its outputs."""
+        if isinstance(a, (list, tuple)):
+            if not a or len(a) != len(b) or any(p.dim() != 2 or q.dim() != 2 or p.shape[0] != q.shape[1] for p, q in zip(a, b)):
+                raise ValueError("need an a [r, in_features] and a b [outputs, r] for each part")
+            a, b = torch.cat(list(a)), torch.block_diag(*b)
+        if not 0 <= slot < self.slots:
+            raise ValueError("no slot %d among %d" % (slot, self.slots))
+        r = a.shape[0]
+        if a.shape != (r, self.in_features) or b.shape != (self.out_features, r) or r > self.rank:
+            raise ValueError("need a [r, %d] and b [%d, r] with r up to %d, got %s and %s" % (self.in_features, self.out_features, self.rank, list(a.shape), list(b.shape)))
+        self.clear(slot)
+        self.lora_a[slot, :r].copy_(a)
+        self.lora_b[slot, :, :r].copy_(b)
+        self.scaling[slot] = scaling
+
+    @torch.no_grad()
+    def clear(self, slot):
+        """Rows that name this slot are as without an adapter."""
+        if not 0 <= slot < self.slots:
+            raise ValueError("no slot %d among %d" % (slot, self.slots))
+        self.lora_a[slot].zero_(), self.lora_b[slot].zero_(), self.scaling[slot].zero_()
+
+    def extra_repr(self):
+        return "in_features=%d, out_features=%d, slots=%d, rank=%d" % (self.in_features, self.out_features, self.slots, self.rank)
 
 
 def save_native(path, native_int32, scales, exponent, mantissa, out_features, in_features, group_exps=None):

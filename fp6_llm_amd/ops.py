@@ -27,6 +27,13 @@ def gate_up_pairs(gate, up, rows=None):
     return pairs.reshape((2 * gate.shape[0],) + tuple(gate.shape[1:]))
 
 
+def gradient_goes_elsewhere(t):
+    """Whether a backward pass from t would reach a node that runs on another stream than the current one: of a graph that was made on that stream, a leaf's own node among them while
+    such a graph lives.  (Without the extension, which can ask, nothing is known and the answer is True.)"""
+    from . import _ext
+    return _ext.gradient_goes_elsewhere(t) if _ext is not None else True
+
+
 def _check_weights(E, M, native_weight, scales, OC, IC, group_exps, dev):
     from . import _BLOCK_BYTES, _bits, _check_group_exps
     bits = _bits(E, M)

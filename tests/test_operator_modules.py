@@ -1,0 +1,269 @@
+"""The modules over the operators around the linear layer: FPxGatedLinear, LowRankAdapters, and FPxLinear with an input gradient.  Tolerances are counted as in test_operators.py."""
+import pytest
+import torch
+
+import fp6_llm_amd as fp6
+from fp6_llm_amd.module import FPxGatedLinear, FPxLinear, LowRankAdapters
+from test_operators import DEV, HALF, TINY, Weight, adapters64, d, gated64, gpu, halves, pairs, preacts, randn, slope64, act64, sum_error, within
+
+
+def layer(w, bias=None):
+    m = FPxLinear(w.IC, w.OC, w.E, w.M, bias, group_scales=w.exps is not None).to(DEV)
+    m.weight_native.copy_(w.native)
+    m.scales.copy_(w.scales)
+    if w.exps is not None:
+        m.group_exps.copy_(w.exps)
+    return m
+
+
+def block(w, act="silu", bias=None):
+    m = FPxGatedLinear(w.IC, w.OC // 2, w.E, w.M, act, bias, group_scales=w.exps is not None).to(DEV)
+    m.weight_native.copy_(w.native)
+    m.scales.copy_(w.scales)
+    if w.exps is not None:
+        m.group_exps.copy_(w.exps)
+    return m
+
+
+@pytest.mark.parametrize("groups", [False, True])
+def test_gated_block_from_two_layers_holds_their_rows_in_pairs(groups):
+    g = torch.Generator().manual_seed(1)
+    gate, up = (torch.randn(256, 192, generator=g) for _ in range(2))
+    biases = [torch.randn(256, generator=g).half() for _ in range(2)]
+    both = FPxLinear.from_float(fp6.gate_up_pairs(gate, up), 2, 2, group_scales=groups)
+    a = FPxGatedLinear.from_layers(*(FPxLinear.from_float(t, 2, 2, b, group_scales=groups) for t, b in zip((gate, up), biases)), activation="gelu")
+    b = FPxGatedLinear.from_float(gate, up, 2, 2, "gelu", biases, group_scales=groups)
+    for m in (a, b):
+        assert (m.in_features, m.out_features, m.activation) == (192, 256, "gelu")
+        assert torch.equal(m.weight_native, both.weight_native) and torch.equal(m.scales, both.scales) and torch.equal(m.bias, fp6.gate_up_pairs(*biases))
+        assert (m.group_exps is None) == (not groups) and (not groups or torch.equal(m.group_exps, both.group_exps))
+    b.load_state_dict(a.state_dict())
+    assert set(a.state_dict()) == {"weight_native", "scales", "bias"} | ({"group_exps"} if groups else set()) and not list(a.parameters())
+
+
+def test_refusals_of_the_modules():
+    lin = lambda i=64, o=256, **kw: FPxLinear(i, o, **kw)   # noqa: E731
+    for pair in ((lin(), lin(o=512)), (lin(), lin(i=128)), (lin(), lin(exponent=2)), (lin(), lin(bias=torch.zeros(256).half())), (lin(group_scales=True), lin())):
+        with pytest.raises(ValueError):
+            FPxGatedLinear.from_layers(*pair)
+    for args in ((64, 64), (32, 128), (64, 0), (64, 128, 3, 2, "relu")):
+        with pytest.raises(ValueError):
+            FPxGatedLinear(*args)
+    for args in ((64, 128, 1, 8), (32, 256, 1, 8), (64, 256, 0, 8), (64, 256, 1, 0), (64, 256, 1, 257)):
+        with pytest.raises(ValueError):
+            LowRankAdapters(*args)
+    ad = LowRankAdapters(64, 256, 3, 12)
+    assert ad.rank == 16
+    a, b = torch.randn(12, 64), torch.randn(256, 12)
+    for args in ((3, a, b), (-1, a, b), (0, a[:, :32], b), (0, a, b[:128]), (0, a[:8], b), (0, torch.randn(17, 64), torch.randn(256, 17)), (0, [a], [b, b]), (0, [], []), (0, [a, a], [b[:100], b[100:, :8]])):
+        with pytest.raises(ValueError):
+            ad.set(*args)
+    with pytest.raises(ValueError):
+        ad.clear(3)
+    assert not ad.lora_a.any() and not ad.scaling.any()
+    m, x, idx = lin(), torch.zeros(2, 64).half(), torch.zeros(2, dtype=torch.int32)
+    for args in ((x, ad), (x, None, idx), (x, lin(), idx), (x, LowRankAdapters(128, 256, 1, 8), idx), (x, ad, idx[:1]), (x, ad, idx.reshape(1, 2)), (x.reshape(1, 2, 64), ad, idx.reshape(2, 1)),
+                 (x[:, :32], ad, idx), (x.clone().requires_grad_(), ad, idx)):
+        with pytest.raises(ValueError):
+            m(*args)
+    with pytest.raises(ValueError):
+        FPxGatedLinear(64, 128)(torch.zeros(2, 128).half())   # (128 features would also be twice as many rows)
+    biased = FPxGatedLinear(64, 128, bias=torch.zeros(256).half().requires_grad_())
+    with pytest.raises(ValueError):
+        biased(x)
+
+
+def test_adapters_of_a_fused_layer_reach_their_parts():
+    g = torch.Generator().manual_seed(2)
+    ad = LowRankAdapters(64, 768, 2, 16)
+    parts = [(torch.randn(r, 64, generator=g).half(), torch.randn(256, r, generator=g).half()) for r in (4, 2, 8)]
+    ad.set(1, torch.ones(16, 64), torch.ones(768, 16), 3.0)
+    ad.set(1, [a for a, _ in parts], [b for _, b in parts], 0.5)
+    want = torch.cat([b.double() @ a.double() for a, b in parts])
+    assert torch.equal(ad.lora_b[1].double() @ ad.lora_a[1].double(), want) and ad.scaling.tolist() == [0.0, 0.5]
+    ad.clear(1)
+    assert not ad.lora_a.any() and not ad.lora_b.any() and not ad.scaling.any()
+
+
+@gpu
+@pytest.mark.parametrize("N,act", [(1, "silu"), (23, "gelu"), (300, "gelu_tanh")])
+def test_gated_module_is_its_function_and_differentiable(N, act):
+    w, b = Weight(N, 2, 2, 512, 320, True), randn(1, 512, scale=0.3)
+    m = block(w, act, b)
+    x, dh = randn(2, N, 320), randn(3, N, 256, scale=0.1)
+    pre = torch.empty(N, 512, device=DEV)
+    h = fp6.gated_forward_native(2, 2, x, w.native, w.scales, 512, act, preact=pre, group_exps=w.exps, bias=b)
+    dx = fp6.gated_backward_native(2, 2, dh, pre, w.native, w.scales, 320, act, group_exps=w.exps)[0]
+    assert torch.equal(m(x), h) and not m(x).requires_grad
+    leaf = x.clone().requires_grad_()
+    y = m(leaf)
+    assert torch.equal(y, h)
+    y.backward(dh)
+    assert torch.equal(leaf.grad, dx)
+    with torch.no_grad():
+        assert not m(leaf).requires_grad
+    # more dimensions, a float32 leaf (whose cast autograd differentiates), a gradient of stride zero
+    wide = x.float().reshape(1, N, 320).requires_grad_()
+    y = m(wide)
+    assert y.shape == (1, N, 256) and torch.equal(y.reshape(N, 256), h)
+    y.sum().backward()
+    ones = fp6.gated_backward_native(2, 2, torch.ones_like(dh), pre, w.native, w.scales, 320, act, group_exps=w.exps)[0]
+    assert wide.grad.dtype == torch.float32 and torch.equal(wide.grad.reshape(N, 320), ones.float())
+    # once only
+    y = m(leaf)
+    (g,) = torch.autograd.grad(y, leaf, dh.clone().requires_grad_(), create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(g.sum(), leaf)
+
+
+@gpu
+@pytest.mark.parametrize("N,dequant_above", [(1, "auto"), (40, "auto"), (200, None), (200, 100)])
+def test_input_gradient_of_the_linear_layer(N, dequant_above):
+    w, b = Weight(N, 3, 2, 768, 448), randn(1, 768)
+    m = layer(w, b)
+    m.dequant_above = dequant_above
+    x, dy = randn(2, N, 448), randn(3, N, 768)
+    want = m(x)
+    leaf = x.clone().requires_grad_()
+    if dequant_above != 100:   # (above it the library's product is differentiated, as it always was)
+        assert not m(leaf).requires_grad
+    m.input_gradient = True
+    y = m(leaf)
+    assert y.requires_grad and torch.equal(y, want) and not m(x).requires_grad
+    y.backward(dy)
+    assert torch.equal(leaf.grad, fp6.linear_input_grad_native(3, 2, dy, w.native, w.scales, 448))
+    # against a difference: the layer is linear, so <dy, m(x + v) - m(x)> is <dx, v> but for the roundings of the two outputs, of x + v and of dx
+    v = randn(4, N, 448)
+    xv = (x + v)
+    lhs = (d(dy) * (d(m(xv)) - d(want))).sum()
+    moved = d(xv) - d(x)
+    (y0, e0), (y1, e1) = preacts(w, x, b), preacts(w, xv, b)
+    base = 2 * HALF if dequant_above == 100 else 0   # (fp16 weights: value times scale is rounded once more; and a bias added to a rounded product)
+    mags = (d(x).abs() + d(xv).abs()) @ w.w.abs().t() + 2 * d(b).abs()
+    tol = (d(dy).abs() * (e0 + e1 + HALF * (y0.abs() + y1.abs()) * (1 + HALF) + 2 * TINY + base * mags)).sum()
+    mag = d(dy).abs() @ w.w.abs()
+    tol = tol + (moved.abs() * ((sum_error(768) + HALF) * mag + HALF * d(leaf.grad).abs() + 2 * TINY)).sum()
+    assert abs(lhs - (d(leaf.grad) * moved).sum()) <= tol
+    m.bias.requires_grad_()
+    with pytest.raises(ValueError):
+        m(leaf)
+
+
+@gpu
+@pytest.mark.parametrize("N", [3, 20, 300])
+def test_one_feed_forward_layer_as_it_is_trained_and_as_it_is_served(N):
+    """Queries, keys and values with a request's adapters, the gated block and the projection down with adapters; and the gradient through block and projection.  Every stage is held to
+    its formula in 64 bits on the values that went into it."""
+    H, F, slots = 512, 768, 4
+    qkv, gu, down = Weight(1, 3, 2, 3 * H, H), Weight(2, 2, 2, 2 * F, H, True), Weight(3, 3, 2, H, F)
+    mq, mg, md = layer(qkv), block(gu), layer(down)
+    ads, oad = LowRankAdapters(H, 3 * H, slots, 40).to(DEV), LowRankAdapters(F, H, slots, 8).to(DEV)
+    for i in range(3):
+        ads.set(i, [randn(10 * i + j, 8 * (i + 1) if j == 0 else 8, H, scale=H ** -0.5) for j in range(3)],
+                [randn(10 * i + j + 5, H, 8 * (i + 1) if j == 0 else 8, scale=0.2) for j in range(3)], 0.5 + i)
+        oad.set(i, randn(40 + i, 8, F, scale=F ** -0.5), randn(50 + i, H, 8, scale=0.2), 1.0)
+    index = (torch.arange(N, device=DEV) % 5 - 1).int()   # (-1: none; 3: a slot that nobody has set)
+    x = randn(4, N, H)
+    y = mq(x.reshape(1, N, H), ads, index.reshape(1, N)).reshape(N, 3 * H)
+    want, tol = adapters64(qkv, x, None, ads.lora_a, ads.lora_b, ads.scaling, index.cpu())
+    within(y, want, tol, "qkv")
+    hidden = y[:, 2 * H:]   # (strided: one part of a fused layer's output)
+    h = mg(hidden)
+    within(h, *gated64(gu, hidden, None, "silu")[2:], "block")
+    out = md(h, oad, index)
+    want, tol = adapters64(down, h, None, oad.lora_a, oad.lora_b, oad.scaling, index.cpu())
+    within(out, want, tol, "down")
+    assert torch.equal(out[index < 0], md(h)[index < 0])   # (the bits of the layer alone)
+
+    md.input_gradient = True
+    leaf, dy = hidden.detach().clone().requires_grad_(), randn(7, N, H, scale=0.1)
+    hh = mg(leaf)
+    hh.retain_grad()
+    md(hh).backward(dy)
+    mag = d(dy).abs() @ down.w.abs()
+    dh = d(dy) @ down.w
+    within(hh.grad, dh, (sum_error(H + 3) + HALF) * mag + TINY * down.w.abs().sum(0) + HALF * dh.abs() + TINY, "dh")
+    p, err = preacts(gu, hidden, None)
+    (g, u), (eg, eu), dd = halves(p), halves(err), d(hh.grad)
+    dp = pairs(dd * u * slope64("silu", g), dd * act64("silu", g))
+    ep = pairs(dd.abs() * (1.3 * eg * u.abs() + 1.13 * eu + 2.0 ** -17 * u.abs()), dd.abs() * (1.13 * eg + 2.0 ** -17 * g.abs())) + (HALF + sum_error(2 * F)) * dp.abs() + TINY
+    dx = dp @ gu.w
+    within(leaf.grad, dx, (ep @ gu.w.abs()) * (1 + HALF) + HALF * dx.abs() + TINY, "dx")
+
+
+@gpu
+def test_slots_written_between_the_replays_of_a_graph():
+    w = Weight(1, 3, 2, 512, 256)
+    m, ad = layer(w), LowRankAdapters(256, 512, 2, 16).to(DEV)
+    x, index = randn(1, 20, 256), (torch.arange(20, device=DEV) % 3 - 1).int()
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        m(x, ad, index)
+        stream.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            y = m(x, ad, index)
+        for i in range(3):
+            ad.set(i % 2, randn(i, 9, 256, scale=0.1), randn(i + 9, 512, 9), 0.5)
+            if i == 2:
+                ad.clear(1)
+            index.copy_(index.roll(1))
+            graph.replay()
+            assert torch.equal(y, m(x, ad, index))
+            want, tol = adapters64(w, x, None, ad.lora_a, ad.lora_b, ad.scaling, index.cpu())
+            within(y, want, tol)
+
+
+@gpu
+def test_captured_training_step():
+    """Forward and backward of block and projection in one graph replay to the eager gradients."""
+    gu, down = Weight(2, 2, 2, 512, 320, True), Weight(3, 3, 2, 512, 256)
+    mg, md = block(gu), layer(down)
+    md.input_gradient = True
+    x, dy = randn(1, 40, 320), randn(2, 40, 512)
+
+    def step(t):
+        return torch.autograd.grad(md(mg(t)), t, dy)[0]
+    if fp6._ext is None:   # (nothing says there where a gradient would go)
+        pytest.skip("a differentiable call is captured with the extension alone")
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        step(x.detach().clone().requires_grad_())
+        leaf = x.detach().clone().requires_grad_()
+        stream.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            g = step(leaf)
+        for seed in range(3):
+            with torch.no_grad():
+                leaf.copy_(randn(10 + seed, 40, 320))
+            want = step(leaf.detach().clone().requires_grad_())
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(g, want)
+
+
+@gpu
+def test_a_capture_beside_an_eager_graph_of_the_same_leaf_is_refused():
+    mg, md = block(Weight(2, 2, 2, 512, 320)), layer(Weight(3, 3, 2, 512, 320))
+    md.input_gradient = True
+    leaf = randn(1, 8, 320).requires_grad_()
+    eager = [mg(leaf), md(leaf)]
+    stream, buf = torch.cuda.Stream(), torch.zeros(8, device=DEV)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        buf.add_(1)
+        for m in (mg, md):
+            for t in (leaf, leaf * 1, leaf.float()):
+                with pytest.raises(RuntimeError):
+                    m(t)
+        with torch.no_grad():   # (no gradient, nothing to refuse)
+            y = mg(leaf)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y, eager[0]) and (buf == 1).all()
+    eager[0].sum().backward()
+    assert leaf.grad is not None
