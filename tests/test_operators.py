@@ -238,6 +238,22 @@ def test_input_gradient_with_scales_of_every_kind(E, M):
     within(got, want, (sum_error(OC) + 2 * HALF) * mag + lost + TINY * (mats / sc.clamp(min=1e-9)[:, None]).abs().nan_to_num().sum(0) + HALF * want.abs() + TINY)
 
 
+@gpu
+@pytest.mark.parametrize("N", [5, 40, 200])
+def test_scales_that_start_between_two_16_byte_boundaries(N):
+    """(scales and bias are halfs, and may start at any of them)"""
+    w = Weight(3, 3, 2, 512, 320)
+    odd, b = torch.empty(513, dtype=torch.float16, device=DEV)[1:].copy_(w.scales), torch.empty(513, dtype=torch.float16, device=DEV)[1:].copy_(randn(9, 512))
+    x, dy, dh = randn(1, N, 320), randn(2, N, 512), randn(3, N, 256)
+    pres, outs = [torch.empty(N, 512, device=DEV) for _ in range(2)], []
+    ad = (*bank(3, 3, 16, 512, 320), (torch.arange(N, device=DEV) % 4 - 1).int())
+    for sc, bias, pre in ((w.scales, b.clone(), pres[0]), (odd, b, pres[1])):
+        assert sc.is_contiguous() and sc.data_ptr() % 16 == (2 if sc is odd else 0)
+        outs.append([fp6.gated_forward_native(3, 2, x, w.native, sc, 512, preact=pre, bias=bias), pre, *fp6.gated_backward_native(3, 2, dh, pre, w.native, sc, 320),
+                     fp6.linear_input_grad_native(3, 2, dy, w.native, sc, 320), fp6.adapter_forward_native(3, 2, x, w.native, sc, 512, *ad, bias=bias)])
+    assert all(torch.equal(p, q) for p, q in zip(*outs))
+
+
 def bank(seed, slots, R, OC, IC):
     a, b = randn(seed, slots, R, IC, scale=IC ** -0.5), randn(seed + 1, slots, OC, R, scale=0.5 * R ** -0.5)
     return a, b, torch.linspace(0.25, 2.0, slots, device=DEV)
