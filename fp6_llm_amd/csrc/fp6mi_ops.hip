@@ -140,7 +140,7 @@ template <int ROWS> __device__ __forceinline__ int adapter_of(const int *__restr
 }
 // The passes of this workgroup, numbered from the tile's first: blockIdx.z-th share of gridDim.z, of TOGETHER at least.  A workgroup without any ends before it has asked for anything but
 // the index.  (A further pass of a workgroup waits for the adapter's matrix alone, a further workgroup for everything: with tiles of 64 rows and 11 requests of random lengths
-// in 2048 rows, 10240 x 8192 at rank 64, one pass a workgroup made the call 366 us where this makes it 343.)
+// in 2048 rows, 10240 x 8192 at rank 64, one pass a workgroup and sixteen side by side made the call 366 us, four and three 343.)
 struct Passes { uint32_t first, end; };
 template <uint32_t TOGETHER> __device__ __forceinline__ Passes passes_of(int mine)
 {
@@ -216,6 +216,13 @@ __global__ __launch_bounds__(256) void adapter_shrink(float *__restrict__ part, 
     });
 }
 
+// Tiles that follow one another, and so have adapters in common more often than not, on one XCD, whose L2 they share: workgroup x runs on XCD x % 8 where there are tiles by the eight.
+__device__ __forceinline__ uint32_t neighbouring_tile()
+{
+    const uint32_t xcd = blockIdx.x & 7, extra = gridDim.x & 7;
+    return xcd * (gridDim.x >> 3) + (xcd < extra ? xcd : extra) + (blockIdx.x >> 3);
+}
+
 // adapter_shrink_tile, for many: tiles of 64 rows, sixteen a wavefront.  Rows and adapter pass through LDS in chunks of 128 columns, loaded as whole rows of 256 bytes a chunk ahead: in
 // operand order sixteen lanes ask for sixteen rows, whose addresses share an L2 channel where K is a power of two (8192 columns, N 2048, rank 64: 41 us, this 22 to 30).  LDS rows
 // are 272 bytes apart, the stride at which the operand reads are free of bank conflicts.
@@ -225,8 +232,9 @@ __global__ __launch_bounds__(256) void adapter_shrink_tile(float *__restrict__ p
 {
     constexpr int kRow = 272, kX = 4, kA = RT; // bytes of an LDS row; loads of a thread
     __shared__ __attribute__((aligned(16))) uint8_t lds[2][(64 + RT * 16) * kRow];
+    const uint32_t tile = neighbouring_tile();
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 15, q = lane >> 4;
-    const int mine = adapter_of<64>(index, blockIdx.x, N, slots), here = __shfl(mine, wave * 16 + col);
+    const int mine = adapter_of<64>(index, tile, N, slots), here = __shfl(mine, wave * 16 + col);
     const Passes mypasses = passes_of<4>(mine);
     if (mypasses.first == mypasses.end) return;
 
@@ -236,7 +244,7 @@ __global__ __launch_bounds__(256) void adapter_shrink_tile(float *__restrict__ p
     const half_t  *xrow[kX];
 #pragma unroll
     for (int j = 0; j < kX; j++) {
-        const uint32_t n = blockIdx.x * 64 + (tid >> 4) + 16 * j;
+        const uint32_t n = tile * 64 + (tid >> 4) + 16 * j;
         xrow[j] = x + (size_t)(n < N ? n : N - 1) * K;
     }
     each_adapter(mine, mypasses, [&](int a, uint64_t) {
@@ -288,7 +296,7 @@ __global__ __launch_bounds__(256) void adapter_shrink_tile(float *__restrict__ p
 #pragma unroll
                 for (int r = 0; r < RT; r++) {
                     const uint32_t rank = r0 + r * 16 + 4 * q;
-                    if (rank < R) *reinterpret_cast<v4f *>(part + ((size_t)blockIdx.y * N + blockIdx.x * 64 + wave * 16 + col) * R + rank) = acc[r];
+                    if (rank < R) *reinterpret_cast<v4f *>(part + ((size_t)blockIdx.y * N + tile * 64 + wave * 16 + col) * R + rank) = acc[r];
                 }
             }
         }
@@ -420,41 +428,45 @@ __global__ __launch_bounds__(256) void adapter_expand(half_t *__restrict__ y, co
     });
 }
 
-// adapter_expand_tile, for many: tiles of 64 rows; t lies in memory (adapter_ranks).  An operand of B feeds four MFMAs.  y is read and written as whole row pieces of 512 bytes, the
-// products reaching them through LDS (sixteen rows a wavefront at once, 32 bytes each, where the row length is a multiple of 4 KB all of one L2 channel: 62 us for 10240 outputs
-// at N 2048, rank 64, eleven requests; this takes 49 to 64, and 26 where one request has all rows).  y is asked for when the products are ready: held from the start it costs 32
-// registers, and a workgroup of every three on a CU.
+// adapter_expand_tile, for many: tiles of 64 rows; t lies in memory (adapter_ranks).  An operand of B feeds four MFMAs.  A row's products are kept from the pass that is its own (a
+// selection: another adapter's infinities must not reach it), so y is read and written once for all passes of a workgroup, as whole row pieces of 512 bytes, the products reaching
+// them through LDS (sixteen rows a wavefront at once, 32 bytes each, where the row length is a multiple of 4 KB all of one L2 channel: 62 us for 10240 outputs at N 2048, rank 64).
+// Bound by the operands' way through L2: 25 us with one adapter a tile (3.4 TB/s of y), 30 to 42 for eleven requests of random lengths, 48 to 58 with four adapters in every tile; with
+// y read and written in every pass 25, 49 to 66 and 62 to 72.
 constexpr int kExpandRow = 256 * 4 + 16;
 // STEPS: of 32 ranks, asked for at once
 template <int STEPS>
-__global__ __launch_bounds__(256, 2) void adapter_expand_tile(half_t *__restrict__ y, const half_t *__restrict__ ranks, const float *__restrict__ factors, const half_t *__restrict__ B,
+__global__ __launch_bounds__(256, 3) void adapter_expand_tile(half_t *__restrict__ y, const half_t *__restrict__ ranks, const float *__restrict__ factors, const half_t *__restrict__ B,
                                                               const int *__restrict__ index, uint32_t M, uint32_t N, uint32_t R, uint32_t slots)
 {
     __shared__ __attribute__((aligned(16))) uint8_t lds[32 * kExpandRow]; // 32 of the rows at a time
+    const uint32_t tile = neighbouring_tile();
     const int      tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 15, q = lane >> 4;
-    const int      mine = adapter_of<64>(index, blockIdx.x, N, slots);
+    const int      mine = adapter_of<64>(index, tile, N, slots);
     const uint32_t m0 = blockIdx.y * 256, Rp = (R + 31) & ~31u;
     const Passes   mypasses = passes_of<4>(mine);
     if (mypasses.first == mypasses.end) return;
     // this thread's pieces of y: eight outputs each of rows tid / 32, tid / 32 + 8, ...
-    half_t *const  ybase = y + (size_t)blockIdx.x * 64 * M + m0 + (tid & 31) * 8;
-    const uint32_t nlast = N - blockIdx.x * 64 < 64 ? N - 1 - blockIdx.x * 64 : 63;
+    half_t *const  ybase = y + (size_t)tile * 64 * M + m0 + (tid & 31) * 8;
+    const uint32_t nlast = N - tile * 64 < 64 ? N - 1 - tile * 64 : 63;
     auto           yp = [&](int j) { const uint32_t n = (tid >> 5) + 8 * j; return ybase + (size_t)(n < nlast ? n : nlast) * M; };
     const half_t *trow[4];
     float         f[4];
+    int           here[4];
+    v4f           acc[4][4];
 #pragma unroll
     for (int s = 0; s < 4; s++) { // (rows without an adapter hold anything, and are not stored)
-        const uint32_t n = blockIdx.x * 64 + (16 * s + col < (int)nlast ? 16 * s + col : nlast);
+        const uint32_t n = tile * 64 + (16 * s + col < (int)nlast ? 16 * s + col : nlast);
         trow[s] = ranks + (size_t)n * Rp;
         f[s] = factors[n];
+        here[s] = __shfl(mine, 16 * s + col);
+#pragma unroll
+        for (int o = 0; o < 4; o++) acc[s][o] = (v4f){ 0.f, 0.f, 0.f, 0.f };
     }
+    uint64_t done = 0; // rows of this workgroup's passes
     each_adapter(mine, mypasses, [&](int a, uint64_t same) {
         const half_t *rows = B + ((size_t)a * M + m0 + wave * 64 + col) * R;
-        v4f           acc[4][4];
-#pragma unroll
-        for (int s = 0; s < 4; s++)
-#pragma unroll
-            for (int o = 0; o < 4; o++) acc[s][o] = (v4f){ 0.f, 0.f, 0.f, 0.f };
+        done |= same;
         for (uint32_t r0 = 0; r0 < R; r0 += 32 * STEPS) { // (the same number of steps in every lane; beyond the rank zeros count)
             v8h w[STEPS][4], t[STEPS][4];
 #pragma unroll
@@ -466,40 +478,45 @@ __global__ __launch_bounds__(256, 2) void adapter_expand_tile(half_t *__restrict
                 for (int s = 0; s < 4; s++) t[i][s] = *reinterpret_cast<const v8h *>(trow[s] + (r < Rp ? r : 0));
             }
 #pragma unroll
-            for (int i = 0; i < STEPS; i++) {
+            for (int i = 0; i < STEPS; i++)
                 if (r0 + 32 * i + 8 * q >= R)
 #pragma unroll
                     for (int o = 0; o < 4; o++) w[i][o] = t[i][o] = (v8h)(half_t)0.f;
 #pragma unroll
-                for (int s = 0; s < 4; s++)
+            for (int s = 0; s < 4; s++)
 #pragma unroll
-                    for (int o = 0; o < 4; o++) acc[s][o] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[i][o], t[i][s], acc[s][o], 0, 0, 0);
-            }
-        }
+                for (int o = 0; o < 4; o++) {
+                    v4f sum = { 0.f, 0.f, 0.f, 0.f };
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-            v8h yv[4];
+                    for (int i = 0; i < STEPS; i++) sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[i][o], t[i][s], sum, 0, 0, 0);
 #pragma unroll
-            for (int j = 0; j < 4; j++) yv[j] = *reinterpret_cast<const v8h *>(yp(4 * h + j));
-#pragma unroll
-            for (int s = 0; s < 2; s++)
-#pragma unroll
-                for (int o = 0; o < 4; o++) *reinterpret_cast<v4f *>(lds + (16 * s + col) * kExpandRow + (wave * 64 + o * 16 + 4 * q) * 4) = acc[2 * h + s][o] * f[2 * h + s];
-            __syncthreads();
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const int row = (tid >> 5) + 8 * j;
-                if (same >> (32 * h + row) & 1) {
-                    const v4f lo = *reinterpret_cast<const v4f *>(lds + row * kExpandRow + (tid & 31) * 32), hi = *reinterpret_cast<const v4f *>(lds + row * kExpandRow + (tid & 31) * 32 + 16);
-                    v8h       out;
-#pragma unroll
-                    for (int i = 0; i < 8; i++) out[i] = (half_t)((float)yv[j][i] + (i < 4 ? lo[i & 3] : hi[i & 3]));
-                    *reinterpret_cast<v8h *>(yp(4 * h + j)) = out;
+                    for (int k = 0; k < 4; k++) acc[s][o][k] += here[s] == a ? sum[k] : 0.f;
                 }
-            }
-            __syncthreads();
         }
     });
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        v8h yv[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) yv[j] = *reinterpret_cast<const v8h *>(yp(4 * h + j));
+        if (h) __syncthreads();
+#pragma unroll
+        for (int s = 0; s < 2; s++)
+#pragma unroll
+            for (int o = 0; o < 4; o++) *reinterpret_cast<v4f *>(lds + (16 * s + col) * kExpandRow + (wave * 64 + o * 16 + 4 * q) * 4) = acc[2 * h + s][o] * f[2 * h + s];
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const int row = (tid >> 5) + 8 * j;
+            if (done >> (32 * h + row) & 1) {
+                const v4f lo = *reinterpret_cast<const v4f *>(lds + row * kExpandRow + (tid & 31) * 32), hi = *reinterpret_cast<const v4f *>(lds + row * kExpandRow + (tid & 31) * 32 + 16);
+                v8h       out;
+#pragma unroll
+                for (int i = 0; i < 8; i++) out[i] = (half_t)((float)yv[j][i] + (i < 4 ? lo[i & 3] : hi[i & 3]));
+                *reinterpret_cast<v8h *>(yp(4 * h + j)) = out;
+            }
+        }
+    }
 }
 
 // How an adapter call is cut: tiles of 64 rows where there are many, K ranges of 256 columns at least that fill the chip, and passes of a tile side by side as far as that leaves
