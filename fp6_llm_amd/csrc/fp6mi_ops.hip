@@ -519,13 +519,14 @@ __global__ __launch_bounds__(256, 3) void adapter_expand_tile(half_t *__restrict
     }
 }
 
-// How an adapter call is cut: tiles of 64 rows where there are many, K ranges of 256 columns at least that fill the chip, and passes of a tile side by side as far as that leaves
-// no crowd of workgroups that find nothing to do (a round of them takes 2 us).
+// How an adapter call is cut.  Tiles of 64 rows where there are many: with every batch row a request of its own, 4096 x 4096, rank 16, tiles of 16 / 64 take 36 / 38 us of 192 rows, 40 / 39 of
+// 256, 52 / 43 of 384 (with eight runs of rows 30 / 37 of 256 and 46 / 46 of 768); 10240 x 8192, rank 64, where a row's ranks weigh more, 53 / 57 of 96, 66 / 62 of 128, 94 / 80 of 256.
+// K ranges of 256 columns at least that fill the chip, and passes of a tile side by side as far as that leaves no crowd of workgroups that find nothing to do (a round of them takes 2 us).
 struct AdapterPlan { uint32_t rows, tiles, ranges, shrink_side, expand_side; };
-inline AdapterPlan adapter_plan(size_t M, size_t N, size_t K, size_t slots)
+inline AdapterPlan adapter_plan(size_t M, size_t N, size_t K, size_t R, size_t slots)
 {
     AdapterPlan p;
-    p.rows = N > 256 ? 64 : 16;
+    p.rows = N > (R > 32 ? 112u : 256u) ? 64 : 16;
     p.tiles = (uint32_t)((N + p.rows - 1) / p.rows);
     const size_t fill = 512, most = K / 256 > 0 ? K / 256 : 1, want = (fill + p.tiles - 1) / p.tiles;
     p.ranges = (uint32_t)(want < most ? want : most);
@@ -703,7 +704,7 @@ int fp6mi_gated_backward_native(int E, int Mb, void *stream, const void *W, cons
 
 size_t fp6mi_adapter_workspace_bytes(size_t M, size_t N, size_t K, size_t R, int splitK)
 {
-    return N == 0 ? 0 : adapter_space(adapter_plan(M, N, K, 1), N, R).total + fp6mi_workspace_bytes(M, N, splitK);
+    return N == 0 ? 0 : adapter_space(adapter_plan(M, N, K, R, 1), N, R).total + fp6mi_workspace_bytes(M, N, splitK);
 }
 
 int fp6mi_adapter_native(int E, int Mb, void *stream, const void *W, const void *sc, const void *group_exps, const void *bias, const void *B, void *C, const void *lora_a, const void *lora_b,
@@ -717,7 +718,7 @@ int fp6mi_adapter_native(int E, int Mb, void *stream, const void *W, const void 
     if (M / 256 > 65535) return FP6MI_ERR_SHAPE; // (a grid dimension)
     if (!aligned16(lora_a) || !aligned16(lora_b) || (reinterpret_cast<uintptr_t>(scaling) & 3u) || (reinterpret_cast<uintptr_t>(index) & 3u)) return FP6MI_ERR_ALIGN;
     hipStream_t        st = static_cast<hipStream_t>(stream);
-    const AdapterPlan  p = adapter_plan(M, N, K, slots);
+    const AdapterPlan  p = adapter_plan(M, N, K, R, slots);
     const AdapterSpace s = adapter_space(p, N, R);
     uint8_t           *base = reinterpret_cast<uint8_t *>(ws);
     half_t            *ranks = reinterpret_cast<half_t *>(base + s.ranks);
