@@ -116,9 +116,9 @@ fp6mi::LaunchCfg gated_shape(int E, int Mb, size_t M, size_t N, size_t K, bool g
         return c;
     }
     if (c.kind == 2 && c.wk == 4 && c.nt == 2) return { 1, 2, 2, 4, 2 };                           // gemm_ws 256 x 32
-    if (c.kind == 2 && c.wr == 2) return { 2, 8, 4, 4, 1 };                                          // gemm_prefill
+    if ((c.kind == 2 && c.wr == 2) || (c.kind == 1 && c.nt == 8))                                    // gemm_prefill, gemm_tile 256 x 128; the wide tiles end at K = 2^20
+        return K <= (size_t)1 << 20 ? fp6mi::LaunchCfg{ 2, 8, 4, 4, 1 } : fp6mi::LaunchCfg{ 1, 4, 2, 8, 1 };
     if (c.kind == 2) return c;
-    if (c.nt == 8) return K <= (size_t)1 << 20 ? fp6mi::LaunchCfg{ 2, 8, 4, 4, 1 } : fp6mi::LaunchCfg{ 1, 4, 2, 8, 1 };
     if (c.nt == 2) return { 1, 2, 2, 4, c.wk >= 4 ? 4 : c.wk };
     if (c.nt == 4 && c.wk == 2) return { 1, 4, 2, 4, 2 };
     return { 1, c.nt, 2, 8, 1 };
@@ -635,7 +635,7 @@ static int check_grad(int E, int Mb, const void *W, const void *sc, const void *
 {
     const int rc = fp6mi::check_linear(E, Mb, W, sc, gexp, nullptr, dY, dX, M, N, K, ws, splits);
     if (rc != FP6MI_OK) return rc;
-    return M > (size_t)1 << 20 ? FP6MI_ERR_SHAPE : FP6MI_OK;
+    return M > (size_t)1 << 20 || K > (size_t)1 << 28 ? FP6MI_ERR_SHAPE : FP6MI_OK; // (32-bit offsets over the rows of a tile, over a row of native blocks)
 }
 
 static int run_grad(int E, int Mb, void *stream, const void *W, const void *sc, const void *gexp, const void *dY, bool premultiplied, void *dX, size_t M, size_t N, size_t K, float *ws, int splits)

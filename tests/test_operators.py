@@ -450,6 +450,19 @@ def test_refusals_of_the_c_abi():
     assert L.fp6mi_grad_workspace_bytes(10, 64, 1) == 0 and L.fp6mi_grad_workspace_bytes(10, 64, 3) == 3 * 10 * 64 * 4
 
 
+def test_shapes_of_the_gated_block_beyond_the_wide_tiles():
+    """The wide tiles take up to 2^20 columns; longer rows have another kernel for every batch, not a refusal."""
+    import ctypes
+    L, shape = _lib.lib(), (ctypes.c_int * 5)()
+    for OC in (256, 768, 2048, 5120, 22016):
+        for N in (1, 17, 40, 100, 145, 200, 300, 513, 1000, 4000):
+            for IC in ((1 << 20) + 64, (1 << 21) + 192):
+                for groups in (0, 1):
+                    assert L.fp6mi_query_gated_launch(3, 2, OC, N, IC, groups, shape) == 0
+                    kind, nt, rt, wr, wk = shape
+                    assert kind < 2 or wk == 4, (OC, N, IC, list(shape))
+
+
 def test_grad_splits_are_in_range():
     L = _lib.lib()
     for OC in (256, 4096, 28672):
