@@ -25,8 +25,8 @@ using fp6mi::LaunchCfg;
 // grad_tile: the product that contracts over the weights' rows.
 //   dX[n, k] = sum over m of dY[n, m] * scale[m] * 2^(b-127) * value[m, k]
 // The scale belongs to the contracted index, so it cannot wait for the epilogue as in the forward product.  It is taken apart, scale = mantissa * 2^e with
-// 1 <= |mantissa| < 2: the conversion instruction applies 2^e along with the group's power of two, which leaves the weights exact (they have four significant bits), and
-// the mantissa goes to dY, whose products are rounded to fp16 once (half a step, 2^-11; with a mantissa below two they keep dY's range).  PRE: dY comes multiplied already.
+// 1/2 <= |mantissa| < 1: the conversion instruction applies 2^e along with the group's power of two, which leaves the weights exact (they have four significant bits), and
+// the mantissa goes to dY, whose products are rounded to fp16 once (half a step, 2^-11) and stay within fp16 wherever dY does.  PRE: dY comes multiplied already.
 //   workgroup = 2 x WN wavefronts; tile = 256 input features (a native block's width) x (NT*WN*16) batch rows, 128 x (NT*16) of it per wavefront
 // The native layout holds eight consecutive columns k of one row m in a lane, the MFMA wants eight consecutive rows m of one column.  So a chunk of OCC rows is
 // converted once per workgroup, written to LDS as rows, and read back by the transposing read (ds_read_b64_tr_b16: of a 4 x 16 piece, lane l of

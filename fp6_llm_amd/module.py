@@ -250,7 +250,7 @@ class FPxLinear(torch.nn.Module):
         if index.numel() != x2.shape[0] or (index.dim() != 1 and index.shape != x.shape[:-1]):
             raise ValueError("index must name an adapter for each of the %d rows, got %s" % (x2.shape[0], list(index.shape)))
         y = ops.adapter_forward_native(self.exponent, self.mantissa, x2, self.weight_native, self.scales, self.out_features, adapters.lora_a, adapters.lora_b, adapters.scaling,
-                                       index.reshape(-1), None, group_exps=self.group_exps, bias=self.bias)
+                                       index.reshape(-1).contiguous(), None, group_exps=self.group_exps, bias=self.bias)
         return y.reshape(*x.shape[:-1], self.out_features)
 
     def forward(self, x, adapters=None, index=None):
@@ -367,6 +367,15 @@ class LowRankAdapters(torch.nn.Module):
         self.register_buffer("lora_a", torch.zeros(slots, self.rank, in_features, dtype=torch.float16))
         self.register_buffer("lora_b", torch.zeros(slots, out_features, self.rank, dtype=torch.float16))
         self.register_buffer("scaling", torch.zeros(slots, dtype=torch.float32))
+
+    def _apply(self, fn, *args, **kwargs):
+        """nn.Module's, but that the buffers keep their types when a model around them is cast (the scalings are float32)."""
+        before = dict(self._buffers)
+        super()._apply(fn, *args, **kwargs)
+        for name, t in before.items():
+            if self._buffers[name].dtype != t.dtype:
+                self._buffers[name] = t.to(self._buffers[name].device)
+        return self
 
     @torch.no_grad()
     def set(self, slot, a, b, scaling=1.0):

@@ -224,8 +224,8 @@ int fp6mi_quantize_native_grouped_gpu(int E, int Mbits, void *stream, void *nati
 /* ---------------------------------------------------------------------------------- operators around the linear layer (beyond the reference)
  * All of them take native-layout weights of M rows and K columns with row scales and, where group_exps_native is not NULL, group exponents; bias may be NULL. */
 
-/* Input gradient of the linear layer: dX[N,K] = dY[N,M] . (scale * 2^(b-127) * value)[M,K].  dY times the mantissa of its row's scale is rounded to fp16, the products are summed in
- * FP32; a weight keeps its value but where value * 2^(b-127) times the power of two of its scale leaves fp16.  M up to 2^20.  splits > 1 cuts the sum over M into that many parts, whose partial sums take fp6mi_grad_workspace_bytes bytes. */
+/* Input gradient of the linear layer: dX[N,K] = dY[N,M] . (scale * 2^(b-127) * value)[M,K].  dY times the mantissa of its row's scale, from 1/2 to 1, is rounded to fp16, the products are summed
+ * in FP32; a weight keeps its value but where value * 2^(b-127) times the power of two above its scale leaves fp16 (from 2^15 on it may be infinite).  M up to 2^20, K up to 2^28.  splits > 1 cuts the sum over M into that many parts, whose partial sums take fp6mi_grad_workspace_bytes bytes. */
 int    fp6mi_linear_grad_native(int E, int Mbits, void *stream, const void *W_native, const void *scales_f16, const void *group_exps_native, const void *dY_f16,
                                 void *dX_f16, size_t M, size_t N, size_t K, float *workspace, int splits);
 int    fp6mi_query_grad_launch(int E, int Mbits, size_t M, size_t N, size_t K, int splits); /* batch rows of a workgroup of the kernel that takes it, or FP6MI_ERR_* */

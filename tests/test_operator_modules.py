@@ -85,6 +85,27 @@ def test_adapters_of_a_fused_layer_reach_their_parts():
     assert not ad.lora_a.any() and not ad.lora_b.any() and not ad.scaling.any()
 
 
+def test_adapters_keep_their_types_in_a_model_that_is_cast():
+    ad = LowRankAdapters(64, 256, 2, 8)
+    ad.set(0, torch.randn(8, 64), torch.randn(256, 8), 1 / 3)
+    want = {k: t.clone() for k, t in ad.state_dict().items()}
+    for cast in (lambda m: m.half(), lambda m: m.to(torch.bfloat16), lambda m: m.double(), lambda m: m.to("cpu", torch.float32)):
+        assert cast(torch.nn.Sequential(ad))[0] is ad
+        assert all(t.dtype == want[k].dtype and torch.equal(t, want[k]) for k, t in ad.state_dict().items())
+
+
+@gpu
+def test_indexes_that_are_views():
+    w = Weight(1, 3, 2, 256, 128)
+    m, ad = layer(w), LowRankAdapters(128, 256, 3, 8).to(DEV)
+    for i in range(3):
+        ad.set(i, randn(i, 8, 128, scale=0.1), randn(i + 5, 256, 8))
+    x, table = randn(7, 6, 4, 128), torch.randint(-1, 3, (6, 2), generator=torch.Generator().manual_seed(1)).int().to(DEV)
+    want = m(x, ad, table[:, 1].reshape(6, 1).repeat(1, 4).contiguous())
+    assert torch.equal(m(x, ad, table[:, 1:].expand(6, 4)), want)
+    assert torch.equal(m(x[:, 0], ad, table[:, 1]), m(x[:, 0].contiguous(), ad, table[:, 1].contiguous()))
+
+
 @gpu
 @pytest.mark.parametrize("N,act", [(1, "silu"), (23, "gelu"), (300, "gelu_tanh")])
 def test_gated_module_is_its_function_and_differentiable(N, act):

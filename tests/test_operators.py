@@ -254,6 +254,33 @@ def test_scales_that_start_between_two_16_byte_boundaries(N):
     assert all(torch.equal(p, q) for p, q in zip(*outs))
 
 
+@gpu
+@pytest.mark.parametrize("N", [3, 30, 100])
+def test_gradients_up_to_the_largest_half(N):
+    """Scaled losses make gradients of any size: up to 65504 they go in as they are, whatever the mantissas of the scales, and what comes out of small weights is finite."""
+    OC, IC = 512, 320
+    w = Weight(4, 3, 2, OC, IC)
+    sc = (torch.linspace(1.0, 1.999, OC, dtype=torch.float64) * 2.0 ** -13).half()
+    mats = w.w / d(w.scales)[:, None] * sc.double()[:, None]
+    g = torch.Generator().manual_seed(N)
+    dy = ((40000 + 25504 * torch.rand(N, OC, generator=g)) * (2 * torch.randint(0, 2, (N, OC), generator=g) - 1)).half().to(DEV)
+    dy[0, :2] = torch.tensor([65504.0, -65504.0])
+    want, mag = d(dy) @ mats, d(dy).abs() @ mats.abs()
+    assert want.abs().max() < 65504
+    got = fp6.linear_input_grad_native(3, 2, dy, w.native, sc.to(DEV), IC)
+    # (weights of small scales may lose bits below the normal halfs: 2^-25, against scales of 2^-13)
+    within(got, want, (sum_error(OC) + HALF) * mag + 2 * TINY * d(dy).abs().sum(1, keepdim=True) + HALF * want.abs() + TINY)
+    # and through the block: g = 0 has slope 1/2 and activation 0, so dp = dh * u / 2 there
+    pre = torch.zeros(N, OC, device=DEV)
+    pre.view(N, -1, 2, 16)[:, :, 1] = 2.0
+    dh = dy[:, :OC // 2]
+    dx, dp = fp6.gated_backward_native(3, 2, dh, pre, w.native, sc.to(DEV), IC)
+    dp64 = pairs(d(dh), torch.zeros(N, OC // 2, dtype=torch.float64))
+    assert torch.equal(d(dp), dp64)
+    want, mag = dp64 @ mats, dp64.abs() @ mats.abs()
+    within(dx, want, (sum_error(OC) + HALF + 2.0 ** -17) * mag + 2 * TINY * dp64.abs().sum(1, keepdim=True) + HALF * want.abs() + TINY)
+
+
 def bank(seed, slots, R, OC, IC):
     a, b = randn(seed, slots, R, IC, scale=IC ** -0.5), randn(seed + 1, slots, OC, R, scale=0.5 * R ** -0.5)
     return a, b, torch.linspace(0.25, 2.0, slots, device=DEV)
