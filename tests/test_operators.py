@@ -365,6 +365,28 @@ def test_adapters_keep_requests_apart():
 
 
 @gpu
+@pytest.mark.parametrize("N,R", [(130, 40), (300, 16), (300, 72)])
+def test_adapters_keep_requests_apart_in_large_tiles(N, R):
+    """The same where a tile of 64 rows holds many adapters, and rows without one: those get the layer's own bits."""
+    w = Weight(5, 2, 2, 512, 320)
+    a, b, s = bank(6, 7, R, 512, 320)
+    x, index = randn(9, N, 320), torch.randint(-1, 7, (N,), generator=torch.Generator().manual_seed(R), dtype=torch.int32)
+    clean = fp6.adapter_forward_native(2, 2, x, w.native, w.scales, 512, a, b, s, index.to(DEV), splitK=1)
+    assert torch.equal(clean[index < 0], fp6.linear_forward_native(2, 2, x, w.native, w.scales, 512)[index < 0])
+    a2, b2, s2, x2 = a.clone(), b.clone(), s.clone(), x.clone()
+    a2[1, 3], b2[2, 200, 5], s2[3] = float("inf"), float("nan"), float("inf")
+    row = int((index == 4).nonzero()[0])
+    x2[row, 5] = float("nan")
+    buf = torch.full((N + 2, 512), 7.0, dtype=torch.float16, device=DEV)
+    got = fp6.adapter_forward_native(2, 2, x2, w.native, w.scales, 512, a2, b2, s2, index.to(DEV), splitK=1, out=buf[:N])
+    keep = [n for n in range(N) if index[n] not in (1, 2, 3) and n != row]
+    assert torch.equal(got[keep], clean[keep]) and torch.isnan(got[row]).all() and (buf[N:] == 7.0).all()
+    assert not torch.isfinite(got[index == 1]).any() and torch.isnan(got[index == 2][:, 200]).all() and not torch.isfinite(got[index == 3]).any()
+    others = [c for c in range(512) if c != 200]
+    assert torch.equal(got[index == 2][:, others], clean[index == 2][:, others])
+
+
+@gpu
 def test_strided_activations_given_outputs_and_another_stream():
     w = Weight(3, 3, 2, 512, 320, True)
     N = 70
