@@ -309,11 +309,13 @@ __global__ __launch_bounds__(2 * WN *kWave, NT >= 6 ? 1 : 2) void grad_tile(cons
 
 // ---------------------------------------------------------------------------------------------------------------
 // grad_stream: the same product for up to 32 batch rows, where the weights' way from memory is the bound.
-//   grid = (blocks of 256 input features, splits)   block = WO wavefronts, which share the weight rows of a split among them, 32 rows (two native blocks) at a time in turn
-// Every wavefront is by itself until the end: it converts two native blocks, half of their columns after the other, into an LDS area of its own (rows 288 bytes apart, in grad_tile's
+//   grid = (blocks of 256 input features, splits)   block = WO wavefronts, which share the weight rows of a split among them, 32 rows (two native blocks) at a time in turn, half of
+//   the columns each
+// Every wavefront is by itself until the end: it converts its halves of two native blocks into an LDS area of its own (rows 288 bytes apart, in grad_tile's
 // order; no barrier, the LDS unit serves a wavefront in order), reads them back transposed, and takes its batch rows from memory in operand order.  The codes of the next
-// 32 rows are asked for before this one's are converted.  Sums meet in LDS.  us, with the reduction of the splits, e3m2: 4096x4096 N 8 11.1 (16 splits), 8192x8192 N 1 15.7 (8), 22016x4096
-// N 8 21.7 (16, 3.1 TB/s).  Half blocks a wavefront, with more of them: 13.3, 35.6 and 47.0 (the codes that the halves share were fetched by two XCDs).
+// 32 rows are asked for before this one's are converted.  Sums meet in LDS.  us, with the reduction of the splits, e3m2, N 8 / 32: 4096x4096 10.8 / 15.5 (16 splits), 8192x8192 17.3 / 21.5 (8),
+// 28672x8192 39 / 48 (8, 4.5 TB/s); with whole blocks a wavefront, twice the sums to meet, 11.2 / 18.2, 17.9 / 27.3, 39 / 65.  (Half blocks of different workgroups 13.3 and 35.6 at N 8, 1:
+// the codes that the halves share were fetched by two XCDs.)
 // ---------------------------------------------------------------------------------------------------------------
 constexpr int kStreamRow = 288, kStreamHalf = 16 * kStreamRow + 16, kStreamMant = 2 * kStreamHalf, kStreamWave = kStreamMant + 64;
 template <int NT, int WO> constexpr int grad_stream_lds() { return WO * (NT * 8192 > kStreamWave ? NT * 8192 : kStreamWave); }
@@ -322,36 +324,19 @@ template <int FM, bool GS, bool PRE, int NT, int WO>
 __global__ __launch_bounds__(WO *kWave) void grad_stream(const uint8_t *__restrict__ W, const half_t *__restrict__ scales, const uint8_t *__restrict__ gexp, const half_t *__restrict__ dY,
                                                          half_t *__restrict__ dX, float *__restrict__ ws, uint32_t M, uint32_t N, uint32_t K, uint32_t units, uint32_t splits)
 {
-    constexpr int RT = 8, kWaveLds = grad_stream_lds<NT, WO>() / WO;
+    constexpr int RT = 8, WR = WO / 2, kWaveLds = grad_stream_lds<NT, WO>() / WO;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-    const int      tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 15, q = lane >> 4;
+    const int      tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 15, q = lane >> 4, wi = wave & 1, wr = wave >> 1;
     const uint32_t kb = blockIdx.x, split = blockIdx.y, chunks = M / 32;
     const uint32_t avg = chunks / splits, extra = chunks % splits, c0 = split * avg + (split < extra ? split : extra), c1 = c0 + avg + (split < extra ? 1u : 0u);
     uint8_t       *mine = lds + wave * kWaveLds;
 
-    v4f acc[2][RT][NT];
+    v4f acc[RT][NT];
 #pragma unroll
-    for (int h = 0; h < 2; h++)
+    for (int r = 0; r < RT; r++)
 #pragma unroll
-        for (int r = 0; r < RT; r++)
-#pragma unroll
-            for (int t = 0; t < NT; t++) acc[h][r][t] = (v4f){ 0.f, 0.f, 0.f, 0.f };
+        for (int t = 0; t < NT; t++) acc[r][t] = (v4f){ 0.f, 0.f, 0.f, 0.f };
 
-    struct Raw { WFrag<FM> w[2]; uint32_t g[2]; half_t sc[2]; v8h b[NT]; };
-    auto load = [&](Raw &f, uint32_t c) __attribute__((always_inline)) {
-#pragma unroll
-        for (int i = 0; i < 2; i++) {
-            const size_t blk = (size_t)(2 * c + i) * units + kb;
-            f.w[i] = load_wfrag<FM>(W + blk * Fmt<FM>::block_bytes, lane);
-            f.g[i] = load_group_exps<GS>(gexp, blk, lane);
-            f.sc[i] = scales[c * 32 + 16 * i + col];
-        }
-#pragma unroll
-        for (int t = 0; t < NT; t++) { // (rows beyond N repeat the last one and are not stored)
-            const uint32_t n = 16 * t + col < N ? 16 * t + col : N - 1;
-            f.b[t] = *reinterpret_cast<const v8h *>(dY + (size_t)n * M + c * 32 + 8 * q);
-        }
-    };
     // (reads of other lanes' writes: the LDS unit serves a wavefront in order, the compiler has to leave them in this one)
     auto in_order = [] {
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
@@ -360,67 +345,79 @@ __global__ __launch_bounds__(WO *kWave) void grad_stream(const uint8_t *__restri
     };
     uint8_t *const       wdst = mine + (col >> 2 & 1) * kStreamHalf + (4 * (col >> 3) + (col & 3)) * kStreamRow + q * 16;
     const uint8_t *const wread = mine + (4 * q + (col >> 2)) * kStreamRow + (col & 3) * 8;
-    auto                 multiply = [&](Raw &f) __attribute__((always_inline)) {
+    auto run = [&](auto half_c) __attribute__((always_inline)) {
+        constexpr int H = decltype(half_c)::value;
+        // what is fetched for 32 rows: codes, exponent and scale of two native blocks, and the batch rows
+        auto load_codes = [&](RawHalf &w, half_t &sc, uint32_t tile) __attribute__((always_inline)) {
+            const size_t blk = (size_t)tile * units + kb;
+            load_raw_half<FM, GS, H>(w, W + blk * Fmt<FM>::block_bytes, GS ? gexp + blk * 32 : nullptr, lane);
+            sc = scales[tile * 16 + col];
+        };
+        auto load_rows = [&](v8h(&b)[NT], uint32_t c) __attribute__((always_inline)) {
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-#pragma unroll
-            for (int i = 0; i < 2; i++) { // row 16 i + col of 32: the (4 (2 i + col / 8) + col % 4)-th of its half
-                const v32h v = grad_weights<FM, GS>(field_string<FM>(f.w[i], h), f.sc[i], h == 0 ? f.g[i] & 0xffu : f.g[i] >> 8);
-#pragma unroll
-                for (int s = 0; s < 4; s++) *reinterpret_cast<v8h *>(wdst + i * 8 * kStreamRow + 64 * s) = slice8(v, s);
-                if (!PRE && h == 0 && q == 0) *reinterpret_cast<half_t *>(mine + kStreamMant + (16 * i + col) * 2) = scale_mantissa(f.sc[i]);
+            for (int t = 0; t < NT; t++) { // (rows beyond N repeat the last one and are not stored)
+                const uint32_t n = 16 * t + col < N ? 16 * t + col : N - 1;
+                b[t] = *reinterpret_cast<const v8h *>(dY + (size_t)n * M + c * 32 + 8 * q);
             }
+        };
+        auto convert_rows = [&](const RawHalf &w, half_t sc, int i) __attribute__((always_inline)) { // row 16 i + col of 32: the (4 (2 i + col / 8) + col % 4)-th of its half
+            const v32h v = grad_weights<FM, GS>(raw_half_fields<FM, H>(w), sc, w.g);
+#pragma unroll
+            for (int s = 0; s < 4; s++) *reinterpret_cast<v8h *>(wdst + i * 8 * kStreamRow + 64 * s) = slice8(v, s);
+            if (!PRE && q == 0) *reinterpret_cast<half_t *>(mine + kStreamMant + (16 * i + col) * 2) = scale_mantissa(sc);
+        };
+        auto multiply = [&](v8h(&b)[NT]) __attribute__((always_inline)) {
             in_order();
             if constexpr (!PRE) {
-                if (h == 0) {
-                    const v8h mant = *reinterpret_cast<const v8h *>(mine + kStreamMant + 16 * q);
+                const v8h mant = *reinterpret_cast<const v8h *>(mine + kStreamMant + 16 * q);
 #pragma unroll
-                    for (int t = 0; t < NT; t++) f.b[t] = f.b[t] * mant;
-                }
+                for (int t = 0; t < NT; t++) b[t] = b[t] * mant;
             }
 #pragma unroll
             for (int r = 0; r < RT; r++) {
                 const v8h a = __builtin_shufflevector(read_transposed(wread + r * 32), read_transposed(wread + kStreamHalf + r * 32), 0, 1, 2, 3, 4, 5, 6, 7);
 #pragma unroll
-                for (int t = 0; t < NT; t++) acc[h][r][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, f.b[t], acc[h][r][t], 0, 0, 0);
+                for (int t = 0; t < NT; t++) acc[r][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b[t], acc[r][t], 0, 0, 0);
             }
             in_order();
+        };
+        RawHalf  w00, w01, w10, w11; // (arrays or one struct of them go to scratch memory)
+        half_t   s00, s01, s10, s11;
+        v8h      b0[NT], b1[NT];
+        uint32_t c = c0 + wr;
+        if (c < c1) load_codes(w00, s00, 2 * c), load_codes(w01, s01, 2 * c + 1), load_rows(b0, c);
+        while (c < c1) {
+            if (c + WR < c1) load_codes(w10, s10, 2 * (c + WR)), load_codes(w11, s11, 2 * (c + WR) + 1), load_rows(b1, c + WR);
+            convert_rows(w00, s00, 0), convert_rows(w01, s01, 1), multiply(b0);
+            c += WR;
+            if (c >= c1) break;
+            if (c + WR < c1) load_codes(w00, s00, 2 * (c + WR)), load_codes(w01, s01, 2 * (c + WR) + 1), load_rows(b0, c + WR);
+            convert_rows(w10, s10, 0), convert_rows(w11, s11, 1), multiply(b1);
+            c += WR;
         }
     };
-    Raw      even, odd;
-    uint32_t c = c0 + wave;
-    if (c < c1) load(even, c);
-    while (c < c1) {
-        if (c + WO < c1) load(odd, c + WO);
-        multiply(even);
-        c += WO;
-        if (c >= c1) break;
-        if (c + WO < c1) load(even, c + WO);
-        multiply(odd);
-        c += WO;
-    }
+    if (wi == 0)
+        run(std::integral_constant<int, 0>{});
+    else
+        run(std::integral_constant<int, 1>{});
 
-    // 128 input features at a time, every wavefront parks its sums in its own area: [r][t][lane] of four input features
+    // every wavefront parks its sums in its own area, [r][t][lane] of four input features
 #pragma unroll
-    for (int h = 0; h < 2; h++) {
-        if (h == 1) __syncthreads();
+    for (int r = 0; r < RT; r++)
 #pragma unroll
-        for (int r = 0; r < RT; r++)
+        for (int t = 0; t < NT; t++) *reinterpret_cast<v4f *>(mine + (r * NT + t) * 1024 + lane * 16) = acc[r][t];
+    __syncthreads();
+    for (uint32_t p = tid; p < N * 64; p += WO * kWave) { // input features 4 f .. of half h, batch row n
+        const uint32_t f = p & 31, h = p >> 5 & 1, n = p >> 6, k = kb * 256 + h * 128 + 4 * f;
+        const uint8_t *src = lds + h * kWaveLds + ((f >> 2) * NT + (n >> 4)) * 1024 + ((f & 3) * 16 + (n & 15)) * 16;
+        v4f            sum = *reinterpret_cast<const v4f *>(src);
 #pragma unroll
-            for (int t = 0; t < NT; t++) *reinterpret_cast<v4f *>(mine + (r * NT + t) * 1024 + lane * 16) = acc[h][r][t];
-        __syncthreads();
-        for (int p = tid; p < NT * 512; p += WO * kWave) { // input features 4 f .. of the 128, batch row n
-            const uint32_t f = p & 31, n = p >> 5, k = kb * 256 + h * 128 + 4 * f;
-            const uint8_t *src = lds + ((f >> 2) * NT + (n >> 4)) * 1024 + ((f & 3) * 16 + (n & 15)) * 16;
-            v4f            sum = *reinterpret_cast<const v4f *>(src);
-#pragma unroll
-            for (int w = 1; w < WO; w++) sum += *reinterpret_cast<const v4f *>(src + w * kWaveLds);
-            if (n < N && k < K) {
-                if (splits == 1)
-                    *reinterpret_cast<v4hh *>(dX + (size_t)n * K + k) = (v4hh){ (half_t)sum[0], (half_t)sum[1], (half_t)sum[2], (half_t)sum[3] };
-                else
-                    *reinterpret_cast<v4f *>(ws + ((size_t)split * N + n) * K + k) = sum;
-            }
+        for (int w = 1; w < WR; w++) sum += *reinterpret_cast<const v4f *>(src + 2 * w * kWaveLds);
+        if (k < K) {
+            if (splits == 1)
+                *reinterpret_cast<v4hh *>(dX + (size_t)n * K + k) = (v4hh){ (half_t)sum[0], (half_t)sum[1], (half_t)sum[2], (half_t)sum[3] };
+            else
+                *reinterpret_cast<v4f *>(ws + ((size_t)split * N + n) * K + k) = sum;
         }
     }
 }
@@ -460,7 +457,9 @@ int grad_cfg(int rows, hipStream_t st, const void *W, const void *sc, const void
 {
     switch (rows) {
     case 16: return launch_grad_stream<FM, GS, PRE, 1, 8>(st, W, sc, gexp, dY, dX, ws, M, N, K, splits);
-    case 32: return launch_grad_stream<FM, GS, PRE, 2, 4>(st, W, sc, gexp, dY, dX, ws, M, N, K, splits);
+    case 32: // (us at N 24, four / eight wavefronts: 8 of these 32 rows a split 14.3 / 15.4 and 13.2 / 13.3, 10 of them 16.1 / 16.1, 32 of them 25.2 / 20.1, 43 31.0 / 23.0, 112 64 / 45)
+        return M / 32 / splits >= 16 ? launch_grad_stream<FM, GS, PRE, 2, 8>(st, W, sc, gexp, dY, dX, ws, M, N, K, splits)
+                                     : launch_grad_stream<FM, GS, PRE, 2, 4>(st, W, sc, gexp, dY, dX, ws, M, N, K, splits);
     case 128: return launch_grad<FM, GS, PRE, 2, 4>(st, W, sc, gexp, dY, dX, ws, M, N, K, splits);
     case 192: return launch_grad<FM, GS, PRE, 6, 2>(st, W, sc, gexp, dY, dX, ws, M, N, K, splits);
     case 256: return launch_grad<FM, GS, PRE, 8, 2>(st, W, sc, gexp, dY, dX, ws, M, N, K, splits);

@@ -613,8 +613,8 @@ int fp6mi_heuristic_grad_splits(int E, int Mb, size_t M, size_t N, size_t K, int
 {
     (void)E, (void)Mb;
     if (M == 0 || N == 0 || K == 0 || num_cus <= 0) return 1;
-    if (N <= 32) { // a workgroup to a CU, of which every wavefront has 32 rows at least
-        const size_t units = (K + 255) / 256, s = ((size_t)num_cus + units / 2) / units, most = M / 256;
+    if (N <= 32) { // a workgroup to a CU and never more (43 blocks of features, us at N 8: four splits 14.5, five 13.7, six 19.4), whose wavefronts have 32 rows at least
+        const size_t units = (K + 255) / 256, s = (size_t)num_cus / units, most = M / 256;
         return (int)(s < 1 ? 1 : s < most ? s : most > 0 ? most : 1);
     }
     int    best = 1;

@@ -161,6 +161,18 @@ def test_gated_block_backward(act, N, OC, IC):
 
 
 @gpu
+@pytest.mark.parametrize("splitK", [1, 2, 5, 16])
+@pytest.mark.parametrize("N", [16, 24, 32, 90])
+def test_gated_block_backward_with_the_sum_split(N, splitK):
+    """(the kernels for few rows take more wavefronts where a split has many weight rows)"""
+    w = Weight(8, 2, 1, 1024, 320, True)
+    dh, pre = randn(3, N, 512, scale=0.1), randn(4, N, 1024).float()
+    dx, dp = fp6.gated_backward_native(2, 1, dh, pre, w.native, w.scales, 320, splitK=splitK, group_exps=w.exps)
+    want, mag = d(dp) @ w.w, d(dp).abs() @ w.w.abs()   # (dp has been rounded once, and what was multiplied once)
+    within(dx, want, (sum_error(1024) + 2 * HALF * (1 + HALF)) * mag + 2 * TINY * w.w.abs().sum(0) + HALF * want.abs() + TINY)
+
+
+@gpu
 @pytest.mark.parametrize("act", ACTS)
 def test_gated_block_gradient_against_differences(act):
     """The whole chain: the slope of sum(dh * h) along a direction, from the kernels' gradient and from central differences of the formula in 64 bits."""
