@@ -351,6 +351,7 @@ __global__ __launch_bounds__(256) void adapter_ranks(half_t *__restrict__ ranks,
 //
 // adapter_expand, for few rows: tiles of sixteen; forms t in LDS from the ranges' sums, which saves a launch and is bound by the latency of it (4096 outputs, 32 rows of 32 requests,
 // rank 16: 7.5 us).
+template <int RT>
 __global__ __launch_bounds__(256) void adapter_expand(half_t *__restrict__ y, const float *__restrict__ part, const half_t *__restrict__ B, const float *__restrict__ scaling,
                                                       const int *__restrict__ index, uint32_t M, uint32_t N, uint32_t R, uint32_t slots, uint32_t ranges)
 {
@@ -386,15 +387,20 @@ __global__ __launch_bounds__(256) void adapter_expand(half_t *__restrict__ y, co
 #pragma unroll
             for (int j = 0; j < 16; j++) v[j] = 0.f;
 #pragma unroll
-            for (int j = 0; j < 16; j++)
-                if (16 * j < (int)R) {
-                    const float *at = src + (c + 16 * j < (int)R ? c + 16 * j : 0);
-                    for (uint32_t s0 = 0; s0 < ranges; s0 += 8) { // eight ranges' sums on their way at once
-                        float t[8];
+            for (int j0 = 0; j0 < 16; j0 += RT)
+                if (16 * j0 < (int)R) {
+                    for (uint32_t s0 = 0; s0 < ranges; s0 += 8) { // the sums of RT x 16 ranks over eight ranges on their way at once
+                        float t[RT][8];
 #pragma unroll
-                        for (int u = 0; u < 8; u++) t[u] = at[(size_t)(s0 + u < ranges ? s0 + u : 0) * N * R];
+                        for (int j = 0; j < RT; j++) {
+                            const float *at = src + (c + 16 * (j0 + j) < (int)R ? c + 16 * (j0 + j) : 0);
 #pragma unroll
-                        for (int u = 0; u < 8; u++) v[j] += s0 + u < ranges ? t[u] : 0.f;
+                            for (int u = 0; u < 8; u++) t[j][u] = at[(size_t)(s0 + u < ranges ? s0 + u : 0) * N * R];
+                        }
+#pragma unroll
+                        for (int j = 0; j < RT; j++)
+#pragma unroll
+                            for (int u = 0; u < 8; u++) v[j0 + j] += s0 + u < ranges ? t[j][u] : 0.f;
                     }
                 }
 #pragma unroll
@@ -567,7 +573,7 @@ int adapter_expand_of(hipStream_t st, const AdapterPlan &p, void *y, const float
         hipLaunchKernelGGL(R <= 32 ? adapter_expand_tile<1> : adapter_expand_tile<2>, grid, dim3(256), 0, st, static_cast<half_t *>(y), ranks, factors, static_cast<const half_t *>(B), index, (uint32_t)M, (uint32_t)N,
                            (uint32_t)R, (uint32_t)slots);
     } else {
-        hipLaunchKernelGGL(adapter_expand, grid, dim3(256), 0, st, static_cast<half_t *>(y), part, static_cast<const half_t *>(B), scaling, index, (uint32_t)M, (uint32_t)N, (uint32_t)R,
+        hipLaunchKernelGGL(R <= 16 ? adapter_expand<1> : R <= 32 ? adapter_expand<2> : adapter_expand<4>, grid, dim3(256), 0, st, static_cast<half_t *>(y), part, static_cast<const half_t *>(B), scaling, index, (uint32_t)M, (uint32_t)N, (uint32_t)R,
                            (uint32_t)slots, p.ranges);
     }
     return (int)hipGetLastError();
