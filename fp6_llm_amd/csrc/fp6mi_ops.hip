@@ -161,13 +161,14 @@ template <typename F> __device__ __forceinline__ void each_adapter(int mine, Pas
     }
 }
 
-// shrink: part[range][n][r] = sum over a range of K of x[n, k] * A[a, r, k], fp32.  grid = (tiles, K ranges, passes side by side).  Ranks are taken RT * 16 at a time.
+// shrink: part[range][n][r] = sum over a range of K of x[n, k] * A[a, r, k], fp32.  grid = (tiles, K ranges, passes side by side).  Ranks are taken RT * 16 at a time, in
+// adapter_shrink by workgroups of their own (in the grid's second dimension, behind the ranges).
 //
 // adapter_shrink, for few rows: tiles of sixteen, operands straight from memory, the four wavefronts of a workgroup taking every fourth 64 columns of its range and meeting in LDS.
 // Bound by latency: three round trips, to the index, to the operands and to the output (4096 columns, 32 rows of 32 requests, rank 16: 4.4 us).
 template <int RT>
 __global__ __launch_bounds__(256) void adapter_shrink(float *__restrict__ part, const half_t *__restrict__ x, const half_t *__restrict__ A, const int *__restrict__ index, uint32_t N,
-                                                      uint32_t K, uint32_t R, uint32_t slots)
+                                                      uint32_t K, uint32_t R, uint32_t slots, uint32_t ranges)
 {
     __shared__ __attribute__((aligned(16))) float sums[3][RT][256];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, q = lane >> 4;
@@ -175,44 +176,42 @@ __global__ __launch_bounds__(256) void adapter_shrink(float *__restrict__ part, 
     const Passes mypasses = passes_of<1>(mine);
     if (mypasses.first == mypasses.end) return;
 
-    const uint32_t pieces = K / 64, avg = pieces / gridDim.y, extra = pieces % gridDim.y;
-    const uint32_t p0 = blockIdx.y * avg + (blockIdx.y < extra ? blockIdx.y : extra), p1 = p0 + avg + (blockIdx.y < extra ? 1u : 0u);
+    const uint32_t range = blockIdx.y % ranges, r0 = blockIdx.y / ranges * (RT * 16), pieces = K / 64, avg = pieces / ranges, extra = pieces % ranges;
+    const uint32_t p0 = range * avg + (range < extra ? range : extra), p1 = p0 + avg + (range < extra ? 1u : 0u);
     const uint32_t n = blockIdx.x * 16 + col;
     const half_t  *xrow = x + (size_t)(n < N ? n : N - 1) * K + 8 * q;
     each_adapter(mine, mypasses, [&](int a, uint64_t) {
-        for (uint32_t r0 = 0; r0 < R; r0 += RT * 16) {
-            const half_t *rows[RT];
-            v4f           acc[RT];
+        const half_t *rows[RT];
+        v4f           acc[RT];
+#pragma unroll
+        for (int r = 0; r < RT; r++) {
+            const uint32_t row = r0 + r * 16 + col < R ? r0 + r * 16 + col : R - 1; // (rows beyond the rank are not stored)
+            rows[r] = A + ((size_t)a * R + row) * K + 8 * q;
+            acc[r] = (v4f){ 0.f, 0.f, 0.f, 0.f };
+        }
+        for (uint32_t p = p0 + wave; p < p1; p += 4) {
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const v8h b = *reinterpret_cast<const v8h *>(xrow + (size_t)p * 64 + 32 * h);
+#pragma unroll
+                for (int r = 0; r < RT; r++)
+                    acc[r] = __builtin_amdgcn_mfma_f32_16x16x32_f16(*reinterpret_cast<const v8h *>(rows[r] + (size_t)p * 64 + 32 * h), b, acc[r], 0, 0, 0);
+            }
+        }
+        if (wave > 0)
+#pragma unroll
+            for (int r = 0; r < RT; r++) *reinterpret_cast<v4f *>(&sums[wave - 1][r][lane * 4]) = acc[r];
+        __syncthreads();
+        if (wave == 0 && here == a) { // acc[r][i]: rank r0 + 16 r + 4 q + i of batch row n
 #pragma unroll
             for (int r = 0; r < RT; r++) {
-                const uint32_t row = r0 + r * 16 + col < R ? r0 + r * 16 + col : R - 1; // (rows beyond the rank are not stored)
-                rows[r] = A + ((size_t)a * R + row) * K + 8 * q;
-                acc[r] = (v4f){ 0.f, 0.f, 0.f, 0.f };
+#pragma unroll
+                for (int w = 0; w < 3; w++) acc[r] += *reinterpret_cast<const v4f *>(&sums[w][r][lane * 4]);
+                const uint32_t rank = r0 + r * 16 + 4 * q;
+                if (rank < R) *reinterpret_cast<v4f *>(part + ((size_t)range * N + n) * R + rank) = acc[r];
             }
-            for (uint32_t p = p0 + wave; p < p1; p += 4) {
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    const v8h b = *reinterpret_cast<const v8h *>(xrow + (size_t)p * 64 + 32 * h);
-#pragma unroll
-                    for (int r = 0; r < RT; r++)
-                        acc[r] = __builtin_amdgcn_mfma_f32_16x16x32_f16(*reinterpret_cast<const v8h *>(rows[r] + (size_t)p * 64 + 32 * h), b, acc[r], 0, 0, 0);
-                }
-            }
-            if (wave > 0)
-#pragma unroll
-                for (int r = 0; r < RT; r++) *reinterpret_cast<v4f *>(&sums[wave - 1][r][lane * 4]) = acc[r];
-            __syncthreads();
-            if (wave == 0 && here == a) { // acc[r][i]: rank r0 + 16 r + 4 q + i of batch row n
-#pragma unroll
-                for (int r = 0; r < RT; r++) {
-#pragma unroll
-                    for (int w = 0; w < 3; w++) acc[r] += *reinterpret_cast<const v4f *>(&sums[w][r][lane * 4]);
-                    const uint32_t rank = r0 + r * 16 + 4 * q;
-                    if (rank < R) *reinterpret_cast<v4f *>(part + ((size_t)blockIdx.y * N + n) * R + rank) = acc[r];
-                }
-            }
-            __syncthreads();
         }
+        __syncthreads();
     });
 }
 
@@ -527,14 +526,15 @@ __global__ __launch_bounds__(256, 3) void adapter_expand_tile(half_t *__restrict
 
 // How an adapter call is cut.  Tiles of 64 rows where there are many: with every batch row a request of its own, 4096 x 4096, rank 16, tiles of 16 / 64 take 36 / 38 us of 192 rows, 40 / 39 of
 // 256, 52 / 43 of 384 (with eight runs of rows 30 / 37 of 256 and 46 / 46 of 768); 10240 x 8192, rank 64, where a row's ranks weigh more, 53 / 57 of 96, 66 / 62 of 128, 94 / 80 of 256.
-// K ranges of 256 columns at least that fill the chip, and passes of a tile side by side as far as that leaves no crowd of workgroups that find nothing to do (a round of them takes 2 us).
+// K ranges of 256 columns at least that fill the chip (of 512 in small tiles above rank 64, whose sums the second kernel has to add up: 8192 x 8192, rank 128, us of 1 / 64 rows 24.5 / 59
+// -> 23.8 / 53; at rank 64 4096 x 4096, 8 rows, 17.9 -> 19.2), and passes of a tile side by side as far as that leaves no crowd of workgroups that find nothing to do (a round of them takes 2 us).
 struct AdapterPlan { uint32_t rows, tiles, ranges, shrink_side, expand_side; };
 inline AdapterPlan adapter_plan(size_t M, size_t N, size_t K, size_t R, size_t slots)
 {
     AdapterPlan p;
     p.rows = N > (R > 32 ? 112u : 256u) ? 64 : 16;
     p.tiles = (uint32_t)((N + p.rows - 1) / p.rows);
-    const size_t fill = 512, most = K / 256 > 0 ? K / 256 : 1, want = (fill + p.tiles - 1) / p.tiles;
+    const size_t fill = 512, cols = p.rows == 16 && R > 64 ? 512 : 256, most = K / cols > 0 ? K / cols : 1, want = (fill + p.tiles - 1) / p.tiles;
     p.ranges = (uint32_t)(want < most ? want : most);
     const size_t rows = N < p.rows ? N : p.rows, passes = rows < slots ? rows : slots;
     auto         side = [&](size_t workgroups, size_t room) { return (uint32_t)(workgroups * passes <= room ? passes : workgroups < room ? room / workgroups : 1); };
@@ -559,8 +559,12 @@ int adapter_ranks_of(hipStream_t st, const AdapterPlan &p, float *part, const vo
 {
     auto go = [&](auto rt_c) {
         constexpr int RT = decltype(rt_c)::value;
-        hipLaunchKernelGGL(p.rows == 64 ? adapter_shrink_tile<RT> : adapter_shrink<RT>, dim3(p.tiles, p.ranges, p.shrink_side), dim3(256), 0, st, part, static_cast<const half_t *>(x),
-                           static_cast<const half_t *>(A), index, (uint32_t)N, (uint32_t)K, (uint32_t)R, (uint32_t)slots);
+        if (p.rows == 64)
+            hipLaunchKernelGGL(adapter_shrink_tile<RT>, dim3(p.tiles, p.ranges, p.shrink_side), dim3(256), 0, st, part, static_cast<const half_t *>(x), static_cast<const half_t *>(A), index,
+                               (uint32_t)N, (uint32_t)K, (uint32_t)R, (uint32_t)slots);
+        else
+            hipLaunchKernelGGL(adapter_shrink<RT>, dim3(p.tiles, p.ranges * (uint32_t)((R + RT * 16 - 1) / (RT * 16)), p.shrink_side), dim3(256), 0, st, part, static_cast<const half_t *>(x),
+                               static_cast<const half_t *>(A), index, (uint32_t)N, (uint32_t)K, (uint32_t)R, (uint32_t)slots, p.ranges);
         return (int)hipGetLastError();
     };
     return R <= 16 ? go(std::integral_constant<int, 1>{}) : R <= 32 ? go(std::integral_constant<int, 2>{}) : go(std::integral_constant<int, 4>{});
