@@ -349,13 +349,14 @@ __global__ __launch_bounds__(256) void adapter_ranks(half_t *__restrict__ ranks,
 // expand: y[n, m] += factor[n] * sum over r of t[n, r] * B[a, m, r].  grid = (tiles, blocks of 256 outputs, passes side by side); 64 outputs a wavefront.
 //
 // adapter_expand, for few rows: tiles of sixteen; forms t in LDS from the ranges' sums, which saves a launch and is bound by the latency of it (4096 outputs, 32 rows of 32 requests,
-// rank 16: 7.5 us).
+// rank 16: 7.5 us).  The sums are held as two halfs, 22 bits: with few rows of few ranks a rounding of one of them is a rounding of the whole row, and two more MFMAs a step are not to be
+// seen in the time.
 template <int RT>
 __global__ __launch_bounds__(256) void adapter_expand(half_t *__restrict__ y, const float *__restrict__ part, const half_t *__restrict__ B, const float *__restrict__ scaling,
                                                       const int *__restrict__ index, uint32_t M, uint32_t N, uint32_t R, uint32_t slots, uint32_t ranges)
 {
     constexpr int kRow = 256 + 8; // halfs
-    __shared__ __attribute__((aligned(16))) half_t t16[16 * kRow];
+    __shared__ __attribute__((aligned(16))) half_t t16[2][16 * kRow]; // what fp16 holds of a sum, and of the rest
     __shared__ float                               row_factor[16];
     const int      lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, q = lane >> 4;
     const int      mine = adapter_of<16>(index, blockIdx.x, N, slots), here = __shfl(mine, col);
@@ -407,7 +408,13 @@ __global__ __launch_bounds__(256) void adapter_expand(half_t *__restrict__ y, co
             const int e = common_exponent<16>(v);
 #pragma unroll
             for (int j = 0; j < 16; j++)
-                if (c + 16 * j < (int)Rp) t16[i * kRow + c + 16 * j] = (half_t)ldexpf(v[j], -e);
+                if (c + 16 * j < (int)Rp) {
+                    const float  sum = ldexpf(v[j], -e);
+                    const half_t most = (half_t)sum;
+                    const float  rest = sum - (float)most;
+                    t16[0][i * kRow + c + 16 * j] = most;
+                    t16[1][i * kRow + c + 16 * j] = fabsf(rest) < 64.f ? (half_t)rest : (half_t)0.f; // (no rest to an infinity or a NaN)
+                }
             if (c == 0) row_factor[i] = ldexpf(1.f, e) * scaling[a];
             __syncthreads();
         }
@@ -415,9 +422,11 @@ __global__ __launch_bounds__(256) void adapter_expand(half_t *__restrict__ y, co
 #pragma unroll
         for (int o = 0; o < 4; o++) acc[o] = (v4f){ 0.f, 0.f, 0.f, 0.f };
         for (uint32_t r = 8 * q; r < R + 8 * q; r += 32) { // (the same number of steps in every lane)
-            const v8h t = *reinterpret_cast<const v8h *>(t16 + col * kRow + r);
+            const v8h t = *reinterpret_cast<const v8h *>(t16[0] + col * kRow + r), rest = *reinterpret_cast<const v8h *>(t16[1] + col * kRow + r);
 #pragma unroll
             for (int o = 0; o < 4; o++) acc[o] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[o], t, acc[o], 0, 0, 0);
+#pragma unroll
+            for (int o = 0; o < 4; o++) acc[o] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[o], rest, acc[o], 0, 0, 0);
             load_w(r + 32);
         }
         if (here == a) {
