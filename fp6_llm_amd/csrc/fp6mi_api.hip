@@ -604,8 +604,6 @@ int linear_native(const fp6mi::FormatOps &ops, hipStream_t st, const void *W, co
 
 namespace fp6mi {
 
-int current_cus() { return current_device_cus(); }
-
 LaunchCfg linear_shape(int E, int Mb, size_t M, size_t N, size_t K, int splitK, bool grouped) { return final_cfg(ops_for(E, Mb)->bits, M, N, K, splitK, grouped, current_device_cus()); }
 
 int run_linear(int E, int Mb, void *stream, const void *W, const void *sc, const void *gexp, const void *bias, const void *B, void *C, size_t M, size_t N, size_t K, float *ws, int splitK,

@@ -48,7 +48,6 @@ inline const BlockOps *block_ops_for(int E, int Mbits)
 
 // fp6mi_api.hip: parts of fp6mi_linear_native for the operators around it (fp6mi_ops.hip)
 int  check_linear(int E, int Mbits, const void *W, const void *sc, const void *gexp, const void *bias, const void *B, const void *C, size_t M, size_t N, size_t K, const float *ws, int splitK);
-int  current_cus();
 // the launch shape of fp6mi_linear_native
 LaunchCfg linear_shape(int E, int Mbits, size_t M, size_t N, size_t K, int splitK, bool grouped);
 // the GEMM by the shape that fp6mi_linear_native takes; partial_only: with a split, the partial sums alone, [splitK][N][M] floats in ws (C is not touched)
