@@ -625,7 +625,7 @@ template <int FM, bool GS> int gated_cfg(const LaunchCfg &c, const GatedArgs &a)
 #define FP6MI_CASE(NT, RT, WV) \
     if (c.kind == 0 && c.nt == NT && c.rt == RT && c.wk == WV) return launch_gated_stream<FM, GS, NT, RT, WV>(a);
     FP6MI_CASE(1, 2, 4) FP6MI_CASE(1, 2, 8) FP6MI_CASE(1, 2, 16) FP6MI_CASE(1, 4, 4) FP6MI_CASE(1, 4, 8) FP6MI_CASE(1, 6, 4) FP6MI_CASE(1, 6, 8) FP6MI_CASE(1, 8, 4)
-    FP6MI_CASE(2, 2, 4) FP6MI_CASE(2, 2, 8) FP6MI_CASE(2, 4, 4) FP6MI_CASE(2, 4, 8) FP6MI_CASE(2, 6, 4) FP6MI_CASE(2, 8, 4)
+    FP6MI_CASE(2, 2, 4) FP6MI_CASE(2, 4, 4) FP6MI_CASE(2, 4, 8) FP6MI_CASE(2, 6, 4) FP6MI_CASE(2, 8, 4)
 #undef FP6MI_CASE
 #define FP6MI_CASE(NT, WR, WK) \
     if (c.kind == 1 && c.nt == NT && c.wr == WR && c.wk == WK) return launch_gated_tile<FM, GS, NT, 2, WR, WK>(a);

@@ -564,3 +564,72 @@ def test_refusals_of_the_python_functions():
         fp6.linear_input_grad_native(5, 2, dy, w.native, w.scales, 320)
     with pytest.raises(fp6.Fp6miError):   # a view that starts between two 16-byte boundaries
         gated(x=randn(1, 6 * 320 + 4)[4:].view(6, 320))
+
+
+# ---- every launch shape ----
+GATED_SHAPES = [  # one problem for every launch shape of the gated block, with and without group exponents: E, M, OC, IC, N, activation, group exponents, bias
+    (3, 2, 256, 576, 1, "silu", False, True), (2, 2, 256, 576, 1, "gelu", True, True), (2, 3, 256, 1088, 1, "gelu_tanh", False, False),
+    (2, 1, 256, 1088, 1, "silu", True, False), (3, 2, 256, 2112, 1, "gelu", False, True), (2, 2, 256, 2112, 1, "gelu_tanh", True, True),
+    (2, 3, 8448, 576, 5, "silu", False, False), (2, 1, 8448, 576, 5, "gelu", True, False), (3, 2, 256, 1088, 513, "gelu_tanh", False, True),
+    (2, 2, 256, 1088, 513, "silu", True, True), (2, 3, 16640, 576, 5, "gelu", False, False), (2, 1, 16640, 576, 5, "gelu_tanh", True, False),
+    (3, 2, 4352, 1408, 49, "silu", False, True), (2, 2, 4352, 1408, 49, "gelu", True, True), (2, 3, 24832, 576, 5, "gelu_tanh", False, False),
+    (2, 1, 24832, 576, 5, "silu", True, False), (3, 2, 6400, 5312, 17, "gelu", False, True), (2, 3, 6400, 5312, 17, "gelu_tanh", True, True),
+    (3, 2, 12544, 1408, 25, "silu", False, False), (2, 3, 12544, 1408, 25, "gelu", True, False), (2, 2, 5632, 1408, 33, "gelu_tanh", False, True),
+    (3, 2, 5632, 1408, 33, "silu", True, True), (2, 1, 17408, 1728, 17, "gelu", False, False), (2, 2, 17408, 1728, 17, "gelu_tanh", True, False),
+    (2, 3, 13312, 6272, 33, "silu", False, True), (3, 2, 13312, 6272, 33, "gelu", True, True), (2, 1, 768, 576, 1345, "gelu_tanh", False, False),
+    (2, 2, 768, 576, 1345, "silu", True, False), (2, 1, 256, 576, 2049, "gelu", False, True), (2, 2, 256, 576, 2049, "gelu_tanh", True, True),
+    (2, 3, 256, 832, 17, "silu", False, False), (2, 1, 256, 832, 17, "gelu", True, False), (2, 1, 15360, 2752, 81, "gelu_tanh", False, True),
+    (3, 2, 33280, 2112, 33, "silu", True, True), (2, 3, 8192, 1408, 193, "gelu", False, False), (3, 2, 8192, 1408, 193, "gelu_tanh", True, False),
+    (2, 2, 22016, 576, 65, "silu", False, True), (2, 3, 22016, 576, 65, "gelu", True, True), (2, 2, 22016, 1408, 129, "gelu_tanh", False, False),
+    (2, 1, 22016, 1408, 129, "silu", True, False), (3, 2, 22016, 1408, 161, "gelu", False, True), (2, 2, 22016, 1408, 161, "gelu_tanh", True, True),
+    (2, 1, 768, 1728, 513, "silu", False, False), (2, 2, 1280, 1408, 385, "gelu", True, False), (2, 3, 5632, 1408, 65, "gelu_tanh", False, True),
+    (3, 2, 5632, 1408, 65, "silu", True, True), (2, 3, 1280, 1408, 385, "gelu", False, False), (2, 1, 1280, 1408, 385, "gelu_tanh", True, False),
+    (3, 2, 2304, 1408, 321, "silu", False, True), (2, 2, 2304, 1408, 321, "gelu", True, True), (2, 3, 5632, 1408, 321, "gelu_tanh", False, False),
+    (2, 2, 4864, 1408, 391, "silu", True, False), (3, 2, 768, 1088, 2689, "gelu", False, True), (2, 3, 8448, 1088, 193, "gelu_tanh", True, True),
+    (2, 1, 16640, 1408, 65, "silu", False, False), (3, 2, 6144, 1408, 257, "gelu", True, False), (2, 1, 22016, 1088, 129, "gelu_tanh", False, True),
+    (2, 2, 22016, 1088, 129, "silu", True, True), (2, 3, 11008, 576, 129, "gelu", False, False), (2, 1, 11008, 576, 129, "gelu_tanh", True, False),
+    (3, 2, 16640, 1408, 81, "silu", False, True), (2, 2, 16640, 1408, 81, "gelu", True, True), (2, 3, 22016, 576, 129, "gelu_tanh", False, False),
+    (2, 1, 22016, 576, 129, "silu", True, False), (2, 2, 1792, 1088, 2881, "gelu", False, True), (2, 1, 1792, 1088, 2881, "gelu_tanh", True, True),
+    (3, 2, 8192, 1088, 385, "silu", False, False), (2, 3, 8192, 1088, 385, "gelu", True, False), (2, 1, 33024, 1344, 97, "gelu_tanh", False, True),
+    (3, 2, 7424, 1088, 769, "silu", True, True), (2, 2, 16640, 576, 97, "gelu", False, False), (2, 3, 16640, 576, 97, "gelu_tanh", True, False),
+    (3, 2, 43776, 576, 65, "silu", False, True), (2, 2, 43776, 576, 65, "gelu", True, True), (2, 3, 33024, 576, 97, "gelu_tanh", False, False),
+    (3, 2, 33024, 576, 97, "silu", True, False)]
+
+
+def gated_shape(E, M, OC, IC, N, groups):
+    import ctypes
+    shape = (ctypes.c_int * 5)()
+    assert _lib.lib().fp6mi_query_gated_launch(E, M, OC, N, IC, int(groups), shape) == 0
+    return tuple(shape)
+
+
+def test_gated_shapes_are_all_there_are():
+    """The problems above reach every launch shape that sizes from the smallest to the largest ask for, and the kernels are compiled for no other."""
+    reached = {(gated_shape(E, M, OC, IC, N, groups), groups) for E, M, OC, IC, N, _, groups, _ in GATED_SHAPES}
+    asked = set()
+    for E, M in FORMATS:
+        for OC in (256, 768, 1280, 2304, 4096, 5632, 6400, 8192, 12544, 13312, 16640, 17408, 22016, 28672, 33024, 43776, 57344):
+            for IC in (64, 576, 1088, 1408, 1536, 2752, 4096, 5312, 6272, 8192, 11008, 28672):
+                for N in (1, 2, 5, 8, 9, 16, 17, 24, 25, 32, 33, 40, 49, 64, 65, 72, 81, 96, 97, 112, 129, 145, 161, 193, 225, 257, 321, 385, 513, 769, 1024, 1345, 2048, 2049, 2689, 2881, 4096):
+                    asked |= {(gated_shape(E, M, OC, IC, N, groups), groups) for groups in (False, True)}
+    assert reached == asked and len(GATED_SHAPES) == len(reached)
+    import os
+    import re
+    with open(os.path.join(os.path.dirname(fp6.__file__), "csrc", "fp6mi_block.hip")) as f:
+        text = f.read()
+    instances = text[text.index("int gated_cfg("):text.index("int op_gated(")]
+    assert len(re.findall(r"FP6MI_CASE\(\d", instances)) == len({shape for shape, _ in reached})
+
+
+@gpu
+@pytest.mark.parametrize("E,M,OC,IC,N,act,groups,bias", GATED_SHAPES, ids=lambda v: str(v))
+def test_gated_block_in_every_shape(E, M, OC, IC, N, act, groups, bias):
+    w = Weight(OC + IC + N, E, M, OC, IC, groups)
+    x, b = randn(N, N, IC), randn(N + 1, OC, scale=0.3) if bias else None
+    y, err, h, tol = gated64(w, x, b, act)
+    buf, pre = torch.full((N + 2, OC // 2), 7.0, dtype=torch.float16, device=DEV), torch.full((N + 2, OC), 7.0, device=DEV)
+    fp6.gated_forward_native(E, M, x, w.native, w.scales, OC, act, out=buf[:N], preact=pre[:N], group_exps=w.exps, bias=b)
+    within(buf[:N], h, tol, "out")
+    within(pre[:N], y, err, "preact")
+    assert (buf[N:] == 7.0).all() and (pre[N:] == 7.0).all()
+    assert torch.equal(fp6.gated_forward_native(E, M, x, w.native, w.scales, OC, act, group_exps=w.exps, bias=b), buf[:N])
