@@ -633,3 +633,33 @@ def test_gated_block_in_every_shape(E, M, OC, IC, N, act, groups, bias):
     within(pre[:N], y, err, "preact")
     assert (buf[N:] == 7.0).all() and (pre[N:] == 7.0).all()
     assert torch.equal(fp6.gated_forward_native(E, M, x, w.native, w.scales, OC, act, group_exps=w.exps, bias=b), buf[:N])
+
+
+BACKWARD = [  # E, M, OC, IC, N, splits, group exponents: every kernel of the input gradient behind gated_grad, which hands it products with the mantissas
+    (3, 2, 512, 320, 9, 1, True), (2, 1, 1024, 448, 13, 3, False), (2, 2, 512, 576, 27, 2, False), (2, 3, 768, 320, 31, 1, True), (2, 2, 1024, 320, 130, 1, False), (3, 2, 512, 704, 99, 3, True),
+    (3, 2, 256, 4928, 1537, 1, True), (2, 1, 512, 7232, 258, 3, False), (2, 3, 512, 6528, 130, 5, True), (2, 2, 256, 6528, 521, 2, False),
+    (2, 2, 512, 7232, 1558, 1, True), (2, 3, 512, 7296, 391, 3, False), (3, 2, 512, 6464, 194, 5, False), (2, 1, 256, 6464, 791, 2, True)]
+
+
+def test_gradient_kernels_behind_the_block():
+    rows = {(_lib.lib().fp6mi_query_grad_launch(E, M, OC, N, IC, s), s > 1, groups) for E, M, OC, IC, N, s, groups in BACKWARD}
+    assert {r for r, _, _ in rows} == {16, 32, 128, 192, 256}
+    assert {r[:2] for r in rows} == {(r, s) for r in (16, 32, 128, 192, 256) for s in (False, True)}
+    assert {r[::2] for r in rows} == {(r, g) for r in (16, 32, 128, 192, 256) for g in (False, True)}
+
+
+@gpu
+@pytest.mark.parametrize("E,M,OC,IC,N,splits,groups", BACKWARD)
+def test_gated_block_backward_by_every_kernel(E, M, OC, IC, N, splits, groups):
+    w = Weight(OC + IC + N, E, M, OC, IC, groups)
+    dh, pre = randn(3, N, OC // 2, scale=0.1), randn(4, N, OC).float()
+    buf = torch.full((N + 2, IC), 7.0, dtype=torch.float16, device=DEV)
+    dx, dp = fp6.gated_backward_native(E, M, dh, pre, w.native, w.scales, IC, "gelu", splitK=splits, grad_in=buf[:N], group_exps=w.exps)
+    (g, u), dd = halves(d(pre)), d(dh)
+    want = pairs(dd * u * slope64("gelu", g), dd * act64("gelu", g))
+    slack = 2.0 ** -18 * pairs(dd.abs() * u.abs() * (1 + g.abs()), dd.abs() * g.abs())   # (slopes and activations as in the test above)
+    within(dp, want, HALF * want.abs() + slack + TINY, "grad_preact")
+    # a product of dp with a mantissa (1/2 and up: below the normal halfs half a step is 2 * TINY of the weight) is rounded once; its float32 value is off by the slack and two roundings more
+    dx64, mag = want @ w.w, want.abs() @ w.w.abs()
+    within(dx, dx64, (sum_error(OC + 2) + HALF) * mag + (slack + 2 * TINY) @ w.w.abs() * (1 + HALF) + HALF * dx64.abs() + TINY, "grad_in")
+    assert (buf[N:] == 7.0).all()
