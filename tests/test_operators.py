@@ -663,3 +663,28 @@ def test_gated_block_backward_by_every_kernel(E, M, OC, IC, N, splits, groups):
     dx64, mag = want @ w.w, want.abs() @ w.w.abs()
     within(dx, dx64, (sum_error(OC + 2) + HALF) * mag + (slack + 2 * TINY) @ w.w.abs() * (1 + HALF) + HALF * dx64.abs() + TINY, "grad_in")
     assert (buf[N:] == 7.0).all()
+
+
+@gpu
+@pytest.mark.parametrize("N,R", [(1, 8), (1, 72), (16, 16), (47, 40), (112, 72), (256, 32)])
+def test_rank_sums_of_few_rows_are_held_as_two_halfs(N, R):
+    """Beside a layer of zeros the output is the adapter's part alone, rounded once; of a row with one value a rank sum is one product, exact in float32, and so are its halfs' products with b.  Tiles
+    of sixteen rows hold it to 2^-22 of itself (two halfs), or 2^-39 of the row's largest (half a step below the normal halfs, where that one is from 2^14 to 2^15).  One half would be off by more than
+    that allows."""
+    OC, IC, slots = 256, 64, 3
+    w = Weight(5, 3, 2, OC, IC)
+    a, b, s = bank(6, slots, R, OC, IC)
+    x, index = torch.zeros(N, IC, dtype=torch.float16, device=DEV), torch.arange(N, dtype=torch.int32) % slots
+    x[torch.arange(N), torch.arange(N) * 7 % IC] = randn(N, N)
+    got = fp6.adapter_forward_native(3, 2, x, w.native, torch.zeros_like(w.scales), OC, a, b, s, index.to(DEV))
+    i = index.long()
+    t = torch.stack([d(a)[i[n]] @ d(x)[n] for n in range(N)])
+    top = t.abs().amax(1, keepdim=True)
+    et = 2.0 ** -22 * t.abs() + 2.0 ** -39 * top
+    part = lambda m, v: torch.stack([m[i[n]] @ v[n] for n in range(N)]) * d(s)[i][:, None]   # noqa: E731
+    want = part(d(b), t)
+    slack = part(d(b).abs(), et + sum_error(2 * R + 2) * t.abs())
+    within(got, want, slack * (1 + HALF) + HALF * want.abs() + TINY)
+    power = torch.exp2(torch.floor(torch.log2(top)) - 14)
+    one = part(d(b), (t / power).half().double() * power)   # (what one half a sum would give: the bound tells them apart)
+    assert ((one - want).abs() > 2 * slack).any()
