@@ -688,3 +688,28 @@ def test_rank_sums_of_few_rows_are_held_as_two_halfs(N, R):
     power = torch.exp2(torch.floor(torch.log2(top)) - 14)
     one = part(d(b), (t / power).half().double() * power)   # (what one half a sum would give: the bound tells them apart)
     assert ((one - want).abs() > 2 * slack).any()
+
+
+@gpu
+@pytest.mark.parametrize("N", [3, 50, 300])
+def test_calls_without_the_extension(N, monkeypatch):
+    """ctypes and the extension launch the same kernels with the same splits, and refuse the same calls."""
+    assert fp6._ext is not None
+    w = Weight(3, 2, 2, 512, 1344, True)
+    x, dy, dh, c = randn(1, N, 1344), randn(2, N, 512), randn(3, N, 256), randn(4, 512)
+    a, b, s = bank(3, 3, 16, 512, 1344)
+    index = (torch.arange(N, device=DEV) % 4 - 1).int()
+    fmt, got = (2, 2), []
+    for ext in (fp6._ext, None):
+        monkeypatch.setattr(fp6, "_ext", ext)
+        for split in (None, 2):
+            pre = torch.empty(N, 512, device=DEV)
+            got.append([fp6.gated_forward_native(*fmt, x, w.native, w.scales, 512, "gelu", splitK=split, preact=pre, group_exps=w.exps, bias=c), pre,
+                        *fp6.gated_backward_native(*fmt, dh, pre, w.native, w.scales, 1344, "gelu", splitK=split, group_exps=w.exps),
+                        fp6.linear_input_grad_native(*fmt, dy, w.native, w.scales, 1344, splitK=split, group_exps=w.exps),
+                        fp6.adapter_forward_native(*fmt, x, w.native, w.scales, 512, a, b, s, index, splitK=split, group_exps=w.exps, bias=c)])
+        assert fp6.gated_backward_native(*fmt, dh, pre, w.native, w.scales, 1344, grad_preact=False, group_exps=w.exps)[1] is None
+    for ours, theirs in zip(got[:2], got[2:]):
+        assert all(torch.equal(p, q) for p, q in zip(ours, theirs))
+    if N == 3:   # (without the extension from here on)
+        test_refusals_of_the_python_functions()
