@@ -49,6 +49,12 @@ def _rows_of(x, features):
     return x2 if x2.dtype == torch.float16 else x2.half()
 
 
+def _gradient(grad):
+    """What autograd hands to a backward pass, as the kernels read it: float16 from a 16-byte boundary on.  (Of a part of a concatenation it is a view into the whole one's, at any place.)"""
+    grad = grad.half()
+    return grad.clone() if grad.is_contiguous() and grad.data_ptr() % 16 else grad
+
+
 class _InputGradient(torch.autograd.Function):
     """FPxLinear.forward, and the product with the weights the other way round.  What a backward pass needs is the weights alone."""
 
@@ -62,7 +68,7 @@ class _InputGradient(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
         weight, scales, exps = ctx.saved_tensors
-        return ops.linear_input_grad_native(*ctx.format, grad.half(), weight, scales, ctx.in_features, group_exps=exps), None
+        return ops.linear_input_grad_native(*ctx.format, _gradient(grad), weight, scales, ctx.in_features, group_exps=exps), None
 
 
 class _GatedBlock(torch.autograd.Function):
@@ -78,7 +84,7 @@ class _GatedBlock(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
         preact, weight, scales, exps = ctx.saved_tensors
-        return ops.gated_backward_native(*ctx.format, grad, preact, weight, scales, ctx.in_features, ctx.activation, grad_preact=False, group_exps=exps)[0], None
+        return ops.gated_backward_native(*ctx.format, _gradient(grad), preact, weight, scales, ctx.in_features, ctx.activation, grad_preact=False, group_exps=exps)[0], None
 
 
 _CROSSOVER, _CROSSOVER_LIBRARY = 32768, 3072   # FPxLinear.PREFILL_CROSSOVER as it is shipped, and the one without the wide tiles

@@ -288,3 +288,18 @@ def test_a_capture_beside_an_eager_graph_of_the_same_leaf_is_refused():
     assert torch.equal(y, eager[0]) and (buf == 1).all()
     eager[0].sum().backward()
     assert leaf.grad is not None
+
+
+@gpu
+@pytest.mark.parametrize("N", [1, 5, 40])
+def test_gradients_that_start_between_two_16_byte_boundaries(N):
+    """The gradient of a concatenation's later part is a view into the whole one's, at whatever place the part has."""
+    mg, md = block(Weight(2, 2, 2, 512, 320, True)), layer(Weight(3, 3, 2, 512, 320))
+    md.input_gradient = True
+    for m in (mg, md):
+        x, dy = randn(1, N, 320), randn(2, N, m.out_features, scale=0.1)
+        leaf = x.clone().requires_grad_()
+        m(leaf).backward(dy)
+        other, first = x.clone().requires_grad_(), torch.ones(1, dtype=torch.float16, device=DEV, requires_grad=True)
+        torch.cat([first, m(other).flatten()]).backward(torch.cat([first.detach(), dy.flatten()]))
+        assert torch.equal(other.grad, leaf.grad) and first.grad == 1
