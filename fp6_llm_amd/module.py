@@ -305,7 +305,8 @@ class FPxGatedLinear(torch.nn.Module):
     (ops.gate_up_pairs).  Differentiable in x; the weights are buffers and have no gradient."""
 
     def __init__(self, in_features, out_features, exponent=3, mantissa=2, activation="silu", bias=None, split_k=None, group_scales=False):
-        """out_features: columns of y, the rows of gate and of up.  activation: "silu", "gelu" or "gelu_tanh".  bias: float16 [2 * out_features] in pair order."""
+        """out_features: columns of y, the rows of gate and of up.  activation: "silu", "gelu" or "gelu_tanh".  bias: float16 [2 * out_features] in pair order.  split_k: number of
+        pieces of K for less than 3072 rows, None for the heuristic's choice."""
         super().__init__()
         if out_features < 128 or out_features % 128 or in_features < 64 or in_features % 64:
             raise ValueError("FPxGatedLinear needs out_features %% 128 == 0 and in_features %% 64 == 0")
@@ -344,7 +345,8 @@ class FPxGatedLinear(torch.nn.Module):
         return m
 
     def _values(self, x2, preact=None):
-        return ops.gated_forward_native(self.exponent, self.mantissa, x2, self.weight_native, self.scales, 2 * self.out_features, self.activation, self.split_k, preact=preact,
+        split = self.split_k or None if x2.shape[0] < _CROSSOVER_LIBRARY else None   # (as in FPxLinear: the partial sums of a long prompt would take gigabytes)
+        return ops.gated_forward_native(self.exponent, self.mantissa, x2, self.weight_native, self.scales, 2 * self.out_features, self.activation, split, preact=preact,
                                         group_exps=self.group_exps, bias=self.bias)
 
     def forward(self, x):

@@ -303,3 +303,26 @@ def test_gradients_that_start_between_two_16_byte_boundaries(N):
         other, first = x.clone().requires_grad_(), torch.ones(1, dtype=torch.float16, device=DEV, requires_grad=True)
         torch.cat([first, m(other).flatten()]).backward(torch.cat([first.detach(), dy.flatten()]))
         assert torch.equal(other.grad, leaf.grad) and first.grad == 1
+
+
+def splits_asked_for(monkeypatch, name):
+    """The splitK that a module hands to a function of ops, call by call (its result is zeros of the right shape)."""
+    asked = []
+
+    def stand_in(E, M, x, native, scales, OC, *args, **kw):
+        asked.append(kw.get("splitK", args[0] if name == "linear_forward_native" else args[1] if name == "gated_forward_native" else args[4]))
+        return torch.zeros(x.shape[0], OC // 2 if name == "gated_forward_native" else OC, dtype=torch.float16)
+    from fp6_llm_amd import module
+    monkeypatch.setattr(module if name == "linear_forward_native" else module.ops, name, stand_in)
+    return asked
+
+
+def test_split_of_a_gated_block_is_for_batches_below_a_long_prompt(monkeypatch):
+    asked = splits_asked_for(monkeypatch, "gated_forward_native")
+    m = FPxGatedLinear(64, 128, split_k=4)
+    for n in (1, 3071, 3072, 9000):
+        m(torch.zeros(n, 64).half())
+    m(torch.zeros(1536, 2, 64).half())
+    for none in (None, 0):
+        FPxGatedLinear(64, 128, split_k=none)(torch.zeros(1, 64).half())
+    assert asked == [4, 4, None, None, None, None, None]
