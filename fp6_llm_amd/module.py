@@ -255,12 +255,14 @@ class FPxLinear(torch.nn.Module):
         x2 = _rows_of(x, self.in_features)
         if index.numel() != x2.shape[0] or (index.dim() != 1 and index.shape != x.shape[:-1]):
             raise ValueError("index must name an adapter for each of the %d rows, got %s" % (x2.shape[0], list(index.shape)))
+        split = None if self._auto and x2.shape[0] >= _CROSSOVER_LIBRARY else self.split_k or None   # (as in forward: rows without an adapter have the layer's own bits)
         y = ops.adapter_forward_native(self.exponent, self.mantissa, x2, self.weight_native, self.scales, self.out_features, adapters.lora_a, adapters.lora_b, adapters.scaling,
-                                       index.reshape(-1).contiguous(), None, group_exps=self.group_exps, bias=self.bias)
+                                       index.reshape(-1).contiguous(), split, group_exps=self.group_exps, bias=self.bias)
         return y.reshape(*x.shape[:-1], self.out_features)
 
     def forward(self, x, adapters=None, index=None):
-        """adapters: a LowRankAdapters of this layer's shape, with index, int32, the slot of every row of x (-1: none)."""
+        """adapters: a LowRankAdapters of this layer's shape, with index, int32, the slot of every row of x (-1: none).  With adapters the kernels take every batch, whatever
+        dequant_above says."""
         if adapters is not None or index is not None:
             return self._with_adapters(x, adapters, index)
         # (two reshapes to the shapes at hand take 0.7 us each; a trace, whose sizes are no plain numbers, keeps them)

@@ -326,3 +326,16 @@ def test_split_of_a_gated_block_is_for_batches_below_a_long_prompt(monkeypatch):
     for none in (None, 0):
         FPxGatedLinear(64, 128, split_k=none)(torch.zeros(1, 64).half())
     assert asked == [4, 4, None, None, None, None, None]
+
+
+def test_split_of_a_layer_holds_with_adapters(monkeypatch):
+    asked = splits_asked_for(monkeypatch, "adapter_forward_native")
+    plain = splits_asked_for(monkeypatch, "linear_forward_native")
+    ad = LowRankAdapters(64, 256, 1, 8)
+    for kw in (dict(split_k=2), dict(split_k=2, dequant_above=None), dict()):
+        m = FPxLinear(64, 256, **kw)
+        for n in (1, 3071, 3072):
+            x, index = torch.zeros(n, 64).half(), torch.zeros(n, dtype=torch.int32)
+            m(x, ad, index), m(x)
+    assert [s for s in asked[:6]] == [2, 2, None, 2, 2, 2] and asked[6:] == [None] * 3
+    assert [p == (a or p) for a, p in zip(asked, plain)] == [True] * 9   # (None: the heuristic's, which the layer asks itself)
