@@ -256,8 +256,12 @@ class FPxLinear(torch.nn.Module):
         if index.numel() != x2.shape[0] or (index.dim() != 1 and index.shape != x.shape[:-1]):
             raise ValueError("index must name an adapter for each of the %d rows, got %s" % (x2.shape[0], list(index.shape)))
         split = None if self._auto and x2.shape[0] >= _CROSSOVER_LIBRARY else self.split_k or None   # (as in forward: rows without an adapter have the layer's own bits)
+        bias = self.bias
+        fused = bias if bias is not None and self._bias_in_kernel(x2) else None
         y = ops.adapter_forward_native(self.exponent, self.mantissa, x2, self.weight_native, self.scales, self.out_features, adapters.lora_a, adapters.lora_b, adapters.scaling,
-                                       index.reshape(-1).contiguous(), split, group_exps=self.group_exps, bias=self.bias)
+                                       index.reshape(-1).contiguous(), split, group_exps=self.group_exps, bias=fused)
+        if bias is not fused:
+            y = y + bias
         return y.reshape(*x.shape[:-1], self.out_features)
 
     def forward(self, x, adapters=None, index=None):

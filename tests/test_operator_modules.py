@@ -339,3 +339,23 @@ def test_split_of_a_layer_holds_with_adapters(monkeypatch):
             m(x, ad, index), m(x)
     assert [s for s in asked[:6]] == [2, 2, None, 2, 2, 2] and asked[6:] == [None] * 3
     assert [p == (a or p) for a, p in zip(asked, plain)] == [True] * 9   # (None: the heuristic's, which the layer asks itself)
+
+
+@gpu
+@pytest.mark.parametrize("N", [3, 40])
+def test_a_layer_with_adapters_is_the_layer_where_there_are_none(N):
+    """Its split, and a bias that torch has to add (a float32 one, a strided one), are the same with adapters as without."""
+    w = Weight(1, 3, 2, 512, 1344)
+    ad, x, index = LowRankAdapters(1344, 512, 2, 8).to(DEV), randn(1, N, 1344), (torch.arange(N, device=DEV) % 3 - 1).int()
+    for i in range(2):
+        ad.set(i, randn(i, 8, 1344, scale=0.1), randn(i + 5, 512, 8))
+    biases = [None, randn(2, 512), randn(2, 512).float(), randn(2, 512, 2)[:, 0]]
+    for bias in biases:
+        for split in (None, 2, 3):
+            m = layer(w, bias)
+            m.split_k = split
+            y, alone = m(x, ad, index), m(x)
+            assert y.dtype == alone.dtype and torch.equal(y[index < 0], alone[index < 0]), (bias is None or bias.dtype, split)
+            want, tol = adapters64(w, x, bias, ad.lora_a, ad.lora_b, ad.scaling, index.cpu())
+            extra = 0 if bias is None else 2 * d(bias).abs()   # (a bias behind the product: what is rounded before it is of the outputs without it, and one rounding more)
+            within(y, want, tol + HALF * (want.abs() + extra) * (1 + 2 * HALF) + TINY)
