@@ -317,6 +317,8 @@ class FPxGatedLinear(torch.nn.Module):
         if out_features < 128 or out_features % 128 or in_features < 64 or in_features % 64:
             raise ValueError("FPxGatedLinear needs out_features %% 128 == 0 and in_features %% 64 == 0")
         ops._activation_code(activation)
+        if bias is not None and (bias.dtype != torch.float16 or bias.shape != (2 * out_features,)):   # (inside the activation, so no addition can follow)
+            raise ValueError("the bias of FPxGatedLinear must be float16 [%d], got %s %s" % (2 * out_features, str(bias.dtype).split(".")[-1], list(bias.shape)))
         self.in_features, self.out_features, self.exponent, self.mantissa = in_features, out_features, exponent, mantissa
         self.activation, self.split_k = activation, split_k
         self.register_buffer("weight_native", torch.zeros(native_bytes(exponent, mantissa, 2 * out_features, in_features) // 4, dtype=torch.int32))

@@ -359,3 +359,11 @@ def test_a_layer_with_adapters_is_the_layer_where_there_are_none(N):
             want, tol = adapters64(w, x, bias, ad.lora_a, ad.lora_b, ad.scaling, index.cpu())
             extra = 0 if bias is None else 2 * d(bias).abs()   # (a bias behind the product: what is rounded before it is of the outputs without it, and one rounding more)
             within(y, want, tol + HALF * (want.abs() + extra) * (1 + 2 * HALF) + TINY)
+
+
+def test_biases_that_a_block_cannot_take():
+    for bias in (torch.zeros(256), torch.zeros(256).bfloat16(), torch.zeros(128).half(), torch.zeros(1, 256).half()):
+        with pytest.raises(ValueError, match="bias"):
+            FPxGatedLinear(64, 128, bias=bias)
+    with pytest.raises(ValueError, match="bias"):
+        FPxGatedLinear.from_layers(*(FPxLinear(64, 256, bias=torch.zeros(256)) for _ in range(2)))
