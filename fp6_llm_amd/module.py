@@ -250,7 +250,7 @@ class FPxLinear(torch.nn.Module):
             raise ValueError("adapters must be a LowRankAdapters, with an index for every row")
         if (adapters.in_features, adapters.out_features) != (self.in_features, self.out_features):
             raise ValueError("the adapters are for %d -> %d features, the layer has %d -> %d" % (adapters.in_features, adapters.out_features, self.in_features, self.out_features))
-        if torch.is_grad_enabled() and (x.requires_grad or (self.bias is not None and self.bias.requires_grad)):
+        if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, self.bias, adapters.lora_a, adapters.lora_b, adapters.scaling)):
             raise ValueError("a product with adapters has no gradient: call it under torch.no_grad()")
         x2 = _rows_of(x, self.in_features)
         if index.numel() != x2.shape[0] or (index.dim() != 1 and index.shape != x.shape[:-1]):

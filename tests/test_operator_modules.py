@@ -367,3 +367,12 @@ def test_biases_that_a_block_cannot_take():
             FPxGatedLinear(64, 128, bias=bias)
     with pytest.raises(ValueError, match="bias"):
         FPxGatedLinear.from_layers(*(FPxLinear(64, 256, bias=torch.zeros(256)) for _ in range(2)))
+
+
+def test_adapters_that_require_a_gradient_are_refused():
+    m, x, index = FPxLinear(64, 256), torch.zeros(2, 64).half(), torch.zeros(2, dtype=torch.int32)
+    for name in ("lora_a", "lora_b", "scaling"):
+        ad = LowRankAdapters(64, 256, 1, 8)
+        getattr(ad, name).requires_grad_()
+        with pytest.raises(ValueError, match="no gradient"):
+            m(x, ad, index)
