@@ -41,8 +41,18 @@ def _differentiates(x):
     return True
 
 
+def _refuse_tangents(x):
+    """A tangent that x carries (forward mode), or a transform of torch.func that x is part of, would be passed by by a kernel that is handed x's address."""
+    if torch.compiler.is_compiling():   # (a call of a kernel ends the graph that is compiled)
+        return
+    wrapped = _peek_transform is None or (_peek_transform() is not None and torch._C._functorch.is_functorch_wrapped_tensor(x))
+    if wrapped or (getattr(torch.autograd.forward_ad, "_current_level", 0) >= 0 and torch.autograd.forward_ad.unpack_dual(x).tangent is not None):
+        raise RuntimeError("this operator has no part in forward mode or in a transform of torch.func")
+
+
 def _rows_of(x, features):
-    """x[..., features] as float16 rows."""
+    """x[..., features] as float16 rows, of which nothing but their values counts or a backward pass."""
+    _refuse_tangents(x)
     if x.dim() < 1 or x.shape[-1] != features:
         raise ValueError("need an input of %d features, got %s" % (features, list(x.shape)))
     x2 = x.reshape(-1, features)
@@ -95,7 +105,7 @@ class FPxLinear(torch.nn.Module):
     the layer is inference-only, like the kernels, but for input_gradient."""
 
     # True: an input that requires a gradient gets one, through the quantized weights (a frozen layer under trained adapters, prompts or layers below it).  Weights and bias have
-    # none.  False, as it has always been: the kernels are no part of an autograd graph.
+    # none, and an input with a tangent (forward mode) is refused.  False, as it has always been: the kernels are no part of an autograd graph.
     input_gradient = False
 
     # Batch size from which dequantize + FP16 library GEMM is no slower than the mixed-input kernels, measured through this module at 4096^2, 8192^2, 28672x8192,
@@ -276,6 +286,7 @@ class FPxLinear(torch.nn.Module):
         if x2.dtype != torch.float16:
             x2 = x2.half()
         if self.input_gradient and _differentiates(x):
+            _refuse_tangents(x)
             if self.bias is not None and self.bias.requires_grad:
                 raise ValueError("input_gradient is for a layer whose bias requires no gradient")
             y = _InputGradient.apply(x2, self)
@@ -289,6 +300,8 @@ class FPxLinear(torch.nn.Module):
             if self.bias is not None:
                 y = y + self.bias
             return y if plain else y.reshape(*shape[:-1], self.out_features)
+        if self.input_gradient:
+            _refuse_tangents(x)
         sk = self.split_k
         if not sk or (self._auto and n >= _CROSSOVER_LIBRARY):   # the heuristic's answer per batch size is remembered: the layer is called once per token
             # (split_k is for the batches up to 3071 rows; the partial sums of a long prompt would take gigabytes)

@@ -376,3 +376,43 @@ def test_adapters_that_require_a_gradient_are_refused():
         getattr(ad, name).requires_grad_()
         with pytest.raises(ValueError, match="no gradient"):
             m(x, ad, index)
+
+
+def no_part_of(x):
+    """The modules whose kernels have a part in autograd, and calls of theirs on x that a kernel would pass by."""
+    mg, ml, ad = FPxGatedLinear(64, 128), FPxLinear(64, 256), LowRankAdapters(64, 256, 1, 8)
+    mg, ml, ad = mg.to(x.device), ml.to(x.device), ad.to(x.device)
+    ml.input_gradient = True
+    index = torch.zeros(x.shape[0], dtype=torch.int32, device=x.device)
+    return [lambda t: mg(t), lambda t: ml(t), lambda t: ml(t, ad, index)]
+
+
+def forward_mode_is_refused(dev):
+    fw = torch.autograd.forward_ad
+    x, t = torch.ones(3, 64, device=dev).half(), torch.ones(3, 64, device=dev).half()
+    for call in no_part_of(x):
+        with fw.dual_level():
+            with pytest.raises(RuntimeError, match="forward mode"):
+                call(fw.make_dual(x, t))
+        with pytest.raises(RuntimeError, match="forward mode"):
+            torch.func.jvp(call, (x,), (t,))
+
+
+def test_forward_mode_is_refused():
+    forward_mode_is_refused("cpu")
+
+
+@gpu
+def test_forward_mode_is_refused_on_the_gpu():
+    forward_mode_is_refused(DEV)
+    # where no tangent comes in, the level that is open is nobody's business
+    x = torch.ones(3, 64, device=DEV).half()
+    for call in no_part_of(x)[:2]:
+        want = call(x)
+        with torch.autograd.forward_ad.dual_level():
+            assert torch.equal(call(x), want)
+    # a long prompt with a tangent goes through the library, as it does without input_gradient
+    m, x = FPxLinear(64, 256).to(DEV), torch.ones(3072, 64, device=DEV).half()
+    m.input_gradient = True
+    with torch.autograd.forward_ad.dual_level():
+        assert torch.autograd.forward_ad.unpack_dual(m(torch.autograd.forward_ad.make_dual(x, x))).tangent is not None
