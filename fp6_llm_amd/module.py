@@ -2,6 +2,7 @@
 on-disk container for them.  (The reference leaves both to the framework that embeds it -- DeepSpeed, README.md:19.)"""
 import json
 import struct
+import sys
 
 import numpy as np
 import torch
@@ -50,9 +51,17 @@ def _refuse_tangents(x):
         raise RuntimeError("this operator has no part in forward mode or in a transform of torch.func")
 
 
+def _refuse_traces():
+    """A trace records the output as it was allocated and not the kernel that fills it."""
+    proxies = sys.modules.get("torch.fx.experimental.proxy_tensor")   # (not loaded: no such trace is being made)
+    if not torch.compiler.is_compiling() and (torch.jit.is_tracing() or (proxies is not None and proxies.get_proxy_mode() is not None)):
+        raise RuntimeError("this operator cannot be recorded by a trace")
+
+
 def _rows_of(x, features):
     """x[..., features] as float16 rows, of which nothing but their values counts or a backward pass."""
     _refuse_tangents(x)
+    _refuse_traces()
     if x.dim() < 1 or x.shape[-1] != features:
         raise ValueError("need an input of %d features, got %s" % (features, list(x.shape)))
     x2 = x.reshape(-1, features)
@@ -287,6 +296,7 @@ class FPxLinear(torch.nn.Module):
             x2 = x2.half()
         if self.input_gradient and _differentiates(x):
             _refuse_tangents(x)
+            _refuse_traces()
             if self.bias is not None and self.bias.requires_grad:
                 raise ValueError("input_gradient is for a layer whose bias requires no gradient")
             y = _InputGradient.apply(x2, self)

@@ -416,3 +416,26 @@ def test_forward_mode_is_refused_on_the_gpu():
     m.input_gradient = True
     with torch.autograd.forward_ad.dual_level():
         assert torch.autograd.forward_ad.unpack_dual(m(torch.autograd.forward_ad.make_dual(x, x))).tangent is not None
+
+
+def traces_are_refused(dev):
+    from torch.fx.experimental.proxy_tensor import make_fx
+    x = torch.ones(3, 64, device=dev).half()
+    for i, call in enumerate(no_part_of(x)):
+        for t in (x, x.clone().requires_grad_()):
+            if (i == 1 and not t.requires_grad) or (i == 2 and t.requires_grad):
+                continue   # (the layer as it always was; refused anyway)
+            with pytest.raises(RuntimeError, match="trace"):
+                torch.jit.trace(call, (t,), check_trace=False)
+            for pre_dispatch in (False, True):
+                with pytest.raises(RuntimeError, match="trace"):
+                    make_fx(call, pre_dispatch=pre_dispatch)(t)
+
+
+def test_traces_are_refused():
+    traces_are_refused("cpu")
+
+
+@gpu
+def test_traces_are_refused_on_the_gpu():
+    traces_are_refused(DEV)
