@@ -462,7 +462,9 @@ int64_t split_of(int64_t splitK, int (*heuristic)(int, int, size_t, size_t, size
     if (splitK < 1 || splitK > INT_MAX) bad("splitK must be >= 1");
     return splitK;
 }
-int linear_split(int E, int Mb, size_t OC, size_t B, size_t IC, int cus) { return fp6mi_heuristic_splitk_within(E, Mb, OC, B, IC, cus, (size_t)96 << 20); } // SPLIT_WORKSPACE_BYTES
+constexpr size_t kSplitWorkspace = (size_t)96 << 20; // SPLIT_WORKSPACE_BYTES
+int linear_split(int E, int Mb, size_t OC, size_t B, size_t IC, int cus) { return fp6mi_heuristic_splitk_within(E, Mb, OC, B, IC, cus, kSplitWorkspace); }
+// (What is kept for the next call on a stream is bounded.  A call that needs more takes long enough for an allocation not to be seen.)
 float *scratch(const OptTensor &given, const at::Device &dev, void *stream, size_t bytes, at::Tensor &keep)
 {
     if (bytes == 0) return nullptr;
@@ -471,7 +473,8 @@ float *scratch(const OptTensor &given, const at::Device &dev, void *stream, size
             bad("workspace must be a contiguous float32 tensor of at least " + std::to_string(bytes) + " bytes on the same GPU");
         keep = *given;
     } else {
-        keep = workspace_for(dev, stream, (int64_t)((bytes + 3) / 4));
+        const int64_t floats = (int64_t)((bytes + 3) / 4);
+        keep = bytes > kSplitWorkspace ? at::empty({ floats }, at::TensorOptions().dtype(at::kFloat).device(dev)) : workspace_for(dev, stream, floats);
     }
     return keep.data_ptr<float>();
 }

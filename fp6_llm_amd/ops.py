@@ -87,12 +87,12 @@ def _split(splitK, default):
 
 
 def _launch(name, dev, need, workspace, call):
-    """call(stream, workspace pointer) on the tensors' device and its current stream, with `need` bytes of scratch."""
-    from . import _workspace
+    """call(stream, workspace pointer) on the tensors' device and its current stream, with `need` bytes of scratch (beyond SPLIT_WORKSPACE_BYTES not kept for the next call)."""
+    from . import SPLIT_WORKSPACE_BYTES, _workspace
     with torch.cuda.device(dev), _launch_lock:
         stream = torch.cuda.current_stream().cuda_stream
         if need and workspace is None:
-            workspace = _workspace(dev, stream, need)
+            workspace = _workspace(dev, stream, need) if need <= SPLIT_WORKSPACE_BYTES else torch.empty((need + 3) // 4, dtype=torch.float32, device=dev)
         elif need and (workspace.dtype != torch.float32 or workspace.numel() * 4 < need or workspace.device != dev or not workspace.is_contiguous()):
             raise ValueError("workspace must be a contiguous float32 tensor of at least %d bytes on the same GPU" % need)
         _lib.check(call(stream, workspace.data_ptr() if need else None), name)

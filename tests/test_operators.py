@@ -713,3 +713,24 @@ def test_calls_without_the_extension(N, monkeypatch):
         assert all(torch.equal(p, q) for p, q in zip(ours, theirs))
     if N == 3:   # (without the extension from here on)
         test_refusals_of_the_python_functions()
+
+
+@gpu
+def test_large_scratch_is_given_back(monkeypatch):
+    """What a call keeps for the next one on its stream is bounded; partial sums and products beyond that are the call's own."""
+    assert fp6._ext is not None
+    OC, IC, N = 512, 8192, 2000
+    w = Weight(1, 3, 2, OC, IC)
+    dy, dh, pre, x = randn(1, N, OC), randn(2, N, OC // 2), randn(3, N, OC).float(), randn(4, N, IC)
+    calls = [lambda: fp6.linear_input_grad_native(3, 2, dy, w.native, w.scales, IC, splitK=3), lambda: fp6.gated_backward_native(3, 2, dh, pre, w.native, w.scales, IC, splitK=3)[0],
+             lambda: fp6.gated_forward_native(3, 2, x, w.native, w.scales, OC, splitK=30)]
+    wants = [call().clone() for call in calls]
+    for ext in (fp6._ext, None):
+        monkeypatch.setattr(fp6, "_ext", ext)
+        fp6.clear_caches()
+        torch.cuda.synchronize()
+        held = torch.cuda.memory_allocated()
+        for _ in range(2):
+            for call, want in zip(calls, wants):
+                assert torch.equal(call(), want)
+        assert torch.cuda.memory_allocated() - held <= fp6.SPLIT_WORKSPACE_BYTES
