@@ -17,6 +17,7 @@ _MAGIC = b"FP6MI\x00\x01\x00"   # name, NUL, layout version 1, reserved
 
 _peek_transform = getattr(getattr(torch._C, "_functorch", None), "peek_interpreter_stack", None)
 _dispatch_modes = getattr(torch._C, "_len_torch_dispatch_stack", None)
+_forward_ad, _is_compiling, _is_tracing = torch.autograd.forward_ad, torch.compiler.is_compiling, torch.jit.is_tracing
 
 
 def _values_only(t):
@@ -42,26 +43,28 @@ def _differentiates(x):
     return True
 
 
-def _refuse_tangents(x):
-    """A tangent that x carries (forward mode), or a transform of torch.func that x is part of, would be passed by by a kernel that is handed x's address."""
-    if torch.compiler.is_compiling():   # (a call of a kernel ends the graph that is compiled)
+def _refuse_unseen(x):
+    """What a kernel that is handed x's address would pass by in silence: a tangent that x carries (forward mode), a transform of torch.func that x is part of, a trace that is being made,
+    which would record the output as it was allocated and not what fills it."""
+    if _is_compiling():   # (a call of a kernel ends the graph that is compiled)
         return
     wrapped = _peek_transform is None or (_peek_transform() is not None and torch._C._functorch.is_functorch_wrapped_tensor(x))
-    if wrapped or (getattr(torch.autograd.forward_ad, "_current_level", 0) >= 0 and torch.autograd.forward_ad.unpack_dual(x).tangent is not None):
+    if wrapped or (getattr(_forward_ad, "_current_level", 0) >= 0 and _forward_ad.unpack_dual(x).tangent is not None):
         raise RuntimeError("this operator has no part in forward mode or in a transform of torch.func")
-
-
-def _refuse_traces():
-    """A trace records the output as it was allocated and not the kernel that fills it."""
     proxies = sys.modules.get("torch.fx.experimental.proxy_tensor")   # (not loaded: no such trace is being made)
-    if not torch.compiler.is_compiling() and (torch.jit.is_tracing() or (proxies is not None and proxies.get_proxy_mode() is not None)):
+    if _is_tracing() or (proxies is not None and proxies.get_proxy_mode() is not None):
         raise RuntimeError("this operator cannot be recorded by a trace")
+
+
+def _held(module, name):
+    """A buffer of a module, which as an attribute takes half a microsecond; or whatever has taken its place."""
+    held = module._buffers
+    return held[name] if name in held else getattr(module, name)
 
 
 def _rows_of(x, features):
     """x[..., features] as float16 rows, of which nothing but their values counts or a backward pass."""
-    _refuse_tangents(x)
-    _refuse_traces()
+    _refuse_unseen(x)
     if x.dim() < 1 or x.shape[-1] != features:
         raise ValueError("need an input of %d features, got %s" % (features, list(x.shape)))
     x2 = x.reshape(-1, features)
@@ -269,15 +272,15 @@ class FPxLinear(torch.nn.Module):
             raise ValueError("adapters must be a LowRankAdapters, with an index for every row")
         if (adapters.in_features, adapters.out_features) != (self.in_features, self.out_features):
             raise ValueError("the adapters are for %d -> %d features, the layer has %d -> %d" % (adapters.in_features, adapters.out_features, self.in_features, self.out_features))
-        if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, self.bias, adapters.lora_a, adapters.lora_b, adapters.scaling)):
+        bias, a, b, scaling = self.bias, _held(adapters, "lora_a"), _held(adapters, "lora_b"), _held(adapters, "scaling")
+        if torch.is_grad_enabled() and (x.requires_grad or a.requires_grad or b.requires_grad or scaling.requires_grad or (bias is not None and bias.requires_grad)):
             raise ValueError("a product with adapters has no gradient: call it under torch.no_grad()")
         x2 = _rows_of(x, self.in_features)
         if index.numel() != x2.shape[0] or (index.dim() != 1 and index.shape != x.shape[:-1]):
             raise ValueError("index must name an adapter for each of the %d rows, got %s" % (x2.shape[0], list(index.shape)))
         split = None if self._auto and x2.shape[0] >= _CROSSOVER_LIBRARY else self.split_k or None   # (as in forward: rows without an adapter have the layer's own bits)
-        bias = self.bias
         fused = bias if bias is not None and self._bias_in_kernel(x2) else None
-        y = ops.adapter_forward_native(self.exponent, self.mantissa, x2, self.weight_native, self.scales, self.out_features, adapters.lora_a, adapters.lora_b, adapters.scaling,
+        y = ops.adapter_forward_native(self.exponent, self.mantissa, x2, self.weight_native, self.scales, self.out_features, a, b, scaling,
                                        index.reshape(-1).contiguous(), split, group_exps=self.group_exps, bias=fused)
         if bias is not fused:
             y = y + bias
@@ -295,8 +298,7 @@ class FPxLinear(torch.nn.Module):
         if x2.dtype != torch.float16:
             x2 = x2.half()
         if self.input_gradient and _differentiates(x):
-            _refuse_tangents(x)
-            _refuse_traces()
+            _refuse_unseen(x)
             if self.bias is not None and self.bias.requires_grad:
                 raise ValueError("input_gradient is for a layer whose bias requires no gradient")
             y = _InputGradient.apply(x2, self)
@@ -311,7 +313,7 @@ class FPxLinear(torch.nn.Module):
                 y = y + self.bias
             return y if plain else y.reshape(*shape[:-1], self.out_features)
         if self.input_gradient:
-            _refuse_tangents(x)
+            _refuse_unseen(x)
         sk = self.split_k
         if not sk or (self._auto and n >= _CROSSOVER_LIBRARY):   # the heuristic's answer per batch size is remembered: the layer is called once per token
             # (split_k is for the batches up to 3071 rows; the partial sums of a long prompt would take gigabytes)
@@ -377,12 +379,13 @@ class FPxGatedLinear(torch.nn.Module):
 
     def _values(self, x2, preact=None):
         split = self.split_k or None if x2.shape[0] < _CROSSOVER_LIBRARY else None   # (as in FPxLinear: the partial sums of a long prompt would take gigabytes)
-        return ops.gated_forward_native(self.exponent, self.mantissa, x2, self.weight_native, self.scales, 2 * self.out_features, self.activation, split, preact=preact,
-                                        group_exps=self.group_exps, bias=self.bias)
+        return ops.gated_forward_native(self.exponent, self.mantissa, x2, _held(self, "weight_native"), _held(self, "scales"), 2 * self.out_features, self.activation, split, preact=preact,
+                                        group_exps=_held(self, "group_exps"), bias=_held(self, "bias"))
 
     def forward(self, x):
         x2 = _rows_of(x, self.in_features)
-        if self.bias is not None and self.bias.requires_grad and torch.is_grad_enabled():
+        bias = _held(self, "bias")
+        if bias is not None and bias.requires_grad and torch.is_grad_enabled():
             raise ValueError("the bias of FPxGatedLinear has no gradient")
         y = _GatedBlock.apply(x2, self) if _differentiates(x) else self._values(x2)
         return y if x.dim() == 2 else y.reshape(*x.shape[:-1], self.out_features)

@@ -376,6 +376,9 @@ def test_adapters_that_require_a_gradient_are_refused():
         getattr(ad, name).requires_grad_()
         with pytest.raises(ValueError, match="no gradient"):
             m(x, ad, index)
+        setattr(ad, name, torch.nn.Parameter(getattr(ad, name).detach()))   # (no buffer any more)
+        with pytest.raises(ValueError, match="no gradient"):
+            m(x, ad, index)
 
 
 def no_part_of(x):
