@@ -36,7 +36,7 @@ using fp6mi::LaunchCfg;
 // the compiler holds the next transposing read back until the transfer is there.)
 // What bounds it: with 128 x 128 outputs a wavefront (256 x 256 a workgroup, one wavefront to a SIMD) the MFMAs, of which 64 take an operand read of 24 KB; the LDS unit is busy for a third
 // of the time, bank conflicts are none.  What was gained on the way, 8192x8192 N 4096, us: 256 x 128 tiles, operands read as they are multiplied 1414; read a step ahead 498;
-// 256 x 256 466; other instructions spread between the MFMAs 448 (1.23 PFLOP/s; the fp16 library product of the card reaches 1.41).  22016x4096 N 4096 598, N 512 105 (8 splits),
+// 256 x 256 466; other instructions spread between the MFMAs 448 (1.23 PFLOP/s; the fp16 library product of the card reaches 1.41).  22016x4096 N 4096 598, N 512 100 to 108 (4 splits),
 // 4608x4544 N 333 33 (4 splits).  Left out: 256 x 128 with two workgroups of four wavefronts to a CU (515) and chunks of 32 rows.
 // Two stages, one barrier a chunk.
 // ---------------------------------------------------------------------------------------------------------------
@@ -313,8 +313,9 @@ __global__ __launch_bounds__(2 * WN *kWave, NT >= 6 ? 1 : 2) void grad_tile(cons
 //   the columns each
 // Every wavefront is by itself until the end: it converts its halves of two native blocks into an LDS area of its own (rows 288 bytes apart, in grad_tile's
 // order; no barrier, the LDS unit serves a wavefront in order), reads them back transposed, and takes its batch rows from memory in operand order.  The codes of the next
-// 32 rows are asked for before this one's are converted.  Sums meet in LDS.  us, with the reduction of the splits, e3m2, N 8 / 32: 4096x4096 10.8 / 15.5 (16 splits), 8192x8192 17.3 / 21.5 (8),
-// 28672x8192 39 / 48 (8, 4.5 TB/s); with whole blocks a wavefront, twice the sums to meet, 11.2 / 18.2, 17.9 / 27.3, 39 / 65.  (Half blocks of different workgroups 13.3 and 35.6 at N 8, 1:
+// 32 rows are asked for before this one's are converted.  Sums meet in LDS.  us a call in a captured graph, the reduction of the splits among it, over weights that no cache holds (several
+// matrices in turn, 300 to 600 MB), e3m2, N 8 / 32: 4096x4096 10.3 / 15.5 (16 splits), 8192x8192 15.8 / 21.4 (8), 28672x8192 36.7 / 46.8 (8, 4.8 TB/s); with whole blocks a wavefront, twice the sums to
+// meet, and at N 32 four wavefronts everywhere, 10.8 / 17.3, 17.1 / 26.0, 34.9 / 55.3.  (4096x4096 N 8 over three matrices, which the memory-side cache holds: 9.6.  Half blocks of different workgroups 13.3 and 35.6 at N 8, 1:
 // the codes that the halves share were fetched by two XCDs.)
 // ---------------------------------------------------------------------------------------------------------------
 constexpr int kStreamRow = 288, kStreamHalf = 16 * kStreamRow + 16, kStreamMant = 2 * kStreamHalf, kStreamWave = kStreamMant + 64;
@@ -470,7 +471,7 @@ int grad_cfg(int rows, hipStream_t st, const void *W, const void *sc, const void
 // ---------------------------------------------------------------------------------------------------------------
 // The gated feed-forward block: the GEMM's kernels (fp6mi_gemm.hip: gemm_stream, gemm_tile, gemm_ws, gemm_wide and gemm_span) with another epilogue.
 // The weights are one matrix of M rows in pair order: a 16-row tile of the gate projection, the same tile of the up projection, and so on.  An even number of row tiles to a
-// wavefront (or, in gemm_stream, a workgroup) then holds both pre-activations of every output, and no launch, no trip through memory follows: 2 * N * M bytes written and read less.
+// workgroup then holds both pre-activations of every output, and no launch, no trip through memory follows: 2 * N * M bytes written and read less.
 // The float32 sums are scaled and parked in LDS as the partial sums of a split are; on the way out a thread takes four rows of gate and the same four of up, adds the biases and
 // writes act(g) * u, and the pre-activations themselves where a backward pass will want them.
 // Parameters as in the GEMM's kernels; preact and bias may be null.
@@ -480,6 +481,7 @@ __device__ __forceinline__ void gated_flush(half_t *__restrict__ out, float *__r
                                             uint32_t N, uint32_t mb, uint32_t nbase, int tid)
 {
     constexpr int TM = WR * RT * 16, TN = NT * 16, kStride = TM * 4 + 16, kPerCol = TM / 8, kPieces = TN * kPerCol; // a piece: four outputs
+    static_assert(TM % 32 == 0, "pairs of row tiles");
     for (int p = tid; p < kPieces; p += NTHREADS) {
         const int      c = p / kPerCol, i = p % kPerCol;
         const uint32_t ng = nbase + c, m = mb * TM + (i >> 2) * 32 + (i & 3) * 4;
@@ -519,7 +521,6 @@ __global__ __launch_bounds__(WR *WK *kWave) void gated_tile(const uint8_t *__res
                                                             half_t *__restrict__ C, float *__restrict__ preact, const half_t *__restrict__ bias, uint32_t M, uint32_t N, uint32_t K,
                                                             uint32_t units, uint32_t activation_code, uint32_t nblocks)
 {
-    static_assert(RT % 2 == 0, "pairs of row tiles");
     constexpr int NTHREADS = WR * WK * kWave;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     const int      tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wr = wave % WR, wk = wave / WR, col = lane & 15, q = lane >> 4;
@@ -544,7 +545,6 @@ __global__ __launch_bounds__((WR + PW) * kWave) void gated_ws(const uint8_t *__r
                                                               half_t *__restrict__ C, float *__restrict__ preact, const half_t *__restrict__ bias, uint32_t M, uint32_t N, uint32_t K,
                                                               uint32_t units, uint32_t activation_code, uint32_t nblocks)
 {
-    static_assert(RT % 2 == 0, "pairs of row tiles");
     constexpr uint32_t splitK = 1;
     float *const       ws = preact;
 #include "fp6mi_ws_tile.inc"
@@ -555,7 +555,6 @@ __global__ __launch_bounds__(4 * WK *kWave, RT *NT <= 8 ? 4 : 2) void gated_wide
                                                                                  half_t *__restrict__ C, float *__restrict__ preact, const half_t *__restrict__ bias, uint32_t M, uint32_t N,
                                                                                  uint32_t K, uint32_t units, uint32_t activation_code, uint32_t nblocks)
 {
-    static_assert(RT % 2 == 0, "pairs of row tiles");
     constexpr uint32_t splitK = 1;
 #include "fp6mi_wide_tile.inc"
 }

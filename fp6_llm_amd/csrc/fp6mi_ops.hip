@@ -165,7 +165,7 @@ template <typename F> __device__ __forceinline__ void each_adapter(int mine, Pas
 // adapter_shrink by workgroups of their own (in the grid's second dimension, behind the ranges).
 //
 // adapter_shrink, for few rows: tiles of sixteen, operands straight from memory, the four wavefronts of a workgroup taking every fourth 64 columns of its range and meeting in LDS.
-// Bound by latency: three round trips, to the index, to the operands and to the output (4096 columns, 32 rows of 32 requests, rank 16: 4.4 us).
+// Bound by latency: three round trips, to the index, to the operands and to the output (4096 columns, 32 rows of 32 requests, rank 16: 4.6 to 4.9 us).
 template <int RT>
 __global__ __launch_bounds__(256) void adapter_shrink(float *__restrict__ part, const half_t *__restrict__ x, const half_t *__restrict__ A, const int *__restrict__ index, uint32_t N,
                                                       uint32_t K, uint32_t R, uint32_t slots, uint32_t ranges)
@@ -349,7 +349,7 @@ __global__ __launch_bounds__(256) void adapter_ranks(half_t *__restrict__ ranks,
 // expand: y[n, m] += factor[n] * sum over r of t[n, r] * B[a, m, r].  grid = (tiles, blocks of 256 outputs, passes side by side); 64 outputs a wavefront.
 //
 // adapter_expand, for few rows: tiles of sixteen; forms t in LDS from the ranges' sums, which saves a launch and is bound by the latency of it (4096 outputs, 32 rows of 32 requests,
-// rank 16: 7.5 us).  The sums are held as two halfs, 22 bits: with few rows of few ranks a rounding of one of them is a rounding of the whole row, and two more MFMAs a step are not to be
+// rank 16: 7.1 to 7.7 us).  The sums are held as two halfs, 22 bits: with few rows of few ranks a rounding of one of them is a rounding of the whole row, and two more MFMAs a step are not to be
 // seen in the time.
 template <int RT>
 __global__ __launch_bounds__(256) void adapter_expand(half_t *__restrict__ y, const float *__restrict__ part, const half_t *__restrict__ B, const float *__restrict__ scaling,

@@ -179,7 +179,8 @@ def adapter_forward_native(EXPONENT, MANTISSA, in_feats, native_weight, scales, 
     """linear_forward_native with a low-rank adapter for every row of the batch:
     out[n] = in_feats[n] @ dequant(W)^T + bias + scaling[a] * (in_feats[n] @ lora_a[a]^T) @ lora_b[a]^T,  a = index[n].
     lora_a: float16 [slots, R, IC], lora_b: float16 [slots, OC, R], scaling: float32 [slots], index: int32 [B], all on the GPU; a row whose index is no slot's number (-1,
-    say) has no adapter.  R is a multiple of 8 up to 256: pad smaller ranks with zeros."""
+    say) has no adapter.  R is a multiple of 8 up to 256: pad smaller ranks with zeros.  The layer's output is rounded to float16 before the adapter's part is added to it, which is
+    rounded once more; of that part the rank sums in_feats[n] @ lora_a[a]^T are held to 2^-11 of themselves in large batches, to 2^-22 in small ones."""
     from . import _ext, heuristic_splitk_mi355x
     if _ext is not None:
         return _ext.adapter_forward(EXPONENT, MANTISSA, in_feats, native_weight, scales, OC, lora_a, lora_b, scaling, index, _HEURISTIC if splitK is None else int(splitK), out,

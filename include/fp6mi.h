@@ -234,7 +234,7 @@ size_t fp6mi_grad_workspace_bytes(size_t N, size_t K, int splits);
 
 /* Gated feed-forward block: H[N,M/2] = act(B . Wg^T + bg) * (B . Wu^T + bu).  The two matrices are one of M rows in PAIR ORDER: 16 rows of Wg, the same 16 of Wu,
  * and so on (scales, group exponents and bias likewise; in the native layout that is whole row tiles in turn).  preact, unless NULL, receives the
- * pre-activations [N,M] in pair order, the FP32 sums as they are, for the backward pass.  workspace: fp6mi_gated_workspace_bytes bytes, none without a split. */
+ * pre-activations [N,M] in pair order, the FP32 sums as they are, for the backward pass.  N * M up to 2^34.  workspace: fp6mi_gated_workspace_bytes bytes, none without a split. */
 #define FP6MI_ACT_SILU 0
 #define FP6MI_ACT_GELU 1      /* g * P(g), P the normal distribution */
 #define FP6MI_ACT_GELU_TANH 2 /* its approximation by a hyperbolic tangent */
@@ -244,7 +244,7 @@ size_t fp6mi_gated_workspace_bytes(size_t M, size_t N, int splitK);
 /* Its launch shape without a split, in the terms of fp6mi_query_launch. */
 int fp6mi_query_gated_launch(int E, int Mbits, size_t M, size_t N, size_t K, int grouped, int *shape);
 /* Its backward pass from the gradient of H: grad_preact[N,M] in pair order (the gradient that a bias sums over N, or an adapter beside the block takes; not written where it
- * is NULL) and grad_in[N,K] = grad_preact . dequant(W).  The weights have no gradient.  workspace: fp6mi_gated_backward_workspace_bytes bytes, always; splits as in
+ * is NULL) and grad_in[N,K] = grad_preact . dequant(W); what is multiplied is grad_preact times the mantissas, rounded to fp16 once.  The weights have no gradient.  workspace: fp6mi_gated_backward_workspace_bytes bytes, always; splits as in
  * fp6mi_linear_grad_native. */
 int    fp6mi_gated_backward_native(int E, int Mbits, void *stream, const void *W_native, const void *scales_f16, const void *group_exps_native, const void *grad_out_f16,
                                    const float *preact, void *grad_preact_f16, void *grad_in_f16, size_t M, size_t N, size_t K, int activation, float *workspace, int splits);
@@ -252,7 +252,8 @@ size_t fp6mi_gated_backward_workspace_bytes(size_t M, size_t N, size_t K, int sp
 
 /* The linear layer with a low-rank adapter for every batch row: C[n] = B[n] . W^T + bias + scaling[a] * (B[n] . A[a]^T) . Bm[a]^T with a = index[n]; a row whose index is
  * no slot's number (-1, say) has none.  lora_a: fp16 [slots][R][K], lora_b: fp16 [slots][M][R], scaling: fp32 [slots], index: int32 [N], all on the device.  R is a multiple of 8 up
- * to 256 (smaller ranks are padded with zeros).  The layer's output is rounded to fp16 before the adapter's part is added to it.  workspace: fp6mi_adapter_workspace_bytes
+ * to 256 (smaller ranks are padded with zeros).  The layer's output is rounded to fp16 before the adapter's part is added to it; of that, the rank sums B[n] . A[a]^T are held to 2^-11 of
+ * themselves in large batches, to 2^-22 in small ones.  workspace: fp6mi_adapter_workspace_bytes
  * bytes, always. */
 int    fp6mi_adapter_native(int E, int Mbits, void *stream, const void *W_native, const void *scales_f16, const void *group_exps_native, const void *bias_f16, const void *B_f16,
                             void *C_f16, const void *lora_a_f16, const void *lora_b_f16, const float *scaling, const int *index, size_t M, size_t N, size_t K, size_t R, size_t slots,
