@@ -442,3 +442,32 @@ def test_traces_are_refused():
 @gpu
 def test_traces_are_refused_on_the_gpu():
     traces_are_refused(DEV)
+
+
+@gpu
+def test_captured_step_with_a_gradient_between_two_boundaries():
+    """The copy of such a gradient is part of the graph, and is made anew in every replay."""
+    if fp6._ext is None:   # (nothing says there where a gradient would go)
+        pytest.skip("a differentiable call is captured with the extension alone")
+    mg = block(Weight(2, 2, 2, 512, 320, True))
+    weights = randn(2, 1 + 40 * 256, scale=0.1)
+
+    def step(t):
+        return torch.autograd.grad(torch.cat([t.flatten()[:1], mg(t).flatten()]), t, weights)[0]
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        step(randn(1, 40, 320).requires_grad_())
+        leaf = randn(1, 40, 320).requires_grad_()
+        stream.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            g = step(leaf)
+        for seed in range(4):
+            weights.copy_(randn(20 + seed, 1 + 40 * 256, scale=0.1))
+            with torch.no_grad():
+                leaf.copy_(randn(10 + seed, 40, 320))
+            want = step(leaf.detach().clone().requires_grad_())
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(g, want)
