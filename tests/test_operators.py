@@ -734,3 +734,17 @@ def test_large_scratch_is_given_back(monkeypatch):
             for call, want in zip(calls, wants):
                 assert torch.equal(call(), want)
         assert torch.cuda.memory_allocated() - held <= fp6.SPLIT_WORKSPACE_BYTES
+
+
+# the projection down of a block: many columns, and so many ranges of them
+@gpu
+@pytest.mark.parametrize("E,M,OC,IC,N,R,slots,bias", [(3, 2, 256, 28672, 1, 16, 3, False), (2, 2, 512, 11008, 20, 72, 5, True), (2, 1, 256, 11072, 33, 136, 4, False), (2, 3, 512, 28672, 120, 64, 30, True),
+                                                      (3, 2, 256, 11008, 300, 24, 9, False), (2, 2, 512, 9152, 700, 40, 5, True)])
+def test_adapters_of_long_rows(E, M, OC, IC, N, R, slots, bias):
+    test_adapters(E, M, OC, IC, N, R, slots, bias, "mixed")
+
+
+@gpu
+@pytest.mark.parametrize("E,M,OC,IC,N,groups", [(3, 2, 512, 28672, 3, False), (2, 2, 1024, 11008, 29, True), (2, 3, 512, 11072, 100, False), (2, 1, 512, 28672, 333, True)])
+def test_input_gradient_of_long_rows(E, M, OC, IC, N, groups):
+    test_input_gradient(E, M, OC, IC, N, groups)
