@@ -3,7 +3,7 @@ import pytest
 import torch
 
 import fp6_llm_amd as fp6
-from fp6_llm_amd.module import FPxGatedLinear, FPxLinear, LowRankAdapters
+from fp6_llm_amd.module import _CROSSOVER_LIBRARY as LONG, FPxGatedLinear, FPxLinear, LowRankAdapters
 from test_operators import DEV, HALF, TINY, Weight, adapters64, d, gated64, gpu, halves, pairs, preacts, randn, slope64, act64, sum_error, within
 
 
@@ -320,7 +320,7 @@ def splits_asked_for(monkeypatch, name):
 def test_split_of_a_gated_block_is_for_batches_below_a_long_prompt(monkeypatch):
     asked = splits_asked_for(monkeypatch, "gated_forward_native")
     m = FPxGatedLinear(64, 128, split_k=4)
-    for n in (1, 3071, 3072, 9000):
+    for n in (1, LONG - 1, LONG, 9000):
         m(torch.zeros(n, 64).half())
     m(torch.zeros(1536, 2, 64).half())
     for none in (None, 0):
@@ -334,7 +334,7 @@ def test_split_of_a_layer_holds_with_adapters(monkeypatch):
     ad = LowRankAdapters(64, 256, 1, 8)
     for kw in (dict(split_k=2), dict(split_k=2, dequant_above=None), dict()):
         m = FPxLinear(64, 256, **kw)
-        for n in (1, 3071, 3072):
+        for n in (1, LONG - 1, LONG):
             x, index = torch.zeros(n, 64).half(), torch.zeros(n, dtype=torch.int32)
             m(x, ad, index), m(x)
     assert [s for s in asked[:6]] == [2, 2, None, 2, 2, 2] and asked[6:] == [None] * 3
@@ -415,7 +415,7 @@ def test_forward_mode_is_refused_on_the_gpu():
         with torch.autograd.forward_ad.dual_level():
             assert torch.equal(call(x), want)
     # a long prompt with a tangent goes through the library, as it does without input_gradient
-    m, x = FPxLinear(64, 256).to(DEV), torch.ones(3072, 64, device=DEV).half()
+    m, x = FPxLinear(64, 256).to(DEV), torch.ones(LONG + 8, 64, device=DEV).half()
     m.input_gradient = True
     with torch.autograd.forward_ad.dual_level():
         assert torch.autograd.forward_ad.unpack_dual(m(torch.autograd.forward_ad.make_dual(x, x))).tangent is not None
