@@ -67,13 +67,13 @@ def _rows_of(x, features):
     _refuse_unseen(x)
     if x.dim() < 1 or x.shape[-1] != features:
         raise ValueError("need an input of %d features, got %s" % (features, list(x.shape)))
-    x2 = x.reshape(-1, features)
+    x2 = x.reshape(-1, features).resolve_neg()
     return x2 if x2.dtype == torch.float16 else x2.half()
 
 
 def _gradient(grad):
     """What autograd hands to a backward pass, as the kernels read it: float16 from a 16-byte boundary on.  (Of a part of a concatenation it is a view into the whole one's, at any place.)"""
-    grad = grad.half()
+    grad = grad.half().resolve_neg()
     return grad.clone() if grad.is_contiguous() and grad.data_ptr() % 16 else grad
 
 

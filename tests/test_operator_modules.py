@@ -471,3 +471,20 @@ def test_captured_step_with_a_gradient_between_two_boundaries():
             graph.replay()
             torch.cuda.synchronize()
             assert torch.equal(g, want)
+
+
+def test_negative_views_are_resolved(monkeypatch):
+    """A tensor may say that its values are those in memory with the other sign (the imaginary part of a conjugate does); the kernels read memory."""
+    from fp6_llm_amd import module
+    seen = []
+
+    def stand_in(E, M, x, *args, **kw):
+        seen.append(not x.is_neg() and (x == -1).all())
+        return torch.zeros(x.shape[0], 256 if args[2] == 256 else 128, dtype=torch.float16)
+    monkeypatch.setattr(module.ops, "gated_forward_native", stand_in)
+    monkeypatch.setattr(module.ops, "adapter_forward_native", stand_in)
+    x = torch._neg_view(torch.ones(3, 64).half())
+    FPxGatedLinear(64, 128)(x)
+    FPxLinear(64, 256)(x, LowRankAdapters(64, 256, 1, 8), torch.zeros(3, dtype=torch.int32))
+    g = module._gradient(x)
+    assert seen == [True, True] and not g.is_neg() and (g == -1).all()
