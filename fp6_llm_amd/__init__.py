@@ -36,7 +36,7 @@ if os.path.exists(_lib.LIB_PATH) and not os.environ.get("FP6MI_NO_TORCH_EXT"):
     try:
         _lib.lib()
         from . import _fp6mi_torch as _ext
-        if "bias" not in (_ext.linear_forward_native.__doc__ or "") or not hasattr(_ext, "gradient_goes_elsewhere"):   # the newest of the names and arguments used below
+        if "bias" not in (_ext.linear_forward_native.__doc__ or "") or not hasattr(_ext, "int4_forward"):   # the newest of the names and arguments used below
             raise ImportError("the extension was built from an older tree")
     except (ImportError, OSError, AttributeError):   # extension not built or stale, or a stale library: the ctypes path reports what is wrong
         _ext = None
@@ -48,6 +48,7 @@ __all__ = [
     "weight_prepacking_native_cpu", "to_native", "linear_forward_native", "native_bytes",
     "weight_dequant_native_cuda", "weight_quantize_native_cuda", "heuristic_splitk_mi355x", "clear_caches",
     "gated_forward_native", "gated_backward_native", "gate_up_pairs", "linear_input_grad_native", "adapter_forward_native",
+    "int4_quantize", "int4_pack_native", "int4_forward_native", "expert_plan", "expert_sort", "expert_combine",
 ]
 
 MI355X_CUS = 256
@@ -451,3 +452,5 @@ def linear_forward_cuda(in_feats, weights, scales, splitK=1):
 
 
 from .ops import adapter_forward_native, gate_up_pairs, gated_backward_native, gated_forward_native, linear_input_grad_native  # noqa: E402,F401
+from .int4 import int4_forward_native, int4_pack_native, int4_quantize  # noqa: E402,F401
+from .experts import expert_combine, expert_plan, expert_sort  # noqa: E402,F401

@@ -630,6 +630,7 @@ const char *fp6mi_error_string(int code)
 {
     switch (code) {
     case FP6MI_OK: return "success";
+    case FP6MI_ERR_TYPE: return "element types: fp16 or bf16 (rows of experts also fp32), sums of float32 rows to any of them";
     case FP6MI_ERR_FORMAT: return "unsupported (E,M): only FP6_e3m2 (3,2), FP5_e2m2 (2,2), FP6_e2m3 (2,3) and FP4_e2m1 (2,1)";
     case FP6MI_ERR_SHAPE: return "unsupported shape: need M % 256 == 0 (64 for CPU packers, 16 for native packers), K % 64 == 0, N >= 1, distinct in/out";
     case FP6MI_ERR_NULL: return "a required pointer is NULL";

@@ -1,0 +1,286 @@
+// Products with 4-bit integer weights and a scale (and zero point) for each group of columns: y[n,m] = sum_k x[n,k] * s[m,g(k)] * (q[m,k] - z[m,g(k)]), for one matrix or, with rows that
+// are sorted by expert, for the matrix of each row's expert; optionally act(gate) * up of the pairs of 16 rows.  Compiled once per activation type (FP6MI_TYPE 0: fp16, 1: bf16).
+// No counterpart in the reference.
+//
+// q - z is an integer from -15 to 15, exact in fp16 and bf16, so the matrix instructions' products are exact and their sums float32; a group's sum is multiplied by its scale in float32.
+// (Scaling the weights before the product would round each of them to 16 bits, and 16-bit sums would be no cheaper.)
+//
+// Layout (fp6mi_int4_pack): blocks of 16 rows x 128 columns of 1024 bytes, [expert][row tile][column block]; lane c + 16 q of a wavefront holds 16 bytes of a block, dword s of which are the
+// columns 32 s + 8 q to 32 s + 8 q + 7 of row c: the operand of one v_mfma_f32_16x16x32.  In a dword the nibbles 0..7 are the columns 0, 2, 4, 6, 1, 3, 5, 7, so that a mask leaves two neighbours
+// 16 bits apart.  Scales: [expert][row tile][column block][row][group of the block], with zero points {scale, zero point} in pairs, both of the activations' type.
+#include <hip/hip_runtime.h>
+
+#include <type_traits>
+
+#include "fp6mi_internal.h"
+#include "fp6mi_activation.inc"
+#include "fp6mi_int4.inc"
+
+namespace {
+
+#if FP6MI_TYPE == 0
+typedef _Float16 T;
+#else
+typedef __bf16 T;
+#endif
+typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+typedef T        v8t __attribute__((ext_vector_type(8)));
+typedef float    v4f __attribute__((ext_vector_type(4)));
+typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+
+using fp6mi::Int4Args;
+
+__device__ __forceinline__ v4f mfma(v8t x, v8t w, v4f acc)
+{
+#if FP6MI_TYPE == 0
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(x, w, acc, 0, 0, 0);
+#else
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, w, acc, 0, 0, 0);
+#endif
+}
+
+// What a group's zero point (8 without one) makes of the codes.
+struct Zero {
+#if FP6MI_TYPE == 0
+    v2h low, high; // -(1024 + z), -(64 + z)
+    __device__ __forceinline__ void set(T z)
+    {
+        const T l = (T)-1024.f - z, h = (T)-64.f - z;
+        low = (v2h){ l, l }, high = (v2h){ h, h };
+    }
+#else
+    float z;
+    __device__ __forceinline__ void set(T v) { z = (float)v; }
+#endif
+};
+
+// Eight codes as q - z, columns 0..7.  fp16: 1024 + q and 1024 + 16 q are read off the bits 0x6400 | nibble, 9 instructions.  bf16 has no packed arithmetic: bytes to float32, and the upper
+// halves of the exact differences, 23.
+__device__ __forceinline__ v8t codes_of(uint32_t w, const Zero &zero)
+{
+#if FP6MI_TYPE == 0
+    union { v2h h[4]; v8t v; } r;
+    const v2h      sixteenth = { (_Float16)0.0625f, (_Float16)0.0625f };
+    const uint32_t w8 = w >> 8;
+    r.h[0] = __builtin_bit_cast(v2h, (w & 0x000f000fu) | 0x64006400u) + zero.low;
+    r.h[1] = __builtin_elementwise_fma(__builtin_bit_cast(v2h, (w & 0x00f000f0u) | 0x64006400u), sixteenth, zero.high);
+    r.h[2] = __builtin_bit_cast(v2h, (w8 & 0x000f000fu) | 0x64006400u) + zero.low;
+    r.h[3] = __builtin_elementwise_fma(__builtin_bit_cast(v2h, (w8 & 0x00f000f0u) | 0x64006400u), sixteenth, zero.high);
+    return r.v;
+#else
+    union { uint32_t d[4]; v8t v; } r;
+    const uint32_t even = w & 0x0f0f0f0fu, odd = (w >> 4) & 0x0f0f0f0fu; // bytes: nibbles 0, 2, 4, 6 and 1, 3, 5, 7
+    auto           pair = [&](uint32_t b, int i) { // nibbles n and n + 4
+        const float lo = (float)(uint8_t)(b >> 8 * i) - zero.z, hi = (float)(uint8_t)(b >> 8 * (i + 2)) - zero.z;
+        return __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, hi), __builtin_bit_cast(uint32_t, lo), 0x07060302u);
+    };
+    r.d[0] = pair(even, 0), r.d[1] = pair(odd, 0), r.d[2] = pair(even, 1), r.d[3] = pair(odd, 1);
+    return r.v;
+#endif
+}
+
+// The scales (and zero points) of one row in one block.
+template <int GPB, bool Z> struct alignas(2 * GPB * (Z ? 2 : 1)) Scales { T v[GPB * (Z ? 2 : 1)]; };
+
+// Rows [row, row + rows) of X against the weights of an expert; or rows that no expert has (expert < 0), which get zeros.
+struct Tile { int expert; uint32_t row, rows; };
+
+// Tile number i of `each` rows: those of one matrix, or of the experts one after another, then of the rows behind them; rows = 0: there are fewer.  The same for all lanes.
+__device__ __forceinline__ Tile tile_of(const Int4Args &a, uint32_t i, uint32_t each)
+{
+    if (!a.offsets) {
+        const uint32_t row = i * each;
+        return { 0, row, row < a.N ? (a.N - row < each ? a.N - row : each) : 0 };
+    }
+    const int lane = threadIdx.x & 63;
+    uint32_t  first = 0; // tiles of the experts before these 64
+    for (uint32_t b = 0; b <= a.E; b += 64) {
+        const uint32_t e = b + lane, lo = e <= a.E ? (uint32_t)a.offsets[e] : a.N, hi = e < a.E ? (uint32_t)a.offsets[e + 1] : a.N, n = hi > lo ? (hi - lo + each - 1) / each : 0;
+        uint32_t       s = n;
+#pragma unroll
+        for (int m = 1; m < 64; m <<= 1) {
+            const uint32_t o = __shfl_up(s, m);
+            if (lane >= m) s += o;
+        }
+        const uint64_t reached = __ballot(first + s > i);
+        if (reached) {
+            const int      at = __builtin_ctzll(reached);
+            const uint32_t row = __builtin_amdgcn_readlane(lo, at) + (i - first - __builtin_amdgcn_readlane(s - n, at)) * each, end = __builtin_amdgcn_readlane(hi, at);
+            return { b + at < a.E ? (int)(b + at) : -1, row, row < end && end <= a.N ? (end - row < each ? end - row : each) : 0 };
+        }
+        first += __builtin_amdgcn_readlane(s, 63);
+    }
+    return { 0, 0, 0 };
+}
+
+__device__ __forceinline__ void store(const Int4Args &a, uint32_t row, uint32_t m, uint32_t ld, float v)
+{
+    const size_t at = (size_t)row * ld + m;
+    if (a.out_f32)
+        static_cast<float *>(a.Y)[at] = v;
+    else
+        static_cast<T *>(a.Y)[at] = (T)v;
+}
+
+// Zeros for the rows of a tile that no expert has, in the columns of row tiles [m0, m0 + mt).
+__device__ __forceinline__ void store_zeros(const Int4Args &a, const Tile &t, uint32_t m0, uint32_t mt, uint32_t threads)
+{
+    const uint32_t per = a.act >= 0 ? 8 : 16, ld = a.Mt * per, lo = m0 * per, w = (m0 + mt < a.Mt ? mt : a.Mt - m0) * per;
+    for (uint32_t i = threadIdx.x; i < t.rows * w; i += threads) store(a, t.row + i / w, lo + i % w, ld, 0.f);
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// Few rows: RT row tiles and NT tiles of 16 rows of X to a workgroup of WK wavefronts, which share K: a wavefront takes every WK-th column block, its weights straight from HBM to registers
+// (the next block's on their way meanwhile) and its part of X from L2.  Bound by the bytes of the weights; the partial sums meet in LDS.
+// ---------------------------------------------------------------------------------------------------------------
+template <int GPB, bool Z, int RT, int NT> struct Block {
+    v4u            w[RT];
+    Scales<GPB, Z> s[RT];
+    v8t            x[NT][4];
+};
+
+template <int GPB, bool Z, int RT, int NT, int WK> __global__ __launch_bounds__(WK * 64) void int4_stream(const Int4Args a)
+{
+    __shared__ v4f part[WK][RT * NT][64];
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, q = lane >> 4;
+    const uint32_t m0 = blockIdx.x * RT;
+    const Tile     t = tile_of(a, blockIdx.y, NT * 16);
+    if (t.rows == 0) return;
+    if (t.expert < 0) return store_zeros(a, t, m0, RT, WK * 64);
+
+    const v4u            *w[RT];
+    const Scales<GPB, Z> *s[RT];
+    const T              *x[NT];
+#pragma unroll
+    for (int r = 0; r < RT; r++) { // (a last workgroup with fewer row tiles takes the last one again)
+        const size_t at = ((size_t)t.expert * a.Mt + (m0 + r < a.Mt ? m0 + r : a.Mt - 1)) * a.KB;
+        w[r] = static_cast<const v4u *>(a.W) + at * 64 + lane;
+        s[r] = static_cast<const Scales<GPB, Z> *>(a.S) + at * 16 + c;
+    }
+#pragma unroll
+    for (int n = 0; n < NT; n++) x[n] = static_cast<const T *>(a.X) + (size_t)(t.row + (n * 16 + c < t.rows ? n * 16 + c : t.rows - 1)) * a.K + q * 8;
+
+    typedef Block<GPB, Z, RT, NT> B;
+    auto load = [&](B &b, uint32_t kb) __attribute__((always_inline)) {
+        const uint32_t steps = (a.K - kb * 128) / 32; // of 32 columns, 4 but for the last block
+#pragma unroll
+        for (int r = 0; r < RT; r++) b.w[r] = __builtin_nontemporal_load(w[r] + (size_t)kb * 64);
+#pragma unroll
+        for (int r = 0; r < RT; r++) b.s[r] = s[r][(size_t)kb * 16];
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (uint32_t i = 0; i < 4; i++) b.x[n][i] = i < steps ? *reinterpret_cast<const v8t *>(x[n] + kb * 128 + i * 32) : v8t{};
+    };
+    v4f sum[RT][NT];
+#pragma unroll
+    for (int r = 0; r < RT; r++)
+#pragma unroll
+        for (int n = 0; n < NT; n++) sum[r][n] = (v4f){ 0.f, 0.f, 0.f, 0.f };
+    auto multiply = [&](const B &b) __attribute__((always_inline)) {
+        constexpr int kEach = 4 / GPB; // steps of a group
+#pragma unroll
+        for (int r = 0; r < RT; r++)
+#pragma unroll
+            for (int g = 0; g < GPB; g++) {
+                const float scale = (float)b.s[r].v[Z ? 2 * g : g];
+                Zero        zero;
+                zero.set(Z ? b.s[r].v[2 * g + 1] : (T)8.f);
+                v8t v[kEach];
+#pragma unroll
+                for (int i = 0; i < kEach; i++) v[i] = codes_of(b.w[r][g * kEach + i], zero);
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+                    v4f y = { 0.f, 0.f, 0.f, 0.f };
+#pragma unroll
+                    for (int i = 0; i < kEach; i++) y = mfma(b.x[n][g * kEach + i], v[i], y);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) sum[r][n][i] += scale * y[i];
+                }
+            }
+    };
+    B b[2];
+    uint32_t kb = wave;
+    if (kb < a.KB) {
+        load(b[0], kb);
+        for (; kb + 2 * WK < a.KB; kb += 2 * WK) {
+            load(b[1], kb + WK);
+            multiply(b[0]);
+            load(b[0], kb + 2 * WK);
+            multiply(b[1]);
+        }
+        if (kb + WK < a.KB) {
+            load(b[1], kb + WK);
+            multiply(b[0]);
+            multiply(b[1]);
+        } else {
+            multiply(b[0]);
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < RT; r++)
+#pragma unroll
+        for (int n = 0; n < NT; n++) part[wave][r * NT + n][lane] = sum[r][n];
+    __syncthreads();
+
+    // the sums of tile (r, n): lane c + 16 q has weight row c and rows 4 q + i of X
+    auto total = [&](int p) __attribute__((always_inline)) {
+        v4f y = part[0][p][lane];
+#pragma unroll
+        for (int k = 1; k < WK; k++) y += part[k][p][lane];
+        return y;
+    };
+    const T *bias = a.bias ? static_cast<const T *>(a.bias) + (size_t)t.expert * a.Mt * 16 : nullptr;
+    if (a.act < 0) {
+        for (uint32_t p = wave; p < RT * NT; p += WK) {
+            const uint32_t r = p / NT, n = p % NT, m = (m0 + r) * 16 + c;
+            if (m0 + r >= a.Mt) continue;
+            v4f         y = total(p);
+            const float add = bias ? (float)bias[m] : 0.f;
+#pragma unroll
+            for (uint32_t i = 0; i < 4; i++)
+                if (n * 16 + 4 * q + i < t.rows) store(a, t.row + n * 16 + 4 * q + i, m, a.Mt * 16, y[i] + add);
+        }
+    } else if constexpr (RT % 2 == 0) {
+        for (uint32_t p = wave; p < RT / 2 * NT; p += WK) {
+            const uint32_t r = p / NT * 2, n = p % NT, m = (m0 + r) * 16 + c;
+            if (m0 + r >= a.Mt) continue;
+            v4f         g = total(r * NT + n), u = total((r + 1) * NT + n);
+            const float bg = bias ? (float)bias[m] : 0.f, bu = bias ? (float)bias[m + 16] : 0.f;
+#pragma unroll
+            for (uint32_t i = 0; i < 4; i++)
+                if (n * 16 + 4 * q + i < t.rows) store(a, t.row + n * 16 + 4 * q + i, (m0 + r) * 8 + c, a.Mt * 8, activated(a.act, g[i] + bg) * (u[i] + bu));
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+template <int GPB, bool Z, int RT, int NT, int WK> int launch_stream(hipStream_t st, const Int4Args &a)
+{
+    const size_t tiles = fp6mi::int4_tiles(a.N, a.offsets ? a.E : 0, NT * 16);
+    if (tiles > 65535) return FP6MI_ERR_SHAPE;
+    hipLaunchKernelGGL((int4_stream<GPB, Z, RT, NT, WK>), dim3((a.Mt + RT - 1) / RT, (uint32_t)tiles), dim3(WK * 64), 0, st, a);
+    return (int)hipGetLastError();
+}
+
+template <int GPB, bool Z> int run(hipStream_t st, const Int4Args &a)
+{
+    if (a.N <= 16 || (a.offsets && a.N <= 16 * a.E)) return launch_stream<GPB, Z, 2, 1, 8>(st, a);
+    return launch_stream<GPB, Z, 2, 4, 4>(st, a);
+}
+
+} // namespace
+
+namespace fp6mi {
+#if FP6MI_TYPE == 0
+int int4_run_f16(void *stream, const Int4Args &a, int group, bool zeros)
+#else
+int int4_run_bf16(void *stream, const Int4Args &a, int group, bool zeros)
+#endif
+{
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    if (group == 128) return zeros ? run<1, true>(st, a) : run<1, false>(st, a);
+    if (group == 64) return zeros ? run<2, true>(st, a) : run<2, false>(st, a);
+    return zeros ? run<4, true>(st, a) : run<4, false>(st, a);
+}
+} // namespace fp6mi

@@ -1,0 +1,124 @@
+// Layout and C ABI of the products with 4-bit integer weights (fp6mi_int4.hip; include/fp6mi.h).  No counterpart in the reference.
+#include <hip/hip_runtime.h>
+
+#include "fp6mi_internal.h"
+#include "fp6mi_int4.inc"
+
+namespace {
+
+inline bool aligned(const void *p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+// The nibble of a dword that column j (0..7) of its eight is held in: even ones in the lower 16 bits, odd ones in the upper.
+__host__ __device__ inline uint32_t nibble_of(uint32_t j) { return (j & 1) * 4 + j / 2; }
+
+// Dword i of the native layout of one matrix from its codes, two to a byte, the even column in the low half.
+__host__ __device__ inline uint32_t native_dword(const uint8_t *codes, size_t i, uint32_t K, uint32_t KB)
+{
+    const uint32_t s = i & 3, lane = i >> 2 & 63, k = (uint32_t)((i >> 8) % KB) * 128 + s * 32 + (lane >> 4) * 8;
+    const size_t   row = (i >> 8) / KB * 16 + (lane & 15);
+    uint32_t       d = 0;
+    if (k < K) // (K is a multiple of 32)
+        for (uint32_t j = 0; j < 8; j++) d |= (codes[(row * K + k + j) / 2] >> 4 * (j & 1) & 15u) << 4 * nibble_of(j);
+    return d;
+}
+
+// Element i of the native scales (16 bits), of {scale, zero point} pairs with zero points; `each` columns to a native group (32, 64 or 128).
+__host__ __device__ inline uint16_t native_scale(const uint16_t *scales, const uint8_t *zeros, int bf16, size_t i, uint32_t K, uint32_t KB, uint32_t group, uint32_t each)
+{
+    const uint32_t per = 128 / each, groups = (K + group - 1) / group;
+    const size_t   p = zeros ? i >> 1 : i;
+    const uint32_t row = (uint32_t)(p / per % 16), k = (uint32_t)(p / per / 16 % KB) * 128 + (uint32_t)(p % per) * each;
+    const size_t   at = (p / per / 16 / KB * 16 + row) * groups + k / group;
+    if (k >= K) return 0;
+    if (!zeros || (i & 1) == 0) return scales[at];
+    const uint32_t z = zeros[at] & 15; // as a number of the scales' type, which holds it exactly
+    if (z == 0) return 0;
+    uint32_t e = 3;
+    while (!(z >> e)) e--;
+    return bf16 ? (uint16_t)((127 + e) << 7 | (z << (7 - e) & 127)) : (uint16_t)((15 + e) << 10 | (z << (10 - e) & 1023));
+}
+
+__global__ __launch_bounds__(256) void pack_codes(uint32_t *__restrict__ out, const uint8_t *__restrict__ codes, size_t count, uint32_t K, uint32_t KB, size_t matrix)
+{
+    const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
+    if (i < count) out[i] = native_dword(codes + i / matrix * (matrix / (KB * 16) * (K / 2)), i % matrix, K, KB);
+}
+__global__ __launch_bounds__(256) void pack_scales(uint16_t *__restrict__ out, const uint16_t *__restrict__ scales, const uint8_t *__restrict__ zeros, int bf16, size_t count, uint32_t K, uint32_t KB,
+                                                   uint32_t group, uint32_t each)
+{
+    const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
+    if (i < count) out[i] = native_scale(scales, zeros, bf16, i, K, KB, group, each);
+}
+
+inline uint32_t native_group(size_t group) { return group % 128 == 0 ? 128 : group % 64 == 0 ? 64 : 32; }
+
+int check_shape(size_t experts, size_t M, size_t K)
+{
+    if (M == 0 || M % 16 || K == 0 || K % 32 || K > (size_t)1 << 24 || M > (size_t)1 << 24 || experts == 0 || experts > 1024) return FP6MI_ERR_SHAPE;
+    return experts * (M / 16) * ((K + 127) / 128) > (size_t)1 << 31 ? FP6MI_ERR_SHAPE : FP6MI_OK;
+}
+
+int check_pack(const void *native, const void *native_scales, const void *codes, const void *scales, int dtype, size_t experts, size_t M, size_t K, size_t group)
+{
+    if (dtype != 0 && dtype != 1) return FP6MI_ERR_TYPE;
+    if (const int e = check_shape(experts, M, K)) return e;
+    if (group == 0 || group % 32 || group > (size_t)1 << 24) return FP6MI_ERR_SHAPE;
+    if (!native || !native_scales || !codes || !scales) return FP6MI_ERR_NULL;
+    return aligned(native, 16) && aligned(native_scales, 16) && aligned(scales, 2) ? FP6MI_OK : FP6MI_ERR_ALIGN;
+}
+
+} // namespace
+
+extern "C" {
+
+size_t fp6mi_int4_weight_bytes(size_t experts, size_t M, size_t K) { return check_shape(experts, M, K) ? 0 : experts * (M / 16) * ((K + 127) / 128) * 1024; }
+
+size_t fp6mi_int4_scale_bytes(size_t experts, size_t M, size_t K, size_t group, int zeros)
+{
+    if (check_shape(experts, M, K) || group == 0 || group % 32) return 0;
+    return experts * M * ((K + 127) / 128) * (128 / native_group(group)) * (zeros ? 4 : 2);
+}
+
+int fp6mi_int4_pack(void *native, void *native_scales, const void *codes, const void *scales, const void *zeros, int dtype, size_t experts, size_t M, size_t K, size_t group)
+{
+    if (const int e = check_pack(native, native_scales, codes, scales, dtype, experts, M, K, group)) return e;
+    const uint32_t KB = (uint32_t)((K + 127) / 128);
+    const size_t   matrix = M / 16 * KB * 256, count = fp6mi_int4_scale_bytes(experts, M, K, group, zeros != nullptr) / 2;
+    for (size_t e = 0; e < experts; e++)
+        for (size_t i = 0; i < matrix; i++) static_cast<uint32_t *>(native)[e * matrix + i] = native_dword(static_cast<const uint8_t *>(codes) + e * M * (K / 2), i, (uint32_t)K, KB);
+    for (size_t i = 0; i < count; i++)
+        static_cast<uint16_t *>(native_scales)[i] =
+            native_scale(static_cast<const uint16_t *>(scales), static_cast<const uint8_t *>(zeros), dtype, i, (uint32_t)K, KB, (uint32_t)group, native_group(group));
+    return FP6MI_OK;
+}
+
+int fp6mi_int4_pack_gpu(void *stream, void *native, void *native_scales, const void *codes, const void *scales, const void *zeros, int dtype, size_t experts, size_t M, size_t K, size_t group)
+{
+    if (const int e = check_pack(native, native_scales, codes, scales, dtype, experts, M, K, group)) return e;
+    const uint32_t KB = (uint32_t)((K + 127) / 128);
+    const size_t   matrix = M / 16 * KB * 256, dwords = experts * matrix, count = fp6mi_int4_scale_bytes(experts, M, K, group, zeros != nullptr) / 2;
+    if (dwords / 256 > 0x7fffffffu || (count + 255) / 256 > 0x7fffffffu) return FP6MI_ERR_SHAPE;
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    hipLaunchKernelGGL(pack_codes, dim3((uint32_t)(dwords / 256)), dim3(256), 0, st, static_cast<uint32_t *>(native), static_cast<const uint8_t *>(codes), dwords, (uint32_t)K, KB, matrix);
+    if (const hipError_t e = hipGetLastError()) return (int)e;
+    hipLaunchKernelGGL(pack_scales, dim3((uint32_t)((count + 255) / 256)), dim3(256), 0, st, static_cast<uint16_t *>(native_scales), static_cast<const uint16_t *>(scales),
+                       static_cast<const uint8_t *>(zeros), dtype, count, (uint32_t)K, KB, (uint32_t)group, native_group(group));
+    return (int)hipGetLastError();
+}
+
+int fp6mi_int4_linear(void *stream, int dtype, const void *W_native, const void *scales_native, int group, int zeros, const void *bias, const void *X, void *Y, int out_f32, int activation,
+                      const int *offsets, size_t experts, size_t M, size_t N, size_t K)
+{
+    if (dtype != 0 && dtype != 1) return FP6MI_ERR_TYPE;
+    if (const int e = check_shape(experts, M, K)) return e;
+    if ((group != 32 && group != 64 && group != 128) || N > (size_t)1 << 30 || (!offsets && experts != 1)) return FP6MI_ERR_SHAPE;
+    if (activation > FP6MI_ACT_GELU_TANH) return FP6MI_ERR_ACTIVATION;
+    if (activation >= 0 && M % 32) return FP6MI_ERR_SHAPE;
+    if (N == 0) return FP6MI_OK;
+    if (!W_native || !scales_native || !X || !Y) return FP6MI_ERR_NULL;
+    if (!aligned(W_native, 16) || !aligned(scales_native, 16) || !aligned(X, 16) || !aligned(Y, 16) || !aligned(bias, 2) || !aligned(offsets, 4)) return FP6MI_ERR_ALIGN;
+    const fp6mi::Int4Args a = { W_native, scales_native, X, bias, Y, offsets, (uint32_t)N, (uint32_t)K, (uint32_t)((K + 127) / 128), (uint32_t)(M / 16), (uint32_t)experts, activation, out_f32 };
+    return dtype ? fp6mi::int4_run_bf16(stream, a, group, zeros != 0) : fp6mi::int4_run_f16(stream, a, group, zeros != 0);
+}
+
+} // extern "C"

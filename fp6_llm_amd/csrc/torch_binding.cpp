@@ -569,6 +569,127 @@ at::Tensor adapter_forward(int64_t E, int64_t Mb, const at::Tensor &in_feats, co
     return out;
 }
 
+// ---- 4-bit integer weights (fp6_llm_amd/int4.py) and rows of experts (fp6_llm_amd/experts.py) ----
+int type_code(at::ScalarType t) { return t == at::kHalf ? 0 : t == at::kBFloat16 ? 1 : t == at::kFloat ? 2 : -1; }
+
+at::Tensor int4_forward(const at::Tensor &in_feats, const at::Tensor &native, const at::Tensor &s, const OptTensor &offsets, int64_t places, int64_t act, const OptTensor &bias, const OptTensor &out_opt,
+                        bool f32)
+{
+    const bool         grouped = offsets.has_value();
+    const int64_t      dims = grouped ? 6 : 5;
+    const at::ScalarType type = s.scalar_type();
+    if ((type != at::kHalf && type != at::kBFloat16) || s.dim() != dims || s.size(-3) != 16 || (s.size(-2) != 1 && s.size(-2) != 2 && s.size(-2) != 4) || (s.size(-1) != 1 && s.size(-1) != 2) ||
+        !s.is_contiguous())
+        bad(std::string("native_scales must be those of int4_pack_native, ") + (grouped ? "of experts" : "of one matrix"));
+    const at::Device dev = s.device();
+    if (in_feats.scalar_type() != type || in_feats.dim() != 2 || !in_feats.is_cuda() || in_feats.device() != dev || native.device() != dev)
+        bad("in_feats must be 2-D of the scales' type, on the weights' GPU");
+    const int64_t B = in_feats.size(0), IC = in_feats.size(1), tiles = s.size(-5), KB = s.size(-4), OC = 16 * tiles, E = grouped ? s.size(0) : 1;
+    if (IC < 32 || IC % 32 || (IC + 127) / 128 != KB) bad("in_feats has IC=" + std::to_string(IC) + " columns, the weights have " + std::to_string(KB) + " blocks of 128");
+    if (native.scalar_type() != at::kInt || native.dim() != dims - 2 || native.size(-1) != 256 || native.size(-2) != KB || native.size(-3) != tiles || (grouped && native.size(0) != E) ||
+        !native.is_contiguous())
+        bad("native_weight must be that of int4_pack_native with these scales");
+    if (act >= 0 && OC % 32) bad("a gated product needs OC % 32 == 0, got " + std::to_string(OC));
+    if (grouped && (offsets->scalar_type() != at::kInt || offsets->dim() != 1 || offsets->size(0) != E + 1 || !offsets->is_contiguous() || offsets->device() != dev || B != places))
+        bad("the plan must be of " + std::to_string(E) + " experts and as many places as in_feats has rows, on the same GPU");
+    if (bias.has_value() && (bias->scalar_type() != type || bias->dim() != (grouped ? 2 : 1) || bias->size(-1) != OC || (grouped && bias->size(0) != E) || !bias->is_contiguous() || bias->device() != dev))
+        bad("bias must be contiguous, of the scales' type, one for each row of the weights, on the same GPU");
+    const at::Tensor     x = in_feats.is_contiguous() ? in_feats : in_feats.contiguous();
+    c10::hip::HIPGuard   guard(dev.index());
+    const at::ScalarType to = f32 ? at::kFloat : type;
+    const int64_t        cols = act >= 0 ? OC / 2 : OC;
+    at::Tensor           out;
+    if (out_opt.has_value()) {
+        out = *out_opt;
+        if (out.dim() != 2 || out.size(0) != B || out.size(1) != cols || out.scalar_type() != to || !out.is_contiguous() || out.device() != dev)
+            bad("out must be a contiguous [" + std::to_string(B) + ", " + std::to_string(cols) + "] tensor of the output's type on the same GPU");
+    } else {
+        out = at::empty({ B, cols }, at::TensorOptions().dtype(to).device(dev));
+    }
+    raise_status(fp6mi_int4_linear(c10::hip::getCurrentHIPStream(dev.index()).stream(), type_code(type), native.data_ptr(), s.data_ptr(), 128 / (int)s.size(-2), (int)s.size(-1) - 1, pointer(bias),
+                                   x.data_ptr(), out.data_ptr(), f32, (int)act, grouped ? offsets->data_ptr<int>() : nullptr, (size_t)E, (size_t)OC, (size_t)B, (size_t)IC),
+                 "fp6mi_int4_linear");
+    return out;
+}
+
+pybind11::object expert_sort(const OptTensor &x_opt, const at::Tensor &index_in, int64_t experts)
+{
+    const at::Device dev = index_in.device();
+    if ((index_in.scalar_type() != at::kInt && index_in.scalar_type() != at::kLong) || index_in.dim() != 2 || !index_in.is_cuda())
+        bad("index must be a 2-D int32 or int64 tensor [tokens, k] on the GPU");
+    const int64_t T = index_in.size(0), k = index_in.size(1);
+    if (k < 1 || k > 64 || experts < 1 || experts > 1024 || T > ((int64_t)1 << 30) / k) bad("need 1 to 64 experts of a token, 1 to 1024 in all, and up to 2^30 places");
+    c10::hip::HIPGuard guard(dev.index());
+    OptTensor          rows;
+    at::Tensor         x;
+    int64_t            H = 0, ld = 0;
+    if (x_opt.has_value()) {
+        x = *x_opt;
+        if (type_code(x.scalar_type()) < 0 || x.dim() != 2 || x.size(0) != T || x.size(1) < 1 || x.size(1) > 1 << 24 || x.device() != dev)
+            bad("x must be float16, bfloat16 or float32 [tokens=" + std::to_string(T) + ", features], on the index's GPU");
+        H = x.size(1);
+        if (x.stride(1) != 1 || (T > 1 && x.stride(0) < H)) x = x.contiguous();
+        ld = x.stride(0);
+        rows = at::empty({ T * k, H }, x.options());
+    }
+    const at::Tensor index = index_in.contiguous();
+    const auto       ints = at::TensorOptions().dtype(at::kInt).device(dev);
+    const at::Tensor offsets = at::empty({ experts + 1 }, ints), order = at::empty({ T * k }, ints), place = at::empty({ T * k }, ints);
+    void            *stream = c10::hip::getCurrentHIPStream(dev.index()).stream();
+    at::Tensor       keep;
+    float           *ws = scratch(c10::nullopt, dev, stream, fp6mi_expert_sort_workspace_bytes((size_t)T, (size_t)k, (size_t)experts), keep);
+    raise_status(fp6mi_expert_sort(stream, index.data_ptr(), index.scalar_type() == at::kLong, offsets.data_ptr<int>(), order.data_ptr<int>(), place.data_ptr<int>(), x.defined() ? x.data_ptr() : nullptr,
+                                   (size_t)ld, rows.has_value() ? rows->data_ptr() : nullptr, (size_t)T, (size_t)k, (size_t)experts, (size_t)H, x.defined() ? type_code(x.scalar_type()) : 0, ws),
+                 "fp6mi_expert_sort");
+    return pybind11::make_tuple(rows, offsets, order, place);
+}
+
+// The plan's tensors come from expert_sort; they are looked at again, since a caller may hold a plan of its own making.
+void check_plan(const at::Tensor &place, const at::Tensor &offsets, int64_t places, const at::Device &dev)
+{
+    if (place.scalar_type() != at::kInt || place.dim() != 1 || place.size(0) != places || !place.is_contiguous() || place.device() != dev || offsets.scalar_type() != at::kInt || offsets.dim() != 1 ||
+        offsets.size(0) < 2 || !offsets.is_contiguous() || offsets.device() != dev)
+        bad("the plan must be that of expert_sort or expert_plan, on the rows' GPU");
+}
+
+at::Tensor expert_combine(const at::Tensor &rows_in, const at::Tensor &place, const at::Tensor &offsets, const OptTensor &weights, int64_t tokens, int64_t k, at::ScalarType to)
+{
+    const int        row_type = type_code(rows_in.scalar_type()), out_type = type_code(to);
+    const at::Device dev = rows_in.device();
+    if (row_type < 0 || rows_in.dim() != 2 || rows_in.size(0) != tokens * k || rows_in.size(1) < 1 || rows_in.size(1) > 1 << 24 || !rows_in.is_cuda() || dev != place.device())
+        bad("rows must be float16, bfloat16 or float32 [tokens * k = " + std::to_string(tokens * k) + ", features], on the plan's GPU");
+    if (out_type < 0 || (out_type != row_type && row_type != 2)) bad("sums have the rows' type, those of float32 rows any");
+    check_plan(place, offsets, tokens * k, dev);
+    if (weights.has_value()) check_tensor(*weights, { tokens, k }, at::kFloat, dev, "weights");
+    c10::hip::HIPGuard guard(dev.index());
+    const at::Tensor   rows = rows_in.contiguous(), out = at::empty({ tokens, rows.size(1) }, at::TensorOptions().dtype(to).device(dev));
+    raise_status(fp6mi_expert_combine(c10::hip::getCurrentHIPStream(dev.index()).stream(), rows.data_ptr(), place.data_ptr<int>(), offsets.data_ptr<int>() + offsets.size(0) - 1,
+                                      static_cast<const float *>(pointer(weights)), out.data_ptr(), (size_t)tokens, (size_t)k, (size_t)rows.size(1), row_type, out_type),
+                 "fp6mi_expert_combine");
+    return out;
+}
+
+pybind11::object expert_combine_backward(const at::Tensor &grad, const OptTensor &rows, const at::Tensor &place, const at::Tensor &offsets, const OptTensor &weights, int64_t k, at::ScalarType row_dtype,
+                                         bool want_rows, bool want_weights)
+{
+    const at::Device dev = grad.device();
+    const int64_t    tokens = grad.size(0), H = grad.size(1);
+    check_plan(place, offsets, tokens * k, dev);
+    if (want_weights && (!rows.has_value() || rows->scalar_type() != row_dtype)) bad("the gradient of the weights needs the rows");
+    if (rows.has_value()) check_tensor(*rows, { tokens * k, H }, rows->scalar_type(), dev, "rows");
+    if (weights.has_value()) check_tensor(*weights, { tokens, k }, at::kFloat, dev, "weights");
+    c10::hip::HIPGuard guard(dev.index());
+    OptTensor          grad_rows, grad_weights;
+    if (want_rows) grad_rows = at::empty({ tokens * k, H }, at::TensorOptions().dtype(row_dtype).device(dev));
+    if (want_weights) grad_weights = at::empty({ tokens, k }, at::TensorOptions().dtype(at::kFloat).device(dev));
+    raise_status(fp6mi_expert_combine_backward(c10::hip::getCurrentHIPStream(dev.index()).stream(), grad.data_ptr(), pointer(rows), place.data_ptr<int>(),
+                                               offsets.data_ptr<int>() + offsets.size(0) - 1, static_cast<const float *>(pointer(weights)), const_cast<void *>(pointer(grad_rows)),
+                                               static_cast<float *>(const_cast<void *>(pointer(grad_weights))), (size_t)tokens, (size_t)k, (size_t)H, type_code(row_dtype),
+                                               type_code(grad.scalar_type())),
+                 "fp6mi_expert_combine_backward");
+    return pybind11::make_tuple(grad_rows, grad_weights);
+}
+
 // Whether a backward pass from t would reach a node that runs on another stream of t's device than the current one: one that an eager graph made, a leaf's own (of an eager graph that
 // still lives) among them.
 bool gradient_goes_elsewhere(const at::Tensor &t)
@@ -610,6 +731,10 @@ PYBIND11_MODULE(_fp6mi_torch, m)
     m.def("gated_backward", &gated_backward);
     m.def("linear_input_grad", &linear_input_grad);
     m.def("adapter_forward", &adapter_forward);
+    m.def("int4_forward", &int4_forward);
+    m.def("expert_sort", &expert_sort);
+    m.def("expert_combine", &expert_combine);
+    m.def("expert_combine_backward", &expert_combine_backward);
     m.def("gradient_goes_elsewhere", &gradient_goes_elsewhere);
     // the reference's bindings, name for name (fp6_llm/csrc/pybind.cpp:8-15)
     m.def("linear_forward_cuda", &fp6_linear_forward_cuda, "Computes FP6-FP16 GEMM.", pybind11::arg("in_feats"), pybind11::arg("weights"),

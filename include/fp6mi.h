@@ -40,6 +40,7 @@ extern "C" {
 #define FP6MI_ERR_ALIGN (-6)     /* a device pointer is not 16-byte aligned (scales, group exponents: 2-byte) */
 #define FP6MI_ERR_TOO_LARGE (-7) /* the problem exceeds the static workspace of fp6mi_linear_native_static */
 #define FP6MI_ERR_ACTIVATION (-9) /* not one of FP6MI_ACT_*                  */
+#define FP6MI_ERR_TYPE (-10)     /* an element type that the operator lacks */
 #define FP6MI_ERR_CAPTURE (-8)   /* the call would have to allocate while its stream is being captured */
 
 const char *fp6mi_error_string(int code);
@@ -259,6 +260,40 @@ int    fp6mi_adapter_native(int E, int Mbits, void *stream, const void *W_native
                             void *C_f16, const void *lora_a_f16, const void *lora_b_f16, const float *scaling, const int *index, size_t M, size_t N, size_t K, size_t R, size_t slots,
                             float *workspace, int splitK);
 size_t fp6mi_adapter_workspace_bytes(size_t M, size_t N, size_t K, size_t R, int splitK);
+
+/* ---------------------------------------------------------------------------------- 4-bit integer weights with a scale for each group of columns (beyond the reference)
+ * w[m,k] = s[m,g] * (q[m,k] - z[m,g]), q a code of 4 bits, g = k / group, z a zero point from 0 to 15 (8 where there are none).  dtype: 0 = fp16, 1 = bf16, of the scales and of the activations
+ * that are multiplied with them.  `experts` matrices of one shape lie one behind the other (1: a single one).  M % 16 == 0, K % 32 == 0, group % 32 == 0 (a last one may be cut).
+ * codes: [experts][M][K/2] bytes, the even column in the low half; scales: 16 bits [experts][M][ceil(K/group)]; zeros: bytes like the scales, or NULL.  The native layout of the weights is
+ * fp6mi_int4_weight_bytes bytes, that of the scales (with the zero points) fp6mi_int4_scale_bytes; in it a group is 128, 64 or 32 columns, the largest of these that divides the group.
+ * Sizes are 0 for a shape that is refused. */
+size_t fp6mi_int4_weight_bytes(size_t experts, size_t M, size_t K);
+size_t fp6mi_int4_scale_bytes(size_t experts, size_t M, size_t K, size_t group, int zeros);
+int    fp6mi_int4_pack(void *native, void *native_scales, const void *codes, const void *scales, const void *zeros, int dtype, size_t experts, size_t M, size_t K, size_t group); /* host */
+int    fp6mi_int4_pack_gpu(void *stream, void *native, void *native_scales, const void *codes, const void *scales, const void *zeros, int dtype, size_t experts, size_t M, size_t K, size_t group);
+/* Y[N,M] = X[N,K] . w^T + bias; with an activation (FP6MI_ACT_*, negative: none) Y[N,M/2] = act(gate) * up for weights whose rows are in pair order, 16 of gate, the same 16 of up, and so on
+ * (M % 32 == 0; bias likewise).  group: the native one (32, 64, 128).  bias: of the activations' type, [experts][M], or NULL.  out_f32: Y is float32, else of the activations' type.
+ * offsets: NULL for one matrix, or experts + 1 row numbers on the device, as fp6mi_expert_sort writes them: rows offsets[e] to offsets[e+1] - 1 are multiplied with the weights of expert e, rows from
+ * offsets[experts] on become zeros.  Products are exact, sums float32 (of a group before its scale, of the scaled groups behind it), rounded once. */
+int    fp6mi_int4_linear(void *stream, int dtype, const void *W_native, const void *scales_native, int group, int zeros, const void *bias, const void *X, void *Y, int out_f32, int activation,
+                         const int *offsets, size_t experts, size_t M, size_t N, size_t K);
+
+/* ---------------------------------------------------------------------------------- rows of experts (beyond the reference)
+ * index[tokens][k] names the experts of every token (int64 if index64, else int32; a number outside 0..experts-1 is none); place p = t * k + j.  Sorting puts the places in order of their
+ * experts, ties in their own order, those without one last: place[p] is where place p goes (a permutation of 0..tokens*k-1), order its inverse (-1 for places without an expert),
+ * offsets[e], e = 0..experts, the number of places of the experts below e.  All int32 on the device.  rows, unless NULL: [tokens*k][H] receives row t of x (ldx elements from one row to the
+ * next) at the places of token t, and zeros at those without an expert.  dtype as in the quantizer (0 = fp16, 1 = bf16, 2 = fp32).  k up to 64, experts up to 1024, tokens * k up to 2^30.
+ * workspace: fp6mi_expert_sort_workspace_bytes bytes (none for few places), 16-byte aligned. */
+size_t fp6mi_expert_sort_workspace_bytes(size_t tokens, size_t k, size_t experts);
+int    fp6mi_expert_sort(void *stream, const void *index, int index64, int *offsets, int *order, int *place, const void *x, size_t ldx, void *rows, size_t tokens, size_t k, size_t experts, size_t H,
+                         int dtype, void *workspace);
+/* out[t] = sum over j of weights[t][j] * rows[place[t*k+j]], those with an expert (place < *valid, which is offsets[experts]), in float32 in the order of j, rounded once.  weights: float32
+ * [tokens][k], NULL: all 1 (the gradient of sorting).  out_type: row_type, or fp16 or bf16 for float32 rows. */
+int    fp6mi_expert_combine(void *stream, const void *rows, const int *place, const int *valid, const float *weights, void *out, size_t tokens, size_t k, size_t H, int row_type, int out_type);
+/* Its gradient from that of out (out_type): grad_rows[place] = weights * grad (row_type; zeros at places without an expert), grad_weights = <grad[t], rows[place]> (float32; zero there).  Either may
+ * be NULL, rows may be without grad_weights. */
+int    fp6mi_expert_combine_backward(void *stream, const void *grad, const void *rows, const int *place, const int *valid, const float *weights, void *grad_rows, float *grad_weights,
+                                     size_t tokens, size_t k, size_t H, int row_type, int out_type);
 
 #ifdef __cplusplus
 }
