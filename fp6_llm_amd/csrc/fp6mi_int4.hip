@@ -10,6 +10,7 @@
 // 16 bits apart.  Scales: [expert][row tile][column block][row][group of the block], with zero points {scale, zero point} in pairs, both of the activations' type.
 #include <hip/hip_runtime.h>
 
+#include <atomic>
 #include <type_traits>
 
 #include "fp6mi_internal.h"
@@ -23,6 +24,8 @@ typedef _Float16 T;
 #else
 typedef __bf16 T;
 #endif
+#include "fp6mi_lds.inc"
+
 typedef _Float16 v2h __attribute__((ext_vector_type(2)));
 typedef T        v8t __attribute__((ext_vector_type(8)));
 typedef float    v4f __attribute__((ext_vector_type(4)));
@@ -263,9 +266,202 @@ template <int GPB, bool Z, int RT, int NT, int WK> int launch_stream(hipStream_t
     return (int)hipGetLastError();
 }
 
+// ---------------------------------------------------------------------------------------------------------------
+// Many rows: tiles of WR * RT * 16 weight rows x WC * NT * 16 rows of X to a workgroup of WR * WC wavefronts.  X goes to LDS by direct transfers, a K block ahead, two stages; a row of a stage is 256
+// bytes whose 16 pieces stand in the order piece ^ (row & 15), which gives the reads of an MFMA operand all banks.  A wavefront holds its rows of X for one block in registers and takes one row tile after
+// another: its codes become operands while the tile before is multiplied.  Bound by the matrix units with the conversions and the scaling of the group sums beside them (VALU).
+// ---------------------------------------------------------------------------------------------------------------
+constexpr size_t tile_lds_bytes(int cols, int rows) // the stages, and the outputs on their way out: a half of them at a time where they are float32
+{
+    const size_t stages = 2 * (size_t)cols * 256, outputs = (size_t)cols * (rows * 2 + 16);
+    return stages > outputs ? stages : outputs;
+}
+
+template <int GPB, bool Z, int RT, int NT, int WR, int WC> __global__ __launch_bounds__(WR *WC * 64) void int4_tile(const Int4Args a, uint32_t col_tiles)
+{
+    static_assert(RT % 2 == 0, "");
+    constexpr int      kWaves = WR * WC, kCols = WC * NT * 16, kTiles = WR * RT, kRows = kTiles * 16, kStage = kCols * 256, kDma = kCols / 4 / kWaves;
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, q = lane >> 4, wr = wave % WR, wc = wave / WR;
+
+    // Workgroups that an XCD runs side by side are panels of eight row blocks by a few column tiles, mostly of one expert.
+    const uint32_t per = gridDim.x >> 3, rem = gridDim.x & 7u, xcd = blockIdx.x & 7u, id = xcd * per + (xcd < rem ? xcd : rem) + (blockIdx.x >> 3);
+    const uint32_t row_blocks = gridDim.x / col_tiles, first = id / (8 * col_tiles) * 8, in = id - first * col_tiles, high = row_blocks - first < 8 ? row_blocks - first : 8;
+    const uint32_t m0 = (first + in % high) * kTiles;
+    const Tile     t = tile_of(a, in / high, kCols);
+    if (t.rows == 0) return;
+    if (t.expert < 0) return store_zeros(a, t, m0, kTiles, kWaves * 64);
+
+    // transfers of X: four rows of one block each
+    typedef __attribute__((address_space(3))) void lvoid;
+    const auto     xbuf = __builtin_amdgcn_make_buffer_rsrc(const_cast<T *>(static_cast<const T *>(a.X) + (size_t)t.row * a.K), 0, (int)(t.rows * a.K * 2), 0x00027000);
+    uint32_t       xrow[kDma], xpiece[kDma];
+#pragma unroll
+    for (uint32_t j = 0; j < kDma; j++) {
+        const uint32_t row = (j * kWaves + wave) * 4 + q;
+        xrow[j] = (row < t.rows ? row : t.rows - 1) * a.K * 2; // 32 bits: the launcher bounds K
+        xpiece[j] = (c ^ (row & 15)) * 8;
+    }
+    auto transfer = [&](uint32_t kb, uint32_t stage) __attribute__((always_inline)) {
+#pragma unroll
+        for (uint32_t j = 0; j < kDma; j++) {
+            const uint32_t k = kb * 128 + xpiece[j], off = xrow[j] + (k < a.K ? k * 2 : 0xc0000000u); // (beyond the buffer, which reads as zeros)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(xbuf, (lvoid *)(lds + stage * kStage + (j * kWaves + wave) * 1024), 16, off, 0, 0, 0);
+        }
+    };
+    const uint8_t *xread = lds + (wc * NT * 16 + c) * 256;
+    v8t            x[NT][4];
+    auto           read_x = [&](int n, uint32_t stage) __attribute__((always_inline)) {
+#pragma unroll
+        for (uint32_t i = 0; i < 4; i++) x[n][i] = *reinterpret_cast<const v8t *>(xread + stage * kStage + n * 16 * 256 + ((4 * i + q) ^ c) * 16);
+    };
+
+    // codes and scales: two blocks on their way
+    const v4u            *w[RT];
+    const Scales<GPB, Z> *s[RT];
+#pragma unroll
+    for (uint32_t r = 0; r < RT; r++) { // (row tiles beyond the last one take it again)
+        const uint32_t m = m0 + wr * RT + r;
+        const size_t   at = ((size_t)t.expert * a.Mt + (m < a.Mt ? m : a.Mt - 1)) * a.KB;
+        w[r] = static_cast<const v4u *>(a.W) + at * 64 + lane;
+        s[r] = static_cast<const Scales<GPB, Z> *>(a.S) + at * 16 + c;
+    }
+    v4u            raw[2][RT];
+    Scales<GPB, Z> scales[2][RT];
+    auto           load_w = [&](int set, uint32_t kb) __attribute__((always_inline)) {
+        kb = kb < a.KB ? kb : a.KB - 1;
+#pragma unroll
+        for (int r = 0; r < RT; r++) raw[set][r] = w[r][(size_t)kb * 64], scales[set][r] = s[r][(size_t)kb * 16];
+    };
+    v8t  op[2][4];
+    auto convert = [&](int to, int set, int r) __attribute__((always_inline)) {
+#pragma unroll
+        for (int g = 0; g < GPB; g++) {
+            Zero zero;
+            zero.set(Z ? scales[set][r].v[2 * g + 1] : (T)8.f);
+#pragma unroll
+            for (int i = 0; i < 4 / GPB; i++) op[to][g * (4 / GPB) + i] = codes_of(raw[set][r][g * (4 / GPB) + i], zero);
+        }
+    };
+    v4f sum[RT][NT];
+#pragma unroll
+    for (int r = 0; r < RT; r++)
+#pragma unroll
+        for (int n = 0; n < NT; n++) sum[r][n] = (v4f){ 0.f, 0.f, 0.f, 0.f };
+
+    // one block, whose X is in registers and whose first row tile is converted; leaves the same of the next one
+    auto block = [&](auto set_c, uint32_t kb) __attribute__((always_inline)) {
+        constexpr int set = decltype(set_c)::value;
+        float         scale[RT][GPB];
+#pragma unroll
+        for (int r = 0; r < RT; r++)
+#pragma unroll
+            for (int g = 0; g < GPB; g++) scale[r][g] = (float)scales[set][r].v[Z ? 2 * g : g];
+#pragma unroll
+        for (int r = 0; r < RT; r++) {
+            if (r == RT - 1) { // the next block's X has landed, and all have read this one's
+                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+                transfer(kb + 2, set);
+                load_w(set, kb + 2);
+                convert(0, set ^ 1, 0);
+            } else {
+                convert((r + 1) & 1, set, r + 1);
+            }
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+#pragma unroll
+                for (int g = 0; g < GPB; g++) {
+                    v4f y = { 0.f, 0.f, 0.f, 0.f };
+#pragma unroll
+                    for (int i = g * (4 / GPB); i < (g + 1) * (4 / GPB); i++) y = mfma(x[n][i], op[r & 1][i], y);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) sum[r][n][i] += scale[r][g] * y[i];
+                }
+                if (r == RT - 1) read_x(n, set ^ 1);
+            }
+        }
+    };
+    transfer(0, 0);
+    load_w(0, 0);
+    asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+    transfer(1, 1);
+    load_w(1, 1);
+#pragma unroll
+    for (int n = 0; n < NT; n++) read_x(n, 0);
+    convert(0, 0, 0);
+    uint32_t kb = 0;
+    for (; kb + 2 <= a.KB; kb += 2) {
+        block(std::integral_constant<int, 0>{}, kb);
+        block(std::integral_constant<int, 1>{}, kb + 1);
+    }
+    if (kb < a.KB) block(std::integral_constant<int, 0>{}, kb);
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); // nothing is on its way to LDS any more
+
+    // outputs through LDS, so that a lane stores 16 bytes: [row of X][weight row], rows 16 bytes apart from a multiple of 512
+    const T *bias = a.bias ? static_cast<const T *>(a.bias) + (size_t)t.expert * a.Mt * 16 : nullptr;
+    auto     out = [&](auto type, auto gated_c) __attribute__((always_inline)) {
+        typedef decltype(type) O;
+        constexpr bool     gated = decltype(gated_c)::value;
+        constexpr uint32_t kHalves = sizeof(O) == 4 && !gated ? 2 : 1, kOut = gated ? kRows / 2 : kRows, kPitch = kOut * sizeof(O) + 16, kEach = 16 / sizeof(O);
+        static_assert((size_t)kCols / kHalves * kPitch <= tile_lds_bytes(kCols, kRows), "");
+        const uint32_t ld = a.Mt * (gated ? 8 : 16), col0 = m0 * (gated ? 8 : 16);
+#pragma unroll
+        for (uint32_t h = 0; h < kHalves; h++) {
+            if (h) __syncthreads();
+#pragma unroll
+            for (uint32_t n = 0; n < NT; n++) {
+                const uint32_t row = (wc * NT + n) * 16 + 4 * q - h * (kCols / kHalves);
+                if (row >= kCols / kHalves) continue; // (the other half's)
+#pragma unroll
+                for (uint32_t r = 0; r < RT; r += gated ? 2 : 1) {
+                    const uint32_t m = (m0 + wr * RT + r) * 16 + c;
+                    const bool     in = bias && m0 + wr * RT + r < a.Mt;
+                    const float    b0 = in ? (float)bias[m] : 0.f, b1 = gated && in ? (float)bias[m + 16] : 0.f;
+#pragma unroll
+                    for (uint32_t i = 0; i < 4; i++) {
+                        float v = sum[r][n][i] + b0;
+                        if constexpr (gated) v = activated(a.act, v) * (sum[r + 1][n][i] + b1);
+                        reinterpret_cast<O *>(lds + (row + i) * kPitch)[gated ? (wr * RT + r) * 8 + c : (wr * RT + r) * 16 + c] = (O)v;
+                    }
+                }
+            }
+            __syncthreads();
+            constexpr uint32_t kPieces = kOut / kEach; // of a row
+            for (uint32_t i = tid; i < kCols / kHalves * kPieces; i += kWaves * 64) {
+                const uint32_t row = i / kPieces, piece = i % kPieces, col = col0 + piece * kEach, n = h * (kCols / kHalves) + row;
+                if (n < t.rows && col < ld) // (ld is a multiple of 8)
+                    *reinterpret_cast<v4u *>(static_cast<O *>(a.Y) + (size_t)(t.row + n) * ld + col) = *reinterpret_cast<const v4u *>(lds + row * kPitch + piece * 16);
+            }
+        }
+    };
+    if (a.act < 0) {
+        if (a.out_f32)
+            out(float{}, std::false_type{});
+        else
+            out(T{}, std::false_type{});
+    } else {
+        if (a.out_f32)
+            out(float{}, std::true_type{});
+        else
+            out(T{}, std::true_type{});
+    }
+}
+
+template <int GPB, bool Z, int RT, int NT, int WR, int WC> int launch_tile(hipStream_t st, const Int4Args &a)
+{
+    constexpr size_t bytes = tile_lds_bytes(WC * NT * 16, WR * RT * 16);
+    const size_t     cols = fp6mi::int4_tiles(a.N, a.offsets ? a.E : 0, WC * NT * 16), rows = (a.Mt + WR * RT - 1) / (WR * RT);
+    if (cols * rows > 0x7fffffffu) return FP6MI_ERR_SHAPE;
+    if constexpr (bytes > 65536)
+        if (const int e = allow_dynamic_lds<int4_tile<GPB, Z, RT, NT, WR, WC>>(bytes)) return e;
+    hipLaunchKernelGGL((int4_tile<GPB, Z, RT, NT, WR, WC>), dim3((uint32_t)(cols * rows)), dim3(WR * WC * 64), bytes, st, a, (uint32_t)cols);
+    return (int)hipGetLastError();
+}
+
 template <int GPB, bool Z> int run(hipStream_t st, const Int4Args &a)
 {
     if (a.N <= 16 || (a.offsets && a.N <= 16 * a.E)) return launch_stream<GPB, Z, 2, 1, 8>(st, a);
+    if (a.K <= 1u << 20 && a.N > (a.offsets ? 64 * a.E : 64)) return launch_tile<GPB, Z, 4, 4, 4, 2>(st, a);
     return launch_stream<GPB, Z, 2, 4, 4>(st, a);
 }
 

@@ -447,3 +447,18 @@ def test_forward_mode_transforms_and_traces_are_refused():
             torch.func.vmap(f)(t.unsqueeze(0))
         with pytest.raises(RuntimeError):
             torch.jit.trace(f, t)
+
+
+def test_objects_of_the_makefile_depend_on_all_that_they_include():
+    import os
+    import re
+    from test_build_sources import PACKAGE, included
+    with open(os.path.join(PACKAGE, "Makefile")) as f:
+        text = f.read()
+    headers = re.search(r"^HDRS = (.*)$", text, re.M).group(1)
+    rules = re.findall(r"^\$\(OBJ2\)/(\S+)\.o: (.*)$", text, re.M)
+    assert {target for target, _ in rules} == {"fp6mi_int4_%", "fp6mi_int4_api", "fp6mi_experts"}
+    for target, needs in rules:
+        needs = [os.path.normpath(os.path.join(PACKAGE, n)) for n in needs.replace("$(HDRS)", headers).split()]
+        missing = included(needs[0]) - set(needs)
+        assert not missing, "%s.o: %s" % (target, sorted(os.path.basename(m) for m in missing))
