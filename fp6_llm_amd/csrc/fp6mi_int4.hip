@@ -42,6 +42,13 @@ __device__ __forceinline__ v4f mfma(v8t x, v8t w, v4f acc)
 #endif
 }
 
+// f(0), ..., f(N - 1) with the index as a compile-time constant
+template <int N, int I = 0, typename F> __device__ __forceinline__ void sections(const F &f)
+{
+    f(std::integral_constant<int, I>{});
+    if constexpr (I + 1 < N) sections<N, I + 1>(f);
+}
+
 // What a group's zero point (8 without one) makes of the codes.
 struct Zero {
 #if FP6MI_TYPE == 0
@@ -57,6 +64,14 @@ struct Zero {
 #endif
 };
 
+// (w & mask) | magic in one instruction: of the two constants one has to be in a vector register, which the compiler does not do by itself.
+__device__ __forceinline__ uint32_t and_or(uint32_t w, uint32_t mask, uint32_t magic)
+{
+    uint32_t r;
+    asm("v_and_or_b32 %0, %1, %2, %3" : "=v"(r) : "v"(w), "s"(mask), "v"(magic));
+    return r;
+}
+
 // Eight codes as q - z, columns 0..7.  fp16: 1024 + q and 1024 + 16 q are read off the bits 0x6400 | nibble, 9 instructions.  bf16 has no packed arithmetic: bytes to float32, and the upper
 // halves of the exact differences, 23.
 __device__ __forceinline__ v8t codes_of(uint32_t w, const Zero &zero)
@@ -65,10 +80,10 @@ __device__ __forceinline__ v8t codes_of(uint32_t w, const Zero &zero)
     union { v2h h[4]; v8t v; } r;
     const v2h      sixteenth = { (_Float16)0.0625f, (_Float16)0.0625f };
     const uint32_t w8 = w >> 8;
-    r.h[0] = __builtin_bit_cast(v2h, (w & 0x000f000fu) | 0x64006400u) + zero.low;
-    r.h[1] = __builtin_elementwise_fma(__builtin_bit_cast(v2h, (w & 0x00f000f0u) | 0x64006400u), sixteenth, zero.high);
-    r.h[2] = __builtin_bit_cast(v2h, (w8 & 0x000f000fu) | 0x64006400u) + zero.low;
-    r.h[3] = __builtin_elementwise_fma(__builtin_bit_cast(v2h, (w8 & 0x00f000f0u) | 0x64006400u), sixteenth, zero.high);
+    r.h[0] = __builtin_bit_cast(v2h, and_or(w, 0x000f000fu, 0x64006400u)) + zero.low;
+    r.h[1] = __builtin_elementwise_fma(__builtin_bit_cast(v2h, and_or(w, 0x00f000f0u, 0x64006400u)), sixteenth, zero.high);
+    r.h[2] = __builtin_bit_cast(v2h, and_or(w8, 0x000f000fu, 0x64006400u)) + zero.low;
+    r.h[3] = __builtin_elementwise_fma(__builtin_bit_cast(v2h, and_or(w8, 0x00f000f0u, 0x64006400u)), sixteenth, zero.high);
     return r.v;
 #else
     union { uint32_t d[4]; v8t v; } r;
@@ -279,7 +294,7 @@ constexpr size_t tile_lds_bytes(int cols, int rows) // the stages, and the outpu
 
 template <int GPB, bool Z, int RT, int NT, int WR, int WC> __global__ __launch_bounds__(WR *WC * 64) void int4_tile(const Int4Args a, uint32_t col_tiles)
 {
-    static_assert(RT % 2 == 0, "");
+    static_assert(RT == 4 && NT == 4, "the steps of a block are written for these");
     constexpr int      kWaves = WR * WC, kCols = WC * NT * 16, kTiles = WR * RT, kRows = kTiles * 16, kStage = kCols * 256, kDma = kCols / 4 / kWaves;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, q = lane >> 4, wr = wave % WR, wc = wave / WR;
@@ -309,92 +324,116 @@ template <int GPB, bool Z, int RT, int NT, int WR, int WC> __global__ __launch_b
             __builtin_amdgcn_raw_ptr_buffer_load_lds(xbuf, (lvoid *)(lds + stage * kStage + (j * kWaves + wave) * 1024), 16, off, 0, 0, 0);
         }
     };
+    // operands of X: of the first two tiles of the next block while this one's are still in use, of the others in their place
     const uint8_t *xread = lds + (wc * NT * 16 + c) * 256;
-    v8t            x[NT][4];
-    auto           read_x = [&](int n, uint32_t stage) __attribute__((always_inline)) {
-#pragma unroll
-        for (uint32_t i = 0; i < 4; i++) x[n][i] = *reinterpret_cast<const v8t *>(xread + stage * kStage + n * 16 * 256 + ((4 * i + q) ^ c) * 16);
+    v8t            early[2][2][4], late[2][4];
+    auto           read_x = [&](v8t &to, int n, uint32_t i, uint32_t stage) __attribute__((always_inline)) {
+        to = *reinterpret_cast<const v8t *>(xread + stage * kStage + n * 16 * 256 + ((4 * i + q) ^ c) * 16);
     };
 
-    // codes and scales: two blocks on their way
-    const v4u            *w[RT];
-    const Scales<GPB, Z> *s[RT];
-#pragma unroll
-    for (uint32_t r = 0; r < RT; r++) { // (row tiles beyond the last one take it again)
-        const uint32_t m = m0 + wr * RT + r;
-        const size_t   at = ((size_t)t.expert * a.Mt + (m < a.Mt ? m : a.Mt - 1)) * a.KB;
-        w[r] = static_cast<const v4u *>(a.W) + at * 64 + lane;
-        s[r] = static_cast<const Scales<GPB, Z> *>(a.S) + at * 16 + c;
-    }
-    v4u            raw[2][RT];
-    Scales<GPB, Z> scales[2][RT];
-    auto           load_w = [&](int set, uint32_t kb) __attribute__((always_inline)) {
-        kb = kb < a.KB ? kb : a.KB - 1;
-#pragma unroll
-        for (int r = 0; r < RT; r++) raw[set][r] = w[r][(size_t)kb * 64], scales[set][r] = s[r][(size_t)kb * 16];
+    // codes and scales, by scalar offsets from the wavefront's first row tile (row tiles beyond the last one take it again); a row tile's are asked for again as soon as they are converted
+    const uint32_t tile0 = m0 + wr * RT < a.Mt ? m0 + wr * RT : a.Mt - 1, tiles = a.Mt - tile0 < RT ? a.Mt - tile0 : RT;
+    const size_t   at = ((size_t)t.expert * a.Mt + tile0) * a.KB;
+    const auto     wbuf = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(static_cast<const uint8_t *>(a.W) + at * 1024), 0, (int)(tiles * a.KB * 1024), 0x00027000);
+    constexpr int  kScaleBytes = sizeof(Scales<GPB, Z>) * 16;
+    const auto     sbuf = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(static_cast<const uint8_t *>(a.S) + at * kScaleBytes), 0, (int)(tiles * a.KB * kScaleBytes), 0x00027000);
+    v4u            raw[RT];
+    Scales<GPB, Z> scales[RT];
+    auto           load_w = [&](int r, uint32_t kb) __attribute__((always_inline)) {
+        const uint32_t block = (r < (int)tiles ? r : tiles - 1) * a.KB + (kb < a.KB ? kb : a.KB - 1);
+        raw[r] = __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(wbuf, lane * 16, block * 1024, 0));
+        if constexpr (sizeof(scales[r]) == 2) scales[r] = __builtin_bit_cast(Scales<GPB, Z>, __builtin_amdgcn_raw_buffer_load_b16(sbuf, c * 2, block * kScaleBytes, 0));
+        if constexpr (sizeof(scales[r]) == 4) scales[r] = __builtin_bit_cast(Scales<GPB, Z>, __builtin_amdgcn_raw_buffer_load_b32(sbuf, c * 4, block * kScaleBytes, 0));
+        if constexpr (sizeof(scales[r]) == 8) scales[r] = __builtin_bit_cast(Scales<GPB, Z>, __builtin_amdgcn_raw_buffer_load_b64(sbuf, c * 8, block * kScaleBytes, 0));
+        if constexpr (sizeof(scales[r]) == 16) scales[r] = __builtin_bit_cast(Scales<GPB, Z>, __builtin_amdgcn_raw_buffer_load_b128(sbuf, c * 16, block * kScaleBytes, 0));
     };
-    v8t  op[2][4];
-    auto convert = [&](int to, int set, int r) __attribute__((always_inline)) {
-#pragma unroll
-        for (int g = 0; g < GPB; g++) {
-            Zero zero;
-            zero.set(Z ? scales[set][r].v[2 * g + 1] : (T)8.f);
-#pragma unroll
-            for (int i = 0; i < 4 / GPB; i++) op[to][g * (4 / GPB) + i] = codes_of(raw[set][r][g * (4 / GPB) + i], zero);
-        }
+    constexpr int kEach = 4 / GPB; // steps of a group
+    v8t           op[2][4];
+    float         scale[2][GPB];
+    auto          convert = [&](int to, int r, int i) __attribute__((always_inline)) {
+        Zero zero;
+        zero.set(Z ? scales[r].v[i / kEach * 2 + 1] : (T)8.f);
+        op[to][i] = codes_of(raw[r][i], zero);
     };
-    v4f sum[RT][NT];
+    auto take_scales = [&](int to, int r) __attribute__((always_inline)) {
+#pragma unroll
+        for (int g = 0; g < GPB; g++) scale[to][g] = (float)scales[r].v[Z ? 2 * g : g];
+    };
+    v4f sum[RT][NT], y[2][2];
 #pragma unroll
     for (int r = 0; r < RT; r++)
 #pragma unroll
         for (int n = 0; n < NT; n++) sum[r][n] = (v4f){ 0.f, 0.f, 0.f, 0.f };
+    y[1][0] = y[1][1] = (v4f){ 0.f, 0.f, 0.f, 0.f };
+#pragma unroll
+    for (int g = 0; g < GPB; g++) scale[(RT - 1) & 1][g] = 0.f;
 
-    // one block, whose X is in registers and whose first row tile is converted; leaves the same of the next one
-    auto block = [&](auto set_c, uint32_t kb) __attribute__((always_inline)) {
-        constexpr int set = decltype(set_c)::value;
-        float         scale[RT][GPB];
-#pragma unroll
-        for (int r = 0; r < RT; r++)
-#pragma unroll
-            for (int g = 0; g < GPB; g++) scale[r][g] = (float)scales[set][r].v[Z ? 2 * g : g];
-#pragma unroll
-        for (int r = 0; r < RT; r++) {
-            if (r == RT - 1) { // the next block's X has landed, and all have read this one's
-                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-                transfer(kb + 2, set);
-                load_w(set, kb + 2);
-                convert(0, set ^ 1, 0);
-            } else {
-                convert((r + 1) & 1, set, r + 1);
-            }
-#pragma unroll
-            for (int n = 0; n < NT; n++) {
-#pragma unroll
-                for (int g = 0; g < GPB; g++) {
-                    v4f y = { 0.f, 0.f, 0.f, 0.f };
-#pragma unroll
-                    for (int i = g * (4 / GPB); i < (g + 1) * (4 / GPB); i++) y = mfma(x[n][i], op[r & 1][i], y);
-#pragma unroll
-                    for (int i = 0; i < 4; i++) sum[r][n][i] += scale[r][g] * y[i];
-                }
-                if (r == RT - 1) read_x(n, set ^ 1);
-            }
+    // A block is RT * 2 steps of two tiles of X by one row tile; a step also converts half of the next row tile, adds up the groups that the step before has multiplied, and reads some of the next
+    // block's X.  The last row tile takes the tiles of X in the other order, which frees the registers of the late ones a step earlier.
+    auto step = [&](auto u_c, auto set_c, uint32_t kb) __attribute__((always_inline)) {
+        constexpr int u = decltype(u_c)::value, set = decltype(set_c)::value, r = u / 2, last = 2 * RT - 1;
+        constexpr int n = (u & 1) ^ (r == RT - 1) ? 2 : 0, next = (r + 1) % RT;
+        constexpr int pu = u == 0 ? last : u - 1, pr = pu / 2, pn = (pu & 1) ^ (pr == RT - 1) ? 2 : 0; // the step before
+        if constexpr (u == 2) { // the next block's X has landed (behind its transfers come the loads of every row tile), and all have read this one's
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(RT) : "memory");
+            transfer(kb + 2, set);
         }
+        if constexpr (u >= 2 && u < 6) {
+#pragma unroll
+            for (int i = 0; i < 2; i++) read_x(early[set ^ 1][(u - 2) / 2][u % 2 * 2 + i], (u - 2) / 2, u % 2 * 2 + i, set ^ 1);
+        }
+        if constexpr (u == last) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) read_x(late[i / 4][i % 4], 2 + i / 4, i % 4, set ^ 1);
+        }
+#pragma unroll
+        for (int g = 0; g < GPB; g++) {
+            constexpr int kPairs = GPB; // of groups in a step
+            const int     v = u * kPairs + g;
+#pragma unroll
+            for (int i = g * kEach; i < (g + 1) * kEach; i++)
+#pragma unroll
+                for (int k = 0; k < 2; k++) y[v & 1][k] = mfma(n == 0 ? early[set][k][i] : late[k][i], op[r & 1][i], i == g * kEach ? (v4f){ 0.f, 0.f, 0.f, 0.f } : y[v & 1][k]);
+            // the pair before
+            const int br = g ? r : pr, bn = g ? n : pn, bg = g ? g - 1 : GPB - 1;
+#pragma unroll
+            for (int k = 0; k < 2; k++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) sum[br][bn + k][i] += scale[br & 1][bg] * y[(v & 1) ^ 1][k][i];
+        }
+        convert((r + 1) & 1, next, (u & 1) * 2);
+        convert((r + 1) & 1, next, (u & 1) * 2 + 1);
+        if constexpr (u & 1) {
+            take_scales((r + 1) & 1, next);
+            load_w(next, r + 1 < RT ? kb + 1 : kb + 2);
+        }
+        __builtin_amdgcn_sched_barrier(0);
     };
+    auto block = [&](auto set_c, uint32_t kb) __attribute__((always_inline)) { sections<2 * RT>([&](auto u_c) __attribute__((always_inline)) { step(u_c, set_c, kb); }); };
     transfer(0, 0);
     load_w(0, 0);
     asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
     transfer(1, 1);
-    load_w(1, 1);
+    asm volatile("" ::: "memory");
 #pragma unroll
-    for (int n = 0; n < NT; n++) read_x(n, 0);
-    convert(0, 0, 0);
+    for (int i = 0; i < 8; i++) read_x(early[0][i / 4][i % 4], i / 4, i % 4, 0);
+#pragma unroll
+    for (int i = 0; i < 8; i++) read_x(late[i / 4][i % 4], 2 + i / 4, i % 4, 0);
+#pragma unroll
+    for (int i = 0; i < 4; i++) convert(0, 0, i);
+    take_scales(0, 0);
+#pragma unroll
+    for (int r = 0; r < RT; r++) load_w(r, r == 0 ? 1 : 0);
     uint32_t kb = 0;
     for (; kb + 2 <= a.KB; kb += 2) {
         block(std::integral_constant<int, 0>{}, kb);
         block(std::integral_constant<int, 1>{}, kb + 1);
     }
     if (kb < a.KB) block(std::integral_constant<int, 0>{}, kb);
+#pragma unroll
+    for (int k = 0; k < 2; k++) // the last pair
+#pragma unroll
+        for (int i = 0; i < 4; i++) sum[RT - 1][k][i] += scale[(RT - 1) & 1][GPB - 1] * y[1][k][i];
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); // nothing is on its way to LDS any more
 
     // outputs through LDS, so that a lane stores 16 bytes: [row of X][weight row], rows 16 bytes apart from a multiple of 512
