@@ -64,37 +64,38 @@ struct Zero {
 #endif
 };
 
-// (w & mask) | magic in one instruction: of the two constants one has to be in a vector register, which the compiler does not do by itself.
-__device__ __forceinline__ uint32_t and_or(uint32_t w, uint32_t mask, uint32_t magic)
-{
-    uint32_t r;
-    asm("v_and_or_b32 %0, %1, %2, %3" : "=v"(r) : "v"(w), "s"(mask), "v"(magic));
-    return r;
-}
+// What the codes are cut out with.  (w & mask) | bits is one instruction where of the two constants one is in a vector register, of which the compiler has to be told.
+struct Cutter {
+#if FP6MI_TYPE == 0
+    uint32_t low = 0x000f000fu, high = 0x00f000f0u, bits = 0x64006400u;
+    __device__ __forceinline__ Cutter() { asm("" : "+s"(low), "+s"(high), "+v"(bits)); }
+#endif
+};
 
-// Eight codes as q - z, columns 0..7.  fp16: 1024 + q and 1024 + 16 q are read off the bits 0x6400 | nibble, 9 instructions.  bf16 has no packed arithmetic: bytes to float32, and the upper
-// halves of the exact differences, 23.
-__device__ __forceinline__ v8t codes_of(uint32_t w, const Zero &zero)
+// Eight codes as q - z, columns 0..7, or (half) four of them.  fp16: 1024 + q and 1024 + 16 q are read off the bits 0x6400 | nibble, 9 instructions.  bf16 has no packed arithmetic: bytes to float32,
+// and the upper halves of the exact differences, 23.
+union Codes { uint32_t d[4]; v8t v; };
+__device__ __forceinline__ void codes_half(Codes &to, uint32_t w, const Zero &zero, const Cutter &cut, int half)
 {
 #if FP6MI_TYPE == 0
-    union { v2h h[4]; v8t v; } r;
-    const v2h      sixteenth = { (_Float16)0.0625f, (_Float16)0.0625f };
-    const uint32_t w8 = w >> 8;
-    r.h[0] = __builtin_bit_cast(v2h, and_or(w, 0x000f000fu, 0x64006400u)) + zero.low;
-    r.h[1] = __builtin_elementwise_fma(__builtin_bit_cast(v2h, and_or(w, 0x00f000f0u, 0x64006400u)), sixteenth, zero.high);
-    r.h[2] = __builtin_bit_cast(v2h, and_or(w8, 0x000f000fu, 0x64006400u)) + zero.low;
-    r.h[3] = __builtin_elementwise_fma(__builtin_bit_cast(v2h, and_or(w8, 0x00f000f0u, 0x64006400u)), sixteenth, zero.high);
-    return r.v;
+    const v2h sixteenth = { (_Float16)0.0625f, (_Float16)0.0625f };
+    if (half) w >>= 8;
+    to.d[2 * half] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(v2h, (w & cut.low) | cut.bits) + zero.low);
+    to.d[2 * half + 1] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(__builtin_bit_cast(v2h, (w & cut.high) | cut.bits), sixteenth, zero.high));
 #else
-    union { uint32_t d[4]; v8t v; } r;
-    const uint32_t even = w & 0x0f0f0f0fu, odd = (w >> 4) & 0x0f0f0f0fu; // bytes: nibbles 0, 2, 4, 6 and 1, 3, 5, 7
-    auto           pair = [&](uint32_t b, int i) { // nibbles n and n + 4
-        const float lo = (float)(uint8_t)(b >> 8 * i) - zero.z, hi = (float)(uint8_t)(b >> 8 * (i + 2)) - zero.z;
+    auto pair = [&](uint32_t b) { // bytes: nibbles n and n + 4 in the lower halves of the words
+        const float lo = (float)(uint8_t)(b >> 8 * half) - zero.z, hi = (float)(uint8_t)(b >> (8 * half + 16)) - zero.z;
         return __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, hi), __builtin_bit_cast(uint32_t, lo), 0x07060302u);
     };
-    r.d[0] = pair(even, 0), r.d[1] = pair(odd, 0), r.d[2] = pair(even, 1), r.d[3] = pair(odd, 1);
-    return r.v;
+    to.d[2 * half] = pair(w & 0x0f0f0f0fu), to.d[2 * half + 1] = pair((w >> 4) & 0x0f0f0f0fu);
 #endif
+}
+__device__ __forceinline__ v8t codes_of(uint32_t w, const Zero &zero, const Cutter &cut)
+{
+    Codes r;
+    codes_half(r, w, zero, cut, 0);
+    codes_half(r, w, zero, cut, 1);
+    return r.v;
 }
 
 // The scales (and zero points) of one row in one block.
@@ -179,6 +180,7 @@ template <int GPB, bool Z, int RT, int NT, int WK> __global__ __launch_bounds__(
     for (int n = 0; n < NT; n++) x[n] = static_cast<const T *>(a.X) + (size_t)(t.row + (n * 16 + c < t.rows ? n * 16 + c : t.rows - 1)) * a.K + q * 8;
 
     typedef Block<GPB, Z, RT, NT> B;
+    const Cutter                  cut;
     auto load = [&](B &b, uint32_t kb) __attribute__((always_inline)) {
         const uint32_t steps = (a.K - kb * 128) / 32; // of 32 columns, 4 but for the last block
 #pragma unroll
@@ -206,7 +208,7 @@ template <int GPB, bool Z, int RT, int NT, int WK> __global__ __launch_bounds__(
                 zero.set(Z ? b.s[r].v[2 * g + 1] : (T)8.f);
                 v8t v[kEach];
 #pragma unroll
-                for (int i = 0; i < kEach; i++) v[i] = codes_of(b.w[r][g * kEach + i], zero);
+                for (int i = 0; i < kEach; i++) v[i] = codes_of(b.w[r][g * kEach + i], zero, cut);
 #pragma unroll
                 for (int n = 0; n < NT; n++) {
                     v4f y = { 0.f, 0.f, 0.f, 0.f };
@@ -292,7 +294,7 @@ constexpr size_t tile_lds_bytes(int cols, int rows) // the stages, and the outpu
     return stages > outputs ? stages : outputs;
 }
 
-template <int GPB, bool Z, int RT, int NT, int WR, int WC> __global__ __launch_bounds__(WR *WC * 64) void int4_tile(const Int4Args a, uint32_t col_tiles)
+template <int GPB, bool Z, int RT, int NT, int WR, int WC> __global__ __launch_bounds__(WR *WC * 64, 2) void int4_tile(const Int4Args a, uint32_t col_tiles)
 {
     static_assert(RT == 4 && NT == 4, "the steps of a block are written for these");
     constexpr int      kWaves = WR * WC, kCols = WC * NT * 16, kTiles = WR * RT, kRows = kTiles * 16, kStage = kCols * 256, kDma = kCols / 4 / kWaves;
@@ -347,13 +349,14 @@ template <int GPB, bool Z, int RT, int NT, int WR, int WC> __global__ __launch_b
         if constexpr (sizeof(scales[r]) == 8) scales[r] = __builtin_bit_cast(Scales<GPB, Z>, __builtin_amdgcn_raw_buffer_load_b64(sbuf, c * 8, block * kScaleBytes, 0));
         if constexpr (sizeof(scales[r]) == 16) scales[r] = __builtin_bit_cast(Scales<GPB, Z>, __builtin_amdgcn_raw_buffer_load_b128(sbuf, c * 16, block * kScaleBytes, 0));
     };
-    constexpr int kEach = 4 / GPB; // steps of a group
-    v8t           op[2][4];
+    constexpr int kEach = 4 / GPB; // matrix instructions of a group
+    Codes         op[2][4];
+    Zero          zero;
+    const Cutter  cut;
     float         scale[2][GPB];
-    auto          convert = [&](int to, int r, int i) __attribute__((always_inline)) {
-        Zero zero;
-        zero.set(Z ? scales[r].v[i / kEach * 2 + 1] : (T)8.f);
-        op[to][i] = codes_of(raw[r][i], zero);
+    auto          convert = [&](int to, int r, int i, int half) __attribute__((always_inline)) {
+        if (half == 0 && i % kEach == 0) zero.set(Z ? scales[r].v[i / kEach * 2 + 1] : (T)8.f);
+        codes_half(op[to][i], raw[r][i], zero, cut, half);
     };
     auto take_scales = [&](int to, int r) __attribute__((always_inline)) {
 #pragma unroll
@@ -386,23 +389,32 @@ template <int GPB, bool Z, int RT, int NT, int WR, int WC> __global__ __launch_b
 #pragma unroll
             for (int i = 0; i < 8; i++) read_x(late[i / 4][i % 4], 2 + i / 4, i % 4, set ^ 1);
         }
+        // of the groups multiplied before: pair v of them, tiles n and n + 1 of X by row tile r, from tile `from` of the two on
+        auto add = [&](int r, int n, int g, int v, int from, int to) __attribute__((always_inline)) {
 #pragma unroll
-        for (int g = 0; g < GPB; g++) {
-            constexpr int kPairs = GPB; // of groups in a step
-            const int     v = u * kPairs + g;
+            for (int k = from; k < to; k++)
 #pragma unroll
-            for (int i = g * kEach; i < (g + 1) * kEach; i++)
+                for (int i = 0; i < 4; i++) sum[r][n + k][i] += scale[r & 1][g] * y[v & 1][k][i];
+        };
 #pragma unroll
-                for (int k = 0; k < 2; k++) y[v & 1][k] = mfma(n == 0 ? early[set][k][i] : late[k][i], op[r & 1][i], i == g * kEach ? (v4f){ 0.f, 0.f, 0.f, 0.f } : y[v & 1][k]);
-            // the pair before
-            const int br = g ? r : pr, bn = g ? n : pn, bg = g ? g - 1 : GPB - 1;
+        for (int i = 0; i < 4; i++) {
+            const int v = u * GPB + i / kEach;
 #pragma unroll
-            for (int k = 0; k < 2; k++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) sum[br][bn + k][i] += scale[br & 1][bg] * y[(v & 1) ^ 1][k][i];
+            for (int k = 0; k < 2; k++) y[v & 1][k] = mfma(n == 0 ? early[set][k][i] : late[k][i], op[r & 1][i].v, i % kEach == 0 ? (v4f){ 0.f, 0.f, 0.f, 0.f } : y[v & 1][k]);
+            if constexpr (GPB == 1) {
+                if (i == 1 || i == 2) add(pr, pn, 0, v + 1, i - 1, i);
+            } else if constexpr (GPB == 2) {
+                if (i == 1) add(pr, pn, 1, v + 1, 0, 2);
+                if (i == 3) add(r, n, 0, v + 1, 0, 2);
+            } else {
+                if (i == 0)
+                    add(pr, pn, 3, v + 1, 0, 2);
+                else
+                    add(r, n, i - 1, v + 1, 0, 2);
+            }
+            convert((r + 1) & 1, next, (u & 1) * 2 + i / 2, i & 1);
+            if (i < 3) __builtin_amdgcn_sched_barrier(0);
         }
-        convert((r + 1) & 1, next, (u & 1) * 2);
-        convert((r + 1) & 1, next, (u & 1) * 2 + 1);
         if constexpr (u & 1) {
             take_scales((r + 1) & 1, next);
             load_w(next, r + 1 < RT ? kb + 1 : kb + 2);
@@ -420,7 +432,7 @@ template <int GPB, bool Z, int RT, int NT, int WR, int WC> __global__ __launch_b
 #pragma unroll
     for (int i = 0; i < 8; i++) read_x(late[i / 4][i % 4], 2 + i / 4, i % 4, 0);
 #pragma unroll
-    for (int i = 0; i < 4; i++) convert(0, 0, i);
+    for (int i = 0; i < 8; i++) convert(0, 0, i / 2, i & 1);
     take_scales(0, 0);
 #pragma unroll
     for (int r = 0; r < RT; r++) load_w(r, r == 0 ? 1 : 0);
@@ -500,7 +512,7 @@ template <int GPB, bool Z, int RT, int NT, int WR, int WC> int launch_tile(hipSt
 template <int GPB, bool Z> int run(hipStream_t st, const Int4Args &a)
 {
     if (a.N <= 16 || (a.offsets && a.N <= 16 * a.E)) return launch_stream<GPB, Z, 2, 1, 8>(st, a);
-    if (a.K <= 1u << 20 && a.N > (a.offsets ? 64 * a.E : 64)) return launch_tile<GPB, Z, 4, 4, 4, 2>(st, a);
+    if (a.K <= 1u << 20 && a.N > (a.offsets ? 64 * a.E : 64)) return launch_tile<GPB, Z, 4, 4, 4, 1>(st, a);
     return launch_stream<GPB, Z, 2, 4, 4>(st, a);
 }
 
