@@ -4,6 +4,7 @@
 // raw pointers to libfp6mi.so.  The Python package uses it when it is built and falls back to its ctypes binding of the
 // same C ABI otherwise; both launch the same kernels.
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
 #include <c10/hip/HIPGuard.h>
@@ -572,10 +573,20 @@ at::Tensor adapter_forward(int64_t E, int64_t Mb, const at::Tensor &in_feats, co
 // ---- 4-bit integer weights (fp6_llm_amd/int4.py) and rows of experts (fp6_llm_amd/experts.py) ----
 int type_code(at::ScalarType t) { return t == at::kHalf ? 0 : t == at::kBFloat16 ? 1 : t == at::kFloat ? 2 : -1; }
 
-at::Tensor int4_forward(const at::Tensor &in_feats, const at::Tensor &native, const at::Tensor &s, const OptTensor &offsets, int64_t places, int64_t act, const OptTensor &bias, const OptTensor &out_opt,
+// A plan is one int32 tensor: offsets [experts + 1], order [places], place [places].
+struct PlanArgs { const int *valid, *place; int *offsets, *order; };
+PlanArgs plan_args(const at::Tensor &table, int64_t experts, int64_t places)
+{
+    if (table.scalar_type() != at::kInt || table.dim() != 1 || table.size(0) != experts + 1 + 2 * places || experts < 1 || !table.is_contiguous() || !table.is_cuda())
+        bad("the plan must be that of expert_sort or expert_plan");
+    int *p = table.data_ptr<int>();
+    return { p + experts, p + experts + 1 + places, p, p + experts + 1 };
+}
+
+at::Tensor int4_forward(const at::Tensor &in_feats, const at::Tensor &native, const at::Tensor &s, const OptTensor &plan, int64_t experts, int64_t places, int64_t act, const OptTensor &bias, const OptTensor &out_opt,
                         bool f32)
 {
-    const bool         grouped = offsets.has_value();
+    const bool         grouped = plan.has_value();
     const int64_t      dims = grouped ? 6 : 5;
     const at::ScalarType type = s.scalar_type();
     if ((type != at::kHalf && type != at::kBFloat16) || s.dim() != dims || s.size(-3) != 16 || (s.size(-2) != 1 && s.size(-2) != 2 && s.size(-2) != 4) || (s.size(-1) != 1 && s.size(-1) != 2) ||
@@ -590,8 +601,11 @@ at::Tensor int4_forward(const at::Tensor &in_feats, const at::Tensor &native, co
         !native.is_contiguous())
         bad("native_weight must be that of int4_pack_native with these scales");
     if (act >= 0 && OC % 32) bad("a gated product needs OC % 32 == 0, got " + std::to_string(OC));
-    if (grouped && (offsets->scalar_type() != at::kInt || offsets->dim() != 1 || offsets->size(0) != E + 1 || !offsets->is_contiguous() || offsets->device() != dev || B != places))
-        bad("the plan must be of " + std::to_string(E) + " experts and as many places as in_feats has rows, on the same GPU");
+    const int *offsets = nullptr;
+    if (grouped) {
+        if (experts != E || plan->device() != dev || B != places) bad("the plan must be of " + std::to_string(E) + " experts and as many places as in_feats has rows, on the same GPU");
+        offsets = plan_args(*plan, experts, places).offsets;
+    }
     if (bias.has_value() && (bias->scalar_type() != type || bias->dim() != (grouped ? 2 : 1) || bias->size(-1) != OC || (grouped && bias->size(0) != E) || !bias->is_contiguous() || bias->device() != dev))
         bad("bias must be contiguous, of the scales' type, one for each row of the weights, on the same GPU");
     const at::Tensor     x = in_feats.is_contiguous() ? in_feats : in_feats.contiguous();
@@ -607,12 +621,14 @@ at::Tensor int4_forward(const at::Tensor &in_feats, const at::Tensor &native, co
         out = at::empty({ B, cols }, at::TensorOptions().dtype(to).device(dev));
     }
     raise_status(fp6mi_int4_linear(c10::hip::getCurrentHIPStream(dev.index()).stream(), type_code(type), native.data_ptr(), s.data_ptr(), 128 / (int)s.size(-2), (int)s.size(-1) - 1, pointer(bias),
-                                   x.data_ptr(), out.data_ptr(), f32, (int)act, grouped ? offsets->data_ptr<int>() : nullptr, (size_t)E, (size_t)OC, (size_t)B, (size_t)IC),
+                                   x.data_ptr(), out.data_ptr(), f32, (int)act, offsets, (size_t)E, (size_t)OC, (size_t)B, (size_t)IC),
                  "fp6mi_int4_linear");
     return out;
 }
 
-pybind11::object expert_sort(const OptTensor &x_opt, const at::Tensor &index_in, int64_t experts)
+void kernel_status(int rc, const char *where) { TORCH_CHECK(rc == 0, where, " failed: ", fp6mi_error_string(rc)); } // (without the interpreter's lock, which a backward pass does not hold)
+
+std::pair<OptTensor, at::Tensor> sort_values(const OptTensor &x_opt, const at::Tensor &index_in, int64_t experts)
 {
     const at::Device dev = index_in.device();
     if ((index_in.scalar_type() != at::kInt && index_in.scalar_type() != at::kLong) || index_in.dim() != 2 || !index_in.is_cuda())
@@ -624,70 +640,136 @@ pybind11::object expert_sort(const OptTensor &x_opt, const at::Tensor &index_in,
     at::Tensor         x;
     int64_t            H = 0, ld = 0;
     if (x_opt.has_value()) {
-        x = *x_opt;
+        x = x_opt->resolve_neg();
         if (type_code(x.scalar_type()) < 0 || x.dim() != 2 || x.size(0) != T || x.size(1) < 1 || x.size(1) > 1 << 24 || x.device() != dev)
             bad("x must be float16, bfloat16 or float32 [tokens=" + std::to_string(T) + ", features], on the index's GPU");
         H = x.size(1);
         if (x.stride(1) != 1 || (T > 1 && x.stride(0) < H)) x = x.contiguous();
         ld = x.stride(0);
-        rows = at::empty({ T * k, H }, x.options());
+        rows = at::empty({ T * k, H }, at::TensorOptions().dtype(x.scalar_type()).device(dev));
     }
-    const at::Tensor index = index_in.contiguous();
-    const auto       ints = at::TensorOptions().dtype(at::kInt).device(dev);
-    const at::Tensor offsets = at::empty({ experts + 1 }, ints), order = at::empty({ T * k }, ints), place = at::empty({ T * k }, ints);
+    const at::Tensor index = index_in.is_contiguous() ? index_in : index_in.contiguous();
+    const at::Tensor table = at::empty({ experts + 1 + 2 * T * k }, at::TensorOptions().dtype(at::kInt).device(dev));
+    const PlanArgs   p = plan_args(table, experts, T * k);
     void            *stream = c10::hip::getCurrentHIPStream(dev.index()).stream();
     at::Tensor       keep;
     float           *ws = scratch(c10::nullopt, dev, stream, fp6mi_expert_sort_workspace_bytes((size_t)T, (size_t)k, (size_t)experts), keep);
-    raise_status(fp6mi_expert_sort(stream, index.data_ptr(), index.scalar_type() == at::kLong, offsets.data_ptr<int>(), order.data_ptr<int>(), place.data_ptr<int>(), x.defined() ? x.data_ptr() : nullptr,
-                                   (size_t)ld, rows.has_value() ? rows->data_ptr() : nullptr, (size_t)T, (size_t)k, (size_t)experts, (size_t)H, x.defined() ? type_code(x.scalar_type()) : 0, ws),
-                 "fp6mi_expert_sort");
-    return pybind11::make_tuple(rows, offsets, order, place);
+    kernel_status(fp6mi_expert_sort(stream, index.data_ptr(), index.scalar_type() == at::kLong, p.offsets, p.order, const_cast<int *>(p.place), x.defined() ? x.data_ptr() : nullptr, (size_t)ld,
+                                    rows.has_value() ? rows->data_ptr() : nullptr, (size_t)T, (size_t)k, (size_t)experts, (size_t)H, x.defined() ? type_code(x.scalar_type()) : 0, ws),
+                  "fp6mi_expert_sort");
+    return { rows, table };
 }
 
-// The plan's tensors come from expert_sort; they are looked at again, since a caller may hold a plan of its own making.
-void check_plan(const at::Tensor &place, const at::Tensor &offsets, int64_t places, const at::Device &dev)
-{
-    if (place.scalar_type() != at::kInt || place.dim() != 1 || place.size(0) != places || !place.is_contiguous() || place.device() != dev || offsets.scalar_type() != at::kInt || offsets.dim() != 1 ||
-        offsets.size(0) < 2 || !offsets.is_contiguous() || offsets.device() != dev)
-        bad("the plan must be that of expert_sort or expert_plan, on the rows' GPU");
-}
-
-at::Tensor expert_combine(const at::Tensor &rows_in, const at::Tensor &place, const at::Tensor &offsets, const OptTensor &weights, int64_t tokens, int64_t k, at::ScalarType to)
+at::Tensor combine_values(const at::Tensor &rows_in, const at::Tensor &table, int64_t tokens, int64_t k, int64_t experts, const OptTensor &weights, at::ScalarType to)
 {
     const int        row_type = type_code(rows_in.scalar_type()), out_type = type_code(to);
     const at::Device dev = rows_in.device();
-    if (row_type < 0 || rows_in.dim() != 2 || rows_in.size(0) != tokens * k || rows_in.size(1) < 1 || rows_in.size(1) > 1 << 24 || !rows_in.is_cuda() || dev != place.device())
+    const PlanArgs   p = plan_args(table, experts, tokens * k);
+    if (row_type < 0 || rows_in.dim() != 2 || rows_in.size(0) != tokens * k || rows_in.size(1) < 1 || rows_in.size(1) > 1 << 24 || dev != table.device())
         bad("rows must be float16, bfloat16 or float32 [tokens * k = " + std::to_string(tokens * k) + ", features], on the plan's GPU");
     if (out_type < 0 || (out_type != row_type && row_type != 2)) bad("sums have the rows' type, those of float32 rows any");
-    check_plan(place, offsets, tokens * k, dev);
-    if (weights.has_value()) check_tensor(*weights, { tokens, k }, at::kFloat, dev, "weights");
     c10::hip::HIPGuard guard(dev.index());
-    const at::Tensor   rows = rows_in.contiguous(), out = at::empty({ tokens, rows.size(1) }, at::TensorOptions().dtype(to).device(dev));
-    raise_status(fp6mi_expert_combine(c10::hip::getCurrentHIPStream(dev.index()).stream(), rows.data_ptr(), place.data_ptr<int>(), offsets.data_ptr<int>() + offsets.size(0) - 1,
-                                      static_cast<const float *>(pointer(weights)), out.data_ptr(), (size_t)tokens, (size_t)k, (size_t)rows.size(1), row_type, out_type),
-                 "fp6mi_expert_combine");
+    const at::Tensor   rows = rows_in.resolve_neg().contiguous(), out = at::empty({ tokens, rows.size(1) }, at::TensorOptions().dtype(to).device(dev));
+    kernel_status(fp6mi_expert_combine(c10::hip::getCurrentHIPStream(dev.index()).stream(), rows.data_ptr(), p.place, p.valid, static_cast<const float *>(pointer(weights)), out.data_ptr(),
+                                       (size_t)tokens, (size_t)k, (size_t)rows.size(1), row_type, out_type),
+                  "fp6mi_expert_combine");
     return out;
 }
 
-pybind11::object expert_combine_backward(const at::Tensor &grad, const OptTensor &rows, const at::Tensor &place, const at::Tensor &offsets, const OptTensor &weights, int64_t k, at::ScalarType row_dtype,
-                                         bool want_rows, bool want_weights)
+// What a backward pass that is itself recorded (create_graph) gives: values whose own gradient is an error.
+torch::autograd::variable_list once_differentiable(torch::autograd::variable_list grads)
 {
-    const at::Device dev = grad.device();
-    const int64_t    tokens = grad.size(0), H = grad.size(1);
-    check_plan(place, offsets, tokens * k, dev);
-    if (want_weights && (!rows.has_value() || rows->scalar_type() != row_dtype)) bad("the gradient of the weights needs the rows");
-    if (rows.has_value()) check_tensor(*rows, { tokens * k, H }, rows->scalar_type(), dev, "rows");
-    if (weights.has_value()) check_tensor(*weights, { tokens, k }, at::kFloat, dev, "weights");
-    c10::hip::HIPGuard guard(dev.index());
-    OptTensor          grad_rows, grad_weights;
-    if (want_rows) grad_rows = at::empty({ tokens * k, H }, at::TensorOptions().dtype(row_dtype).device(dev));
-    if (want_weights) grad_weights = at::empty({ tokens, k }, at::TensorOptions().dtype(at::kFloat).device(dev));
-    raise_status(fp6mi_expert_combine_backward(c10::hip::getCurrentHIPStream(dev.index()).stream(), grad.data_ptr(), pointer(rows), place.data_ptr<int>(),
-                                               offsets.data_ptr<int>() + offsets.size(0) - 1, static_cast<const float *>(pointer(weights)), const_cast<void *>(pointer(grad_rows)),
-                                               static_cast<float *>(const_cast<void *>(pointer(grad_weights))), (size_t)tokens, (size_t)k, (size_t)H, type_code(row_dtype),
-                                               type_code(grad.scalar_type())),
-                 "fp6mi_expert_combine_backward");
-    return pybind11::make_tuple(grad_rows, grad_weights);
+    if (!at::GradMode::is_enabled()) return grads;
+    std::vector<size_t> at;
+    torch::autograd::variable_list defined;
+    for (size_t i = 0; i < grads.size(); i++)
+        if (grads[i].defined()) at.push_back(i), defined.push_back(grads[i].detach().requires_grad_());
+    if (defined.empty()) return grads;
+    auto refuse = std::make_shared<torch::autograd::DelayedError>("trying to differentiate twice a function that is differentiable once", (int64_t)defined.size());
+    defined = (*refuse)(std::move(defined));
+    for (size_t i = 0; i < at.size(); i++) grads[at[i]] = defined[i];
+    return grads;
+}
+
+// (As Python classes both took 30 to 40 us a pass more.)
+struct SortRows : torch::autograd::Function<SortRows> {
+    static torch::autograd::variable_list forward(torch::autograd::AutogradContext *ctx, const at::Tensor &x, const at::Tensor &index, int64_t experts)
+    {
+        auto [rows, table] = sort_values(x, index, experts);
+        ctx->save_for_backward({ table });
+        ctx->saved_data["tokens"] = index.size(0), ctx->saved_data["k"] = index.size(1), ctx->saved_data["experts"] = experts;
+        ctx->mark_non_differentiable({ table });
+        return { *rows, table };
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list grads)
+    {
+        torch::autograd::variable_list out(3);
+        if (grads[0].defined()) {
+            at::AutoGradMode off(false);
+            out[0] = combine_values(grads[0], ctx->get_saved_variables()[0], ctx->saved_data["tokens"].toInt(), ctx->saved_data["k"].toInt(), ctx->saved_data["experts"].toInt(), c10::nullopt,
+                                    grads[0].scalar_type());
+        }
+        return once_differentiable(std::move(out));
+    }
+};
+
+struct CombineRows : torch::autograd::Function<CombineRows> {
+    static at::Tensor forward(torch::autograd::AutogradContext *ctx, const at::Tensor &rows_in, const OptTensor &weights, const at::Tensor &table, int64_t tokens, int64_t k, int64_t experts, int64_t to)
+    {
+        const at::Tensor rows = rows_in.resolve_neg().contiguous();
+        const at::Tensor out = combine_values(rows, table, tokens, k, experts, weights, (at::ScalarType)to);
+        ctx->saved_data["row_type"] = (int64_t)rows.scalar_type(), ctx->saved_data["k"] = k, ctx->saved_data["experts"] = experts;
+        ctx->saved_data["want_rows"] = rows_in.requires_grad(), ctx->saved_data["want_weights"] = weights.has_value() && weights->requires_grad();
+        ctx->save_for_backward({ weights.has_value() && weights->requires_grad() ? rows : at::Tensor(), weights.has_value() ? *weights : at::Tensor(), table });
+        return out;
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list grads)
+    {
+        torch::autograd::variable_list out(7);
+        if (grads[0].defined()) {
+            at::AutoGradMode off(false);
+            const auto           saved = ctx->get_saved_variables();
+            const at::Tensor     grad = grads[0].resolve_neg().contiguous();
+            const at::Tensor    &rows = saved[0], &weights = saved[1], &table = saved[2];
+            const int64_t        tokens = grad.size(0), H = grad.size(1), k = ctx->saved_data["k"].toInt();
+            const at::ScalarType row_type = (at::ScalarType)ctx->saved_data["row_type"].toInt();
+            const PlanArgs       p = plan_args(table, ctx->saved_data["experts"].toInt(), tokens * k);
+            const bool           want_rows = ctx->saved_data["want_rows"].toBool(), want_weights = ctx->saved_data["want_weights"].toBool();
+            c10::hip::HIPGuard   guard(grad.device().index());
+            if (want_rows) out[0] = at::empty({ tokens * k, H }, at::TensorOptions().dtype(row_type).device(grad.device()));
+            if (want_weights) out[1] = at::empty({ tokens, k }, at::TensorOptions().dtype(at::kFloat).device(grad.device()));
+            if (want_rows || want_weights)
+                kernel_status(fp6mi_expert_combine_backward(c10::hip::getCurrentHIPStream(grad.device().index()).stream(), grad.data_ptr(), rows.defined() ? rows.data_ptr() : nullptr, p.place, p.valid,
+                                                            weights.defined() ? weights.data_ptr<float>() : nullptr, want_rows ? out[0].data_ptr() : nullptr,
+                                                            want_weights ? out[1].data_ptr<float>() : nullptr, (size_t)tokens, (size_t)k, (size_t)H, type_code(row_type),
+                                                            type_code(grad.scalar_type())),
+                              "fp6mi_expert_combine_backward");
+        }
+        return once_differentiable(std::move(out));
+    }
+};
+
+pybind11::tuple expert_sort(const OptTensor &x, const at::Tensor &index, int64_t experts)
+{
+    if (x.has_value() && x->requires_grad() && at::GradMode::is_enabled()) {
+        const auto both = SortRows::apply(*x, index, experts);
+        return pybind11::make_tuple(both[0], both[1]);
+    }
+    auto [rows, table] = sort_values(x, index, experts);
+    return pybind11::make_tuple(rows, table);
+}
+
+at::Tensor expert_combine(const at::Tensor &rows, const at::Tensor &table, int64_t tokens, int64_t k, int64_t experts, const OptTensor &weights_in, const c10::optional<at::ScalarType> &to_opt)
+{
+    OptTensor weights = weights_in;
+    if (weights.has_value()) {
+        if (weights->dim() != 2 || weights->size(0) != tokens || weights->size(1) != k || !weights->is_floating_point() || weights->device() != table.device())
+            bad("weights must be float [tokens=" + std::to_string(tokens) + ", k=" + std::to_string(k) + "] on the plan's GPU");
+        weights = weights->to(at::kFloat).resolve_neg().contiguous();
+    }
+    const at::ScalarType to = to_opt.has_value() ? *to_opt : rows.scalar_type();
+    if (at::GradMode::is_enabled() && (rows.requires_grad() || (weights.has_value() && weights->requires_grad()))) return CombineRows::apply(rows, weights, table, tokens, k, experts, (int64_t)to);
+    return combine_values(rows, table, tokens, k, experts, weights, to);
 }
 
 // Whether a backward pass from t would reach a node that runs on another stream of t's device than the current one: one that an eager graph made, a leaf's own (of an eager graph that
@@ -734,7 +816,6 @@ PYBIND11_MODULE(_fp6mi_torch, m)
     m.def("int4_forward", &int4_forward);
     m.def("expert_sort", &expert_sort);
     m.def("expert_combine", &expert_combine);
-    m.def("expert_combine_backward", &expert_combine_backward);
     m.def("gradient_goes_elsewhere", &gradient_goes_elsewhere);
     // the reference's bindings, name for name (fp6_llm/csrc/pybind.cpp:8-15)
     m.def("linear_forward_cuda", &fp6_linear_forward_cuda, "Computes FP6-FP16 GEMM.", pybind11::arg("in_feats"), pybind11::arg("weights"),

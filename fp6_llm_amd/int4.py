@@ -78,8 +78,8 @@ def int4_forward_native(in_feats, native_weight, native_scales, plan=None, activ
         raise ValueError("out_dtype must be float32 or the scales' type")
     if _ext is not None:
         if plan is None:
-            return _ext.int4_forward(in_feats, native_weight, native_scales, None, 0, act, bias, out, f32)
-        return _ext.int4_forward(in_feats, native_weight, native_scales, plan.offsets, plan.places, act, bias, out, f32)
+            return _ext.int4_forward(in_feats, native_weight, native_scales, None, 0, 0, act, bias, out, f32)
+        return _ext.int4_forward(in_feats, native_weight, native_scales, plan.table, plan.experts, plan.places, act, bias, out, f32)
     s = native_scales
     dims = 6 if plan is not None else 5
     if s.dtype not in TYPES or s.dim() != dims or s.shape[-3] != 16 or s.shape[-2] not in (1, 2, 4) or s.shape[-1] not in (1, 2) or not s.is_contiguous():
@@ -98,14 +98,15 @@ def int4_forward_native(in_feats, native_weight, native_scales, plan=None, activ
         raise ValueError("a gated product needs OC %% 32 == 0, got %d" % OC)
     E, offsets = 1, None
     if plan is not None:
-        E, offsets = s.shape[0], plan.offsets
-        if offsets.dtype != torch.int32 or offsets.shape != (E + 1,) or not offsets.is_contiguous() or offsets.device != dev or B != plan.places:
+        E = s.shape[0]
+        if plan.experts != E or plan.table.device != dev or B != plan.places:
             raise ValueError("the plan must be of %d experts and as many places as in_feats has rows, on the same GPU" % E)
+        offsets = plan._addresses()[0]
     if bias is not None and (bias.dtype != s.dtype or bias.shape != ((E, OC) if plan is not None else (OC,)) or not bias.is_contiguous() or bias.device != dev):
         raise ValueError("bias must be contiguous, of the scales' type, one for each row of the weights, on the same GPU")
     x = x.contiguous()
     out = ops._result(out, (B, OC // 2 if act >= 0 else OC), dev, dtype=torch.float32 if f32 else s.dtype)
     L = _lib.lib()
     ops._launch("fp6mi_int4_linear", dev, 0, None, lambda stream, ws: L.fp6mi_int4_linear(
-        stream, TYPES[s.dtype], native_weight.data_ptr(), s.data_ptr(), 128 // s.shape[-2], s.shape[-1] - 1, ops._ptr(bias), x.data_ptr(), out.data_ptr(), f32, act, ops._ptr(offsets), E, OC, B, IC))
+        stream, TYPES[s.dtype], native_weight.data_ptr(), s.data_ptr(), 128 // s.shape[-2], s.shape[-1] - 1, ops._ptr(bias), x.data_ptr(), out.data_ptr(), f32, act, offsets, E, OC, B, IC))
     return out

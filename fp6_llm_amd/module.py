@@ -43,13 +43,13 @@ def _differentiates(x):
     return True
 
 
-def _refuse_unseen(x):
-    """What a kernel that is handed x's address would pass by in silence: a tangent that x carries (forward mode), a transform of torch.func that x is part of, a trace that is being made,
+def _refuse_unseen(*tensors):
+    """What a kernel that is handed a tensor's address would pass by in silence: a tangent that it carries (forward mode), a transform of torch.func that it is part of, a trace that is being made,
     which would record the output as it was allocated and not what fills it."""
     if _is_compiling():   # (a call of a kernel ends the graph that is compiled)
         return
-    wrapped = _peek_transform is None or (_peek_transform() is not None and torch._C._functorch.is_functorch_wrapped_tensor(x))
-    if wrapped or (getattr(_forward_ad, "_current_level", 0) >= 0 and _forward_ad.unpack_dual(x).tangent is not None):
+    wrapped = _peek_transform is None or (_peek_transform() is not None and any(torch._C._functorch.is_functorch_wrapped_tensor(x) for x in tensors))
+    if wrapped or (getattr(_forward_ad, "_current_level", 0) >= 0 and any(_forward_ad.unpack_dual(x).tangent is not None for x in tensors)):
         raise RuntimeError("this operator has no part in forward mode or in a transform of torch.func")
     proxies = sys.modules.get("torch.fx.experimental.proxy_tensor")   # (not loaded: no such trace is being made)
     if _is_tracing() or (proxies is not None and proxies.get_proxy_mode() is not None):

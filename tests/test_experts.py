@@ -316,7 +316,7 @@ def test_calls_without_the_extension(T, monkeypatch):
         y = fp6.expert_combine(rows, plan, w)
         grads = torch.autograd.grad(y, (x, w), g)
         product = fp6.int4_forward_native(rows.detach()[:, :128].contiguous(), weights.native, weights.native_scales, plan=plan)
-        return [rows, plan.offsets, plan.order, plan.place, y, *grads, fp6.expert_combine(wide, plan, None, torch.bfloat16), product]
+        return [rows, plan.table, y, *grads, fp6.expert_combine(wide, plan, None, torch.bfloat16), product]
     first = all_of()
     monkeypatch.setattr(fp6, "_ext", None)
     for a, b in zip(first, all_of()):
@@ -408,8 +408,8 @@ def test_refusals_of_the_c_abi():
 
 def refusals(dev, monkeypatch):
     index, x = torch.zeros(4, 2, dtype=torch.int64, device=dev), torch.zeros(4, 64, dtype=torch.float16, device=dev)
-    ints = torch.zeros(8, dtype=torch.int32, device=dev)
-    plan = fp6.experts.ExpertPlan(torch.zeros(4, dtype=torch.int32, device=dev), ints, ints, 4, 2)
+    plan = fp6.experts.ExpertPlan(torch.zeros(20, dtype=torch.int32, device=dev), 4, 2, 3)
+    short = fp6.experts.ExpertPlan(torch.zeros(19, dtype=torch.int32, device=dev), 4, 2, 3)
     rows, weights = torch.zeros(8, 64, dtype=torch.float16, device=dev), torch.zeros(4, 2, device=dev)
     for ext in (fp6._ext, None):
         monkeypatch.setattr(fp6, "_ext", ext)
@@ -417,7 +417,7 @@ def refusals(dev, monkeypatch):
                     dict(x=x.int()), dict(x=x[:, :0]), dict(index=index.cpu()), dict(x=x.cpu() if dev != "cpu" else x)):
             with pytest.raises(ValueError):
                 fp6.expert_sort(**{**dict(x=x, index=index, experts=3), **bad})
-        for bad in (dict(rows=rows[:7]), dict(rows=rows[0]), dict(rows=rows.double()), dict(rows=rows.int()), dict(dtype=torch.float32), dict(dtype=torch.bfloat16), dict(dtype=torch.float64), dict(weights=weights[:3]),
+        for bad in (dict(rows=rows[:7]), dict(rows=rows[0]), dict(rows=rows.double()), dict(rows=rows.int()), dict(plan=short), dict(dtype=torch.float32), dict(dtype=torch.bfloat16), dict(dtype=torch.float64), dict(weights=weights[:3]),
                     dict(weights=weights[:, :1]), dict(weights=weights.int()), dict(rows=rows.cpu() if dev != "cpu" else rows[:7]), dict(weights=weights.cpu() if dev != "cpu" else weights[:3])):
             for grad in (False, True):
                 args = {**dict(rows=rows, plan=plan, weights=weights), **bad}
@@ -462,3 +462,36 @@ def test_objects_of_the_makefile_depend_on_all_that_they_include():
         needs = [os.path.normpath(os.path.join(PACKAGE, n)) for n in needs.replace("$(HDRS)", headers).split()]
         missing = included(needs[0]) - set(needs)
         assert not missing, "%s.o: %s" % (target, sorted(os.path.basename(m) for m in missing))
+
+
+@gpu
+def test_second_derivatives_are_refused(monkeypatch):
+    T, k, E, H = 5, 2, 3, 16
+    index = route(1, T, k, E)
+    for ext in (fp6._ext, None):
+        monkeypatch.setattr(fp6, "_ext", ext)
+        x, w = randn(1, T, H, dtype=torch.float32).requires_grad_(), torch.rand(T, k, device=DEV).requires_grad_()
+        rows, plan = fp6.expert_sort(x, index, E)
+        for y, leaves in ((rows.square().sum(), (x,)), (fp6.expert_combine(rows, plan, w).square().sum(), (x, w))):
+            for g in torch.autograd.grad(y, leaves, create_graph=True):
+                with pytest.raises(RuntimeError):
+                    torch.autograd.grad(g.sum(), x, retain_graph=True)
+
+
+@gpu
+def test_gradients_that_are_not_asked_for():
+    T, k, E, H = 6, 2, 3, 40
+    index, rows = route(1, T, k, E), randn(1, T * k, H)
+    plan, w = fp6.expert_plan(index, E), torch.rand(T, k, device=DEV)
+    both_r, both_w = rows.clone().requires_grad_(), w.clone().requires_grad_()
+    g = randn(2, T, H)
+    want = torch.autograd.grad(fp6.expert_combine(both_r, plan, both_w), (both_r, both_w), g)
+    r = rows.clone().requires_grad_()
+    assert torch.equal(torch.autograd.grad(fp6.expert_combine(r, plan, w), r, g)[0], want[0])
+    v = w.clone().requires_grad_()
+    assert torch.equal(torch.autograd.grad(fp6.expert_combine(rows, plan, v), v, g)[0], want[1])
+    half = w.double().requires_grad_()   # (weights of another type are converted, and so is their gradient)
+    got, = torch.autograd.grad(fp6.expert_combine(rows, plan, half), half, g)
+    assert got.dtype == torch.float64 and torch.equal(got.float(), want[1])
+    with torch.no_grad():
+        assert not fp6.expert_combine(both_r, plan, both_w).requires_grad

@@ -312,8 +312,7 @@ def test_refusals_of_the_c_abi():
 
 def refusals(x, w, monkeypatch):
     ok = dict(in_feats=x, native_weight=w.native, native_scales=w.native_scales)
-    offsets = torch.zeros(3, dtype=torch.int32, device=x.device)
-    plan = fp6.experts.ExpertPlan(offsets, None, None, 1, 2)
+    plan = fp6.experts.ExpertPlan(torch.zeros(7, dtype=torch.int32, device=x.device), 1, 2, 2)
     cases = [dict(in_feats=x.float()), dict(in_feats=x.bfloat16()), dict(in_feats=x[0]), dict(in_feats=x[:, :32]), dict(in_feats=x[:, :40]), dict(in_feats=x.cpu()), dict(native_weight=w.native.float()),
              dict(native_weight=w.native[:1]), dict(native_weight=w.native[..., :128]), dict(native_scales=w.native_scales[..., 0]), dict(native_scales=w.native_scales.float()), dict(activation="relu"),
              dict(activation=3), dict(out_dtype=torch.bfloat16), dict(out_dtype=torch.float64), dict(out=torch.empty(2, 32, device=x.device)), dict(out=torch.empty(2, 31, dtype=torch.float16, device=x.device)),
