@@ -13,10 +13,22 @@ namespace {
 
 typedef _Float16 half_t;
 typedef __bf16   bf16_t;
+typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 
 constexpr int kWave = 64, kMostChosen = 64, kMostExperts = 1024;
 
 template <typename T, int VEC> struct alignas(sizeof(T) * VEC) Vec { T v[VEC]; };
+
+// Stores past the caches: outputs of many rows are read again when they have long been displaced (the copies of a sort of 4099 tokens x 2 of 8 KB: 28.4 us through the caches, 15.8 past them).
+template <typename T, int VEC> __device__ __forceinline__ void store_past(Vec<T, VEC> *to, const Vec<T, VEC> &v)
+{
+    if constexpr (sizeof(T) * VEC == 16)
+        __builtin_nontemporal_store(__builtin_bit_cast(v4u, v), reinterpret_cast<v4u *>(to));
+    else if constexpr (sizeof(T) * VEC == 8)
+        __builtin_nontemporal_store(__builtin_bit_cast(uint64_t, v), reinterpret_cast<uint64_t *>(to));
+    else
+        *to = v;
+}
 
 __device__ __forceinline__ int wave_sum(int v)
 {
@@ -41,24 +53,6 @@ template <typename I> __device__ __forceinline__ int expert_of(const I *index, s
 // ---------------------------------------------------------------------------------------------------------------
 // Sorting
 // ---------------------------------------------------------------------------------------------------------------
-// One row of x to the rows of its token's places (to[j] < 0: a row of zeros at ~to[j]), by `lanes` threads of which this is number `lane`.  The row is read once.
-template <typename V> __device__ __forceinline__ void copy_row(V *rows, const V *x, size_t nvec, const int *to, int k, uint32_t lane, uint32_t lanes)
-{
-    for (size_t i = lane; i < nvec; i += 4 * lanes) { // four loads on their way
-        V v[4];
-#pragma unroll
-        for (int u = 0; u < 4; u++)
-            if (i + u * lanes < nvec) v[u] = x[i + u * lanes];
-        for (int j = 0; j < k; j++) {
-            const int at = to[j];
-            V        *row = rows + (size_t)(at < 0 ? ~at : at) * nvec;
-#pragma unroll
-            for (int u = 0; u < 4; u++)
-                if (i + u * lanes < nvec) row[i + u * lanes] = at < 0 ? V{} : v[u];
-        }
-    }
-}
-
 // offsets[0..E] from counts[0..E-1] in LDS, by the first wavefront; starts[e] likewise (may be counts itself).
 __device__ __forceinline__ void scan_counts(const int *counts, int *starts, int *offsets, int E, int lane)
 {
@@ -101,32 +95,51 @@ __global__ __launch_bounds__(256) void sort_few(const I *__restrict__ index, int
         return;
     }
     __shared__ int to[kMostChosen];
+    V              v[4]; // the row's first pieces, asked for before it is known where they go
+#pragma unroll
+    for (uint32_t u = 0; u < 4; u++)
+        if (rows && tid + 256 * u < nvec) v[u] = x[t * ldx + tid + 256 * u];
     for (int j0 = 0; j0 < k; j0 += 8) {
         const int n = k - j0 < 8 ? k - j0 : 8;
-        int       mine[8], below[8];
+        int       mine[8], below[4] = {}; // (counts of 16 bits, two to a word)
 #pragma unroll
-        for (int j = 0; j < 8; j++) mine[j] = j < n ? expert_of(index, (size_t)t * k + j0 + j, E) : -1, below[j] = 0;
+        for (int j = 0; j < 8; j++) mine[j] = j < n ? expert_of(index, (size_t)t * k + j0 + j, E) : -1;
         for (uint32_t p = tid; p < P; p += 256) {
             const int e = expert_of(index, p, E);
 #pragma unroll
-            for (int j = 0; j < 8; j++) below[j] += e < mine[j] || (e == mine[j] && p < t * k + j0 + j);
+            for (int j = 0; j < 8; j++) below[j / 2] += (e < mine[j] || (e == mine[j] && p < t * k + j0 + j)) << 16 * (j & 1);
         }
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
+        for (int j = 0; j < 4; j++) {
+            if (2 * j >= n) break;
             const int s = wave_sum(below[j]);
-            if (lane == 0) shared[wave * 8 + j] = s;
+            if (lane == 0) shared[wave * 8 + 2 * j] = s & 0xffff, shared[wave * 8 + 2 * j + 1] = (uint32_t)s >> 16;
         }
         __syncthreads();
         if (tid < n) {
             const int at = shared[tid] + shared[8 + tid] + shared[16 + tid] + shared[24 + tid];
-            const bool none = expert_of(index, (size_t)t * k + j0 + tid, E) == E;
+            bool      none = false;
+#pragma unroll
+            for (int j = 0; j < 8; j++) none |= tid == j && mine[j] == E;
             to[j0 + tid] = none ? ~at : at;
             place[(size_t)t * k + j0 + tid] = at;
             order[at] = none ? -1 : (int)(t * k + j0 + tid);
         }
         __syncthreads();
     }
-    if (rows) copy_row(rows, x + (size_t)t * ldx, nvec, to, k, tid, 256);
+    if (!rows) return;
+    for (size_t i0 = 0; i0 < nvec; i0 += 1024) {
+        for (int j = 0; j < k; j++) {
+            const int at = to[j];
+            V        *row = rows + (size_t)(at < 0 ? ~at : at) * nvec + i0;
+#pragma unroll
+            for (uint32_t u = 0; u < 4; u++)
+                if (i0 + tid + 256 * u < nvec) row[tid + 256 * u] = at < 0 ? V{} : v[u];
+        }
+#pragma unroll
+        for (uint32_t u = 0; u < 4; u++)
+            if (i0 + 1024 + tid + 256 * u < nvec) v[u] = x[t * ldx + i0 + 1024 + tid + 256 * u];
+    }
 }
 
 // Many places, first launch: how many places of each expert every chunk of tokens holds, table[e][chunk] (rows of `stride` chunks).
@@ -142,65 +155,77 @@ template <typename I> __global__ __launch_bounds__(256) void count_chunks(const 
     for (int e = threadIdx.x; e < E; e += 256) table[(size_t)e * stride + b] = (uint16_t)counts[e];
 }
 
-// Second launch: a workgroup to a chunk.  It adds up the table for itself (all of it is in L2; a scan in between would be a third launch), ranks its places a few hundred at a time by comparing
-// them with each other, and copies the rows of their tokens, one to a wavefront.
-template <typename I, typename V>
-__global__ __launch_bounds__(512) void sort_chunks(const I *__restrict__ index, const uint16_t *__restrict__ table, int *__restrict__ offsets, int *__restrict__ order, int *__restrict__ place,
-                                                   const V *__restrict__ x, V *__restrict__ rows, size_t ldx, size_t nvec, uint32_t P, uint32_t each, uint32_t stride, int k, int E)
+// Second launch: a workgroup to a chunk.  It adds up the table for itself and ranks its places, 512 at a time.
+template <typename I>
+__global__ __launch_bounds__(512) void place_chunks(const I *__restrict__ index, const uint16_t *__restrict__ table, int *__restrict__ offsets, int *__restrict__ order, int *__restrict__ place,
+                                                    uint32_t P, uint32_t each, uint32_t stride, int E)
 {
     __shared__ int next[kMostExperts + 1], total[kMostExperts + 1]; // next: where the next place of an expert goes
-    __shared__ alignas(16) int keys[512];
-    __shared__ int             to[512];
+    __shared__ int counts[8];
     const int      tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const uint32_t b = blockIdx.x, chunks = gridDim.x, lo = b * each, hi = lo + each < P ? lo + each : P;
-    for (int e = wave; e < E; e += 8) {
+    int            e = lo + tid < hi ? expert_of(index, (size_t)lo + tid, E) : -1;
+#pragma unroll 4
+    for (int f = wave; f < E; f += 8) {
         int before = 0, all = 0;
-        for (uint32_t c0 = lane * 8; c0 < chunks; c0 += kWave * 8) { // (rows of the table end at a multiple of eight)
-            const Vec<uint16_t, 8> n = *reinterpret_cast<const Vec<uint16_t, 8> *>(table + (size_t)e * stride + c0);
-#pragma unroll
-            for (uint32_t i = 0; i < 8; i++) {
-                const int v = c0 + i < chunks ? n.v[i] : 0;
-                all += v, before += c0 + i < b ? v : 0;
-            }
+        for (uint32_t c = lane; c < chunks; c += kWave) {
+            const int v = table[(size_t)f * stride + c];
+            all += v, before += c < b ? v : 0;
         }
         all = wave_sum(all), before = wave_sum(before);
-        if (lane == 0) total[e] = all, next[e] = before;
+        if (lane == 0) total[f] = all, next[f] = before;
     }
     __syncthreads();
     if (wave == 0) scan_counts(total, total, b == 0 ? offsets : nullptr, E, lane);
     __syncthreads();
     // (those without an expert: behind all others, and of those in the chunks before this one there are as many as have none of the counted ones)
     int counted = 0;
-    for (int e = tid; e < E; e += 512) counted += next[e], next[e] += total[e];
+    for (int f = tid; f < E; f += 512) counted += next[f], next[f] += total[f];
     counted = wave_sum(counted);
-    if (lane == 0) keys[wave] = counted;
+    if (lane == 0) counts[wave] = counted;
     __syncthreads();
     if (tid == 0) {
-        for (int w = 1; w < 8; w++) counted += keys[w];
+        for (int w = 1; w < 8; w++) counted += counts[w];
         next[E] = total[E] + (int)lo - counted;
     }
-    const uint32_t pass = 512 / k * k; // whole tokens
-    for (uint32_t p0 = lo; p0 < hi; p0 += pass) {
-        __syncthreads();
-        const uint32_t n = hi - p0 < pass ? hi - p0 : pass;
-        const int      e = (uint32_t)tid < n ? expert_of(index, (size_t)p0 + tid, E) : -1;
-        keys[tid] = e;
-        __syncthreads();
-        int rank = 0;
-        for (int i = 0; i < tid; i += 4) {
-            const int4 o = *reinterpret_cast<const int4 *>(&keys[i]);
-            rank += (o.x == e) + (o.y == e && i + 1 < tid) + (o.z == e && i + 2 < tid) + (o.w == e && i + 3 < tid);
+    // Ranks: the lanes of a wavefront that share an expert find each other bit by bit of its number; the wavefronts, one after another, let the first lane of each move the expert's next place on.
+    for (uint32_t p0 = lo; p0 < hi; p0 += 512) {
+        uint64_t same = __ballot(e >= 0);
+        for (int bit = 1; bit <= E; bit <<= 1) {
+            const uint64_t set = __ballot(e >= 0 && (e & bit));
+            same &= e & bit ? set : ~set;
         }
-        if ((uint32_t)tid < n) {
-            const int at = next[e] + rank;
-            to[tid] = e == E ? ~at : at;
+        const int rank = __builtin_popcountll(same & ((1ull << lane) - 1)), leader = __builtin_ctzll(same | 1ull << 63);
+        int       at = 0;
+        for (int w = 0; w < 8; w++) {
+            __syncthreads();
+            if (wave == w && e >= 0 && rank == 0) at = atomicAdd(&next[e], __builtin_popcountll(same));
+        }
+        at = __shfl(at, leader) + rank;
+        if (e >= 0) {
             place[(size_t)p0 + tid] = at;
             order[at] = e == E ? -1 : (int)(p0 + tid);
         }
-        __syncthreads();
-        if ((uint32_t)tid < n) atomicAdd(&next[e], 1);
-        if (rows)
-            for (uint32_t t = wave; t < n / k; t += 8) copy_row(rows, x + (size_t)(p0 / k + t) * ldx, nvec, to + t * k, k, lane, kWave);
+        e = p0 + 512 + tid < hi ? expert_of(index, (size_t)p0 + 512 + tid, E) : -1;
+    }
+}
+
+// Third launch: the rows.  A piece of a row is read once and written to its token's places; those without an expert get zeros.
+template <typename V>
+__global__ __launch_bounds__(256) void copy_tokens(V *__restrict__ rows, const V *__restrict__ x, const int *__restrict__ place, const int *__restrict__ valid_at, size_t ldx, uint32_t nvec,
+                                                   uint32_t pieces, int k)
+{
+    const uint32_t t = blockIdx.x / pieces, i = (blockIdx.x - t * pieces) * 512 + threadIdx.x;
+    const int      valid = *valid_at;
+    V              v[2];
+#pragma unroll
+    for (uint32_t u = 0; u < 2; u++)
+        if (i + 256 * u < nvec) v[u] = x[t * ldx + i + 256 * u];
+    for (int j = 0; j < k; j++) {
+        const int at = place[(size_t)t * k + j];
+#pragma unroll
+        for (uint32_t u = 0; u < 2; u++)
+            if (i + 256 * u < nvec) __builtin_nontemporal_store(at < valid ? v[u] : V{}, &rows[(size_t)at * nvec + i + 256 * u]);
     }
 }
 
@@ -234,7 +259,7 @@ __global__ __launch_bounds__(256) void combine_rows(O *__restrict__ out, const R
     Vec<O, VEC> o;
 #pragma unroll
     for (int v = 0; v < VEC; v++) o.v[v] = (O)sum[v];
-    reinterpret_cast<Vec<O, VEC> *>(out)[(size_t)t * nvec + i] = o;
+    store_past(reinterpret_cast<Vec<O, VEC> *>(out) + (size_t)t * nvec + i, o);
 }
 
 // Its gradient: grad_rows[place[t,j]] = w[t,j] * grad[t] (zeros where there is no expert), grad_weights[t,j] = <grad[t], rows[place[t,j]]>; either may be left out.  A workgroup to a token.
@@ -269,7 +294,7 @@ __global__ __launch_bounds__(256) void combine_gradient(R *__restrict__ grad_row
                 Vec<R, VEC> d;
 #pragma unroll
                 for (int v = 0; v < VEC; v++) d.v[v] = at[j] < valid ? (R)(w[j] * (float)g.v[v]) : (R)0.f;
-                if (grad_rows) reinterpret_cast<Vec<R, VEC> *>(grad_rows)[(size_t)at[j] * nvec + i] = d;
+                if (grad_rows) store_past(reinterpret_cast<Vec<R, VEC> *>(grad_rows) + (size_t)at[j] * nvec + i, d);
                 if (grad_weights && at[j] < valid) {
 #pragma unroll
                     for (int v = 0; v < VEC; v++) dot[j] += (float)g.v[v] * (float)r[j].v[v];
@@ -295,17 +320,16 @@ inline bool aligned(const void *p, size_t n) { return (reinterpret_cast<uintptr_
 inline size_t type_size(int dtype) { return dtype == 2 ? 4 : 2; }
 inline bool known_type(int dtype) { return dtype >= 0 && dtype <= 2; }
 
-// From how many places on the sort takes two launches.
+// Up to how many places the sort takes one launch.
 constexpr size_t kFewPlaces = 2048;
 
-struct Chunks { uint32_t tokens, count, stride; }; // tokens of a chunk; how many chunks; the table's row length
-Chunks chunks_of(size_t tokens, size_t k, size_t E)
+struct Chunks { uint32_t each, count, stride; }; // places of a chunk; how many chunks; the table's row length
+Chunks chunks_of(size_t places)
 {
-    size_t count = ((size_t)16 << 20) / (E * 512);                             // every workgroup reads the whole table
-    count = count > 512 ? 512 : count < 64 ? 64 : count;
-    size_t each = (tokens + count - 1) / count;
-    if (each * k > 65535) each = 65535 / k;                                    // (counts have 16 bits)
-    count = (tokens + each - 1) / each;
+    size_t count = (places + 511) / 512; // (as many as a workgroup ranks at a time; every workgroup reads the whole table)
+    count = count > 256 ? 256 : count;
+    const size_t each = (places + count - 1) / count < 65535 ? (places + count - 1) / count : 65535; // (counts have 16 bits)
+    count = (places + each - 1) / each;
     return { (uint32_t)each, (uint32_t)count, (uint32_t)((count + 7) / 8 * 8) };
 }
 
@@ -320,12 +344,14 @@ int launch_sort(hipStream_t st, const void *index, int *offsets, int *order, int
                            nvec, (uint32_t)tokens, (int)k, (int)E);
         return (int)hipGetLastError();
     }
-    const Chunks c = chunks_of(tokens, k, E);
+    const Chunks c = chunks_of(P);
     uint16_t    *table = static_cast<uint16_t *>(ws);
-    hipLaunchKernelGGL(count_chunks<I>, dim3(c.count), dim3(256), 0, st, static_cast<const I *>(index), table, (uint32_t)P, c.tokens * (uint32_t)k, c.stride, (int)E);
+    hipLaunchKernelGGL(count_chunks<I>, dim3(c.count), dim3(256), 0, st, static_cast<const I *>(index), table, (uint32_t)P, c.each, c.stride, (int)E);
     if (const hipError_t e = hipGetLastError()) return (int)e;
-    hipLaunchKernelGGL((sort_chunks<I, V>), dim3(c.count), dim3(512), 0, st, static_cast<const I *>(index), table, offsets, order, place, static_cast<const V *>(x), static_cast<V *>(rows), ldx, nvec,
-                       (uint32_t)P, c.tokens * (uint32_t)k, c.stride, (int)k, (int)E);
+    hipLaunchKernelGGL(place_chunks<I>, dim3(c.count), dim3(512), 0, st, static_cast<const I *>(index), table, offsets, order, place, (uint32_t)P, c.each, c.stride, (int)E);
+    if (const hipError_t e = hipGetLastError(); e != hipSuccess || !rows) return (int)e;
+    const uint32_t pieces = (uint32_t)((nvec + 511) / 512);
+    hipLaunchKernelGGL(copy_tokens<V>, dim3((uint32_t)tokens * pieces), dim3(256), 0, st, static_cast<V *>(rows), static_cast<const V *>(x), place, offsets + E, ldx, (uint32_t)nvec, pieces, (int)k);
     return (int)hipGetLastError();
 }
 
@@ -363,7 +389,7 @@ extern "C" {
 size_t fp6mi_expert_sort_workspace_bytes(size_t tokens, size_t k, size_t experts)
 {
     if (tokens == 0 || check_places(tokens, k, experts) != FP6MI_OK || tokens * k <= kFewPlaces) return 0;
-    return experts * chunks_of(tokens, k, experts).stride * sizeof(uint16_t);
+    return experts * chunks_of(tokens * k).stride * sizeof(uint16_t);
 }
 
 int fp6mi_expert_sort(void *stream, const void *index, int index64, int *offsets, int *order, int *place, const void *x, size_t ldx, void *rows, size_t tokens, size_t k, size_t experts, size_t H,
@@ -380,6 +406,7 @@ int fp6mi_expert_sort(void *stream, const void *index, int index64, int *offsets
         if (H < 1 || H > (size_t)1 << 24 || (ldx < H && tokens > 1) || ldx > (size_t)1 << 40) return FP6MI_ERR_SHAPE;
         unit = type_size(dtype);
         if (!aligned(x, unit) || !aligned(rows, unit)) return FP6MI_ERR_ALIGN;
+        if (tokens * ((H * unit + 511) / 512) > 0x7fffffffu) return FP6MI_ERR_SHAPE;
         if (aligned(x, 16) && aligned(rows, 16) && H * unit % 16 == 0 && (ldx * unit % 16 == 0 || tokens == 1)) unit = 16;
     }
     if (fp6mi_expert_sort_workspace_bytes(tokens, k, experts) && !workspace) return FP6MI_ERR_WORKSPACE;
@@ -389,7 +416,7 @@ int fp6mi_expert_sort(void *stream, const void *index, int index64, int *offsets
     void        *to = copies ? rows : nullptr;
     return by_index(index64, [&](auto wide) {
         typedef std::conditional_t<decltype(wide)::value, int64_t, int32_t> I;
-        if (unit == 16) return launch_sort<I, Vec<uint32_t, 4>>(st, index, offsets, order, place, x, to, ld, nvec, tokens, k, experts, workspace);
+        if (unit == 16) return launch_sort<I, v4u>(st, index, offsets, order, place, x, to, ld, nvec, tokens, k, experts, workspace);
         if (unit == 4) return launch_sort<I, uint32_t>(st, index, offsets, order, place, x, to, ld, nvec, tokens, k, experts, workspace);
         return launch_sort<I, uint16_t>(st, index, offsets, order, place, x, to, ld, nvec, tokens, k, experts, workspace);
     });
