@@ -284,22 +284,24 @@ template <int GPB, bool Z, int RT, int NT, int WK> int launch_stream(hipStream_t
 }
 
 // ---------------------------------------------------------------------------------------------------------------
-// Many rows: tiles of WR * RT * 16 weight rows x WC * NT * 16 rows of X to a workgroup of WR * WC wavefronts.  X goes to LDS by direct transfers, a K block ahead, two stages; a row of a stage is 256
-// bytes whose 16 pieces stand in the order piece ^ (row & 15), which gives the reads of an MFMA operand all banks.  A wavefront holds its rows of X for one block in registers and takes one row tile after
-// another: its codes become operands while the tile before is multiplied.  Bound by the matrix units with the conversions and the scaling of the group sums beside them (VALU).
+// More rows: tiles of WR * 64 weight rows x NT * 16 rows of X to a workgroup of WR x WK wavefronts; the WK groups take every WK-th column block.  X goes to LDS by direct transfers, a K block ahead, two
+// stages to a group; a row of a stage is 256 bytes whose 16 pieces stand in the order piece ^ (row & 15), which gives the reads of an MFMA operand all banks.  A wavefront holds its X of one block in
+// registers and takes one of its four row tiles after another: its codes become operands while the tile before is multiplied.  Bound by the matrix units with the conversions and the scaling of the
+// group sums beside them (3.6 VALU instructions to a matrix instruction; twice the columns to a wavefront, 2.6, was no faster, nor were 32x32x16 instructions, which draw more power).
+// Two workgroups to a CU where LDS allows, so that one multiplies while the other waits at its barrier.
 // ---------------------------------------------------------------------------------------------------------------
-constexpr size_t tile_lds_bytes(int cols, int rows) // the stages, and the outputs on their way out: a half of them at a time where they are float32
+template <int NT, int WR, int WK> constexpr size_t tile_lds_bytes() // the stages; the sums of the groups on their way to the first; the outputs on their way out (a half at a time where they are float32)
 {
-    const size_t stages = 2 * (size_t)cols * 256, outputs = (size_t)cols * (rows * 2 + 16);
-    return stages > outputs ? stages : outputs;
+    const size_t stages = (size_t)WK * 2 * NT * 4096, sums = (size_t)(WK - 1) * WR * NT * 4096, outputs = NT * 16 * ((size_t)WR * 128 + 16);
+    return stages > outputs ? (stages > sums ? stages : sums) : (outputs > sums ? outputs : sums);
 }
 
-template <int GPB, bool Z, int RT, int NT, int WR, int WC> __global__ __launch_bounds__(WR *WC * 64, 2) void int4_tile(const Int4Args a, uint32_t col_tiles)
+template <int GPB, bool Z, int NT, int WR, int WK> __global__ __launch_bounds__(WR *WK * 64, 2) void int4_tile(const Int4Args a, uint32_t col_tiles)
 {
-    static_assert(RT == 4 && NT == 4, "the steps of a block are written for these");
-    constexpr int      kWaves = WR * WC, kCols = WC * NT * 16, kTiles = WR * RT, kRows = kTiles * 16, kStage = kCols * 256, kDma = kCols / 4 / kWaves;
+    static_assert(NT == 2 || NT == 4, "the steps of a block are written for these");
+    constexpr int      RT = 4, kWaves = WR * WK, kCols = NT * 16, kTiles = WR * RT, kRows = kTiles * 16, kStage = kCols * 256, kDma = kCols / 4 / WR;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, q = lane >> 4, wr = wave % WR, wc = wave / WR;
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, q = lane >> 4, wr = wave % WR, wk = wave / WR;
 
     // Workgroups that an XCD runs side by side are panels of eight row blocks by a few column tiles, mostly of one expert.
     const uint32_t per = gridDim.x >> 3, rem = gridDim.x & 7u, xcd = blockIdx.x & 7u, id = xcd * per + (xcd < rem ? xcd : rem) + (blockIdx.x >> 3);
@@ -312,23 +314,19 @@ template <int GPB, bool Z, int RT, int NT, int WR, int WC> __global__ __launch_b
     // transfers of X: four rows of one block each
     typedef __attribute__((address_space(3))) void lvoid;
     const auto     xbuf = __builtin_amdgcn_make_buffer_rsrc(const_cast<T *>(static_cast<const T *>(a.X) + (size_t)t.row * a.K), 0, (int)(t.rows * a.K * 2), 0x00027000);
-    uint32_t       xrow[kDma], xpiece[kDma];
-#pragma unroll
-    for (uint32_t j = 0; j < kDma; j++) {
-        const uint32_t row = (j * kWaves + wave) * 4 + q;
-        xrow[j] = (row < t.rows ? row : t.rows - 1) * a.K * 2; // 32 bits: the launcher bounds K
-        xpiece[j] = (c ^ (row & 15)) * 8;
-    }
-    auto transfer = [&](uint32_t kb, uint32_t stage) __attribute__((always_inline)) {
+    uint8_t *const xstage = lds + wk * 2 * kStage;
+    const uint32_t xpiece = c ^ q, xlast = (t.rows - 1) * a.K * 2; // 32 bits: the launcher bounds K
+    auto           transfer = [&](uint32_t kb, uint32_t stage) __attribute__((always_inline)) {
 #pragma unroll
         for (uint32_t j = 0; j < kDma; j++) {
-            const uint32_t k = kb * 128 + xpiece[j], off = xrow[j] + (k < a.K ? k * 2 : 0xc0000000u); // (beyond the buffer, which reads as zeros)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(xbuf, (lvoid *)(lds + stage * kStage + (j * kWaves + wave) * 1024), 16, off, 0, 0, 0);
+            const uint32_t row4 = j * WR + wr, row = (row4 * 4 + q) * a.K * 2, k = kb * 128 + (xpiece ^ 4 * (row4 & 3)) * 8;
+            const uint32_t off = (row < xlast ? row : xlast) + (k < a.K ? k * 2 : 0xc0000000u); // (beyond the buffer, which reads as zeros)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(xbuf, (lvoid *)(xstage + stage * kStage + row4 * 1024), 16, off, 0, 0, 0);
         }
     };
     // operands of X: of the first two tiles of the next block while this one's are still in use, of the others in their place
-    const uint8_t *xread = lds + (wc * NT * 16 + c) * 256;
-    v8t            early[2][2][4], late[2][4];
+    const uint8_t *xread = xstage + c * 256;
+    v8t            early[2][2][4], late[NT > 2 ? NT - 2 : 1][4];
     auto           read_x = [&](v8t &to, int n, uint32_t i, uint32_t stage) __attribute__((always_inline)) {
         to = *reinterpret_cast<const v8t *>(xread + stage * kStage + n * 16 * 256 + ((4 * i + q) ^ c) * 16);
     };
@@ -371,23 +369,26 @@ template <int GPB, bool Z, int RT, int NT, int WR, int WC> __global__ __launch_b
 #pragma unroll
     for (int g = 0; g < GPB; g++) scale[(RT - 1) & 1][g] = 0.f;
 
-    // A block is RT * 2 steps of two tiles of X by one row tile; a step also converts half of the next row tile, adds up the groups that the step before has multiplied, and reads some of the next
-    // block's X.  The last row tile takes the tiles of X in the other order, which frees the registers of the late ones a step earlier.
-    auto step = [&](auto u_c, auto set_c, uint32_t kb) __attribute__((always_inline)) {
-        constexpr int u = decltype(u_c)::value, set = decltype(set_c)::value, r = u / 2, last = 2 * RT - 1;
-        constexpr int n = (u & 1) ^ (r == RT - 1) ? 2 : 0, next = (r + 1) % RT;
-        constexpr int pu = u == 0 ? last : u - 1, pr = pu / 2, pn = (pu & 1) ^ (pr == RT - 1) ? 2 : 0; // the step before
-        if constexpr (u == 2) { // the next block's X has landed (behind its transfers come the loads of every row tile), and all have read this one's
+    // A block is RT * NT / 2 steps of two tiles of X by one row tile; a step also converts its share of the next row tile, adds up the groups that the step before has multiplied, and reads some of the
+    // next block's X.  The last row tile takes the early tiles of X last, so that the registers of the others are free for the next block's.
+    constexpr int kPairs = NT / 2, kSteps = RT * kPairs;
+    auto          step = [&](auto u_c, auto set_c, uint32_t kb) __attribute__((always_inline)) {
+        constexpr int u = decltype(u_c)::value, set = decltype(set_c)::value, r = u / kPairs, p = u % kPairs;
+        constexpr int n = 2 * (r == RT - 1 ? (p + 1) % kPairs : p), next = (r + 1) % RT;
+        constexpr int pu = u == 0 ? kSteps - 1 : u - 1, pr = pu / kPairs, pn = 2 * (pr == RT - 1 ? (pu % kPairs + 1) % kPairs : pu % kPairs); // the step before
+        if constexpr (u == kPairs) { // the next block's X has landed (behind its transfers come the loads of every row tile), and all have read this one's
             asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(RT) : "memory");
-            transfer(kb + 2, set);
+            transfer(kb + 2 * WK, set);
+            asm volatile("" ::: "memory");
         }
-        if constexpr (u >= 2 && u < 6) {
+        constexpr int kReads = NT == 2 ? 4 : 2; // of an early tile's operands in a step
+        if constexpr (u >= kPairs && u < kPairs + 8 / kReads) {
 #pragma unroll
-            for (int i = 0; i < 2; i++) read_x(early[set ^ 1][(u - 2) / 2][u % 2 * 2 + i], (u - 2) / 2, u % 2 * 2 + i, set ^ 1);
+            for (int e = (u - kPairs) * kReads; e < (u - kPairs + 1) * kReads; e++) read_x(early[set ^ 1][e / 4][e % 4], e / 4, e % 4, set ^ 1);
         }
-        if constexpr (u == last) {
+        if constexpr (r == RT - 1 && p > 0) { // in the place of the step before
 #pragma unroll
-            for (int i = 0; i < 8; i++) read_x(late[i / 4][i % 4], 2 + i / 4, i % 4, set ^ 1);
+            for (int i = 0; i < 8; i++) read_x(late[pn - 2 + i / 4][i % 4], pn + i / 4, i % 4, set ^ 1);
         }
         // of the groups multiplied before: pair v of them, tiles n and n + 1 of X by row tile r, from tile `from` of the two on
         auto add = [&](int r, int n, int g, int v, int from, int to) __attribute__((always_inline)) {
@@ -400,7 +401,8 @@ template <int GPB, bool Z, int RT, int NT, int WR, int WC> __global__ __launch_b
         for (int i = 0; i < 4; i++) {
             const int v = u * GPB + i / kEach;
 #pragma unroll
-            for (int k = 0; k < 2; k++) y[v & 1][k] = mfma(n == 0 ? early[set][k][i] : late[k][i], op[r & 1][i].v, i % kEach == 0 ? (v4f){ 0.f, 0.f, 0.f, 0.f } : y[v & 1][k]);
+            for (int k = 0; k < 2; k++)
+                y[v & 1][k] = mfma(n == 0 ? early[set][k][i] : late[n == 0 ? 0 : n - 2 + k][i], op[r & 1][i].v, i % kEach == 0 ? (v4f){ 0.f, 0.f, 0.f, 0.f } : y[v & 1][k]);
             if constexpr (GPB == 1) {
                 if (i == 1 || i == 2) add(pr, pn, 0, v + 1, i - 1, i);
             } else if constexpr (GPB == 2) {
@@ -412,74 +414,95 @@ template <int GPB, bool Z, int RT, int NT, int WR, int WC> __global__ __launch_b
                 else
                     add(r, n, i - 1, v + 1, 0, 2);
             }
-            convert((r + 1) & 1, next, (u & 1) * 2 + i / 2, i & 1);
+            if constexpr (kPairs == 2) {
+                convert((r + 1) & 1, next, p * 2 + i / 2, i & 1);
+            } else {
+                convert((r + 1) & 1, next, i, 0);
+                convert((r + 1) & 1, next, i, 1);
+            }
             if (i < 3) __builtin_amdgcn_sched_barrier(0);
         }
-        if constexpr (u & 1) {
+        if constexpr (p == kPairs - 1) {
             take_scales((r + 1) & 1, next);
-            load_w(next, r + 1 < RT ? kb + 1 : kb + 2);
+            load_w(next, kb + (r + 1 < RT ? WK : 2 * WK));
         }
         __builtin_amdgcn_sched_barrier(0);
     };
-    auto block = [&](auto set_c, uint32_t kb) __attribute__((always_inline)) { sections<2 * RT>([&](auto u_c) __attribute__((always_inline)) { step(u_c, set_c, kb); }); };
-    transfer(0, 0);
-    load_w(0, 0);
+    auto block = [&](auto set_c, uint32_t kb) __attribute__((always_inline)) { sections<kSteps>([&](auto u_c) __attribute__((always_inline)) { step(u_c, set_c, kb); }); };
+    transfer(wk, 0);
+    load_w(0, wk);
     asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
-    transfer(1, 1);
+    transfer(wk + WK, 1);
     asm volatile("" ::: "memory");
 #pragma unroll
     for (int i = 0; i < 8; i++) read_x(early[0][i / 4][i % 4], i / 4, i % 4, 0);
 #pragma unroll
-    for (int i = 0; i < 8; i++) read_x(late[i / 4][i % 4], 2 + i / 4, i % 4, 0);
+    for (int i = 0; i < 4 * (NT - 2); i++) read_x(late[i / 4][i % 4], 2 + i / 4, i % 4, 0);
 #pragma unroll
     for (int i = 0; i < 8; i++) convert(0, 0, i / 2, i & 1);
     take_scales(0, 0);
 #pragma unroll
-    for (int r = 0; r < RT; r++) load_w(r, r == 0 ? 1 : 0);
-    uint32_t kb = 0;
-    for (; kb + 2 <= a.KB; kb += 2) {
+    for (int r = 0; r < RT; r++) load_w(r, r == 0 ? wk + WK : wk);
+    uint32_t kb = wk, left = (a.KB + WK - 1) / WK; // blocks of every group (of those beyond the last one X reads as zeros)
+    for (; left >= 2; left -= 2, kb += 2 * WK) {
         block(std::integral_constant<int, 0>{}, kb);
-        block(std::integral_constant<int, 1>{}, kb + 1);
+        block(std::integral_constant<int, 1>{}, kb + WK);
     }
-    if (kb < a.KB) block(std::integral_constant<int, 0>{}, kb);
+    if (left) block(std::integral_constant<int, 0>{}, kb);
 #pragma unroll
     for (int k = 0; k < 2; k++) // the last pair
 #pragma unroll
         for (int i = 0; i < 4; i++) sum[RT - 1][k][i] += scale[(RT - 1) & 1][GPB - 1] * y[1][k][i];
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); // nothing is on its way to LDS any more
 
-    // outputs through LDS, so that a lane stores 16 bytes: [row of X][weight row], rows 16 bytes apart from a multiple of 512
+    if constexpr (WK > 1) { // the sums of the other groups to the first, [group][row wavefront][r][n][lane]
+        auto at = [&](int g, int r, int n) { return reinterpret_cast<v4f *>(lds) + ((((g - 1) * WR + wr) * RT + r) * NT + n) * 64 + lane; };
+#pragma unroll
+        for (int r = 0; r < RT; r++)
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+                if (wk > 0) *at(wk, r, n) = sum[r][n];
+        __syncthreads();
+        if (wk == 0)
+#pragma unroll
+            for (int r = 0; r < RT; r++)
+#pragma unroll
+                for (int n = 0; n < NT; n++)
+#pragma unroll
+                    for (int g = 1; g < WK; g++) sum[r][n] += *at(g, r, n);
+        __syncthreads();
+    }
+
+    // outputs through LDS, so that a lane stores 16 bytes: [row of X][weight row], rows 16 bytes apart from a multiple of 128
     const T *bias = a.bias ? static_cast<const T *>(a.bias) + (size_t)t.expert * a.Mt * 16 : nullptr;
     auto     out = [&](auto type, auto gated_c) __attribute__((always_inline)) {
         typedef decltype(type) O;
         constexpr bool     gated = decltype(gated_c)::value;
-        constexpr uint32_t kHalves = sizeof(O) == 4 && !gated ? 2 : 1, kOut = gated ? kRows / 2 : kRows, kPitch = kOut * sizeof(O) + 16, kEach = 16 / sizeof(O);
-        static_assert((size_t)kCols / kHalves * kPitch <= tile_lds_bytes(kCols, kRows), "");
+        constexpr uint32_t kHalves = sizeof(O) == 4 && !gated ? 2 : 1, kOut = gated ? kRows / 2 : kRows, kPitch = kOut * sizeof(O) + 16, kEach = 16 / sizeof(O), kNs = NT / kHalves;
+        static_assert((size_t)kCols / kHalves * kPitch <= tile_lds_bytes<NT, WR, WK>(), "");
         const uint32_t ld = a.Mt * (gated ? 8 : 16), col0 = m0 * (gated ? 8 : 16);
 #pragma unroll
         for (uint32_t h = 0; h < kHalves; h++) {
             if (h) __syncthreads();
+            if (wk == 0)
 #pragma unroll
-            for (uint32_t n = 0; n < NT; n++) {
-                const uint32_t row = (wc * NT + n) * 16 + 4 * q - h * (kCols / kHalves);
-                if (row >= kCols / kHalves) continue; // (the other half's)
+                for (uint32_t n = h * kNs; n < (h + 1) * kNs; n++)
 #pragma unroll
-                for (uint32_t r = 0; r < RT; r += gated ? 2 : 1) {
-                    const uint32_t m = (m0 + wr * RT + r) * 16 + c;
-                    const bool     in = bias && m0 + wr * RT + r < a.Mt;
-                    const float    b0 = in ? (float)bias[m] : 0.f, b1 = gated && in ? (float)bias[m + 16] : 0.f;
+                    for (uint32_t r = 0; r < RT; r += gated ? 2 : 1) {
+                        const uint32_t m = (m0 + wr * RT + r) * 16 + c, row = (n - h * kNs) * 16 + 4 * q;
+                        const bool     in = bias && m0 + wr * RT + r < a.Mt;
+                        const float    b0 = in ? (float)bias[m] : 0.f, b1 = gated && in ? (float)bias[m + 16] : 0.f;
 #pragma unroll
-                    for (uint32_t i = 0; i < 4; i++) {
-                        float v = sum[r][n][i] + b0;
-                        if constexpr (gated) v = activated(a.act, v) * (sum[r + 1][n][i] + b1);
-                        reinterpret_cast<O *>(lds + (row + i) * kPitch)[gated ? (wr * RT + r) * 8 + c : (wr * RT + r) * 16 + c] = (O)v;
+                        for (uint32_t i = 0; i < 4; i++) {
+                            float v = sum[r][n][i] + b0;
+                            if constexpr (gated) v = activated(a.act, v) * (sum[r + 1][n][i] + b1);
+                            reinterpret_cast<O *>(lds + (row + i) * kPitch)[gated ? (wr * RT + r) * 8 + c : (wr * RT + r) * 16 + c] = (O)v;
+                        }
                     }
-                }
-            }
             __syncthreads();
             constexpr uint32_t kPieces = kOut / kEach; // of a row
-            for (uint32_t i = tid; i < kCols / kHalves * kPieces; i += kWaves * 64) {
-                const uint32_t row = i / kPieces, piece = i % kPieces, col = col0 + piece * kEach, n = h * (kCols / kHalves) + row;
+            for (uint32_t i = tid; i < kNs * 16 * kPieces; i += kWaves * 64) {
+                const uint32_t row = i / kPieces, piece = i % kPieces, col = col0 + piece * kEach, n = h * kNs * 16 + row;
                 if (n < t.rows && col < ld) // (ld is a multiple of 8)
                     *reinterpret_cast<v4u *>(static_cast<O *>(a.Y) + (size_t)(t.row + n) * ld + col) = *reinterpret_cast<const v4u *>(lds + row * kPitch + piece * 16);
             }
@@ -498,22 +521,22 @@ template <int GPB, bool Z, int RT, int NT, int WR, int WC> __global__ __launch_b
     }
 }
 
-template <int GPB, bool Z, int RT, int NT, int WR, int WC> int launch_tile(hipStream_t st, const Int4Args &a)
+template <int GPB, bool Z, int NT, int WR, int WK> int launch_tile(hipStream_t st, const Int4Args &a)
 {
-    constexpr size_t bytes = tile_lds_bytes(WC * NT * 16, WR * RT * 16);
-    const size_t     cols = fp6mi::int4_tiles(a.N, a.offsets ? a.E : 0, WC * NT * 16), rows = (a.Mt + WR * RT - 1) / (WR * RT);
+    constexpr size_t bytes = tile_lds_bytes<NT, WR, WK>();
+    const size_t     cols = fp6mi::int4_tiles(a.N, a.offsets ? a.E : 0, NT * 16), rows = (a.Mt + WR * 4 - 1) / (WR * 4);
     if (cols * rows > 0x7fffffffu) return FP6MI_ERR_SHAPE;
     if constexpr (bytes > 65536)
-        if (const int e = allow_dynamic_lds<int4_tile<GPB, Z, RT, NT, WR, WC>>(bytes)) return e;
-    hipLaunchKernelGGL((int4_tile<GPB, Z, RT, NT, WR, WC>), dim3((uint32_t)(cols * rows)), dim3(WR * WC * 64), bytes, st, a, (uint32_t)cols);
+        if (const int e = allow_dynamic_lds<int4_tile<GPB, Z, NT, WR, WK>>(bytes)) return e;
+    hipLaunchKernelGGL((int4_tile<GPB, Z, NT, WR, WK>), dim3((uint32_t)(cols * rows)), dim3(WR * WK * 64), bytes, st, a, (uint32_t)cols);
     return (int)hipGetLastError();
 }
 
 template <int GPB, bool Z> int run(hipStream_t st, const Int4Args &a)
 {
     if (a.N <= 16 || (a.offsets && a.N <= 16 * a.E)) return launch_stream<GPB, Z, 2, 1, 8>(st, a);
-    if (a.K <= 1u << 20 && a.N > (a.offsets ? 64 * a.E : 64)) return launch_tile<GPB, Z, 4, 4, 4, 1>(st, a);
-    return launch_stream<GPB, Z, 2, 4, 4>(st, a);
+    if (a.N <= 32 || (a.offsets && a.N <= 32 * a.E)) return launch_tile<GPB, Z, 2, 1, 4>(st, a);
+    return launch_tile<GPB, Z, 4, 4, 1>(st, a);
 }
 
 } // namespace
