@@ -9,7 +9,7 @@ ROOT = os.path.dirname(HERE)
 # (source, object name, extra flags): the kernel files are compiled once per weight format (tag = 10*E + M), the objects in parallel
 FORMAT_TAGS = (32, 22, 23, 21)
 UNITS = [("fp6mi_%s.hip" % f, "fp6mi_%s_%d.o" % (f, t), ["-DFP6MI_FORMAT=%d" % t]) for f in ("gemm", "block") for t in FORMAT_TAGS] + \
-        [("fp6mi_int4.hip", "fp6mi_int4_%s.o" % n, ["-DFP6MI_TYPE=%d" % t]) for t, n in enumerate(("f16", "bf16"))] + \
+        [("fp6mi_int4.hip", "fp6mi_int4_%d_%d.o" % (t, g), ["-DFP6MI_TYPE=%d" % t, "-DFP6MI_GROUPS=%d" % g]) for t in (0, 1) for g in (1, 2, 4)] + \
         [("fp6mi_int4_api.hip", "fp6mi_int4_api.o", []), ("fp6mi_experts.hip", "fp6mi_experts.o", [])] + \
         [("fp6mi_host.cpp", "fp6mi_host.o", []), ("fp6mi_api.hip", "fp6mi_api.o", []), ("fp6mi_ops.hip", "fp6mi_ops.o", [])]
 OBJ_DIR = os.path.join(HERE, "csrc", "obj")

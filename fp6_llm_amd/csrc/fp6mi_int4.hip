@@ -2,8 +2,9 @@
 // are sorted by expert, for the matrix of each row's expert; optionally act(gate) * up of the pairs of 16 rows.  Compiled once per activation type (FP6MI_TYPE 0: fp16, 1: bf16).
 // No counterpart in the reference.
 //
-// q - z is an integer from -15 to 15, exact in fp16 and bf16, so the matrix instructions' products are exact and their sums float32; a group's sum is multiplied by its scale in float32.
-// (Scaling the weights before the product would round each of them to 16 bits, and 16-bit sums would be no cheaper.)
+// q - z is an integer from -15 to 15, exact in fp16, so the matrix instructions' products are exact and their sums float32; a group's sum is multiplied by its scale in float32.
+// (Scaling the weights before the product would round each of them to 16 bits, and 16-bit sums would be no cheaper.)  bf16 has no packed arithmetic that would make q - z of codes: the kernel of
+// few rows multiplies 128 + q, which are bits, and -(128 + z), the one of many rows is given X in fp16 with an exponent for each row (rows_to_halfs).
 //
 // Layout (fp6mi_int4_pack): blocks of 16 rows x 128 columns of 1024 bytes, [expert][row tile][column block]; lane c + 16 q of a wavefront holds 16 bytes of a block, dword s of which are the
 // columns 32 s + 8 q to 32 s + 8 q + 7 of row c: the operand of one v_mfma_f32_16x16x32.  In a dword the nibbles 0..7 are the columns 0, 2, 4, 6, 1, 3, 5, 7, so that a mask leaves two neighbours
@@ -26,7 +27,9 @@ typedef __bf16 T;
 #endif
 #include "fp6mi_lds.inc"
 
-typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+typedef _Float16 half_t;
+typedef half_t   v2h __attribute__((ext_vector_type(2)));
+typedef half_t   v8h __attribute__((ext_vector_type(8)));
 typedef T        v8t __attribute__((ext_vector_type(8)));
 typedef float    v4f __attribute__((ext_vector_type(4)));
 typedef uint32_t v4u __attribute__((ext_vector_type(4)));
@@ -42,6 +45,8 @@ __device__ __forceinline__ v4f mfma(v8t x, v8t w, v4f acc)
 #endif
 }
 
+__device__ __forceinline__ v4f mfma_halfs(v8h x, v8h w, v4f acc) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(x, w, acc, 0, 0, 0); }
+
 // f(0), ..., f(N - 1) with the index as a compile-time constant
 template <int N, int I = 0, typename F> __device__ __forceinline__ void sections(const F &f)
 {
@@ -49,54 +54,71 @@ template <int N, int I = 0, typename F> __device__ __forceinline__ void sections
     if constexpr (I + 1 < N) sections<N, I + 1>(f);
 }
 
-// What a group's zero point (8 without one) makes of the codes.
-struct Zero {
-#if FP6MI_TYPE == 0
-    v2h low, high; // -(1024 + z), -(64 + z)
-    __device__ __forceinline__ void set(T z)
-    {
-        const T l = (T)-1024.f - z, h = (T)-64.f - z;
-        low = (v2h){ l, l }, high = (v2h){ h, h };
-    }
-#else
-    float z;
-    __device__ __forceinline__ void set(T v) { z = (float)v; }
-#endif
-};
-
 // What the codes are cut out with.  (w & mask) | bits is one instruction where of the two constants one is in a vector register, of which the compiler has to be told.
 struct Cutter {
-#if FP6MI_TYPE == 0
     uint32_t low = 0x000f000fu, high = 0x00f000f0u, bits = 0x64006400u;
     __device__ __forceinline__ Cutter() { asm("" : "+s"(low), "+s"(high), "+v"(bits)); }
-#endif
 };
 
-// Eight codes as q - z, columns 0..7, or (half) four of them.  fp16: 1024 + q and 1024 + 16 q are read off the bits 0x6400 | nibble, 9 instructions.  bf16 has no packed arithmetic: bytes to float32,
-// and the upper halves of the exact differences, 23.
-union Codes { uint32_t d[4]; v8t v; };
+// What a group's zero point (8 without one) makes of the codes: -(1024 + z), -(64 + z).
+struct Zero {
+    v2h low, high;
+    __device__ __forceinline__ void set(T zero)
+    {
+        const half_t z = (half_t)(float)zero, l = (half_t)-1024.f - z, h = (half_t)-64.f - z;
+        low = (v2h){ l, l }, high = (v2h){ h, h };
+    }
+};
+
+// Eight codes as q - z in fp16, columns 0..7, or (half) four of them: 1024 + q and 1024 + 16 q are read off the bits 0x6400 | nibble, 9 instructions.
+union Codes { uint32_t d[4]; v8h v; };
 __device__ __forceinline__ void codes_half(Codes &to, uint32_t w, const Zero &zero, const Cutter &cut, int half)
 {
-#if FP6MI_TYPE == 0
-    const v2h sixteenth = { (_Float16)0.0625f, (_Float16)0.0625f };
+    const v2h sixteenth = { (half_t)0.0625f, (half_t)0.0625f };
     if (half) w >>= 8;
     to.d[2 * half] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(v2h, (w & cut.low) | cut.bits) + zero.low);
     to.d[2 * half + 1] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(__builtin_bit_cast(v2h, (w & cut.high) | cut.bits), sixteenth, zero.high));
-#else
-    auto pair = [&](uint32_t b) { // bytes: nibbles n and n + 4 in the lower halves of the words
-        const float lo = (float)(uint8_t)(b >> 8 * half) - zero.z, hi = (float)(uint8_t)(b >> (8 * half + 16)) - zero.z;
-        return __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, hi), __builtin_bit_cast(uint32_t, lo), 0x07060302u);
-    };
-    to.d[2 * half] = pair(w & 0x0f0f0f0fu), to.d[2 * half + 1] = pair((w >> 4) & 0x0f0f0f0fu);
-#endif
 }
-__device__ __forceinline__ v8t codes_of(uint32_t w, const Zero &zero, const Cutter &cut)
+
+// The operands of the kernel of few rows.  fp16: q - z.  bf16: 128 + q, the bits 0x4300 | nibble, 7 instructions (q - z by way of float32 takes 23, which bound that kernel), beside which a second matrix
+// instruction, of which it has plenty, takes -(128 + z); what is lost of the float32 sums is 2^-24 of 30 times their magnitude, a thousandth of an output's rounding (an infinity in X comes out as NaN).
+#if FP6MI_TYPE == 0
+struct FewCutter : Cutter { };
+struct FewZero : Zero { };
+__device__ __forceinline__ v8t codes_of(uint32_t w, const FewZero &zero, const FewCutter &cut)
 {
     Codes r;
     codes_half(r, w, zero, cut, 0);
     codes_half(r, w, zero, cut, 1);
     return r.v;
 }
+#else
+struct FewCutter {
+    uint32_t mask = 0x000f000fu, bits = 0x43004300u;
+    __device__ __forceinline__ FewCutter() { asm("" : "+s"(mask), "+v"(bits)); }
+};
+struct FewZero {
+    v8t all; // -(128 + z)
+    __device__ __forceinline__ void set(T zero)
+    {
+        const T z = (T)(-128.f - (float)zero);
+        all = (v8t){ z, z, z, z, z, z, z, z };
+    }
+};
+__device__ __forceinline__ v8t codes_of(uint32_t w, const FewZero &, const FewCutter &cut)
+{
+    union { uint32_t d[4]; v8t v; } r;
+#pragma unroll
+    for (int i = 0; i < 4; i++) r.d[i] = (w >> 4 * i & cut.mask) | cut.bits;
+    return r.v;
+}
+#endif
+
+#if FP6MI_TYPE == 0
+__device__ __forceinline__ v4f second(v8t, const FewZero &, v4f acc) { return acc; }
+#else
+__device__ __forceinline__ v4f second(v8t x, const FewZero &zero, v4f acc) { return mfma(x, zero.all, acc); }
+#endif
 
 // The scales (and zero points) of one row in one block.
 template <int GPB, bool Z> struct alignas(2 * GPB * (Z ? 2 : 1)) Scales { T v[GPB * (Z ? 2 : 1)]; };
@@ -158,7 +180,7 @@ template <int GPB, bool Z, int RT, int NT> struct Block {
     v8t            x[NT][4];
 };
 
-template <int GPB, bool Z, int RT, int NT, int WK> __global__ __launch_bounds__(WK * 64) void int4_stream(const Int4Args a)
+template <int GPB, bool Z, int RT, int NT, int WK> __global__ __launch_bounds__(WK * 64, WK > 4 ? 1 : 2) void int4_stream(const Int4Args a)
 {
     __shared__ v4f part[WK][RT * NT][64];
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, q = lane >> 4;
@@ -180,7 +202,7 @@ template <int GPB, bool Z, int RT, int NT, int WK> __global__ __launch_bounds__(
     for (int n = 0; n < NT; n++) x[n] = static_cast<const T *>(a.X) + (size_t)(t.row + (n * 16 + c < t.rows ? n * 16 + c : t.rows - 1)) * a.K + q * 8;
 
     typedef Block<GPB, Z, RT, NT> B;
-    const Cutter                  cut;
+    const FewCutter               cut;
     auto load = [&](B &b, uint32_t kb) __attribute__((always_inline)) {
         const uint32_t steps = (a.K - kb * 128) / 32; // of 32 columns, 4 but for the last block
 #pragma unroll
@@ -199,21 +221,38 @@ template <int GPB, bool Z, int RT, int NT, int WK> __global__ __launch_bounds__(
         for (int n = 0; n < NT; n++) sum[r][n] = (v4f){ 0.f, 0.f, 0.f, 0.f };
     auto multiply = [&](const B &b) __attribute__((always_inline)) {
         constexpr int kEach = 4 / GPB; // steps of a group
+        constexpr bool kSecond = FP6MI_TYPE == 1;
+        FewZero        zero;
+        zero.set((T)8.f);
+        v4f first[NT][GPB]; // what the second instruction gives where all rows share it
+        if constexpr (kSecond && !Z) {
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int g = 0; g < GPB; g++) {
+                    first[n][g] = (v4f){ 0.f, 0.f, 0.f, 0.f };
+#pragma unroll
+                    for (int i = 0; i < kEach; i++) first[n][g] = second(b.x[n][g * kEach + i], zero, first[n][g]);
+                }
+        }
 #pragma unroll
         for (int r = 0; r < RT; r++)
 #pragma unroll
             for (int g = 0; g < GPB; g++) {
                 const float scale = (float)b.s[r].v[Z ? 2 * g : g];
-                Zero        zero;
-                zero.set(Z ? b.s[r].v[2 * g + 1] : (T)8.f);
+                if constexpr (Z) zero.set(b.s[r].v[2 * g + 1]);
                 v8t v[kEach];
 #pragma unroll
                 for (int i = 0; i < kEach; i++) v[i] = codes_of(b.w[r][g * kEach + i], zero, cut);
 #pragma unroll
                 for (int n = 0; n < NT; n++) {
                     v4f y = { 0.f, 0.f, 0.f, 0.f };
+                    if constexpr (kSecond && !Z) y = first[n][g];
 #pragma unroll
-                    for (int i = 0; i < kEach; i++) y = mfma(b.x[n][g * kEach + i], v[i], y);
+                    for (int i = 0; i < kEach; i++) {
+                        if constexpr (kSecond && Z) y = second(b.x[n][g * kEach + i], zero, y);
+                        y = mfma(b.x[n][g * kEach + i], v[i], y);
+                    }
 #pragma unroll
                     for (int i = 0; i < 4; i++) sum[r][n][i] += scale * y[i];
                 }
@@ -283,6 +322,48 @@ template <int GPB, bool Z, int RT, int NT, int WK> int launch_stream(hipStream_t
     return (int)hipGetLastError();
 }
 
+#if FP6MI_TYPE == 1 && FP6MI_GROUPS == 1
+// Rows in bf16 as fp16 times a power of two for each row, which puts the largest finite magnitude from 2^14 to 2^15.  What is smaller than 2^-29 of that loses bits, at most 2^-40 of it: a float32 sum of such
+// products has been rounded by more.  Infinities and NaN stay.  A workgroup to a row, which reads it twice (from L2); 4096 rows of 4096 take 13 us.
+__global__ __launch_bounds__(256) void rows_to_halfs(half_t *__restrict__ out, int *__restrict__ exponents, const T *__restrict__ X, uint32_t K)
+{
+    __shared__ uint32_t most[4];
+    const uint32_t tid = threadIdx.x, pieces = K / 8;
+    const v4u     *x = reinterpret_cast<const v4u *>(X + (size_t)blockIdx.x * K);
+    uint32_t       top = 0; // exponent field and mantissa of the largest finite magnitude
+    auto           field = [](uint32_t b) { return b < 0x7f80u ? b : 0u; };
+    for (uint32_t i = tid; i < pieces; i += 256) {
+        const v4u v = x[i];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const uint32_t lo = field(v[j] & 0x7fffu), hi = field(v[j] >> 16 & 0x7fffu);
+            top = top > lo ? top : lo, top = top > hi ? top : hi;
+        }
+    }
+#pragma unroll
+    for (int m = 32; m; m >>= 1) {
+        const uint32_t o = __shfl_xor(top, m);
+        top = top > o ? top : o;
+    }
+    if ((tid & 63) == 0) most[tid >> 6] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 4; w++) top = top > most[w] ? top : most[w];
+    const int e = top ? (int)(top >> 7 > 1 ? top >> 7 : 1) - 127 - 14 : 0;
+    if (tid == 0) exponents[blockIdx.x] = e;
+    for (uint32_t i = tid; i < pieces; i += 256) {
+        const v4u v = x[i];
+        v8h       h;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            h[2 * j] = (half_t)__builtin_ldexpf(__builtin_bit_cast(float, v[j] << 16), -e);
+            h[2 * j + 1] = (half_t)__builtin_ldexpf(__builtin_bit_cast(float, v[j] & 0xffff0000u), -e);
+        }
+        reinterpret_cast<v8h *>(out + (size_t)blockIdx.x * K)[i] = h;
+    }
+}
+#endif
+
 // ---------------------------------------------------------------------------------------------------------------
 // More rows: tiles of WR * 64 weight rows x NT * 16 rows of X to a workgroup of WR x WK wavefronts; the WK groups take every WK-th column block.  X goes to LDS by direct transfers, a K block ahead, two
 // stages to a group; a row of a stage is 256 bytes whose 16 pieces stand in the order piece ^ (row & 15), which gives the reads of an MFMA operand all banks.  A wavefront holds its X of one block in
@@ -313,22 +394,24 @@ template <int GPB, bool Z, int NT, int WR, int WK> __global__ __launch_bounds__(
 
     // transfers of X: four rows of one block each
     typedef __attribute__((address_space(3))) void lvoid;
-    const auto     xbuf = __builtin_amdgcn_make_buffer_rsrc(const_cast<T *>(static_cast<const T *>(a.X) + (size_t)t.row * a.K), 0, (int)(t.rows * a.K * 2), 0x00027000);
+    const auto     xbuf = __builtin_amdgcn_make_buffer_rsrc(const_cast<half_t *>(static_cast<const half_t *>(a.X) + (size_t)t.row * a.K), 0, (int)(t.rows * a.K * 2), 0x00027000);
     uint8_t *const xstage = lds + wk * 2 * kStage;
-    const uint32_t xpiece = c ^ q, xlast = (t.rows - 1) * a.K * 2; // 32 bits: the launcher bounds K
+    const uint32_t xrow0 = (4 * wr + q) * a.K * 2, xlast = (t.rows - 1) * a.K * 2; // 32 bits: the launcher bounds K
     auto           transfer = [&](uint32_t kb, uint32_t stage) __attribute__((always_inline)) {
 #pragma unroll
         for (uint32_t j = 0; j < kDma; j++) {
-            const uint32_t row4 = j * WR + wr, row = (row4 * 4 + q) * a.K * 2, k = kb * 128 + (xpiece ^ 4 * (row4 & 3)) * 8;
-            const uint32_t off = (row < xlast ? row : xlast) + (k < a.K ? k * 2 : 0xc0000000u); // (beyond the buffer, which reads as zeros)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(xbuf, (lvoid *)(xstage + stage * kStage + row4 * 1024), 16, off, 0, 0, 0);
+            uint32_t row = xrow0, piece = c ^ q;
+            if constexpr (kDma > 4) asm("" : "+v"(row), "+v"(piece)); // (each address for itself when it is needed: kept, they take the registers of a tile)
+            row += j * WR * 8 * a.K, piece ^= 4 * ((j * WR + wr) & 3);
+            const uint32_t k = kb * 128 + piece * 8, off = (row < xlast ? row : xlast) + (k < a.K ? k * 2 : 0xc0000000u); // (beyond the buffer, which reads as zeros)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(xbuf, (lvoid *)(xstage + stage * kStage + (j * WR + wr) * 1024), 16, off, 0, 0, 0);
         }
     };
     // operands of X: of the first two tiles of the next block while this one's are still in use, of the others in their place
     const uint8_t *xread = xstage + c * 256;
-    v8t            early[2][2][4], late[NT > 2 ? NT - 2 : 1][4];
-    auto           read_x = [&](v8t &to, int n, uint32_t i, uint32_t stage) __attribute__((always_inline)) {
-        to = *reinterpret_cast<const v8t *>(xread + stage * kStage + n * 16 * 256 + ((4 * i + q) ^ c) * 16);
+    v8h            early[2][2][4], late[NT > 2 ? NT - 2 : 1][4];
+    auto           read_x = [&](v8h &to, int n, uint32_t i, uint32_t stage) __attribute__((always_inline)) {
+        to = *reinterpret_cast<const v8h *>(xread + stage * kStage + n * 16 * 256 + ((4 * i + q) ^ c) * 16);
     };
 
     // codes and scales, by scalar offsets from the wavefront's first row tile (row tiles beyond the last one take it again); a row tile's are asked for again as soon as they are converted
@@ -402,7 +485,7 @@ template <int GPB, bool Z, int NT, int WR, int WK> __global__ __launch_bounds__(
             const int v = u * GPB + i / kEach;
 #pragma unroll
             for (int k = 0; k < 2; k++)
-                y[v & 1][k] = mfma(n == 0 ? early[set][k][i] : late[n == 0 ? 0 : n - 2 + k][i], op[r & 1][i].v, i % kEach == 0 ? (v4f){ 0.f, 0.f, 0.f, 0.f } : y[v & 1][k]);
+                y[v & 1][k] = mfma_halfs(n == 0 ? early[set][k][i] : late[n == 0 ? 0 : n - 2 + k][i], op[r & 1][i].v, i % kEach == 0 ? (v4f){ 0.f, 0.f, 0.f, 0.f } : y[v & 1][k]);
             if constexpr (GPB == 1) {
                 if (i == 1 || i == 2) add(pr, pn, 0, v + 1, i - 1, i);
             } else if constexpr (GPB == 2) {
@@ -474,6 +557,8 @@ template <int GPB, bool Z, int NT, int WR, int WK> __global__ __launch_bounds__(
     }
 
     // outputs through LDS, so that a lane stores 16 bytes: [row of X][weight row], rows 16 bytes apart from a multiple of 128
+    auto     exponent = [&](uint32_t n, uint32_t i) { return FP6MI_TYPE == 1 && n * 16 + 4 * q + i < t.rows ? a.exponents[t.row + n * 16 + 4 * q + i] : 0; };
+    auto     scaled = [&](float v, int e) { return FP6MI_TYPE == 1 ? __builtin_ldexpf(v, e) : v; };
     const T *bias = a.bias ? static_cast<const T *>(a.bias) + (size_t)t.expert * a.Mt * 16 : nullptr;
     auto     out = [&](auto type, auto gated_c) __attribute__((always_inline)) {
         typedef decltype(type) O;
@@ -494,8 +579,9 @@ template <int GPB, bool Z, int NT, int WR, int WK> __global__ __launch_bounds__(
                         const float    b0 = in ? (float)bias[m] : 0.f, b1 = gated && in ? (float)bias[m + 16] : 0.f;
 #pragma unroll
                         for (uint32_t i = 0; i < 4; i++) {
-                            float v = sum[r][n][i] + b0;
-                            if constexpr (gated) v = activated(a.act, v) * (sum[r + 1][n][i] + b1);
+                            const int e = exponent(n, i);
+                            float     v = scaled(sum[r][n][i], e) + b0;
+                            if constexpr (gated) v = activated(a.act, v) * (scaled(sum[r + 1][n][i], e) + b1);
                             reinterpret_cast<O *>(lds + (row + i) * kPitch)[gated ? (wr * RT + r) * 8 + c : (wr * RT + r) * 16 + c] = (O)v;
                         }
                     }
@@ -532,25 +618,38 @@ template <int GPB, bool Z, int NT, int WR, int WK> int launch_tile(hipStream_t s
     return (int)hipGetLastError();
 }
 
-template <int GPB, bool Z> int run(hipStream_t st, const Int4Args &a)
+template <int GPB, bool Z> int run(hipStream_t st, const Int4Args &a, int kernel)
 {
-    if (a.N <= 16 || (a.offsets && a.N <= 16 * a.E)) return launch_stream<GPB, Z, 2, 1, 8>(st, a);
-    if (a.N <= 32 || (a.offsets && a.N <= 32 * a.E)) return launch_tile<GPB, Z, 2, 1, 4>(st, a);
-    return launch_tile<GPB, Z, 4, 4, 1>(st, a);
+    switch (kernel) { // (in the order of fp6mi::kInt4Kernels)
+    case 0: return launch_stream<GPB, Z, 1, 1, 16>(st, a);
+    case 1: return launch_stream<GPB, Z, 2, 1, 8>(st, a);
+    case 2: return launch_stream<GPB, Z, 4, 1, 8>(st, a);
+    case 3: return launch_stream<GPB, Z, 4, 1, 4>(st, a);
+    case 4: return launch_tile<GPB, Z, 2, 1, 4>(st, a);
+    case 5: return launch_tile<GPB, Z, 2, 2, 4>(st, a);
+    case 6: return launch_tile<GPB, Z, 2, 2, 2>(st, a);
+    case 7: return launch_tile<GPB, Z, 4, 2, 2>(st, a);
+    case 8: return launch_tile<GPB, Z, 4, 4, 1>(st, a);
+    }
+    return FP6MI_ERR_SHAPE;
 }
 
 } // namespace
 
+#define FP6MI_NAME2(type, groups) int4_run_##type##_##groups
+#define FP6MI_NAME(type, groups) FP6MI_NAME2(type, groups)
 namespace fp6mi {
-#if FP6MI_TYPE == 0
-int int4_run_f16(void *stream, const Int4Args &a, int group, bool zeros)
-#else
-int int4_run_bf16(void *stream, const Int4Args &a, int group, bool zeros)
-#endif
+int FP6MI_NAME(FP6MI_TYPE, FP6MI_GROUPS)(void *stream, const Int4Args &a, bool zeros, int kernel)
 {
     hipStream_t st = static_cast<hipStream_t>(stream);
-    if (group == 128) return zeros ? run<1, true>(st, a) : run<1, false>(st, a);
-    if (group == 64) return zeros ? run<2, true>(st, a) : run<2, false>(st, a);
-    return zeros ? run<4, true>(st, a) : run<4, false>(st, a);
+    return zeros ? run<FP6MI_GROUPS, true>(st, a, kernel) : run<FP6MI_GROUPS, false>(st, a, kernel);
 }
+
+#if FP6MI_TYPE == 1 && FP6MI_GROUPS == 1
+int int4_rows_to_halfs(void *stream, void *out, int *exponents, const void *X, size_t N, size_t K)
+{
+    hipLaunchKernelGGL(rows_to_halfs, dim3((uint32_t)N), dim3(256), 0, static_cast<hipStream_t>(stream), static_cast<half_t *>(out), exponents, static_cast<const T *>(X), (uint32_t)K);
+    return (int)hipGetLastError();
+}
+#endif
 } // namespace fp6mi

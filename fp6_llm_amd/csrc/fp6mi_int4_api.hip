@@ -67,6 +67,19 @@ int check_pack(const void *native, const void *native_scales, const void *codes,
     return aligned(native, 16) && aligned(native_scales, 16) && aligned(scales, 2) ? FP6MI_OK : FP6MI_ERR_ALIGN;
 }
 
+// Which kernel takes a product (an index of kInt4Kernels).
+int choice(size_t experts, bool grouped, size_t M, size_t N, size_t K)
+{
+    (void)M;
+    if (K > (size_t)1 << 20) return 1; // (the tiles' offsets have 32 bits)
+    const size_t each = grouped ? N / experts : N;
+    return each <= 16 ? 1 : each <= 32 ? 4 : 8;
+}
+
+// Scratch of a product by kernel `kernel`: of bf16 tiles the rows of X as halfs, behind their exponents.
+size_t round16(size_t n) { return (n + 15) / 16 * 16; }
+size_t scratch_bytes(int dtype, int kernel, size_t N, size_t K) { return dtype == 1 && fp6mi::kInt4Kernels[kernel].tile ? round16(N * sizeof(int)) + N * K * 2 : 0; }
+
 } // namespace
 
 extern "C" {
@@ -106,8 +119,24 @@ int fp6mi_int4_pack_gpu(void *stream, void *native, void *native_scales, const v
     return (int)hipGetLastError();
 }
 
+size_t fp6mi_int4_workspace_bytes(int dtype, size_t experts, int grouped, size_t M, size_t N, size_t K)
+{
+    if ((dtype != 0 && dtype != 1) || check_shape(experts, M, K) || N == 0 || N > (size_t)1 << 30) return 0;
+    return scratch_bytes(dtype, choice(experts, grouped != 0, M, N, K), N, K);
+}
+
+int fp6mi_int4_query_kernel(size_t experts, int grouped, size_t M, size_t N, size_t K, int *shape)
+{
+    if (check_shape(experts, M, K) || N == 0 || N > (size_t)1 << 30) return FP6MI_ERR_SHAPE;
+    if (!shape) return FP6MI_ERR_NULL;
+    const int               k = choice(experts, grouped != 0, M, N, K);
+    const fp6mi::Int4Kernel &c = fp6mi::kInt4Kernels[k];
+    shape[0] = c.tile, shape[1] = c.cols, shape[2] = c.row_tiles, shape[3] = c.k_split;
+    return FP6MI_OK;
+}
+
 int fp6mi_int4_linear(void *stream, int dtype, const void *W_native, const void *scales_native, int group, int zeros, const void *bias, const void *X, void *Y, int out_f32, int activation,
-                      const int *offsets, size_t experts, size_t M, size_t N, size_t K)
+                      const int *offsets, size_t experts, size_t M, size_t N, size_t K, void *workspace)
 {
     if (dtype != 0 && dtype != 1) return FP6MI_ERR_TYPE;
     if (const int e = check_shape(experts, M, K)) return e;
@@ -116,9 +145,18 @@ int fp6mi_int4_linear(void *stream, int dtype, const void *W_native, const void 
     if (activation >= 0 && M % 32) return FP6MI_ERR_SHAPE;
     if (N == 0) return FP6MI_OK;
     if (!W_native || !scales_native || !X || !Y) return FP6MI_ERR_NULL;
-    if (!aligned(W_native, 16) || !aligned(scales_native, 16) || !aligned(X, 16) || !aligned(Y, 16) || !aligned(bias, 2) || !aligned(offsets, 4)) return FP6MI_ERR_ALIGN;
-    const fp6mi::Int4Args a = { W_native, scales_native, X, bias, Y, offsets, (uint32_t)N, (uint32_t)K, (uint32_t)((K + 127) / 128), (uint32_t)(M / 16), (uint32_t)experts, activation, out_f32 };
-    return dtype ? fp6mi::int4_run_bf16(stream, a, group, zeros != 0) : fp6mi::int4_run_f16(stream, a, group, zeros != 0);
+    if (!aligned(W_native, 16) || !aligned(scales_native, 16) || !aligned(X, 16) || !aligned(Y, 16) || !aligned(bias, 2) || !aligned(offsets, 4) || !aligned(workspace, 16)) return FP6MI_ERR_ALIGN;
+    const int       kernel = choice(experts, offsets != nullptr, M, N, K);
+    fp6mi::Int4Args a = { W_native, scales_native, X, bias, Y, offsets, (uint32_t)N, (uint32_t)K, (uint32_t)((K + 127) / 128), (uint32_t)(M / 16), (uint32_t)experts, activation, out_f32, nullptr };
+    if (scratch_bytes(dtype, kernel, N, K)) {
+        if (!workspace) return FP6MI_ERR_WORKSPACE;
+        int  *exponents = static_cast<int *>(workspace);
+        void *halfs = static_cast<uint8_t *>(workspace) + round16(N * sizeof(int));
+        if (const int e = fp6mi::int4_rows_to_halfs(stream, halfs, exponents, X, N, K)) return e;
+        a.X = halfs, a.exponents = exponents;
+    }
+    if (dtype == 0) return group == 128 ? fp6mi::int4_run_0_1(stream, a, zeros != 0, kernel) : group == 64 ? fp6mi::int4_run_0_2(stream, a, zeros != 0, kernel) : fp6mi::int4_run_0_4(stream, a, zeros != 0, kernel);
+    return group == 128 ? fp6mi::int4_run_1_1(stream, a, zeros != 0, kernel) : group == 64 ? fp6mi::int4_run_1_2(stream, a, zeros != 0, kernel) : fp6mi::int4_run_1_4(stream, a, zeros != 0, kernel);
 }
 
 } // extern "C"

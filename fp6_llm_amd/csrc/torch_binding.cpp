@@ -583,8 +583,8 @@ PlanArgs plan_args(const at::Tensor &table, int64_t experts, int64_t places)
     return { p + experts, p + experts + 1 + places, p, p + experts + 1 };
 }
 
-at::Tensor int4_forward(const at::Tensor &in_feats, const at::Tensor &native, const at::Tensor &s, const OptTensor &plan, int64_t experts, int64_t places, int64_t act, const OptTensor &bias, const OptTensor &out_opt,
-                        bool f32)
+at::Tensor int4_forward(const at::Tensor &in_feats, const at::Tensor &native, const at::Tensor &s, const OptTensor &plan, int64_t experts, int64_t places, int64_t act, const OptTensor &bias,
+                        const OptTensor &out_opt, bool f32, const OptTensor &ws_opt)
 {
     const bool         grouped = plan.has_value();
     const int64_t      dims = grouped ? 6 : 5;
@@ -620,8 +620,11 @@ at::Tensor int4_forward(const at::Tensor &in_feats, const at::Tensor &native, co
     } else {
         out = at::empty({ B, cols }, at::TensorOptions().dtype(to).device(dev));
     }
-    raise_status(fp6mi_int4_linear(c10::hip::getCurrentHIPStream(dev.index()).stream(), type_code(type), native.data_ptr(), s.data_ptr(), 128 / (int)s.size(-2), (int)s.size(-1) - 1, pointer(bias),
-                                   x.data_ptr(), out.data_ptr(), f32, (int)act, offsets, (size_t)E, (size_t)OC, (size_t)B, (size_t)IC),
+    void      *stream = c10::hip::getCurrentHIPStream(dev.index()).stream();
+    at::Tensor keep;
+    float     *ws = type == at::kHalf ? nullptr : scratch(ws_opt, dev, stream, fp6mi_int4_workspace_bytes(1, (size_t)E, grouped, (size_t)OC, (size_t)B, (size_t)IC), keep);
+    raise_status(fp6mi_int4_linear(stream, type_code(type), native.data_ptr(), s.data_ptr(), 128 / (int)s.size(-2), (int)s.size(-1) - 1, pointer(bias), x.data_ptr(), out.data_ptr(), f32, (int)act, offsets,
+                                   (size_t)E, (size_t)OC, (size_t)B, (size_t)IC, ws),
                  "fp6mi_int4_linear");
     return out;
 }

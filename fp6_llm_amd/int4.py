@@ -66,11 +66,11 @@ def int4_pack_native(codes, scales, zeros=None, group=128):
     return w, s
 
 
-def int4_forward_native(in_feats, native_weight, native_scales, plan=None, activation=None, bias=None, out=None, out_dtype=None):
+def int4_forward_native(in_feats, native_weight, native_scales, plan=None, activation=None, bias=None, out=None, out_dtype=None, workspace=None):
     """out[B, OC] = in_feats[B, IC] @ w^T (+ bias[OC]) with the weights of int4_pack_native.  activation ("silu", "gelu", "gelu_tanh"): out[B, OC/2] = act(gate) * up, for weights (and bias) whose
     rows are in pair order (16 rows of gate, the same 16 of up, and so on: gate_up_pairs).
     plan: that of expert_sort or expert_plan, for the weights of experts [E, ...] (bias [E, OC]): rows sorted by expert, each multiplied with its expert's weights; rows behind those come out as zeros.
-    in_feats has the scales' type, out too or (out_dtype) float32.  Not part of an autograd graph."""
+    in_feats has the scales' type, out too or (out_dtype) float32.  workspace: float32, of fp6mi_int4_workspace_bytes (many bfloat16 rows need one).  Not part of an autograd graph."""
     from . import _ext
     act = -1 if activation is None else ops._activation_code(activation)
     f32 = out_dtype == torch.float32
@@ -78,8 +78,8 @@ def int4_forward_native(in_feats, native_weight, native_scales, plan=None, activ
         raise ValueError("out_dtype must be float32 or the scales' type")
     if _ext is not None:
         if plan is None:
-            return _ext.int4_forward(in_feats, native_weight, native_scales, None, 0, 0, act, bias, out, f32)
-        return _ext.int4_forward(in_feats, native_weight, native_scales, plan.table, plan.experts, plan.places, act, bias, out, f32)
+            return _ext.int4_forward(in_feats, native_weight, native_scales, None, 0, 0, act, bias, out, f32, workspace)
+        return _ext.int4_forward(in_feats, native_weight, native_scales, plan.table, plan.experts, plan.places, act, bias, out, f32, workspace)
     s = native_scales
     dims = 6 if plan is not None else 5
     if s.dtype not in TYPES or s.dim() != dims or s.shape[-3] != 16 or s.shape[-2] not in (1, 2, 4) or s.shape[-1] not in (1, 2) or not s.is_contiguous():
@@ -107,6 +107,6 @@ def int4_forward_native(in_feats, native_weight, native_scales, plan=None, activ
     x = x.contiguous()
     out = ops._result(out, (B, OC // 2 if act >= 0 else OC), dev, dtype=torch.float32 if f32 else s.dtype)
     L = _lib.lib()
-    ops._launch("fp6mi_int4_linear", dev, 0, None, lambda stream, ws: L.fp6mi_int4_linear(
-        stream, TYPES[s.dtype], native_weight.data_ptr(), s.data_ptr(), 128 // s.shape[-2], s.shape[-1] - 1, ops._ptr(bias), x.data_ptr(), out.data_ptr(), f32, act, offsets, E, OC, B, IC))
+    ops._launch("fp6mi_int4_linear", dev, L.fp6mi_int4_workspace_bytes(TYPES[s.dtype], E, plan is not None, OC, B, IC), workspace, lambda stream, ws: L.fp6mi_int4_linear(
+        stream, TYPES[s.dtype], native_weight.data_ptr(), s.data_ptr(), 128 // s.shape[-2], s.shape[-1] - 1, ops._ptr(bias), x.data_ptr(), out.data_ptr(), f32, act, offsets, E, OC, B, IC, ws))
     return out

@@ -296,8 +296,8 @@ def test_refusals_of_the_c_abi():
     assert L.fp6mi_int4_weight_bytes(1, 24, 64) == 0 and L.fp6mi_int4_weight_bytes(1, 16, 48) == 0 and L.fp6mi_int4_weight_bytes(0, 16, 64) == 0 and L.fp6mi_int4_weight_bytes(3, 32, 160) == 3 * 2 * 2 * 1024
     assert L.fp6mi_int4_scale_bytes(1, 16, 64, 40, 0) == 0 and L.fp6mi_int4_scale_bytes(2, 16, 160, 96, 1) == 2 * 16 * 2 * 4 * 4
 
-    def linear(dtype=0, W=p, S=p, group=64, zeros=0, bias=None, X=p, Y=p, f32=0, act=-1, offsets=None, E=1, M=32, N=2, K=64):
-        return L.fp6mi_int4_linear(None, dtype, W, S, group, zeros, bias, X, Y, f32, act, offsets, E, M, N, K)
+    def linear(dtype=0, W=p, S=p, group=64, zeros=0, bias=None, X=p, Y=p, f32=0, act=-1, offsets=None, E=1, M=32, N=2, K=64, ws=None):
+        return L.fp6mi_int4_linear(None, dtype, W, S, group, zeros, bias, X, Y, f32, act, offsets, E, M, N, K, ws)
     assert linear(dtype=2) == TYPE and linear(dtype=-1) == TYPE
     for bad in (dict(group=96), dict(group=0), dict(M=24), dict(M=0), dict(K=48), dict(K=0), dict(E=2), dict(E=0), dict(E=2000, offsets=p), dict(act=0, M=48), dict(N=(1 << 30) + 1), dict(M=1 << 25), dict(K=1 << 25)):
         assert linear(**bad) == SHAPE, bad
@@ -305,7 +305,8 @@ def test_refusals_of_the_c_abi():
     for name in ("W", "S", "X", "Y"):
         assert linear(**{name: None}) == NULL and linear(**{name: p + 8}) == ALIGN
     assert linear(bias=p + 1) == ALIGN and linear(offsets=p + 2) == ALIGN
-    assert linear(N=0, X=None, Y=None) == 0
+    assert linear(N=0, X=None, Y=None) == 0 and linear(dtype=1, N=500) == -4 and linear(ws=p + 8) == ALIGN
+    assert L.fp6mi_int4_workspace_bytes(0, 1, 0, 32, 500, 64) == 0 and L.fp6mi_int4_workspace_bytes(1, 1, 0, 32, 500, 64) == 2000 + 500 * 128 and L.fp6mi_int4_workspace_bytes(1, 1, 0, 32, 1, 64) == 0
     assert L.fp6mi_int4_pack(p, p, p, p, None, 2, 1, 16, 64, 64) == TYPE and L.fp6mi_int4_pack(p, p, p, None, None, 0, 1, 16, 64, 64) == NULL
     assert L.fp6mi_int4_pack_gpu(None, p, p, p, p, None, 0, 1, 16, 64, 33) == SHAPE and L.fp6mi_int4_pack_gpu(None, p + 4, p, p, p, None, 0, 1, 16, 64, 64) == ALIGN
 
