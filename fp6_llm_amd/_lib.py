@@ -77,8 +77,9 @@ def lib():
         "fp6mi_int4_pack": (ci, [vp, vp, vp, vp, vp, ci, sz, sz, sz, sz]),
         "fp6mi_int4_pack_gpu": (ci, [vp, vp, vp, vp, vp, vp, ci, sz, sz, sz, sz]),
         "fp6mi_int4_linear": (ci, [vp, ci, vp, vp, ci, ci, vp, vp, vp, ci, ci, vp, sz, sz, sz, sz, vp]),
-        "fp6mi_int4_workspace_bytes": (sz, [ci, sz, ci, sz, sz, sz]),
-        "fp6mi_int4_query_kernel": (ci, [sz, ci, sz, sz, sz, ctypes.POINTER(ci)]),
+        "fp6mi_int4_workspace_bytes": (sz, [ci, sz, ci, sz, sz, sz, ci, ci]),
+        "fp6mi_int4_linear_cfg": (ci, [vp, ci, vp, vp, ci, ci, vp, vp, vp, ci, ci, vp, sz, sz, sz, sz, vp, ci]),
+        "fp6mi_int4_query_kernel": (ci, [ci, sz, ci, sz, sz, sz, ci, ctypes.POINTER(ci)]),
         "fp6mi_expert_sort_workspace_bytes": (sz, [sz, sz, sz]),
         "fp6mi_expert_sort": (ci, [vp, vp, ci, vp, vp, vp, vp, sz, vp, sz, sz, sz, sz, ci, vp]),
         "fp6mi_expert_combine": (ci, [vp, vp, vp, vp, vp, vp, sz, sz, sz, ci, ci]),
@@ -102,7 +103,7 @@ EXPORTED = ["fp6mi_error_string", "fp6mi_version", "fp6mi_tuning_info", "fp6mi_p
             "fp6mi_dequant_native_grouped_gpu", "fp6mi_quantize_native_grouped_gpu",
             "fp6mi_linear_grad_native", "fp6mi_query_grad_launch", "fp6mi_heuristic_grad_splits", "fp6mi_grad_workspace_bytes", "fp6mi_gated_native", "fp6mi_gated_workspace_bytes", "fp6mi_query_gated_launch",
             "fp6mi_gated_backward_native", "fp6mi_gated_backward_workspace_bytes", "fp6mi_adapter_native", "fp6mi_adapter_workspace_bytes",
-            "fp6mi_int4_weight_bytes", "fp6mi_int4_scale_bytes", "fp6mi_int4_pack", "fp6mi_int4_pack_gpu", "fp6mi_int4_linear", "fp6mi_int4_workspace_bytes", "fp6mi_int4_query_kernel",
+            "fp6mi_int4_weight_bytes", "fp6mi_int4_scale_bytes", "fp6mi_int4_pack", "fp6mi_int4_pack_gpu", "fp6mi_int4_linear", "fp6mi_int4_linear_cfg", "fp6mi_int4_workspace_bytes", "fp6mi_int4_query_kernel",
             "fp6mi_expert_sort_workspace_bytes", "fp6mi_expert_sort", "fp6mi_expert_combine", "fp6mi_expert_combine_backward"]
 
 

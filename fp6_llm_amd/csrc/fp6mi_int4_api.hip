@@ -1,6 +1,9 @@
 // Layout and C ABI of the products with 4-bit integer weights (fp6mi_int4.hip; include/fp6mi.h).  No counterpart in the reference.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+#include <cmath>
+
 #include "fp6mi_internal.h"
 #include "fp6mi_int4.inc"
 
@@ -67,18 +70,47 @@ int check_pack(const void *native, const void *native_scales, const void *codes,
     return aligned(native, 16) && aligned(native_scales, 16) && aligned(scales, 2) ? FP6MI_OK : FP6MI_ERR_ALIGN;
 }
 
-// Which kernel takes a product (an index of kInt4Kernels).
-int choice(size_t experts, bool grouped, size_t M, size_t N, size_t K)
+// Which kernel takes a product (an index of kInt4Kernels): the fastest by this model of its time, us.  A workgroup's column blocks one after another take `step` each while every CU has one at the most,
+// `share` times the workgroups of a CU beyond, which come in rounds of as many as fit; and no kernel reads the weights faster than memory.  Rows of experts are taken to be spread evenly, with half a tile
+// to spare for each expert.  Fitted to 720 times (2048x8192 to 28672x8192 at 1 to 777 rows, 8 to 128 experts at 1 to 700 tokens, fp16 and bf16), off by 8 to 20 % rms for a kernel; the choice takes 1.03 times
+// the fastest measured in the mean, at worst 1.3.
+struct Times { double base, step, share, rows; int fit; }; // rows: how much longer a step takes with 16 rows than with none, of the kernel that streams weights
+constexpr Times kTimes[] = { { 5.5, 0.94, 0.94, 0.99, 2 }, { 3.9, 0.80, 0.88, 0.26, 2 }, { 2.6, 1.37, 2.00, 0, 1 }, { 2.5, 0.74, 0.65, 0.13, 3 }, { 5.9, 0.81, 0.90, 0, 2 }, { 6.2, 1.15, 1.75, 0, 1 },
+                             { 5.3, 0.79, 0.72, 0, 2 }, { 8.1, 0.92, 1.14, 0, 2 },    { 8.2, 0.83, 1.01, 0, 2 } };
+
+constexpr int    kKernels = sizeof(kTimes) / sizeof(kTimes[0]);
+constexpr size_t kMostTileColumns = (size_t)1 << 20; // (offsets in a tile have 32 bits)
+
+double time_of(int kernel, int dtype, size_t experts, bool grouped, size_t M, size_t N, size_t K)
 {
-    (void)M;
-    if (K > (size_t)1 << 20) return 1; // (the tiles' offsets have 32 bits)
-    const size_t each = grouped ? N / experts : N;
-    return each <= 16 ? 1 : each <= 32 ? 4 : 8;
+    const fp6mi::Int4Kernel &k = fp6mi::kInt4Kernels[kernel];
+    const Times             &t = kTimes[kernel];
+    const double used = grouped ? experts * (1 - std::exp(-(double)N / experts)) : 1.0, tiles = grouped ? std::max(used, (double)N / k.cols + 0.5 * used) : (double)((N + k.cols - 1) / k.cols);
+    const double load = (double)((M / 16 + k.row_tiles - 1) / k.row_tiles) * tiles / 256, steps = (double)(((K + 127) / 128 + k.k_split - 1) / k.k_split);
+    const double more = 1 + t.rows * std::min(16.0, (double)N / used) / 16;
+    const double among = load <= 1 ? load : (load + t.fit * std::ceil(load / t.fit)) / 2;
+    double       us = t.base + steps * more * std::max(t.step, t.share * among);
+    if (dtype == 1 && k.tile) us += 3 + (double)N * K * 4 / 4.0e6; // (the rows on their way to fp16)
+    return std::max(us, used * M * K * 0.515 / 5.1e6 + 1.5);
+}
+
+int choice(int dtype, size_t experts, bool grouped, size_t M, size_t N, size_t K, bool gated)
+{
+    int       best = -1;
+    double    least = 0;
+    for (int k = 0; k < kKernels; k++) {
+        if ((fp6mi::kInt4Kernels[k].tile && K > kMostTileColumns) || (gated && fp6mi::kInt4Kernels[k].row_tiles % 2)) continue; // (gate and up are two row tiles)
+        const size_t tiles = fp6mi::int4_tiles(N, grouped ? experts : 0, fp6mi::kInt4Kernels[k].cols);
+        if (!fp6mi::kInt4Kernels[k].tile && tiles > 65535) continue; // (a grid dimension)
+        const double us = time_of(k, dtype, experts, grouped, M, N, K);
+        if (best < 0 || us < least) best = k, least = us;
+    }
+    return best;
 }
 
 // Scratch of a product by kernel `kernel`: of bf16 tiles the rows of X as halfs, behind their exponents.
 size_t round16(size_t n) { return (n + 15) / 16 * 16; }
-size_t scratch_bytes(int dtype, int kernel, size_t N, size_t K) { return dtype == 1 && fp6mi::kInt4Kernels[kernel].tile ? round16(N * sizeof(int)) + N * K * 2 : 0; }
+size_t scratch_bytes(int dtype, int kernel, size_t N, size_t K) { return dtype == 1 && kernel >= 0 && fp6mi::kInt4Kernels[kernel].tile ? round16(N * sizeof(int)) + N * K * 2 : 0; }
 
 } // namespace
 
@@ -119,34 +151,36 @@ int fp6mi_int4_pack_gpu(void *stream, void *native, void *native_scales, const v
     return (int)hipGetLastError();
 }
 
-size_t fp6mi_int4_workspace_bytes(int dtype, size_t experts, int grouped, size_t M, size_t N, size_t K)
+size_t fp6mi_int4_workspace_bytes(int dtype, size_t experts, int grouped, size_t M, size_t N, size_t K, int gated, int kernel)
 {
-    if ((dtype != 0 && dtype != 1) || check_shape(experts, M, K) || N == 0 || N > (size_t)1 << 30) return 0;
-    return scratch_bytes(dtype, choice(experts, grouped != 0, M, N, K), N, K);
+    if ((dtype != 0 && dtype != 1) || check_shape(experts, M, K) || N == 0 || N > (size_t)1 << 30 || kernel >= kKernels) return 0;
+    return scratch_bytes(dtype, kernel >= 0 ? kernel : choice(dtype, experts, grouped != 0, M, N, K, gated != 0), N, K);
 }
 
-int fp6mi_int4_query_kernel(size_t experts, int grouped, size_t M, size_t N, size_t K, int *shape)
+int fp6mi_int4_query_kernel(int dtype, size_t experts, int grouped, size_t M, size_t N, size_t K, int gated, int *shape)
 {
+    if (dtype != 0 && dtype != 1) return FP6MI_ERR_TYPE;
     if (check_shape(experts, M, K) || N == 0 || N > (size_t)1 << 30) return FP6MI_ERR_SHAPE;
-    if (!shape) return FP6MI_ERR_NULL;
-    const int               k = choice(experts, grouped != 0, M, N, K);
+    const int k = choice(dtype, experts, grouped != 0, M, N, K, gated != 0);
+    if (k < 0) return FP6MI_ERR_SHAPE;
     const fp6mi::Int4Kernel &c = fp6mi::kInt4Kernels[k];
-    shape[0] = c.tile, shape[1] = c.cols, shape[2] = c.row_tiles, shape[3] = c.k_split;
-    return FP6MI_OK;
+    if (shape) shape[0] = c.tile, shape[1] = c.cols, shape[2] = c.row_tiles, shape[3] = c.k_split;
+    return k;
 }
 
-int fp6mi_int4_linear(void *stream, int dtype, const void *W_native, const void *scales_native, int group, int zeros, const void *bias, const void *X, void *Y, int out_f32, int activation,
-                      const int *offsets, size_t experts, size_t M, size_t N, size_t K, void *workspace)
+int fp6mi_int4_linear_cfg(void *stream, int dtype, const void *W_native, const void *scales_native, int group, int zeros, const void *bias, const void *X, void *Y, int out_f32, int activation,
+                          const int *offsets, size_t experts, size_t M, size_t N, size_t K, void *workspace, int kernel)
 {
     if (dtype != 0 && dtype != 1) return FP6MI_ERR_TYPE;
     if (const int e = check_shape(experts, M, K)) return e;
-    if ((group != 32 && group != 64 && group != 128) || N > (size_t)1 << 30 || (!offsets && experts != 1)) return FP6MI_ERR_SHAPE;
+    if ((group != 32 && group != 64 && group != 128) || N > (size_t)1 << 30 || (!offsets && experts != 1) || kernel >= kKernels) return FP6MI_ERR_SHAPE;
     if (activation > FP6MI_ACT_GELU_TANH) return FP6MI_ERR_ACTIVATION;
     if (activation >= 0 && M % 32) return FP6MI_ERR_SHAPE;
     if (N == 0) return FP6MI_OK;
     if (!W_native || !scales_native || !X || !Y) return FP6MI_ERR_NULL;
     if (!aligned(W_native, 16) || !aligned(scales_native, 16) || !aligned(X, 16) || !aligned(Y, 16) || !aligned(bias, 2) || !aligned(offsets, 4) || !aligned(workspace, 16)) return FP6MI_ERR_ALIGN;
-    const int       kernel = choice(experts, offsets != nullptr, M, N, K);
+    if (kernel < 0) kernel = choice(dtype, experts, offsets != nullptr, M, N, K, activation >= 0);
+    if (kernel < 0 || (activation >= 0 && fp6mi::kInt4Kernels[kernel].row_tiles % 2) || (fp6mi::kInt4Kernels[kernel].tile && K > kMostTileColumns)) return FP6MI_ERR_SHAPE;
     fp6mi::Int4Args a = { W_native, scales_native, X, bias, Y, offsets, (uint32_t)N, (uint32_t)K, (uint32_t)((K + 127) / 128), (uint32_t)(M / 16), (uint32_t)experts, activation, out_f32, nullptr };
     if (scratch_bytes(dtype, kernel, N, K)) {
         if (!workspace) return FP6MI_ERR_WORKSPACE;
@@ -157,6 +191,12 @@ int fp6mi_int4_linear(void *stream, int dtype, const void *W_native, const void 
     }
     if (dtype == 0) return group == 128 ? fp6mi::int4_run_0_1(stream, a, zeros != 0, kernel) : group == 64 ? fp6mi::int4_run_0_2(stream, a, zeros != 0, kernel) : fp6mi::int4_run_0_4(stream, a, zeros != 0, kernel);
     return group == 128 ? fp6mi::int4_run_1_1(stream, a, zeros != 0, kernel) : group == 64 ? fp6mi::int4_run_1_2(stream, a, zeros != 0, kernel) : fp6mi::int4_run_1_4(stream, a, zeros != 0, kernel);
+}
+
+int fp6mi_int4_linear(void *stream, int dtype, const void *W_native, const void *scales_native, int group, int zeros, const void *bias, const void *X, void *Y, int out_f32, int activation,
+                      const int *offsets, size_t experts, size_t M, size_t N, size_t K, void *workspace)
+{
+    return fp6mi_int4_linear_cfg(stream, dtype, W_native, scales_native, group, zeros, bias, X, Y, out_f32, activation, offsets, experts, M, N, K, workspace, -1);
 }
 
 } // extern "C"

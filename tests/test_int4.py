@@ -1,7 +1,8 @@
 """Products with 4-bit integer weights and group scales against their definition in 64 bits.
 
 Tolerances count roundings: half a step of fp16 is 2^-11 of the value (2^-25 below the normal numbers), of bf16 2^-8; products x * (q - z) are exact, and a float32 sum of n of them, the scaling of
-each group and the sum over groups are off by at most (n + 2) * 2^-23 of the sum of all magnitudes, whatever the order and however the matrix unit rounds between them."""
+each group and the sum over groups are off by at most (n + 2) * 2^-23 of the sum of all magnitudes, whatever the order and however the matrix unit rounds between them.  (In products of few bf16 rows the
+terms are x * (128 + q) and -x * (128 + z), at most 143 each.)"""
 import numpy as np
 import pytest
 import torch
@@ -50,9 +51,11 @@ def randn(seed, *shape, dtype=torch.float16, scale=1.0, device=DEV):
     return (torch.randn(*shape, generator=torch.Generator().manual_seed(seed)) * scale).to(dtype).to(device)
 
 
-def product64(w, x, bias=None):
-    """x @ w^T + bias in 64 bits, and how far float32 sums may be from it."""
+def product64(w, x, bias=None, extra=None):
+    """x @ w^T + bias in 64 bits, and how far float32 sums may be from it (extra: of the 128 + q and -(128 + z) that stand for the codes and zero points of that weight)."""
     y, mag = d(x) @ w.t(), d(x).abs() @ w.abs().t()
+    if extra is not None:
+        mag = mag + d(x).abs() @ (2 * 143 * extra.scales.cpu().double().repeat_interleave(extra.group, 1)[:, :extra.IC]).t()
     if bias is not None:
         y, mag = y + d(bias), mag + d(bias).abs()
     return y, (w.shape[1] + 3) * 2.0 ** -23 * mag
@@ -156,7 +159,7 @@ SHAPES = [  # OC, IC, N, group, zeros, type, bias
 def test_product(OC, IC, N, group, zeros, type, bias):
     w = Weight(OC + IC + N, OC, IC, group, zeros, type)
     x, b = randn(N, N, IC, dtype=w.dtype), randn(N + 1, OC, dtype=w.dtype) if bias else None
-    y, err = product64(w.w, x, b)
+    y, err = product64(w.w, x, b, extra=w if type == "bf16" and choice(OC, N, IC, type) < 4 else None)
     within(fp6.int4_forward_native(x, w.native, w.native_scales, bias=b), *plain(y, err, w.dtype))
     within(fp6.int4_forward_native(x, w.native, w.native_scales, bias=b, out_dtype=torch.float32), *plain(y, err, torch.float32), "float32")
 
@@ -305,8 +308,13 @@ def test_refusals_of_the_c_abi():
     for name in ("W", "S", "X", "Y"):
         assert linear(**{name: None}) == NULL and linear(**{name: p + 8}) == ALIGN
     assert linear(bias=p + 1) == ALIGN and linear(offsets=p + 2) == ALIGN
-    assert linear(N=0, X=None, Y=None) == 0 and linear(dtype=1, N=500) == -4 and linear(ws=p + 8) == ALIGN
-    assert L.fp6mi_int4_workspace_bytes(0, 1, 0, 32, 500, 64) == 0 and L.fp6mi_int4_workspace_bytes(1, 1, 0, 32, 500, 64) == 2000 + 500 * 128 and L.fp6mi_int4_workspace_bytes(1, 1, 0, 32, 1, 64) == 0
+    assert linear(N=0, X=None, Y=None) == 0 and linear(dtype=1, M=8192, K=8192, N=500) == -4 and linear(ws=p + 8) == ALIGN
+    assert L.fp6mi_int4_workspace_bytes(0, 1, 0, 32, 500, 64, 0, 8) == 0 and L.fp6mi_int4_workspace_bytes(1, 1, 0, 32, 500, 64, 0, 8) == 2000 + 500 * 128
+    assert L.fp6mi_int4_workspace_bytes(1, 1, 0, 32, 500, 64, 0, 3) == 0 and L.fp6mi_int4_workspace_bytes(1, 1, 0, 32, 500, 64, 0, 9) == 0 and L.fp6mi_int4_workspace_bytes(1, 1, 0, 32, 0, 64, 0, 8) == 0
+
+    def cfg(kernel, act=-1, K=64):
+        return L.fp6mi_int4_linear_cfg(None, 1, p, p, 64, 0, None, p, p, 0, act, None, 1, 32, 2, K, None, kernel)
+    assert cfg(9) == SHAPE and cfg(0, act=0) == SHAPE and cfg(4, K=(1 << 20) + 32) == SHAPE and cfg(8) == -4
     assert L.fp6mi_int4_pack(p, p, p, p, None, 2, 1, 16, 64, 64) == TYPE and L.fp6mi_int4_pack(p, p, p, None, None, 0, 1, 16, 64, 64) == NULL
     assert L.fp6mi_int4_pack_gpu(None, p, p, p, p, None, 0, 1, 16, 64, 33) == SHAPE and L.fp6mi_int4_pack_gpu(None, p + 4, p, p, p, None, 0, 1, 16, 64, 64) == ALIGN
 
@@ -337,3 +345,87 @@ def test_refusals_of_the_function(monkeypatch):
 def test_refusals_of_the_function_on_the_gpu(monkeypatch):
     w = Weight(1, 32, 160, 32, True)
     refusals(randn(1, 2, 160), w, monkeypatch)
+
+
+# ---------------------------------------------------------------------------------------------------------------- the kernels by number
+KERNELS = [(0, 16, 1, 16), (0, 16, 2, 8), (0, 16, 4, 8), (0, 16, 4, 4), (1, 32, 4, 4), (1, 32, 8, 4), (1, 32, 8, 2), (1, 64, 8, 2), (1, 64, 16, 1)]   # tile kernel, rows of X, row tiles, K parts
+
+
+def choice(OC, N, IC, type="fp16", E=0, gated=False):
+    import ctypes
+    shape = (ctypes.c_int * 4)()
+    k = _lib.lib().fp6mi_int4_query_kernel(0 if type == "fp16" else 1, E or 1, E > 0, OC, N, IC, gated, shape)
+    assert k < 0 or tuple(shape) == KERNELS[k]
+    return k
+
+
+def test_every_kernel_is_asked_for():
+    """Each of the kernels is the choice somewhere in the range that is used."""
+    for gated in (False, True):
+        found = {choice(OC, N, IC, gated=gated) for OC in (256, 1008, 2064, 4112, 8208, 14352, 28688) for IC in (288, 1056, 2080, 4192, 8192, 11040, 28672) for N in (1, 8, 14, 20, 33, 61, 75, 125, 193, 260, 400, 521, 800, 2000)}
+        assert found == set(range(1 if gated else 0, len(KERNELS)))   # (kernel 0 has one row tile, and gate and up are two)
+
+
+def test_choices_are_in_range():
+    for type in ("fp16", "bf16"):
+        for E in (0, 1, 7, 128, 1024):
+            for OC in (32, 4128, 1 << 20):
+                for N in (1, 100, 5000, 1 << 22, 1 << 30):
+                    for IC in (32, 4128, 1 << 21):
+                        for gated in (False, True):
+                            k = choice(OC, N, IC, type, E, gated)
+                            assert k == -2 or (0 <= k < 9 and (k < 4 or IC <= 1 << 20) and (k > 0 or not gated))
+
+
+def by_kernel(kernel, w, x, bias=None, act=-1, f32=False, plan=None):
+    """The product by one kernel, into rows with others behind them that have to stay as they are."""
+    L, s = _lib.lib(), w.native_scales
+    N, E, type = x.shape[0], w.E or 1, 0 if w.dtype == torch.float16 else 1
+    cols = w.OC // 2 if act >= 0 else w.OC
+    whole = torch.full((N + 3, cols), 7.0, dtype=torch.float32 if f32 else w.dtype, device=DEV)
+    need = L.fp6mi_int4_workspace_bytes(type, E, plan is not None, w.OC, N, w.IC, act >= 0, kernel)
+    ws = torch.empty(need, dtype=torch.uint8, device=DEV)
+    rc = L.fp6mi_int4_linear_cfg(torch.cuda.current_stream().cuda_stream, type, w.native.data_ptr(), s.data_ptr(), 128 // s.shape[-2], s.shape[-1] - 1, None if bias is None else bias.data_ptr(), x.data_ptr(),
+                                 whole.data_ptr(), f32, act, None if plan is None else plan.offsets.data_ptr(), E, w.OC, N, w.IC, ws.data_ptr() if need else None, kernel)
+    assert rc == 0, rc
+    assert (whole[N:] == 7.0).all()
+    return whole[:N]
+
+
+@gpu
+@pytest.mark.parametrize("group,zeros", [(32, True), (32, False), (64, True), (64, False), (128, True), (128, False)])
+@pytest.mark.parametrize("type", ["fp16", "bf16"])
+@pytest.mark.parametrize("kernel", range(9))
+def test_every_kernel_with_every_layout(kernel, type, group, zeros):
+    """Row tiles that do not fill a workgroup, one to five parts of K, the last block cut, rows of X at the borders of a tile; sums as they are, rounded, with a bias, gated."""
+    cols = KERNELS[kernel][1]
+    for OC, IC, N in ((48, 32, 1), (272, 96, cols), (96, 1184, cols + 1), (1056, 608, 2 * cols - 1), (32, 4128, 3), (288, 2048, 3 * cols + 5)):
+        w = Weight(OC + N + kernel, OC, IC, group, zeros, type)
+        x, b = randn(N, N, IC, dtype=w.dtype), randn(N + 1, OC, dtype=w.dtype)
+        # (in few bf16 rows -(128 + z) and 128 + q stand for q - z)
+        y, err = product64(w.w, x, b, extra=w if type == "bf16" and kernel < 4 else None)
+        within(by_kernel(kernel, w, x, b), *plain(y, err, w.dtype), "%s" % ((OC, IC, N),))
+        within(by_kernel(kernel, w, x, b, f32=True), *plain(y, err, torch.float32), "float32 %s" % ((OC, IC, N),))
+        if kernel > 0 and OC % 32 == 0:
+            within(by_kernel(kernel, w, x, b, act=1), *gated64(y, err, "gelu", w.dtype), "gated %s" % ((OC, IC, N),))
+
+
+@gpu
+@pytest.mark.parametrize("kernel", [4, 5, 6, 7, 8])
+def test_bf16_rows_of_every_size_in_tiles(kernel):
+    """Rows of bf16 are multiplied as fp16 with a power of two each: magnitudes from the smallest to the largest, zeros, infinities and NaN."""
+    w = Weight(5, 64, 160, 32, True, "bf16")
+    x = randn(3, 12, 160, dtype=torch.float32, device="cpu")
+    x *= torch.exp2(torch.tensor([0, -60, 60, -126, 100, -133, 10, 0, 0, 0, 0, 0])).unsqueeze(1)
+    x[7] = 0
+    x[8, 3], x[9, 5], x[10, 0], x[11, 1:] = float("inf"), float("nan"), 2.0 ** 30, 2.0 ** -20
+    x[11, 0] = 2.0 ** 19
+    x = x.bfloat16().to(DEV)
+    got = by_kernel(kernel, w, x, f32=True)
+    fine = [n for n in range(12) if n not in (8, 9)]
+    y, err = product64(w.w, x[fine])
+    # (values below 2^-29 of their row's largest: 2^-40 of that, times the sum of the weights)
+    lost = 2.0 ** -40 * d(x[fine]).abs().amax(1, keepdim=True) * w.w.abs().sum(1)
+    within(got[fine], y, err * (1 + 2.0 ** -24) + lost + 2.0 ** -24 * y.abs() + 2.0 ** -149)
+    k = w.w[:, 3]
+    assert torch.equal(torch.isinf(d(got[8])), k != 0) and torch.equal(d(got[8])[k != 0] > 0, k[k != 0] > 0) and got[9].isnan().all()
