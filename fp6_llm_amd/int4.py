@@ -33,6 +33,12 @@ def int4_quantize(weight, group=128, zeros=False):
     return q[..., 0::2] | q[..., 1::2] << 4, scales, None if z is None else z.to(torch.uint8)
 
 
+def native_shapes(OC, IC, group, zeros, experts=None):
+    """Of the native weights (int32) and scales of int4_pack_native."""
+    lead = (() if experts is None else (experts,)) + (OC // 16, (IC + 127) // 128)
+    return lead + (256,), lead + (16, 128 // (128 if group % 128 == 0 else 64 if group % 64 == 0 else 32), 2 if zeros else 1)
+
+
 def int4_pack_native(codes, scales, zeros=None, group=128):
     """(native_weight, native_scales) of int4_forward_native from weights as a checkpoint holds them: codes uint8 [OC, IC/2], two to a byte, the even column in the low half; scales float16 or
     bfloat16 [OC, ceil(IC/group)]; zeros uint8 like the scales, 0..15, or None: 8 everywhere.  Or all three for experts, [E, ...].  On the tensors' device, a GPU's or the host's.
@@ -52,10 +58,8 @@ def int4_pack_native(codes, scales, zeros=None, group=128):
         raise ValueError("zeros must be uint8 %s on the codes' device" % list(shape))
     if codes.device.type not in ("cuda", "cpu"):
         raise ValueError("codes must be on a GPU or on the host")
-    each = 128 if group % 128 == 0 else 64 if group % 64 == 0 else 32
-    lead, KB = ((E,) if codes.dim() == 3 else ()) + (OC // 16,), (IC + 127) // 128
-    w = torch.empty(lead + (KB, 256), dtype=torch.int32, device=codes.device)
-    s = torch.empty(lead + (KB, 16, 128 // each, 1 if zeros is None else 2), dtype=scales.dtype, device=codes.device)
+    native, native_scales = native_shapes(OC, IC, group, zeros is not None, E if codes.dim() == 3 else None)
+    w, s = torch.empty(native, dtype=torch.int32, device=codes.device), torch.empty(native_scales, dtype=scales.dtype, device=codes.device)
     codes, scales, zeros = codes.contiguous(), scales.contiguous(), None if zeros is None else zeros.contiguous()
     args = (w.data_ptr(), s.data_ptr(), codes.data_ptr(), scales.data_ptr(), ops._ptr(zeros), TYPES[scales.dtype], E, OC, IC, group)
     if codes.device.type == "cpu":

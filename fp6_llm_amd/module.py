@@ -10,7 +10,7 @@ import torch
 from . import quant
 from . import (MI355X_CUS, group_exps_bytes, heuristic_splitk_mi355x, linear_forward_native, native_bytes, pack_group_exps, to_native,
                weight_dequant_native_cuda, weight_prepacking_native_cpu, weight_quantize_native_cuda)
-from . import ops
+from . import int4, ops
 
 _MAGIC = b"FP6MI\x00\x01\x00"   # name, NUL, layout version 1, reserved
 
@@ -62,13 +62,23 @@ def _held(module, name):
     return held[name] if name in held else getattr(module, name)
 
 
-def _rows_of(x, features):
-    """x[..., features] as float16 rows, of which nothing but their values counts or a backward pass."""
+def _rows_of(x, features, dtype=torch.float16):
+    """x[..., features] as rows of dtype, of which nothing but their values counts or a backward pass."""
     _refuse_unseen(x)
     if x.dim() < 1 or x.shape[-1] != features:
         raise ValueError("need an input of %d features, got %s" % (features, list(x.shape)))
     x2 = x.reshape(-1, features).resolve_neg()
-    return x2 if x2.dtype == torch.float16 else x2.half()
+    return x2 if x2.dtype == dtype else x2.to(dtype)
+
+
+def _keep_types(module, apply, fn, args, kwargs):
+    """nn.Module._apply, but that the buffers keep their types when a model around the module is cast."""
+    before = dict(module._buffers)
+    apply(fn, *args, **kwargs)
+    for name, t in before.items():
+        if t is not None and module._buffers[name].dtype != t.dtype:
+            module._buffers[name] = t.to(module._buffers[name].device)
+    return module
 
 
 def _gradient(grad):
@@ -412,12 +422,7 @@ class LowRankAdapters(torch.nn.Module):
 
     def _apply(self, fn, *args, **kwargs):
         """nn.Module's, but that the buffers keep their types when a model around them is cast (the scalings are float32)."""
-        before = dict(self._buffers)
-        super()._apply(fn, *args, **kwargs)
-        for name, t in before.items():
-            if self._buffers[name].dtype != t.dtype:
-                self._buffers[name] = t.to(self._buffers[name].device)
-        return self
+        return _keep_types(self, super()._apply, fn, args, kwargs)
 
     @torch.no_grad()
     def set(self, slot, a, b, scaling=1.0):
@@ -445,6 +450,112 @@ class LowRankAdapters(torch.nn.Module):
 
     def extra_repr(self):
         return "in_features=%d, out_features=%d, slots=%d, rank=%d" % (self.in_features, self.out_features, self.slots, self.rank)
+
+
+class Int4Linear(torch.nn.Module):
+    """y = x @ w^T (+ bias) with 4-bit integer weights and a scale, possibly a zero point, for each row and group of columns (int4.int4_forward_native).  Weights, scales and bias are buffers that
+    keep their types when a model around them is cast; the layer is inference-only: an input that is to get a gradient is refused."""
+
+    def __init__(self, in_features, out_features, group=128, zeros=False, bias=None, dtype=torch.float16):
+        """group: columns of a scale, a multiple of 32.  zeros: the weights have zero points.  dtype: of scales, bias and activations, float16 or bfloat16 (inputs of another type are converted)."""
+        super().__init__()
+        if out_features < 16 or out_features % 16 or in_features < 32 or in_features % 32 or group < 32 or group % 32:
+            raise ValueError("Int4Linear needs out_features %% 16 == 0, in_features %% 32 == 0 and a group that is a multiple of 32")
+        if dtype not in int4.TYPES or (bias is not None and (bias.dtype != dtype or bias.shape != (out_features,))):
+            raise ValueError("Int4Linear is float16 or bfloat16, a bias [%d] of the same type" % out_features)
+        self.in_features, self.out_features, self.group, self.dtype = in_features, out_features, group, dtype
+        native, scales = int4.native_shapes(out_features, in_features, group, zeros)
+        self.register_buffer("weight_native", torch.zeros(native, dtype=torch.int32))
+        self.register_buffer("weight_scales", torch.zeros(scales, dtype=dtype))
+        self.register_buffer("bias", bias)
+
+    @classmethod
+    def from_codes(cls, codes, scales, zeros=None, group=128, bias=None):
+        """Weights as a checkpoint holds them (int4.int4_pack_native)."""
+        native, native_scales = int4.int4_pack_native(codes, scales, zeros, group)
+        m = cls(2 * codes.shape[1], codes.shape[0], group, zeros is not None, bias, scales.dtype).to(codes.device)
+        m.weight_native, m.weight_scales = native, native_scales
+        return m
+
+    @classmethod
+    def from_float(cls, weight, group=128, zeros=False, bias=None):
+        """Quantizes a float [out_features, in_features] weight, rounding to nearest (int4.int4_quantize)."""
+        return cls.from_codes(*int4.int4_quantize(weight, group, zeros), group, bias)
+
+    def _apply(self, fn, *args, **kwargs):
+        return _keep_types(self, super()._apply, fn, args, kwargs)
+
+    def forward(self, x):
+        if x.requires_grad and torch.is_grad_enabled():
+            raise ValueError("a product with 4-bit weights has no gradient: call it under torch.no_grad()")
+        scales = _held(self, "weight_scales")
+        x2 = _aligned(_rows_of(x, self.in_features, scales.dtype))
+        y = int4.int4_forward_native(x2, _held(self, "weight_native"), scales, bias=_held(self, "bias"))
+        return y if x.dim() == 2 else y.reshape(*x.shape[:-1], self.out_features)
+
+    def extra_repr(self):
+        return "in_features=%d, out_features=%d, group=%d, zeros=%s" % (self.in_features, self.out_features, self.group, self.weight_scales.shape[-1] == 2)
+
+
+def _aligned(x2):
+    """Rows that begin between two 16-byte boundaries, copied."""
+    return x2.clone() if x2.is_contiguous() and x2.data_ptr() % 16 else x2
+
+
+class Int4Experts(torch.nn.Module):
+    """The feed-forward layer of a mixture of experts, gated blocks on 4-bit integer weights with group scales: out[t] = sum over token t's experts e of
+    weights[t, j] * down_e(act(gate_e(x[t])) * up_e(x[t])).  Four operators: tokens sorted by expert, the gated product of their rows, the product down (float32), the weighted sum back.
+    Everything stays on the GPU, so index and weights may change between the replays of a graph.  Inference-only, like Int4Linear."""
+
+    def __init__(self, in_features, hidden_features, experts, group=128, zeros=False, activation="silu", dtype=torch.float16):
+        super().__init__()
+        if in_features < 32 or in_features % 32 or hidden_features < 32 or hidden_features % 32 or group < 32 or group % 32:
+            raise ValueError("Int4Experts needs in_features and hidden_features that are multiples of 32, and a group that is one")
+        if not 1 <= experts <= MAX_EXPERTS or dtype not in int4.TYPES:
+            raise ValueError("Int4Experts needs 1 to %d experts, float16 or bfloat16" % MAX_EXPERTS)
+        ops._activation_code(activation)
+        self.in_features, self.hidden_features, self.experts, self.group, self.activation, self.dtype = in_features, hidden_features, experts, group, activation, dtype
+        for name, rows, cols in (("gate_up", 2 * hidden_features, in_features), ("down", in_features, hidden_features)):
+            native, scales = int4.native_shapes(rows, cols, group, zeros, experts)
+            self.register_buffer(name + "_native", torch.zeros(native, dtype=torch.int32))
+            self.register_buffer(name + "_scales", torch.zeros(scales, dtype=dtype))
+
+    @classmethod
+    def from_codes(cls, gate, up, down, group=128, activation="silu"):
+        """gate, up, down: (codes, scales, zeros or None) each, as int4.int4_pack_native takes them for experts; gate and up [E, hidden, ...], down [E, features, ...]."""
+        E, F = gate[0].shape[:2]
+        if any((a is None) != (b is None) for a, b in ((gate[2], up[2]), (gate[2], down[2]))) or down[0].shape != (E, 2 * gate[0].shape[2], F // 2):
+            raise ValueError("gate, up and down must be [E, hidden, features / 2], the same, and [E, features, hidden / 2], all with zero points or all without")
+        both = [None if g is None else ops.gate_up_pairs(g.flatten(0, 1), u.flatten(0, 1)).unflatten(0, (E, 2 * F)) for g, u in zip(gate, up)]
+        m = cls(2 * gate[0].shape[2], F, E, group, gate[2] is not None, activation, gate[1].dtype).to(gate[0].device)
+        m.gate_up_native, m.gate_up_scales = int4.int4_pack_native(*both, group)
+        m.down_native, m.down_scales = int4.int4_pack_native(*down, group)
+        return m
+
+    @classmethod
+    def from_float(cls, gate, up, down, group=128, zeros=False, activation="silu"):
+        """Quantizes float weights, gate and up [E, hidden, features], down [E, features, hidden], rounding to nearest."""
+        return cls.from_codes(*(int4.int4_quantize(w, group, zeros) for w in (gate, up, down)), group, activation)
+
+    def _apply(self, fn, *args, **kwargs):
+        return _keep_types(self, super()._apply, fn, args, kwargs)
+
+    def forward(self, x, index, weights=None):
+        """x: [..., features]; index: [..., k], int32 or int64, the experts of every token (a number outside 0..experts-1 for none); weights: [..., k], float, 1 without."""
+        if torch.is_grad_enabled() and (x.requires_grad or (weights is not None and weights.requires_grad)):
+            raise ValueError("a product with 4-bit weights has no gradient: call it under torch.no_grad()")
+        scales = _held(self, "gate_up_scales")
+        x2 = _rows_of(x, self.in_features, scales.dtype)
+        if index.dim() < 2 or index.shape[:-1] != x.shape[:-1] or (weights is not None and weights.shape != index.shape):
+            raise ValueError("index, and weights like it, must name k experts for each of the tokens, got %s for an input %s" % (list(index.shape), list(x.shape)))
+        rows, plan = expert_sort(x2, index.reshape(-1, index.shape[-1]), self.experts)
+        h = int4.int4_forward_native(rows, _held(self, "gate_up_native"), scales, plan, self.activation)
+        y = int4.int4_forward_native(h, _held(self, "down_native"), _held(self, "down_scales"), plan, out_dtype=torch.float32)
+        out = expert_combine(y, plan, None if weights is None else weights.reshape(-1, weights.shape[-1]), scales.dtype)
+        return out if x.dim() == 2 else out.reshape(x.shape)
+
+    def extra_repr(self):
+        return "in_features=%d, hidden_features=%d, experts=%d, group=%d, activation=%s" % (self.in_features, self.hidden_features, self.experts, self.group, self.activation)
 
 
 def save_native(path, native_int32, scales, exponent, mantissa, out_features, in_features, group_exps=None):
@@ -497,3 +608,6 @@ def load_native(path):
                 raise ValueError("file is truncated")
             hdr["group_exps"] = torch.from_numpy(ge.copy())
     return torch.from_numpy(nat.copy()), torch.from_numpy(sc.copy()), hdr
+
+
+from .experts import MAX_EXPERTS, expert_combine, expert_sort  # noqa: E402  (it imports what is above)
