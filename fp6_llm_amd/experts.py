@@ -13,10 +13,14 @@ MAX_CHOSEN, MAX_EXPERTS = 64, 1024
 class ExpertPlan:
     """Where an index [tokens, k] sends every place, int32 on the GPU: place[tokens * k], the row of a place among the sorted ones (a permutation); order[tokens * k], its inverse, -1 for
     rows behind the last one with an expert; offsets[experts + 1], the first row of every expert, and in the end the number of places that have one.  (One tensor, `table`, holds all three.)"""
-    __slots__ = ("table", "tokens", "k", "experts", "places")
+    __slots__ = ("table", "tokens", "k", "experts")
 
     def __init__(self, table, tokens, k, experts):
-        self.table, self.tokens, self.k, self.experts, self.places = table, tokens, k, experts, tokens * k
+        self.table, self.tokens, self.k, self.experts = table, tokens, k, experts
+
+    @property
+    def places(self):
+        return self.tokens * self.k
 
     @property
     def offsets(self):
@@ -147,7 +151,7 @@ def expert_sort(x, index, experts):
     differentiates = _differentiates(x)
     if _ext is not None:
         rows, table = _ext.expert_sort(x, index, experts)
-        return rows, ExpertPlan(table, *index.shape, experts)
+        return rows, ExpertPlan(table, index.shape[0], index.shape[1], experts)
     if not differentiates:
         return _sorted(x, index, experts)
     plans = []

@@ -61,6 +61,7 @@ def test_experts_layer(T, k, E, F, K, group, zeros, type, act, drop):
     assert torch.equal(layer(x.view(T, 1, K), index.view(T, 1, k), weights.view(T, 1, k)), got.view(T, 1, K))
     assert torch.equal(layer(x.float(), index.int(), weights.double()), got)
     within(layer(x, index), *layer64(gate, up, down, x, index, torch.ones(T, k), act, gate.dtype))
+    assert layer(x[:0], index[:0], weights[:0]).shape == (0, K)
 
 
 @gpu

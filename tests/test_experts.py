@@ -8,7 +8,7 @@ import torch
 
 import fp6_llm_amd as fp6
 from fp6_llm_amd import _lib
-from test_int4 import HALF, TINY, Weight, d, gated64, plain, product64, randn, within
+from test_int4 import HALF, TINY, Weight, by_kernel, d, gated64, plain, product64, randn, within
 
 DEV = "cuda:0"
 gpu = pytest.mark.gpu
@@ -495,3 +495,68 @@ def test_gradients_that_are_not_asked_for():
     assert got.dtype == torch.float64 and torch.equal(got.float(), want[1])
     with torch.no_grad():
         assert not fp6.expert_combine(both_r, plan, both_w).requires_grad
+
+
+@gpu
+@pytest.mark.parametrize("kernel", range(1, 9))
+@pytest.mark.parametrize("type", ["fp16", "bf16"])
+def test_every_kernel_with_rows_of_experts(kernel, type):
+    """Borders of experts inside tiles, experts without rows, rows behind the last expert's that hold NaN."""
+    E, sizes = 5, [3, 0, 40, 17, 129]
+    index = torch.tensor([e for e, n in enumerate(sizes) for _ in range(n)] + [-1] * 20).unsqueeze(1).to(DEV)
+    w = Weight(kernel, 96, 416, 64, True, type, E)
+    rows, plan = fp6.expert_sort(randn(2, len(index), 416, dtype=w.dtype), index, E)
+    want = Plan64(index, E)
+    b = randn(3, E, 96, dtype=w.dtype)
+    y, tol = grouped64(w, want, rows, b, None, w.dtype)
+    h, htol = grouped64(w, want, rows, b, "silu", w.dtype)
+    extra = 30 if type == "bf16" and kernel < 4 else 1   # (128 + q and -(128 + z), 143 at most, stand for a difference that is 5 in the mean)
+    rows[int(want.n):] = float("nan")
+    within(by_kernel(kernel, w, rows, b, plan=plan), y, tol * extra)
+    within(by_kernel(kernel, w, rows, b, act=0, plan=plan), h, htol * extra)
+
+
+@gpu
+def test_weights_beyond_32_bit_offsets():
+    """The last of many experts, six gigabytes in, against the same matrix by itself."""
+    E, OC, IC = 32, 16384, 24576
+    codes = torch.empty(E, OC, IC // 2, dtype=torch.uint8, device=DEV)
+    for e in range(E):
+        codes[e] = torch.randint(0, 256, (OC, IC // 2), dtype=torch.uint8, device=DEV)
+    scales = torch.rand(E, OC, IC // 128, device=DEV).half() / 100
+    native, native_scales = fp6.int4_pack_native(codes, scales)
+    one, one_scales = fp6.int4_pack_native(codes[E - 1], scales[E - 1])
+    assert native.numel() * 4 > 2 ** 32 and torch.equal(native[E - 1], one) and torch.equal(native_scales[E - 1], one_scales)
+    for T in (3, 70):
+        x, index = randn(1, T, IC), torch.full((T, 1), E - 1, device=DEV)
+        rows, plan = fp6.expert_sort(x, index, E)
+        k = 3 if T == 3 else 8
+        both = Weight.__new__(Weight)
+        both.native, both.native_scales, both.OC, both.IC, both.E, both.dtype = native, native_scales, OC, IC, E, torch.float16
+        alone = Weight.__new__(Weight)
+        alone.native, alone.native_scales, alone.OC, alone.IC, alone.E, alone.dtype = one, one_scales, OC, IC, 0, torch.float16
+        assert torch.equal(by_kernel(k, both, rows, plan=plan), by_kernel(k, alone, x))
+
+
+@gpu
+def test_two_threads_on_one_stream():
+    """Calls with scratch (many places; bf16 tiles) from two threads: each has the results of its own."""
+    import threading
+    E, k, T, H = 8, 2, 2000, 256
+    w = Weight(1, 512, H, 64, True, "bf16")
+    inputs = [(route(s, T, k, E), randn(s, T, H, dtype=torch.bfloat16)) for s in (1, 2)]
+    want = [(fp6.expert_sort(x, i, E)[0], fp6.int4_forward_native(x, w.native, w.native_scales)) for i, x in inputs]
+    failed = []
+
+    def work(n):
+        i, x = inputs[n]
+        for _ in range(30):
+            rows, y = fp6.expert_sort(x, i, E)[0], fp6.int4_forward_native(x, w.native, w.native_scales)
+            if not (torch.equal(rows, want[n][0]) and torch.equal(y, want[n][1])):
+                failed.append(n)
+    threads = [threading.Thread(target=work, args=(n,)) for n in (0, 1)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed
