@@ -171,38 +171,38 @@ __device__ __forceinline__ void store_zeros(const Int4Args &a, const Tile &t, ui
 }
 
 // ---------------------------------------------------------------------------------------------------------------
-// Few rows: RT row tiles and NT tiles of 16 rows of X to a workgroup of WK wavefronts, which share K: a wavefront takes every WK-th column block, its weights straight from HBM to registers
-// (the next block's on their way meanwhile) and its part of X from L2.  Bound by the bytes of the weights; the partial sums meet in LDS.
+// Few rows: RT row tiles and 16 rows of X to a workgroup of WK wavefronts, which share K: a wavefront takes every WK-th column block, its weights straight from HBM to registers
+// (the next block's on their way meanwhile) and its part of X from L2; the partial sums meet in LDS.  Bound by the bytes of the weights where there are many (28672x8192: 23.1 us at 1 row, 28.2 at 16, of which
+// the bytes take 23.6; 8192x8192: 9.2 and 12.1 of 6.8), by a wavefront's few blocks one after another where there are few (4096x4096 at 1 row: 4.3 us with 16 wavefronts to a row tile, 5.2 with 8 to two).
+// Three and four blocks on their way were no faster, nor were two tiles of rows of X to a workgroup.
 // ---------------------------------------------------------------------------------------------------------------
-template <int GPB, bool Z, int RT, int NT> struct Block {
+template <int GPB, bool Z, int RT> struct Block {
     v4u            w[RT];
     Scales<GPB, Z> s[RT];
-    v8t            x[NT][4];
+    v8t            x[4];
 };
 
-template <int GPB, bool Z, int RT, int NT, int WK> __global__ __launch_bounds__(WK * 64, WK > 4 ? 1 : 2) void int4_stream(const Int4Args a)
+template <int GPB, bool Z, int RT, int WK> __global__ __launch_bounds__(WK * 64, WK > 4 ? 1 : 2) void int4_stream(const Int4Args a)
 {
-    __shared__ v4f part[WK][RT * NT][64];
+    __shared__ v4f part[WK][RT][64];
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, q = lane >> 4;
     const uint32_t m0 = blockIdx.x * RT;
-    const Tile     t = tile_of(a, blockIdx.y, NT * 16);
+    const Tile     t = tile_of(a, blockIdx.y, 16);
     if (t.rows == 0) return;
     if (t.expert < 0) return store_zeros(a, t, m0, RT, WK * 64);
 
     const v4u            *w[RT];
     const Scales<GPB, Z> *s[RT];
-    const T              *x[NT];
 #pragma unroll
     for (int r = 0; r < RT; r++) { // (a last workgroup with fewer row tiles takes the last one again)
         const size_t at = ((size_t)t.expert * a.Mt + (m0 + r < a.Mt ? m0 + r : a.Mt - 1)) * a.KB;
         w[r] = static_cast<const v4u *>(a.W) + at * 64 + lane;
         s[r] = static_cast<const Scales<GPB, Z> *>(a.S) + at * 16 + c;
     }
-#pragma unroll
-    for (int n = 0; n < NT; n++) x[n] = static_cast<const T *>(a.X) + (size_t)(t.row + (n * 16 + c < t.rows ? n * 16 + c : t.rows - 1)) * a.K + q * 8;
+    const T *x = static_cast<const T *>(a.X) + (size_t)(t.row + (c < t.rows ? c : t.rows - 1)) * a.K + q * 8;
 
-    typedef Block<GPB, Z, RT, NT> B;
-    const FewCutter               cut;
+    typedef Block<GPB, Z, RT> B;
+    const FewCutter           cut;
     auto load = [&](B &b, uint32_t kb) __attribute__((always_inline)) {
         const uint32_t steps = (a.K - kb * 128) / 32; // of 32 columns, 4 but for the last block
 #pragma unroll
@@ -210,30 +210,24 @@ template <int GPB, bool Z, int RT, int NT, int WK> __global__ __launch_bounds__(
 #pragma unroll
         for (int r = 0; r < RT; r++) b.s[r] = s[r][(size_t)kb * 16];
 #pragma unroll
-        for (int n = 0; n < NT; n++)
-#pragma unroll
-            for (uint32_t i = 0; i < 4; i++) b.x[n][i] = i < steps ? *reinterpret_cast<const v8t *>(x[n] + kb * 128 + i * 32) : v8t{};
+        for (uint32_t i = 0; i < 4; i++) b.x[i] = i < steps ? *reinterpret_cast<const v8t *>(x + kb * 128 + i * 32) : v8t{};
     };
-    v4f sum[RT][NT];
+    v4f sum[RT];
 #pragma unroll
-    for (int r = 0; r < RT; r++)
-#pragma unroll
-        for (int n = 0; n < NT; n++) sum[r][n] = (v4f){ 0.f, 0.f, 0.f, 0.f };
+    for (int r = 0; r < RT; r++) sum[r] = (v4f){ 0.f, 0.f, 0.f, 0.f };
     auto multiply = [&](const B &b) __attribute__((always_inline)) {
         constexpr int kEach = 4 / GPB; // steps of a group
         constexpr bool kSecond = FP6MI_TYPE == 1;
         FewZero        zero;
         zero.set((T)8.f);
-        v4f first[NT][GPB]; // what the second instruction gives where all rows share it
+        v4f first[GPB]; // what the second instruction gives where all rows share it
         if constexpr (kSecond && !Z) {
 #pragma unroll
-            for (int n = 0; n < NT; n++)
+            for (int g = 0; g < GPB; g++) {
+                first[g] = (v4f){ 0.f, 0.f, 0.f, 0.f };
 #pragma unroll
-                for (int g = 0; g < GPB; g++) {
-                    first[n][g] = (v4f){ 0.f, 0.f, 0.f, 0.f };
-#pragma unroll
-                    for (int i = 0; i < kEach; i++) first[n][g] = second(b.x[n][g * kEach + i], zero, first[n][g]);
-                }
+                for (int i = 0; i < kEach; i++) first[g] = second(b.x[g * kEach + i], zero, first[g]);
+            }
         }
 #pragma unroll
         for (int r = 0; r < RT; r++)
@@ -244,18 +238,15 @@ template <int GPB, bool Z, int RT, int NT, int WK> __global__ __launch_bounds__(
                 v8t v[kEach];
 #pragma unroll
                 for (int i = 0; i < kEach; i++) v[i] = codes_of(b.w[r][g * kEach + i], zero, cut);
+                v4f y = { 0.f, 0.f, 0.f, 0.f };
+                if constexpr (kSecond && !Z) y = first[g];
 #pragma unroll
-                for (int n = 0; n < NT; n++) {
-                    v4f y = { 0.f, 0.f, 0.f, 0.f };
-                    if constexpr (kSecond && !Z) y = first[n][g];
-#pragma unroll
-                    for (int i = 0; i < kEach; i++) {
-                        if constexpr (kSecond && Z) y = second(b.x[n][g * kEach + i], zero, y);
-                        y = mfma(b.x[n][g * kEach + i], v[i], y);
-                    }
-#pragma unroll
-                    for (int i = 0; i < 4; i++) sum[r][n][i] += scale * y[i];
+                for (int i = 0; i < kEach; i++) {
+                    if constexpr (kSecond && Z) y = second(b.x[g * kEach + i], zero, y);
+                    y = mfma(b.x[g * kEach + i], v[i], y);
                 }
+#pragma unroll
+                for (int i = 0; i < 4; i++) sum[r][i] += scale * y[i];
             }
     };
     B b[2];
@@ -277,54 +268,52 @@ template <int GPB, bool Z, int RT, int NT, int WK> __global__ __launch_bounds__(
         }
     }
 #pragma unroll
-    for (int r = 0; r < RT; r++)
-#pragma unroll
-        for (int n = 0; n < NT; n++) part[wave][r * NT + n][lane] = sum[r][n];
+    for (int r = 0; r < RT; r++) part[wave][r][lane] = sum[r];
     __syncthreads();
 
-    // the sums of tile (r, n): lane c + 16 q has weight row c and rows 4 q + i of X
-    auto total = [&](int p) __attribute__((always_inline)) {
-        v4f y = part[0][p][lane];
+    // the sums of row tile r: lane c + 16 q has weight row c and rows 4 q + i of X
+    auto total = [&](int r) __attribute__((always_inline)) {
+        v4f y = part[0][r][lane];
 #pragma unroll
-        for (int k = 1; k < WK; k++) y += part[k][p][lane];
+        for (int k = 1; k < WK; k++) y += part[k][r][lane];
         return y;
     };
     const T *bias = a.bias ? static_cast<const T *>(a.bias) + (size_t)t.expert * a.Mt * 16 : nullptr;
     if (a.act < 0) {
-        for (uint32_t p = wave; p < RT * NT; p += WK) {
-            const uint32_t r = p / NT, n = p % NT, m = (m0 + r) * 16 + c;
+        for (uint32_t r = wave; r < RT; r += WK) {
+            const uint32_t m = (m0 + r) * 16 + c;
             if (m0 + r >= a.Mt) continue;
-            v4f         y = total(p);
+            v4f         y = total(r);
             const float add = bias ? (float)bias[m] : 0.f;
 #pragma unroll
             for (uint32_t i = 0; i < 4; i++)
-                if (n * 16 + 4 * q + i < t.rows) store(a, t.row + n * 16 + 4 * q + i, m, a.Mt * 16, y[i] + add);
+                if (4 * q + i < t.rows) store(a, t.row + 4 * q + i, m, a.Mt * 16, y[i] + add);
         }
     } else if constexpr (RT % 2 == 0) {
-        for (uint32_t p = wave; p < RT / 2 * NT; p += WK) {
-            const uint32_t r = p / NT * 2, n = p % NT, m = (m0 + r) * 16 + c;
+        for (uint32_t r = 2 * wave; r < RT; r += 2 * WK) {
+            const uint32_t m = (m0 + r) * 16 + c;
             if (m0 + r >= a.Mt) continue;
-            v4f         g = total(r * NT + n), u = total((r + 1) * NT + n);
+            v4f         g = total(r), u = total(r + 1);
             const float bg = bias ? (float)bias[m] : 0.f, bu = bias ? (float)bias[m + 16] : 0.f;
 #pragma unroll
             for (uint32_t i = 0; i < 4; i++)
-                if (n * 16 + 4 * q + i < t.rows) store(a, t.row + n * 16 + 4 * q + i, (m0 + r) * 8 + c, a.Mt * 8, activated(a.act, g[i] + bg) * (u[i] + bu));
+                if (4 * q + i < t.rows) store(a, t.row + 4 * q + i, (m0 + r) * 8 + c, a.Mt * 8, activated(a.act, g[i] + bg) * (u[i] + bu));
         }
     }
 }
 
 // ---------------------------------------------------------------------------------------------------------------
-template <int GPB, bool Z, int RT, int NT, int WK> int launch_stream(hipStream_t st, const Int4Args &a)
+template <int GPB, bool Z, int RT, int WK> int launch_stream(hipStream_t st, const Int4Args &a)
 {
-    const size_t tiles = fp6mi::int4_tiles(a.N, a.offsets ? a.E : 0, NT * 16);
+    const size_t tiles = fp6mi::int4_tiles(a.N, a.offsets ? a.E : 0, 16);
     if (tiles > 65535) return FP6MI_ERR_SHAPE;
-    hipLaunchKernelGGL((int4_stream<GPB, Z, RT, NT, WK>), dim3((a.Mt + RT - 1) / RT, (uint32_t)tiles), dim3(WK * 64), 0, st, a);
+    hipLaunchKernelGGL((int4_stream<GPB, Z, RT, WK>), dim3((a.Mt + RT - 1) / RT, (uint32_t)tiles), dim3(WK * 64), 0, st, a);
     return (int)hipGetLastError();
 }
 
 #if FP6MI_TYPE == 1 && FP6MI_GROUPS == 1
 // Rows in bf16 as fp16 times a power of two for each row, which puts the largest finite magnitude from 2^14 to 2^15.  What is smaller than 2^-29 of that loses bits, at most 2^-40 of it: a float32 sum of such
-// products has been rounded by more.  Infinities and NaN stay.  A workgroup to a row, which reads it twice (from L2); 4096 rows of 4096 take 13 us.
+// products has been rounded by more.  Infinities and NaN stay.  A workgroup to a row, which reads it twice (from L2); 4096 rows of 4096 take 15.4 us, 4.4 TB/s.
 __global__ __launch_bounds__(256) void rows_to_halfs(half_t *__restrict__ out, int *__restrict__ exponents, const T *__restrict__ X, uint32_t K)
 {
     __shared__ uint32_t most[4];
@@ -368,8 +357,8 @@ __global__ __launch_bounds__(256) void rows_to_halfs(half_t *__restrict__ out, i
 // More rows: tiles of WR * 64 weight rows x NT * 16 rows of X to a workgroup of WR x WK wavefronts; the WK groups take every WK-th column block.  X goes to LDS by direct transfers, a K block ahead, two
 // stages to a group; a row of a stage is 256 bytes whose 16 pieces stand in the order piece ^ (row & 15), which gives the reads of an MFMA operand all banks.  A wavefront holds its X of one block in
 // registers and takes one of its four row tiles after another: its codes become operands while the tile before is multiplied.  Bound by the matrix units with the conversions and the scaling of the
-// group sums beside them (3.6 VALU instructions to a matrix instruction; twice the columns to a wavefront, 2.6, was no faster, nor were 32x32x16 instructions, which draw more power).
-// Two workgroups to a CU where LDS allows, so that one multiplies while the other waits at its barrier.
+// group sums beside them (3.6 VALU instructions to a matrix instruction; twice the columns to a wavefront, 2.6, was no faster, nor were 32x32x16 instructions, which draw more power): 8192x8192 at 777 rows takes
+// 108 to 112 us, 8 experts of 22016x4096 at 4096 rows 720 to 740, 1.0 PFLOP/s, where a library's product of large dense fp16 matrices reaches 1.2.  Two workgroups to a CU where LDS allows, so that one multiplies while the other waits at its barrier.
 // ---------------------------------------------------------------------------------------------------------------
 template <int NT, int WR, int WK> constexpr size_t tile_lds_bytes() // the stages; the sums of the groups on their way to the first; the outputs on their way out (a half at a time where they are float32)
 {
@@ -621,10 +610,10 @@ template <int GPB, bool Z, int NT, int WR, int WK> int launch_tile(hipStream_t s
 template <int GPB, bool Z> int run(hipStream_t st, const Int4Args &a, int kernel)
 {
     switch (kernel) { // (in the order of fp6mi::kInt4Kernels)
-    case 0: return launch_stream<GPB, Z, 1, 1, 16>(st, a);
-    case 1: return launch_stream<GPB, Z, 2, 1, 8>(st, a);
-    case 2: return launch_stream<GPB, Z, 4, 1, 8>(st, a);
-    case 3: return launch_stream<GPB, Z, 4, 1, 4>(st, a);
+    case 0: return launch_stream<GPB, Z, 1, 16>(st, a);
+    case 1: return launch_stream<GPB, Z, 2, 8>(st, a);
+    case 2: return launch_stream<GPB, Z, 4, 8>(st, a);
+    case 3: return launch_stream<GPB, Z, 4, 4>(st, a);
     case 4: return launch_tile<GPB, Z, 2, 1, 4>(st, a);
     case 5: return launch_tile<GPB, Z, 2, 2, 4>(st, a);
     case 6: return launch_tile<GPB, Z, 2, 2, 2>(st, a);

@@ -71,12 +71,12 @@ int check_pack(const void *native, const void *native_scales, const void *codes,
 }
 
 // Which kernel takes a product (an index of kInt4Kernels): the fastest by this model of its time, us.  A workgroup's column blocks one after another take `step` each while every CU has one at the most,
-// `share` times the workgroups of a CU beyond, which come in rounds of as many as fit; and no kernel reads the weights faster than memory.  Rows of experts are taken to be spread evenly, with half a tile
-// to spare for each expert.  Fitted to 720 times (2048x8192 to 28672x8192 at 1 to 777 rows, 8 to 128 experts at 1 to 700 tokens, fp16 and bf16), off by 8 to 20 % rms for a kernel; the choice takes 1.03 times
-// the fastest measured in the mean, at worst 1.3.
-struct Times { double base, step, share, rows; int fit; }; // rows: how much longer a step takes with 16 rows than with none, of the kernel that streams weights
-constexpr Times kTimes[] = { { 5.5, 0.94, 0.94, 0.99, 2 }, { 3.9, 0.80, 0.88, 0.26, 2 }, { 2.6, 1.37, 2.00, 0, 1 }, { 2.5, 0.74, 0.65, 0.13, 3 }, { 5.9, 0.81, 0.90, 0, 2 }, { 6.2, 1.15, 1.75, 0, 1 },
-                             { 5.3, 0.79, 0.72, 0, 2 }, { 8.1, 0.92, 1.14, 0, 2 },    { 8.2, 0.83, 1.01, 0, 2 } };
+// `share` times the workgroups of a CU beyond; and no kernel reads the weights faster than memory.  Rows of experts are taken to be spread evenly, with half a tile to spare for each expert.
+// Fitted to 2344 times of 265 products in graphs, weights from HBM (512x2048 to 28672x8192 at 1 to 777 rows, 8 to 128 experts at 1 to 700 tokens, fp16 and bf16): a kernel's own time is off by 15 to 26 % rms,
+// the choice takes 1.01 times the fastest measured in the mean, at worst 1.29; for 126 other products 1.02 and 1.55.
+struct Times { double base, step, share, rows; }; // rows: how much longer a step takes with 16 rows than with none, of the kernel that streams weights
+constexpr Times kTimes[] = { { 1.84, 0.86, 1.51, 0.43 }, { 2.20, 1.07, 1.09, 0.18 }, { 2.42, 1.59, 1.97, 0 }, { 2.71, 1.10, 0.74, 0 }, { 3.35, 1.07, 1.10, 0 }, { 3.27, 1.50, 2.10, 0 },
+                             { 3.83, 1.06, 0.99, 0 },    { 2.94, 1.36, 1.62, 0 },    { 2.95, 1.05, 1.09, 0 } };
 
 constexpr int    kKernels = sizeof(kTimes) / sizeof(kTimes[0]);
 constexpr size_t kMostTileColumns = (size_t)1 << 20; // (offsets in a tile have 32 bits)
@@ -88,7 +88,7 @@ double time_of(int kernel, int dtype, size_t experts, bool grouped, size_t M, si
     const double used = grouped ? experts * (1 - std::exp(-(double)N / experts)) : 1.0, tiles = grouped ? std::max(used, (double)N / k.cols + 0.5 * used) : (double)((N + k.cols - 1) / k.cols);
     const double load = (double)((M / 16 + k.row_tiles - 1) / k.row_tiles) * tiles / 256, steps = (double)(((K + 127) / 128 + k.k_split - 1) / k.k_split);
     const double more = 1 + t.rows * std::min(16.0, (double)N / used) / 16;
-    const double among = load <= 1 ? load : (load + t.fit * std::ceil(load / t.fit)) / 2;
+    const double among = load <= 1 ? load : (load + std::ceil(load)) / 2;
     double       us = t.base + steps * more * std::max(t.step, t.share * among);
     if (dtype == 1 && k.tile) us += 3 + (double)N * K * 4 / 4.0e6; // (the rows on their way to fp16)
     return std::max(us, used * M * K * 0.515 / 5.1e6 + 1.5);

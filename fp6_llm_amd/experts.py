@@ -2,9 +2,13 @@
 
 A place p = t * k + j is the j-th expert of token t.  The functions enqueue on the current stream and check shapes, types and devices on the host; nothing is copied to the host, so the routing may
 change between the replays of a graph.  What they compute is in include/fp6mi.h.  They go through the torch extension where it is built, else through ctypes."""
+import sys
+
 import torch
 
 from . import _lib, ops
+
+_package = sys.modules[__package__]
 
 TYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
 MAX_CHOSEN, MAX_EXPERTS = 64, 1024
@@ -137,7 +141,7 @@ class _Combine(torch.autograd.Function):
 # ---------------------------------------------------------------------------------------------------------------- the operators
 def expert_plan(index, experts):
     """The ExpertPlan of index, int32 or int64 [tokens, k] on the GPU: the experts of every token, numbers outside 0..experts-1 (-1, say) for none."""
-    from . import _ext
+    _ext = _package._ext
     if _ext is not None:
         return ExpertPlan(_ext.expert_sort(None, index, experts)[1], *index.shape, experts)
     return _sorted(None, index, experts)[1]
@@ -146,7 +150,7 @@ def expert_plan(index, experts):
 def expert_sort(x, index, experts):
     """(rows, plan): rows[tokens * k, features] holds row t of x for each of token t's experts, sorted by expert, ties in the order of tokens and of their places; rows behind the last one that
     has an expert are zeros.  Differentiable in x (float16, bfloat16 or float32): the gradients of a token's rows are summed in float32."""
-    from . import _ext
+    _ext = _package._ext
     _refuse_unseen(x)
     differentiates = _differentiates(x)
     if _ext is not None:
@@ -162,7 +166,7 @@ def expert_sort(x, index, experts):
 def expert_combine(rows, plan, weights=None, dtype=None):
     """out[t] = sum over token t's experts of weights[t, j] * (its row among the sorted ones), in float32, rounded once; without weights all are 1.  weights: [tokens, k], float32 (other float types
     are converted).  dtype: of out, the rows' type by default; float32 rows may be summed to float16 or bfloat16.  Differentiable in rows and weights."""
-    from . import _ext
+    _ext = _package._ext
     differentiates = _differentiates(rows)
     if weights is None:
         _refuse_unseen(rows)

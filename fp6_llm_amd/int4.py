@@ -3,9 +3,13 @@ one scale a row.)  Activations and scales are float16 or bfloat16; products are 
 
 The functions enqueue on the current stream and check shapes, types and devices on the host, like linear_forward_native; what they compute is in include/fp6mi.h.  They go through the torch extension
 where it is built, else through ctypes."""
+import sys
+
 import torch
 
 from . import _lib, ops
+
+_package = sys.modules[__package__]   # (an attribute of it takes a tenth of the time of an import in a call)
 
 TYPES = {torch.float16: 0, torch.bfloat16: 1}
 
@@ -75,7 +79,7 @@ def int4_forward_native(in_feats, native_weight, native_scales, plan=None, activ
     rows are in pair order (16 rows of gate, the same 16 of up, and so on: gate_up_pairs).
     plan: that of expert_sort or expert_plan, for the weights of experts [E, ...] (bias [E, OC]): rows sorted by expert, each multiplied with its expert's weights; rows behind those come out as zeros.
     in_feats has the scales' type, out too or (out_dtype) float32.  workspace: float32, of fp6mi_int4_workspace_bytes (many bfloat16 rows need one).  Not part of an autograd graph."""
-    from . import _ext
+    _ext = _package._ext
     act = -1 if activation is None else ops._activation_code(activation)
     f32 = out_dtype == torch.float32
     if out_dtype is not None and not f32 and out_dtype != native_scales.dtype:
