@@ -77,9 +77,9 @@ def lib():
         "fp6mi_int4_pack": (ci, [vp, vp, vp, vp, vp, ci, sz, sz, sz, sz]),
         "fp6mi_int4_pack_gpu": (ci, [vp, vp, vp, vp, vp, vp, ci, sz, sz, sz, sz]),
         "fp6mi_int4_linear": (ci, [vp, ci, vp, vp, ci, ci, vp, vp, vp, ci, ci, vp, sz, sz, sz, sz, vp]),
-        "fp6mi_int4_workspace_bytes": (sz, [ci, sz, ci, sz, sz, sz, ci, ci]),
+        "fp6mi_int4_workspace_bytes": (sz, [ci, ci, sz, ci, sz, sz, sz, ci, ci]),
         "fp6mi_int4_linear_cfg": (ci, [vp, ci, vp, vp, ci, ci, vp, vp, vp, ci, ci, vp, sz, sz, sz, sz, vp, ci]),
-        "fp6mi_int4_query_kernel": (ci, [ci, sz, ci, sz, sz, sz, ci, ctypes.POINTER(ci)]),
+        "fp6mi_int4_query_kernel": (ci, [ci, ci, sz, ci, sz, sz, sz, ci, ctypes.POINTER(ci)]),
         "fp6mi_expert_sort_workspace_bytes": (sz, [sz, sz, sz]),
         "fp6mi_expert_sort": (ci, [vp, vp, ci, vp, vp, vp, vp, sz, vp, sz, sz, sz, sz, ci, vp]),
         "fp6mi_expert_combine": (ci, [vp, vp, vp, vp, vp, vp, sz, sz, sz, ci, ci]),

@@ -312,8 +312,8 @@ template <int GPB, bool Z, int RT, int WK> int launch_stream(hipStream_t st, con
 }
 
 #if FP6MI_TYPE == 1 && FP6MI_GROUPS == 1
-// Rows in bf16 as fp16 times a power of two for each row, which puts the largest finite magnitude from 2^14 to 2^15.  What is smaller than 2^-29 of that loses bits, at most 2^-40 of it: a float32 sum of such
-// products has been rounded by more.  Infinities and NaN stay.  A workgroup to a row, which reads it twice (from L2); 4096 rows of 4096 take 15.4 us, 4.4 TB/s.
+// Rows in bf16 as fp16 times a power of two for each row, which puts the largest finite magnitude from 2^15 to 2^16 (65280 at most: eight bits).  What is smaller than 2^-32 of that loses bits, half of 2^-24
+// and so 2^-40 of it at most: a float32 sum of such products has been rounded by more.  Infinities and NaN stay.  A workgroup to a row, which reads it twice (from L2); 4096 rows of 4096 take 15.4 us, 4.4 TB/s.
 __global__ __launch_bounds__(256) void rows_to_halfs(half_t *__restrict__ out, int *__restrict__ exponents, const T *__restrict__ X, uint32_t K)
 {
     __shared__ uint32_t most[4];
@@ -338,7 +338,7 @@ __global__ __launch_bounds__(256) void rows_to_halfs(half_t *__restrict__ out, i
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < 4; w++) top = top > most[w] ? top : most[w];
-    const int e = top ? (int)(top >> 7 > 1 ? top >> 7 : 1) - 127 - 14 : 0;
+    const int e = top ? (int)(top >> 7 > 1 ? top >> 7 : 1) - 127 - 15 : 0;
     if (tid == 0) exponents[blockIdx.x] = e;
     for (uint32_t i = tid; i < pieces; i += 256) {
         const v4u v = x[i];
@@ -354,22 +354,26 @@ __global__ __launch_bounds__(256) void rows_to_halfs(half_t *__restrict__ out, i
 #endif
 
 // ---------------------------------------------------------------------------------------------------------------
-// More rows: tiles of WR * 64 weight rows x NT * 16 rows of X to a workgroup of WR x WK wavefronts; the WK groups take every WK-th column block.  X goes to LDS by direct transfers, a K block ahead, two
+// More rows: tiles of WR * RT row tiles x NT * 16 rows of X to a workgroup of WR x WK wavefronts; the WK groups take every WK-th column block.  X goes to LDS by direct transfers, a K block ahead, two
 // stages to a group; a row of a stage is 256 bytes whose 16 pieces stand in the order piece ^ (row & 15), which gives the reads of an MFMA operand all banks.  A wavefront holds its X of one block in
-// registers and takes one of its four row tiles after another: its codes become operands while the tile before is multiplied.  Bound by the matrix units with the conversions and the scaling of the
-// group sums beside them (3.6 VALU instructions to a matrix instruction; twice the columns to a wavefront, 2.6, was no faster, nor were 32x32x16 instructions, which draw more power): 8192x8192 at 777 rows takes
-// 108 to 112 us, 8 experts of 22016x4096 at 4096 rows 720 to 740, 1.0 PFLOP/s, where a library's product of large dense fp16 matrices reaches 1.2.  Two workgroups to a CU where LDS allows, so that one multiplies while the other waits at its barrier.
+// registers and takes one of its RT row tiles after another: its codes become operands while the tile before is multiplied.
+// Many rows are bound by the matrix units with the conversions and the scaling of the group sums beside them (3.6 VALU instructions to a matrix instruction; twice the columns to a wavefront, 2.6, was no
+// faster, nor were 32x32x16 instructions, which draw more power): 8192x8192 at 777 rows takes 108 to 114 us, 8 experts of 22016x4096 at 4096 rows 720 to 750, 1.0 PFLOP/s, where a library's product of large
+// dense fp16 matrices reaches 1.2.  Two workgroups to a CU where LDS allows, so that one multiplies while the other waits at its barrier.
+// 17 to some 100 rows are bound by what a CU takes of the weights, some 20 bytes a ns, so that their tiles are as many as there are CUs, of two, three, four, six or eight row tiles (10240x4576 at 19 rows:
+// 13.0 us in 160 workgroups of four row tiles, 11.1 in 214 of three; 8192x8192: 20.2 in 128 of four, 14.9 in 256 of two; more stages or blocks ahead did nothing).
 // ---------------------------------------------------------------------------------------------------------------
-template <int NT, int WR, int WK> constexpr size_t tile_lds_bytes() // the stages; the sums of the groups on their way to the first; the outputs on their way out (a half at a time where they are float32)
+template <int RT, int NT, int WR, int WK> constexpr size_t tile_lds_bytes() // the stages; the sums of the groups on their way to the first; the outputs on their way out (a half at a time where they are float32)
 {
-    const size_t stages = (size_t)WK * 2 * NT * 4096, sums = (size_t)(WK - 1) * WR * NT * 4096, outputs = NT * 16 * ((size_t)WR * 128 + 16);
+    const size_t stages = (size_t)WK * 2 * NT * 4096, sums = (size_t)(WK - 1) * WR * RT * NT * 1024, outputs = NT * 16 * ((size_t)WR * RT * 32 + 16);
     return stages > outputs ? (stages > sums ? stages : sums) : (outputs > sums ? outputs : sums);
 }
 
-template <int GPB, bool Z, int NT, int WR, int WK> __global__ __launch_bounds__(WR *WK * 64, 2) void int4_tile(const Int4Args a, uint32_t col_tiles)
+template <int GPB, bool Z, int RT, int NT, int WR, int WK> __global__ __launch_bounds__(WR *WK * 64, 2) void int4_tile(const Int4Args a, uint32_t col_tiles)
 {
-    static_assert(NT == 2 || NT == 4, "the steps of a block are written for these");
-    constexpr int      RT = 4, kWaves = WR * WK, kCols = NT * 16, kTiles = WR * RT, kRows = kTiles * 16, kStage = kCols * 256, kDma = kCols / 4 / WR;
+    static_assert((NT == 2 && RT >= 2 && RT <= 4) || (NT == 4 && RT == 4), "the steps of a block are written for these");
+    constexpr int      A = WR == 1 && RT < 4 ? 2 : 1; // blocks of codes on their way: two where a wavefront asks for few at a time (10240x4576 at 19 rows 11.6 -> 11.1 us; 1 to 4 % slower elsewhere)
+    constexpr int      kWaves = WR * WK, kCols = NT * 16, kTiles = WR * RT, kRows = kTiles * 16, kStage = kCols * 256, kDma = kCols / 4 / WR;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, q = lane >> 4, wr = wave % WR, wk = wave / WR;
 
@@ -409,28 +413,28 @@ template <int GPB, bool Z, int NT, int WR, int WK> __global__ __launch_bounds__(
     const auto     wbuf = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(static_cast<const uint8_t *>(a.W) + at * 1024), 0, (int)(tiles * a.KB * 1024), 0x00027000);
     constexpr int  kScaleBytes = sizeof(Scales<GPB, Z>) * 16;
     const auto     sbuf = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(static_cast<const uint8_t *>(a.S) + at * kScaleBytes), 0, (int)(tiles * a.KB * kScaleBytes), 0x00027000);
-    v4u            raw[RT];
-    Scales<GPB, Z> scales[RT];
-    auto           load_w = [&](int r, uint32_t kb) __attribute__((always_inline)) {
+    v4u            raw[A][RT];
+    Scales<GPB, Z> scales[A][RT];
+    auto           load_w = [&](int set, int r, uint32_t kb) __attribute__((always_inline)) {
         const uint32_t block = (r < (int)tiles ? r : tiles - 1) * a.KB + (kb < a.KB ? kb : a.KB - 1);
-        raw[r] = __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(wbuf, lane * 16, block * 1024, 0));
-        if constexpr (sizeof(scales[r]) == 2) scales[r] = __builtin_bit_cast(Scales<GPB, Z>, __builtin_amdgcn_raw_buffer_load_b16(sbuf, c * 2, block * kScaleBytes, 0));
-        if constexpr (sizeof(scales[r]) == 4) scales[r] = __builtin_bit_cast(Scales<GPB, Z>, __builtin_amdgcn_raw_buffer_load_b32(sbuf, c * 4, block * kScaleBytes, 0));
-        if constexpr (sizeof(scales[r]) == 8) scales[r] = __builtin_bit_cast(Scales<GPB, Z>, __builtin_amdgcn_raw_buffer_load_b64(sbuf, c * 8, block * kScaleBytes, 0));
-        if constexpr (sizeof(scales[r]) == 16) scales[r] = __builtin_bit_cast(Scales<GPB, Z>, __builtin_amdgcn_raw_buffer_load_b128(sbuf, c * 16, block * kScaleBytes, 0));
+        raw[set][r] = __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(wbuf, lane * 16, block * 1024, 0));
+        if constexpr (sizeof(scales[set][r]) == 2) scales[set][r] = __builtin_bit_cast(Scales<GPB, Z>, __builtin_amdgcn_raw_buffer_load_b16(sbuf, c * 2, block * kScaleBytes, 0));
+        if constexpr (sizeof(scales[set][r]) == 4) scales[set][r] = __builtin_bit_cast(Scales<GPB, Z>, __builtin_amdgcn_raw_buffer_load_b32(sbuf, c * 4, block * kScaleBytes, 0));
+        if constexpr (sizeof(scales[set][r]) == 8) scales[set][r] = __builtin_bit_cast(Scales<GPB, Z>, __builtin_amdgcn_raw_buffer_load_b64(sbuf, c * 8, block * kScaleBytes, 0));
+        if constexpr (sizeof(scales[set][r]) == 16) scales[set][r] = __builtin_bit_cast(Scales<GPB, Z>, __builtin_amdgcn_raw_buffer_load_b128(sbuf, c * 16, block * kScaleBytes, 0));
     };
     constexpr int kEach = 4 / GPB; // matrix instructions of a group
     Codes         op[2][4];
     Zero          zero;
     const Cutter  cut;
     float         scale[2][GPB];
-    auto          convert = [&](int to, int r, int i, int half) __attribute__((always_inline)) {
-        if (half == 0 && i % kEach == 0) zero.set(Z ? scales[r].v[i / kEach * 2 + 1] : (T)8.f);
-        codes_half(op[to][i], raw[r][i], zero, cut, half);
+    auto          convert = [&](int set, int to, int r, int i, int half) __attribute__((always_inline)) {
+        if (half == 0 && i % kEach == 0) zero.set(Z ? scales[set][r].v[i / kEach * 2 + 1] : (T)8.f);
+        codes_half(op[to][i], raw[set][r][i], zero, cut, half);
     };
-    auto take_scales = [&](int to, int r) __attribute__((always_inline)) {
+    auto take_scales = [&](int set, int to, int r) __attribute__((always_inline)) {
 #pragma unroll
-        for (int g = 0; g < GPB; g++) scale[to][g] = (float)scales[r].v[Z ? 2 * g : g];
+        for (int g = 0; g < GPB; g++) scale[to][g] = (float)scales[set][r].v[Z ? 2 * g : g];
     };
     v4f sum[RT][NT], y[2][2];
 #pragma unroll
@@ -439,21 +443,22 @@ template <int GPB, bool Z, int NT, int WR, int WK> __global__ __launch_bounds__(
         for (int n = 0; n < NT; n++) sum[r][n] = (v4f){ 0.f, 0.f, 0.f, 0.f };
     y[1][0] = y[1][1] = (v4f){ 0.f, 0.f, 0.f, 0.f };
 #pragma unroll
-    for (int g = 0; g < GPB; g++) scale[(RT - 1) & 1][g] = 0.f;
+    for (int g = 0; g < GPB; g++) scale[1][g] = 0.f;
 
     // A block is RT * NT / 2 steps of two tiles of X by one row tile; a step also converts its share of the next row tile, adds up the groups that the step before has multiplied, and reads some of the
     // next block's X.  The last row tile takes the early tiles of X last, so that the registers of the others are free for the next block's.
     constexpr int kPairs = NT / 2, kSteps = RT * kPairs;
     auto          step = [&](auto u_c, auto set_c, uint32_t kb) __attribute__((always_inline)) {
-        constexpr int u = decltype(u_c)::value, set = decltype(set_c)::value, r = u / kPairs, p = u % kPairs;
-        constexpr int n = 2 * (r == RT - 1 ? (p + 1) % kPairs : p), next = (r + 1) % RT;
+        constexpr int u = decltype(u_c)::value, set = decltype(set_c)::value, r = u / kPairs, p = u % kPairs, odd = set * RT; // (a block of three row tiles swaps what alternates)
+        constexpr int n = 2 * (r == RT - 1 ? (p + 1) % kPairs : p), next = (r + 1) % RT, nset = A == 1 ? 0 : r + 1 < RT ? set : set ^ 1;
         constexpr int pu = u == 0 ? kSteps - 1 : u - 1, pr = pu / kPairs, pn = 2 * (pr == RT - 1 ? (pu % kPairs + 1) % kPairs : pu % kPairs); // the step before
-        if constexpr (u == kPairs) { // the next block's X has landed (behind its transfers come the loads of every row tile), and all have read this one's
-            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(RT) : "memory");
+        constexpr int before = r + odd - (p == 0 ? 1 : 0) + 2;
+        if constexpr (u == kPairs) { // the next block's X has landed (behind its transfers come two loads for every row tile), and all have read this one's
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * RT) : "memory");
             transfer(kb + 2 * WK, set);
             asm volatile("" ::: "memory");
         }
-        constexpr int kReads = NT == 2 ? 4 : 2; // of an early tile's operands in a step
+        constexpr int kReads = RT == 2 ? 8 : NT == 2 ? 4 : 2; // of an early tile's operands in a step
         if constexpr (u >= kPairs && u < kPairs + 8 / kReads) {
 #pragma unroll
             for (int e = (u - kPairs) * kReads; e < (u - kPairs + 1) * kReads; e++) read_x(early[set ^ 1][e / 4][e % 4], e / 4, e % 4, set ^ 1);
@@ -463,46 +468,51 @@ template <int GPB, bool Z, int NT, int WR, int WK> __global__ __launch_bounds__(
             for (int i = 0; i < 8; i++) read_x(late[pn - 2 + i / 4][i % 4], pn + i / 4, i % 4, set ^ 1);
         }
         // of the groups multiplied before: pair v of them, tiles n and n + 1 of X by row tile r, from tile `from` of the two on
-        auto add = [&](int r, int n, int g, int v, int from, int to) __attribute__((always_inline)) {
+        auto add = [&](int r, int s, int n, int g, int v, int from, int to) __attribute__((always_inline)) {
 #pragma unroll
             for (int k = from; k < to; k++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) sum[r][n + k][i] += scale[r & 1][g] * y[v & 1][k][i];
+                for (int i = 0; i < 4; i++) sum[r][n + k][i] += scale[s & 1][g] * y[v & 1][k][i];
         };
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const int v = u * GPB + i / kEach;
+            const int v = (u + odd) * GPB + i / kEach;
 #pragma unroll
             for (int k = 0; k < 2; k++)
-                y[v & 1][k] = mfma_halfs(n == 0 ? early[set][k][i] : late[n == 0 ? 0 : n - 2 + k][i], op[r & 1][i].v, i % kEach == 0 ? (v4f){ 0.f, 0.f, 0.f, 0.f } : y[v & 1][k]);
+                y[v & 1][k] = mfma_halfs(n == 0 ? early[set][k][i] : late[n == 0 ? 0 : n - 2 + k][i], op[(r + odd) & 1][i].v, i % kEach == 0 ? (v4f){ 0.f, 0.f, 0.f, 0.f } : y[v & 1][k]);
             if constexpr (GPB == 1) {
-                if (i == 1 || i == 2) add(pr, pn, 0, v + 1, i - 1, i);
+                if (i == 1 || i == 2) add(pr, before, pn, 0, v + 1, i - 1, i);
             } else if constexpr (GPB == 2) {
-                if (i == 1) add(pr, pn, 1, v + 1, 0, 2);
-                if (i == 3) add(r, n, 0, v + 1, 0, 2);
+                if (i == 1) add(pr, before, pn, 1, v + 1, 0, 2);
+                if (i == 3) add(r, r + odd, n, 0, v + 1, 0, 2);
             } else {
                 if (i == 0)
-                    add(pr, pn, 3, v + 1, 0, 2);
+                    add(pr, before, pn, 3, v + 1, 0, 2);
                 else
-                    add(r, n, i - 1, v + 1, 0, 2);
+                    add(r, r + odd, n, i - 1, v + 1, 0, 2);
             }
             if constexpr (kPairs == 2) {
-                convert((r + 1) & 1, next, p * 2 + i / 2, i & 1);
+                convert(nset, (r + odd + 1) & 1, next, p * 2 + i / 2, i & 1);
             } else {
-                convert((r + 1) & 1, next, i, 0);
-                convert((r + 1) & 1, next, i, 1);
+                convert(nset, (r + odd + 1) & 1, next, i, 0);
+                convert(nset, (r + odd + 1) & 1, next, i, 1);
             }
             if (i < 3) __builtin_amdgcn_sched_barrier(0);
         }
         if constexpr (p == kPairs - 1) {
-            take_scales((r + 1) & 1, next);
-            load_w(next, kb + (r + 1 < RT ? WK : 2 * WK));
+            take_scales(nset, (r + odd + 1) & 1, next);
+            if constexpr (A == 2) { // (the codes and scales are used before their registers are loaded again, or they would be loaded to others and waited for at the loop's end to be moved)
+#pragma unroll
+                for (int g = 0; g < GPB; g++) asm volatile("" : "+v"(scale[(r + odd + 1) & 1][g]));
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            load_w(nset, next, kb + (r + 1 < RT ? A : A + 1) * WK);
         }
         __builtin_amdgcn_sched_barrier(0);
     };
     auto block = [&](auto set_c, uint32_t kb) __attribute__((always_inline)) { sections<kSteps>([&](auto u_c) __attribute__((always_inline)) { step(u_c, set_c, kb); }); };
     transfer(wk, 0);
-    load_w(0, wk);
+    load_w(0, 0, wk);
     asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
     transfer(wk + WK, 1);
     asm volatile("" ::: "memory");
@@ -511,20 +521,26 @@ template <int GPB, bool Z, int NT, int WR, int WK> __global__ __launch_bounds__(
 #pragma unroll
     for (int i = 0; i < 4 * (NT - 2); i++) read_x(late[i / 4][i % 4], 2 + i / 4, i % 4, 0);
 #pragma unroll
-    for (int i = 0; i < 8; i++) convert(0, 0, i / 2, i & 1);
-    take_scales(0, 0);
+    for (int i = 0; i < 8; i++) convert(0, 0, 0, i / 2, i & 1);
+    take_scales(0, 0, 0);
 #pragma unroll
-    for (int r = 0; r < RT; r++) load_w(r, r == 0 ? wk + WK : wk);
+    for (int set = 0; set < A; set++)
+#pragma unroll
+        for (int r = 0; r < RT; r++) load_w(set, r, set == 0 && r == 0 ? wk + A * WK : wk + set * WK);
     uint32_t kb = wk, left = (a.KB + WK - 1) / WK; // blocks of every group (of those beyond the last one X reads as zeros)
     for (; left >= 2; left -= 2, kb += 2 * WK) {
         block(std::integral_constant<int, 0>{}, kb);
         block(std::integral_constant<int, 1>{}, kb + WK);
     }
     if (left) block(std::integral_constant<int, 0>{}, kb);
+    const bool swapped = RT % 2 == 1 && left; // (of three row tiles an odd number of blocks)
 #pragma unroll
     for (int k = 0; k < 2; k++) // the last pair
 #pragma unroll
-        for (int i = 0; i < 4; i++) sum[RT - 1][k][i] += scale[(RT - 1) & 1][GPB - 1] * y[1][k][i];
+        for (int i = 0; i < 4; i++) {
+            const float last = swapped ? scale[0][GPB - 1] * y[GPB % 2 == 1 ? 0 : 1][k][i] : scale[1][GPB - 1] * y[1][k][i];
+            sum[RT - 1][k][i] += last;
+        }
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); // nothing is on its way to LDS any more
 
     if constexpr (WK > 1) { // the sums of the other groups to the first, [group][row wavefront][r][n][lane]
@@ -553,7 +569,7 @@ template <int GPB, bool Z, int NT, int WR, int WK> __global__ __launch_bounds__(
         typedef decltype(type) O;
         constexpr bool     gated = decltype(gated_c)::value;
         constexpr uint32_t kHalves = sizeof(O) == 4 && !gated ? 2 : 1, kOut = gated ? kRows / 2 : kRows, kPitch = kOut * sizeof(O) + 16, kEach = 16 / sizeof(O), kNs = NT / kHalves;
-        static_assert((size_t)kCols / kHalves * kPitch <= tile_lds_bytes<NT, WR, WK>(), "");
+        static_assert((size_t)kCols / kHalves * kPitch <= tile_lds_bytes<RT, NT, WR, WK>(), "");
         const uint32_t ld = a.Mt * (gated ? 8 : 16), col0 = m0 * (gated ? 8 : 16);
 #pragma unroll
         for (uint32_t h = 0; h < kHalves; h++) {
@@ -588,7 +604,7 @@ template <int GPB, bool Z, int NT, int WR, int WK> __global__ __launch_bounds__(
             out(float{}, std::false_type{});
         else
             out(T{}, std::false_type{});
-    } else {
+    } else if constexpr (RT % 2 == 0) {
         if (a.out_f32)
             out(float{}, std::true_type{});
         else
@@ -596,14 +612,14 @@ template <int GPB, bool Z, int NT, int WR, int WK> __global__ __launch_bounds__(
     }
 }
 
-template <int GPB, bool Z, int NT, int WR, int WK> int launch_tile(hipStream_t st, const Int4Args &a)
+template <int GPB, bool Z, int RT, int NT, int WR, int WK> int launch_tile(hipStream_t st, const Int4Args &a)
 {
-    constexpr size_t bytes = tile_lds_bytes<NT, WR, WK>();
-    const size_t     cols = fp6mi::int4_tiles(a.N, a.offsets ? a.E : 0, NT * 16), rows = (a.Mt + WR * 4 - 1) / (WR * 4);
+    constexpr size_t bytes = tile_lds_bytes<RT, NT, WR, WK>();
+    const size_t     cols = fp6mi::int4_tiles(a.N, a.offsets ? a.E : 0, NT * 16), rows = (a.Mt + WR * RT - 1) / (WR * RT);
     if (cols * rows > 0x7fffffffu) return FP6MI_ERR_SHAPE;
     if constexpr (bytes > 65536)
-        if (const int e = allow_dynamic_lds<int4_tile<GPB, Z, NT, WR, WK>>(bytes)) return e;
-    hipLaunchKernelGGL((int4_tile<GPB, Z, NT, WR, WK>), dim3((uint32_t)(cols * rows)), dim3(WR * WK * 64), bytes, st, a, (uint32_t)cols);
+        if (const int e = allow_dynamic_lds<int4_tile<GPB, Z, RT, NT, WR, WK>>(bytes)) return e;
+    hipLaunchKernelGGL((int4_tile<GPB, Z, RT, NT, WR, WK>), dim3((uint32_t)(cols * rows)), dim3(WR * WK * 64), bytes, st, a, (uint32_t)cols);
     return (int)hipGetLastError();
 }
 
@@ -612,13 +628,20 @@ template <int GPB, bool Z> int run(hipStream_t st, const Int4Args &a, int kernel
     switch (kernel) { // (in the order of fp6mi::kInt4Kernels)
     case 0: return launch_stream<GPB, Z, 1, 16>(st, a);
     case 1: return launch_stream<GPB, Z, 2, 8>(st, a);
-    case 2: return launch_stream<GPB, Z, 4, 8>(st, a);
-    case 3: return launch_stream<GPB, Z, 4, 4>(st, a);
-    case 4: return launch_tile<GPB, Z, 2, 1, 4>(st, a);
-    case 5: return launch_tile<GPB, Z, 2, 2, 4>(st, a);
-    case 6: return launch_tile<GPB, Z, 2, 2, 2>(st, a);
-    case 7: return launch_tile<GPB, Z, 4, 2, 2>(st, a);
-    case 8: return launch_tile<GPB, Z, 4, 4, 1>(st, a);
+    case 2: return launch_stream<GPB, Z, 3, 8>(st, a);
+    case 3: return launch_stream<GPB, Z, 4, 8>(st, a);
+    case 4: return launch_stream<GPB, Z, 4, 4>(st, a);
+    case 5: return launch_tile<GPB, Z, 2, 2, 1, 8>(st, a);
+    case 6: return launch_tile<GPB, Z, 3, 2, 1, 4>(st, a);
+    case 7: return launch_tile<GPB, Z, 4, 2, 1, 4>(st, a);
+    case 8: return launch_tile<GPB, Z, 2, 2, 2, 4>(st, a);
+    case 9: return launch_tile<GPB, Z, 3, 2, 2, 4>(st, a);
+    case 10: return launch_tile<GPB, Z, 4, 2, 2, 4>(st, a);
+    case 11: return launch_tile<GPB, Z, 4, 2, 2, 2>(st, a);
+    case 12:
+        if constexpr (GPB == 1) return launch_tile<GPB, Z, 4, 4, 2, 2>(st, a);
+        break;
+    case 13: return launch_tile<GPB, Z, 4, 4, 4, 1>(st, a);
     }
     return FP6MI_ERR_SHAPE;
 }

@@ -72,13 +72,15 @@ int check_pack(const void *native, const void *native_scales, const void *codes,
 
 // Which kernel takes a product (an index of kInt4Kernels): the fastest by this model of its time, us.  A workgroup's column blocks one after another take `step` each while every CU has one at the most,
 // `share` times the workgroups of a CU beyond; and no kernel reads the weights faster than memory.  Rows of experts are taken to be spread evenly, with half a tile to spare for each expert.
-// Fitted to 2344 times of 265 products in graphs, weights from HBM (512x2048 to 28672x8192 at 1 to 777 rows, 8 to 128 experts at 1 to 700 tokens, fp16 and bf16): a kernel's own time is off by 15 to 26 % rms,
-// the choice takes 1.01 times the fastest measured in the mean, at worst 1.29; for 126 other products 1.02 and 1.55.
+// Fitted to 3734 times of 281 products in graphs, weights from HBM (512x2048 to 28672x8192 at 1 to 777 rows, 8 to 128 experts at 1 to 700 tokens, fp16 and bf16): a kernel's own time is off by 13 to 33 % rms,
+// the choice takes 1.01 times the fastest measured in the mean, at worst 1.43; for 126 other products 1.02 and 1.31.
 struct Times { double base, step, share, rows; }; // rows: how much longer a step takes with 16 rows than with none, of the kernel that streams weights
-constexpr Times kTimes[] = { { 1.84, 0.86, 1.51, 0.43 }, { 2.20, 1.07, 1.09, 0.18 }, { 2.42, 1.59, 1.97, 0 }, { 2.71, 1.10, 0.74, 0 }, { 3.35, 1.07, 1.10, 0 }, { 3.27, 1.50, 2.10, 0 },
-                             { 3.83, 1.06, 0.99, 0 },    { 2.94, 1.36, 1.62, 0 },    { 2.95, 1.05, 1.09, 0 } };
+constexpr Times kTimes[] = { { 1.60, 0.64, 1.45, 0.49 }, { 1.74, 1.03, 1.04, 0.28 }, { 2.63, 1.21, 1.35, 0.25 }, { 1.70, 1.95, 2.08, 0 }, { 2.36, 1.15, 0.75, 0 },
+                             { 3.67, 1.41, 1.69, 0 },    { 3.33, 0.97, 1.00, 0 },    { 4.28, 1.12, 1.17, 0 },    { 2.38, 1.10, 1.27, 0 }, { 3.57, 1.36, 1.55, 0 },
+                             { 2.62, 1.70, 2.14, 0 },    { 2.66, 1.09, 1.02, 0 },    { 2.53, 1.31, 1.61, 0 },    { 2.11, 1.08, 1.13, 0 } };
 
 constexpr int    kKernels = sizeof(kTimes) / sizeof(kTimes[0]);
+static_assert(kKernels == sizeof(fp6mi::kInt4Kernels) / sizeof(fp6mi::kInt4Kernels[0]), "");
 constexpr size_t kMostTileColumns = (size_t)1 << 20; // (offsets in a tile have 32 bits)
 
 double time_of(int kernel, int dtype, size_t experts, bool grouped, size_t M, size_t N, size_t K)
@@ -94,12 +96,19 @@ double time_of(int kernel, int dtype, size_t experts, bool grouped, size_t M, si
     return std::max(us, used * M * K * 0.515 / 5.1e6 + 1.5);
 }
 
-int choice(int dtype, size_t experts, bool grouped, size_t M, size_t N, size_t K, bool gated)
+// Whether a kernel has the problem.
+bool lacks(int kernel, int group, size_t K, bool gated)
+{
+    const fp6mi::Int4Kernel &k = fp6mi::kInt4Kernels[kernel];
+    return (k.tile && K > kMostTileColumns) || (gated && !k.pairs) || (k.group128 && group != 128);
+}
+
+int choice(int dtype, int group, size_t experts, bool grouped, size_t M, size_t N, size_t K, bool gated)
 {
     int       best = -1;
     double    least = 0;
     for (int k = 0; k < kKernels; k++) {
-        if ((fp6mi::kInt4Kernels[k].tile && K > kMostTileColumns) || (gated && fp6mi::kInt4Kernels[k].row_tiles % 2)) continue; // (gate and up are two row tiles)
+        if (lacks(k, group, K, gated)) continue;
         const size_t tiles = fp6mi::int4_tiles(N, grouped ? experts : 0, fp6mi::kInt4Kernels[k].cols);
         if (!fp6mi::kInt4Kernels[k].tile && tiles > 65535) continue; // (a grid dimension)
         const double us = time_of(k, dtype, experts, grouped, M, N, K);
@@ -151,17 +160,17 @@ int fp6mi_int4_pack_gpu(void *stream, void *native, void *native_scales, const v
     return (int)hipGetLastError();
 }
 
-size_t fp6mi_int4_workspace_bytes(int dtype, size_t experts, int grouped, size_t M, size_t N, size_t K, int gated, int kernel)
+size_t fp6mi_int4_workspace_bytes(int dtype, int group, size_t experts, int grouped, size_t M, size_t N, size_t K, int gated, int kernel)
 {
-    if ((dtype != 0 && dtype != 1) || check_shape(experts, M, K) || N == 0 || N > (size_t)1 << 30 || kernel >= kKernels) return 0;
-    return scratch_bytes(dtype, kernel >= 0 ? kernel : choice(dtype, experts, grouped != 0, M, N, K, gated != 0), N, K);
+    if ((dtype != 0 && dtype != 1) || (group != 32 && group != 64 && group != 128) || check_shape(experts, M, K) || N == 0 || N > (size_t)1 << 30 || kernel >= kKernels) return 0;
+    return scratch_bytes(dtype, kernel >= 0 ? kernel : choice(dtype, group, experts, grouped != 0, M, N, K, gated != 0), N, K);
 }
 
-int fp6mi_int4_query_kernel(int dtype, size_t experts, int grouped, size_t M, size_t N, size_t K, int gated, int *shape)
+int fp6mi_int4_query_kernel(int dtype, int group, size_t experts, int grouped, size_t M, size_t N, size_t K, int gated, int *shape)
 {
     if (dtype != 0 && dtype != 1) return FP6MI_ERR_TYPE;
-    if (check_shape(experts, M, K) || N == 0 || N > (size_t)1 << 30) return FP6MI_ERR_SHAPE;
-    const int k = choice(dtype, experts, grouped != 0, M, N, K, gated != 0);
+    if ((group != 32 && group != 64 && group != 128) || check_shape(experts, M, K) || N == 0 || N > (size_t)1 << 30) return FP6MI_ERR_SHAPE;
+    const int k = choice(dtype, group, experts, grouped != 0, M, N, K, gated != 0);
     if (k < 0) return FP6MI_ERR_SHAPE;
     const fp6mi::Int4Kernel &c = fp6mi::kInt4Kernels[k];
     if (shape) shape[0] = c.tile, shape[1] = c.cols, shape[2] = c.row_tiles, shape[3] = c.k_split;
@@ -179,8 +188,8 @@ int fp6mi_int4_linear_cfg(void *stream, int dtype, const void *W_native, const v
     if (N == 0) return FP6MI_OK;
     if (!W_native || !scales_native || !X || !Y) return FP6MI_ERR_NULL;
     if (!aligned(W_native, 16) || !aligned(scales_native, 16) || !aligned(X, 16) || !aligned(Y, 16) || !aligned(bias, 2) || !aligned(offsets, 4) || !aligned(workspace, 16)) return FP6MI_ERR_ALIGN;
-    if (kernel < 0) kernel = choice(dtype, experts, offsets != nullptr, M, N, K, activation >= 0);
-    if (kernel < 0 || (activation >= 0 && fp6mi::kInt4Kernels[kernel].row_tiles % 2) || (fp6mi::kInt4Kernels[kernel].tile && K > kMostTileColumns)) return FP6MI_ERR_SHAPE;
+    if (kernel < 0) kernel = choice(dtype, group, experts, offsets != nullptr, M, N, K, activation >= 0);
+    if (kernel < 0 || lacks(kernel, group, K, activation >= 0)) return FP6MI_ERR_SHAPE;
     fp6mi::Int4Args a = { W_native, scales_native, X, bias, Y, offsets, (uint32_t)N, (uint32_t)K, (uint32_t)((K + 127) / 128), (uint32_t)(M / 16), (uint32_t)experts, activation, out_f32, nullptr };
     if (scratch_bytes(dtype, kernel, N, K)) {
         if (!workspace) return FP6MI_ERR_WORKSPACE;

@@ -622,7 +622,7 @@ at::Tensor int4_forward(const at::Tensor &in_feats, const at::Tensor &native, co
     }
     void      *stream = c10::hip::getCurrentHIPStream(dev.index()).stream();
     at::Tensor keep;
-    float     *ws = type == at::kHalf ? nullptr : scratch(ws_opt, dev, stream, fp6mi_int4_workspace_bytes(1, (size_t)E, grouped, (size_t)OC, (size_t)B, (size_t)IC, act >= 0, -1), keep);
+    float     *ws = type == at::kHalf ? nullptr : scratch(ws_opt, dev, stream, fp6mi_int4_workspace_bytes(1, 128 / (int)s.size(-2), (size_t)E, grouped, (size_t)OC, (size_t)B, (size_t)IC, act >= 0, -1), keep);
     raise_status(fp6mi_int4_linear(stream, type_code(type), native.data_ptr(), s.data_ptr(), 128 / (int)s.size(-2), (int)s.size(-1) - 1, pointer(bias), x.data_ptr(), out.data_ptr(), f32, (int)act, offsets,
                                    (size_t)E, (size_t)OC, (size_t)B, (size_t)IC, ws),
                  "fp6mi_int4_linear");

@@ -115,6 +115,6 @@ def int4_forward_native(in_feats, native_weight, native_scales, plan=None, activ
     x = x.contiguous()
     out = ops._result(out, (B, OC // 2 if act >= 0 else OC), dev, dtype=torch.float32 if f32 else s.dtype)
     L = _lib.lib()
-    ops._launch("fp6mi_int4_linear", dev, L.fp6mi_int4_workspace_bytes(TYPES[s.dtype], E, plan is not None, OC, B, IC, act >= 0, -1), workspace, lambda stream, ws: L.fp6mi_int4_linear(
+    ops._launch("fp6mi_int4_linear", dev, L.fp6mi_int4_workspace_bytes(TYPES[s.dtype], 128 // s.shape[-2], E, plan is not None, OC, B, IC, act >= 0, -1), workspace, lambda stream, ws: L.fp6mi_int4_linear(
         stream, TYPES[s.dtype], native_weight.data_ptr(), s.data_ptr(), 128 // s.shape[-2], s.shape[-1] - 1, ops._ptr(bias), x.data_ptr(), out.data_ptr(), f32, act, offsets, E, OC, B, IC, ws))
     return out

@@ -277,13 +277,13 @@ int    fp6mi_int4_pack_gpu(void *stream, void *native, void *native_scales, cons
  * offsets[experts] on become zeros.  Products are exact, sums float32 (of a group before its scale, of the scaled groups behind it), rounded once. */
 int    fp6mi_int4_linear(void *stream, int dtype, const void *W_native, const void *scales_native, int group, int zeros, const void *bias, const void *X, void *Y, int out_f32, int activation,
                          const int *offsets, size_t experts, size_t M, size_t N, size_t K, void *workspace);
-/* The workspace of that product, 16-byte aligned (grouped: with offsets, gated: with an activation): none but for many bf16 rows, which are multiplied as fp16 with a power of two for each row (a value
- * below 2^-29 of its row's largest loses bits, 2^-40 of that at most).  In products of few bf16 rows an infinity in X comes out as NaN.  kernel: -1, or that of fp6mi_int4_linear_cfg. */
-size_t fp6mi_int4_workspace_bytes(int dtype, size_t experts, int grouped, size_t M, size_t N, size_t K, int gated, int kernel);
+/* The workspace of that product, 16-byte aligned (group: the native one, grouped: with offsets, gated: with an activation): none but for many bf16 rows, which are multiplied as fp16 with a power of two for each row (a value
+ * below 2^-32 of its row's largest loses bits, 2^-40 of that at most).  In products of few bf16 rows an infinity in X comes out as NaN.  kernel: -1, or that of fp6mi_int4_linear_cfg. */
+size_t fp6mi_int4_workspace_bytes(int dtype, int group, size_t experts, int grouped, size_t M, size_t N, size_t K, int gated, int kernel);
 /* Which kernel takes it, by its number; shape, unless NULL: [0] 0 for the one that streams weights past few rows, 1 for tiles; rows of X, tiles of 16 weight rows, and K parts of a workgroup.
  * Negative: FP6MI_ERR_*.  Pure host code. */
-int    fp6mi_int4_query_kernel(int dtype, size_t experts, int grouped, size_t M, size_t N, size_t K, int gated, int *shape);
-/* The product by kernel 0 to 8 (-1: the choice).  FP6MI_ERR_SHAPE where it lacks the problem: the tiles (4 to 8) end at K = 2^20, kernel 0 has no gated product.  (Tuning hook.) */
+int    fp6mi_int4_query_kernel(int dtype, int group, size_t experts, int grouped, size_t M, size_t N, size_t K, int gated, int *shape);
+/* The product by kernel 0 to 13 (-1: the choice).  FP6MI_ERR_SHAPE where it lacks the problem: the tiles (5 to 13) end at K = 2^20, kernels 0, 2, 6 and 9 have no gated product, kernel 12 has groups of 128 only.  (Tuning hook.) */
 int    fp6mi_int4_linear_cfg(void *stream, int dtype, const void *W_native, const void *scales_native, int group, int zeros, const void *bias, const void *X, void *Y, int out_f32, int activation,
                              const int *offsets, size_t experts, size_t M, size_t N, size_t K, void *workspace, int kernel);
 

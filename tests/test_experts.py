@@ -8,7 +8,7 @@ import torch
 
 import fp6_llm_amd as fp6
 from fp6_llm_amd import _lib
-from test_int4 import HALF, TINY, Weight, by_kernel, d, gated64, plain, product64, randn, within
+from test_int4 import HALF, TILES, TINY, UNPAIRED, Weight, by_kernel, d, gated64, plain, product64, randn, within
 
 DEV = "cuda:0"
 gpu = pytest.mark.gpu
@@ -498,22 +498,23 @@ def test_gradients_that_are_not_asked_for():
 
 
 @gpu
-@pytest.mark.parametrize("kernel", range(1, 9))
+@pytest.mark.parametrize("kernel", range(14))
 @pytest.mark.parametrize("type", ["fp16", "bf16"])
 def test_every_kernel_with_rows_of_experts(kernel, type):
     """Borders of experts inside tiles, experts without rows, rows behind the last expert's that hold NaN."""
     E, sizes = 5, [3, 0, 40, 17, 129]
     index = torch.tensor([e for e, n in enumerate(sizes) for _ in range(n)] + [-1] * 20).unsqueeze(1).to(DEV)
-    w = Weight(kernel, 96, 416, 64, True, type, E)
+    w = Weight(kernel, 96, 416, 128 if kernel == 12 else 64, True, type, E)
     rows, plan = fp6.expert_sort(randn(2, len(index), 416, dtype=w.dtype), index, E)
     want = Plan64(index, E)
     b = randn(3, E, 96, dtype=w.dtype)
     y, tol = grouped64(w, want, rows, b, None, w.dtype)
     h, htol = grouped64(w, want, rows, b, "silu", w.dtype)
-    extra = 30 if type == "bf16" and kernel < 4 else 1   # (128 + q and -(128 + z), 143 at most, stand for a difference that is 5 in the mean)
+    extra = 30 if type == "bf16" and kernel not in TILES else 1   # (128 + q and -(128 + z), 143 at most, stand for a difference that is 5 in the mean)
     rows[int(want.n):] = float("nan")
     within(by_kernel(kernel, w, rows, b, plan=plan), y, tol * extra)
-    within(by_kernel(kernel, w, rows, b, act=0, plan=plan), h, htol * extra)
+    if kernel not in UNPAIRED:
+        within(by_kernel(kernel, w, rows, b, act=0, plan=plan), h, htol * extra)
 
 
 @gpu
@@ -530,7 +531,7 @@ def test_weights_beyond_32_bit_offsets():
     for T in (3, 70):
         x, index = randn(1, T, IC), torch.full((T, 1), E - 1, device=DEV)
         rows, plan = fp6.expert_sort(x, index, E)
-        k = 3 if T == 3 else 8
+        k = 4 if T == 3 else 13
         both = Weight.__new__(Weight)
         both.native, both.native_scales, both.OC, both.IC, both.E, both.dtype = native, native_scales, OC, IC, E, torch.float16
         alone = Weight.__new__(Weight)
