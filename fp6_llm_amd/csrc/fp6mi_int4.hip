@@ -171,20 +171,23 @@ __device__ __forceinline__ void store_zeros(const Int4Args &a, const Tile &t, ui
 }
 
 // ---------------------------------------------------------------------------------------------------------------
-// Few rows: RT row tiles and 16 rows of X to a workgroup of WK wavefronts, which share K: a wavefront takes every WK-th column block, its weights straight from HBM to registers
-// (the next block's on their way meanwhile) and its part of X from L2; the partial sums meet in LDS.  Bound by the bytes of the weights where there are many (28672x8192: 23.1 us at 1 row, 28.2 at 16, of which
-// the bytes take 23.6; 8192x8192: 9.2 and 12.1 of 6.8), by a wavefront's few blocks one after another where there are few (4096x4096 at 1 row: 4.3 us with 16 wavefronts to a row tile, 5.2 with 8 to two).
-// Three and four blocks on their way were no faster, nor were two tiles of rows of X to a workgroup.
+// Few rows: RT row tiles and 16 rows of X to a workgroup of WK wavefronts, which share K: a wavefront takes every WK-th column block, its weights straight from HBM to registers (the next block's on their
+// way meanwhile) and its part of X from L2; the partial sums meet in LDS.  X is read in whole rows, two blocks ahead, and turned into operands through LDS a block ahead: as operands, 64 bytes of each of 16
+// rows to a load, 8192x8192 at 16 rows took 11.8 us and 28672x8192 27.8, in whole rows 10.5 and 26.2.  (Only the kernel of one row tile, which is for few blocks, reads operands: to turn them
+// takes it 0.4 us, and at one row there is nothing to be won.)
+// Bound by the bytes of the weights where there are many (28672x8192: 23.2 us at 1 row, 26 at 16, of which the bytes take 23.6 at a copy's rate; 8192x8192: 8.5 and 10.5 of 6.8), by a wavefront's few blocks
+// one after another where there are few (4096x4096 at 1 row: 4.3 us with 16 wavefronts to a row tile, 5.4 with 8 to two).  Three and four blocks of weights on their way were no faster, nor were two
+// tiles of rows of X to a workgroup.
 // ---------------------------------------------------------------------------------------------------------------
 template <int GPB, bool Z, int RT> struct Block {
     v4u            w[RT];
     Scales<GPB, Z> s[RT];
-    v8t            x[4];
 };
 
 template <int GPB, bool Z, int RT, int WK> __global__ __launch_bounds__(WK * 64, WK > 4 ? 1 : 2) void int4_stream(const Int4Args a)
 {
-    __shared__ v4f part[WK][RT][64];
+    static_assert(RT <= 4, "");
+    __shared__ v4f shared[WK][RT > 1 ? 4 : 1][64]; // of a wavefront: a block of X on its way into operand order, in the end its sums
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, q = lane >> 4;
     const uint32_t m0 = blockIdx.x * RT;
     const Tile     t = tile_of(a, blockIdx.y, 16);
@@ -199,23 +202,43 @@ template <int GPB, bool Z, int RT, int WK> __global__ __launch_bounds__(WK * 64,
         w[r] = static_cast<const v4u *>(a.W) + at * 64 + lane;
         s[r] = static_cast<const Scales<GPB, Z> *>(a.S) + at * 16 + c;
     }
-    const T *x = static_cast<const T *>(a.X) + (size_t)(t.row + (c < t.rows ? c : t.rows - 1)) * a.K + q * 8;
+    // X: in whole rows, four of 256 bytes to a load, lane c + 16 q with piece c of row 4 i + q, or (one row tile) as operands, piece 4 i + q of row c.  Rows behind the last one: that again.
+    constexpr bool kTurn = RT > 1;
+    const auto     xbuf = __builtin_amdgcn_make_buffer_rsrc(const_cast<T *>(static_cast<const T *>(a.X) + (size_t)t.row * a.K), 0, (int)(t.rows * a.K * 2), 0x00027000);
+    uint32_t       xoff[4], beyond[4]; // (beyond: what puts an offset in the last block behind the buffer, which reads as zeros)
+#pragma unroll
+    for (uint32_t i = 0; i < 4; i++) {
+        const uint32_t row = kTurn ? 4 * i + q : c, piece = kTurn ? c : 4 * i + q;
+        xoff[i] = (row < t.rows ? row : t.rows - 1) * a.K * 2 + piece * 16;
+        beyond[i] = (a.KB - 1) * 128 + piece * 8 < a.K ? 0 : 0x80000000u;
+    }
 
     typedef Block<GPB, Z, RT> B;
     const FewCutter           cut;
     auto load = [&](B &b, uint32_t kb) __attribute__((always_inline)) {
-        const uint32_t steps = (a.K - kb * 128) / 32; // of 32 columns, 4 but for the last block
 #pragma unroll
         for (int r = 0; r < RT; r++) b.w[r] = __builtin_nontemporal_load(w[r] + (size_t)kb * 64);
 #pragma unroll
         for (int r = 0; r < RT; r++) b.s[r] = s[r][(size_t)kb * 16];
+    };
+    auto load_x = [&](v8t(&rows)[4], uint32_t kb) __attribute__((always_inline)) {
+        const uint32_t last = kb + 1 < a.KB ? 0 : ~0u;
+        kb = kb < a.KB ? kb : a.KB - 1;
 #pragma unroll
-        for (uint32_t i = 0; i < 4; i++) b.x[i] = i < steps ? *reinterpret_cast<const v8t *>(x + kb * 128 + i * 32) : v8t{};
+        for (uint32_t i = 0; i < 4; i++) rows[i] = __builtin_bit_cast(v8t, __builtin_amdgcn_raw_buffer_load_b128(xbuf, xoff[i] + (beyond[i] & last), kb * 256, 0));
+    };
+    // rows to operands; in LDS the pieces of a row stand in the order piece ^ row, which gives reads and writes all banks
+    v8t *const stage = reinterpret_cast<v8t *>(shared[wave]);
+    auto       turn = [&](v8t(&x)[4], const v8t(&rows)[4]) __attribute__((always_inline)) {
+#pragma unroll
+        for (uint32_t i = 0; i < 4; i++) stage[(4 * i + q) * 16 + (c ^ (4 * i + q))] = rows[i];
+#pragma unroll
+        for (uint32_t i = 0; i < 4; i++) x[i] = stage[c * 16 + ((4 * i + q) ^ c)];
     };
     v4f sum[RT];
 #pragma unroll
     for (int r = 0; r < RT; r++) sum[r] = (v4f){ 0.f, 0.f, 0.f, 0.f };
-    auto multiply = [&](const B &b) __attribute__((always_inline)) {
+    auto multiply = [&](const B &b, const v8t(&x)[4]) __attribute__((always_inline)) {
         constexpr int kEach = 4 / GPB; // steps of a group
         constexpr bool kSecond = FP6MI_TYPE == 1;
         FewZero        zero;
@@ -226,7 +249,7 @@ template <int GPB, bool Z, int RT, int WK> __global__ __launch_bounds__(WK * 64,
             for (int g = 0; g < GPB; g++) {
                 first[g] = (v4f){ 0.f, 0.f, 0.f, 0.f };
 #pragma unroll
-                for (int i = 0; i < kEach; i++) first[g] = second(b.x[g * kEach + i], zero, first[g]);
+                for (int i = 0; i < kEach; i++) first[g] = second(x[g * kEach + i], zero, first[g]);
             }
         }
 #pragma unroll
@@ -242,40 +265,61 @@ template <int GPB, bool Z, int RT, int WK> __global__ __launch_bounds__(WK * 64,
                 if constexpr (kSecond && !Z) y = first[g];
 #pragma unroll
                 for (int i = 0; i < kEach; i++) {
-                    if constexpr (kSecond && Z) y = second(b.x[g * kEach + i], zero, y);
-                    y = mfma(b.x[g * kEach + i], v[i], y);
+                    if constexpr (kSecond && Z) y = second(x[g * kEach + i], zero, y);
+                    y = mfma(x[g * kEach + i], v[i], y);
                 }
 #pragma unroll
                 for (int i = 0; i < 4; i++) sum[r][i] += scale * y[i];
+                if (kSecond && Z && GPB == 4 && RT == 4 && g == GPB - 1 && r % 2 == 1) __builtin_amdgcn_sched_barrier(0); // (or conversions come so early that registers spill: 16 -> 28 us for 8192x8192)
             }
     };
-    B b[2];
+    B        b[2];
+    v8t      x[2][4], rows[4]; // operands of this block and the next, rows of the one behind it
     uint32_t kb = wave;
+    auto next = [&](v8t(&to)[4], uint32_t kb) __attribute__((always_inline)) {
+        if constexpr (kTurn) {
+            turn(to, rows);
+            load_x(rows, kb + WK);
+        } else {
+            load_x(to, kb);
+        }
+    };
     if (kb < a.KB) {
+        load_x(x[kTurn], kb);
         load(b[0], kb);
+        if constexpr (kTurn) {
+            load_x(rows, kb + WK);
+            turn(x[0], x[1]);
+        }
         for (; kb + 2 * WK < a.KB; kb += 2 * WK) {
             load(b[1], kb + WK);
-            multiply(b[0]);
+            next(x[1], kb + WK);
+            multiply(b[0], x[0]);
             load(b[0], kb + 2 * WK);
-            multiply(b[1]);
+            next(x[0], kb + 2 * WK);
+            multiply(b[1], x[1]);
         }
         if (kb + WK < a.KB) {
             load(b[1], kb + WK);
-            multiply(b[0]);
-            multiply(b[1]);
+            if constexpr (kTurn)
+                turn(x[1], rows);
+            else
+                load_x(x[1], kb + WK);
+            multiply(b[0], x[0]);
+            multiply(b[1], x[1]);
         } else {
-            multiply(b[0]);
+            multiply(b[0], x[0]);
         }
     }
 #pragma unroll
-    for (int r = 0; r < RT; r++) part[wave][r][lane] = sum[r];
+    for (int r = 0; r < RT; r++) shared[wave][r][lane] = sum[r];
     __syncthreads();
 
     // the sums of row tile r: lane c + 16 q has weight row c and rows 4 q + i of X
     auto total = [&](int r) __attribute__((always_inline)) {
-        v4f y = part[0][r][lane];
+        v4f y = shared[0][r][lane];
 #pragma unroll
-        for (int k = 1; k < WK; k++) y += part[k][r][lane];
+        for (int k = 1; k < WK; k++) y += shared[k][r][lane];
         return y;
     };
     const T *bias = a.bias ? static_cast<const T *>(a.bias) + (size_t)t.expert * a.Mt * 16 : nullptr;
@@ -360,8 +404,8 @@ __global__ __launch_bounds__(256) void rows_to_halfs(half_t *__restrict__ out, i
 // Many rows are bound by the matrix units with the conversions and the scaling of the group sums beside them (3.6 VALU instructions to a matrix instruction; twice the columns to a wavefront, 2.6, was no
 // faster, nor were 32x32x16 instructions, which draw more power): 8192x8192 at 777 rows takes 108 to 114 us, 8 experts of 22016x4096 at 4096 rows 720 to 750, 1.0 PFLOP/s, where a library's product of large
 // dense fp16 matrices reaches 1.2.  Two workgroups to a CU where LDS allows, so that one multiplies while the other waits at its barrier.
-// 17 to some 100 rows are bound by what a CU takes of the weights, some 20 bytes a ns, so that their tiles are as many as there are CUs, of two, three, four, six or eight row tiles (10240x4576 at 19 rows:
-// 13.0 us in 160 workgroups of four row tiles, 11.1 in 214 of three; 8192x8192: 20.2 in 128 of four, 14.9 in 256 of two; more stages or blocks ahead did nothing).
+// 17 to some 100 rows are bound by what a CU takes of the weights, some 20 bytes a ns, so that their tiles are as many as there are CUs, of three, four, six or eight row tiles (10240x4576 at 19 rows:
+// 13.0 us in 160 workgroups of four row tiles, 11.1 in 214 of three; more stages or blocks ahead did nothing for the others).
 // ---------------------------------------------------------------------------------------------------------------
 template <int RT, int NT, int WR, int WK> constexpr size_t tile_lds_bytes() // the stages; the sums of the groups on their way to the first; the outputs on their way out (a half at a time where they are float32)
 {
@@ -631,17 +675,15 @@ template <int GPB, bool Z> int run(hipStream_t st, const Int4Args &a, int kernel
     case 2: return launch_stream<GPB, Z, 3, 8>(st, a);
     case 3: return launch_stream<GPB, Z, 4, 8>(st, a);
     case 4: return launch_stream<GPB, Z, 4, 4>(st, a);
-    case 5: return launch_tile<GPB, Z, 2, 2, 1, 8>(st, a);
-    case 6: return launch_tile<GPB, Z, 3, 2, 1, 4>(st, a);
-    case 7: return launch_tile<GPB, Z, 4, 2, 1, 4>(st, a);
-    case 8: return launch_tile<GPB, Z, 2, 2, 2, 4>(st, a);
-    case 9: return launch_tile<GPB, Z, 3, 2, 2, 4>(st, a);
-    case 10: return launch_tile<GPB, Z, 4, 2, 2, 4>(st, a);
-    case 11: return launch_tile<GPB, Z, 4, 2, 2, 2>(st, a);
-    case 12:
+    case 5: return launch_tile<GPB, Z, 3, 2, 1, 4>(st, a);
+    case 6: return launch_tile<GPB, Z, 2, 2, 2, 4>(st, a);
+    case 7: return launch_tile<GPB, Z, 3, 2, 2, 4>(st, a);
+    case 8: return launch_tile<GPB, Z, 4, 2, 2, 4>(st, a);
+    case 9: return launch_tile<GPB, Z, 4, 2, 2, 2>(st, a);
+    case 10:
         if constexpr (GPB == 1) return launch_tile<GPB, Z, 4, 4, 2, 2>(st, a);
         break;
-    case 13: return launch_tile<GPB, Z, 4, 4, 4, 1>(st, a);
+    case 11: return launch_tile<GPB, Z, 4, 4, 4, 1>(st, a);
     }
     return FP6MI_ERR_SHAPE;
 }

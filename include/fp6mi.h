@@ -283,7 +283,7 @@ size_t fp6mi_int4_workspace_bytes(int dtype, int group, size_t experts, int grou
 /* Which kernel takes it, by its number; shape, unless NULL: [0] 0 for the one that streams weights past few rows, 1 for tiles; rows of X, tiles of 16 weight rows, and K parts of a workgroup.
  * Negative: FP6MI_ERR_*.  Pure host code. */
 int    fp6mi_int4_query_kernel(int dtype, int group, size_t experts, int grouped, size_t M, size_t N, size_t K, int gated, int *shape);
-/* The product by kernel 0 to 13 (-1: the choice).  FP6MI_ERR_SHAPE where it lacks the problem: the tiles (5 to 13) end at K = 2^20, kernels 0, 2, 6 and 9 have no gated product, kernel 12 has groups of 128 only.  (Tuning hook.) */
+/* The product by kernel 0 to 11 (-1: the choice).  FP6MI_ERR_SHAPE where it lacks the problem: the tiles (5 to 11) end at K = 2^20, kernels 0, 2, 5 and 7 have no gated product, kernel 10 has groups of 128 only.  (Tuning hook.) */
 int    fp6mi_int4_linear_cfg(void *stream, int dtype, const void *W_native, const void *scales_native, int group, int zeros, const void *bias, const void *X, void *Y, int out_f32, int activation,
                              const int *offsets, size_t experts, size_t M, size_t N, size_t K, void *workspace, int kernel);
 

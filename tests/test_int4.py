@@ -310,11 +310,11 @@ def test_refusals_of_the_c_abi():
     assert linear(bias=p + 1) == ALIGN and linear(offsets=p + 2) == ALIGN
     assert linear(N=0, X=None, Y=None) == 0 and linear(dtype=1, M=8192, K=8192, N=500) == -4 and linear(ws=p + 8) == ALIGN
     assert L.fp6mi_int4_workspace_bytes(0, 64, 1, 0, 32, 500, 64, 0, 8) == 0 and L.fp6mi_int4_workspace_bytes(1, 64, 1, 0, 32, 500, 64, 0, 8) == 2000 + 500 * 128
-    assert L.fp6mi_int4_workspace_bytes(1, 64, 1, 0, 32, 500, 64, 0, 3) == 0 and L.fp6mi_int4_workspace_bytes(1, 64, 1, 0, 32, 500, 64, 0, 14) == 0 and L.fp6mi_int4_workspace_bytes(1, 64, 1, 0, 32, 0, 64, 0, 8) == 0 and L.fp6mi_int4_workspace_bytes(1, 96, 1, 0, 32, 500, 64, 0, 8) == 0
+    assert L.fp6mi_int4_workspace_bytes(1, 64, 1, 0, 32, 500, 64, 0, 3) == 0 and L.fp6mi_int4_workspace_bytes(1, 64, 1, 0, 32, 500, 64, 0, 12) == 0 and L.fp6mi_int4_workspace_bytes(1, 64, 1, 0, 32, 0, 64, 0, 8) == 0 and L.fp6mi_int4_workspace_bytes(1, 96, 1, 0, 32, 500, 64, 0, 8) == 0
 
     def cfg(kernel, act=-1, K=64):
         return L.fp6mi_int4_linear_cfg(None, 1, p, p, 64, 0, None, p, p, 0, act, None, 1, 32, 2, K, None, kernel)
-    assert cfg(14) == SHAPE and all(cfg(k, act=0) == SHAPE for k in UNPAIRED) and all(cfg(k, K=(1 << 20) + 32) == SHAPE and cfg(k) == (SHAPE if k == 12 else -4) for k in TILES)   # (12: groups of 128)
+    assert cfg(12) == SHAPE and all(cfg(k, act=0) == SHAPE for k in UNPAIRED) and all(cfg(k, K=(1 << 20) + 32) == SHAPE and cfg(k) == (SHAPE if k == 10 else -4) for k in TILES)   # (10: groups of 128)
     assert L.fp6mi_int4_pack(p, p, p, p, None, 2, 1, 16, 64, 64) == TYPE and L.fp6mi_int4_pack(p, p, p, None, None, 0, 1, 16, 64, 64) == NULL
     assert L.fp6mi_int4_pack_gpu(None, p, p, p, p, None, 0, 1, 16, 64, 33) == SHAPE and L.fp6mi_int4_pack_gpu(None, p + 4, p, p, p, None, 0, 1, 16, 64, 64) == ALIGN
 
@@ -349,8 +349,8 @@ def test_refusals_of_the_function_on_the_gpu(monkeypatch):
 
 # ---------------------------------------------------------------------------------------------------------------- the kernels by number
 KERNELS = [(0, 16, 1, 16), (0, 16, 2, 8), (0, 16, 3, 8), (0, 16, 4, 8), (0, 16, 4, 4),
-           (1, 32, 2, 8), (1, 32, 3, 4), (1, 32, 4, 4), (1, 32, 4, 4), (1, 32, 6, 4), (1, 32, 8, 4), (1, 32, 8, 2), (1, 64, 8, 2), (1, 64, 16, 1)]   # tiles, rows of X, row tiles, parts of K
-TILES, UNPAIRED = range(5, 14), (0, 2, 6, 9)   # (those without a gated product: a wavefront's row tiles are not pairs)
+           (1, 32, 3, 4), (1, 32, 4, 4), (1, 32, 6, 4), (1, 32, 8, 4), (1, 32, 8, 2), (1, 64, 8, 2), (1, 64, 16, 1)]   # tiles, rows of X, row tiles, parts of K
+TILES, UNPAIRED = range(5, 12), (0, 2, 5, 7)   # (those without a gated product: a wavefront's row tiles are not pairs)
 
 
 def choice(OC, N, IC, type="fp16", E=0, gated=False, group=128):
@@ -376,7 +376,7 @@ def test_choices_are_in_range():
                     for IC in (32, 4128, 1 << 21):
                         for gated in (False, True):
                             k = choice(OC, N, IC, type, E, gated, 64)
-                            assert k == -2 or (0 <= k < len(KERNELS) and (k not in TILES or IC <= 1 << 20) and (k not in UNPAIRED or not gated) and k != 12)
+                            assert k == -2 or (0 <= k < len(KERNELS) and (k not in TILES or IC <= 1 << 20) and (k not in UNPAIRED or not gated) and k != 10)
 
 
 def by_kernel(kernel, w, x, bias=None, act=-1, f32=False, plan=None):
@@ -400,7 +400,7 @@ def by_kernel(kernel, w, x, bias=None, act=-1, f32=False, plan=None):
 @pytest.mark.parametrize("kernel", range(len(KERNELS)))
 def test_every_kernel_with_every_layout(kernel, type, group, zeros):
     """Row tiles that do not fill a workgroup, one to five parts of K, the last block cut, rows of X at the borders of a tile; sums as they are, rounded, with a bias, gated."""
-    if kernel == 12 and group != 128:
+    if kernel == 10 and group != 128:
         pytest.skip("this kernel has groups of 128 only")
     cols = KERNELS[kernel][1]
     for OC, IC, N in ((48, 32, 1), (272, 96, cols), (96, 1184, cols + 1), (1056, 608, 2 * cols - 1), (32, 4128, 3), (288, 2048, 3 * cols + 5)):
@@ -418,7 +418,7 @@ def test_every_kernel_with_every_layout(kernel, type, group, zeros):
 @pytest.mark.parametrize("kernel", TILES)
 def test_bf16_rows_of_every_size_in_tiles(kernel):
     """Rows of bf16 are multiplied as fp16 with a power of two each: magnitudes from the smallest to the largest, zeros, infinities and NaN."""
-    w = Weight(5, 64, 160, 128 if kernel == 12 else 32, True, "bf16")
+    w = Weight(5, 64, 160, 128 if kernel == 10 else 32, True, "bf16")
     x = randn(3, 12, 160, dtype=torch.float32, device="cpu")
     x *= torch.exp2(torch.tensor([0, -60, 60, -126, 100, -133, 10, 0, 0, 0, 0, 0])).unsqueeze(1)
     x[7] = 0
@@ -455,7 +455,7 @@ def test_waits_of_the_tile_kernels_cover_the_transfers(tmp_path):
             return re.findall(r"^(_ZN\w*int4_tile\w*):[^\n]*\n(.*?)s_endpgm", f.read(), re.S | re.M)
     with ThreadPoolExecutor(len(units)) as pool:
         kernels = [k for ks in pool.map(kernels_of, units) for k in ks]
-    assert len(kernels) == 12 * 8 + 4   # (kernels 5 to 13, of which 12 has groups of 128 only)
+    assert len(kernels) == 12 * 6 + 4   # (kernels 5 to 11, of which 10 has groups of 128 only)
     vector = re.compile(r"(buffer|global|scratch|flat)_(load|store|atomic)")
     for name, text in kernels:
         loop = max(re.split(r"\n\.LBB[^\n]*:", text), key=lambda b: b.count("v_mfma"))
