@@ -227,7 +227,7 @@ template <int GPB, bool Z, int RT, int WK> __global__ __launch_bounds__(WK * 64,
 #pragma unroll
         for (uint32_t i = 0; i < 4; i++) rows[i] = __builtin_bit_cast(v8t, __builtin_amdgcn_raw_buffer_load_b128(xbuf, xoff[i] + (beyond[i] & last), kb * 256, 0));
     };
-    // rows to operands; in LDS the pieces of a row stand in the order piece ^ row, which gives reads and writes all banks
+    // rows to operands; in LDS the pieces of a row stand in the order piece ^ row, which gives reads and writes all banks (within a wavefront, whose accesses to LDS keep their order)
     v8t *const stage = reinterpret_cast<v8t *>(shared[wave]);
     auto       turn = [&](v8t(&x)[4], const v8t(&rows)[4]) __attribute__((always_inline)) {
 #pragma unroll

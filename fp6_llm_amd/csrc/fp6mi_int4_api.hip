@@ -12,10 +12,10 @@ namespace {
 inline bool aligned(const void *p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
 // The nibble of a dword that column j (0..7) of its eight is held in: even ones in the lower 16 bits, odd ones in the upper.
-__host__ __device__ inline uint32_t nibble_of(uint32_t j) { return (j & 1) * 4 + j / 2; }
+inline uint32_t nibble_of(uint32_t j) { return (j & 1) * 4 + j / 2; }
 
 // Dword i of the native layout of one matrix from its codes, two to a byte, the even column in the low half.
-__host__ __device__ inline uint32_t native_dword(const uint8_t *codes, size_t i, uint32_t K, uint32_t KB)
+inline uint32_t native_dword(const uint8_t *codes, size_t i, uint32_t K, uint32_t KB)
 {
     const uint32_t s = i & 3, lane = i >> 2 & 63, k = (uint32_t)((i >> 8) % KB) * 128 + s * 32 + (lane >> 4) * 8;
     const size_t   row = (i >> 8) / KB * 16 + (lane & 15);
@@ -25,32 +25,61 @@ __host__ __device__ inline uint32_t native_dword(const uint8_t *codes, size_t i,
     return d;
 }
 
-// Element i of the native scales (16 bits), of {scale, zero point} pairs with zero points; `each` columns to a native group (32, 64 or 128).
-__host__ __device__ inline uint16_t native_scale(const uint16_t *scales, const uint8_t *zeros, int bf16, size_t i, uint32_t K, uint32_t KB, uint32_t group, uint32_t each)
+// A zero point as a number of the scales' type, which holds it exactly.
+__host__ __device__ inline uint16_t zero_bits(uint32_t z, int bf16)
 {
-    const uint32_t per = 128 / each, groups = (K + group - 1) / group;
-    const size_t   p = zeros ? i >> 1 : i;
-    const uint32_t row = (uint32_t)(p / per % 16), k = (uint32_t)(p / per / 16 % KB) * 128 + (uint32_t)(p % per) * each;
-    const size_t   at = (p / per / 16 / KB * 16 + row) * groups + k / group;
-    if (k >= K) return 0;
-    if (!zeros || (i & 1) == 0) return scales[at];
-    const uint32_t z = zeros[at] & 15; // as a number of the scales' type, which holds it exactly
+    z &= 15;
     if (z == 0) return 0;
     uint32_t e = 3;
     while (!(z >> e)) e--;
     return bf16 ? (uint16_t)((127 + e) << 7 | (z << (7 - e) & 127)) : (uint16_t)((15 + e) << 10 | (z << (10 - e) & 1023));
 }
 
-__global__ __launch_bounds__(256) void pack_codes(uint32_t *__restrict__ out, const uint8_t *__restrict__ codes, size_t count, uint32_t K, uint32_t KB, size_t matrix)
+// The scales (with zero points: {scale, zero point}) of 16 rows, `each` columns (32, 64 or 128) to a native group: j from `first` in strides up to their number, [column block][row][group of the block].
+__host__ __device__ inline void native_scales_of(uint16_t *to, const uint16_t *scales, const uint8_t *zeros, int bf16, uint32_t K, uint32_t KB, uint32_t group, uint32_t each, uint32_t first, uint32_t stride)
 {
-    const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
-    if (i < count) out[i] = native_dword(codes + i / matrix * (matrix / (KB * 16) * (K / 2)), i % matrix, K, KB);
+    const uint32_t per = 128 / each, groups = (K + group - 1) / group;
+    for (uint32_t j = first; j < KB * 16 * per; j += stride) {
+        const uint32_t k = j / (16 * per) * 128 + j % per * each;
+        const size_t   at = (size_t)(j / per % 16) * groups + k / group;
+        const uint16_t scale = k < K ? scales[at] : 0;
+        if (zeros)
+            to[2 * (size_t)j] = scale, to[2 * (size_t)j + 1] = k < K ? zero_bits(zeros[at], bf16) : 0;
+        else
+            to[j] = scale;
+    }
 }
-__global__ __launch_bounds__(256) void pack_scales(uint16_t *__restrict__ out, const uint16_t *__restrict__ scales, const uint8_t *__restrict__ zeros, int bf16, size_t count, uint32_t K, uint32_t KB,
-                                                   uint32_t group, uint32_t each)
+
+// A wavefront to a block of 16 rows x 128 columns: lane c + 16 s reads the 16 bytes of row c from column 32 s on, puts the nibbles of each dword in order, and the four lanes of a row trade dwords by way of LDS.
+// (28672x8192 with its scales: 39 us, 6 TB/s read and written; with a thread to a dword that reads its bytes one by one 390.)
+template <bool ALIGNED> __global__ __launch_bounds__(256) void pack_codes(uint32_t *__restrict__ out, const uint8_t *__restrict__ codes, uint32_t blocks, uint32_t K, uint32_t KB)
 {
-    const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
-    if (i < count) out[i] = native_scale(scales, zeros, bf16, i, K, KB, group, each);
+    __shared__ uint32_t stage[4][256];
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, s = lane >> 4, b = blockIdx.x * 4 + wave, k = b % KB * 128 + s * 32;
+    typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+    v4u d = { 0, 0, 0, 0 };
+    if (b < blocks && k < K) { // (K is a multiple of 32)
+        const uint8_t *row = codes + (((size_t)(b / KB) * 16 + c) * K + k) / 2;
+        if constexpr (ALIGNED)
+            d = *reinterpret_cast<const v4u *>(row);
+        else
+            for (int i = 0; i < 16; i++) d[i / 4] |= (uint32_t)row[i] << i % 4 * 8;
+    }
+#pragma unroll
+    for (uint32_t q = 0; q < 4; q++) {
+        uint32_t even = d[q] & 0x0f0f0f0fu, odd = d[q] >> 4 & 0x0f0f0f0fu;
+        even = (even | even >> 4) & 0x00ff00ffu, odd = (odd | odd >> 4) & 0x00ff00ffu;
+        stage[wave][(c + 16 * q) * 4 + s] = ((even | even >> 8) & 0xffffu) | (odd | odd >> 8) << 16;
+    }
+    __syncthreads();
+    if (b < blocks) reinterpret_cast<v4u *>(out)[(size_t)b * 64 + lane] = *reinterpret_cast<const v4u *>(&stage[wave][lane * 4]);
+}
+
+// A workgroup to 16 rows.
+__global__ __launch_bounds__(256) void pack_scales(uint16_t *__restrict__ out, const uint16_t *__restrict__ scales, const uint8_t *__restrict__ zeros, int bf16, uint32_t K, uint32_t KB, uint32_t group, uint32_t each)
+{
+    const size_t rows = (size_t)blockIdx.x * 16, groups = (K + group - 1) / group;
+    native_scales_of(out + rows * KB * (128 / each) * (zeros ? 2 : 1), scales + rows * groups, zeros ? zeros + rows * groups : nullptr, bf16, K, KB, group, each, threadIdx.x, 256);
 }
 
 inline uint32_t native_group(size_t group) { return group % 128 == 0 ? 128 : group % 64 == 0 ? 64 : 32; }
@@ -136,12 +165,12 @@ int fp6mi_int4_pack(void *native, void *native_scales, const void *codes, const 
 {
     if (const int e = check_pack(native, native_scales, codes, scales, dtype, experts, M, K, group)) return e;
     const uint32_t KB = (uint32_t)((K + 127) / 128);
-    const size_t   matrix = M / 16 * KB * 256, count = fp6mi_int4_scale_bytes(experts, M, K, group, zeros != nullptr) / 2;
+    const size_t   matrix = M / 16 * KB * 256, tiles = experts * (M / 16), groups = (K + group - 1) / group, of_tile = fp6mi_int4_scale_bytes(1, 16, K, group, zeros != nullptr) / 2;
     for (size_t e = 0; e < experts; e++)
         for (size_t i = 0; i < matrix; i++) static_cast<uint32_t *>(native)[e * matrix + i] = native_dword(static_cast<const uint8_t *>(codes) + e * M * (K / 2), i, (uint32_t)K, KB);
-    for (size_t i = 0; i < count; i++)
-        static_cast<uint16_t *>(native_scales)[i] =
-            native_scale(static_cast<const uint16_t *>(scales), static_cast<const uint8_t *>(zeros), dtype, i, (uint32_t)K, KB, (uint32_t)group, native_group(group));
+    for (size_t t = 0; t < tiles; t++)
+        native_scales_of(static_cast<uint16_t *>(native_scales) + t * of_tile, static_cast<const uint16_t *>(scales) + t * 16 * groups,
+                         zeros ? static_cast<const uint8_t *>(zeros) + t * 16 * groups : nullptr, dtype, (uint32_t)K, KB, (uint32_t)group, native_group(group), 0, 1);
     return FP6MI_OK;
 }
 
@@ -149,13 +178,15 @@ int fp6mi_int4_pack_gpu(void *stream, void *native, void *native_scales, const v
 {
     if (const int e = check_pack(native, native_scales, codes, scales, dtype, experts, M, K, group)) return e;
     const uint32_t KB = (uint32_t)((K + 127) / 128);
-    const size_t   matrix = M / 16 * KB * 256, dwords = experts * matrix, count = fp6mi_int4_scale_bytes(experts, M, K, group, zeros != nullptr) / 2;
-    if (dwords / 256 > 0x7fffffffu || (count + 255) / 256 > 0x7fffffffu) return FP6MI_ERR_SHAPE;
-    hipStream_t st = static_cast<hipStream_t>(stream);
-    hipLaunchKernelGGL(pack_codes, dim3((uint32_t)(dwords / 256)), dim3(256), 0, st, static_cast<uint32_t *>(native), static_cast<const uint8_t *>(codes), dwords, (uint32_t)K, KB, matrix);
+    const size_t   tiles = experts * (M / 16), blocks = tiles * KB; // up to 2^31
+    hipStream_t    st = static_cast<hipStream_t>(stream);
+    if (aligned(codes, 16))
+        hipLaunchKernelGGL(pack_codes<true>, dim3((uint32_t)((blocks + 3) / 4)), dim3(256), 0, st, static_cast<uint32_t *>(native), static_cast<const uint8_t *>(codes), (uint32_t)blocks, (uint32_t)K, KB);
+    else
+        hipLaunchKernelGGL(pack_codes<false>, dim3((uint32_t)((blocks + 3) / 4)), dim3(256), 0, st, static_cast<uint32_t *>(native), static_cast<const uint8_t *>(codes), (uint32_t)blocks, (uint32_t)K, KB);
     if (const hipError_t e = hipGetLastError()) return (int)e;
-    hipLaunchKernelGGL(pack_scales, dim3((uint32_t)((count + 255) / 256)), dim3(256), 0, st, static_cast<uint16_t *>(native_scales), static_cast<const uint16_t *>(scales),
-                       static_cast<const uint8_t *>(zeros), dtype, count, (uint32_t)K, KB, (uint32_t)group, native_group(group));
+    hipLaunchKernelGGL(pack_scales, dim3((uint32_t)tiles), dim3(256), 0, st, static_cast<uint16_t *>(native_scales), static_cast<const uint16_t *>(scales), static_cast<const uint8_t *>(zeros), dtype,
+                       (uint32_t)K, KB, (uint32_t)group, native_group(group));
     return (int)hipGetLastError();
 }
 

@@ -125,6 +125,9 @@ def test_layout_of_experts_is_that_of_each():
 def test_layout_made_on_the_gpu_is_that_of_the_host(OC, IC, group, zeros, type, E):
     a, b = Weight(5, OC, IC, group, zeros, type, E, "cpu"), Weight(5, OC, IC, group, zeros, type, E)
     assert torch.equal(a.native, b.native.cpu()) and torch.equal(a.native_scales, b.native_scales.cpu())
+    apart = torch.cat((b.codes.new_zeros(3), b.codes.flatten()))[3:].view(b.codes.shape)   # (codes that begin between two 16-byte boundaries)
+    native, scales = fp6.int4_pack_native(apart, b.scales, b.zeros, group)
+    assert torch.equal(native, b.native) and torch.equal(scales, b.native_scales)
 
 
 @pytest.mark.parametrize("zeros", [False, True])
