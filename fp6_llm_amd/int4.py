@@ -78,7 +78,7 @@ def int4_forward_native(in_feats, native_weight, native_scales, plan=None, activ
     """out[B, OC] = in_feats[B, IC] @ w^T (+ bias[OC]) with the weights of int4_pack_native.  activation ("silu", "gelu", "gelu_tanh"): out[B, OC/2] = act(gate) * up, for weights (and bias) whose
     rows are in pair order (16 rows of gate, the same 16 of up, and so on: gate_up_pairs).
     plan: that of expert_sort or expert_plan, for the weights of experts [E, ...] (bias [E, OC]): rows sorted by expert, each multiplied with its expert's weights; rows behind those come out as zeros.
-    in_feats has the scales' type, out too or (out_dtype) float32.  workspace: float32, of fp6mi_int4_workspace_bytes (many bfloat16 rows need one).  Not part of an autograd graph."""
+    IC is that of the weights, which their native shape tells to 128 columns only.  in_feats has the scales' type, out too or (out_dtype) float32.  workspace: float32, of fp6mi_int4_workspace_bytes (many bfloat16 rows need one).  Not part of an autograd graph."""
     _ext = _package._ext
     act = -1 if activation is None else ops._activation_code(activation)
     f32 = out_dtype == torch.float32

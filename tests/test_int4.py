@@ -228,6 +228,18 @@ def test_scales_of_every_size(N):
 
 
 @gpu
+@pytest.mark.parametrize("N", [3, 40])
+@pytest.mark.parametrize("type", ["fp16", "bf16"])
+def test_rows_longer_than_a_tile_takes(N, type):
+    """More than 2^20 columns: offsets of 16 rows pass 2^25 bytes, and the kernels that stream weights take any number of rows."""
+    w = Weight(3, 32, (1 << 20) + 160, 128, True, type)
+    x = randn(4, N, w.IC, dtype=w.dtype)
+    assert choice(32, N, w.IC, type) not in TILES
+    y, err = product64(w.w, x, extra=w if type == "bf16" else None)
+    within(fp6.int4_forward_native(x, w.native, w.native_scales), *plain(y, err, w.dtype))
+
+
+@gpu
 def test_no_rows_give_no_rows():
     w = Weight(1, 32, 64, 32)
     got = fp6.int4_forward_native(torch.empty(0, 64, dtype=torch.float16, device=DEV), w.native, w.native_scales)
