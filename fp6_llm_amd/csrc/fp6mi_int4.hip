@@ -173,10 +173,10 @@ __device__ __forceinline__ void store_zeros(const Int4Args &a, const Tile &t, ui
 // ---------------------------------------------------------------------------------------------------------------
 // Few rows: RT row tiles and 16 rows of X to a workgroup of WK wavefronts, which share K: a wavefront takes every WK-th column block, its weights straight from HBM to registers (the next block's on their
 // way meanwhile) and its part of X from L2; the partial sums meet in LDS.  X is read in whole rows, two blocks ahead, and turned into operands through LDS a block ahead: as operands, 64 bytes of each of 16
-// rows to a load, 8192x8192 at 16 rows took 11.8 us and 28672x8192 27.8, in whole rows 10.5 and 26.2.  (Only the kernel of one row tile, which is for few blocks, reads operands: to turn them
+// rows to a load, 8192x8192 at 16 rows took 11.8 us and 28672x8192 27.8, in whole rows 10.2 and 24.8.  (Only the kernel of one row tile, which is for few blocks, reads operands: to turn them
 // takes it 0.4 us, and at one row there is nothing to be won.)
-// Bound by the bytes of the weights where there are many (28672x8192: 23.2 us at 1 row, 26 at 16, of which the bytes take 23.6 at a copy's rate; 8192x8192: 8.5 and 10.5 of 6.8), by a wavefront's few blocks
-// one after another where there are few (4096x4096 at 1 row: 4.3 us with 16 wavefronts to a row tile, 5.4 with 8 to two).  Three and four blocks of weights on their way were no faster, nor were two
+// Bound by the bytes of the weights where there are many (28672x8192: 22.4 us at 1 row, 24.8 at 16, of which the bytes take 23.6 at a copy's rate; 8192x8192: 8.5 and 10.2 of 6.8), by a wavefront's few blocks
+// one after another where there are few (4096x4096 at 1 row: 4.3 us with 16 wavefronts to a row tile, 5.2 with 8 to two).  Three and four blocks of weights on their way were no faster, nor were two
 // tiles of rows of X to a workgroup.
 // ---------------------------------------------------------------------------------------------------------------
 template <int GPB, bool Z, int RT> struct Block {
@@ -202,14 +202,14 @@ template <int GPB, bool Z, int RT, int WK> __global__ __launch_bounds__(WK * 64,
         w[r] = static_cast<const v4u *>(a.W) + at * 64 + lane;
         s[r] = static_cast<const Scales<GPB, Z> *>(a.S) + at * 16 + c;
     }
-    // X: in whole rows, four of 256 bytes to a load, lane c + 16 q with piece c of row 4 i + q, or (one row tile) as operands, piece 4 i + q of row c.  Rows behind the last one: that again.
+    // X: in whole rows, four of 256 bytes to a load, lane c + 16 q with piece c of row 4 i + q, or (one row tile) as operands, piece 4 i + q of row c.  Rows behind the last one are behind the buffer: they read as zeros and ask for nothing.
     constexpr bool kTurn = RT > 1;
     const auto     xbuf = __builtin_amdgcn_make_buffer_rsrc(const_cast<T *>(static_cast<const T *>(a.X) + (size_t)t.row * a.K), 0, (int)(t.rows * a.K * 2), 0x00027000);
     uint32_t       xoff[4], beyond[4]; // (beyond: what puts an offset in the last block behind the buffer, which reads as zeros)
 #pragma unroll
     for (uint32_t i = 0; i < 4; i++) {
         const uint32_t row = kTurn ? 4 * i + q : c, piece = kTurn ? c : 4 * i + q;
-        xoff[i] = (row < t.rows ? row : t.rows - 1) * a.K * 2 + piece * 16;
+        xoff[i] = row * a.K * 2 + piece * 16;
         beyond[i] = (a.KB - 1) * 128 + piece * 8 < a.K ? 0 : 0x80000000u;
     }
 
@@ -295,9 +295,11 @@ template <int GPB, bool Z, int RT, int WK> __global__ __launch_bounds__(WK * 64,
             load(b[1], kb + WK);
             next(x[1], kb + WK);
             multiply(b[0], x[0]);
+            __builtin_amdgcn_sched_barrier(0); // (or loads sink behind the next block's conversions: 37.6 -> 32.2 us for 64 experts of 2560x2048 at 320 rows)
             load(b[0], kb + 2 * WK);
             next(x[0], kb + 2 * WK);
             multiply(b[1], x[1]);
+            __builtin_amdgcn_sched_barrier(0);
         }
         if (kb + WK < a.KB) {
             load(b[1], kb + WK);
@@ -433,14 +435,14 @@ template <int GPB, bool Z, int RT, int NT, int WR, int WK> __global__ __launch_b
     typedef __attribute__((address_space(3))) void lvoid;
     const auto     xbuf = __builtin_amdgcn_make_buffer_rsrc(const_cast<half_t *>(static_cast<const half_t *>(a.X) + (size_t)t.row * a.K), 0, (int)(t.rows * a.K * 2), 0x00027000);
     uint8_t *const xstage = lds + wk * 2 * kStage;
-    const uint32_t xrow0 = (4 * wr + q) * a.K * 2, xlast = (t.rows - 1) * a.K * 2; // 32 bits: the launcher bounds K
+    const uint32_t xrow0 = (4 * wr + q) * a.K * 2; // 32 bits: the launcher bounds K
     auto           transfer = [&](uint32_t kb, uint32_t stage) __attribute__((always_inline)) {
 #pragma unroll
         for (uint32_t j = 0; j < kDma; j++) {
             uint32_t row = xrow0, piece = c ^ q;
             if constexpr (kDma > 4) asm("" : "+v"(row), "+v"(piece)); // (each address for itself when it is needed: kept, they take the registers of a tile)
             row += j * WR * 8 * a.K, piece ^= 4 * ((j * WR + wr) & 3);
-            const uint32_t k = kb * 128 + piece * 8, off = (row < xlast ? row : xlast) + (k < a.K ? k * 2 : 0xc0000000u); // (beyond the buffer, which reads as zeros)
+            const uint32_t k = kb * 128 + piece * 8, off = row + (k < a.K ? k * 2 : 0xc0000000u); // (beyond the buffer, as the rows behind the last one: reads as zeros and asks for nothing)
             __builtin_amdgcn_raw_ptr_buffer_load_lds(xbuf, (lvoid *)(xstage + stage * kStage + (j * WR + wr) * 1024), 16, off, 0, 0, 0);
         }
     };

@@ -101,11 +101,11 @@ int check_pack(const void *native, const void *native_scales, const void *codes,
 
 // Which kernel takes a product (an index of kInt4Kernels): the fastest by this model of its time, us.  A workgroup's column blocks one after another take `step` each while every CU has one at the most,
 // `share` times the workgroups of a CU beyond; and no kernel reads the weights faster than memory.  Rows of experts are taken to be spread evenly, with half a tile to spare for each expert.
-// Fitted to 3172 times of 281 products in graphs, weights from HBM (512x2048 to 28672x8192 at 1 to 777 rows, 8 to 128 experts at 1 to 700 tokens, fp16 and bf16): a kernel's own time is off by 18 to 31 % rms,
-// the choice takes 1.01 times the fastest measured in the mean, at worst 1.47; for 126 other products 1.01 and 1.30.
-struct Times { double base, step, share, rows; }; // rows: how much longer a step takes with 16 rows than with none, of the kernel that reads X as operands
-constexpr Times kTimes[] = { { 1.06, 1.36, 1.35, 1.16 }, { 1.81, 0.93, 1.20, 0 }, { 2.45, 1.39, 1.54, 0 }, { 1.63, 1.78, 1.95, 0 }, { 1.82, 1.19, 0.75, 0 }, { 3.05, 1.02, 1.00, 0 },
-                             { 2.65, 1.09, 1.25, 0 },    { 3.01, 1.43, 1.65, 0 }, { 2.22, 1.78, 2.14, 0 }, { 5.92, 1.04, 0.87, 0 }, { 2.38, 1.33, 1.56, 0 }, { 1.26, 1.14, 1.17, 0 } };
+// Fitted to 4372 times of 407 products in graphs, weights from HBM (512x2048 to 28672x8192 at 1 to 1000 rows, 8 to 128 experts at 1 to 700 tokens, fp16 and bf16): a kernel's own time is off by 17 to 31 % rms, the
+// choice takes 1.01 times the fastest measured in the mean, at worst 1.29; for 100 other products 1.02 and 1.25.
+struct Times { double base, step, share, rows; }; // rows: how much longer a step takes with 16 rows than with none
+constexpr Times kTimes[] = { { 1.25, 1.19, 1.28, 1.12 }, { 1.78, 0.87, 1.13, 0 }, { 2.65, 1.17, 1.35, 0.10 }, { 1.61, 1.64, 1.93, 0 }, { 2.01, 1.08, 0.70, 0 }, { 3.25, 0.99, 0.97, 0 },
+                             { 2.78, 1.05, 1.20, 0 },    { 3.07, 1.35, 1.57, 0 }, { 2.18, 1.75, 2.14, 0 },    { 6.59, 0.99, 0.78, 0 }, { 2.58, 1.26, 1.44, 0 }, { 2.18, 1.03, 1.10, 0 } };
 
 constexpr int    kKernels = sizeof(kTimes) / sizeof(kTimes[0]);
 static_assert(kKernels == sizeof(fp6mi::kInt4Kernels) / sizeof(fp6mi::kInt4Kernels[0]), "");
