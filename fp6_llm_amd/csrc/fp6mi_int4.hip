@@ -80,8 +80,10 @@ __device__ __forceinline__ void codes_half(Codes &to, uint32_t w, const Zero &ze
     to.d[2 * half + 1] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(__builtin_bit_cast(v2h, (w & cut.high) | cut.bits), sixteenth, zero.high));
 }
 
-// The operands of the kernel of few rows.  fp16: q - z.  bf16: 128 + q, the bits 0x4300 | nibble, 7 instructions (q - z by way of float32 takes 23, which bound that kernel), beside which a second matrix
-// instruction, of which it has plenty, takes -(128 + z); what is lost of the float32 sums is 2^-24 of 30 times their magnitude, a thousandth of an output's rounding (an infinity in X comes out as NaN).
+// The operands of the kernel of few rows.  fp16: q - z.  bf16: 128 + q, the bits 0x4300 | nibble, 7 instructions (q - z by way of float32 takes 23, which bound that kernel); what is too much, 128 + z times
+// the sum of a group's X, is where the products start from, a sum that a matrix instruction with ones makes for all row tiles (28672x8192 at 4 rows with groups of 64 and zero points 26.7 -> 24.9 us
+// against one with -(128 + z) for each).  What is lost of the float32 sums is 2^-24 of 30 times their magnitude, a
+// thousandth of an output's rounding (an infinity in X comes out as NaN).
 #if FP6MI_TYPE == 0
 struct FewCutter : Cutter { };
 struct FewZero : Zero { };
@@ -98,12 +100,8 @@ struct FewCutter {
     __device__ __forceinline__ FewCutter() { asm("" : "+s"(mask), "+v"(bits)); }
 };
 struct FewZero {
-    v8t all; // -(128 + z)
-    __device__ __forceinline__ void set(T zero)
-    {
-        const T z = (T)(-128.f - (float)zero);
-        all = (v8t){ z, z, z, z, z, z, z, z };
-    }
+    float all; // -(128 + z)
+    __device__ __forceinline__ void set(T zero) { all = -128.f - (float)zero; }
 };
 __device__ __forceinline__ v8t codes_of(uint32_t w, const FewZero &, const FewCutter &cut)
 {
@@ -112,12 +110,6 @@ __device__ __forceinline__ v8t codes_of(uint32_t w, const FewZero &, const FewCu
     for (int i = 0; i < 4; i++) r.d[i] = (w >> 4 * i & cut.mask) | cut.bits;
     return r.v;
 }
-#endif
-
-#if FP6MI_TYPE == 0
-__device__ __forceinline__ v4f second(v8t, const FewZero &, v4f acc) { return acc; }
-#else
-__device__ __forceinline__ v4f second(v8t x, const FewZero &zero, v4f acc) { return mfma(x, zero.all, acc); }
 #endif
 
 // The scales (and zero points) of one row in one block.
@@ -240,18 +232,20 @@ template <int GPB, bool Z, int RT, int WK> __global__ __launch_bounds__(WK * 64,
     for (int r = 0; r < RT; r++) sum[r] = (v4f){ 0.f, 0.f, 0.f, 0.f };
     auto multiply = [&](const B &b, const v8t(&x)[4]) __attribute__((always_inline)) {
         constexpr int kEach = 4 / GPB; // steps of a group
-        constexpr bool kSecond = FP6MI_TYPE == 1;
+        constexpr bool kStart = FP6MI_TYPE == 1;
         FewZero        zero;
         zero.set((T)8.f);
-        v4f first[GPB]; // what the second instruction gives where all rows share it
-        if constexpr (kSecond && !Z) {
+        v4f start[GPB]; // the groups' sums of X; without zero points -136 times that, which all rows' products start from
+#if FP6MI_TYPE == 1
+        const T   each = (T)(Z ? 1.f : -136.f);
+        const v8t ones = { each, each, each, each, each, each, each, each };
 #pragma unroll
-            for (int g = 0; g < GPB; g++) {
-                first[g] = (v4f){ 0.f, 0.f, 0.f, 0.f };
+        for (int g = 0; g < GPB; g++) {
+            start[g] = (v4f){ 0.f, 0.f, 0.f, 0.f };
 #pragma unroll
-                for (int i = 0; i < kEach; i++) first[g] = second(x[g * kEach + i], zero, first[g]);
-            }
+            for (int i = 0; i < kEach; i++) start[g] = mfma(x[g * kEach + i], ones, start[g]);
         }
+#endif
 #pragma unroll
         for (int r = 0; r < RT; r++)
 #pragma unroll
@@ -262,15 +256,14 @@ template <int GPB, bool Z, int RT, int WK> __global__ __launch_bounds__(WK * 64,
 #pragma unroll
                 for (int i = 0; i < kEach; i++) v[i] = codes_of(b.w[r][g * kEach + i], zero, cut);
                 v4f y = { 0.f, 0.f, 0.f, 0.f };
-                if constexpr (kSecond && !Z) y = first[g];
+#if FP6MI_TYPE == 1
+                y = Z ? start[g] * zero.all : start[g];
+#endif
 #pragma unroll
-                for (int i = 0; i < kEach; i++) {
-                    if constexpr (kSecond && Z) y = second(x[g * kEach + i], zero, y);
-                    y = mfma(x[g * kEach + i], v[i], y);
-                }
+                for (int i = 0; i < kEach; i++) y = mfma(x[g * kEach + i], v[i], y);
 #pragma unroll
                 for (int i = 0; i < 4; i++) sum[r][i] += scale * y[i];
-                if (kSecond && Z && GPB == 4 && RT == 4 && g == GPB - 1 && r % 2 == 1) __builtin_amdgcn_sched_barrier(0); // (or conversions come so early that registers spill: 16 -> 28 us for 8192x8192)
+                if (kStart && Z && GPB == 4 && RT == 4 && g == GPB - 1 && r % 2 == 1) __builtin_amdgcn_sched_barrier(0); // (or conversions come so early that registers spill: 16 -> 28 us for 8192x8192)
             }
     };
     B        b[2];
