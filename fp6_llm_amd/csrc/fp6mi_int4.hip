@@ -4,7 +4,7 @@
 //
 // q - z is an integer from -15 to 15, exact in fp16, so the matrix instructions' products are exact and their sums float32; a group's sum is multiplied by its scale in float32.
 // (Scaling the weights before the product would round each of them to 16 bits, and 16-bit sums would be no cheaper.)  bf16 has no packed arithmetic that would make q - z of codes: the kernel of
-// few rows multiplies 128 + q, which are bits, and -(128 + z), the one of many rows is given X in fp16 with an exponent for each row (rows_to_halfs).
+// few rows multiplies 128 + q, which are bits, from sums that start at -(128 + z) times those of X; the one of many rows is given X in fp16 with an exponent for each row (rows_to_halfs).
 //
 // Layout (fp6mi_int4_pack): blocks of 16 rows x 128 columns of 1024 bytes, [expert][row tile][column block]; lane c + 16 q of a wavefront holds 16 bytes of a block, dword s of which are the
 // columns 32 s + 8 q to 32 s + 8 q + 7 of row c: the operand of one v_mfma_f32_16x16x32.  In a dword the nibbles 0..7 are the columns 0, 2, 4, 6, 1, 3, 5, 7, so that a mask leaves two neighbours
