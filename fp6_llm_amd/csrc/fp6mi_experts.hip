@@ -262,55 +262,53 @@ __global__ __launch_bounds__(256) void combine_rows(O *__restrict__ out, const R
     store_past(reinterpret_cast<Vec<O, VEC> *>(out) + (size_t)t * nvec + i, o);
 }
 
-// Its gradient: grad_rows[place[t,j]] = w[t,j] * grad[t] (zeros where there is no expert), grad_weights[t,j] = <grad[t], rows[place[t,j]]>; either may be left out.  A workgroup to a token.
+// Its gradient: grad_rows[place[t,j]] = w[t,j] * grad[t] (zeros where there is no expert), grad_weights[t,j] = <grad[t], rows[place[t,j]]>; either may be left out.  A workgroup to a token
+// and four of its experts (64 tokens x 8 of 4096: 10.1 us for all eight one after another, 6.2; 8192 x 8 of 2048 102 and 100).
 template <typename R, typename O, int VEC>
 __global__ __launch_bounds__(256) void combine_gradient(R *__restrict__ grad_rows, float *__restrict__ grad_weights, const O *__restrict__ grad, const R *__restrict__ rows,
-                                                        const int *__restrict__ place, const int *__restrict__ valid_at, const float *__restrict__ weights, uint32_t nvec, int k)
+                                                        const int *__restrict__ place, const int *__restrict__ valid_at, const float *__restrict__ weights, uint32_t nvec, int k, uint32_t parts)
 {
     constexpr int  J = 4;
     __shared__ float part[4][J];
-    const uint32_t t = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int      valid = *valid_at;
+    const uint32_t t = blockIdx.x / parts, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int      valid = *valid_at, j0 = (int)(blockIdx.x - t * parts) * J;
     const auto    *g_row = reinterpret_cast<const Vec<O, VEC> *>(grad) + (size_t)t * nvec;
-    for (int j0 = 0; j0 < k; j0 += J) {
-        int   at[J];
-        float w[J], dot[J] = {};
+    int            at[J];
+    float          w[J], dot[J] = {};
 #pragma unroll
-        for (int j = 0; j < J; j++) {
-            at[j] = j0 + j < k ? place[(size_t)t * k + j0 + j] : -1;
-            w[j] = j0 + j < k ? (weights ? weights[(size_t)t * k + j0 + j] : 1.f) : 0.f;
-        }
-        for (uint32_t i = tid; i < nvec; i += 256) {
-            const Vec<O, VEC> g = g_row[i];
-            Vec<R, VEC>       r[J];
-            if (grad_weights) {
-#pragma unroll
-                for (int j = 0; j < J; j++)
-                    if (at[j] >= 0 && at[j] < valid) r[j] = reinterpret_cast<const Vec<R, VEC> *>(rows)[(size_t)at[j] * nvec + i];
-            }
-#pragma unroll
-            for (int j = 0; j < J; j++) {
-                if (at[j] < 0) continue;
-                Vec<R, VEC> d;
-#pragma unroll
-                for (int v = 0; v < VEC; v++) d.v[v] = at[j] < valid ? (R)(w[j] * (float)g.v[v]) : (R)0.f;
-                if (grad_rows) store_past(reinterpret_cast<Vec<R, VEC> *>(grad_rows) + (size_t)at[j] * nvec + i, d);
-                if (grad_weights && at[j] < valid) {
-#pragma unroll
-                    for (int v = 0; v < VEC; v++) dot[j] += (float)g.v[v] * (float)r[j].v[v];
-                }
-            }
-        }
-        if (!grad_weights) continue;
-#pragma unroll
-        for (int j = 0; j < J; j++) {
-            const float s = wave_sum(dot[j]);
-            if (lane == 0) part[wave][j] = s;
-        }
-        __syncthreads();
-        if (tid < J && j0 + (int)tid < k) grad_weights[(size_t)t * k + j0 + tid] = (part[0][tid] + part[1][tid]) + (part[2][tid] + part[3][tid]);
-        __syncthreads();
+    for (int j = 0; j < J; j++) {
+        at[j] = j0 + j < k ? place[(size_t)t * k + j0 + j] : -1;
+        w[j] = j0 + j < k ? (weights ? weights[(size_t)t * k + j0 + j] : 1.f) : 0.f;
     }
+    for (uint32_t i = tid; i < nvec; i += 256) {
+        const Vec<O, VEC> g = g_row[i];
+        Vec<R, VEC>       r[J];
+        if (grad_weights) {
+#pragma unroll
+            for (int j = 0; j < J; j++)
+                if (at[j] >= 0 && at[j] < valid) r[j] = reinterpret_cast<const Vec<R, VEC> *>(rows)[(size_t)at[j] * nvec + i];
+        }
+#pragma unroll
+        for (int j = 0; j < J; j++) {
+            if (at[j] < 0) continue;
+            Vec<R, VEC> d;
+#pragma unroll
+            for (int v = 0; v < VEC; v++) d.v[v] = at[j] < valid ? (R)(w[j] * (float)g.v[v]) : (R)0.f;
+            if (grad_rows) store_past(reinterpret_cast<Vec<R, VEC> *>(grad_rows) + (size_t)at[j] * nvec + i, d);
+            if (grad_weights && at[j] < valid) {
+#pragma unroll
+                for (int v = 0; v < VEC; v++) dot[j] += (float)g.v[v] * (float)r[j].v[v];
+            }
+        }
+    }
+    if (!grad_weights) return;
+#pragma unroll
+    for (int j = 0; j < J; j++) {
+        const float s = wave_sum(dot[j]);
+        if (lane == 0) part[wave][j] = s;
+    }
+    __syncthreads();
+    if (tid < J && j0 + (int)tid < k) grad_weights[(size_t)t * k + j0 + tid] = (part[0][tid] + part[1][tid]) + (part[2][tid] + part[3][tid]);
 }
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -452,9 +450,11 @@ int fp6mi_expert_combine_backward(void *stream, const void *grad, const void *ro
     return by_types(row_type, out_type, H, aligned(rows, 16) && aligned(grad_rows, 16) && aligned(grad, 16), [&](auto r, auto o, auto vec) {
         typedef decltype(r) R;
         typedef decltype(o) O;
-        constexpr int V = decltype(vec)::value;
-        hipLaunchKernelGGL((combine_gradient<R, O, V>), dim3((uint32_t)tokens), dim3(256), 0, static_cast<hipStream_t>(stream), static_cast<R *>(grad_rows), grad_weights, static_cast<const O *>(grad),
-                           static_cast<const R *>(rows), place, valid, weights, (uint32_t)(H / V), (int)k);
+        constexpr int  V = decltype(vec)::value;
+        const uint32_t parts = (uint32_t)((k + 3) / 4);
+        if (tokens * parts > 0x7fffffffu) return FP6MI_ERR_SHAPE;
+        hipLaunchKernelGGL((combine_gradient<R, O, V>), dim3((uint32_t)(tokens * parts)), dim3(256), 0, static_cast<hipStream_t>(stream), static_cast<R *>(grad_rows), grad_weights, static_cast<const O *>(grad),
+                           static_cast<const R *>(rows), place, valid, weights, (uint32_t)(H / V), (int)k, parts);
         return (int)hipGetLastError();
     });
 }
