@@ -83,7 +83,7 @@ __device__ __forceinline__ void codes_half(Codes &to, uint32_t w, const Zero &ze
 // The operands of the kernel of few rows.  fp16: q - z.  bf16: 128 + q, the bits 0x4300 | nibble, 7 instructions (q - z by way of float32 takes 23, which bound that kernel); what is too much, 128 + z times
 // the sum of a group's X, is where the products start from, a sum that a matrix instruction with ones makes for all row tiles (28672x8192 at 4 rows with groups of 64 and zero points 26.7 -> 24.9 us
 // against one with -(128 + z) for each).  What is lost of the float32 sums is 2^-24 of 30 times their magnitude, a
-// thousandth of an output's rounding (an infinity in X comes out as NaN).
+// thousandth of an output's rounding; sums that leave float32's range on the way are made again at the end, with q - z.
 #if FP6MI_TYPE == 0
 struct FewCutter : Cutter { };
 struct FewZero : Zero { };
@@ -306,6 +306,51 @@ template <int GPB, bool Z, int RT, int WK> __global__ __launch_bounds__(WK * 64,
             multiply(b[0], x[0]);
         }
     }
+#if FP6MI_TYPE == 1
+    // Sums that are no numbers: 128 + q times a value of X has left float32's range, or there are infinities or NaN in X (or the scales).  The wavefront goes over its blocks again with (q - z) / 4096, which is exact in
+    // bf16 and keeps any sum of 128 products in range, so that what is finite comes out finite and an infinity as one, as from the tiles; finite sums stay as they are.  (28672x8192, 4 rows, one of which holds an
+    // infinity: 74 us instead of 26.)
+    bool lost = false;
+#pragma unroll
+    for (int r = 0; r < RT; r++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) lost |= !__builtin_isfinite(sum[r][i]);
+    if (__builtin_expect(__any(lost), 0)) {
+        constexpr int kEach = 4 / GPB;
+        uint32_t      expert = t.expert;
+        asm("" : "+s"(expert)); // (addresses of their own: those above need not be kept for this)
+#pragma unroll
+        for (int r = 0; r < RT; r++) {
+            const size_t at = ((size_t)expert * a.Mt + (m0 + r < a.Mt ? m0 + r : a.Mt - 1)) * a.KB;
+            v4f          whole = { 0.f, 0.f, 0.f, 0.f };
+#pragma unroll 1
+            for (uint32_t k = wave; k < a.KB; k += WK) {
+                const v4u            codes = static_cast<const v4u *>(a.W)[(at + k) * 64 + lane];
+                const Scales<GPB, Z> of = static_cast<const Scales<GPB, Z> *>(a.S)[(at + k) * 16 + c];
+#pragma unroll
+                for (int g = 0; g < GPB; g++) {
+                    const float zero = Z ? (float)of.v[2 * g + 1] : 8.f;
+                    v4f         y = { 0.f, 0.f, 0.f, 0.f };
+#pragma unroll
+                    for (uint32_t i = g * kEach; i < (g + 1) * kEach; i++) {
+                        const uint32_t column = k * 128 + i * 32 + q * 8;
+                        const v8t      x = __builtin_bit_cast(v8t, __builtin_amdgcn_raw_buffer_load_b128(xbuf, column < a.K ? (c * a.K + column) * 2 : 0x80000000u, 0, 0));
+                        v8t            v;
+#pragma unroll
+                        for (int j = 0; j < 8; j++) v[j] = (T)(((float)(codes[i] >> 4 * (j % 2 * 4 + j / 2) & 15u) - zero) * 0x1p-12f);
+                        y = mfma(x, v, y);
+                    }
+                    const float scale = (float)of.v[Z ? 2 * g : g];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) whole[i] += scale * y[i];
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (!__builtin_isfinite(sum[r][i])) sum[r][i] = whole[i] * 0x1p12f;
+        }
+    }
+#endif
 #pragma unroll
     for (int r = 0; r < RT; r++) shared[wave][r][lane] = sum[r];
     __syncthreads();

@@ -278,7 +278,7 @@ int    fp6mi_int4_pack_gpu(void *stream, void *native, void *native_scales, cons
 int    fp6mi_int4_linear(void *stream, int dtype, const void *W_native, const void *scales_native, int group, int zeros, const void *bias, const void *X, void *Y, int out_f32, int activation,
                          const int *offsets, size_t experts, size_t M, size_t N, size_t K, void *workspace);
 /* The workspace of that product, 16-byte aligned (group: the native one, grouped: with offsets, gated: with an activation): none but for many bf16 rows, which are multiplied as fp16 with a power of two for each row (a value
- * below 2^-32 of its row's largest loses bits, 2^-40 of that at most).  In products of few bf16 rows an infinity in X comes out as NaN.  kernel: -1, or that of fp6mi_int4_linear_cfg. */
+ * below 2^-32 of its row's largest loses bits, 2^-40 of that at most).   kernel: -1, or that of fp6mi_int4_linear_cfg. */
 size_t fp6mi_int4_workspace_bytes(int dtype, int group, size_t experts, int grouped, size_t M, size_t N, size_t K, int gated, int kernel);
 /* Which kernel takes it, by its number; shape, unless NULL: [0] 0 for the one that streams weights past few rows, 1 for tiles; rows of X, tiles of 16 weight rows, and K parts of a workgroup.
  * Negative: FP6MI_ERR_*.  Pure host code. */
