@@ -5,8 +5,10 @@
 // same C ABI otherwise; both launch the same kernels.
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <hip/hip_runtime_api.h>
@@ -583,9 +585,25 @@ PlanArgs plan_args(const at::Tensor &table, int64_t experts, int64_t places)
     return { p + experts, p + experts + 1 + places, p, p + experts + 1 };
 }
 
+// Refuses tensors that are to get a gradient of a function that has none, and what module._refuse_unseen does (which takes a microsecond where none of its cases is at hand).
+void refuse_unseen(std::initializer_list<const at::Tensor *> tensors)
+{
+    bool special = torch::jit::tracer::isTracing() || c10::impl::TorchDispatchModeTLS::any_modes_set() || c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::PreDispatch);
+    for (const at::Tensor *t : tensors) {
+        if (!t) continue;
+        if (at::GradMode::is_enabled() && t->requires_grad()) bad("a product with 4-bit weights has no gradient: call it under torch.no_grad()");
+        special |= t->key_set().has_any(c10::functorch_transforms_ks | c10::DispatchKeySet(c10::DispatchKey::Functionalize)) || t->_fw_grad(0).defined();
+    }
+    if (!special) return;
+    const auto refuse = pybind11::module_::import("fp6_llm_amd.module").attr("_refuse_unseen");
+    for (const at::Tensor *t : tensors)
+        if (t) refuse(*t);
+}
+
 at::Tensor int4_forward(const at::Tensor &in_feats, const at::Tensor &native, const at::Tensor &s, const OptTensor &plan, int64_t experts, int64_t places, int64_t act, const OptTensor &bias,
                         const OptTensor &out_opt, bool f32, const OptTensor &ws_opt)
 {
+    refuse_unseen({ &in_feats, &s, bias.has_value() ? &*bias : nullptr });
     const bool         grouped = plan.has_value();
     const int64_t      dims = grouped ? 6 : 5;
     const at::ScalarType type = s.scalar_type();

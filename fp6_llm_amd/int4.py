@@ -78,7 +78,7 @@ def int4_forward_native(in_feats, native_weight, native_scales, plan=None, activ
     """out[B, OC] = in_feats[B, IC] @ w^T (+ bias[OC]) with the weights of int4_pack_native.  activation ("silu", "gelu", "gelu_tanh"): out[B, OC/2] = act(gate) * up, for weights (and bias) whose
     rows are in pair order (16 rows of gate, the same 16 of up, and so on: gate_up_pairs).
     plan: that of expert_sort or expert_plan, for the weights of experts [E, ...] (bias [E, OC]): rows sorted by expert, each multiplied with its expert's weights; rows behind those come out as zeros.
-    IC is that of the weights, which their native shape tells to 128 columns only.  in_feats has the scales' type, out too or (out_dtype) float32.  workspace: float32, of fp6mi_int4_workspace_bytes (many bfloat16 rows need one).  Not part of an autograd graph."""
+    IC is that of the weights, which their native shape tells to 128 columns only.  in_feats has the scales' type, out too or (out_dtype) float32.  workspace: float32, of fp6mi_int4_workspace_bytes (many bfloat16 rows need one).  The product has no gradient: inputs that are to get one, tangents, transforms of torch.func and traces are refused."""
     _ext = _package._ext
     act = -1 if activation is None else ops._activation_code(activation)
     f32 = out_dtype == torch.float32
@@ -88,6 +88,10 @@ def int4_forward_native(in_feats, native_weight, native_scales, plan=None, activ
         if plan is None:
             return _ext.int4_forward(in_feats, native_weight, native_scales, None, 0, 0, act, bias, out, f32, workspace)
         return _ext.int4_forward(in_feats, native_weight, native_scales, plan.table, plan.experts, plan.places, act, bias, out, f32, workspace)
+    seen = [t for t in (in_feats, native_scales, bias) if t is not None]
+    if torch.is_grad_enabled() and any(t.requires_grad for t in seen):
+        raise ValueError("a product with 4-bit weights has no gradient: call it under torch.no_grad()")
+    _refuse_unseen(*seen)
     s = native_scales
     dims = 6 if plan is not None else 5
     if s.dtype not in TYPES or s.dim() != dims or s.shape[-3] != 16 or s.shape[-2] not in (1, 2, 4) or s.shape[-1] not in (1, 2) or not s.is_contiguous():
@@ -118,3 +122,6 @@ def int4_forward_native(in_feats, native_weight, native_scales, plan=None, activ
     ops._launch("fp6mi_int4_linear", dev, L.fp6mi_int4_workspace_bytes(TYPES[s.dtype], 128 // s.shape[-2], E, plan is not None, OC, B, IC, act >= 0, -1), workspace, lambda stream, ws: L.fp6mi_int4_linear(
         stream, TYPES[s.dtype], native_weight.data_ptr(), s.data_ptr(), 128 // s.shape[-2], s.shape[-1] - 1, ops._ptr(bias), x.data_ptr(), out.data_ptr(), f32, act, offsets, E, OC, B, IC, ws))
     return out
+
+
+from .module import _refuse_unseen  # noqa: E402  (it imports this module)

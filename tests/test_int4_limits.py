@@ -55,3 +55,58 @@ def test_an_infinity_in_a_bf16_row_does_not_depend_on_how_many_rows_there_are(ac
     assert choice(4096, 1, 512, "bf16", gated=act is not None) in STREAMS and choice(4096, 2048, 512, "bf16", gated=act is not None) in TILES
     few, many = (fp6.int4_forward_native(x[:n], w.native, w.native_scales, activation=act, out_dtype=torch.float32)[0] for n in (1, 2048))
     assert torch.equal(few.isnan(), many.isnan()) and torch.equal(few[~few.isnan()], many[~many.isnan()]) and few.isinf().any()
+
+
+# ---------------------------------------------------------------------------------------------------------------- what the product has no part in
+def no_part_in(dev, monkeypatch):
+    from torch.fx.experimental.proxy_tensor import make_fx
+    w = Weight(1, 32, 160, 32, True, device=dev)
+    x, b = randn(1, 2, 160, device=dev), randn(2, 32, device=dev)
+    call = lambda t: fp6.int4_forward_native(t, w.native, w.native_scales)   # noqa: E731
+    for ext in (fp6._ext, None):
+        monkeypatch.setattr(fp6, "_ext", ext)
+        for bad in (dict(in_feats=x.clone().requires_grad_()), dict(bias=b.clone().requires_grad_()), dict(native_scales=w.native_scales.clone().requires_grad_())):
+            with pytest.raises(ValueError, match="no gradient"):
+                fp6.int4_forward_native(**{**dict(in_feats=x, native_weight=w.native, native_scales=w.native_scales, bias=b), **bad})
+        with torch.autograd.forward_ad.dual_level(), pytest.raises(RuntimeError, match="forward mode"):
+            call(torch.autograd.forward_ad.make_dual(x, torch.ones_like(x)))
+        for transform in (lambda: torch.func.vmap(call)(x.unsqueeze(0)), lambda: torch.func.jvp(call, (x,), (x,)), lambda: torch.func.vmap(lambda v: fp6.int4_forward_native(x, w.native, w.native_scales, bias=v))(b.unsqueeze(0))):
+            with pytest.raises(RuntimeError, match="transform"):
+                transform()
+        with pytest.raises((RuntimeError, ValueError), match="transform|no gradient"):
+            torch.func.grad(lambda t: call(t).float().sum())(x)
+        with pytest.raises(RuntimeError, match="trace"):
+            torch.jit.trace(call, (x,), check_trace=False)
+        for pre_dispatch in (False, True):
+            with pytest.raises(RuntimeError, match="trace"):
+                make_fx(call, pre_dispatch=pre_dispatch)(x)
+
+
+def test_gradients_forward_mode_transforms_and_traces_are_refused(monkeypatch):
+    no_part_in("cpu", monkeypatch)
+
+
+@gpu
+def test_gradients_forward_mode_transforms_and_traces_are_refused_on_the_gpu(monkeypatch):
+    assert fp6._ext is not None
+    no_part_in(DEV, monkeypatch)
+
+
+@gpu
+@pytest.mark.parametrize("extension", [True, False])
+def test_the_product_between_sort_and_sum(extension, monkeypatch):
+    """A gradient of the tokens would end at the product: the call is refused, and works where the tokens are to get none; the sum's weights have theirs."""
+    if not extension:
+        monkeypatch.setattr(fp6, "_ext", None)
+    E, T = 3, 5
+    w = Weight(2, 64, 96, 32, True, E=E)
+    index = torch.arange(2 * T, device=DEV).view(T, 2) % E
+    x, weights = randn(3, T, 96).requires_grad_(), torch.rand(T, 2, device=DEV).requires_grad_()
+    rows, plan = fp6.expert_sort(x, index, E)
+    with pytest.raises(ValueError, match="no gradient"):
+        fp6.int4_forward_native(rows, w.native, w.native_scales, plan)
+    with torch.no_grad():
+        y = fp6.int4_forward_native(rows, w.native, w.native_scales, plan)
+    assert torch.equal(fp6.int4_forward_native(rows.detach(), w.native, w.native_scales, plan), y) and not y.requires_grad
+    fp6.expert_combine(y, plan, weights).float().sum().backward()
+    assert x.grad is None and weights.grad.shape == (T, 2)
