@@ -43,6 +43,9 @@ __device__ __forceinline__ float wave_sum(float v)
     return v;
 }
 
+// A dimension of a grid has fewer than 2^32 threads: workgroups beyond 2^23 stand in further rows of it (grid_of), the last of which may have some too many.
+__device__ __forceinline__ uint32_t workgroup() { return blockIdx.y * gridDim.x + blockIdx.x; }
+
 // The expert of a place, E for none.
 template <typename I> __device__ __forceinline__ int expert_of(const I *index, size_t p, int E)
 {
@@ -213,9 +216,10 @@ __global__ __launch_bounds__(512) void place_chunks(const I *__restrict__ index,
 // Third launch: the rows.  A piece of a row is read once and written to its token's places; those without an expert get zeros.
 template <typename V>
 __global__ __launch_bounds__(256) void copy_tokens(V *__restrict__ rows, const V *__restrict__ x, const int *__restrict__ place, const int *__restrict__ valid_at, size_t ldx, uint32_t nvec,
-                                                   uint32_t pieces, int k)
+                                                   uint32_t pieces, uint32_t tokens, int k)
 {
-    const uint32_t t = blockIdx.x / pieces, i = (blockIdx.x - t * pieces) * 512 + threadIdx.x;
+    const uint32_t id = workgroup(), t = id / pieces, i = (id - t * pieces) * 512 + threadIdx.x;
+    if (t >= tokens) return;
     const int      valid = *valid_at;
     V              v[2];
 #pragma unroll
@@ -234,10 +238,10 @@ __global__ __launch_bounds__(256) void copy_tokens(V *__restrict__ rows, const V
 // ---------------------------------------------------------------------------------------------------------------
 template <typename R, typename O, int VEC>
 __global__ __launch_bounds__(256) void combine_rows(O *__restrict__ out, const R *__restrict__ rows, const int *__restrict__ place, const int *__restrict__ valid_at, const float *__restrict__ weights,
-                                                    uint32_t nvec, uint32_t pieces, int k)
+                                                    uint32_t nvec, uint32_t pieces, uint32_t tokens, int k)
 {
-    const uint32_t t = blockIdx.x / pieces, i = (blockIdx.x - t * pieces) * 256 + threadIdx.x;
-    if (i >= nvec) return;
+    const uint32_t id = workgroup(), t = id / pieces, i = (id - t * pieces) * 256 + threadIdx.x;
+    if (t >= tokens || i >= nvec) return;
     const int valid = *valid_at;
     float     sum[VEC] = {};
     for (int j0 = 0; j0 < k; j0 += 4) { // four rows on their way
@@ -266,12 +270,13 @@ __global__ __launch_bounds__(256) void combine_rows(O *__restrict__ out, const R
 // and four of its experts (64 tokens x 8 of 4096: 10.1 us for all eight one after another, 6.2; 8192 x 8 of 2048 102 and 100).
 template <typename R, typename O, int VEC>
 __global__ __launch_bounds__(256) void combine_gradient(R *__restrict__ grad_rows, float *__restrict__ grad_weights, const O *__restrict__ grad, const R *__restrict__ rows,
-                                                        const int *__restrict__ place, const int *__restrict__ valid_at, const float *__restrict__ weights, uint32_t nvec, int k, uint32_t parts)
+                                                        const int *__restrict__ place, const int *__restrict__ valid_at, const float *__restrict__ weights, uint32_t nvec, uint32_t tokens, int k, uint32_t parts)
 {
     constexpr int  J = 4;
     __shared__ float part[4][J];
-    const uint32_t t = blockIdx.x / parts, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int      valid = *valid_at, j0 = (int)(blockIdx.x - t * parts) * J;
+    const uint32_t id = workgroup(), t = id / parts, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    if (t >= tokens) return;
+    const int      valid = *valid_at, j0 = (int)(id - t * parts) * J;
     const auto    *g_row = reinterpret_cast<const Vec<O, VEC> *>(grad) + (size_t)t * nvec;
     int            at[J];
     float          w[J], dot[J] = {};
@@ -318,6 +323,12 @@ inline bool aligned(const void *p, size_t n) { return (reinterpret_cast<uintptr_
 inline size_t type_size(int dtype) { return dtype == 2 ? 4 : 2; }
 inline bool known_type(int dtype) { return dtype >= 0 && dtype <= 2; }
 
+inline dim3 grid_of(size_t workgroups) // (up to 2^31)
+{
+    constexpr size_t kRow = (size_t)1 << 23;
+    return workgroups <= kRow ? dim3((uint32_t)workgroups) : dim3((uint32_t)kRow, (uint32_t)((workgroups + kRow - 1) / kRow));
+}
+
 // Up to how many places the sort takes one launch.
 constexpr size_t kFewPlaces = 2048;
 
@@ -349,7 +360,8 @@ int launch_sort(hipStream_t st, const void *index, int *offsets, int *order, int
     hipLaunchKernelGGL(place_chunks<I>, dim3(c.count), dim3(512), 0, st, static_cast<const I *>(index), table, offsets, order, place, (uint32_t)P, c.each, c.stride, (int)E);
     if (const hipError_t e = hipGetLastError(); e != hipSuccess || !rows) return (int)e;
     const uint32_t pieces = (uint32_t)((nvec + 511) / 512);
-    hipLaunchKernelGGL(copy_tokens<V>, dim3((uint32_t)tokens * pieces), dim3(256), 0, st, static_cast<V *>(rows), static_cast<const V *>(x), place, offsets + E, ldx, (uint32_t)nvec, pieces, (int)k);
+    hipLaunchKernelGGL(copy_tokens<V>, grid_of(tokens * pieces), dim3(256), 0, st, static_cast<V *>(rows), static_cast<const V *>(x), place, offsets + E, ldx, (uint32_t)nvec, pieces, (uint32_t)tokens,
+                       (int)k);
     return (int)hipGetLastError();
 }
 
@@ -432,8 +444,8 @@ int fp6mi_expert_combine(void *stream, const void *rows, const int *place, const
         constexpr int  V = decltype(vec)::value;
         const uint32_t nvec = (uint32_t)(H / V), pieces = (nvec + 255) / 256;
         if (tokens * pieces > 0x7fffffffu) return FP6MI_ERR_SHAPE;
-        hipLaunchKernelGGL((combine_rows<R, O, V>), dim3((uint32_t)(tokens * pieces)), dim3(256), 0, static_cast<hipStream_t>(stream), static_cast<O *>(out), static_cast<const R *>(rows), place, valid,
-                           weights, nvec, pieces, (int)k);
+        hipLaunchKernelGGL((combine_rows<R, O, V>), grid_of(tokens * pieces), dim3(256), 0, static_cast<hipStream_t>(stream), static_cast<O *>(out), static_cast<const R *>(rows), place, valid,
+                           weights, nvec, pieces, (uint32_t)tokens, (int)k);
         return (int)hipGetLastError();
     });
 }
@@ -453,8 +465,8 @@ int fp6mi_expert_combine_backward(void *stream, const void *grad, const void *ro
         constexpr int  V = decltype(vec)::value;
         const uint32_t parts = (uint32_t)((k + 3) / 4);
         if (tokens * parts > 0x7fffffffu) return FP6MI_ERR_SHAPE;
-        hipLaunchKernelGGL((combine_gradient<R, O, V>), dim3((uint32_t)(tokens * parts)), dim3(256), 0, static_cast<hipStream_t>(stream), static_cast<R *>(grad_rows), grad_weights, static_cast<const O *>(grad),
-                           static_cast<const R *>(rows), place, valid, weights, (uint32_t)(H / V), (int)k, parts);
+        hipLaunchKernelGGL((combine_gradient<R, O, V>), grid_of(tokens * parts), dim3(256), 0, static_cast<hipStream_t>(stream), static_cast<R *>(grad_rows), grad_weights, static_cast<const O *>(grad),
+                           static_cast<const R *>(rows), place, valid, weights, (uint32_t)(H / V), (uint32_t)tokens, (int)k, parts);
         return (int)hipGetLastError();
     });
 }
