@@ -11,6 +11,8 @@
 
 namespace {
 
+#include "fp6mi_grid.inc"
+
 typedef _Float16 half_t;
 typedef __bf16   bf16_t;
 typedef uint32_t v4u __attribute__((ext_vector_type(4)));
@@ -42,9 +44,6 @@ __device__ __forceinline__ float wave_sum(float v)
     for (int m = 32; m; m >>= 1) v += __shfl_xor(v, m);
     return v;
 }
-
-// A dimension of a grid has fewer than 2^32 threads: workgroups beyond 2^23 stand in further rows of it (grid_of), the last of which may have some too many.
-__device__ __forceinline__ uint32_t workgroup() { return blockIdx.y * gridDim.x + blockIdx.x; }
 
 // The expert of a place, E for none.
 template <typename I> __device__ __forceinline__ int expert_of(const I *index, size_t p, int E)
@@ -322,12 +321,6 @@ __global__ __launch_bounds__(256) void combine_gradient(R *__restrict__ grad_row
 inline bool aligned(const void *p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 inline size_t type_size(int dtype) { return dtype == 2 ? 4 : 2; }
 inline bool known_type(int dtype) { return dtype >= 0 && dtype <= 2; }
-
-inline dim3 grid_of(size_t workgroups) // (up to 2^31)
-{
-    constexpr size_t kRow = (size_t)1 << 23;
-    return workgroups <= kRow ? dim3((uint32_t)workgroups) : dim3((uint32_t)kRow, (uint32_t)((workgroups + kRow - 1) / kRow));
-}
 
 // Up to how many places the sort takes one launch.
 constexpr size_t kFewPlaces = 2048;

@@ -390,7 +390,6 @@ template <int GPB, bool Z, int RT, int WK> __global__ __launch_bounds__(WK * 64,
 template <int GPB, bool Z, int RT, int WK> int launch_stream(hipStream_t st, const Int4Args &a)
 {
     const size_t tiles = fp6mi::int4_tiles(a.N, a.offsets ? a.E : 0, 16);
-    if (tiles > 65535) return FP6MI_ERR_SHAPE;
     hipLaunchKernelGGL((int4_stream<GPB, Z, RT, WK>), dim3((a.Mt + RT - 1) / RT, (uint32_t)tiles), dim3(WK * 64), 0, st, a);
     return (int)hipGetLastError();
 }
@@ -398,41 +397,45 @@ template <int GPB, bool Z, int RT, int WK> int launch_stream(hipStream_t st, con
 #if FP6MI_TYPE == 1 && FP6MI_GROUPS == 1
 // Rows in bf16 as fp16 times a power of two for each row, which puts the largest finite magnitude from 2^15 to 2^16 (65280 at most: eight bits).  What is smaller than 2^-32 of that loses bits, half of 2^-24
 // and so 2^-40 of it at most: a float32 sum of such products has been rounded by more.  Infinities and NaN stay.  A workgroup to a row, which reads it twice (from L2); 4096 rows of 4096 take 15.4 us, 4.4 TB/s.
-__global__ __launch_bounds__(256) void rows_to_halfs(half_t *__restrict__ out, int *__restrict__ exponents, const T *__restrict__ X, uint32_t K)
+// (From 2^23 rows on a workgroup has more than one: a grid has fewer than 2^32 threads.)
+__global__ __launch_bounds__(256) void rows_to_halfs(half_t *__restrict__ out, int *__restrict__ exponents, const T *__restrict__ X, uint32_t N, uint32_t K)
 {
     __shared__ uint32_t most[4];
     const uint32_t tid = threadIdx.x, pieces = K / 8;
-    const v4u     *x = reinterpret_cast<const v4u *>(X + (size_t)blockIdx.x * K);
-    uint32_t       top = 0; // exponent field and mantissa of the largest finite magnitude
-    auto           field = [](uint32_t b) { return b < 0x7f80u ? b : 0u; };
-    for (uint32_t i = tid; i < pieces; i += 256) {
-        const v4u v = x[i];
+    for (uint32_t row = blockIdx.x; row < N; row += gridDim.x) {
+        const v4u     *x = reinterpret_cast<const v4u *>(X + (size_t)row * K);
+        uint32_t       top = 0; // exponent field and mantissa of the largest finite magnitude
+        auto           field = [](uint32_t b) { return b < 0x7f80u ? b : 0u; };
+        for (uint32_t i = tid; i < pieces; i += 256) {
+            const v4u v = x[i];
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const uint32_t lo = field(v[j] & 0x7fffu), hi = field(v[j] >> 16 & 0x7fffu);
-            top = top > lo ? top : lo, top = top > hi ? top : hi;
+            for (int j = 0; j < 4; j++) {
+                const uint32_t lo = field(v[j] & 0x7fffu), hi = field(v[j] >> 16 & 0x7fffu);
+                top = top > lo ? top : lo, top = top > hi ? top : hi;
+            }
         }
-    }
 #pragma unroll
-    for (int m = 32; m; m >>= 1) {
-        const uint32_t o = __shfl_xor(top, m);
-        top = top > o ? top : o;
-    }
-    if ((tid & 63) == 0) most[tid >> 6] = top;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < 4; w++) top = top > most[w] ? top : most[w];
-    const int e = top ? (int)(top >> 7 > 1 ? top >> 7 : 1) - 127 - 15 : 0;
-    if (tid == 0) exponents[blockIdx.x] = e;
-    for (uint32_t i = tid; i < pieces; i += 256) {
-        const v4u v = x[i];
-        v8h       h;
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            h[2 * j] = (half_t)__builtin_ldexpf(__builtin_bit_cast(float, v[j] << 16), -e);
-            h[2 * j + 1] = (half_t)__builtin_ldexpf(__builtin_bit_cast(float, v[j] & 0xffff0000u), -e);
+        for (int m = 32; m; m >>= 1) {
+            const uint32_t o = __shfl_xor(top, m);
+            top = top > o ? top : o;
         }
-        reinterpret_cast<v8h *>(out + (size_t)blockIdx.x * K)[i] = h;
+        if ((tid & 63) == 0) most[tid >> 6] = top;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < 4; w++) top = top > most[w] ? top : most[w];
+        const int e = top ? (int)(top >> 7 > 1 ? top >> 7 : 1) - 127 - 15 : 0;
+        if (tid == 0) exponents[row] = e;
+        for (uint32_t i = tid; i < pieces; i += 256) {
+            const v4u v = x[i];
+            v8h       h;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                h[2 * j] = (half_t)__builtin_ldexpf(__builtin_bit_cast(float, v[j] << 16), -e);
+                h[2 * j + 1] = (half_t)__builtin_ldexpf(__builtin_bit_cast(float, v[j] & 0xffff0000u), -e);
+            }
+            reinterpret_cast<v8h *>(out + (size_t)row * K)[i] = h;
+        }
+        __syncthreads(); // (the maxima are overwritten)
     }
 }
 #endif
@@ -700,7 +703,7 @@ template <int GPB, bool Z, int RT, int NT, int WR, int WK> int launch_tile(hipSt
 {
     constexpr size_t bytes = tile_lds_bytes<RT, NT, WR, WK>();
     const size_t     cols = fp6mi::int4_tiles(a.N, a.offsets ? a.E : 0, NT * 16), rows = (a.Mt + WR * RT - 1) / (WR * RT);
-    if (cols * rows > 0x7fffffffu) return FP6MI_ERR_SHAPE;
+    static_assert(WR * WK <= 8, "workgroups of up to 512 threads (fp6mi::kInt4MostTiles)");
     if constexpr (bytes > 65536)
         if (const int e = allow_dynamic_lds<int4_tile<GPB, Z, RT, NT, WR, WK>>(bytes)) return e;
     hipLaunchKernelGGL((int4_tile<GPB, Z, RT, NT, WR, WK>), dim3((uint32_t)(cols * rows)), dim3(WR * WK * 64), bytes, st, a, (uint32_t)cols);
@@ -742,7 +745,8 @@ int FP6MI_NAME(FP6MI_TYPE, FP6MI_GROUPS)(void *stream, const Int4Args &a, bool z
 #if FP6MI_TYPE == 1 && FP6MI_GROUPS == 1
 int int4_rows_to_halfs(void *stream, void *out, int *exponents, const void *X, size_t N, size_t K)
 {
-    hipLaunchKernelGGL(rows_to_halfs, dim3((uint32_t)N), dim3(256), 0, static_cast<hipStream_t>(stream), static_cast<half_t *>(out), exponents, static_cast<const T *>(X), (uint32_t)K);
+    hipLaunchKernelGGL(rows_to_halfs, dim3((uint32_t)(N < 1u << 23 ? N : 1u << 23)), dim3(256), 0, static_cast<hipStream_t>(stream), static_cast<half_t *>(out), exponents, static_cast<const T *>(X), (uint32_t)N,
+                       (uint32_t)K);
     return (int)hipGetLastError();
 }
 #endif

@@ -9,6 +9,8 @@
 
 namespace {
 
+#include "fp6mi_grid.inc"
+
 inline bool aligned(const void *p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
 // The nibble of a dword that column j (0..7) of its eight is held in: even ones in the lower 16 bits, odd ones in the upper.
@@ -55,7 +57,7 @@ __host__ __device__ inline void native_scales_of(uint16_t *to, const uint16_t *s
 template <bool ALIGNED> __global__ __launch_bounds__(256) void pack_codes(uint32_t *__restrict__ out, const uint8_t *__restrict__ codes, uint32_t blocks, uint32_t K, uint32_t KB)
 {
     __shared__ uint32_t stage[4][256];
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, s = lane >> 4, b = blockIdx.x * 4 + wave, k = b % KB * 128 + s * 32;
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, s = lane >> 4, b = workgroup() * 4 + wave, k = b % KB * 128 + s * 32;
     typedef uint32_t v4u __attribute__((ext_vector_type(4)));
     v4u d = { 0, 0, 0, 0 };
     if (b < blocks && k < K) { // (K is a multiple of 32)
@@ -76,9 +78,10 @@ template <bool ALIGNED> __global__ __launch_bounds__(256) void pack_codes(uint32
 }
 
 // A workgroup to 16 rows.
-__global__ __launch_bounds__(256) void pack_scales(uint16_t *__restrict__ out, const uint16_t *__restrict__ scales, const uint8_t *__restrict__ zeros, int bf16, uint32_t K, uint32_t KB, uint32_t group, uint32_t each)
+__global__ __launch_bounds__(256) void pack_scales(uint16_t *__restrict__ out, const uint16_t *__restrict__ scales, const uint8_t *__restrict__ zeros, uint32_t tiles, int bf16, uint32_t K, uint32_t KB, uint32_t group, uint32_t each)
 {
-    const size_t rows = (size_t)blockIdx.x * 16, groups = (K + group - 1) / group;
+    if (workgroup() >= tiles) return;
+    const size_t rows = (size_t)workgroup() * 16, groups = (K + group - 1) / group;
     native_scales_of(out + rows * KB * (128 / each) * (zeros ? 2 : 1), scales + rows * groups, zeros ? zeros + rows * groups : nullptr, bf16, K, KB, group, each, threadIdx.x, 256);
 }
 
@@ -131,6 +134,13 @@ bool lacks(int kernel, int group, size_t K, bool gated)
     return (k.tile && K > kMostTileColumns) || (gated && !k.pairs) || (k.group128 && group != 128);
 }
 
+// Whether a kernel's grid would not hold the tiles of N that there are by those of M.
+bool too_many(int kernel, size_t tiles, size_t M)
+{
+    const fp6mi::Int4Kernel &k = fp6mi::kInt4Kernels[kernel];
+    return k.tile ? tiles * ((M / 16 + k.row_tiles - 1) / k.row_tiles) > fp6mi::kInt4MostTiles : tiles > fp6mi::kInt4MostStreams;
+}
+
 int choice(int dtype, int group, size_t experts, bool grouped, size_t M, size_t N, size_t K, bool gated)
 {
     int       best = -1;
@@ -138,7 +148,7 @@ int choice(int dtype, int group, size_t experts, bool grouped, size_t M, size_t 
     for (int k = 0; k < kKernels; k++) {
         if (lacks(k, group, K, gated)) continue;
         const size_t tiles = fp6mi::int4_tiles(N, grouped ? experts : 0, fp6mi::kInt4Kernels[k].cols);
-        if (!fp6mi::kInt4Kernels[k].tile && tiles > 65535) continue; // (a grid dimension)
+        if (too_many(k, tiles, M)) continue;
         const double us = time_of(k, dtype, experts, grouped, M, N, K);
         if (best < 0 || us < least) best = k, least = us;
     }
@@ -181,11 +191,11 @@ int fp6mi_int4_pack_gpu(void *stream, void *native, void *native_scales, const v
     const size_t   tiles = experts * (M / 16), blocks = tiles * KB; // up to 2^31
     hipStream_t    st = static_cast<hipStream_t>(stream);
     if (aligned(codes, 16))
-        hipLaunchKernelGGL(pack_codes<true>, dim3((uint32_t)((blocks + 3) / 4)), dim3(256), 0, st, static_cast<uint32_t *>(native), static_cast<const uint8_t *>(codes), (uint32_t)blocks, (uint32_t)K, KB);
+        hipLaunchKernelGGL(pack_codes<true>, grid_of((blocks + 3) / 4), dim3(256), 0, st, static_cast<uint32_t *>(native), static_cast<const uint8_t *>(codes), (uint32_t)blocks, (uint32_t)K, KB);
     else
-        hipLaunchKernelGGL(pack_codes<false>, dim3((uint32_t)((blocks + 3) / 4)), dim3(256), 0, st, static_cast<uint32_t *>(native), static_cast<const uint8_t *>(codes), (uint32_t)blocks, (uint32_t)K, KB);
+        hipLaunchKernelGGL(pack_codes<false>, grid_of((blocks + 3) / 4), dim3(256), 0, st, static_cast<uint32_t *>(native), static_cast<const uint8_t *>(codes), (uint32_t)blocks, (uint32_t)K, KB);
     if (const hipError_t e = hipGetLastError()) return (int)e;
-    hipLaunchKernelGGL(pack_scales, dim3((uint32_t)tiles), dim3(256), 0, st, static_cast<uint16_t *>(native_scales), static_cast<const uint16_t *>(scales), static_cast<const uint8_t *>(zeros), dtype,
+    hipLaunchKernelGGL(pack_scales, grid_of(tiles), dim3(256), 0, st, static_cast<uint16_t *>(native_scales), static_cast<const uint16_t *>(scales), static_cast<const uint8_t *>(zeros), (uint32_t)tiles, dtype,
                        (uint32_t)K, KB, (uint32_t)group, native_group(group));
     return (int)hipGetLastError();
 }
@@ -219,7 +229,7 @@ int fp6mi_int4_linear_cfg(void *stream, int dtype, const void *W_native, const v
     if (!W_native || !scales_native || !X || !Y) return FP6MI_ERR_NULL;
     if (!aligned(W_native, 16) || !aligned(scales_native, 16) || !aligned(X, 16) || !aligned(Y, 16) || !aligned(bias, 2) || !aligned(offsets, 4) || !aligned(workspace, 16)) return FP6MI_ERR_ALIGN;
     if (kernel < 0) kernel = choice(dtype, group, experts, offsets != nullptr, M, N, K, activation >= 0);
-    if (kernel < 0 || lacks(kernel, group, K, activation >= 0)) return FP6MI_ERR_SHAPE;
+    if (kernel < 0 || lacks(kernel, group, K, activation >= 0) || too_many(kernel, fp6mi::int4_tiles(N, offsets ? experts : 0, fp6mi::kInt4Kernels[kernel].cols), M)) return FP6MI_ERR_SHAPE;
     fp6mi::Int4Args a = { W_native, scales_native, X, bias, Y, offsets, (uint32_t)N, (uint32_t)K, (uint32_t)((K + 127) / 128), (uint32_t)(M / 16), (uint32_t)experts, activation, out_f32, nullptr };
     if (scratch_bytes(dtype, kernel, N, K)) {
         if (!workspace) return FP6MI_ERR_WORKSPACE;

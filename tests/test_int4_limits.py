@@ -110,3 +110,50 @@ def test_the_product_between_sort_and_sum(extension, monkeypatch):
     assert torch.equal(fp6.int4_forward_native(rows.detach(), w.native, w.native_scales, plan), y) and not y.requires_grad
     fp6.expert_combine(y, plan, weights).float().sum().backward()
     assert x.grad is None and weights.grad.shape == (T, 2)
+
+
+# ---------------------------------------------------------------------------------------------------------------- sizes
+def test_more_workgroups_than_a_grid_holds_are_refused():
+    """A launch of 2^32 threads does nothing and says nothing."""
+    from fp6_llm_amd import _lib
+    L, p, SHAPE = _lib.lib(), 1 << 20, -2   # (an address that nothing reads: every call is refused before a launch)
+
+    def cfg(kernel, M, N, dtype=0, offsets=None, E=1):
+        return L.fp6mi_int4_linear_cfg(None, dtype, p, p, 128, 0, None, p, p, 0, -1, offsets, E, M, N, 128, p, kernel)
+    for k in TILES:
+        _, cols, row_tiles, _ = KERNELS[k]
+        for M, N in ((16, cols << 23), (16 * row_tiles << 12, cols << 11)):
+            assert all(cfg(k, M, N, dtype) == SHAPE for dtype in (0, 1)), k
+        assert cfg(k, 16, 1 << 30, 0, p, 64) == SHAPE
+    for k in STREAMS:
+        assert cfg(k, 16, 65536 * 16) == SHAPE
+    # the choice takes kernels that hold the problem, as long as there are any
+    for N, of in ((65535 * 16, range(12)), (65536 * 16, TILES), (1 << 26, TILES), ((1 << 29) - 64, (10, 11)), ((1 << 29), (-2,)), (1 << 30, (-2,))):
+        assert choice(16, N, 128) in of and choice(16, N, 128, "bf16") in of, N
+
+
+@gpu
+def test_more_bf16_rows_than_a_grid_has_workgroups():
+    N = (1 << 24) + 3
+    x, w = whole_numbers(Weight(1, 32, 64, 32, True, "bf16"), 2, 97)
+    x = x.bfloat16().to(DEV)[torch.arange(N, device=DEV) * 5 % 97]
+    assert choice(32, N, 64, "bf16", group=32) in TILES
+    got = fp6.int4_forward_native(x, w.native, w.native_scales)
+    want = (x[:97].double() @ w.w.t().to(DEV)).bfloat16()
+    assert (x[:97].double() @ w.w.t().to(DEV)).abs().max() < 2 ** 24
+    for first in range(0, N, 1 << 22):
+        rows = torch.arange(first, min(N, first + (1 << 22)), device=DEV)
+        assert torch.equal(got[first:first + (1 << 22)], want[rows % 97]), first
+
+
+@gpu
+def test_packing_more_than_a_grid_has_workgroups():
+    """Blocks and scales of 65 matrices of 2^24 rows: the last one as by itself."""
+    E, OC = 65, 1 << 24
+    codes, scales = torch.empty(E, OC, 16, dtype=torch.uint8, device=DEV), torch.empty(E, OC, 1, dtype=torch.float16, device=DEV)
+    for e in range(E):
+        codes[e].random_(0, 256), scales[e].uniform_()
+    native, native_scales = fp6.int4_pack_native(codes, scales, group=32)
+    for e in (0, 15, 16, 31, 64):
+        one, one_scales = fp6.int4_pack_native(codes[e], scales[e], group=32)
+        assert torch.equal(native[e], one) and torch.equal(native_scales[e], one_scales), e
