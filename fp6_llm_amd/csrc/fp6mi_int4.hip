@@ -4,7 +4,7 @@
 //
 // q - z is an integer from -15 to 15, exact in fp16, so the matrix instructions' products are exact and their sums float32; a group's sum is multiplied by its scale in float32.
 // (Scaling the weights before the product would round each of them to 16 bits, and 16-bit sums would be no cheaper.)  bf16 has no packed arithmetic that would make q - z of codes: the kernel of
-// few rows multiplies 128 + q, which are bits, from sums that start at -(128 + z) times those of X; the one of many rows is given X in fp16 with an exponent for each row (rows_to_halfs).
+// few rows multiplies 16 + q, which are bits, from sums that start at -(16 + z) times those of X; the one of many rows is given X in fp16 with an exponent for each row (rows_to_halfs).
 //
 // Layout (fp6mi_int4_pack): blocks of 16 rows x 128 columns of 1024 bytes, [expert][row tile][column block]; lane c + 16 q of a wavefront holds 16 bytes of a block, dword s of which are the
 // columns 32 s + 8 q to 32 s + 8 q + 7 of row c: the operand of one v_mfma_f32_16x16x32.  In a dword the nibbles 0..7 are the columns 0, 2, 4, 6, 1, 3, 5, 7, so that a mask leaves two neighbours
@@ -80,10 +80,11 @@ __device__ __forceinline__ void codes_half(Codes &to, uint32_t w, const Zero &ze
     to.d[2 * half + 1] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(__builtin_bit_cast(v2h, (w & cut.high) | cut.bits), sixteenth, zero.high));
 }
 
-// The operands of the kernel of few rows.  fp16: q - z.  bf16: 128 + q, the bits 0x4300 | nibble, 7 instructions (q - z by way of float32 takes 23, which bound that kernel); what is too much, 128 + z times
+// The operands of the kernel of few rows.  fp16: q - z.  bf16: 16 + q, the bits 0x4180 | nibble << 3, 8 instructions (q - z by way of float32 takes 23, which bound that kernel); what is too much, 16 + z times
 // the sum of a group's X, is where the products start from, a sum that a matrix instruction with ones makes for all row tiles (28672x8192 at 4 rows with groups of 64 and zero points 26.7 -> 24.9 us
-// against one with -(128 + z) for each).  What is lost of the float32 sums is 2^-24 of 30 times their magnitude, a
-// thousandth of an output's rounding; sums that leave float32's range on the way are made again at the end, with q - z.
+// against one with -(16 + z) for each).  That costs float32 sums a factor of some five in rounding: of 8192 columns they are off by 1e-7 to 3e-7 rms (values of mean 0 or 1, one of 3000 among them), where
+// a product in float32 is by 4e-7 to 8e-7; 128 + q, the nibble as it stands, takes an instruction less (26.1 us, with these 26.6) and is off by 7e-7 to 3e-6.  Sums that leave float32's range on the way
+// are made again at the end, with q - z.
 #if FP6MI_TYPE == 0
 struct FewCutter : Cutter { };
 struct FewZero : Zero { };
@@ -96,18 +97,18 @@ __device__ __forceinline__ v8t codes_of(uint32_t w, const FewZero &zero, const F
 }
 #else
 struct FewCutter {
-    uint32_t mask = 0x000f000fu, bits = 0x43004300u;
+    uint32_t mask = 0x00780078u, bits = 0x41804180u;
     __device__ __forceinline__ FewCutter() { asm("" : "+s"(mask), "+v"(bits)); }
 };
 struct FewZero {
-    float all; // -(128 + z)
-    __device__ __forceinline__ void set(T zero) { all = -128.f - (float)zero; }
+    float all; // -(16 + z)
+    __device__ __forceinline__ void set(T zero) { all = -16.f - (float)zero; }
 };
 __device__ __forceinline__ v8t codes_of(uint32_t w, const FewZero &, const FewCutter &cut)
 {
     union { uint32_t d[4]; v8t v; } r;
 #pragma unroll
-    for (int i = 0; i < 4; i++) r.d[i] = (w >> 4 * i & cut.mask) | cut.bits;
+    for (int i = 0; i < 4; i++) r.d[i] = ((i ? w >> (4 * i - 3) : w << 3) & cut.mask) | cut.bits;
     return r.v;
 }
 #endif
@@ -235,9 +236,9 @@ template <int GPB, bool Z, int RT, int WK> __global__ __launch_bounds__(WK * 64,
         constexpr bool kStart = FP6MI_TYPE == 1;
         FewZero        zero;
         zero.set((T)8.f);
-        v4f start[GPB]; // the groups' sums of X; without zero points -136 times that, which all rows' products start from
+        v4f start[GPB]; // the groups' sums of X; without zero points -24 times that, which all rows' products start from
 #if FP6MI_TYPE == 1
-        const T   each = (T)(Z ? 1.f : -136.f);
+        const T   each = (T)(Z ? 1.f : -24.f);
         const v8t ones = { each, each, each, each, each, each, each, each };
 #pragma unroll
         for (int g = 0; g < GPB; g++) {
@@ -307,9 +308,9 @@ template <int GPB, bool Z, int RT, int WK> __global__ __launch_bounds__(WK * 64,
         }
     }
 #if FP6MI_TYPE == 1
-    // Sums that are no numbers: 128 + q times a value of X has left float32's range, or there are infinities or NaN in X (or the scales).  The wavefront goes over its blocks again with (q - z) / 4096, which is exact in
+    // Sums that are no numbers: 16 + q times a value of X has left float32's range, or there are infinities or NaN in X (or the scales).  The wavefront goes over its blocks again with (q - z) / 4096, which is exact in
     // bf16 and keeps any sum of 128 products in range, so that what is finite comes out finite and an infinity as one, as from the tiles; finite sums stay as they are.  (28672x8192, 4 rows, one of which holds an
-    // infinity: 74 us instead of 26.)
+    // infinity: 76 us instead of 26.6.)
     bool lost = false;
 #pragma unroll
     for (int r = 0; r < RT; r++)

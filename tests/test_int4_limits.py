@@ -25,7 +25,7 @@ def whole_numbers(w, seed, N):
 @pytest.mark.parametrize("group,zeros", [(32, True), (64, False), (128, True), (128, False)])
 @pytest.mark.parametrize("kernel", STREAMS)
 def test_bf16_rows_of_every_size_in_the_stream_kernels(kernel, group, zeros):
-    """These multiply 128 + q, which leaves float32's range before q - z does: all that float32 sums of the weights' own products can hold comes out, and infinities as the definition has them.  Rows of
+    """These multiply 16 + q, which leaves float32's range before q - z does: all that float32 sums of the weights' own products can hold comes out, and infinities as the definition has them.  Rows of
     whole numbers times a power of two, so that every sum is exact; of the last size 15 * 3 * 128 of a group's magnitudes come to 2^138."""
     w = Weight(5 + kernel, 80, 1184, group, zeros, "bf16")
     x, w = whole_numbers(w, 3, 9)
@@ -44,6 +44,18 @@ def test_bf16_rows_of_every_size_in_the_stream_kernels(kernel, group, zeros):
     assert torch.equal(got[7].isnan(), a == 0) and torch.equal(got[7][a != 0], a[a != 0].sign() * float("inf"))
     nan = (b == 0) | (c == 0) | (b.sign() == c.sign())
     assert torch.equal(got[8].isnan(), nan) and torch.equal(got[8][~nan], b[~nan].sign() * float("inf"))
+
+
+@gpu
+@pytest.mark.parametrize("group,zeros", [(32, True), (64, False), (128, True), (128, False)])
+@pytest.mark.parametrize("kernel", STREAMS)
+def test_a_large_value_among_small_ones_costs_bf16_sums_nothing(kernel, group, zeros):
+    """16 + q and 16 + z stand for q and z there: a group's sum is exact while 31 times its magnitudes come to less than 2^24, here 2^18 and up to 128 ones."""
+    w = Weight(11 + kernel, 80, 1184, group, zeros, "bf16")
+    x, w = whole_numbers(w, 5, 16)
+    x[:, 70], x[:, 333] = 2.0 ** 18, -2.0 ** 17   # (in two groups; with scales of 1 and 2 all sums come to 2 * 15 * (2^18 + 2^17 + 1184) < 2^24 at the most)
+    want = x @ w.w.t()
+    assert torch.equal(d(by_kernel(kernel, w, x.bfloat16().to(DEV), f32=True)), want)
 
 
 @gpu
