@@ -3,21 +3,108 @@ import pytest
 import torch
 
 import fp6_llm_amd as fp6
-from test_int4 import DEV, KERNELS, TILES, TYPES, Weight, by_kernel, choice, d, gpu, randn
+from test_int4 import DEV, KERNELS, TILES, Weight, by_kernel, choice, d, gated64, gpu, halves, randn, within
 
 STREAMS = [k for k in range(len(KERNELS)) if k not in TILES]
 
 
-def whole_numbers(w, seed, N):
-    """Rows of -1, 0 and 1 for a weight whose scales become 1 and 2: sums of whole numbers, which float32 holds in any order, and the same in 64 bits."""
-    s = torch.exp2(torch.randint(0, 2, w.scales.shape, generator=torch.Generator().manual_seed(seed)).double())
+def whole_numbers(w, seed, N, unit=1.0, device=DEV):
+    """Rows of -1, 0 and 1 for a weight whose scales become 1 and 2 (times a power of two): sums of whole numbers, which float32 holds in any order as long as their magnitudes come to less than 2^24."""
+    s = unit * torch.exp2(torch.randint(0, 2, w.scales.shape, generator=torch.Generator().manual_seed(seed)).double())
     each = torch.arange(w.IC) // w.group
     old = w.scales.cpu().double()
     w.w = (w.w / old[..., each]).round() * s[..., each]
-    w.scales = s.to(w.dtype).to(DEV)
+    w.scales = s.to(w.dtype).to(device)
     w.native, w.native_scales = fp6.int4_pack_native(w.codes, w.scales, w.zeros, w.group)
     x = torch.randint(-1, 2, (N, w.IC), generator=torch.Generator().manual_seed(seed + 1)).double()
+    assert w.E or float((x.abs() @ w.w.abs().t()).max()) < unit * 2 ** 24
     return x, w
+
+
+# ---------------------------------------------------------------------------------------------------------------- whole numbers: every sum is exact, and an output off by anything is seen
+EXACT = [  # OC, IC, N, group, zeros, type, the kernels that may be the choice
+    (256, 8192, 1, 64, True, "bf16", STREAMS), (512, 4576, 16, 32, False, "bf16", STREAMS), (256, 28672, 2, 64, False, "fp16", STREAMS), (256, 28672, 70, 128, False, "bf16", range(12)), (4096, 4096, 16, 128, True, "fp16", STREAMS),
+    (2064, 544, 31, 32, True, "bf16", STREAMS), (10240, 4576, 19, 32, True, "fp16", TILES), (4112, 11040, 64, 64, True, "fp16", TILES), (528, 1120, 65, 128, True, "bf16", STREAMS), (8208, 2080, 130, 128, False, "fp16", TILES),
+    (4096, 4096, 256, 128, True, "bf16", TILES), (4112, 4128, 300, 32, True, "bf16", TILES), (8208, 2048, 777, 64, False, "bf16", TILES), (1072, 992, 513, 128, True, "fp16", STREAMS), (4112, 416, 1030, 64, False, "fp16", TILES), (2064, 28672, 150, 96, True, "bf16", TILES),
+    (32, (1 << 20) + 160, 3, 128, True, "fp16", STREAMS), (32, (1 << 20) + 160, 40, 64, True, "bf16", STREAMS), (48, 1 << 19, 50, 128, False, "fp16", range(12))]
+
+
+def native_group(group):
+    return 128 if group % 128 == 0 else 64 if group % 64 == 0 else 32
+
+
+@pytest.mark.parametrize("OC,IC,N,group,zeros,type,kernels", EXACT)
+def test_whole_numbers_show_what_is_missing(OC, IC, N, group, zeros, type, kernels):
+    """Of what is compared below: outputs of zeros, or without the last block of 128 columns (or what there is of it), the first group or one in the middle, are seen in most places; and the choice is what the case is there for."""
+    x, w = whole_numbers(Weight(OC + IC + N, OC, IC, group, zeros, type, device="cpu"), OC, min(N, 16), device="cpu")
+    assert choice(OC, N, IC, type, group=native_group(group)) in kernels
+    want = x @ w.w.t()
+    last = (IC - 1) // 128 * 128
+    for columns in (slice(0, IC), slice(last, IC), slice(0, group), slice(IC // 2 // group * group, (IC // 2 // group + 1) * group)):
+        part = x[:, columns] @ w.w[:, columns].t()
+        assert (part != 0).double().mean() > 0.9, columns
+        assert ((want - part).to(w.dtype) != want.to(w.dtype)).double().mean() > 0.6, columns   # (rounded outputs too)
+
+
+@gpu
+@pytest.mark.parametrize("OC,IC,N,group,zeros,type,kernels", EXACT)
+def test_product_of_whole_numbers(OC, IC, N, group, zeros, type, kernels):
+    x, w = whole_numbers(Weight(OC + IC + N, OC, IC, group, zeros, type), OC, N)
+    want, x = x @ w.w.t(), x.to(w.dtype).to(DEV)
+    b = torch.arange(OC).remainder(17).double() - 8
+    assert torch.equal(fp6.int4_forward_native(x, w.native, w.native_scales).cpu(), want.to(w.dtype))
+    got = fp6.int4_forward_native(x, w.native, w.native_scales, bias=b.to(w.dtype).to(DEV), out_dtype=torch.float32)
+    assert torch.equal(d(got), want + b)
+
+
+@gpu
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+@pytest.mark.parametrize("OC,IC,N,group,zeros,type,kernels", [(288, 28672, 7, 64, True, "bf16", STREAMS), (2080, 8192, 20, 32, False, "fp16", range(12)), (4096, 4096, 256, 128, True, "bf16", TILES), (4128, 8192, 70, 128, True, "fp16", TILES),
+                                                              (544, 2080, 150, 32, True, "bf16", range(12))])
+def test_gated_product_of_whole_numbers(act, OC, IC, N, group, zeros, type, kernels):
+    """Exact pre-activations: what is left is the activation's own error (2^-18 of its argument) and the rounding."""
+    assert choice(OC, N, IC, type, gated=True, group=native_group(group)) in kernels
+    x, w = whole_numbers(Weight(OC + IC + N, OC, IC, group, zeros, type), OC, N, 2.0 ** -8)
+    y, x = x @ w.w.t(), x.to(w.dtype).to(DEV)
+    for dtype in (w.dtype, torch.float32):
+        got = fp6.int4_forward_native(x, w.native, w.native_scales, activation=act, out_dtype=dtype)
+        h, tol = gated64(y, torch.zeros_like(y), act, dtype)
+        within(got, h, tol, str(dtype))
+        g, u = halves(y)
+        assert (h.abs() > 4 * tol)[(g > 0.5) & (u != 0)].all()   # (an output of zeros, or without the part of a column that is 2^-8 or more of it, is off by more)
+
+
+@gpu
+@pytest.mark.parametrize("T,k,E,OC,IC,group,zeros,type", [(1, 2, 8, 288, 11008, 128, False, "fp16"), (40, 8, 64, 288, 2080, 64, True, "bf16"), (700, 2, 8, 1056, 4128, 32, True, "fp16"), (1500, 2, 4, 2064, 2048, 128, True, "bf16"),
+                                                          (320, 1, 64, 2048, 2560, 128, True, "fp16"), (320, 1, 64, 2048, 2560, 64, False, "bf16")])
+def test_product_of_sorted_rows_of_whole_numbers(T, k, E, OC, IC, group, zeros, type):
+    """Float32 outputs, as the product down of Int4Experts has them; the last two cases with all rows on one expert of many."""
+    x, w = whole_numbers(Weight(T + OC + IC, OC, IC, group, zeros, type, E), E, T)
+    assert 30 * IC < 2 ** 24
+    g = torch.Generator().manual_seed(T)
+    index = torch.full((T, k), 5) if T == 320 else torch.randint(-1, E, (T, k), generator=g)
+    rows, plan = fp6.expert_sort(x.to(w.dtype).to(DEV), index.to(DEV), E)
+    got = fp6.int4_forward_native(rows, w.native, w.native_scales, plan, out_dtype=torch.float32)
+    rounded = fp6.int4_forward_native(rows, w.native, w.native_scales, plan)
+    offsets, rows = plan.offsets.tolist(), d(rows)
+    for e in range(E):
+        want = rows[offsets[e]:offsets[e + 1]] @ w.w[e].t()
+        assert torch.equal(d(got[offsets[e]:offsets[e + 1]]), want) and torch.equal(rounded[offsets[e]:offsets[e + 1]].cpu(), want.to(w.dtype)), e
+    assert (got[offsets[-1]:] == 0).all() and (rounded[offsets[-1]:] == 0).all()
+
+
+@gpu
+@pytest.mark.parametrize("group,zeros", [(32, True), (64, False), (96, True), (128, True), (128, False)])
+@pytest.mark.parametrize("type", ["fp16", "bf16"])
+@pytest.mark.parametrize("kernel", range(len(KERNELS)))
+def test_every_kernel_in_whole_numbers(kernel, type, group, zeros):
+    if kernel == 10 and group != 128:
+        pytest.skip("this kernel has groups of 128 only")
+    cols = KERNELS[kernel][1]
+    for OC, IC, N in ((48, 32, 1), (272, 96, cols), (96, 1184, cols + 1), (1056, 608, 2 * cols - 1), (32, 28704, 3), (288, 2048, 3 * cols + 5)):
+        x, w = whole_numbers(Weight(OC + N + kernel, OC, IC, group, zeros, type), N, N)
+        want, x = x @ w.w.t(), x.to(w.dtype).to(DEV)
+        assert torch.equal(d(by_kernel(kernel, w, x, f32=True)), want) and torch.equal(by_kernel(kernel, w, x).cpu(), want.to(w.dtype)), (OC, IC, N)
 
 
 # ---------------------------------------------------------------------------------------------------------------- infinities and large values
