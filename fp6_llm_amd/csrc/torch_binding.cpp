@@ -600,10 +600,12 @@ void refuse_unseen(std::initializer_list<const at::Tensor *> tensors)
         if (t) refuse(*t);
 }
 
-at::Tensor int4_forward(const at::Tensor &in_feats, const at::Tensor &native, const at::Tensor &s, const OptTensor &plan, int64_t experts, int64_t places, int64_t act, const OptTensor &bias,
+at::Tensor int4_forward(const at::Tensor &in_feats, const at::Tensor &native, const at::Tensor &scales, const OptTensor &plan, int64_t experts, int64_t places, int64_t act, const OptTensor &bias_opt,
                         const OptTensor &out_opt, bool f32, const OptTensor &ws_opt)
 {
-    refuse_unseen({ &in_feats, &s, bias.has_value() ? &*bias : nullptr });
+    refuse_unseen({ &in_feats, &scales, bias_opt.has_value() ? &*bias_opt : nullptr });
+    const at::Tensor   s = scales.resolve_neg();
+    const OptTensor    bias = bias_opt.has_value() ? OptTensor(bias_opt->resolve_neg()) : c10::nullopt;
     const bool         grouped = plan.has_value();
     const int64_t      dims = grouped ? 6 : 5;
     const at::ScalarType type = s.scalar_type();
@@ -626,14 +628,14 @@ at::Tensor int4_forward(const at::Tensor &in_feats, const at::Tensor &native, co
     }
     if (bias.has_value() && (bias->scalar_type() != type || bias->dim() != (grouped ? 2 : 1) || bias->size(-1) != OC || (grouped && bias->size(0) != E) || !bias->is_contiguous() || bias->device() != dev))
         bad("bias must be contiguous, of the scales' type, one for each row of the weights, on the same GPU");
-    const at::Tensor     x = in_feats.is_contiguous() ? in_feats : in_feats.contiguous();
+    const at::Tensor     x = in_feats.resolve_neg().contiguous();
     c10::hip::HIPGuard   guard(dev.index());
     const at::ScalarType to = f32 ? at::kFloat : type;
     const int64_t        cols = act >= 0 ? OC / 2 : OC;
     at::Tensor           out;
     if (out_opt.has_value()) {
         out = *out_opt;
-        if (out.dim() != 2 || out.size(0) != B || out.size(1) != cols || out.scalar_type() != to || !out.is_contiguous() || out.device() != dev)
+        if (out.dim() != 2 || out.size(0) != B || out.size(1) != cols || out.scalar_type() != to || !out.is_contiguous() || out.device() != dev || out.is_neg())
             bad("out must be a contiguous [" + std::to_string(B) + ", " + std::to_string(cols) + "] tensor of the output's type on the same GPU");
     } else {
         out = at::empty({ B, cols }, at::TensorOptions().dtype(to).device(dev));

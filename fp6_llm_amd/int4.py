@@ -64,7 +64,7 @@ def int4_pack_native(codes, scales, zeros=None, group=128):
         raise ValueError("codes must be on a GPU or on the host")
     native, native_scales = native_shapes(OC, IC, group, zeros is not None, E if codes.dim() == 3 else None)
     w, s = torch.empty(native, dtype=torch.int32, device=codes.device), torch.empty(native_scales, dtype=scales.dtype, device=codes.device)
-    codes, scales, zeros = codes.contiguous(), scales.contiguous(), None if zeros is None else zeros.contiguous()
+    codes, scales, zeros = codes.contiguous(), scales.resolve_neg().contiguous(), None if zeros is None else zeros.contiguous()
     args = (w.data_ptr(), s.data_ptr(), codes.data_ptr(), scales.data_ptr(), ops._ptr(zeros), TYPES[scales.dtype], E, OC, IC, group)
     if codes.device.type == "cpu":
         _lib.check(_lib.lib().fp6mi_int4_pack(*args), "fp6mi_int4_pack")
@@ -92,7 +92,7 @@ def int4_forward_native(in_feats, native_weight, native_scales, plan=None, activ
     if torch.is_grad_enabled() and any(t.requires_grad for t in seen):
         raise ValueError("a product with 4-bit weights has no gradient: call it under torch.no_grad()")
     _refuse_unseen(*seen)
-    s = native_scales
+    s, bias = native_scales.resolve_neg(), None if bias is None else bias.resolve_neg()
     dims = 6 if plan is not None else 5
     if s.dtype not in TYPES or s.dim() != dims or s.shape[-3] != 16 or s.shape[-2] not in (1, 2, 4) or s.shape[-1] not in (1, 2) or not s.is_contiguous():
         raise ValueError("native_scales must be those of int4_pack_native, %s" % ("of experts" if plan is not None else "of one matrix"))
@@ -116,7 +116,9 @@ def int4_forward_native(in_feats, native_weight, native_scales, plan=None, activ
         offsets = plan._addresses()[0]
     if bias is not None and (bias.dtype != s.dtype or bias.shape != ((E, OC) if plan is not None else (OC,)) or not bias.is_contiguous() or bias.device != dev):
         raise ValueError("bias must be contiguous, of the scales' type, one for each row of the weights, on the same GPU")
-    x = x.contiguous()
+    x = x.resolve_neg().contiguous()
+    if out is not None and out.is_neg():
+        raise ValueError("out must not be a negative view")
     out = ops._result(out, (B, OC // 2 if act >= 0 else OC), dev, dtype=torch.float32 if f32 else s.dtype)
     L = _lib.lib()
     ops._launch("fp6mi_int4_linear", dev, L.fp6mi_int4_workspace_bytes(TYPES[s.dtype], 128 // s.shape[-2], E, plan is not None, OC, B, IC, act >= 0, -1), workspace, lambda stream, ws: L.fp6mi_int4_linear(

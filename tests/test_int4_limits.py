@@ -256,3 +256,28 @@ def test_packing_more_than_a_grid_has_workgroups():
     for e in (0, 15, 16, 31, 64):
         one, one_scales = fp6.int4_pack_native(codes[e], scales[e], group=32)
         assert torch.equal(native[e], one) and torch.equal(native_scales[e], one_scales), e
+
+
+# ---------------------------------------------------------------------------------------------------------------- views with a lazy negative sign
+def test_packing_resolves_negative_views():
+    w = Weight(3, 32, 96, 32, True, device="cpu")
+    native, scales = fp6.int4_pack_native(w.codes, torch._neg_view(w.scales), w.zeros, 32)
+    assert torch.equal(native, w.native) and torch.equal(scales[..., 0], -w.native_scales[..., 0]) and torch.equal(scales[..., 1], w.native_scales[..., 1])
+
+
+@gpu
+@pytest.mark.parametrize("N", [2, 100])
+@pytest.mark.parametrize("extension", [True, False])
+def test_negative_views(extension, N, monkeypatch):
+    assert fp6._ext is not None
+    if not extension:
+        monkeypatch.setattr(fp6, "_ext", None)
+    w = Weight(4, 64, 160, 32, False)
+    x, b = randn(1, N, 160), randn(2, 64)
+    want = fp6.int4_forward_native(x, w.native, w.native_scales, bias=b)
+    neg = torch._neg_view
+    assert torch.equal(fp6.int4_forward_native(neg(x), w.native, w.native_scales, bias=neg(b)), -want)
+    assert torch.equal(fp6.int4_forward_native(x, w.native, neg(w.native_scales), bias=neg(b)), -want)
+    assert torch.equal(fp6.int4_pack_native(w.codes, neg(w.scales), None, 32)[1], -w.native_scales)
+    with pytest.raises(ValueError):
+        fp6.int4_forward_native(x, w.native, w.native_scales, out=neg(torch.empty_like(want)))
