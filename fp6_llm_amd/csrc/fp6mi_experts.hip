@@ -167,7 +167,6 @@ __global__ __launch_bounds__(512) void place_chunks(const I *__restrict__ index,
     const int      tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const uint32_t b = blockIdx.x, chunks = gridDim.x, lo = b * each, hi = lo + each < P ? lo + each : P;
     int            e = lo + tid < hi ? expert_of(index, (size_t)lo + tid, E) : -1;
-#pragma unroll 4
     for (int f = wave; f < E; f += 8) {
         int before = 0, all = 0;
         for (uint32_t c = lane; c < chunks; c += kWave) {
