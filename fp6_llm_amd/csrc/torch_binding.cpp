@@ -600,6 +600,12 @@ void refuse_unseen(std::initializer_list<const at::Tensor *> tensors)
         if (t) refuse(*t);
 }
 
+bool overlap(const at::Tensor &a, const at::Tensor &b) // (of contiguous ones)
+{
+    const auto *p = static_cast<const uint8_t *>(a.data_ptr()), *q = static_cast<const uint8_t *>(b.data_ptr());
+    return p < q + b.nbytes() && q < p + a.nbytes();
+}
+
 at::Tensor int4_forward(const at::Tensor &in_feats, const at::Tensor &native, const at::Tensor &scales, const OptTensor &plan, int64_t experts, int64_t places, int64_t act, const OptTensor &bias_opt,
                         const OptTensor &out_opt, bool f32, const OptTensor &ws_opt)
 {
@@ -637,6 +643,7 @@ at::Tensor int4_forward(const at::Tensor &in_feats, const at::Tensor &native, co
         out = *out_opt;
         if (out.dim() != 2 || out.size(0) != B || out.size(1) != cols || out.scalar_type() != to || !out.is_contiguous() || out.device() != dev || out.is_neg())
             bad("out must be a contiguous [" + std::to_string(B) + ", " + std::to_string(cols) + "] tensor of the output's type on the same GPU");
+        if (overlap(out, x) || overlap(out, native) || overlap(out, s) || (bias.has_value() && overlap(out, *bias))) bad("out must have memory of its own");
     } else {
         out = at::empty({ B, cols }, at::TensorOptions().dtype(to).device(dev));
     }

@@ -74,11 +74,15 @@ def int4_pack_native(codes, scales, zeros=None, group=128):
     return w, s
 
 
+def _overlap(a, b):
+    return a.data_ptr() < b.data_ptr() + b.numel() * b.element_size() and b.data_ptr() < a.data_ptr() + a.numel() * a.element_size()
+
+
 def int4_forward_native(in_feats, native_weight, native_scales, plan=None, activation=None, bias=None, out=None, out_dtype=None, workspace=None):
     """out[B, OC] = in_feats[B, IC] @ w^T (+ bias[OC]) with the weights of int4_pack_native.  activation ("silu", "gelu", "gelu_tanh"): out[B, OC/2] = act(gate) * up, for weights (and bias) whose
     rows are in pair order (16 rows of gate, the same 16 of up, and so on: gate_up_pairs).
     plan: that of expert_sort or expert_plan, for the weights of experts [E, ...] (bias [E, OC]): rows sorted by expert, each multiplied with its expert's weights; rows behind those come out as zeros.
-    IC is that of the weights, which their native shape tells to 128 columns only.  in_feats has the scales' type, out too or (out_dtype) float32.  workspace: float32, of fp6mi_int4_workspace_bytes (many bfloat16 rows need one).  The product has no gradient: inputs that are to get one, tangents, transforms of torch.func and traces are refused."""
+    IC is that of the weights, which their native shape tells to 128 columns only.  in_feats has the scales' type, out too or (out_dtype) float32; out may not lie over an input.  workspace: float32, of fp6mi_int4_workspace_bytes (many bfloat16 rows need one).  The product has no gradient: inputs that are to get one, tangents, transforms of torch.func and traces are refused."""
     _ext = _package._ext
     act = -1 if activation is None else ops._activation_code(activation)
     f32 = out_dtype == torch.float32
@@ -117,8 +121,8 @@ def int4_forward_native(in_feats, native_weight, native_scales, plan=None, activ
     if bias is not None and (bias.dtype != s.dtype or bias.shape != ((E, OC) if plan is not None else (OC,)) or not bias.is_contiguous() or bias.device != dev):
         raise ValueError("bias must be contiguous, of the scales' type, one for each row of the weights, on the same GPU")
     x = x.resolve_neg().contiguous()
-    if out is not None and out.is_neg():
-        raise ValueError("out must not be a negative view")
+    if out is not None and (out.is_neg() or any(_overlap(out, t) for t in (x, native_weight, s, bias) if t is not None)):
+        raise ValueError("out must have memory of its own, and be no negative view")
     out = ops._result(out, (B, OC // 2 if act >= 0 else OC), dev, dtype=torch.float32 if f32 else s.dtype)
     L = _lib.lib()
     ops._launch("fp6mi_int4_linear", dev, L.fp6mi_int4_workspace_bytes(TYPES[s.dtype], 128 // s.shape[-2], E, plan is not None, OC, B, IC, act >= 0, -1), workspace, lambda stream, ws: L.fp6mi_int4_linear(

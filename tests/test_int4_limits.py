@@ -281,3 +281,26 @@ def test_negative_views(extension, N, monkeypatch):
     assert torch.equal(fp6.int4_pack_native(w.codes, neg(w.scales), None, 32)[1], -w.native_scales)
     with pytest.raises(ValueError):
         fp6.int4_forward_native(x, w.native, w.native_scales, out=neg(torch.empty_like(want)))
+
+
+# ---------------------------------------------------------------------------------------------------------------- outputs over inputs
+@gpu
+@pytest.mark.parametrize("extension", [True, False])
+def test_outputs_over_inputs_are_refused(extension, monkeypatch):
+    """Workgroups write rows of the output while others still read the input."""
+    assert fp6._ext is not None
+    if not extension:
+        monkeypatch.setattr(fp6, "_ext", None)
+    w = Weight(5, 64, 64, 32, True)
+    both = randn(1, 41, 64)
+    x = both[:40]
+    want = fp6.int4_forward_native(x, w.native, w.native_scales)
+    for out in (x, both[1:]):
+        with pytest.raises(ValueError, match="memory of its own"):
+            fp6.int4_forward_native(x, w.native, w.native_scales, out=out)
+    beside = torch.empty(80, 64, dtype=torch.float16, device=DEV)
+    beside[:40] = x
+    assert torch.equal(fp6.int4_forward_native(beside[:40], w.native, w.native_scales, out=beside[40:]), want)
+    strided = torch.empty(40, 128, dtype=torch.float16, device=DEV)   # (rows that are copied before the product)
+    strided[:, ::2] = x
+    assert torch.equal(fp6.int4_forward_native(strided[:, ::2], w.native, w.native_scales, out=strided.view(-1)[:40 * 64].view(40, 64)), want)
