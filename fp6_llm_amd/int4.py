@@ -17,7 +17,7 @@ TYPES = {torch.float16: 0, torch.bfloat16: 1}
 def int4_quantize(weight, group=128, zeros=False):
     """codes uint8 [..., OC, IC/2], scales [..., OC, ceil(IC/group)] and zero points (uint8 like the scales, or None) of a float16, bfloat16 or float32 weight [..., OC, IC], rounded to nearest.
     Without zero points the codes are 1..15 about 8 and a scale is the group's largest magnitude / 7; with them a group's range (0 included) is cut into 15 steps.
-    Scales have the weight's type, float16 for float32."""
+    Scales have the weight's type, float16 for float32; a weight that they do not reach, or that is not finite, is refused (which waits for a GPU)."""
     if weight.dtype not in (torch.float16, torch.bfloat16, torch.float32) or weight.dim() < 2 or weight.shape[-1] % 2 or weight.numel() == 0:
         raise ValueError("weight must be float16, bfloat16 or float32 [..., OC, IC], IC even")
     if group < 32 or group % 32:
@@ -32,6 +32,8 @@ def int4_quantize(weight, group=128, zeros=False):
         low, high = w.amin(-1).clamp(max=0), w.amax(-1).clamp(min=0)
         scales = ((high - low) / 15).to(dtype)
         z = torch.where(scales > 0, torch.round(-low / scales.float()), 0).clamp(0, 15)
+    if not bool(scales.isfinite().all()):
+        raise ValueError("the weight holds infinities, NaN or values beyond what scales in %s reach" % str(dtype).split(".")[-1])
     step = torch.where(scales > 0, scales.float(), 1.0).unsqueeze(-1)
     q = torch.round(w / step).add_(8 if z is None else z.unsqueeze(-1)).clamp_(0 if zeros else 1, 15).to(torch.uint8).flatten(-2)[..., :IC]
     return q[..., 0::2] | q[..., 1::2] << 4, scales, None if z is None else z.to(torch.uint8)

@@ -304,3 +304,20 @@ def test_outputs_over_inputs_are_refused(extension, monkeypatch):
     strided = torch.empty(40, 128, dtype=torch.float16, device=DEV)   # (rows that are copied before the product)
     strided[:, ::2] = x
     assert torch.equal(fp6.int4_forward_native(strided[:, ::2], w.native, w.native_scales, out=strided.view(-1)[:40 * 64].view(40, 64)), want)
+
+
+# ---------------------------------------------------------------------------------------------------------------- weights that have no codes
+@pytest.mark.parametrize("zeros", [False, True])
+def test_quantizer_refuses_what_has_no_codes(zeros):
+    """A scale of infinity or NaN would make a group NaN whatever its codes; a float32 weight of 7 * 65504, or a range of 15 times that, still has a scale in fp16."""
+    for dtype, value in ((torch.float32, float("inf")), (torch.float32, float("-inf")), (torch.float16, float("nan")), (torch.bfloat16, float("inf")), (torch.float32, 1.0e6), (torch.float32, 3.0e38)):
+        w = torch.ones(2, 16, 64, dtype=dtype)
+        w[1, 3, 40] = value
+        if value == 1.0e6 and zeros:
+            w[1, 3, 40] = 15 * 65600.0
+        with pytest.raises(ValueError, match="infinities"):
+            fp6.int4_quantize(w, 32, zeros)
+    w = torch.ones(16, 64)
+    w[3, 40] = 15 * 65504.0 if zeros else 7 * 65504.0
+    codes, scales, z = fp6.int4_quantize(w, 32, zeros)
+    assert scales[3, 1] == 65504 and codes[3, 20] & 15 == 15 and (z is None or z[3, 1] == 0)
