@@ -146,6 +146,24 @@ def test_a_large_value_among_small_ones_costs_bf16_sums_nothing(kernel, group, z
 
 
 @gpu
+@pytest.mark.parametrize("group,zeros", [(32, True), (128, False)])
+@pytest.mark.parametrize("kernel", [k for k in range(len(KERNELS)) if k != 10])
+def test_fp16_rows_of_every_size(kernel, group, zeros):
+    """From the smallest number below the normal ones to the largest power of two; infinities and NaN as the definition has them."""
+    w = Weight(7 + kernel, 96, 1184, group, zeros, "fp16")
+    x, w = whole_numbers(w, 4, 9)
+    x *= torch.exp2(torch.tensor([0, -24, -20, -15, -14, 15, 10, 0, 0]).double()).unsqueeze(1)
+    want = x @ w.w.t()
+    x[7, 5], x[8, 3], x[6, 1183] = float("inf"), float("nan"), 65504.0
+    want[6] = x[6] @ w.w.t()
+    assert float((x[6].abs() @ w.w.abs().t()).max()) < 2 ** 30   # (of multiples of 2^5: 2^24 of them, and 65504 is one)
+    got = d(by_kernel(kernel, w, x.half().to(DEV), f32=True))
+    assert torch.equal(got[:7], want[:7]) and got[8].isnan().all()
+    a = w.w[:, 5]
+    assert torch.equal(got[7].isnan(), a == 0) and torch.equal(got[7][a != 0], a[a != 0].sign() * float("inf"))
+
+
+@gpu
 @pytest.mark.parametrize("act", [None, "silu"])
 def test_an_infinity_in_a_bf16_row_does_not_depend_on_how_many_rows_there_are(act):
     w = Weight(6, 4096, 512, 128, True, "bf16")
