@@ -600,6 +600,8 @@ void refuse_unseen(std::initializer_list<const at::Tensor *> tensors)
         if (t) refuse(*t);
 }
 
+at::Tensor signed_values(const at::Tensor &t) { return t.is_neg() ? t.resolve_neg() : t; } // (asked first: resolve_neg itself goes through torch's dispatcher)
+
 bool overlap(const at::Tensor &a, const at::Tensor &b) // (of contiguous ones)
 {
     const auto *p = static_cast<const uint8_t *>(a.data_ptr()), *q = static_cast<const uint8_t *>(b.data_ptr());
@@ -610,8 +612,8 @@ at::Tensor int4_forward(const at::Tensor &in_feats, const at::Tensor &native, co
                         const OptTensor &out_opt, bool f32, const OptTensor &ws_opt)
 {
     refuse_unseen({ &in_feats, &scales, bias_opt.has_value() ? &*bias_opt : nullptr });
-    const at::Tensor   s = scales.resolve_neg();
-    const OptTensor    bias = bias_opt.has_value() ? OptTensor(bias_opt->resolve_neg()) : c10::nullopt;
+    const at::Tensor   s = signed_values(scales);
+    const OptTensor    bias = bias_opt.has_value() ? OptTensor(signed_values(*bias_opt)) : c10::nullopt;
     const bool         grouped = plan.has_value();
     const int64_t      dims = grouped ? 6 : 5;
     const at::ScalarType type = s.scalar_type();
@@ -634,7 +636,7 @@ at::Tensor int4_forward(const at::Tensor &in_feats, const at::Tensor &native, co
     }
     if (bias.has_value() && (bias->scalar_type() != type || bias->dim() != (grouped ? 2 : 1) || bias->size(-1) != OC || (grouped && bias->size(0) != E) || !bias->is_contiguous() || bias->device() != dev))
         bad("bias must be contiguous, of the scales' type, one for each row of the weights, on the same GPU");
-    const at::Tensor     x = in_feats.resolve_neg().contiguous();
+    const at::Tensor     x = signed_values(in_feats).contiguous();
     c10::hip::HIPGuard   guard(dev.index());
     const at::ScalarType to = f32 ? at::kFloat : type;
     const int64_t        cols = act >= 0 ? OC / 2 : OC;
