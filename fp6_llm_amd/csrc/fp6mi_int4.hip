@@ -448,8 +448,9 @@ __global__ __launch_bounds__(256) void rows_to_halfs(half_t *__restrict__ out, i
 // Many rows are bound by the matrix units with the conversions and the scaling of the group sums beside them (3.6 VALU instructions to a matrix instruction; twice the columns to a wavefront, 2.6, was no
 // faster, nor were 32x32x16 instructions, which draw more power): 8192x8192 at 777 rows takes 108 to 114 us, 8 experts of 22016x4096 at 4096 rows 720 to 750, 1.0 PFLOP/s, where a library's product of large
 // dense fp16 matrices reaches 1.2.  Two workgroups to a CU where LDS allows, so that one multiplies while the other waits at its barrier.
-// 17 to some 100 rows are bound by what a CU takes of the weights, some 20 bytes a ns, so that their tiles are as many as there are CUs, of three, four, six or eight row tiles (10240x4576 at 19 rows:
-// 13.0 us in 160 workgroups of four row tiles, 11.1 in 214 of three; more stages or blocks ahead did nothing for the others).
+// 17 to some 100 rows reach neither the matrix units nor memory: 11 to 14 bytes of the weights a ns and CU, of a copy 20.  Tiles are as many there as there are CUs, of three, four, six or eight row tiles
+// (10240x4576 at 19 rows: 13.0 us in 160 workgroups of four row tiles, 11.1 in 214 of three), so that weights are loaded and converted again for every 32 rows; of 21.7 us of 8192x8192 at 64 rows, without
+// codes and scales 13.0 were left, without the transfers of X 18.8, without conversions 19.4, and more stages or blocks ahead did nothing.
 // ---------------------------------------------------------------------------------------------------------------
 template <int RT, int NT, int WR, int WK> constexpr size_t tile_lds_bytes() // the stages; the sums of the groups on their way to the first; the outputs on their way out (a half at a time where they are float32)
 {

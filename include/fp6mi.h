@@ -275,7 +275,7 @@ int    fp6mi_int4_pack_gpu(void *stream, void *native, void *native_scales, cons
  * (M % 32 == 0; bias likewise).  group: the native one (32, 64, 128).  bias: of the activations' type, [experts][M], or NULL.  out_f32: Y is float32, else of the activations' type.
  * offsets: NULL for one matrix, or experts + 1 row numbers on the device, as fp6mi_expert_sort writes them: rows offsets[e] to offsets[e+1] - 1 are multiplied with the weights of expert e, rows from
  * offsets[experts] on become zeros.  FP6MI_ERR_SHAPE also where no kernel's grid holds the tiles: from 2^29 rows or some 2^37 outputs on.  Products are exact, sums float32 (of a group before its scale, of the scaled groups behind it), rounded once.
- * In bf16 the kernels 0 to 4 of fp6mi_int4_linear_cfg, which the choice takes for few rows and, where matrices are small, for hundreds, sum x * (16 + q) from -(16 + z) * sum(x) on: a float32 sum of terms of up to 31 times x. */
+ * In bf16 the kernels 0 to 4 of fp6mi_int4_linear_cfg, which the choice takes for few rows and, where matrices are small, for up to a thousand, sum x * (16 + q) from -(16 + z) * sum(x) on: a float32 sum of terms of up to 31 times x. */
 int    fp6mi_int4_linear(void *stream, int dtype, const void *W_native, const void *scales_native, int group, int zeros, const void *bias, const void *X, void *Y, int out_f32, int activation,
                          const int *offsets, size_t experts, size_t M, size_t N, size_t K, void *workspace);
 /* The workspace of that product, 16-byte aligned (group: the native one, grouped: with offsets, gated: with an activation): none but for many bf16 rows, which are multiplied as fp16 with a power of two for each row (a value
