@@ -274,12 +274,12 @@ int    fp6mi_int4_pack_gpu(void *stream, void *native, void *native_scales, cons
 /* Y[N,M] = X[N,K] . w^T + bias; with an activation (FP6MI_ACT_*, negative: none) Y[N,M/2] = act(gate) * up for weights whose rows are in pair order, 16 of gate, the same 16 of up, and so on
  * (M % 32 == 0; bias likewise).  group: the native one (32, 64, 128).  bias: of the activations' type, [experts][M], or NULL.  out_f32: Y is float32, else of the activations' type.
  * offsets: NULL for one matrix, or experts + 1 row numbers on the device, as fp6mi_expert_sort writes them: rows offsets[e] to offsets[e+1] - 1 are multiplied with the weights of expert e, rows from
- * offsets[experts] on become zeros.  FP6MI_ERR_SHAPE also where no kernel's grid holds the tiles: from 2^29 rows or some 2^37 outputs on.  Products are exact, sums float32 (of a group before its scale, of the scaled groups behind it), rounded once.
- * In bf16 the kernels 0 to 4 of fp6mi_int4_linear_cfg, which the choice takes for few rows and, where matrices are small, for up to a thousand, sum x * (16 + q) from -(16 + z) * sum(x) on: a float32 sum of terms of up to 31 times x. */
+ * offsets[experts] on become zeros.  FP6MI_ERR_SHAPE also where no kernel's grid holds the tiles: from 2^29 rows (beyond K = 2^20 from 2^20 rows) or some 2^37 outputs on.  Products are exact, sums float32 (of a group before its scale, of the scaled groups behind it), rounded once.
+ * In bf16 the kernels 0 to 4 of fp6mi_int4_linear_cfg, which the choice takes for few rows, where matrices are small for a thousand and more, and beyond K = 2^20 for any number, sum x * (16 + q) from -(16 + z) * sum(x) on: a float32 sum of terms of up to 31 times x. */
 int    fp6mi_int4_linear(void *stream, int dtype, const void *W_native, const void *scales_native, int group, int zeros, const void *bias, const void *X, void *Y, int out_f32, int activation,
                          const int *offsets, size_t experts, size_t M, size_t N, size_t K, void *workspace);
 /* The workspace of that product, 16-byte aligned (group: the native one, grouped: with offsets, gated: with an activation): none but for many bf16 rows, which are multiplied as fp16 with a power of two for each row (a value
- * below 2^-32 of its row's largest loses bits, 2^-40 of that at most).   kernel: -1, or that of fp6mi_int4_linear_cfg. */
+ * below 2^-32 of its row's largest loses bits, 2^-40 of that at most; scales from about 2^98 on may overflow there).   kernel: -1, or that of fp6mi_int4_linear_cfg. */
 size_t fp6mi_int4_workspace_bytes(int dtype, int group, size_t experts, int grouped, size_t M, size_t N, size_t K, int gated, int kernel);
 /* Which kernel takes it, by its number; shape, unless NULL: [0] 0 for the one that streams weights past few rows, 1 for tiles; rows of X, tiles of 16 weight rows, and K parts of a workgroup.
  * Negative: FP6MI_ERR_*.  Pure host code. */

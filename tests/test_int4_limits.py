@@ -274,6 +274,8 @@ def test_packing_more_than_a_grid_has_workgroups():
     for e in (0, 15, 16, 31, 64):
         one, one_scales = fp6.int4_pack_native(codes[e], scales[e], group=32)
         assert torch.equal(native[e], one) and torch.equal(native_scales[e], one_scales), e
+    del codes, scales, native, native_scales, one, one_scales
+    torch.cuda.empty_cache()   # (100 GB)
 
 
 # ---------------------------------------------------------------------------------------------------------------- views with a lazy negative sign
